@@ -24,6 +24,8 @@ __all__ = [
     "build", "load", "HelixError", "Sequence", "BlockManager", "PagedKvCache", "DecodeBatch",
     "PagedBlockTable", "paged_attention_out", "paged_attention_with_tail_out",
     "paged_decode_attention", "decode_workspace_bytes", "decode_workspace", "append_slots",
+    "paged_tree_attention", "tree_workspace_bytes", "tree_workspace", "verify_tree",
+    "verify_workspace_bytes", "verify_workspace", "append_path",
     "PagedPrefixCache", "PREFIX_INSERTED", "PREFIX_ALREADY_PRESENT", "PREFIX_REJECTED_TOO_LARGE",
     "INVALID_ARGUMENT", "OUT_OF_RANGE", "UNSUPPORTED", "RESOURCE_EXHAUSTED", "RUNTIME", "INTERNAL",
 ]
@@ -105,6 +107,10 @@ class BlockManager:
 
     def release_sequence(self, seq):
         check(_lib().helix_block_manager_release_sequence(self._h, seq))
+
+    def truncate_sequence(self, seq, length):
+        """Drops the tokens from `length` on and frees the pages they alone held."""
+        check(_lib().helix_block_manager_truncate(self._h, seq, length))
 
     def contains(self, seq):
         out = ctypes.c_int()
@@ -320,6 +326,10 @@ class PagedKvCache:
 
     def release_sequence(self, seq):
         check(_lib().helix_paged_cache_release_sequence(self._h, seq))
+
+    def truncate_sequence(self, seq, length):
+        """Drops the tokens from `length` on and frees the pages they alone held."""
+        check(_lib().helix_paged_cache_truncate_sequence(self._h, seq, length))
 
     def retrieve_layer(self, seq, layer):
         """Allocating gather: returns device (keys, values) [kv_heads, length, dim]."""
@@ -604,6 +614,218 @@ def append_chunk(keys, values, key_pool, value_pool, slots, stream=None):
                                           _stream(stream)))
 
 
+# ------------------------------------------------------------ tree steps ----
+def _require_tensor(t, name, dtypes, shape, device=None, strided=False):
+    """A device tensor of one of `dtypes` and of `shape` (None: any size),
+    contiguous, or with `strided` contiguous in its last dimension."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        names = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+        raise HelixError(INVALID_ARGUMENT, f"{name} must be a {names} tensor")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("*" if n is None else str(n) for n in shape)
+        raise HelixError(INVALID_ARGUMENT,
+                         f"{name} must have shape [{want}], got {list(t.shape)}")
+    if strided:
+        if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise HelixError(INVALID_ARGUMENT, f"{name} must be contiguous in its last dimension")
+    elif not t.is_contiguous():
+        raise HelixError(INVALID_ARGUMENT, f"{name} must be contiguous")
+    if device is not None and t.device != device:
+        raise HelixError(INVALID_ARGUMENT, f"{name} must be on {device}, got {t.device}")
+
+
+def _on(device):
+    """The device of a call's tensors as the current one."""
+    import torch
+    if device.type != "cuda":
+        raise HelixError(INVALID_ARGUMENT, f"tensors must be on a GPU, got {device}")
+    return torch.cuda.device(device)
+
+
+def _device_stream(stream, device):
+    import torch
+    return _stream(torch.cuda.current_stream(device) if stream is None else stream)
+
+
+def tree_workspace_bytes(batch, q_heads, kv_heads, nodes):
+    out = ctypes.c_size_t()
+    check(_lib().helix_paged_tree_workspace_bytes(batch, q_heads, kv_heads, nodes,
+                                                  ctypes.byref(out)))
+    return out.value
+
+
+def tree_workspace(batch, q_heads, kv_heads, nodes, device="cuda:0"):
+    """A workspace for paged_tree_attention (torch uint8 tensor; no initial
+    value needed).  Calls that overlap need one each."""
+    import torch
+    n = tree_workspace_bytes(batch, q_heads, kv_heads, nodes)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def paged_tree_attention(query, key_pool, value_pool, tables, lengths, tree_key, tree_value,
+                         parents, output, workspace, node_counts=None, stream=None,
+                         pool_shape=None, page_dtype="f32", k_scale=1.0, v_scale=1.0):
+    """Attention of a tree of up to 64 drafted tokens per sequence: query row
+    (h, t) sees the sequence's history, the ancestors of node t and node t.
+    query, output [B, Hq, T, 128]; pools [N, Hkv, 16, 128] tensors (or raw
+    device addresses with pool_shape) of page_dtype "f32", "bf16" or "fp8";
+    tables [B, max_blocks] int32/uint32; lengths [B] int32 history tokens;
+    tree_key / tree_value [B, Hkv, T, 128]; parents [B, T] int32 (parent of
+    each node, before it, or -1 for a root) or None for chains; node_counts [B]
+    int32 or None: each sequence's own number of nodes, rows of `output` behind
+    it stay as they were.  Any Hq that is a multiple of Hkv."""
+    import torch
+    if query.dim() != 4:
+        raise HelixError(INVALID_ARGUMENT, "query must have shape [batch, q_heads, nodes, dim]")
+    b, hq, t, d = query.shape
+    f32, i32 = (torch.float32,), (torch.int32,)
+    if pool_shape is None:
+        for pool, name in ((key_pool, "key_pool"), (value_pool, "value_pool")):
+            width = {"f32": 4, "bf16": 2, "fp8": 1}.get(page_dtype)
+            if width is not None and pool.element_size() != width:
+                raise HelixError(INVALID_ARGUMENT, f"{name} must hold {width}-byte elements")
+            _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), query.device)
+        pool_shape = tuple(key_pool.shape)
+        key_pool, value_pool = key_pool.data_ptr(), value_pool.data_ptr()
+    if len(pool_shape) != 4:
+        raise HelixError(INVALID_ARGUMENT, "pools must have shape [blocks, kv_heads, tokens, dim]")
+    n, hkv, p, pd = pool_shape
+    if pd != d:
+        raise HelixError(INVALID_ARGUMENT, "query and pools must have the same head size")
+    dev = query.device
+    _require_tensor(query, "query", f32, (b, hq, t, d))
+    _require_tensor(output, "output", f32, (b, hq, t, d), dev)
+    _require_tensor(tree_key, "tree_key", f32, (b, hkv, t, d), dev)
+    _require_tensor(tree_value, "tree_value", f32, (b, hkv, t, d), dev)
+    _require_tensor(tables, "tables", (torch.int32, torch.uint32), (b, None), dev)
+    _require_tensor(lengths, "lengths", i32, (b,), dev)
+    if parents is not None:
+        _require_tensor(parents, "parents", i32, (b, t), dev)
+    if node_counts is not None:
+        _require_tensor(node_counts, "node_counts", i32, (b,), dev)
+    _require_tensor(workspace, "workspace", (workspace.dtype,), (None,), dev)
+    dtype = _PAGE_DTYPES.get(page_dtype, -1)
+    with _on(dev):
+        check(_lib().helix_paged_tree_attention(
+            _ptr(query), b, hq, hkv, t, d, ctypes.c_void_p(key_pool), ctypes.c_void_p(value_pool),
+            n, p, _ptr(tables), tables.shape[1], _ptr(lengths), _ptr(tree_key), _ptr(tree_value),
+            _ptr(parents), _ptr(node_counts), _ptr(output), _ptr(workspace),
+            workspace.numel() * workspace.element_size(), dtype, k_scale, v_scale,
+            _device_stream(stream, dev)))
+
+
+def verify_workspace_bytes(batch, nodes, vocab):
+    out = ctypes.c_size_t()
+    check(_lib().helix_verify_tree_workspace_bytes(batch, nodes, vocab, ctypes.byref(out)))
+    return out.value
+
+
+def verify_workspace(batch, nodes, vocab, device="cuda:0"):
+    """A workspace for verify_tree (torch uint8 tensor; no initial value
+    needed).  Calls that overlap need one each."""
+    import torch
+    n = verify_workspace_bytes(batch, nodes, vocab)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def _verify_arguments(target, draft, tokens, parents, uniforms, bonus_uniforms, path, accepted,
+                      next_token, node_counts):
+    """The checked arguments of a verification up to its strides, and behind
+    its sizes."""
+    import torch
+    f32, i32 = (torch.float32,), (torch.int32,)
+    _require_tensor(target, "target", f32, (None, None, None), strided=True)
+    b, t, v = target.shape
+    dev = target.device
+    if draft is not None:
+        _require_tensor(draft, "draft", f32, (b, t, v), dev, strided=True)
+    _require_tensor(tokens, "tokens", i32, (b, t), dev)
+    if parents is not None:
+        _require_tensor(parents, "parents", i32, (b, t), dev)
+    if node_counts is not None:
+        _require_tensor(node_counts, "node_counts", i32, (b,), dev)
+    _require_tensor(uniforms, "uniforms", f32, (b, t), dev)
+    _require_tensor(bonus_uniforms, "bonus_uniforms", f32, (b,), dev)
+    _require_tensor(path, "path", i32, (b, t), dev)
+    _require_tensor(accepted, "accepted", i32, (b,), dev)
+    _require_tensor(next_token, "next_token", i32, (b,), dev)
+
+    def strides(x):  # a dimension of one row may have any stride
+        return (0, 0) if x is None else (x.stride(0) if b > 1 else 0,
+                                         x.stride(1) if t > 1 else v)
+
+    rows = (_ptr(target), *strides(target), _ptr(draft), *strides(draft))
+    lists = (_ptr(tokens), _ptr(parents), _ptr(node_counts), _ptr(uniforms),
+             _ptr(bonus_uniforms))
+    return rows, lists, (_ptr(path), _ptr(accepted), _ptr(next_token))
+
+
+def verify_tree(target, draft, tokens, parents, uniforms, bonus_uniforms, path, accepted,
+                next_token, workspace, node_counts=None, stream=None):
+    """Which drafted tokens the target's probabilities accept, and the token
+    that follows them.  target [B, T, V]: row n is the target's distribution
+    after node n; draft [B, T, V] or None: row n is the distribution the children
+    of node n were drawn from (None: they were certain); both may be strided in
+    their first two dimensions.  tokens [B, T] int32; parents [B, T] int32 or
+    None for chains (node 0 is the root); uniforms [B, T] and bonus_uniforms [B]
+    in [0, 1); node_counts [B] int32 or None.  Writes path [B, T] (accepted
+    nodes from the root, then -1), accepted [B] (their number) and next_token
+    [B], all int32."""
+    rows, lists, out = _verify_arguments(target, draft, tokens, parents, uniforms, bonus_uniforms,
+                                         path, accepted, next_token, node_counts)
+    b, t, v = target.shape
+    dev = target.device
+    _require_tensor(workspace, "workspace", (workspace.dtype,), (None,), dev)
+    with _on(dev):
+        check(_lib().helix_verify_tree(
+            *rows, b, t, v, *lists, *out, _ptr(workspace),
+            workspace.numel() * workspace.element_size(), _device_stream(stream, dev)))
+
+
+def append_path(keys, values, key_pool, value_pool, slots, path, accepted, stream=None,
+                page_dtype="f32", k_scale=1.0, v_scale=1.0):
+    """Write the rows of the accepted nodes, path[b, i] for i < accepted[b], to
+    slots[b, i]: keys / values [B, Hkv, T, D] and pools [N, Hkv, P, D], or with
+    a leading dimension of layers each (a pool's layers may lie apart); slots
+    [B, T] int64, path [B, T] and accepted [B] int32."""
+    import torch
+    layered = key_pool.dim() == 5
+    if key_pool.dim() not in (4, 5):
+        raise HelixError(INVALID_ARGUMENT,
+                         "pools must have shape [(layers,) blocks, kv_heads, tokens, dim]")
+    dev = keys.device
+    layers = key_pool.shape[0] if layered else 1
+    n, hkv, p, d = key_pool.shape[-4:]
+    lead = (layers,) if layered else ()
+    _require_tensor(slots, "slots", (torch.int64,), (None, None), dev)
+    b, t = slots.shape
+    _require_tensor(keys, "keys", (torch.float32,), (*lead, b, hkv, t, d))
+    _require_tensor(values, "values", (torch.float32,), (*lead, b, hkv, t, d), dev)
+    _require_tensor(path, "path", (torch.int32,), (b, t), dev)
+    _require_tensor(accepted, "accepted", (torch.int32,), (b,), dev)
+    width = {"f32": 4, "bf16": 2, "fp8": 1}.get(page_dtype)
+    stride = 0
+    for pool, name in ((key_pool, "key_pool"), (value_pool, "value_pool")):
+        if width is not None and pool.element_size() != width:
+            raise HelixError(INVALID_ARGUMENT, f"{name} must hold {width}-byte elements")
+        if layered:
+            _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), dev, strided=True)
+            if layers:
+                _require_tensor(pool[0], name, (pool.dtype,), tuple(key_pool.shape[1:]), dev)
+            if layers > 1:
+                if pool.stride(0) != key_pool.stride(0):
+                    raise HelixError(INVALID_ARGUMENT, "pools must have the same layer stride")
+                stride = pool.stride(0)
+        else:
+            _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), dev)
+    with _on(dev):
+        check(_lib().helix_paged_append_path(
+            _ptr(keys), _ptr(values), _ptr(key_pool), _ptr(value_pool), layers, stride, n, hkv, p,
+            d, _ptr(slots), _ptr(path), _ptr(accepted), b, t, _PAGE_DTYPES.get(page_dtype, -1),
+            k_scale, v_scale, _device_stream(stream, dev)))
+
+
 class DecodeBatch:
     """Batched decode driver over a PagedKvCache (persistent device tables)."""
 
@@ -615,6 +837,7 @@ class DecodeBatch:
         self._h = h
         self._cache = cache
         self.batch = len(sequences)
+        self.q_heads = q_heads
 
     def close(self):
         h = getattr(self, "_h", None)
@@ -669,6 +892,66 @@ class DecodeBatch:
         check(_lib().helix_decode_batch_attention_layer(self._h, layer, _ptr(query),
                                                         _ptr(tail_key), _ptr(tail_value),
                                                         _ptr(output), _stream(stream)))
+
+    def prepare_tree(self, nodes, stream=None):
+        """Reserve the slots of a tree of `nodes` drafted tokens (up to 64) per
+        sequence: tree_layer() in every layer, then accept_tree() or
+        commit_path().  An uncommitted tree step is dropped by the next
+        prepare call."""
+        check(_lib().helix_decode_batch_prepare_tree(self._h, nodes, _stream(stream)))
+        self._nodes = nodes
+
+    def tree_layer(self, layer, query, tree_key, tree_value, parents, output, node_counts=None,
+                   stream=None):
+        """paged_tree_attention over the batch: query, output [batch, q_heads,
+        nodes, dim], tree rows [batch, kv_heads, nodes, dim]."""
+        import torch
+        t, hkv, d = getattr(self, "_nodes", 0), self._cache.kv_heads, self._cache.head_dimension
+        dev = torch.device("cuda", self._cache.device)
+        for x, name, heads in ((query, "query", self.q_heads), (tree_key, "tree_key", hkv),
+                               (tree_value, "tree_value", hkv), (output, "output", self.q_heads)):
+            _require_tensor(x, name, (torch.float32,), (self.batch, heads, t, d), dev)
+        for x, name, shape in ((parents, "parents", (self.batch, t)),
+                               (node_counts, "node_counts", (self.batch,))):
+            if x is not None:
+                _require_tensor(x, name, (torch.int32,), shape, dev)
+        check(_lib().helix_decode_batch_tree_layer(
+            self._h, layer, _ptr(query), _ptr(tree_key), _ptr(tree_value), _ptr(parents),
+            _ptr(node_counts), _ptr(output), _device_stream(stream, dev)))
+
+    def _tree_rows(self, keys, values):
+        import torch
+        shape = (self._cache.layers, self.batch, self._cache.kv_heads, getattr(self, "_nodes", 0),
+                 self._cache.head_dimension)
+        dev = torch.device("cuda", self._cache.device)
+        _require_tensor(keys, "keys", (torch.float32,), shape, dev)
+        _require_tensor(values, "values", (torch.float32,), shape, dev)
+        return dev
+
+    def commit_path(self, keys, values, path, accepted, stream=None):
+        """End a tree step: the rows [layers, batch, kv_heads, nodes, dim] of the
+        accepted nodes go to their pages in every layer, and each sequence keeps
+        its accepted tokens (path [batch, nodes], accepted [batch] int32, as
+        verify_tree leaves them).  Synchronises the stream."""
+        import torch
+        dev = self._tree_rows(keys, values)
+        _require_tensor(path, "path", (torch.int32,), (self.batch, keys.shape[3]), dev)
+        _require_tensor(accepted, "accepted", (torch.int32,), (self.batch,), dev)
+        check(_lib().helix_decode_batch_commit_path(self._h, _ptr(keys), _ptr(values), _ptr(path),
+                                                    _ptr(accepted), _device_stream(stream, dev)))
+
+    def accept_tree(self, target, draft, tokens, parents, uniforms, bonus_uniforms, keys, values,
+                    path, accepted, next_token, node_counts=None, stream=None):
+        """verify_tree of the step's drafts, then commit_path of what it accepts."""
+        dev = self._tree_rows(keys, values)
+        rows, lists, out = _verify_arguments(target, draft, tokens, parents, uniforms,
+                                             bonus_uniforms, path, accepted, next_token,
+                                             node_counts)
+        _require_tensor(target, "target", (target.dtype,), (self.batch, keys.shape[3], None), dev,
+                        strided=True)
+        check(_lib().helix_decode_batch_accept_tree(
+            self._h, *rows, target.shape[2], *lists, _ptr(keys), _ptr(values), *out,
+            _device_stream(stream, dev)))
 
     def shared_pages(self):
         """Leading pages the prepared decode step attends once for the batch."""

@@ -93,6 +93,7 @@ SIGNATURES = {
     "helix_block_manager_fork_sequence": (c_int, [vp, Sequence, c_size, c_int, P(Sequence), P(CowCopy)]),
     "helix_block_manager_append": (c_int, [vp, Sequence, c_size, P(c_u64)]),
     "helix_block_manager_release_sequence": (c_int, [vp, Sequence]),
+    "helix_block_manager_truncate": (c_int, [vp, Sequence, c_size]),
     "helix_block_manager_contains": (c_int, [vp, Sequence, P(c_int)]),
     "helix_block_manager_length": (c_int, [vp, Sequence, P(c_size)]),
     "helix_block_manager_block_table": (c_int, [vp, Sequence, P(c_u32), c_size, P(c_size)]),
@@ -108,6 +109,7 @@ SIGNATURES = {
     "helix_paged_cache_append": (c_int, [vp, Sequence, vp, vp, vp]),
     "helix_paged_cache_append_layer_major": (c_int, [vp, Sequence, P(vp), P(vp), c_size, vp]),
     "helix_paged_cache_release_sequence": (c_int, [vp, Sequence]),
+    "helix_paged_cache_truncate_sequence": (c_int, [vp, Sequence, c_size]),
     "helix_paged_cache_copy_layer_out": (c_int, [vp, Sequence, c_size, vp, vp, vp]),
     "helix_paged_cache_copy_layer_prefix_out": (c_int, [vp, Sequence, c_size, c_size, vp, vp, c_size, vp]),
     "helix_paged_cache_contains": (c_int, [vp, Sequence, P(c_int)]),
@@ -161,6 +163,24 @@ SIGNATURES = {
                 vp, vp, vp, vp, vp]),
     "helix_paged_append_chunk": (
         c_int, [vp, vp, vp, vp, c_size, c_size, c_size, c_size, vp, c_size, c_size, vp]),
+    # tree steps
+    "helix_paged_tree_workspace_bytes": (c_int, [c_size] * 4 + [P(c_size)]),
+    "helix_paged_tree_attention": (
+        c_int, [vp, c_size, c_size, c_size, c_size, c_size, vp, vp, c_size, c_size, vp, c_size,
+                vp, vp, vp, vp, vp, vp, vp, c_size, c_int, c_float, c_float, vp]),
+    "helix_verify_tree_workspace_bytes": (c_int, [c_size] * 3 + [P(c_size)]),
+    "helix_verify_tree": (
+        c_int, [vp, c_size, c_size, vp, c_size, c_size, c_size, c_size, c_size, vp, vp, vp, vp,
+                vp, vp, vp, vp, vp, c_size, vp]),
+    "helix_paged_append_path": (
+        c_int, [vp, vp, vp, vp, c_size, c_size, c_size, c_size, c_size, c_size, vp, vp, vp,
+                c_size, c_size, c_int, c_float, c_float, vp]),
+    "helix_decode_batch_prepare_tree": (c_int, [vp, c_size, vp]),
+    "helix_decode_batch_tree_layer": (c_int, [vp, c_size, vp, vp, vp, vp, vp, vp, vp]),
+    "helix_decode_batch_commit_path": (c_int, [vp, vp, vp, vp, vp, vp]),
+    "helix_decode_batch_accept_tree": (
+        c_int, [vp, vp, c_size, c_size, vp, c_size, c_size, c_size, vp, vp, vp, vp, vp, vp, vp,
+                vp, vp, vp, vp]),
     "helix_decode_batch_prepare_chunk": (c_int, [vp, c_size, vp]),
     "helix_decode_batch_append_attention_layer": (c_int, [vp, c_size, vp, vp, vp, vp, vp]),
     "helix_decode_batch_prefill_layer": (c_int, [vp, c_size, vp, vp, vp, vp, vp]),

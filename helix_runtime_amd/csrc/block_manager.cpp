@@ -240,35 +240,65 @@ std::uint64_t BlockManager::commit_fork(const ForkPlan& plan) {
 // FIFO tail in table order.
 void BlockManager::release(std::uint64_t sequence) {
   const Sequence& s = require(sequence, "release_sequence");
+  drop_blocks(s.blocks.data(), s.blocks.size());
+  --stats_.active_sequence_count;
+  stats_.active_tokens -= s.length;
+  ++stats_.release_count;
+  sequences_.erase(sequence);
+}
+
+// One reference less on each of `count` blocks.
+void BlockManager::drop_blocks(const std::uint32_t* blocks, std::size_t count) {
   std::size_t released = 0, resident = 0, unshared = 0;
-  for (const std::uint32_t b : s.blocks) {
-    if (refs_[b] == 1) {
+  for (std::size_t i = 0; i < count; ++i) {
+    const std::uint32_t b = blocks[i];
+    if (--refs_[b] == 0) {
       ++released;
       resident += tokens_[b];
-    } else if (refs_[b] == 2) {
-      ++unshared;
-    }
-  }
-  for (const std::uint32_t b : s.blocks) {
-    if (--refs_[b] == 0) {
       tokens_[b] = 0;
       fifo_[fifo_tail_] = b;
       fifo_tail_ = (fifo_tail_ + 1) % fifo_.size();
       ++free_count_;
+    } else if (refs_[b] == 1) {
+      ++unshared;
     }
   }
   stats_.used_blocks -= released;
   stats_.free_blocks += released;
   stats_.bytes_used -= released * block_bytes_;
   stats_.bytes_free += released * block_bytes_;
-  --stats_.active_sequence_count;
-  stats_.active_tokens -= s.length;
   stats_.resident_tokens -= resident;
   stats_.allocated_token_slots -= released * config_.block_tokens;
-  stats_.block_reference_count -= s.blocks.size();
+  stats_.block_reference_count -= count;
   stats_.shared_blocks -= unshared;
-  ++stats_.release_count;
-  sequences_.erase(sequence);
+}
+
+void BlockManager::require_truncatable(std::uint64_t sequence, std::size_t length) const {
+  const Sequence& s = require(sequence, "truncate_sequence");
+  check(length <= s.length, Status::kOutOfRange,
+        "truncate_sequence length exceeds the sequence length");
+  if (length == 0) return;
+  const std::size_t last = (length - 1) / config_.block_tokens;
+  const std::uint32_t b = s.blocks[last];
+  check(tokens_[b] == length - last * config_.block_tokens || refs_[b] == 1,
+        Status::kInvalidArgument,
+        "truncate_sequence would cut inside a page that another sequence shares");
+}
+
+void BlockManager::truncate(std::uint64_t sequence, std::size_t length) {
+  require_truncatable(sequence, length);
+  Sequence& s = sequences_.find(sequence)->second;
+  const std::size_t keep = blocks_for(length, config_.block_tokens);
+  if (keep != 0) {
+    std::size_t& tokens = tokens_[s.blocks[keep - 1]];
+    const std::size_t rest = length - (keep - 1) * config_.block_tokens;
+    stats_.resident_tokens -= tokens - rest;
+    tokens = rest;
+  }
+  stats_.active_tokens -= s.length - length;
+  drop_blocks(s.blocks.data() + keep, s.blocks.size() - keep);
+  s.blocks.resize(keep);
+  s.length = length;
 }
 
 void BlockManager::validate() const {

@@ -103,6 +103,12 @@ public:
                                    bool allow_copy_on_write) const;
   std::uint64_t commit_fork(const ForkPlan& plan);
   void release(std::uint64_t sequence);
+  // Drops the tokens of a sequence from `length` on (no reference counterpart):
+  // pages that hold none of the rest lose its reference, those without another
+  // go to the FIFO tail in table order.  A shared page cannot be cut inside.
+  void truncate(std::uint64_t sequence, std::size_t length);
+  // Throws what truncate() would.
+  void require_truncatable(std::uint64_t sequence, std::size_t length) const;
 
   // Free blocks the FIFO can still hand out.
   [[nodiscard]] std::size_t free_block_count() const noexcept { return free_count_; }
@@ -127,6 +133,7 @@ private:
     return fifo_[(fifo_head_ + i) % fifo_.size()];
   }
   void take_block(Sequence& s, std::uint32_t block);
+  void drop_blocks(const std::uint32_t* blocks, std::size_t count);
 
   PagedConfig config_;
   std::uint64_t cache_id_ = 0;

@@ -214,6 +214,14 @@ int helix_paged_cache_append_layer_major(helix_paged_cache* cache, helix_sequenc
   });
 }
 
+int helix_paged_cache_truncate_sequence(helix_paged_cache* cache, helix_sequence sequence,
+                                        size_t length) {
+  return guarded([&] {
+    REQUIRE_CACHE();
+    cache->cache.truncate(sequence.id, sequence.cache_id, length);
+  });
+}
+
 int helix_paged_cache_release_sequence(helix_paged_cache* cache, helix_sequence sequence) {
   return guarded([&] {
     REQUIRE_CACHE();
@@ -1207,6 +1215,262 @@ int helix_paged_prefill_attention_typed(const float* query, size_t batch, size_t
     a.physical_blocks = physical_blocks;
     a.page_type = fmt;
     helix::hip_check(helix::hip::launch_prefill(a, as_stream(stream)), op);
+  });
+}
+
+}  // extern "C"
+
+namespace {
+
+// Grid and index ranges of the tree kernels.
+void check_tree_shape(const char* op, std::size_t batch, std::size_t q_heads, std::size_t kv_heads,
+                      std::size_t nodes) {
+  check(kv_heads != 0 && q_heads != 0 && q_heads % kv_heads == 0, Status::kInvalidArgument, op,
+        "query heads must be a positive multiple of the key/value heads");
+  check(nodes <= helix::hip::kMaxTreeNodes, Status::kUnsupported, op, "trees of at most 64 nodes");
+  constexpr std::size_t kMost = std::size_t{1} << 30;
+  check(q_heads <= kMost / 64 && batch <= kMost / (q_heads * 64), Status::kInvalidArgument, op,
+        "batch too large");
+}
+
+void check_tree_tensors(const char* op, const float* query, const float* tree_key,
+                        const float* tree_value, const float* output, std::size_t batch,
+                        std::size_t q_heads, std::size_t kv_heads, std::size_t nodes) {
+  check(query && tree_key && tree_value && output, Status::kInvalidArgument, op,
+        "device pointers must be non-null");
+  check(aligned16(query) && aligned16(tree_key) && aligned16(tree_value) && aligned16(output),
+        Status::kInvalidArgument, op, "tensors must be 16-byte aligned");
+  const std::size_t row = nodes * helix::hip::kDecodeHeadDim * sizeof(float);
+  const std::size_t ob = batch * q_heads * row, tb = batch * kv_heads * row;
+  check(!overlap(output, ob, query, ob) && !overlap(output, ob, tree_key, tb) &&
+            !overlap(output, ob, tree_value, tb),
+        Status::kInvalidArgument, op, "output must not alias query or tree rows");
+}
+
+// The verification's arguments without its workspace; batch and nodes must be
+// positive.
+helix::hip::VerifyArgs verify_args(const char* op, const float* target, std::size_t target_batch_stride,
+                                   std::size_t target_node_stride, const float* draft,
+                                   std::size_t draft_batch_stride, std::size_t draft_node_stride,
+                                   std::size_t batch, std::size_t nodes, std::size_t vocab,
+                                   const int32_t* tokens, const int32_t* parents,
+                                   const int32_t* node_counts, const float* uniforms,
+                                   const float* bonus_uniforms, int32_t* path, int32_t* accepted,
+                                   int32_t* next_token) {
+  check(nodes <= helix::hip::kMaxTreeNodes, Status::kUnsupported, op, "trees of at most 64 nodes");
+  check(vocab != 0 && vocab <= (std::size_t{1} << 30), Status::kInvalidArgument, op,
+        "vocabulary size out of range");
+  check(batch <= (std::size_t{1} << 20), Status::kInvalidArgument, op, "batch too large");
+  check(target && tokens && uniforms && bonus_uniforms && path && accepted && next_token,
+        Status::kInvalidArgument, op, "device pointers must be non-null");
+  constexpr std::size_t kStride = std::size_t{1} << 40;
+  check(target_node_stride >= vocab && target_node_stride <= kStride &&
+            target_batch_stride <= kStride &&
+            (draft == nullptr || (draft_node_stride >= vocab && draft_node_stride <= kStride &&
+                                  draft_batch_stride <= kStride)),
+        Status::kInvalidArgument, op, "node strides must hold a row of the vocabulary");
+  helix::hip::VerifyArgs v{};
+  v.target = target;
+  v.target_batch_stride = target_batch_stride;
+  v.target_node_stride = target_node_stride;
+  v.draft = draft;
+  v.draft_batch_stride = draft_batch_stride;
+  v.draft_node_stride = draft_node_stride;
+  v.tokens = tokens;
+  v.parents = parents;
+  v.node_counts = node_counts;
+  v.uniforms = uniforms;
+  v.bonus_uniforms = bonus_uniforms;
+  v.path = path;
+  v.accepted = accepted;
+  v.next_token = next_token;
+  v.batch = batch;
+  v.nodes = nodes;
+  v.vocab = vocab;
+  return v;
+}
+
+}  // namespace
+
+extern "C" {
+
+// ------------------------------------------------------------ tree steps ----
+int helix_paged_tree_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t nodes,
+                                     size_t* out) {
+  return guarded([&] {
+    require_out(out);
+    check_tree_shape("paged_tree_workspace_bytes", batch, q_heads, kv_heads, nodes);
+    *out = helix::hip::tree_workspace_bytes(batch, q_heads, kv_heads, nodes);
+  });
+}
+
+int helix_paged_tree_attention(const float* query, size_t batch, size_t q_heads, size_t kv_heads,
+                               size_t nodes, size_t head_dim, const void* key_blocks,
+                               const void* value_blocks, size_t physical_blocks,
+                               size_t block_tokens, const uint32_t* tables, size_t max_blocks,
+                               const int32_t* lengths, const float* tree_key,
+                               const float* tree_value, const int32_t* parents,
+                               const int32_t* node_counts, float* output, void* workspace,
+                               size_t workspace_bytes, int page_dtype, float key_scale,
+                               float value_scale, helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "paged_tree_attention";
+    const helix::hip::PageFormat fmt = page_format(page_dtype, key_scale, value_scale, op);
+    require_kernel_geometry(head_dim, block_tokens, op);
+    check_tree_shape(op, batch, q_heads, kv_heads, nodes);
+    check(physical_blocks != 0 && physical_blocks <= std::numeric_limits<std::uint32_t>::max(),
+          Status::kInvalidArgument, op, "physical block count out of range");
+    check(max_blocks != 0 && max_blocks <= static_cast<std::size_t>(
+                                               std::numeric_limits<std::int32_t>::max() / 32),
+          Status::kInvalidArgument, op, "max_blocks out of range");
+    if (batch == 0 || nodes == 0) return;
+    check(key_blocks && value_blocks && tables && lengths, Status::kInvalidArgument, op,
+          "device pointers must be non-null");
+    check(aligned16(key_blocks) && aligned16(value_blocks), Status::kInvalidArgument, op,
+          "tensors must be 16-byte aligned");
+    check_tree_tensors(op, query, tree_key, tree_value, output, batch, q_heads, kv_heads, nodes);
+    check(workspace != nullptr && aligned16(workspace), Status::kInvalidArgument, op,
+          "workspace must be a non-null 16-byte aligned device pointer");
+    check(workspace_bytes >= helix::hip::tree_workspace_bytes(batch, q_heads, kv_heads, nodes),
+          Status::kInvalidArgument, op, "workspace is too small");
+    check(!overlap(output, batch * q_heads * nodes * head_dim * sizeof(float), workspace,
+                   workspace_bytes),
+          Status::kInvalidArgument, op, "output must not alias the workspace");
+    helix::hip::TreeAttentionArgs a{};
+    a.query = query;
+    a.key_pool = key_blocks;
+    a.value_pool = value_blocks;
+    a.tables = tables;
+    a.lengths = lengths;
+    a.tree_key = tree_key;
+    a.tree_value = tree_value;
+    a.parents = parents;
+    a.node_counts = node_counts;
+    a.out = output;
+    a.workspace = workspace;
+    a.batch = batch;
+    a.q_heads = q_heads;
+    a.kv_heads = kv_heads;
+    a.nodes = nodes;
+    a.max_blocks = max_blocks;
+    a.physical_blocks = physical_blocks;
+    a.page_type = fmt;
+    helix::hip_check(helix::hip::launch_tree_attention(a, as_stream(stream)), op);
+  });
+}
+
+int helix_verify_tree_workspace_bytes(size_t batch, size_t nodes, size_t vocab, size_t* out) {
+  return guarded([&] {
+    require_out(out);
+    check(nodes <= helix::hip::kMaxTreeNodes, Status::kUnsupported, "verify_tree_workspace_bytes",
+          "trees of at most 64 nodes");
+    check(batch <= (std::size_t{1} << 20) && vocab <= (std::size_t{1} << 30),
+          Status::kInvalidArgument, "verify_tree_workspace_bytes", "batch or vocabulary too large");
+    *out = helix::hip::verify_workspace_bytes(batch, nodes, vocab);
+  });
+}
+
+int helix_verify_tree(const float* target, size_t target_batch_stride, size_t target_node_stride,
+                      const float* draft, size_t draft_batch_stride, size_t draft_node_stride,
+                      size_t batch, size_t nodes, size_t vocab, const int32_t* tokens,
+                      const int32_t* parents, const int32_t* node_counts, const float* uniforms,
+                      const float* bonus_uniforms, int32_t* path, int32_t* accepted,
+                      int32_t* next_token, void* workspace, size_t workspace_bytes,
+                      helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "verify_tree";
+    if (batch == 0 || nodes == 0) return;
+    helix::hip::VerifyArgs v = verify_args(
+        op, target, target_batch_stride, target_node_stride, draft, draft_batch_stride,
+        draft_node_stride, batch, nodes, vocab, tokens, parents, node_counts, uniforms,
+        bonus_uniforms, path, accepted, next_token);
+    check(workspace != nullptr && aligned16(workspace), Status::kInvalidArgument, op,
+          "workspace must be a non-null 16-byte aligned device pointer");
+    check(workspace_bytes >= helix::hip::verify_workspace_bytes(batch, nodes, vocab),
+          Status::kInvalidArgument, op, "workspace is too small");
+    v.workspace = workspace;
+    helix::hip_check(helix::hip::launch_verify(v, as_stream(stream)), op);
+  });
+}
+
+int helix_paged_append_path(const float* keys, const float* values, void* key_blocks,
+                            void* value_blocks, size_t layers, size_t layer_stride,
+                            size_t physical_blocks, size_t kv_heads, size_t block_tokens,
+                            size_t head_dim, const int64_t* slots, const int32_t* path,
+                            const int32_t* accepted, size_t batch, size_t nodes, int page_dtype,
+                            float key_scale, float value_scale, helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "append_path";
+    const helix::hip::PageFormat fmt = page_format(page_dtype, key_scale, value_scale, op);
+    check(physical_blocks != 0 && kv_heads != 0 && block_tokens != 0 && head_dim != 0,
+          Status::kInvalidArgument, op, "geometry must be positive");
+    const std::size_t page = mul(mul(kv_heads, block_tokens), head_dim);
+    const std::size_t layer = mul(page, physical_blocks);
+    check(layers <= 32767, Status::kInvalidArgument, op, "at most 32767 layers");
+    check(layers <= 1 || layer_stride >= layer, Status::kInvalidArgument, op,
+          "the layer stride must hold a layer's pool");
+    static_cast<void>(mul(mul(layer_stride, layers), sizeof(float)));
+    check(kv_heads <= 0xffffffffu / head_dim && nodes <= 0xffffffffu &&
+              (nodes == 0 || batch <= 0xffffffffu / nodes) && block_tokens <= 0xffffffffu,
+          Status::kInvalidArgument, op, "rows out of range");
+    if (batch == 0 || nodes == 0 || layers == 0) return;
+    check(keys && values && key_blocks && value_blocks && slots && path && accepted,
+          Status::kInvalidArgument, op, "device pointers must be non-null");
+    helix::hip_check(
+        helix::hip::launch_append_path(
+            keys, values, key_blocks, value_blocks,
+            helix::hip::PageGeometry{physical_blocks, kv_heads, block_tokens, head_dim}, slots,
+            path, accepted, batch, nodes, as_stream(stream), fmt, layers, layer_stride),
+        op);
+  });
+}
+
+int helix_decode_batch_prepare_tree(helix_decode_batch* b, size_t nodes, helix_stream stream) {
+  return guarded([&] {
+    check(b != nullptr, Status::kInvalidArgument, "decode batch must not be NULL");
+    b->batch->prepare_tree(as_stream(stream), nodes);
+  });
+}
+
+int helix_decode_batch_tree_layer(helix_decode_batch* b, size_t layer, const float* query,
+                                  const float* tree_key, const float* tree_value,
+                                  const int32_t* parents, const int32_t* node_counts,
+                                  float* output, helix_stream stream) {
+  return guarded([&] {
+    check(b != nullptr, Status::kInvalidArgument, "decode batch must not be NULL");
+    check_tree_tensors("decode batch tree attention", query, tree_key, tree_value, output,
+                       b->batch->batch(), b->batch->q_heads(), b->batch->kv_heads(),
+                       b->batch->step_tokens());
+    b->batch->tree_layer(layer, query, tree_key, tree_value, parents, node_counts, output,
+                         as_stream(stream));
+  });
+}
+
+int helix_decode_batch_commit_path(helix_decode_batch* b, const float* keys, const float* values,
+                                   const int32_t* path, const int32_t* accepted,
+                                   helix_stream stream) {
+  return guarded([&] {
+    check(b != nullptr, Status::kInvalidArgument, "decode batch must not be NULL");
+    b->batch->commit_path(keys, values, path, accepted, as_stream(stream));
+  });
+}
+
+int helix_decode_batch_accept_tree(helix_decode_batch* b, const float* target,
+                                   size_t target_batch_stride, size_t target_node_stride,
+                                   const float* draft, size_t draft_batch_stride,
+                                   size_t draft_node_stride, size_t vocab, const int32_t* tokens,
+                                   const int32_t* parents, const int32_t* node_counts,
+                                   const float* uniforms, const float* bonus_uniforms,
+                                   const float* keys, const float* values, int32_t* path,
+                                   int32_t* accepted, int32_t* next_token, helix_stream stream) {
+  return guarded([&] {
+    check(b != nullptr, Status::kInvalidArgument, "decode batch must not be NULL");
+    const helix::hip::VerifyArgs v = verify_args(
+        "decode batch accept_tree", target, target_batch_stride, target_node_stride, draft,
+        draft_batch_stride, draft_node_stride, b->batch->batch(),
+        std::min(b->batch->step_tokens(), helix::hip::kMaxTreeNodes),
+        vocab, tokens, parents, node_counts, uniforms, bonus_uniforms, path, accepted, next_token);
+    b->batch->accept_tree(v, keys, values, as_stream(stream));
   });
 }
 

@@ -128,6 +128,15 @@ int helix_block_manager_release_sequence(helix_block_manager* m, helix_sequence 
   });
 }
 
+int helix_block_manager_truncate(helix_block_manager* m, helix_sequence sequence, size_t length) {
+  return guarded([&] {
+    check(m != nullptr, Status::kInvalidArgument, "manager must not be NULL");
+    std::scoped_lock lock(m->mutex);
+    require_manager_handle(m->manager, sequence, "truncate_sequence");
+    m->manager.truncate(sequence.id, length);
+  });
+}
+
 int helix_block_manager_contains(const helix_block_manager* m, helix_sequence sequence,
                                  int* out) {
   return guarded([&] {

@@ -210,6 +210,44 @@ __global__ __launch_bounds__(256) void append_slots_kernel(
   }
 }
 
+// Append of a tree step's accepted nodes: row path[b, i], i < accepted[b], of
+// sequence b goes to slots[b, i].  One thread moves W elements of one row of
+// one layer's K or V; grid as append_slots_kernel's, y over (sequence, i).
+template <typename S, int W>
+__global__ __launch_bounds__(256) void append_path_kernel(
+    const float* __restrict__ keys, const float* __restrict__ values, S* key_pool, S* value_pool,
+    std::size_t layer_stride, unsigned heads, unsigned block_tokens, unsigned dim,
+    const std::int64_t* __restrict__ slots, const std::int32_t* __restrict__ path,
+    const std::int32_t* __restrict__ accepted, unsigned count, unsigned tokens,
+    std::size_t slot_limit, float2 scale) {
+  const unsigned dv = dim / W;
+  const unsigned i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= heads * dv) return;
+  const unsigned h = i / dv;
+  const unsigned c = i - h * dv;
+  const bool is_value = (blockIdx.z & 1u) != 0;
+  const std::size_t l = blockIdx.z >> 1;
+  const float* src = is_value ? values : keys;
+  const float sc = is_value ? scale.y : scale.x;
+  S* pool = (is_value ? value_pool : key_pool) + l * layer_stride;
+  const unsigned rows = count * tokens;
+  for (unsigned bt = blockIdx.y; bt < rows; bt += gridDim.y) {
+    const unsigned b = bt / tokens;
+    if (static_cast<std::int64_t>(bt - b * tokens) >= accepted[b]) continue;
+    const std::int32_t node = path[bt];
+    const std::int64_t slot = slots[bt];
+    if (node < 0 || static_cast<unsigned>(node) >= tokens || slot < 0 ||
+        static_cast<std::size_t>(slot) >= slot_limit) {
+      continue;
+    }
+    const std::size_t block = static_cast<std::size_t>(slot) / block_tokens;
+    const std::size_t off = static_cast<std::size_t>(slot) % block_tokens;
+    const std::size_t e = (((l * count + b) * heads + h) * tokens + node) * dv + c;
+    Elems<S, W>::put(pool + ((block * heads + h) * block_tokens + off) * dim + c * W, src + e * W,
+                     sc);
+  }
+}
+
 // ---------------------------------------------------------------- rope ----
 // Rotary embedding of adjacent pairs (2i, 2i+1) of head vectors, as
 // cpu::rope_out (src/kernels/cpu/reference.cpp:490-533): out[2i] =
@@ -2402,6 +2440,33 @@ hipError_t launch_append_slots(const float* keys, const float* values, void* key
         static_cast<unsigned>(g.kv_heads), static_cast<unsigned>(g.block_tokens),
         static_cast<unsigned>(g.head_dim), slots, static_cast<unsigned>(count),
         static_cast<unsigned>(tokens), scales(type));
+  });
+}
+
+hipError_t launch_append_path(const float* keys, const float* values, void* key_pool,
+                              void* value_pool, const PageGeometry& g, const std::int64_t* slots,
+                              const std::int32_t* path, const std::int32_t* accepted,
+                              std::size_t count, std::size_t tokens, hipStream_t stream,
+                              PageFormat type, std::size_t layers, std::size_t layer_stride) {
+  if (count == 0 || tokens == 0 || layers == 0) return hipSuccess;
+  const bool vec = g.head_dim % 4 == 0 && aligned16(keys) && aligned16(values) &&
+                   aligned16(key_pool) && aligned16(value_pool) && layer_stride % 4 == 0;
+  const std::size_t per_row = g.kv_heads * (vec ? g.head_dim / 4 : g.head_dim);
+  const std::size_t rows = count * tokens;
+  if (rows > 0xffffffffu || layers * 2 > 65535 || per_row > 0xffffffffu) {
+    return hipErrorInvalidValue;
+  }
+  const dim3 grid(static_cast<unsigned>((per_row + kThreads - 1) / kThreads),
+                  static_cast<unsigned>(rows < 65535 ? rows : 65535),
+                  static_cast<unsigned>(layers * 2));
+  return with_page_type(type, vec, [&](auto s, auto w) {
+    using S = decltype(s);
+    constexpr int W = decltype(w)::value;
+    append_path_kernel<S, W><<<grid, kThreads, 0, stream>>>(
+        keys, values, as_pages<S>(key_pool), as_pages<S>(value_pool), layer_stride,
+        static_cast<unsigned>(g.kv_heads), static_cast<unsigned>(g.block_tokens),
+        static_cast<unsigned>(g.head_dim), slots, path, accepted, static_cast<unsigned>(count),
+        static_cast<unsigned>(tokens), g.physical_blocks * g.block_tokens, scales(type));
   });
 }
 

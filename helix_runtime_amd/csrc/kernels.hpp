@@ -75,6 +75,17 @@ hipError_t launch_append_slots(const float* keys, const float* values, void* key
                                PageFormat type = PageFormat(), std::size_t layers = 1,
                                std::size_t layer_stride = 0);
 
+// Append of a tree step's accepted path: src [layers, count, kv_heads, tokens,
+// dim]; for i < accepted[b], row path[b * tokens + i] of sequence b goes to the
+// flat slot slots[b * tokens + i] of each layer (a node outside [0, tokens) or
+// a slot outside the pool: skipped).
+hipError_t launch_append_path(const float* keys, const float* values, void* key_pool,
+                              void* value_pool, const PageGeometry& g, const std::int64_t* slots,
+                              const std::int32_t* path, const std::int32_t* accepted,
+                              std::size_t count, std::size_t tokens, hipStream_t stream,
+                              PageFormat type = PageFormat(), std::size_t layers = 1,
+                              std::size_t layer_stride = 0);
+
 // Rotary embedding (cpu::rope_out, bit-exact) of up to two tensors
 // [rows, vectors, head_dim] whose rows share positions; row r uses cache row
 // positions[r] (positions == nullptr: row r).  rows * vectors * head_dim / 2

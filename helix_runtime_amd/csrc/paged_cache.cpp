@@ -250,6 +250,15 @@ void DevicePagedCache::release(std::uint64_t sequence, std::uint64_t cache_id) {
   state_->releases.fetch_add(1, std::memory_order_release);
 }
 
+void DevicePagedCache::truncate(std::uint64_t sequence, std::uint64_t cache_id,
+                                std::size_t length) {
+  std::scoped_lock lock(state_->mutex);
+  state_->require_sequence(sequence, cache_id, "truncate_sequence");
+  state_->manager.truncate(sequence, length);
+  ++state_->truncations;
+  state_->releases.fetch_add(1, std::memory_order_release);
+}
+
 void DevicePagedCache::copy_layer_out(std::uint64_t sequence, std::uint64_t cache_id,
                                       std::size_t layer, std::size_t expected_length,
                                       float* keys_out, float* values_out, std::size_t dest_tokens,
@@ -481,10 +490,24 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
   CacheState& s = *state_;
   std::scoped_lock lock(s.mutex);
   prepared_ = false;
-  step_tokens_ = 0;
   s.require_healthy("decode batch prepare");
+  drop_tree();
+  step_tokens_ = 0;
   const PagedConfig& c = s.manager.config();
   const std::size_t B = batch();
+  if (seen_truncations_ != s.truncations) {
+    // A member's row may have shrunk and grown again: the entries that still
+    // hold count as mirrored, the others are uploaded with this step.
+    for (std::size_t i = 0; i < B; ++i) {
+      if (!s.manager.contains(sequences_[i])) continue;
+      const std::vector<std::uint32_t>& row = s.manager.blocks(sequences_[i]);
+      const std::size_t most = std::min(mirrored_[i], row.size());
+      std::size_t k = 0;
+      while (k < most && mirror_[i * max_blocks_ + k] == row[k]) ++k;
+      mirrored_[i] = k;
+    }
+    seen_truncations_ = s.truncations;
+  }
   check(tokens != 0, Status::kInvalidArgument, "decode batch prepare needs at least one token");
   check(tokens <= max_blocks_ * c.block_tokens, Status::kOutOfRange,
         "decode batch prepare: more tokens than the batch's max_tokens");
@@ -625,6 +648,12 @@ void DecodeBatch::begin_call(hipStream_t stream, const char* op) const {
     for (std::uint64_t seq : sequences_) {
       check(s.manager.contains(seq), Status::kInvalidArgument,
             std::string(op) + ": a sequence of the batch was released after prepare");
+    }
+    for (std::size_t i = 0; i < batch(); ++i) {
+      check(s.manager.length(sequences_[i]) >=
+                static_cast<std::size_t>(host_lengths_[i]) + step_tokens_,
+            Status::kInvalidArgument,
+            std::string(op) + ": a sequence of the batch was truncated after prepare");
     }
     prepared_releases_ = s.releases.load(std::memory_order_acquire);
   }
@@ -774,6 +803,149 @@ void DecodeBatch::prefill_layer(std::size_t layer, const float* query, const flo
   DeviceGuard guard(state_->device);
   begin_call(stream, "decode batch prefill");
   hip_check(hip::launch_prefill(a, stream), "decode batch prefill launch");
+}
+
+// Takes the slots of an uncommitted tree step back (under the cache mutex).
+// The step's calls read the pages before them only.
+void DecodeBatch::drop_tree() {
+  if (!tree_step_) return;
+  CacheState& s = *state_;
+  // (A member that someone released, truncated or appended to is theirs.)
+  const auto reserved = [&](std::size_t i) {
+    return s.manager.contains(sequences_[i]) &&
+           s.manager.length(sequences_[i]) ==
+               static_cast<std::size_t>(host_lengths_[i]) + step_tokens_;
+  };
+  for (std::size_t i = 0; i < batch(); ++i) {
+    if (reserved(i)) {
+      s.manager.require_truncatable(sequences_[i], static_cast<std::size_t>(host_lengths_[i]));
+    }
+  }
+  for (std::size_t i = 0; i < batch(); ++i) {
+    if (reserved(i)) {
+      s.manager.truncate(sequences_[i], static_cast<std::size_t>(host_lengths_[i]));
+    }
+  }
+  tree_step_ = false;
+  ++s.truncations;
+  s.releases.fetch_add(1, std::memory_order_release);
+}
+
+void DecodeBatch::prepare_tree(hipStream_t stream, std::size_t nodes) {
+  check(nodes != 0 && nodes <= hip::kMaxTreeNodes, Status::kInvalidArgument,
+        "decode batch prepare_tree: trees of 1 to 64 nodes");
+  const PagedConfig& c = state_->manager.config();
+  const std::size_t bytes = hip::tree_workspace_bytes(batch(), q_heads_, c.kv_heads, nodes);
+  if (tree_workspace_.size() < bytes || accepted_.data() == nullptr) {
+    DeviceGuard guard(state_->device);
+    // Queued kernels of earlier steps may still use the smaller one.
+    hip_check(hipDeviceSynchronize(), "decode batch tree workspace");
+    if (tree_workspace_.size() < bytes) tree_workspace_ = DeviceBuffer(bytes, state_->device);
+    if (accepted_.data() == nullptr) accepted_ = PinnedBuffer(batch() * sizeof(std::int32_t));
+  }
+  prepare(stream, nodes);
+  tree_step_ = true;
+}
+
+void DecodeBatch::require_tree_step(const char* op) const {
+  check(prepared_ && tree_step_, Status::kInvalidArgument,
+        std::string(op) + " needs a step of prepare_tree");
+}
+
+void DecodeBatch::tree_layer(std::size_t layer, const float* query, const float* tree_key,
+                             const float* tree_value, const std::int32_t* parents,
+                             const std::int32_t* node_counts, float* out,
+                             hipStream_t stream) const {
+  const PagedConfig& c = state_->manager.config();
+  require_tree_step("decode batch tree attention");
+  check(layer < c.layers, Status::kOutOfRange, "decode batch layer is out of range");
+  check(query != nullptr && tree_key != nullptr && tree_value != nullptr && out != nullptr,
+        Status::kInvalidArgument, "decode batch tree attention needs query, tree rows and output");
+  hip::TreeAttentionArgs a{};
+  a.query = query;
+  a.key_pool = state_->key_pool(layer);
+  a.value_pool = state_->value_pool(layer);
+  a.tables = tables();
+  a.lengths = lengths();
+  a.tree_key = tree_key;
+  a.tree_value = tree_value;
+  a.parents = parents;
+  a.node_counts = node_counts;
+  a.out = out;
+  a.workspace = tree_workspace_.data();
+  a.batch = batch();
+  a.q_heads = q_heads_;
+  a.kv_heads = c.kv_heads;
+  a.nodes = step_tokens_;
+  a.max_blocks = max_blocks_;
+  a.physical_blocks = c.physical_blocks;
+  a.page_type = state_->page_type;
+  DeviceGuard guard(state_->device);
+  begin_call(stream, "decode batch tree attention");
+  hip_check(hip::launch_tree_attention(a, stream), "decode batch tree attention launch");
+}
+
+void DecodeBatch::append_path(const float* keys, const float* values, const std::int32_t* path,
+                              const std::int32_t* accepted, hipStream_t stream) {
+  const PagedConfig& c = state_->manager.config();
+  hip_check(hip::launch_append_path(keys, values, state_->key_pool(0), state_->value_pool(0),
+                                    geometry(c), slots(), path, accepted, batch(), step_tokens_,
+                                    stream, state_->page_type, c.layers, state_->layer_stride()),
+            "decode batch path append launch");
+  hip_check(hipMemcpyAsync(accepted_.data(), accepted, batch() * sizeof(std::int32_t),
+                           hipMemcpyDeviceToHost, stream),
+            "decode batch accepted download");
+  CacheState& s = *state_;
+  std::scoped_lock lock(s.mutex);
+  synchronize_or_poison(s, stream, "decode batch commit_path");
+  const auto* number = static_cast<const std::int32_t*>(accepted_.data());
+  for (std::size_t i = 0; i < batch(); ++i) {
+    check(number[i] >= 0 && static_cast<std::size_t>(number[i]) <= step_tokens_,
+          Status::kInvalidArgument, "decode batch commit_path: accepted counts lie in [0, nodes]");
+    check(s.manager.contains(sequences_[i]) &&
+              s.manager.length(sequences_[i]) ==
+                  static_cast<std::size_t>(host_lengths_[i]) + step_tokens_,
+          Status::kInvalidArgument,
+          "decode batch commit_path: a sequence changed after prepare_tree");
+    s.manager.require_truncatable(sequences_[i],
+                                  static_cast<std::size_t>(host_lengths_[i] + number[i]));
+  }
+  for (std::size_t i = 0; i < batch(); ++i) {
+    s.manager.truncate(sequences_[i], static_cast<std::size_t>(host_lengths_[i] + number[i]));
+  }
+  ++s.truncations;
+  s.releases.fetch_add(1, std::memory_order_release);
+  tree_step_ = false;
+  prepared_ = false;
+}
+
+void DecodeBatch::commit_path(const float* keys, const float* values, const std::int32_t* path,
+                              const std::int32_t* accepted, hipStream_t stream) {
+  require_tree_step("decode batch commit_path");
+  check(keys != nullptr && values != nullptr && path != nullptr && accepted != nullptr,
+        Status::kInvalidArgument, "decode batch commit_path needs rows, path and accepted counts");
+  DeviceGuard guard(state_->device);
+  begin_call(stream, "decode batch commit_path");
+  append_path(keys, values, path, accepted, stream);
+}
+
+void DecodeBatch::accept_tree(hip::VerifyArgs v, const float* keys, const float* values,
+                              hipStream_t stream) {
+  require_tree_step("decode batch accept_tree");
+  check(keys != nullptr && values != nullptr, Status::kInvalidArgument,
+        "decode batch accept_tree needs the tree's key and value rows");
+  v.batch = batch();
+  v.nodes = step_tokens_;
+  const std::size_t bytes = hip::verify_workspace_bytes(v.batch, v.nodes, v.vocab);
+  DeviceGuard guard(state_->device);
+  if (verify_workspace_.size() < bytes) {
+    hip_check(hipDeviceSynchronize(), "decode batch verification workspace");
+    verify_workspace_ = DeviceBuffer(bytes, state_->device);
+  }
+  v.workspace = verify_workspace_.data();
+  begin_call(stream, "decode batch accept_tree");
+  hip_check(hip::launch_verify(v, stream), "decode batch verification launch");
+  append_path(keys, values, v.path, v.accepted, stream);
 }
 
 }  // namespace helix

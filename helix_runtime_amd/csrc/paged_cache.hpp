@@ -11,6 +11,7 @@
 
 #include "block_manager.hpp"
 #include "kernels.hpp"
+#include "tree.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -83,6 +84,9 @@ struct CacheState {
   // value at its last prepare() to notice that a member may have been
   // released between the step's calls.
   std::atomic<std::uint64_t> releases{0};
+  // Truncations so far, for the same purpose (counted among `releases` too):
+  // the rows of a truncated member's table may have shrunk.
+  std::uint64_t truncations = 0;
   DeviceBuffer staging;            // transient upload area (grown on demand)
 
   // Layer pools: fp32 elements, or bf16 / fp8 bits for a reduced-precision
@@ -124,6 +128,7 @@ public:
                           const float* const* layer_keys, const float* const* layer_values,
                           std::size_t tokens, hipStream_t stream);
   void release(std::uint64_t sequence, std::uint64_t cache_id);
+  void truncate(std::uint64_t sequence, std::uint64_t cache_id, std::size_t length);
   // Gathers exactly `expected_length` tokens (or the current length when
   // expected_length is SIZE_MAX) of one layer into [kv_heads, dest_tokens,
   // head_dim] device buffers and synchronises the stream.
@@ -172,7 +177,8 @@ private:
 //    prepare(): each prepare() uploads every table entry the device copy
 //    does not hold yet;
 //  - a member released after prepare() makes every later per-step call fail
-//    (kInvalidArgument) until the next prepare(), which fails too;
+//    (kInvalidArgument) until the next prepare(), which fails too; so does one
+//    truncated below the step, until the next prepare();
 //  - a per-step call on a stream other than prepare()'s waits for the step
 //    upload, and prepare() on a stream other than the previous step's last
 //    call waits for that call.  Per-step calls of one step on different
@@ -209,12 +215,36 @@ public:
   void append_attention_layer(std::size_t layer, const float* query, const float* keys,
                               const float* values, float* out, hipStream_t stream) const;
 
+  // A step over a tree of `nodes` drafted tokens per sequence: reserves their
+  // slots; tree_layer() is each layer's attention, commit_path() keeps the
+  // accepted nodes, accept_tree() verifies the drafts and then does.  A tree
+  // step that the next prepare finds uncommitted is dropped: its members go
+  // back to their lengths before it.
+  void prepare_tree(hipStream_t stream, std::size_t nodes);
+  // query, out [batch, q_heads, nodes, 128]; tree_key/value [batch, kv_heads,
+  // nodes, 128]; parents [batch, nodes] (nullptr: a chain), node_counts [batch]
+  // (nullptr: all nodes), device arrays.
+  void tree_layer(std::size_t layer, const float* query, const float* tree_key,
+                  const float* tree_value, const std::int32_t* parents,
+                  const std::int32_t* node_counts, float* out, hipStream_t stream) const;
+  // Writes the rows [layers, batch, kv_heads, nodes, dim] of path[b, i], i <
+  // accepted[b], to the sequence's next slots in every layer, synchronises the
+  // stream and truncates each member to its accepted tokens.  path [batch,
+  // nodes], accepted [batch]: device arrays.
+  void commit_path(const float* keys, const float* values, const std::int32_t* path,
+                   const std::int32_t* accepted, hipStream_t stream);
+  // launch_verify, then commit_path() of what it accepted (`v` without a
+  // workspace: the batch's own is used).
+  void accept_tree(hip::VerifyArgs v, const float* keys, const float* values, hipStream_t stream);
+
   [[nodiscard]] const std::uint32_t* tables() const;
   [[nodiscard]] const std::int32_t* lengths() const;
   [[nodiscard]] const std::int64_t* slots() const;
   [[nodiscard]] std::size_t max_blocks() const noexcept { return max_blocks_; }
   [[nodiscard]] std::size_t pages_per_split() const noexcept { return pages_per_split_; }
   [[nodiscard]] std::size_t batch() const noexcept { return sequences_.size(); }
+  [[nodiscard]] std::size_t q_heads() const noexcept { return q_heads_; }
+  [[nodiscard]] std::size_t kv_heads() const noexcept { return state_->manager.config().kv_heads; }
   [[nodiscard]] std::size_t step_tokens() const noexcept { return step_tokens_; }
   [[nodiscard]] std::size_t shared_pages() const noexcept { return shared_pages_; }
   // Measurement hook: when set, attention_layer() records this event between
@@ -258,6 +288,12 @@ private:
   // device copy holds (table rows only grow while a sequence lives).
   std::vector<std::uint32_t> mirror_;
   std::vector<std::size_t> mirrored_;
+  std::uint64_t seen_truncations_ = 0;
+  // A tree step was prepared and is neither committed nor dropped.
+  bool tree_step_ = false;
+  DeviceBuffer tree_workspace_;
+  DeviceBuffer verify_workspace_;
+  PinnedBuffer accepted_;
   mutable std::uint64_t prepared_releases_ = 0;
   hipStream_t prepared_stream_ = nullptr;
   int prepared_event_ = 0;  // uploaded_[prepared_event_] follows the step upload
@@ -266,6 +302,10 @@ private:
   hipEvent_t order_event_ = nullptr;
 
   void reserve_step(std::size_t tokens);
+  void drop_tree();
+  void require_tree_step(const char* op) const;
+  void append_path(const float* keys, const float* values, const std::int32_t* path,
+                   const std::int32_t* accepted, hipStream_t stream);
   // Checks that the step is prepared and its members still live, and orders
   // `stream` after the step upload.
   void begin_call(hipStream_t stream, const char* op) const;

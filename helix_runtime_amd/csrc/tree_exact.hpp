@@ -1,0 +1,235 @@
+// Attention of 16 query rows of a drafted tree by one wavefront, in plain
+// fp32 arithmetic: every score a sum of products of fp32 values, every key a
+// row does not see left out rather than weighted with 0, so that infinities
+// and NaN reach exactly the rows that see them.
+//
+// A lane holds dims 2 lane, 2 lane + 1 of the 16 query rows, of a key and of
+// its value.  A key's 16 scores are partial sums in every lane; four halving
+// exchanges and two additions leave row lane / 4's score in each lane, which
+// keeps that row's maximum and sum.  The 16 probabilities come back through
+// v_readlane.  About 130 vector instructions per key and 16 rows: 0.2 us a
+// key, so this is for what needs it, not for the usual case.
+#pragma once
+
+#include "prefill_body.hpp"
+#include "tree.hpp"
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+namespace helix::hip::tree_detail {
+
+using prefill_detail::exp2_ratio;
+
+constexpr int D = 128;
+constexpr int P = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct TreeKernelArgs {
+  const float* query;
+  const void* key_pool;
+  const void* value_pool;
+  const std::uint32_t* tables;
+  const std::int32_t* lengths;
+  const float* tree_key;
+  const float* tree_value;
+  const std::int32_t* parents;
+  const std::int32_t* node_counts;
+  float* out;
+  int batch, q_heads, kv_heads, nodes, max_blocks;
+  int rows;  // query rows of a (sequence, kv head): q_heads / kv_heads * nodes
+  std::uint32_t physical_blocks;
+  float qscale;  // log2(e) / sqrt(128)
+  float k_scale, v_scale;
+};
+
+// One sequence's history, nodes and ancestor words.
+struct TreeSequence {
+  int hist;   // history tokens; 0 where the given length is outside the table
+  int count;  // nodes
+  bool bad;   // length outside the table, or a page outside the pool
+  // Lane t: the nodes that node t sees (itself among them), 0 for a node
+  // behind the count; `broken`: node t or one of its ancestors has a parent
+  // that does not come before it.
+  unsigned long long seen;
+  bool broken;
+};
+
+__device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int src) {
+  const unsigned lo = __shfl(static_cast<unsigned>(v), src, 64);
+  const unsigned hi = __shfl(static_cast<unsigned>(v >> 32), src, 64);
+  return static_cast<unsigned long long>(hi) << 32 | lo;
+}
+
+__device__ __forceinline__ int clamped_history(const TreeKernelArgs& a, int b) {
+  const int hist = a.lengths[b];
+  return hist < 0 || hist > a.max_blocks * P ? -1 : hist;
+}
+
+__device__ __forceinline__ int clamped_nodes(const TreeKernelArgs& a, int b) {
+  return a.node_counts != nullptr ? min(max(a.node_counts[b], 0), a.nodes) : a.nodes;
+}
+
+// The ancestors of all nodes by doubling: after step k a lane's word holds the
+// 2^k nearest, itself first.
+__device__ __forceinline__ TreeSequence tree_sequence(const TreeKernelArgs& a, int b, int lane) {
+  TreeSequence s{};
+  const int hist = clamped_history(a, b);
+  s.bad = hist < 0;
+  s.hist = __builtin_amdgcn_readfirstlane(max(hist, 0));
+  s.count = __builtin_amdgcn_readfirstlane(clamped_nodes(a, b));
+  int up = -1;
+  bool wrong = false;
+  if (lane < s.count) {
+    up = a.parents != nullptr ? a.parents[static_cast<std::size_t>(b) * a.nodes + lane] : lane - 1;
+    wrong = up < -1 || up >= lane;
+    if (wrong) up = -1;
+    s.seen = 1ull << lane;
+  }
+#pragma unroll 1
+  for (int k = 1; k < a.nodes; k *= 2) {
+    const unsigned long long more = shfl64(s.seen, max(up, 0));
+    const int next = __shfl(up, max(up, 0), 64);
+    if (up >= 0) {
+      s.seen |= more;
+      up = next;
+    }
+  }
+  s.broken = (s.seen & __ballot(wrong)) != 0;
+  return s;
+}
+
+// Two consecutive elements at element offset e of a pool, as the values they
+// stand for.
+template <int PF>
+__device__ __forceinline__ float2 page_pair(const void* pool, std::size_t e, float scale) {
+  if constexpr (PF == 1) {
+    const unsigned w = *reinterpret_cast<const unsigned*>(
+        static_cast<const unsigned short*>(pool) + e);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else if constexpr (PF == 2) {
+    const unsigned w =
+        *reinterpret_cast<const unsigned short*>(static_cast<const unsigned char*>(pool) + e);
+    const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+    return make_float2(v[0] * scale, v[1] * scale);
+  } else {
+    return *reinterpret_cast<const float2*>(static_cast<const float*>(pool) + e);
+  }
+}
+
+// Two fp32 values of a tree row as their page will hold them.
+template <int PF>
+__device__ __forceinline__ float2 row_pair(const float* row, float scale) {
+  const float2 x = *reinterpret_cast<const float2*>(row);
+  if constexpr (PF == 1) {
+    return make_float2(bf16_value(bf16_round(x.x)), bf16_value(bf16_round(x.y)));
+  } else if constexpr (PF == 2) {
+    const float4 r = fp8_rounded(make_float4(x.x, x.y, 0.f, 0.f), scale);
+    return make_float2(r.x, r.y);
+  } else {
+    return x;
+  }
+}
+
+// Rows [row0, row0 + 16) of the (sequence b, kv head) over history tokens
+// [k0, k1) and tree nodes [n0, n1).  Leaves row i's unnormalised output in
+// o[i] (this lane's two dims) and row lane / 4's maximum (log2 units) and sum.
+template <int PF>
+__device__ __forceinline__ void exact_rows(const TreeKernelArgs& a, const TreeSequence& s, int b,
+                                           int kvh, int row0, int k0, int k1, int n0, int n1,
+                                           int lane, float2 (&o)[16], float& m, float& l,
+                                           bool& bad_page) {
+  const std::uint32_t* const table = a.tables + static_cast<std::size_t>(b) * a.max_blocks;
+  const std::size_t unit_rows =
+      (static_cast<std::size_t>(b) * a.q_heads + static_cast<std::size_t>(kvh) *
+                                                     (a.q_heads / a.kv_heads)) * a.nodes;
+  float2 q[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    q[i] = o[i] = make_float2(0.f, 0.f);
+    if (row0 + i < a.rows) {
+      q[i] = *reinterpret_cast<const float2*>(a.query + (unit_rows + row0 + i) * D + 2 * lane);
+      q[i].x *= a.qscale;
+      q[i].y *= a.qscale;
+    }
+  }
+  m = -INFINITY;
+  l = 0.f;
+  // Ancestor word of row lane / 4 (row r is node r % nodes of its head).
+  const int my_row = row0 + (lane >> 2);
+  const unsigned long long word = shfl64(s.seen, my_row % a.nodes);
+  const unsigned long long mine = my_row < a.rows ? word : 0ull;
+
+  auto key = [&](const float2& k, const float2& v, bool seen, unsigned long long rows_seeing) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = q[i].x * k.x + q[i].y * k.y;
+#pragma unroll
+    for (int w = 8, bit = 32; w >= 1; w /= 2, bit /= 2) {
+      const bool high = (lane & bit) != 0;
+#pragma unroll
+      for (int i = 0; i < w; ++i) {
+        const float give = high ? x[i] : x[i + w];
+        const float keep = high ? x[i + w] : x[i];
+        x[i] = keep + __shfl_xor(give, bit, 64);
+      }
+    }
+    float sc = x[0] + __shfl_xor(x[0], 2, 64);
+    sc += __shfl_xor(sc, 1, 64);
+    const float mn = seen ? fmaxf(m, sc) : m;
+    const float alpha = exp2_ratio(m, mn);
+    const float p = seen ? exp2_ratio(sc, mn) : 0.f;
+    l = l * alpha + p;
+    const bool moved = __ballot(!(mn == m)) != 0;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (moved) {
+        const float al =
+            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(alpha), 4 * i));
+        o[i].x *= al;
+        o[i].y *= al;
+      }
+      if ((rows_seeing >> (4 * i)) & 1) {
+        const float pi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), 4 * i));
+        o[i].x += pi * v.x;
+        o[i].y += pi * v.y;
+      }
+    }
+  };
+
+  constexpr int A = 4;  // keys whose rows are loaded at once
+  const float ks = PF == 2 ? a.k_scale : 1.0f, vs = PF == 2 ? a.v_scale : 1.0f;
+  for (int j = k0; j < k1; j += A) {
+    float2 k[A], v[A];
+#pragma unroll
+    for (int u = 0; u < A; ++u) {
+      const int pos = min(j + u, k1 - 1);
+      const std::uint32_t page = table[pos / P];
+      const bool ok = page < a.physical_blocks;
+      bad_page = bad_page || !ok;
+      k[u] = v[u] = make_float2(0.f, 0.f);
+      if (ok) {
+        const std::size_t e =
+            ((static_cast<std::size_t>(page) * a.kv_heads + kvh) * P + pos % P) * D + 2 * lane;
+        k[u] = page_pair<PF>(a.key_pool, e, ks);
+        v[u] = page_pair<PF>(a.value_pool, e, vs);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < A; ++u) {
+      if (j + u < k1) key(k[u], v[u], true, ~0ull);
+    }
+  }
+  const std::size_t tree0 = (static_cast<std::size_t>(b) * a.kv_heads + kvh) * a.nodes;
+  for (int j = n0; j < n1; ++j) {
+    const float2 k = row_pair<PF>(a.tree_key + (tree0 + j) * D + 2 * lane, ks);
+    const float2 v = row_pair<PF>(a.tree_value + (tree0 + j) * D + 2 * lane, vs);
+    const bool seen = ((mine >> j) & 1) != 0;
+    key(k, v, seen, __ballot(seen));
+  }
+}
+
+}  // namespace helix::hip::tree_detail

@@ -99,6 +99,12 @@ int helix_block_manager_append(helix_block_manager* m, helix_sequence sequence, 
                                uint64_t* slots);
 /* PagedKvCache::release_sequence (paged.cpp:952-1001). */
 int helix_block_manager_release_sequence(helix_block_manager* m, helix_sequence sequence);
+/* Drops the tokens from `length` on (extension; no reference counterpart):
+ * pages that hold none of the rest lose the sequence's reference, and those
+ * without another return to the FIFO tail in table order.  HELIX_OUT_OF_RANGE
+ * past the sequence's length; HELIX_INVALID_ARGUMENT where it would cut inside
+ * a page that another sequence shares. */
+int helix_block_manager_truncate(helix_block_manager* m, helix_sequence sequence, size_t length);
 int helix_block_manager_contains(const helix_block_manager* m, helix_sequence sequence, int* out);
 int helix_block_manager_length(const helix_block_manager* m, helix_sequence sequence,
                                size_t* out);
@@ -170,6 +176,10 @@ int helix_paged_cache_append_layer_major(helix_paged_cache* cache, helix_sequenc
                                          helix_stream stream);
 /* CudaPagedKvCache::release_sequence (cuda_paged.cpp:613-643). */
 int helix_paged_cache_release_sequence(helix_paged_cache* cache, helix_sequence sequence);
+/* helix_block_manager_truncate of a cache's sequence (extension): metadata
+ * only, as release_sequence is. */
+int helix_paged_cache_truncate_sequence(helix_paged_cache* cache, helix_sequence sequence,
+                                        size_t length);
 /* PagedKvCache::copy_layer_out (paged.cpp:887-893): device outputs
  * [kv_heads, length, head_dim]; synchronises the stream. */
 int helix_paged_cache_copy_layer_out(helix_paged_cache* cache, helix_sequence sequence,
@@ -425,6 +435,77 @@ int helix_paged_append_chunk(const float* keys, const float* values, float* key_
                              size_t block_tokens, size_t head_dim, const int64_t* slots,
                              size_t batch, size_t tokens, helix_stream stream);
 
+/* -------------------------------------------- tree steps (extension) ---- */
+/* A step that checks a tree of drafted tokens per sequence at once (no
+ * reference counterpart): attention in every layer, verification of the
+ * drafts, append of the accepted ones.  A tree has up to 64 nodes.  Node 0 is
+ * its root, the last generated token (whose K/V row is not in the pages yet);
+ * parents[b, t] < t is node t's parent, -1 that of a root, and parents NULL
+ * makes every tree a chain.  node_counts [batch] (NULL: all nodes) gives each
+ * sequence's own number of nodes, taken into [0, nodes]; rows behind it are
+ * not computed, and outputs there stay as they were.
+ *
+ * Attention: query row (h, t) sees the lengths[b] history tokens of row b of
+ * `tables`, its ancestors' rows of tree_key / tree_value and its own.
+ *   query, output [batch, q_heads, nodes, head_dim];
+ *   tree_key, tree_value [batch, kv_heads, nodes, head_dim] fp32, rounded onto
+ *   the pools' grid as helix_paged_decode_attention_typed rounds its tail;
+ *   pools, tables, lengths, page_dtype and scales as there.
+ * head_dim 128 and 16-token pages, any multiple of kv_heads as q_heads;
+ * HELIX_UNSUPPORTED otherwise, and for trees of more than 64 nodes.  A length
+ * outside the table, a page outside the pool or a parent that does not come
+ * before its node give NaN in the rows they reach.  The workspace needs no
+ * initial value; calls that overlap on one workspace race. */
+int helix_paged_tree_workspace_bytes(size_t batch, size_t q_heads, size_t kv_heads, size_t nodes,
+                                     size_t* out);
+int helix_paged_tree_attention(const float* query, size_t batch, size_t q_heads, size_t kv_heads,
+                               size_t nodes, size_t head_dim, const void* key_blocks,
+                               const void* value_blocks, size_t physical_blocks,
+                               size_t block_tokens, const uint32_t* tables, size_t max_blocks,
+                               const int32_t* lengths, const float* tree_key,
+                               const float* tree_value, const int32_t* parents,
+                               const int32_t* node_counts, float* output, void* workspace,
+                               size_t workspace_bytes, int page_dtype, float key_scale,
+                               float value_scale, helix_stream stream);
+/* Verification against the target's probabilities, from given uniform random
+ * numbers in [0, 1).  target row (b, n) is the target's distribution after node
+ * n, draft row (b, n) the one that the children of n were drawn from, each
+ * vocab entries with the given batch and node strides (in elements); draft NULL:
+ * the drafts were certain.  From n = 0 with w = target row 0, the children of n
+ * are tried in order: child c with token x is accepted, and becomes n, where
+ * uniforms[c] * draft_n(x) < w(x); otherwise w becomes max(w - draft_n, 0)
+ * divided by its sum.  (draft NULL: accepted where uniforms[c] * m < w(x), m
+ * being 1 less the target's probabilities of the children rejected before; a
+ * rejected token's w becomes 0.)  Where no child is left, next_token is the
+ * smallest v with w(0) + .. + w(v) > bonus_uniforms[b] * sum w; where rounding
+ * has left w no positive entry, the target's row stands for it, and next_token
+ * is -1 where that has none either.  All of it in 64 bits.
+ *   path [batch, nodes]: the accepted nodes from the root down, then -1;
+ *   accepted [batch]: their number, the root among them (0 and next_token -1
+ *   for a sequence without nodes).
+ * Nodes with a token outside the vocabulary or a parent that does not come
+ * before them are never accepted.  The workspace as above. */
+int helix_verify_tree_workspace_bytes(size_t batch, size_t nodes, size_t vocab, size_t* out);
+int helix_verify_tree(const float* target, size_t target_batch_stride, size_t target_node_stride,
+                      const float* draft, size_t draft_batch_stride, size_t draft_node_stride,
+                      size_t batch, size_t nodes, size_t vocab, const int32_t* tokens,
+                      const int32_t* parents, const int32_t* node_counts, const float* uniforms,
+                      const float* bonus_uniforms, int32_t* path, int32_t* accepted,
+                      int32_t* next_token, void* workspace, size_t workspace_bytes,
+                      helix_stream stream);
+/* Append of the accepted nodes in one launch: rows [layers, batch, kv_heads,
+ * nodes, head_dim] of node path[b, i], i < accepted[b], go to slots[b, i] =
+ * block * block_tokens + offset of each of `layers` pools that start
+ * layer_stride elements apart (a node outside [0, nodes) or a slot outside the
+ * pool is skipped; two rows of one slot race).  Any head size and page size;
+ * page_dtype and scales as helix_paged_decode_attention_typed. */
+int helix_paged_append_path(const float* keys, const float* values, void* key_blocks,
+                            void* value_blocks, size_t layers, size_t layer_stride,
+                            size_t physical_blocks, size_t kv_heads, size_t block_tokens,
+                            size_t head_dim, const int64_t* slots, const int32_t* path,
+                            const int32_t* accepted, size_t batch, size_t nodes, int page_dtype,
+                            float key_scale, float value_scale, helix_stream stream);
+
 /* A decode driver over a cache: persistent device block tables for a fixed
  * set of sequences.  prepare() reserves one slot per sequence (allocating
  * pages), append_layer() writes it, attention_layer() attends over the
@@ -484,6 +565,31 @@ int helix_decode_batch_attention_layer(helix_decode_batch* b, size_t layer, cons
 int helix_decode_batch_prefill_layer(helix_decode_batch* b, size_t layer, const float* query,
                                      const float* chunk_key, const float* chunk_value,
                                      float* output, helix_stream stream);
+/* A tree step (helix_paged_tree_attention, helix_verify_tree,
+ * helix_paged_append_path over the batch): prepare_tree() reserves `nodes` slots
+ * per sequence, tree_layer() is one layer's attention, and commit_path() writes
+ * the accepted nodes' rows [layers, batch, kv_heads, nodes, head_dim] to the
+ * sequences' next slots in every layer, synchronises the stream and truncates
+ * each sequence to its accepted tokens, which frees the pages behind them.
+ * accept_tree() verifies the drafts first.  path, accepted and next_token are
+ * device arrays.  A tree step that the next prepare call finds uncommitted is
+ * dropped: its sequences go back to their lengths before it. */
+int helix_decode_batch_prepare_tree(helix_decode_batch* b, size_t nodes, helix_stream stream);
+int helix_decode_batch_tree_layer(helix_decode_batch* b, size_t layer, const float* query,
+                                  const float* tree_key, const float* tree_value,
+                                  const int32_t* parents, const int32_t* node_counts,
+                                  float* output, helix_stream stream);
+int helix_decode_batch_commit_path(helix_decode_batch* b, const float* keys, const float* values,
+                                   const int32_t* path, const int32_t* accepted,
+                                   helix_stream stream);
+int helix_decode_batch_accept_tree(helix_decode_batch* b, const float* target,
+                                   size_t target_batch_stride, size_t target_node_stride,
+                                   const float* draft, size_t draft_batch_stride,
+                                   size_t draft_node_stride, size_t vocab, const int32_t* tokens,
+                                   const int32_t* parents, const int32_t* node_counts,
+                                   const float* uniforms, const float* bonus_uniforms,
+                                   const float* keys, const float* values, int32_t* path,
+                                   int32_t* accepted, int32_t* next_token, helix_stream stream);
 int helix_decode_batch_tables(const helix_decode_batch* b, const uint32_t** tables,
                               const int32_t** lengths, const int64_t** slots,
                               size_t* max_blocks, size_t* pages_per_split);
