@@ -1,14 +1,8 @@
-// Attention of 16 query rows of a drafted tree by one wavefront, in plain
-// fp32 arithmetic: every score a sum of products of fp32 values, every key a
-// row does not see left out rather than weighted with 0, so that infinities
-// and NaN reach exactly the rows that see them.
-//
-// A lane holds dims 2 lane, 2 lane + 1 of the 16 query rows, of a key and of
-// its value.  A key's 16 scores are partial sums in every lane; four halving
-// exchanges and two additions leave row lane / 4's score in each lane, which
-// keeps that row's maximum and sum.  The 16 probabilities come back through
-// v_readlane.  About 130 vector instructions per key and 16 rows: 0.2 us a
-// key, so this is for what needs it, not for the usual case.
+// What the kernels of a tree step's attention share, and its plain form: one
+// query row by one wavefront in fp32 arithmetic, every score a sum of products
+// of fp32 values, every key the row does not see left out rather than weighted
+// with 0, so that infinities and NaN reach exactly the rows that see them.
+// A lane holds dims 2 lane, 2 lane + 1 of the row, of a key and of its value.
 #pragma once
 
 #include "prefill_body.hpp"
@@ -49,12 +43,12 @@ struct TreeKernelArgs {
 struct TreeSequence {
   int hist;   // history tokens; 0 where the given length is outside the table
   int count;  // nodes
-  bool bad;   // length outside the table, or a page outside the pool
+  int bad;    // length outside the table, or a page outside the pool
   // Lane t: the nodes that node t sees (itself among them), 0 for a node
   // behind the count; `broken`: node t or one of its ancestors has a parent
   // that does not come before it.
   unsigned long long seen;
-  bool broken;
+  int broken;
 };
 
 __device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int src) {
@@ -133,85 +127,48 @@ __device__ __forceinline__ float2 row_pair(const float* row, float scale) {
   }
 }
 
-// Rows [row0, row0 + 16) of the (sequence b, kv head) over history tokens
-// [k0, k1) and tree nodes [n0, n1).  Leaves row i's unnormalised output in
-// o[i] (this lane's two dims) and row lane / 4's maximum (log2 units) and sum.
+// Row `row` of the (sequence b, kv head) over history tokens [k0, k1) and the
+// nodes [n0, n1) that its word `seen` has: its maximum (log2 units), its sum and
+// this lane's two dims of its unnormalised output.  (Pages outside the pool are
+// left out; the caller knows of them.)
 template <int PF>
-__device__ __forceinline__ void exact_rows(const TreeKernelArgs& a, const TreeSequence& s, int b,
-                                           int kvh, int row0, int k0, int k1, int n0, int n1,
-                                           int lane, float2 (&o)[16], float& m, float& l,
-                                           bool& bad_page) {
+__device__ __forceinline__ void exact_row(const TreeKernelArgs& a, int b, int kvh, int row, int k0,
+                                          int k1, int n0, int n1, unsigned long long seen,
+                                          int lane, float2& o, float& m, float& l) {
   const std::uint32_t* const table = a.tables + static_cast<std::size_t>(b) * a.max_blocks;
   const std::size_t unit_rows =
       (static_cast<std::size_t>(b) * a.q_heads + static_cast<std::size_t>(kvh) *
                                                      (a.q_heads / a.kv_heads)) * a.nodes;
-  float2 q[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    q[i] = o[i] = make_float2(0.f, 0.f);
-    if (row0 + i < a.rows) {
-      q[i] = *reinterpret_cast<const float2*>(a.query + (unit_rows + row0 + i) * D + 2 * lane);
-      q[i].x *= a.qscale;
-      q[i].y *= a.qscale;
-    }
-  }
+  float2 q = *reinterpret_cast<const float2*>(a.query + (unit_rows + row) * D + 2 * lane);
+  q.x *= a.qscale;
+  q.y *= a.qscale;
+  o = make_float2(0.f, 0.f);
   m = -INFINITY;
   l = 0.f;
-  // Ancestor word of row lane / 4 (row r is node r % nodes of its head).
-  const int my_row = row0 + (lane >> 2);
-  const unsigned long long word = shfl64(s.seen, my_row % a.nodes);
-  const unsigned long long mine = my_row < a.rows ? word : 0ull;
-
-  auto key = [&](const float2& k, const float2& v, bool seen, unsigned long long rows_seeing) {
-    float x[16];
+  auto key = [&](const float2& k, const float2& v) {
+    float x = q.x * k.x + q.y * k.y;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = q[i].x * k.x + q[i].y * k.y;
-#pragma unroll
-    for (int w = 8, bit = 32; w >= 1; w /= 2, bit /= 2) {
-      const bool high = (lane & bit) != 0;
-#pragma unroll
-      for (int i = 0; i < w; ++i) {
-        const float give = high ? x[i] : x[i + w];
-        const float keep = high ? x[i + w] : x[i];
-        x[i] = keep + __shfl_xor(give, bit, 64);
-      }
-    }
-    float sc = x[0] + __shfl_xor(x[0], 2, 64);
-    sc += __shfl_xor(sc, 1, 64);
-    const float mn = seen ? fmaxf(m, sc) : m;
-    const float alpha = exp2_ratio(m, mn);
-    const float p = seen ? exp2_ratio(sc, mn) : 0.f;
+    for (int bit = 32; bit >= 1; bit /= 2) x += __shfl_xor(x, bit, 64);
+    const float mn = fmaxf(m, x);
+    const float alpha = exp2_ratio(m, mn), p = exp2_ratio(x, mn);
     l = l * alpha + p;
-    const bool moved = __ballot(!(mn == m)) != 0;
+    o.x = o.x * alpha + p * v.x;
+    o.y = o.y * alpha + p * v.y;
     m = mn;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (moved) {
-        const float al =
-            __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(alpha), 4 * i));
-        o[i].x *= al;
-        o[i].y *= al;
-      }
-      if ((rows_seeing >> (4 * i)) & 1) {
-        const float pi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), 4 * i));
-        o[i].x += pi * v.x;
-        o[i].y += pi * v.y;
-      }
-    }
   };
-
-  constexpr int A = 4;  // keys whose rows are loaded at once
+  constexpr int A = 8;  // keys whose rows are loaded at once
   const float ks = PF == 2 ? a.k_scale : 1.0f, vs = PF == 2 ? a.v_scale : 1.0f;
+#pragma unroll 1
   for (int j = k0; j < k1; j += A) {
     float2 k[A], v[A];
+    bool ok[A];
 #pragma unroll
     for (int u = 0; u < A; ++u) {
       const int pos = min(j + u, k1 - 1);
       const std::uint32_t page = table[pos / P];
-      const bool ok = page < a.physical_blocks;
-      bad_page = bad_page || !ok;
+      ok[u] = j + u < k1 && page < a.physical_blocks;
       k[u] = v[u] = make_float2(0.f, 0.f);
-      if (ok) {
+      if (ok[u]) {
         const std::size_t e =
             ((static_cast<std::size_t>(page) * a.kv_heads + kvh) * P + pos % P) * D + 2 * lane;
         k[u] = page_pair<PF>(a.key_pool, e, ks);
@@ -220,15 +177,15 @@ __device__ __forceinline__ void exact_rows(const TreeKernelArgs& a, const TreeSe
     }
 #pragma unroll
     for (int u = 0; u < A; ++u) {
-      if (j + u < k1) key(k[u], v[u], true, ~0ull);
+      if (ok[u]) key(k[u], v[u]);
     }
   }
   const std::size_t tree0 = (static_cast<std::size_t>(b) * a.kv_heads + kvh) * a.nodes;
+#pragma unroll 1
   for (int j = n0; j < n1; ++j) {
-    const float2 k = row_pair<PF>(a.tree_key + (tree0 + j) * D + 2 * lane, ks);
-    const float2 v = row_pair<PF>(a.tree_value + (tree0 + j) * D + 2 * lane, vs);
-    const bool seen = ((mine >> j) & 1) != 0;
-    key(k, v, seen, __ballot(seen));
+    if (((seen >> j) & 1) == 0) continue;
+    key(row_pair<PF>(a.tree_key + (tree0 + j) * D + 2 * lane, ks),
+        row_pair<PF>(a.tree_value + (tree0 + j) * D + 2 * lane, vs));
   }
 }
 
