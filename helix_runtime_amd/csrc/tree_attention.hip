@@ -143,7 +143,7 @@ __device__ __forceinline__ uint4 codes_fp16(unsigned w0, unsigned w1) {
 // 16 bytes of each plane a chunk of 8 elements becomes in LDS: from 8 fp32
 // values (a tree row, or an fp32 page), rounded onto the page grid.
 template <int PF>
-__device__ __forceinline__ void chunk_of_rows(const v4f& x0, const v4f& x1, float scale,
+__device__ __forceinline__ void chunk_of_rows(v4f x0, v4f x1, float scale,
                                               uint4 (&t)[page_terms(PF)]) {
   if constexpr (PF == 0) {
     unsigned w[4][3];
@@ -349,8 +349,11 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         const int node = (c.blk - c.nbh) * kBlock + min(row, seen - 1);
         const std::size_t e =
             ((static_cast<std::size_t>(c.b) * a.kv_heads + c.kvh) * a.nodes + node) * D + part * 8;
-        const auto* k = reinterpret_cast<const v4f*>(a.tree_key + e);
-        const auto* v = reinterpret_cast<const v4f*>(a.tree_value + e);
+        // (Global address space, or the compiler merges these loads with reads of
+        // kr and vr, which must stay in registers.)
+        using Rows = const __attribute__((address_space(1))) v4f*;
+        const auto k = reinterpret_cast<Rows>(reinterpret_cast<std::uintptr_t>(a.tree_key + e));
+        const auto v = reinterpret_cast<Rows>(reinterpret_cast<std::uintptr_t>(a.tree_value + e));
         chunk_of_rows<PF>(k[0], k[1], a.k_scale, kt);
         chunk_of_rows<PF>(v[0], v[1], a.v_scale, vt);
       } else if constexpr (PF == 0) {
@@ -661,7 +664,7 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
 }
 
 template <int PF, int W, int RT>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(RT == 2 ? 2 : W == 4 ? (PF == 0 ? 3 : 4) : W == 2 ? (PF == 0 ? 2 : 3) : (PF==0?1:2)))) void tree_mma_kernel(TreeKernelArgs a, TreeStream st) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PF == 0 ? (W == 1 ? 1 : 2) : W <= 2 || RT == 2 ? 2 : 3))) void tree_mma_kernel(TreeKernelArgs a, TreeStream st) {
   __shared__ TreeShared<PF, W * RT> sh;
   tree_mma_body<PF, W, RT>(a, st, sh);
 }
