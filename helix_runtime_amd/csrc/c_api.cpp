@@ -1355,6 +1355,8 @@ int helix_paged_tree_attention(const float* query, size_t batch, size_t q_heads,
     a.max_blocks = max_blocks;
     a.physical_blocks = physical_blocks;
     a.page_type = fmt;
+    check(helix::hip::tree_fits(a), Status::kUnsupported, op,
+          "the block tables span too many keys for one call");
     helix::hip_check(helix::hip::launch_tree_attention(a, as_stream(stream)), op);
   });
 }

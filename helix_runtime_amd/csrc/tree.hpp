@@ -45,6 +45,8 @@ struct TreeAttentionArgs {
 };
 std::size_t tree_workspace_bytes(std::size_t batch, std::size_t q_heads, std::size_t kv_heads,
                                  std::size_t nodes);
+// Whether the launch's blocks of keys can be counted; where not, it fails.
+bool tree_fits(const TreeAttentionArgs& a);
 hipError_t launch_tree_attention(const TreeAttentionArgs& a, hipStream_t stream);
 
 // Row strides in elements; draft == nullptr: every drafted token was certain

@@ -29,7 +29,7 @@
 //   terms (22 bits and a sign: the rounding of an fp32 number): 2 products.
 //   Terms must stay above fp16's smallest numbers: a query row is scaled by a
 //   power of two that puts its largest element in [2^10, 2^11), and
-//   probabilities (with them sums and outputs) carry a factor of 2^14;
+//   probabilities (with them sums and outputs) carry a factor of 2^8;
 // - fp32 pages: three bf16 terms on either side, less the products below
 //   2^-26 of the largest: 6 products, 2.7 times the rate of fp32 matrix
 //   instructions.
@@ -44,6 +44,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -74,7 +75,11 @@ constexpr int kBlock = 32;  // keys of a block: two pages
 // Terms of a page element and of the fp32 factor against it.
 constexpr int page_terms(int pf) { return pf == 0 ? 3 : 1; }
 constexpr int row_terms(int pf) { return pf == 2 ? 2 : 3; }
-constexpr float kProbScale = 16384.0f;  // fp8 pages
+// fp8 pages: the factor on probabilities, and its logarithm.
+constexpr float kProbScale = 256.0f, kProbLog = 8.0f;
+// A row's reference stays while no score is above it by more than this (log2
+// units): fp16's largest number is 2^16.
+constexpr float kSlack = 7.0f;
 
 constexpr int kMaxTiles = 16;           // 16-row tiles of a unit
 
@@ -104,11 +109,15 @@ struct TreeStream {
 template <int PF>
 __device__ __forceinline__ void split_pair(float x, float y, unsigned (&t)[3]) {
   if constexpr (PF == 2) {
-    const v2h hi = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
-    const v2h lo = {static_cast<_Float16>(x - static_cast<float>(hi[0])),
-                    static_cast<_Float16>(y - static_cast<float>(hi[1]))};
+    const v2h hi = __builtin_convertvector((v2f{x, y}), v2h);
+    // One mixed-precision instruction a remainder: the compiler must not see
+    // that the factor is -1.
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    x = __builtin_fmaf(static_cast<float>(hi[0]), minus, x);
+    y = __builtin_fmaf(static_cast<float>(hi[1]), minus, y);
     t[0] = __builtin_bit_cast(unsigned, hi);
-    t[1] = __builtin_bit_cast(unsigned, lo);
+    t[1] = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2h));
   } else {
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -120,8 +129,14 @@ __device__ __forceinline__ void split_pair(float x, float y, unsigned (&t)[3]) {
   }
 }
 
+// The larger of two numbers, NaN where either is one (one instruction; fmaxf
+// takes two more to quiet its arguments).
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
 template <int PF>
-__device__ __forceinline__ v4f matrix_step(uint4 a, uint4 b, v4f c) {
+__device__ __forceinline__ v4f matrix_step(v4u a, v4u b, v4f c) {
   if constexpr (PF == 2) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
                                                   __builtin_bit_cast(v8h, b), c, 0, 0, 0);
@@ -132,19 +147,19 @@ __device__ __forceinline__ v4f matrix_step(uint4 a, uint4 b, v4f c) {
 }
 
 // Eight fp8 codes as fp16.
-__device__ __forceinline__ uint4 codes_fp16(unsigned w0, unsigned w1) {
-  return make_uint4(
+__device__ __forceinline__ v4u codes_fp16(unsigned w0, unsigned w1) {
+  return v4u{
       __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false)),
       __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true)),
       __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false)),
-      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true)));
+      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true))};
 }
 
-// 16 bytes of each plane a chunk of 8 elements becomes in LDS: from 8 fp32
-// values (a tree row, or an fp32 page), rounded onto the page grid.
+// 16 bytes of each plane that 8 elements become in LDS: from 8 fp32 values (a
+// tree row, or an fp32 page), rounded onto the page grid.
 template <int PF>
 __device__ __forceinline__ void chunk_of_rows(v4f x0, v4f x1, float scale,
-                                              uint4 (&t)[page_terms(PF)]) {
+                                              v4u (&t)[page_terms(PF)]) {
   if constexpr (PF == 0) {
     unsigned w[4][3];
     split_pair<0>(x0[0], x0[1], w[0]);
@@ -152,22 +167,35 @@ __device__ __forceinline__ void chunk_of_rows(v4f x0, v4f x1, float scale,
     split_pair<0>(x1[0], x1[1], w[2]);
     split_pair<0>(x1[2], x1[3], w[3]);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) t[i] = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
+    for (int i = 0; i < 3; ++i) t[i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
   } else if constexpr (PF == 1) {
-    t[0] = make_uint4(bf16_pack(x0[0], x0[1]), bf16_pack(x0[2], x0[3]), bf16_pack(x1[0], x1[1]),
-                      bf16_pack(x1[2], x1[3]));
+    t[0] = v4u{bf16_pack(x0[0], x0[1]), bf16_pack(x0[2], x0[3]), bf16_pack(x1[0], x1[1]),
+               bf16_pack(x1[2], x1[3])};
   } else {
     t[0] = codes_fp16(fp8_pack4_scaled(make_float4(x0[0], x0[1], x0[2], x0[3]), scale),
                       fp8_pack4_scaled(make_float4(x1[0], x1[1], x1[2], x1[3]), scale));
   }
 }
 
-template <int PF, int TILES>
+// Whether the wavefronts of a workgroup take turns (tree_mma_body), and the
+// LDS buffers that takes: a block is put there two steps before its use, or one
+// step, or (fp32 pages, whose three planes would take the space of a second
+// workgroup) just before it.
+constexpr bool in_turns(int pf, int waves) { return pf == 1 && waves > 4; }
+constexpr int stage_buffers(int pf, int waves) {
+  return pf == 0 ? 1 : in_turns(pf, waves) ? 3 : 2;
+}
+
+template <int PF, int W, int RT>
 struct TreeShared {
-  __align__(1024) unsigned char k[page_terms(PF)][kBlock * 2 * D];
-  __align__(1024) unsigned char v[page_terms(PF)][kBlock * 2 * D];
+  // Item i: K of block i and V of block i - 1.
+  struct Item {
+    __align__(1024) unsigned char k[page_terms(PF)][kBlock * 2 * D];
+    __align__(1024) unsigned char v[page_terms(PF)][kBlock * 2 * D];
+  };
+  Item item[stage_buffers(PF, W)];
   // The third terms of the query operands: [tile][step][lane].
-  __align__(16) uint4 low[row_terms(PF) == 3 ? TILES : 1][row_terms(PF) == 3 ? 4 : 1][64];
+  __align__(16) v4u low[row_terms(PF) == 3 ? W * RT : 1][row_terms(PF) == 3 ? 4 : 1][64];
 };
 
 // A place in the flat list of blocks.
@@ -214,7 +242,7 @@ __device__ __forceinline__ long long lane_scan(int v, int lane) {
 
 // This group's range of blocks [g0, g1) (ranges of `each`) and its first place.
 struct TreeRange {
-  long long g0, g1, each;
+  long long g0, g1, each;  // (a range's length fits 31 bits: tree_fits)
 };
 __device__ __forceinline__ TreeRange first_place(const TreeKernelArgs& a, const TreeStream& st,
                                                  int group, int lane, TreeCursor& c) {
@@ -267,134 +295,229 @@ __device__ __forceinline__ void advance(const TreeKernelArgs& a, const TreeStrea
   } while (c.nb == 0);
 }
 
+// The rows of a block that is, or is not, one of tree rows.
+struct TreeSource {
+  std::size_t at;  // element offset of its tree rows
+  int tree;        // tree rows
+  int rows;        // rows of it that are the sequence's
+  int bad;         // of a sequence with a length or page that is none
+};
+
 // W wavefronts of RT tiles of 16 query rows: units of RB = 16 W RT rows.
+//
+// Step n of a wavefront: it puts its share of a later item (K of a block, V of
+// the block before) from registers into LDS and sends for the next one's; turns
+// block n's scores into probabilities; and, past a barrier, takes block n's P V
+// and the scores of block n + 1, matrix instructions one behind another.
+// With up to four wavefronts a workgroup has one on each SIMD, and those of
+// other workgroups run beside it.  With more, the first four and the others
+// take turns: a second barrier and half a step between them have one of a
+// SIMD's two wavefronts at its matrix instructions while the other is at its
+// vector instructions.
 template <int PF, int W, int RT>
 __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const TreeStream& st,
-                                              TreeShared<PF, W * RT>& sh) {
-  constexpr int NT = 64 * W;
-  constexpr int NC = kBlock * D / 8 / NT;  // 8-element chunks of K (and of V) per thread
+                                              TreeShared<PF, W, RT>& sh) {
+  // 1 KiB of 16-bit elements in LDS, four rows, is a job of a wavefront: eight
+  // for K, and the same rows' for V.
+  static_assert(8 % W == 0);
+  constexpr int NJ = 8 / W;
   constexpr int RB = 16 * W * RT;
   constexpr int KT = page_terms(PF), QT = row_terms(PF);
+  constexpr int NB = stage_buffers(PF, W);
+  constexpr bool kTurns = in_turns(PF, W);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int group = static_cast<int>(blockIdx.x);
+  // (Between scheduling barriers: register work that the compiler moves across
+  // lands among the matrix instructions behind it.)
   auto barrier = [] {
-    if constexpr (W == 1) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   if (tid == 0) st.jobs[group] = TreeJob{-1, 0, 0, 0, 0, 0};
   TreeCursor cur{};
   const TreeRange range = first_place(a, st, group, lane, cur);
   if (range.g0 >= range.g1) return;
+  const int blocks = static_cast<int>(range.g1 - range.g0);
 
-  // Pages of the unit in hand, 64 at a time: lane i holds page ids_at + i.
-  unsigned ids = 0;
-  int ids_b = -1, ids_at = 0;
-  bool bad_page = false;
-
-  // A block's rows on their way: chunk tid + NT i, row chunk / 16.
-  using Raw = std::conditional_t<PF == 0, v4f, std::conditional_t<PF == 1, v4u, v2u>>;
-  constexpr int RW = PF == 0 ? 2 : 1;
-  Raw kr[NC * RW], vr[NC * RW];
-  auto load_block = [&](const TreeCursor& c) {
-    if (c.blk >= c.nbh) return;  // tree rows are loaded when they are stored
-    const int first = 2 * c.blk;
-    if (ids_b != c.b || first < ids_at || first >= ids_at + 64) {
-      ids_b = c.b;
-      ids_at = first;
-      const int last = (c.hist - 1) / P;
-      ids = a.tables[static_cast<std::size_t>(c.b) * a.max_blocks + min(first + lane, last)];
-    }
-    // (Behind the history the last page is read again; a page outside the pool
-    // is not read.)
-    auto page_at = [&](int h) {
-      unsigned page = __builtin_amdgcn_readlane(ids, first + h - ids_at);
-      if (page >= a.physical_blocks) {
-        bad_page = true;
-        page = 0;
-      }
-      return (static_cast<std::size_t>(page) * a.kv_heads + c.kvh) * (P * D);
-    };
-    const std::size_t at0 = page_at(0), at1 = page_at(1);
-    constexpr int kElem = PF == 0 ? 4 : PF == 1 ? 2 : 1;
+  // Pages of the (sequence, kv head) being loaded, 64 at a time: lane i holds
+  // the byte offset of page pages_at + i in the pools.  (Behind the history the
+  // last page is read again; a page outside the pool is not read.)
+  constexpr int kElem = PF == 0 ? 4 : PF == 1 ? 2 : 1;
+  unsigned page_lo = 0, page_hi = 0;
+  int pages_of = -1, pages_at = 0;
+  int bad_page = 0;  // some of them are none
+  // Job i of this wavefront: rows 4 j + grp, j = wave + W i, 8 elements from 8 col
+  // on, of K and V.  key_at[i]: this lane's bytes of K in the page pool, of
+  // the block located last; V's are as far on in its pool, one block later.
+  // Before any block of pages: page 0.
+  unsigned long long key_at[NJ], value_at[NJ];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int base = wave * 64 + NT * i;  // of the wavefront's chunks, in one page
-      const std::size_t e = ((base >= 256 ? at1 : at0) + (base & 255) * 8) * kElem;
-      const auto* k = reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(a.key_pool) + e) +
-                      static_cast<unsigned>(lane * RW);
-      const auto* v = reinterpret_cast<const Raw*>(static_cast<const unsigned char*>(a.value_pool) + e) +
-                      static_cast<unsigned>(lane * RW);
+  for (int i = 0; i < NJ; ++i) {
+    key_at[i] = reinterpret_cast<std::uintptr_t>(a.key_pool);
+    value_at[i] = reinterpret_cast<std::uintptr_t>(a.value_pool);
+  }
+  const unsigned long long value_off = static_cast<unsigned long long>(
+      static_cast<const unsigned char*>(a.value_pool) - static_cast<const unsigned char*>(a.key_pool));
+  auto job = [&](int i) { return wave + W * i; };
+  auto locate_pages = [&](int first) {
 #pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        kr[i * RW + w] = k[w];
-        vr[i * RW + w] = v[w];
-      }
+    for (int i = 0; i < NJ; ++i) {
+      const int n = first + ((job(i) >> 2) & 1);
+      const unsigned lo = __builtin_amdgcn_readlane(page_lo, n);
+      const unsigned hi = __builtin_amdgcn_readlane(page_hi, n);
+      key_at[i] = (static_cast<unsigned long long>(hi) << 32 | lo) +
+                  static_cast<unsigned>((4 * job(i) % P) * (D * kElem) + lane * (8 * kElem)) +
+                  reinterpret_cast<std::uintptr_t>(a.key_pool);
     }
   };
-  auto store_block = [&](const TreeCursor& c) {
-    const bool tree = c.blk >= c.nbh;
-    const int seen = tree ? c.count - (c.blk - c.nbh) * kBlock : c.hist - c.blk * kBlock;
+  auto locate = [&](const TreeCursor& c) {
+    TreeSource s{};
+    s.bad = c.bad;
+    if (__builtin_expect(c.blk >= c.nbh, 0)) {
+      const int first = (c.blk - c.nbh) * kBlock;
+      s.tree = 1;
+      s.rows = c.count - first;
+      s.at = ((static_cast<std::size_t>(c.b) * a.kv_heads + c.kvh) * a.nodes + first) * D;
+      return s;
+    }
+    s.rows = c.hist - c.blk * kBlock;
+    const int unit = c.kvh * a.batch + c.b;
+    int first = 2 * c.blk - pages_at;
+    if (__builtin_expect(pages_of != unit || first < 0 || first >= 64, 0)) {
+      pages_of = unit;
+      pages_at = 2 * c.blk;
+      first = 0;
+      unsigned page = a.tables[static_cast<std::size_t>(c.b) * a.max_blocks +
+                               min(pages_at + lane, (c.hist - 1) / P)];
+      const bool outside = page >= a.physical_blocks;
+      bad_page = __ballot(outside) != 0 ? 1 : 0;
+      if (outside) page = 0;
+      const unsigned long long at =
+          (static_cast<unsigned long long>(page) * a.kv_heads + c.kvh) * (P * D * kElem);
+      page_lo = static_cast<unsigned>(at);
+      page_hi = static_cast<unsigned>(at >> 32);
+    }
+    s.bad |= bad_page;
+    locate_pages(first);
+    return s;
+  };
+
+  using Raw = std::conditional_t<PF == 0, v4f, std::conditional_t<PF == 1, v4u, v2u>>;
+  using Global = const __attribute__((address_space(1))) Raw*;
+  using GlobalRows = const __attribute__((address_space(1))) v4f*;
+  constexpr int RW = PF == 0 ? 2 : 1;
+  Raw key_raw[NJ * RW], value_raw[NJ * RW];
+  auto load_pages = [&] {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int chunk = tid + NT * i, row = chunk >> 4, part = chunk & 15;
-      uint4 kt[KT], vt[KT];
-      if (tree) {
-        const int node = (c.blk - c.nbh) * kBlock + min(row, seen - 1);
-        const std::size_t e =
-            ((static_cast<std::size_t>(c.b) * a.kv_heads + c.kvh) * a.nodes + node) * D + part * 8;
-        // (Global address space, or the compiler merges these loads with reads of
-        // kr and vr, which must stay in registers.)
-        using Rows = const __attribute__((address_space(1))) v4f*;
-        const auto k = reinterpret_cast<Rows>(reinterpret_cast<std::uintptr_t>(a.tree_key + e));
-        const auto v = reinterpret_cast<Rows>(reinterpret_cast<std::uintptr_t>(a.tree_value + e));
-        chunk_of_rows<PF>(k[0], k[1], a.k_scale, kt);
-        chunk_of_rows<PF>(v[0], v[1], a.v_scale, vt);
-      } else if constexpr (PF == 0) {
-        chunk_of_rows<0>(kr[2 * i], kr[2 * i + 1], 1.0f, kt);
-        chunk_of_rows<0>(vr[2 * i], vr[2 * i + 1], 1.0f, vt);
-      } else if constexpr (PF == 1) {
-        kt[0] = __builtin_bit_cast(uint4, kr[i]);
-        vt[0] = __builtin_bit_cast(uint4, vr[i]);
+    for (int i = 0; i < NJ; ++i) {
+#pragma unroll
+      for (int w = 0; w < RW; ++w) key_raw[RW * i + w] = reinterpret_cast<Global>(key_at[i])[w];
+    }
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) {
+#pragma unroll
+      for (int w = 0; w < RW; ++w) value_raw[RW * i + w] = reinterpret_cast<Global>(value_at[i])[w];
+    }
+  };
+  auto from_pages = [&](const Raw* x, v4u (&t)[KT]) {
+    if constexpr (PF == 0) {
+      chunk_of_rows<0>(x[0], x[1], 1.0f, t);
+    } else if constexpr (PF == 1) {
+      t[0] = x[0];
+    } else {
+      t[0] = codes_fp16(x[0][0], x[0][1]);
+    }
+  };
+  auto put_key = [&](int buf, int i, const v4u (&t)[KT]) {
+#pragma unroll
+    for (int n = 0; n < KT; ++n) {
+      *reinterpret_cast<v4u*>(sh.item[buf].k[n] + bmma_k_at(4 * job(i) + grp, col)) = t[n];
+    }
+  };
+  auto put_value = [&](int buf, int i, const v4u (&t)[KT]) {
+#pragma unroll
+    for (int n = 0; n < KT; ++n) {
+      *reinterpret_cast<v4u*>(sh.item[buf].v[n] + bmma_v_at(4 * job(i) + grp, col)) = t[n];
+    }
+  };
+  // An item of whole pages into LDS.
+  auto store_pages = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) {
+      v4u t[KT];
+      from_pages(key_raw + RW * i, t);
+      put_key(buf, i, t);
+      from_pages(value_raw + RW * i, t);
+      put_value(buf, i, t);
+    }
+  };
+  // Any item: what was loaded, or (`s.tree`) rows read now.  (Those read ahead
+  // into the pages' registers would have the pages' loads waited for at once.)
+  auto from_rows = [&](const TreeSource& s, const float* rows, float scale, int i,
+                       v4u (&t)[KT]) {
+    const auto x = reinterpret_cast<GlobalRows>(reinterpret_cast<std::uintptr_t>(
+        rows + s.at + min(4 * job(i) + grp, s.rows - 1) * D + col * 8));
+    chunk_of_rows<PF>(x[0], x[1], scale, t);
+  };
+  auto store_key = [&](int buf, const TreeSource& s) {
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) {
+      v4u t[KT];
+      if (s.tree != 0) {
+        from_rows(s, a.tree_key, a.k_scale, i, t);
       } else {
-        kt[0] = codes_fp16(kr[i][0], kr[i][1]);
-        vt[0] = codes_fp16(vr[i][0], vr[i][1]);
+        from_pages(key_raw + RW * i, t);
       }
+      put_key(buf, i, t);
+    }
+  };
+  auto store_value = [&](int buf, const TreeSource& s) {
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        if (row >= seen) kt[t] = vt[t] = make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(sh.k[t] + bmma_k_at(row, part)) = kt[t];
-        *reinterpret_cast<uint4*>(sh.v[t] + bmma_v_at(row, part)) = vt[t];
+    for (int i = 0; i < NJ; ++i) {
+      v4u t[KT];
+      if (s.tree != 0) {
+        from_rows(s, a.tree_value, a.v_scale, i, t);
+      } else {
+        from_pages(value_raw + RW * i, t);
       }
+      // Rows behind the sequence's must be finite.
+#pragma unroll
+      for (int n = 0; n < KT; ++n) t[n] = 4 * job(i) + grp >= s.rows ? v4u{0u, 0u, 0u, 0u} : t[n];
+      put_value(buf, i, t);
     }
   };
 
   // The wavefront's rows of the unit: tile t's row `col`.
-  uint4 qop[RT][2][4];  // (the third term of three is in LDS)
+  v4u qop[RT][2][4];  // (the third term of three is in LDS)
   float unscale[RT];  // fp8 pages: what undoes the row's power of two
+  int parent = -1;    // of node `lane`
+  v4f o[RT][8];       // o[t][dt][i]: dim 16 dt + 4 grp + i of row col
+  float m[RT], l[RT];
+  bool finite = false;  // every row's reference is a number
+  unsigned long long broken = 0;  // the nodes with a wrong parent on their way
   auto unit_rows = [&](const TreeCursor& c) {
     return (static_cast<std::size_t>(c.b) * a.q_heads +
             static_cast<std::size_t>(c.kvh) * (a.q_heads / a.kv_heads)) *
            a.nodes;
   };
-  auto load_query = [&](const TreeCursor& c) {
+  auto start = [&](const TreeCursor& c) {
     const float scale = PF == 2 ? a.qscale * a.k_scale : a.qscale;
+    parent = node_parent(a, c.b, c.count, lane);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int row = c.rb * RB + (wave * RT + t) * 16 + col;
-      float4 x[4][2];
+      v4f x[4][2];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        x[s][0] = x[s][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        x[s][0] = x[s][1] = v4f{0.f, 0.f, 0.f, 0.f};
         if (row < a.rows) {
           const auto* q =
-              reinterpret_cast<const float4*>(a.query + (unit_rows(c) + row) * D + 32 * s + 8 * grp);
+              reinterpret_cast<const v4f*>(a.query + (unit_rows(c) + row) * D + 32 * s + 8 * grp);
           x[s][0] = q[0];
           x[s][1] = q[1];
         }
@@ -406,8 +529,8 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         for (int s = 0; s < 4; ++s)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(x[s][w].x), fabsf(x[s][w].y)),
-                                     fmaxf(fabsf(x[s][w].z), fabsf(x[s][w].w))));
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(x[s][w][0]), fabsf(x[s][w][1])),
+                                     fmaxf(fabsf(x[s][w][2]), fabsf(x[s][w][3]))));
           }
         most = row_max(most);
         // most * 2^(10 - e) in [2^10, 2^11), as far as 2^(10 - e) is a normal
@@ -418,56 +541,59 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const float y[8] = {x[s][0].x, x[s][0].y, x[s][0].z, x[s][0].w,
-                            x[s][1].x, x[s][1].y, x[s][1].z, x[s][1].w};
         unsigned w[4][3];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_pair<PF>(y[2 * i] * grow, y[2 * i + 1] * grow, w[i]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          qop[t][i][s] = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
+        for (int i = 0; i < 4; ++i) {
+          split_pair<PF>(x[s][i >> 1][2 * (i & 1)] * grow, x[s][i >> 1][2 * (i & 1) + 1] * grow, w[i]);
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qop[t][i][s] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
         if constexpr (QT == 3) {
-          sh.low[wave * RT + t][s][lane] = make_uint4(w[0][2], w[1][2], w[2][2], w[3][2]);
+          sh.low[wave * RT + t][s][lane] = v4u{w[0][2], w[1][2], w[2][2], w[3][2]};
         }
       }
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) o[t][dt] = v4f{0.f, 0.f, 0.f, 0.f};
+      m[t] = -INFINITY;
+      l[t] = 0.f;
     }
+    broken = 0;
+    finite = false;
   };
 
-  v4f o[RT][8];  // o[t][dt][i]: dim 16 dt + 4 grp + i of row col
-  float m[RT], l[RT];
-  unsigned long long broken = 0;  // the nodes with a wrong parent on their way
-
+  // Scores of a block: sc[t][h][i] is key 16 h + 4 grp + i of tile t's row col.
   const unsigned k_at = bmma_k_at(col, grp);
-  const unsigned v_at =
-      bmma_v_at(4 * grp + (col >> 2), 0) + static_cast<unsigned>((col & 3) * 8);
-  auto compute = [&](const TreeCursor& c) {
-    v4f sc[RT][2];
+  // (Operands come out of LDS two steps of 32 dims, or four tiles of 16, ahead
+  // of the instructions that take them.)
+  constexpr int kProducts = PF == 0 ? 6 : QT;
+  auto scores = [&](int buf, v4f (&sc)[RT][2]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) sc[t][0] = sc[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      uint4 low[RT];
+      v4u low[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        if constexpr (QT == 3) low[t] = sh.low[wave * RT + t][s][lane];
+        if constexpr (QT == 3) {
+          low[t] = sh.low[wave * RT + t][s][lane];
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint4 kop[KT];
+        v4u kop[KT];
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
-          kop[i] = *reinterpret_cast<const uint4*>(sh.k[i] + h * (P * 2 * D) + (k_at ^ (64u * s)));
+          kop[i] =
+              *reinterpret_cast<const v4u*>(sh.item[buf].k[i] + h * (P * 2 * D) + (k_at ^ (64u * s)));
         }
+        // Smallest products first.
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          // Smallest products first.
+        for (int sum = QT - 1; sum >= 0; --sum) {
 #pragma unroll
-          for (int sum = QT - 1; sum >= 0; --sum) {
+          for (int i = KT - 1; i >= 0; --i) {
+            if (sum - i < 0 || sum - i >= QT) continue;
 #pragma unroll
-            for (int i = KT - 1; i >= 0; --i) {
-              if (sum - i < 0 || sum - i >= QT) continue;
+            for (int t = 0; t < RT; ++t) {
               sc[t][h] =
                   matrix_step<PF>(kop[i], sum - i == 2 ? low[t] : qop[t][sum - i & 1][s], sc[t][h]);
             }
@@ -475,62 +601,92 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         }
       }
     }
-    __builtin_amdgcn_s_setprio(0);
+    constexpr int kReads = 2 * KT + (QT == 3 ? RT : 0), kSteps = 2 * RT * kProducts;
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kReads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, kSteps, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, kSteps, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, 2 * kSteps, 0);
+  };
+  // m[t] is a reference near the row's maximum: it moves where a score is above
+  // it by more than kSlack, and what was summed with it.  `vis[t]`: the lane's
+  // keys (bit 4 h + i) that the row sees.  Returns whether every key is seen and
+  // every reference finite.
+  auto maxima = [&](const TreeCursor& c, v4f (&sc)[RT][2], unsigned (&vis)[RT]) {
     const bool in_tree = c.blk >= c.nbh;
-    const int seen = in_tree ? 0 : c.hist - c.blk * kBlock;
-    unsigned bits[RT];  // the block's keys that the row sees
-    if (in_tree) {
-      const TreeSequence tree = tree_sequence(a, c.b, lane);
-      broken = __ballot(tree.broken != 0);
+    const int seen = c.hist - c.blk * kBlock;
+    const bool full = !in_tree && seen >= kBlock;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) vis[t] = 0xffu;
+    if (__builtin_expect(!full, 0)) {
+      unsigned bits[RT];  // the block's keys that the row sees
+      if (in_tree) {
+        TreeSequence tree{};
+        tree_words(parent, c.count, lane, tree);
+        broken = __ballot(tree.broken != 0);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const int row = c.rb * RB + (wave * RT + t) * 16 + col;
+          const unsigned long long w = shfl64(tree.seen, row % a.nodes);
+          bits[t] = row < a.rows ? static_cast<unsigned>(w >> ((c.blk - c.nbh) * kBlock)) : 0u;
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) bits[t] = (1u << seen) - 1u;
+      }
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const int row = c.rb * RB + (wave * RT + t) * 16 + col;
-        const unsigned long long w = shfl64(tree.seen, row % a.nodes);
-        bits[t] = row < a.rows ? static_cast<unsigned>(w >> ((c.blk - c.nbh) * kBlock)) : 0u;
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) bits[t] = seen >= kBlock ? ~0u : (1u << seen) - 1u;
-    }
-    uint4 pop[RT][QT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      // x[j]: key 16 (j / 4) + 4 grp + j % 4.
-      float x[8], p[8];
-      unsigned vis = 0xffu;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = sc[t][j >> 2][j & 3];
-      if constexpr (PF == 2) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= unscale[t];
-      }
-      const bool full = !in_tree && seen >= kBlock;
-      if (!full) {
-        vis = ((bits[t] >> (4 * grp)) & 0xfu) | ((bits[t] >> (16 + 4 * grp)) & 0xfu) << 4;
+        vis[t] = ((bits[t] >> (4 * grp)) & 0xfu) | ((bits[t] >> (16 + 4 * grp)) & 0xfu) << 4;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (((vis >> j) & 1u) == 0) x[j] = -INFINITY;
+          if (((vis[t] >> j) & 1u) == 0) sc[t][j >> 2][j & 3] = -INFINITY;
         }
       }
-      const float mx = row_max(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                                     fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
-      const float mn = fmaxf(m[t], mx);
-      if (__ballot(!(mn == m[t])) != 0) {  // some row's maximum moved
+    }
+    float mx[RT];
+    bool above = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const v4f x0 = sc[t][0], x1 = sc[t][1];
+      mx[t] = larger(larger(larger(x0[0], x0[1]), larger(x0[2], x0[3])),
+                     larger(larger(x1[0], x1[1]), larger(x1[2], x1[3])));
+      if constexpr (PF == 2) mx[t] *= unscale[t];
+      above = above || mx[t] > m[t] + kSlack;
+    }
+    if (__ballot(above) != 0) {
+      finite = true;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float mn = fmaxf(m[t], row_max(mx[t]));
         const float alpha = exp2_ratio(m[t], mn);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) o[t][dt] *= alpha;
         l[t] *= alpha;
         m[t] = mn;
+        finite = finite && __ballot(!(fabsf(mn) < INFINITY)) == 0;
       }
-      if (full && __ballot(!(fabsf(mn) < INFINITY)) == 0) {
-        const float shift = PF == 2 ? mn - 14.0f : mn;
+    }
+    return full && finite;
+  };
+  // Probabilities of the block's scores as operands; FINE: maxima() said so.
+  auto probabilities = [&](auto fine_tag, v4f (&sc)[RT][2], const unsigned (&vis)[RT],
+                           v4u (&pop)[RT][QT]) {
+    constexpr bool FINE = decltype(fine_tag)::value;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(x[j] - shift);
-      } else {
+    for (int t = 0; t < RT; ++t) {
+      float p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          p[j] = ((vis >> j) & 1u) != 0 ? exp2_ratio(x[j], mn) : 0.f;
-          if constexpr (PF == 2) p[j] *= kProbScale;
+      for (int j = 0; j < 8; ++j) {
+        const float x = sc[t][j >> 2][j & 3];
+        if constexpr (FINE && PF == 2) {
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, unscale[t], kProbLog - m[t]));
+        } else if constexpr (FINE) {
+          p[j] = __builtin_amdgcn_exp2f(x - m[t]);
+        } else if constexpr (PF == 2) {
+          p[j] = ((vis[t] >> j) & 1u) != 0 ? exp2_ratio(x * unscale[t], m[t]) * kProbScale : 0.f;
+        } else {
+          p[j] = ((vis[t] >> j) & 1u) != 0 ? exp2_ratio(x, m[t]) : 0.f;
         }
       }
       // The lane's own keys; the row's four lanes are added at the end.
@@ -539,42 +695,52 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
 #pragma unroll
       for (int i = 0; i < 4; ++i) split_pair<PF>(p[2 * i], p[2 * i + 1], w[i]);
 #pragma unroll
-      for (int i = 0; i < QT; ++i) pop[t][i] = make_uint4(w[0][i], w[1][i], w[2][i], w[3][i]);
+      for (int i = 0; i < QT; ++i) pop[t][i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
     }
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-      using LdsV4s = __attribute__((address_space(3))) v4s;
-      uint4 vop[KT];
+  };
+  const unsigned v_at =
+      bmma_v_at(4 * grp + (col >> 2), 0) + static_cast<unsigned>((col & 3) * 8);
+  auto add_values = [&](int buf, const v4u (&pop)[RT][QT]) {
+    using LdsV4s = __attribute__((address_space(3))) v4s;
+    constexpr int kAhead = PF == 0 ? 2 : 4;
+    v4u vop[kAhead][KT];
+    auto read = [&](int dt) {
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
-        const unsigned char* vp = sh.v[i] + (v_at ^ (32u * dt));
+        unsigned char* const vp = sh.item[buf].v[i] + (v_at ^ (32u * dt));
         const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(vp));
         const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(vp + P * 2 * D));
-        vop[i] = __builtin_bit_cast(uint4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        vop[dt % kAhead][i] =
+            __builtin_bit_cast(v4u, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
       }
+    };
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
+    for (int dt = 0; dt < kAhead; ++dt) read(dt);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int sum = QT - 1; sum >= 0; --sum) {
+    for (int dt = 0; dt < 8; ++dt) {
 #pragma unroll
-          for (int i = KT - 1; i >= 0; --i) {
-            if (sum - i < 0 || sum - i >= QT) continue;
-            o[t][dt] = matrix_step<PF>(vop[i], pop[t][sum - i], o[t][dt]);
+      for (int sum = QT - 1; sum >= 0; --sum) {
+#pragma unroll
+        for (int i = KT - 1; i >= 0; --i) {
+          if (sum - i < 0 || sum - i >= QT) continue;
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            o[t][dt] = matrix_step<PF>(vop[dt % kAhead][i], pop[t][sum - i], o[t][dt]);
           }
         }
       }
+      if (dt + kAhead < 8) read(dt + kAhead);
+      // (Or the compiler reads each operand where it is needed, and waits.)
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
   };
 
   // Ends the unit's part [from, c.blk] in this range.
-  auto finish = [&](const TreeCursor& c, int from, long long g) {
+  auto finish = [&](const TreeCursor& c, int from, long long g, bool bad) {
     const bool starts = from == 0, ends = c.blk + 1 == c.nb;
     const bool complete = starts && ends;
     const float vscale = PF == 2 ? a.v_scale : 1.0f;
-    const bool bad = bad_page || c.bad;
-    bad_page = false;
     const int slot = 2 * group + (starts ? 1 : 0);
     const int row_base = complete ? 0 : c.rb * RB;
     float* const rows =
@@ -622,69 +788,119 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
     }
   };
 
-  load_block(cur);
-  int from = cur.blk;  // the unit's first block in this range
-  bool fresh = true;
-  for (long long g = range.g0;; ++g) {
-    barrier();
-    store_block(cur);
-    barrier();
-    const bool more = g + 1 < range.g1;
-    if (fresh) {
-      load_query(cur);
+  // Item i of the range, K of its block i and V of block i - 1, is put into
+  // buffer i % NB.  Behind the range, items go on that no one reads.
+  TreeCursor ahead = cur;  // the block of `key`
+  TreeSource key = locate(ahead), value{};
+  unsigned bads = key.bad;  // bit i % 32: of block i, as far as it was located
+  int item = 0;             // the one on its way,
+  int into = 0;             // the buffer it goes to
+  // Items from this one on that are whole pages of one sequence, with page
+  // offsets in hand, and have such a one behind them.
+  int plain = 0;
+  auto put = [&] {
+    // Everything sent for is there.  (Said here, or the compiler waits where the
+    // registers are loaded next.)
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    if (__builtin_expect(plain > 0, 1)) {
+      store_pages(into);
+    } else {
+      if (item < blocks) store_key(into, key);
+      if (item > 0 && item <= blocks) store_value(into, value);
+    }
+    into = into + 1 == NB ? 0 : into + 1;
+    ++item;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) o[t][dt] = v4f{0.f, 0.f, 0.f, 0.f};
-        m[t] = -INFINITY;
-        l[t] = 0.f;
+    for (int i = 0; i < NJ; ++i) value_at[i] = key_at[i] + value_off;
+    if (__builtin_expect(plain > 0, 1)) {
+      --plain;
+      ++ahead.blk;
+      key.rows -= kBlock;
+      locate_pages(2 * ahead.blk - pages_at);
+    } else {
+      value = key;
+      if (item < blocks) {
+        advance(a, st, ahead);
+        key = locate(ahead);
+        bads |= static_cast<unsigned>(key.bad) << (item & 31);
+        if (key.tree == 0 && ahead.blk > 0 && item > 1) {
+          plain = min(min(ahead.nbh - 1, (pages_at >> 1) + 31) - ahead.blk, blocks - 1 - item);
+        }
       }
-      fresh = false;
-      broken = 0;
     }
-    const bool bad_before = bad_page;
-    bad_page = false;
-    TreeCursor next = cur;
-    if (more) {
-      advance(a, st, next);
-      load_block(next);
+    // (On every path, where what is located is needed or not: loads on some paths
+    // only are copied, and so waited for, where the paths meet.)
+    load_pages();
+  };
+  load_pages();
+  put();
+  if constexpr (NB == 3) put();
+  start(cur);
+  v4f sc[RT][2];
+  barrier();
+  scores(0, sc);
+  const bool second = kTurns && wave >= 4;
+  if (second) barrier();
+  int from = cur.blk;  // the unit's first block in this range
+  int bad = 0;         // of the unit
+  for (int n = 0, buf = 0;; ++n) {
+    if constexpr (NB == 1) barrier();  // the last step's reads are done
+    put();
+    __builtin_amdgcn_sched_barrier(0);
+    bad |= static_cast<int>(bads >> (n & 31)) & 1;
+    bads &= ~(1u << (n & 31));
+    unsigned vis[RT];
+    v4u pop[RT][QT];
+    if (maxima(cur, sc, vis)) {
+      probabilities(std::true_type{}, sc, vis, pop);
+    } else {
+      probabilities(std::false_type{}, sc, vis, pop);
     }
-    const bool bad_next = bad_page;
-    bad_page = bad_before;
-    compute(cur);
-    if (!more || cur.blk + 1 == cur.nb) {
-      finish(cur, from, g);
-      from = 0;
-      fresh = true;
+    barrier();
+    buf = buf + 1 == NB ? 0 : buf + 1;
+    __builtin_amdgcn_s_setprio(1);
+    add_values(buf, pop);
+    const bool last = n + 1 == blocks;
+    if (last || cur.blk + 1 == cur.nb) {
+      __builtin_amdgcn_s_setprio(0);
+      finish(cur, from, range.g0 + n, bad != 0);
+      if (last) break;
+      advance(a, st, cur);
+      from = bad = 0;
+      start(cur);
+    } else {
+      ++cur.blk;
     }
-    bad_page = bad_page || bad_next;
-    if (!more) break;
-    cur = next;
+    scores(buf, sc);
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kTurns) barrier();
   }
+  if (kTurns && !second) barrier();
 }
 
 template <int PF, int W, int RT>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(PF == 0 ? (W == 1 ? 1 : 2) : W <= 2 || RT == 2 ? 2 : 3))) void tree_mma_kernel(TreeKernelArgs a, TreeStream st) {
-  __shared__ TreeShared<PF, W * RT> sh;
+__global__ __launch_bounds__(64 * W)
+    __attribute__((amdgpu_waves_per_eu(2))) void tree_mma_kernel(TreeKernelArgs a, TreeStream st) {
+  __shared__ TreeShared<PF, W, RT> sh;
   tree_mma_body<PF, W, RT>(a, st, sh);
 }
 
 // Joins the partials of the units that cross ranges: blockIdx.x is the group
 // whose range ends such a unit, its partials the first group's second slot and
-// the later groups' first ones.  A wavefront takes a row, a lane two dims.
-// Marked parts are computed again here; those of finished units by the
-// workgroups with blockIdx.y = 0.
-constexpr int kMergeRows = 4;
+// the later groups' first ones.  16 lanes take a row, 8 dims each, and 16
+// partials' statistics at a time.  (A wavefront a row: 60 us where this takes
+// 30, 64 sequences of 64 nodes.)  Marked parts are computed again here; those
+// of finished units by the workgroups with blockIdx.y = 0.
+constexpr int kMergeRows = 16;
 template <int PF>
-__global__ __launch_bounds__(64 * kMergeRows) void tree_merge_kernel(TreeKernelArgs a,
-                                                                     TreeStream st, int rb_rows) {
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeKernelArgs a, TreeStream st,
+                                                         int rb_rows) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   auto out_row = [&](int b, int kvh, int row) {
-    return reinterpret_cast<float2*>(
-               a.out + ((static_cast<std::size_t>(b) * a.q_heads +
-                         static_cast<std::size_t>(kvh) * (a.q_heads / a.kv_heads)) * a.nodes +
-                        row) * D) + lane;
+    return a.out + ((static_cast<std::size_t>(b) * a.q_heads +
+                     static_cast<std::size_t>(kvh) * (a.q_heads / a.kv_heads)) * a.nodes +
+                    row) * D;
   };
   if (blockIdx.y == 0) {
     const std::size_t units = static_cast<std::size_t>(a.batch) * a.kv_heads * st.row_blocks;
@@ -696,7 +912,7 @@ __global__ __launch_bounds__(64 * kMergeRows) void tree_merge_kernel(TreeKernelA
       const int kvh = static_cast<int>(u / st.row_blocks / a.batch);
       const TreeSequence s = tree_sequence(a, b, lane);
       if (s.count == 0) continue;  // no one wrote its marks
-      for (int i = wave; i < rb_rows; i += kMergeRows) {
+      for (int i = wave; i < rb_rows; i += 4) {
         const int row = rb * rb_rows + i, node = row % a.nodes;
         if (st.unit_marks[u * kMaxTiles + i / 16] == 0 || row >= a.rows || node >= s.count) continue;
         if (((__ballot(s.broken != 0) >> node) & 1) != 0) continue;
@@ -704,82 +920,115 @@ __global__ __launch_bounds__(64 * kMergeRows) void tree_merge_kernel(TreeKernelA
         float m, l;
         exact_row<PF>(a, b, kvh, row, 0, s.hist, 0, s.count, shfl64(s.seen, node), lane, o, m, l);
         const float f = m == -INFINITY ? NAN : 1.0f / l;
-        *out_row(b, kvh, row) = make_float2(o.x * f, o.y * f);
+        reinterpret_cast<float2*>(out_row(b, kvh, row))[lane] = make_float2(o.x * f, o.y * f);
       }
     }
   }
   const TreeJob job = st.jobs[blockIdx.x];
   if (job.b < 0) return;
-  const int local = static_cast<int>(blockIdx.y) * kMergeRows + wave;
+  const int part = lane & 15;
+  const int local = static_cast<int>(blockIdx.y) * kMergeRows + wave * 4 + (lane >> 4);
   const int row = job.rb * rb_rows + local;
-  if (local >= rb_rows || row >= a.rows || row % a.nodes >= clamped_nodes(a, job.b)) return;
+  const bool live =
+      local < rb_rows && row < a.rows && row % a.nodes < clamped_nodes(a, job.b);
+  if (__ballot(live) == 0) return;
+  const int at = live ? local : 0;  // (a row of the unit's, where there is one)
   const int n = static_cast<int>(blockIdx.x) - job.first + 1;
   auto slot = [&](int i) {
     return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0));
   };
   float top = -INFINITY, sum = 0.f;
-  float2 o = make_float2(0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 64) {
+  v4f o[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+  bool again = false;  // some part of a row of this wavefront is marked
+  for (int i0 = 0; i0 < n; i0 += 16) {
     float m = -INFINITY, l = 0.f;
-    bool again = false;
-    if (i0 + lane < n) {
-      const std::size_t at = slot(i0 + lane);
-      const float2 x = *reinterpret_cast<const float2*>(st.part_ml + (at * rb_rows + local) * 2);
-      again = st.part_marks[at * kMaxTiles + local / 16] != 0;
-      if (!again) {
+    bool marked = false;
+    if (i0 + part < n) {
+      const std::size_t s = slot(i0 + part);
+      const float2 x = *reinterpret_cast<const float2*>(st.part_ml + (s * rb_rows + at) * 2);
+      marked = live && st.part_marks[s * kMaxTiles + at / 16] != 0;
+      if (live && !marked) {
         m = x.x;
         l = x.y;
       }
     }
+    again = again || __ballot(marked) != 0;
     float mx = m;
 #pragma unroll
-    for (int k = 32; k > 0; k /= 2) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
+    for (int k = 8; k > 0; k /= 2) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
     const float mn = fmaxf(top, mx);
     const float alpha = exp2_ratio(top, mn);
-    const float w = i0 + lane < n && !again ? exp2_ratio(m, mn) : 0.f;
+    const float w = i0 + part < n && live && !marked ? exp2_ratio(m, mn) : 0.f;
     float add = w * l;
 #pragma unroll
-    for (int k = 32; k > 0; k /= 2) add += __shfl_xor(add, k, 64);
+    for (int k = 8; k > 0; k /= 2) add += __shfl_xor(add, k, 64);
     sum = sum * alpha + add;
-    o.x *= alpha;
-    o.y *= alpha;
+    o[0] *= alpha;
+    o[1] *= alpha;
     top = mn;
-    unsigned long long marked = __ballot(again);
-    const int end = min(n - i0, 64);
+    const int end = min(n - i0, 16);
     for (int i = 0; i < end; ++i) {
-      if (((marked >> i) & 1) != 0) continue;
-      const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
-      const float2 x = *reinterpret_cast<const float2*>(
-          st.part_o + (slot(i0 + i) * rb_rows + local) * D + 2 * lane);
-      o.x += wi * x.x;
-      o.y += wi * x.y;
-    }
-    for (; marked != 0; marked &= marked - 1) {
-      const int i = i0 + __ffsll(static_cast<long long>(marked)) - 1;
-      const TreeSequence s = tree_sequence(a, job.b, lane);
-      const int nbh = (s.hist + kBlock - 1) / kBlock;
-      const long long from = i == 0 ? 0 : job.head + static_cast<long long>(i - 1) * job.each;
-      const long long to = job.head + static_cast<long long>(i) * job.each;
-      auto tokens = [&](long long blocks) {
-        return static_cast<int>(min(static_cast<long long>(s.hist), blocks * kBlock));
-      };
-      auto nodes = [&](long long blocks) {
-        return static_cast<int>(min(static_cast<long long>(s.count), max(blocks - nbh, 0ll) * kBlock));
-      };
-      float2 e;
-      float em, el;
-      exact_row<PF>(a, job.b, job.kvh, row, tokens(from), tokens(to), nodes(from), nodes(to),
-                    shfl64(s.seen, row % a.nodes), lane, e, em, el);
-      const float en = fmaxf(top, em);
-      const float f = exp2_ratio(top, en), g = exp2_ratio(em, en) * (PF == 2 ? kProbScale : 1.0f);
-      sum = sum * f + el * g;
-      o.x = o.x * f + e.x * g;
-      o.y = o.y * f + e.y * g;
-      top = en;
+      const int from = (lane & 48) + i;
+      const float wi = __shfl(w, from, 64);
+      const bool skip = __shfl(marked ? 1 : 0, from, 64) != 0;
+      const auto* x = reinterpret_cast<const v4f*>(st.part_o + (slot(i0 + i) * rb_rows + at) * D) +
+                      2 * part;
+      const v4f x0 = x[0], x1 = x[1];
+      if (!skip) {
+        o[0] += wi * x0;
+        o[1] += wi * x1;
+      }
     }
   }
+  if (again) {
+    // The marked parts of the wavefront's four rows, a row after another; lane
+    // i of 64 holds dims 2 i, 2 i + 1 there and hands them over.
+    const TreeSequence s = tree_sequence(a, job.b, lane);
+    const int nbh = (s.hist + kBlock - 1) / kBlock;
+    auto tokens = [&](long long blocks) {
+      return static_cast<int>(min(static_cast<long long>(s.hist), blocks * kBlock));
+    };
+    auto nodes = [&](long long blocks) {
+      return static_cast<int>(
+          min(static_cast<long long>(s.count), max(blocks - nbh, 0ll) * kBlock));
+    };
+#pragma unroll 1
+    for (int r = 0; r < 4; ++r) {
+      const int one = static_cast<int>(blockIdx.y) * kMergeRows + wave * 4 + r;
+      const int one_row = job.rb * rb_rows + one;
+      if (one >= rb_rows || one_row >= a.rows || one_row % a.nodes >= s.count) continue;
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        if (st.part_marks[slot(i) * kMaxTiles + one / 16] == 0) continue;
+        const long long from = i == 0 ? 0 : job.head + static_cast<long long>(i - 1) * job.each;
+        const long long to = job.head + static_cast<long long>(i) * job.each;
+        float2 e;
+        float em, el;
+        exact_row<PF>(a, job.b, job.kvh, one_row, tokens(from), tokens(to), nodes(from), nodes(to),
+                      shfl64(s.seen, one_row % a.nodes), lane, e, em, el);
+        float d[8];  // this lane's dims, had it the row
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          d[2 * k] = __shfl(e.x, 4 * part + k, 64);
+          d[2 * k + 1] = __shfl(e.y, 4 * part + k, 64);
+        }
+        if (lane >> 4 == r) {
+          const float en = fmaxf(top, em);
+          const float f = exp2_ratio(top, en);
+          const float g = exp2_ratio(em, en) * (PF == 2 ? kProbScale : 1.0f);
+          sum = sum * f + el * g;
+          o[0] = o[0] * f + v4f{d[0], d[1], d[2], d[3]} * g;
+          o[1] = o[1] * f + v4f{d[4], d[5], d[6], d[7]} * g;
+          top = en;
+        }
+      }
+    }
+  }
+  if (!live) return;
   const float f = top == -INFINITY ? NAN : 1.0f / sum;
-  *out_row(job.b, job.kvh, row) = make_float2(o.x * f, o.y * f);
+  auto* const dst = reinterpret_cast<v4f*>(out_row(job.b, job.kvh, row)) + 2 * part;
+  dst[0] = o[0] * f;
+  dst[1] = o[1] * f;
 }
 
 // ----------------------------------------------------------------- host ----
@@ -791,13 +1040,15 @@ struct TreeShape {
   std::size_t rows() const { return static_cast<std::size_t>(waves) * tiles * 16; }
 };
 
-TreeShape tree_shape(std::size_t rows) {
-  const std::size_t tiles = (rows + 15) / 16;
-  if (tiles <= 1) return {1, 1, 4 * kTreeCus};
-  if (tiles <= 2) return {2, 1, 3 * kTreeCus};
-  if (tiles <= 4) return {4, 1, 2 * kTreeCus};
-  if (tiles <= 8) return {4, 2, 2 * kTreeCus};
-  return {8, 2, kTreeCus};
+// A unit's rows: enough wavefronts to load pages with, and the fewest row blocks
+// that registers allow, as each reads the pages again.  As many workgroups as
+// fit on the chip at once.
+TreeShape tree_shape(PageType type, std::size_t rows) {
+  if (type == PageType::kFP8) {
+    return rows <= 64 ? TreeShape{4, 1, 3 * kTreeCus} : TreeShape{4, 2, 2 * kTreeCus};
+  }
+  if (rows <= 64) return {4, 1, 2 * kTreeCus};
+  return rows <= 128 ? TreeShape{8, 1, kTreeCus} : TreeShape{8, 2, kTreeCus};
 }
 
 std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
@@ -829,20 +1080,21 @@ void launch_mma(const TreeKernelArgs& k, const TreeStream& st, hipStream_t strea
 template <int PF>
 hipError_t launch_tree(const TreeKernelArgs& k, const TreeStream& st, const TreeShape& s,
                        hipStream_t stream) {
-  switch (s.waves * 10 + s.tiles) {
-    case 11: launch_mma<PF, 1, 1>(k, st, stream); break;
-    case 21: launch_mma<PF, 2, 1>(k, st, stream); break;
-    case 41: launch_mma<PF, 4, 1>(k, st, stream); break;
-    case 42: launch_mma<PF, 4, 2>(k, st, stream); break;
-    case 82: launch_mma<PF, 8, 2>(k, st, stream); break;
-    default: return hipErrorInvalidValue;
+  if (s.rows() == 64) {
+    launch_mma<PF, 4, 1>(k, st, stream);
+  } else if constexpr (PF == 2) {
+    launch_mma<PF, 4, 2>(k, st, stream);
+  } else if (s.rows() == 128) {
+    launch_mma<PF, 8, 1>(k, st, stream);
+  } else {
+    launch_mma<PF, 8, 2>(k, st, stream);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int rows = static_cast<int>(s.rows()) < k.rows ? static_cast<int>(s.rows()) : k.rows;
   const dim3 grid(static_cast<unsigned>(st.groups),
                   static_cast<unsigned>((rows + kMergeRows - 1) / kMergeRows));
-  tree_merge_kernel<PF><<<grid, 64 * kMergeRows, 0, stream>>>(k, st, static_cast<int>(s.rows()));
+  tree_merge_kernel<PF><<<grid, 256, 0, stream>>>(k, st, static_cast<int>(s.rows()));
   return hipGetLastError();
 }
 
@@ -851,11 +1103,24 @@ hipError_t launch_tree(const TreeKernelArgs& k, const TreeStream& st, const Tree
 std::size_t tree_workspace_bytes(std::size_t batch, std::size_t q_heads, std::size_t kv_heads,
                                  std::size_t nodes) {
   const std::size_t rows = q_heads / kv_heads * nodes;
-  return TreeLayout(tree_shape(rows), batch, kv_heads, rows).bytes;
+  std::size_t bytes = 0;  // for any type of page
+  for (const PageType type : {PageType::kF32, PageType::kBF16, PageType::kFP8}) {
+    bytes = std::max(bytes, TreeLayout(tree_shape(type, rows), batch, kv_heads, rows).bytes);
+  }
+  return bytes;
+}
+
+bool tree_fits(const TreeAttentionArgs& a) {
+  // Ranges, and places in them, are counted in 32 bits: of 2^38 blocks, a
+  // group's are 2^30 at most.  (The grid's limits keep the product in 64 bits.)
+  const std::size_t rows = a.q_heads / a.kv_heads * a.nodes;
+  const std::size_t units = a.batch * a.kv_heads * ((rows + 63) / 64);
+  return units == 0 || a.max_blocks / 2 + 3 <= (std::size_t{1} << 38) / units;
 }
 
 hipError_t launch_tree_attention(const TreeAttentionArgs& a, hipStream_t stream) {
   if (a.batch == 0 || a.nodes == 0) return hipSuccess;
+  if (!tree_fits(a)) return hipErrorInvalidValue;
   TreeKernelArgs k{};
   k.query = a.query;
   k.key_pool = a.key_pool;
@@ -877,7 +1142,7 @@ hipError_t launch_tree_attention(const TreeAttentionArgs& a, hipStream_t stream)
   k.qscale = kLog2e / sqrtf(static_cast<float>(D));
   k.k_scale = a.page_type.k_scale;
   k.v_scale = a.page_type.v_scale;
-  const TreeShape s = tree_shape(static_cast<std::size_t>(k.rows));
+  const TreeShape s = tree_shape(a.page_type.type, static_cast<std::size_t>(k.rows));
   const TreeLayout layout(s, a.batch, a.kv_heads, static_cast<std::size_t>(k.rows));
   auto* const base = static_cast<unsigned char*>(a.workspace);
   TreeStream st{};

@@ -66,24 +66,21 @@ __device__ __forceinline__ int clamped_nodes(const TreeKernelArgs& a, int b) {
   return a.node_counts != nullptr ? min(max(a.node_counts[b], 0), a.nodes) : a.nodes;
 }
 
-// The ancestors of all nodes by doubling: after step k a lane's word holds the
-// 2^k nearest, itself first.
-__device__ __forceinline__ TreeSequence tree_sequence(const TreeKernelArgs& a, int b, int lane) {
-  TreeSequence s{};
-  const int hist = clamped_history(a, b);
-  s.bad = hist < 0;
-  s.hist = __builtin_amdgcn_readfirstlane(max(hist, 0));
-  s.count = __builtin_amdgcn_readfirstlane(clamped_nodes(a, b));
-  int up = -1;
-  bool wrong = false;
-  if (lane < s.count) {
-    up = a.parents != nullptr ? a.parents[static_cast<std::size_t>(b) * a.nodes + lane] : lane - 1;
-    wrong = up < -1 || up >= lane;
-    if (wrong) up = -1;
-    s.seen = 1ull << lane;
-  }
+// Parent of node `lane` as given (-1 behind the count).
+__device__ __forceinline__ int node_parent(const TreeKernelArgs& a, int b, int count, int lane) {
+  if (lane >= count) return -1;
+  if (a.parents == nullptr) return lane - 1;
+  return a.parents[static_cast<std::size_t>(b) * a.nodes + lane];
+}
+
+// The words of all nodes from their parents, by doubling: after step k a
+// lane's word holds the 2^k nearest, itself first.
+__device__ __forceinline__ void tree_words(int up, int count, int lane, TreeSequence& s) {
+  const bool wrong = lane < count && (up < -1 || up >= lane);
+  if (wrong) up = -1;
+  s.seen = lane < count ? 1ull << lane : 0ull;
 #pragma unroll 1
-  for (int k = 1; k < a.nodes; k *= 2) {
+  for (int k = 1; k < count; k *= 2) {
     const unsigned long long more = shfl64(s.seen, max(up, 0));
     const int next = __shfl(up, max(up, 0), 64);
     if (up >= 0) {
@@ -92,6 +89,15 @@ __device__ __forceinline__ TreeSequence tree_sequence(const TreeKernelArgs& a, i
     }
   }
   s.broken = (s.seen & __ballot(wrong)) != 0;
+}
+
+__device__ __forceinline__ TreeSequence tree_sequence(const TreeKernelArgs& a, int b, int lane) {
+  TreeSequence s{};
+  const int hist = clamped_history(a, b);
+  s.bad = hist < 0;
+  s.hist = __builtin_amdgcn_readfirstlane(max(hist, 0));
+  s.count = __builtin_amdgcn_readfirstlane(clamped_nodes(a, b));
+  tree_words(node_parent(a, b, s.count, lane), s.count, lane, s);
   return s;
 }
 
