@@ -11,6 +11,7 @@ kernels of ``libhelix_paged.so``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import sys
 import os
@@ -622,7 +623,8 @@ def _require_tensor(t, name, dtypes, shape, device=None, strided=False):
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         names = " or ".join(str(d).replace("torch.", "") for d in dtypes)
         raise HelixError(INVALID_ARGUMENT, f"{name} must be a {names} tensor")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    if t.shape != shape and (t.dim() != len(shape) or any(
+            n is not None and n != m for n, m in zip(shape, t.shape))):
         want = ", ".join("*" if n is None else str(n) for n in shape)
         raise HelixError(INVALID_ARGUMENT,
                          f"{name} must have shape [{want}], got {list(t.shape)}")
@@ -635,17 +637,26 @@ def _require_tensor(t, name, dtypes, shape, device=None, strided=False):
         raise HelixError(INVALID_ARGUMENT, f"{name} must be on {device}, got {t.device}")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The device of a call's tensors as the current one."""
     import torch
     if device.type != "cuda":
         raise HelixError(INVALID_ARGUMENT, f"tensors must be on a GPU, got {device}")
+    if torch.cuda.current_device() == device.index:
+        return _HERE
     return torch.cuda.device(device)
 
 
 def _device_stream(stream, device):
     import torch
-    return _stream(torch.cuda.current_stream(device) if stream is None else stream)
+    return (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def tree_workspace_bytes(batch, q_heads, kv_heads, nodes):
@@ -708,11 +719,11 @@ def paged_tree_attention(query, key_pool, value_pool, tables, lengths, tree_key,
     dtype = _PAGE_DTYPES.get(page_dtype, -1)
     with _on(dev):
         check(_lib().helix_paged_tree_attention(
-            _ptr(query), b, hq, hkv, t, d, ctypes.c_void_p(key_pool), ctypes.c_void_p(value_pool),
-            n, p, _ptr(tables), tables.shape[1], _ptr(lengths), _ptr(tree_key), _ptr(tree_value),
-            _ptr(parents), _ptr(node_counts), _ptr(output), _ptr(workspace),
-            workspace.numel() * workspace.element_size(), dtype, k_scale, v_scale,
-            _device_stream(stream, dev)))
+            _address(query), b, hq, hkv, t, d, key_pool, value_pool,
+            n, p, _address(tables), tables.shape[1], _address(lengths), _address(tree_key),
+            _address(tree_value), _address(parents), _address(node_counts), _address(output),
+            _address(workspace), workspace.numel() * workspace.element_size(), dtype, k_scale,
+            v_scale, _device_stream(stream, dev)))
 
 
 def verify_workspace_bytes(batch, nodes, vocab):
@@ -755,10 +766,10 @@ def _verify_arguments(target, draft, tokens, parents, uniforms, bonus_uniforms, 
         return (0, 0) if x is None else (x.stride(0) if b > 1 else 0,
                                          x.stride(1) if t > 1 else v)
 
-    rows = (_ptr(target), *strides(target), _ptr(draft), *strides(draft))
-    lists = (_ptr(tokens), _ptr(parents), _ptr(node_counts), _ptr(uniforms),
-             _ptr(bonus_uniforms))
-    return rows, lists, (_ptr(path), _ptr(accepted), _ptr(next_token))
+    rows = (_address(target), *strides(target), _address(draft), *strides(draft))
+    lists = (_address(tokens), _address(parents), _address(node_counts), _address(uniforms),
+             _address(bonus_uniforms))
+    return rows, lists, (_address(path), _address(accepted), _address(next_token))
 
 
 def verify_tree(target, draft, tokens, parents, uniforms, bonus_uniforms, path, accepted,
@@ -779,7 +790,7 @@ def verify_tree(target, draft, tokens, parents, uniforms, bonus_uniforms, path, 
     _require_tensor(workspace, "workspace", (workspace.dtype,), (None,), dev)
     with _on(dev):
         check(_lib().helix_verify_tree(
-            *rows, b, t, v, *lists, *out, _ptr(workspace),
+            *rows, b, t, v, *lists, *out, _address(workspace),
             workspace.numel() * workspace.element_size(), _device_stream(stream, dev)))
 
 
@@ -821,9 +832,9 @@ def append_path(keys, values, key_pool, value_pool, slots, path, accepted, strea
             _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), dev)
     with _on(dev):
         check(_lib().helix_paged_append_path(
-            _ptr(keys), _ptr(values), _ptr(key_pool), _ptr(value_pool), layers, stride, n, hkv, p,
-            d, _ptr(slots), _ptr(path), _ptr(accepted), b, t, _PAGE_DTYPES.get(page_dtype, -1),
-            k_scale, v_scale, _device_stream(stream, dev)))
+            _address(keys), _address(values), _address(key_pool), _address(value_pool), layers,
+            stride, n, hkv, p, d, _address(slots), _address(path), _address(accepted), b, t,
+            _PAGE_DTYPES.get(page_dtype, -1), k_scale, v_scale, _device_stream(stream, dev)))
 
 
 class DecodeBatch:

@@ -411,9 +411,10 @@ struct VerifyShape {
     chunk = ((vocab + chunks - 1) / chunks + 3) / 4 * 4;
     // A chain has one sum, as a rejection ends its walk, and so have trees
     // without a drafter's rows.  Of others, 64 trees of 16 nodes at a vocabulary
-    // of 128256 take 73 us with one such launch, 58 with two, 44 with three, 46
-    // with four and 57 with eight (one that finds nothing to do takes 2.5).
-    passes = many ? std::min<std::size_t>(std::max<std::size_t>(nodes - 1, 1), 3) : 1;
+    // of 128256 take 41 us with three such launches and 44 with four where three
+    // are enough, 64 and 50 where they are not: one that finds nothing to do
+    // takes 2.5 us, a sum left to verify_finish_kernel 15.
+    passes = many ? std::min<std::size_t>(std::max<std::size_t>(nodes - 1, 1), 4) : 1;
   }
   std::size_t walk_bytes(std::size_t batch) const { return passes * batch * sizeof(Walk); }
   std::size_t bytes(std::size_t batch) const {
