@@ -177,14 +177,21 @@ __device__ __forceinline__ void chunk_of_rows(v4f x0, v4f x1, float scale,
   }
 }
 
-// Whether the wavefronts of a workgroup take turns (tree_mma_body), and the
-// LDS buffers that takes: a block is put there two steps before its use, or one
-// step, or (fp32 pages, whose three planes would take the space of a second
-// workgroup) just before it.
-constexpr bool in_turns(int pf, int waves) { return pf == 1 && waves > 4; }
-constexpr int stage_buffers(int pf, int waves) {
-  return pf == 0 ? 1 : in_turns(pf, waves) ? 3 : 2;
+// Whether the two wavefronts of each SIMD take turns (tree_mma_body), and the LDS
+// buffers that takes: an item is put there two steps before its use, or one step,
+// or (fp32 pages, whose three planes would take the space of a second workgroup)
+// just before it.  (131071 bf16 tokens, 33 nodes: 331 us in turns, 351 without.)
+constexpr bool in_turns(int pf, int waves, int tiles) {
+  return pf == 1 && waves == 8 && tiles == 2;
 }
+constexpr int stage_buffers(int pf, int waves, int tiles) {
+  return pf == 0 ? 1 : in_turns(pf, waves, tiles) ? 3 : 2;
+}
+
+// Items on their way from memory to registers.  (64 bf16 sequences of 16 nodes:
+// 178 us with two, 190 with one.  fp32 pages gain nothing, and fp8 pages more from
+// the registers of a third workgroup on the CU.)
+constexpr int load_depth(int pf, int tiles) { return pf == 1 && tiles == 1 ? 2 : 1; }
 
 template <int PF, int W, int RT>
 struct TreeShared {
@@ -193,7 +200,7 @@ struct TreeShared {
     __align__(1024) unsigned char k[page_terms(PF)][kBlock * 2 * D];
     __align__(1024) unsigned char v[page_terms(PF)][kBlock * 2 * D];
   };
-  Item item[stage_buffers(PF, W)];
+  Item item[stage_buffers(PF, W, RT)];
   // The third terms of the query operands: [tile][step][lane].
   __align__(16) v4u low[row_terms(PF) == 3 ? W * RT : 1][row_terms(PF) == 3 ? 4 : 1][64];
 };
@@ -309,22 +316,29 @@ struct TreeSource {
 // the block before) from registers into LDS and sends for the next one's; turns
 // block n's scores into probabilities; and, past a barrier, takes block n's P V
 // and the scores of block n + 1, matrix instructions one behind another.
-// With up to four wavefronts a workgroup has one on each SIMD, and those of
-// other workgroups run beside it.  With more, the first four and the others
-// take turns: a second barrier and half a step between them have one of a
-// SIMD's two wavefronts at its matrix instructions while the other is at its
-// vector instructions.
+// Where they take turns, the first four wavefronts and the others are half a step
+// apart, with a second barrier: one of a SIMD's two is at its matrix instructions
+// while the other is at its vector instructions.
+// Steps whose items are whole pages of one unit run in a loop of their own, where
+// the compiler knows which loads are on their way.
 template <int PF, int W, int RT>
 __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const TreeStream& st,
                                               TreeShared<PF, W, RT>& sh) {
-  // 1 KiB of 16-bit elements in LDS, four rows, is a job of a wavefront: eight
-  // for K, and the same rows' for V.
+  // Four tree rows are a job of a wavefront: eight for K, and the same rows' for
+  // V.  Of pages a job is what loads of 16 bytes a lane bring, without gaps: four
+  // rows in two loads or one, or eight rows of fp8.
   static_assert(8 % W == 0);
-  constexpr int NJ = 8 / W;
+  constexpr int NT = 8 / W;
+  constexpr int kJobRows = PF == 2 ? 8 : 4;
+  constexpr int NJ = kBlock / kJobRows / W;
+  constexpr int RW = PF == 0 ? 2 : 1;
   constexpr int RB = 16 * W * RT;
   constexpr int KT = page_terms(PF), QT = row_terms(PF);
-  constexpr int NB = stage_buffers(PF, W);
-  constexpr bool kTurns = in_turns(PF, W);
+  constexpr int NB = stage_buffers(PF, W, RT);
+  constexpr bool kTurns = in_turns(PF, W, RT);
+  constexpr int DEPTH = load_depth(PF, RT);
+  // Blocks from the one whose scores are taken to the one located last.
+  constexpr int kLead = kTurns ? DEPTH + 1 : DEPTH;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -351,9 +365,8 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
   unsigned page_lo = 0, page_hi = 0;
   int pages_of = -1, pages_at = 0;
   int bad_page = 0;  // some of them are none
-  // Job i of this wavefront: rows 4 j + grp, j = wave + W i, 8 elements from 8 col
-  // on, of K and V.  key_at[i]: this lane's bytes of K in the page pool, of
-  // the block located last; V's are as far on in its pool, one block later.
+  // key_at[i]: K of job i in the page pool, 16 bytes a lane from there on, of the
+  // block located last; V is as far on in its pool, one block later.
   // Before any block of pages: page 0.
   unsigned long long key_at[NJ], value_at[NJ];
 #pragma unroll
@@ -364,14 +377,15 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
   const unsigned long long value_off = static_cast<unsigned long long>(
       static_cast<const unsigned char*>(a.value_pool) - static_cast<const unsigned char*>(a.key_pool));
   auto job = [&](int i) { return wave + W * i; };
+  auto job_row = [&](int i) { return kJobRows * job(i); };
   auto locate_pages = [&](int first) {
 #pragma unroll
     for (int i = 0; i < NJ; ++i) {
-      const int n = first + ((job(i) >> 2) & 1);
+      const int n = first + job_row(i) / P;
       const unsigned lo = __builtin_amdgcn_readlane(page_lo, n);
       const unsigned hi = __builtin_amdgcn_readlane(page_hi, n);
       key_at[i] = (static_cast<unsigned long long>(hi) << 32 | lo) +
-                  static_cast<unsigned>((4 * job(i) % P) * (D * kElem) + lane * (8 * kElem)) +
+                  static_cast<unsigned>(job_row(i) % P * (D * kElem)) +
                   reinterpret_cast<std::uintptr_t>(a.key_pool);
     }
   };
@@ -407,53 +421,78 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
     return s;
   };
 
-  using Raw = std::conditional_t<PF == 0, v4f, std::conditional_t<PF == 1, v4u, v2u>>;
+  using Raw = std::conditional_t<PF == 0, v4f, v4u>;
   using Global = const __attribute__((address_space(1))) Raw*;
+  using GlobalBytes = const __attribute__((address_space(1))) unsigned char*;
+  const unsigned lane_at = static_cast<unsigned>(lane) * 16u;
+  auto stream = [&](unsigned long long at, int w) {  // (each byte is read once)
+    return __builtin_nontemporal_load(
+        reinterpret_cast<Global>(reinterpret_cast<GlobalBytes>(at + 1024u * w) + lane_at));
+  };
   using GlobalRows = const __attribute__((address_space(1))) v4f*;
-  constexpr int RW = PF == 0 ? 2 : 1;
-  Raw key_raw[NJ * RW], value_raw[NJ * RW];
-  auto load_pages = [&] {
+  Raw key_raw[DEPTH][NJ * RW], value_raw[DEPTH][NJ * RW];
+  auto load_pages = [&](auto set) {
+    constexpr int S = decltype(set)::value;
+    // (Or loads from an address that was loaded from before become copies.)
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < NJ; ++i) {
 #pragma unroll
-      for (int w = 0; w < RW; ++w) key_raw[RW * i + w] = reinterpret_cast<Global>(key_at[i])[w];
+      for (int w = 0; w < RW; ++w) {
+        key_raw[S][RW * i + w] = stream(key_at[i], w);
+      }
     }
 #pragma unroll
     for (int i = 0; i < NJ; ++i) {
 #pragma unroll
-      for (int w = 0; w < RW; ++w) value_raw[RW * i + w] = reinterpret_cast<Global>(value_at[i])[w];
+      for (int w = 0; w < RW; ++w) {
+        value_raw[S][RW * i + w] = stream(value_at[i], w);
+      }
     }
   };
-  auto from_pages = [&](const Raw* x, v4u (&t)[KT]) {
+  // A job's loads into the planes `to`, chunks of 8 elements at at(row, chunk);
+  // rows from `rows` on become 0.
+  auto put_raw = [&](unsigned char* to, auto at, int row0, const Raw* x, int rows) {
+    constexpr std::size_t kPlane = kBlock * 2 * D;
     if constexpr (PF == 0) {
-      chunk_of_rows<0>(x[0], x[1], 1.0f, t);
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
+        const int row = row0 + 2 * w + (lane >> 5);
+        unsigned p[2][3];
+        split_pair<0>(x[w][0], x[w][1], p[0]);
+        split_pair<0>(x[w][2], x[w][3], p[1]);
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          *reinterpret_cast<v2u*>(to + n * kPlane + at(row, (lane & 31) >> 1) + 8 * (lane & 1)) =
+              row >= rows ? v2u{0u, 0u} : v2u{p[0][n], p[1][n]};
+        }
+      }
     } else if constexpr (PF == 1) {
-      t[0] = x[0];
+      const int row = row0 + grp;
+      *reinterpret_cast<v4u*>(to + at(row, col)) = row >= rows ? v4u{0u, 0u, 0u, 0u} : x[0];
     } else {
-      t[0] = codes_fp16(x[0][0], x[0][1]);
+      const int row = row0 + (lane >> 3);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<v4u*>(to + at(row, 2 * (lane & 7) + h)) =
+            row >= rows ? v4u{0u, 0u, 0u, 0u} : codes_fp16(x[0][2 * h], x[0][2 * h + 1]);
+      }
     }
   };
-  auto put_key = [&](int buf, int i, const v4u (&t)[KT]) {
-#pragma unroll
-    for (int n = 0; n < KT; ++n) {
-      *reinterpret_cast<v4u*>(sh.item[buf].k[n] + bmma_k_at(4 * job(i) + grp, col)) = t[n];
-    }
+  auto k_place = [](int row, int chunk) { return bmma_k_at(row, chunk); };
+  auto v_place = [](int row, int chunk) { return bmma_v_at(row, chunk); };
+  auto put_key_raw = [&](auto set, int buf, int i) {
+    put_raw(sh.item[buf].k[0], k_place, job_row(i), key_raw[decltype(set)::value] + RW * i, kBlock);
   };
-  auto put_value = [&](int buf, int i, const v4u (&t)[KT]) {
-#pragma unroll
-    for (int n = 0; n < KT; ++n) {
-      *reinterpret_cast<v4u*>(sh.item[buf].v[n] + bmma_v_at(4 * job(i) + grp, col)) = t[n];
-    }
+  auto put_value_raw = [&](auto set, int buf, int i, int rows) {
+    put_raw(sh.item[buf].v[0], v_place, job_row(i), value_raw[decltype(set)::value] + RW * i, rows);
   };
   // An item of whole pages into LDS.
-  auto store_pages = [&](int buf) {
+  auto store_pages = [&](auto set, int buf) {
 #pragma unroll
     for (int i = 0; i < NJ; ++i) {
-      v4u t[KT];
-      from_pages(key_raw + RW * i, t);
-      put_key(buf, i, t);
-      from_pages(value_raw + RW * i, t);
-      put_value(buf, i, t);
+      put_key_raw(set, buf, i);
+      put_value_raw(set, buf, i, kBlock);
     }
   };
   // Any item: what was loaded, or (`s.tree`) rows read now.  (Those read ahead
@@ -464,35 +503,44 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         rows + s.at + min(4 * job(i) + grp, s.rows - 1) * D + col * 8));
     chunk_of_rows<PF>(x[0], x[1], scale, t);
   };
-  auto store_key = [&](int buf, const TreeSource& s) {
+  auto store_key = [&](auto set, int buf, const TreeSource& s) {
+    if (s.tree == 0) {
 #pragma unroll
-    for (int i = 0; i < NJ; ++i) {
+      for (int i = 0; i < NJ; ++i) put_key_raw(set, buf, i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
       v4u t[KT];
-      if (s.tree != 0) {
-        from_rows(s, a.tree_key, a.k_scale, i, t);
-      } else {
-        from_pages(key_raw + RW * i, t);
+      from_rows(s, a.tree_key, a.k_scale, i, t);
+#pragma unroll
+      for (int n = 0; n < KT; ++n) {
+        *reinterpret_cast<v4u*>(sh.item[buf].k[n] + bmma_k_at(4 * job(i) + grp, col)) = t[n];
       }
-      put_key(buf, i, t);
     }
   };
-  auto store_value = [&](int buf, const TreeSource& s) {
+  // (Rows behind the sequence's must be finite.)
+  auto store_value = [&](auto set, int buf, const TreeSource& s) {
+    if (s.tree == 0) {
 #pragma unroll
-    for (int i = 0; i < NJ; ++i) {
+      for (int i = 0; i < NJ; ++i) put_value_raw(set, buf, i, s.rows);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
       v4u t[KT];
-      if (s.tree != 0) {
-        from_rows(s, a.tree_value, a.v_scale, i, t);
-      } else {
-        from_pages(value_raw + RW * i, t);
-      }
-      // Rows behind the sequence's must be finite.
+      from_rows(s, a.tree_value, a.v_scale, i, t);
 #pragma unroll
-      for (int n = 0; n < KT; ++n) t[n] = 4 * job(i) + grp >= s.rows ? v4u{0u, 0u, 0u, 0u} : t[n];
-      put_value(buf, i, t);
+      for (int n = 0; n < KT; ++n) {
+        *reinterpret_cast<v4u*>(sh.item[buf].v[n] + bmma_v_at(4 * job(i) + grp, col)) =
+            4 * job(i) + grp >= s.rows ? v4u{0u, 0u, 0u, 0u} : t[n];
+      }
     }
   };
 
-  // The wavefront's rows of the unit: tile t's row `col`.
+  // The wavefront's rows of the unit: tile t's row `col`, from tile_row(t) on.
+  auto tile_row = [&](int t) { return (t * W + wave) * 16; };
+  bool live = false;  // the first of them has rows
   v4u qop[RT][2][4];  // (the third term of three is in LDS)
   float unscale[RT];  // fp8 pages: what undoes the row's power of two
   int parent = -1;    // of node `lane`
@@ -508,9 +556,10 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
   auto start = [&](const TreeCursor& c) {
     const float scale = PF == 2 ? a.qscale * a.k_scale : a.qscale;
     parent = node_parent(a, c.b, c.count, lane);
+    live = c.rb * RB + tile_row(0) < a.rows;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int row = c.rb * RB + (wave * RT + t) * 16 + col;
+      const int row = c.rb * RB + tile_row(t) + col;
       v4f x[4][2];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -563,62 +612,64 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
 
   // Scores of a block: sc[t][h][i] is key 16 h + 4 grp + i of tile t's row col.
   const unsigned k_at = bmma_k_at(col, grp);
-  // (Operands come out of LDS two steps of 32 dims, or four tiles of 16, ahead
-  // of the instructions that take them.)
-  constexpr int kProducts = PF == 0 ? 6 : QT;
-  auto scores = [&](int buf, v4f (&sc)[RT][2]) {
+  // (Operands come out of LDS ahead of the instructions that take them: a half
+  // block's 32 dims, or a tile's 16, are 48 to 96 cycles of these.)
+  constexpr int kAhead = PF == 0 || RT == 1 ? 2 : PF == 2 ? 3 : 4;
+  auto scores = [&](auto tiles, int buf, v4f (&sc)[RT][2]) {
+    constexpr int LT = decltype(tiles)::value;
+    static_assert(QT != 3 || kAhead == 2 || kAhead == 4);
+    v4u kop[kAhead][KT], low[2][RT];
+    auto read = [&](int u) {  // 32 dims, from 32 (u / 2) on, of keys 16 (u % 2) and on
+      const int s = u / 2, h = u % 2;
+      // (Of `low` two 32 dims' are there: the next ones' come after the last use.)
+      if (QT == 3 && h == (kAhead == 4 ? 1 : 0)) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) sc[t][0] = sc[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      v4u low[RT];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        if constexpr (QT == 3) {
-          low[t] = sh.low[wave * RT + t][s][lane];
-        }
+        for (int t = 0; t < LT; ++t) low[s % 2][t] = sh.low[wave * RT + t][QT == 3 ? s : 0][lane];
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v4u kop[KT];
+      for (int i = 0; i < KT; ++i) {
+        kop[u % kAhead][i] =
+            *reinterpret_cast<const v4u*>(sh.item[buf].k[i] + h * (P * 2 * D) + (k_at ^ (64u * s)));
+      }
+    };
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-          kop[i] =
-              *reinterpret_cast<const v4u*>(sh.item[buf].k[i] + h * (P * 2 * D) + (k_at ^ (64u * s)));
-        }
-        // Smallest products first.
+    for (int u = 0; u < kAhead; ++u) read(u);
 #pragma unroll
-        for (int sum = QT - 1; sum >= 0; --sum) {
+    for (int t = 0; t < LT; ++t) sc[t][0] = sc[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = KT - 1; i >= 0; --i) {
-            if (sum - i < 0 || sum - i >= QT) continue;
+    for (int u = 0; u < 8; ++u) {
+      const int s = u / 2, h = u % 2;
+      // Smallest products first.
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-              sc[t][h] =
-                  matrix_step<PF>(kop[i], sum - i == 2 ? low[t] : qop[t][sum - i & 1][s], sc[t][h]);
-            }
+      for (int sum = QT - 1; sum >= 0; --sum) {
+#pragma unroll
+        for (int i = KT - 1; i >= 0; --i) {
+          if (sum - i < 0 || sum - i >= QT) continue;
+#pragma unroll
+          for (int t = 0; t < LT; ++t) {
+            sc[t][h] = matrix_step<PF>(kop[u % kAhead][i],
+                                       sum - i == 2 ? low[s % 2][t] : qop[t][sum - i & 1][s],
+                                       sc[t][h]);
           }
         }
       }
+      if (u + kAhead < 8) read(u + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    constexpr int kReads = 2 * KT + (QT == 3 ? RT : 0), kSteps = 2 * RT * kProducts;
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kReads, 0);
-    __builtin_amdgcn_sched_group_barrier(0x8, kSteps, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
-    __builtin_amdgcn_sched_group_barrier(0x8, kSteps, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
-    __builtin_amdgcn_sched_group_barrier(0x8, 2 * kSteps, 0);
   };
   // m[t] is a reference near the row's maximum: it moves where a score is above
   // it by more than kSlack, and what was summed with it.  `vis[t]`: the lane's
   // keys (bit 4 h + i) that the row sees.  Returns whether every key is seen and
   // every reference finite.
-  auto maxima = [&](const TreeCursor& c, v4f (&sc)[RT][2], unsigned (&vis)[RT]) {
+  auto maxima = [&](auto tiles, auto whole, const TreeCursor& c, v4f (&sc)[RT][2],
+                    unsigned (&vis)[RT]) {
+    constexpr int LT = decltype(tiles)::value;
     const bool in_tree = c.blk >= c.nbh;
     const int seen = c.hist - c.blk * kBlock;
-    const bool full = !in_tree && seen >= kBlock;
+    const bool full = decltype(whole)::value || (!in_tree && seen >= kBlock);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) vis[t] = 0xffu;
+    for (int t = 0; t < LT; ++t) vis[t] = 0xffu;
     if (__builtin_expect(!full, 0)) {
       unsigned bits[RT];  // the block's keys that the row sees
       if (in_tree) {
@@ -626,17 +677,17 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         tree_words(parent, c.count, lane, tree);
         broken = __ballot(tree.broken != 0);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const int row = c.rb * RB + (wave * RT + t) * 16 + col;
+        for (int t = 0; t < LT; ++t) {
+          const int row = c.rb * RB + tile_row(t) + col;
           const unsigned long long w = shfl64(tree.seen, row % a.nodes);
           bits[t] = row < a.rows ? static_cast<unsigned>(w >> ((c.blk - c.nbh) * kBlock)) : 0u;
         }
       } else {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) bits[t] = (1u << seen) - 1u;
+        for (int t = 0; t < LT; ++t) bits[t] = (1u << seen) - 1u;
       }
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
+      for (int t = 0; t < LT; ++t) {
         vis[t] = ((bits[t] >> (4 * grp)) & 0xfu) | ((bits[t] >> (16 + 4 * grp)) & 0xfu) << 4;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -647,7 +698,7 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
     float mx[RT];
     bool above = false;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < LT; ++t) {
       const v4f x0 = sc[t][0], x1 = sc[t][1];
       mx[t] = larger(larger(larger(x0[0], x0[1]), larger(x0[2], x0[3])),
                      larger(larger(x1[0], x1[1]), larger(x1[2], x1[3])));
@@ -657,7 +708,7 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
     if (__ballot(above) != 0) {
       finite = true;
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
+      for (int t = 0; t < LT; ++t) {
         const float mn = fmaxf(m[t], row_max(mx[t]));
         const float alpha = exp2_ratio(m[t], mn);
 #pragma unroll
@@ -670,11 +721,12 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
     return full && finite;
   };
   // Probabilities of the block's scores as operands; FINE: maxima() said so.
-  auto probabilities = [&](auto fine_tag, v4f (&sc)[RT][2], const unsigned (&vis)[RT],
+  auto probabilities = [&](auto tiles, auto fine_tag, v4f (&sc)[RT][2], const unsigned (&vis)[RT],
                            v4u (&pop)[RT][QT]) {
+    constexpr int LT = decltype(tiles)::value;
     constexpr bool FINE = decltype(fine_tag)::value;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < LT; ++t) {
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -700,9 +752,9 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
   };
   const unsigned v_at =
       bmma_v_at(4 * grp + (col >> 2), 0) + static_cast<unsigned>((col & 3) * 8);
-  auto add_values = [&](int buf, const v4u (&pop)[RT][QT]) {
+  auto add_values = [&](auto tiles, int buf, const v4u (&pop)[RT][QT]) {
+    constexpr int LT = decltype(tiles)::value;
     using LdsV4s = __attribute__((address_space(3))) v4s;
-    constexpr int kAhead = PF == 0 ? 2 : 4;
     v4u vop[kAhead][KT];
     auto read = [&](int dt) {
 #pragma unroll
@@ -725,7 +777,7 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         for (int i = KT - 1; i >= 0; --i) {
           if (sum - i < 0 || sum - i >= QT) continue;
 #pragma unroll
-          for (int t = 0; t < RT; ++t) {
+          for (int t = 0; t < LT; ++t) {
             o[t][dt] = matrix_step<PF>(vop[dt % kAhead][i], pop[t][sum - i], o[t][dt]);
           }
         }
@@ -752,7 +804,7 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         complete ? st.unit_marks + unit * kMaxTiles : st.part_marks + slot * kMaxTiles;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int row = c.rb * RB + (wave * RT + t) * 16 + col, node = row % a.nodes;
+      const int row = c.rb * RB + tile_row(t) + col, node = row % a.nodes;
       const bool live = row < a.rows && node < c.count;
       const bool lost = bad || ((broken >> node) & 1) != 0;
       const float sum = row_sum(l[t]);
@@ -763,8 +815,8 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
         for (int i = 0; i < 4; ++i) nan = nan || isnan(o[t][dt][i]);
       const bool again = __ballot(nan && live && !lost) != 0;
       if (lane == 0) {
-        marks[wave * RT + t] = again ? 1 : 0;
-        if (ends && !starts) st.unit_marks[unit * kMaxTiles + wave * RT + t] = 0;
+        marks[t * W + wave] = again ? 1 : 0;
+        if (ends && !starts) st.unit_marks[unit * kMaxTiles + t * W + wave] = 0;
       }
       if (!live) continue;
       float f = vscale;
@@ -789,98 +841,178 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
   };
 
   // Item i of the range, K of its block i and V of block i - 1, is put into
-  // buffer i % NB.  Behind the range, items go on that no one reads.
-  TreeCursor ahead = cur;  // the block of `key`
-  TreeSource key = locate(ahead), value{};
-  unsigned bads = key.bad;  // bit i % 32: of block i, as far as it was located
-  int item = 0;             // the one on its way,
-  int into = 0;             // the buffer it goes to
-  // Items from this one on that are whole pages of one sequence, with page
-  // offsets in hand, and have such a one behind them.
+  // buffer i % NB from register set i % DEPTH; DEPTH items are on their way.
+  // Behind the range, items go on that no one reads.
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, DEPTH - 1>;
+  TreeCursor ahead = cur;        // the block located last,
+  int located = 0;               // and its item
+  TreeSource key[DEPTH], value;  // of the item to put, and later ones; of the one before
+  key[0] = locate(ahead);
+  value = key[0];
+  unsigned bads = key[0].bad;  // bit i % 32: of block i, as far as it was located
+  int item = 0;                // the one to put,
+  int into = 0;                // the buffer it goes to
+  // Steps from the next one on whose item to put is whole pages, of the unit of
+  // the blocks before it, and that locate such a block with page offsets in hand.
   int plain = 0;
-  auto put = [&] {
-    // Everything sent for is there.  (Said here, or the compiler waits where the
-    // registers are loaded next.)
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    if (__builtin_expect(plain > 0, 1)) {
-      store_pages(into);
-    } else {
-      if (item < blocks) store_key(into, key);
-      if (item > 0 && item <= blocks) store_value(into, value);
+  auto locate_next = [&] {
+    TreeSource s = key[DEPTH - 1];
+    plain = 0;
+    if (++located < blocks) {
+      advance(a, st, ahead);
+      s = locate(ahead);
+      bads |= static_cast<unsigned>(s.bad) << (located & 31);
+      if (s.tree == 0 && ahead.blk >= kLead && located > kLead) {
+        plain = min(min(ahead.nbh - 1, (pages_at >> 1) + 31) - ahead.blk, blocks - 1 - located);
+      }
     }
+    return s;
+  };
+  // The item sent for first goes to LDS, and the next one is sent for: of whole
+  // pages, or any.
+  auto put_pages = [&](auto set) {
+    // What was sent for first is there.  (Said here, or the compiler waits for all
+    // where the registers are loaded next.)
+    __builtin_amdgcn_s_waitcnt(0x0f70 + (DEPTH - 1) * 2 * NJ * RW);
+    store_pages(set, into);
+    into = into + 1 == NB ? 0 : into + 1;
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) value_at[i] = key_at[i] + value_off;
+    ++ahead.blk;
+    locate_pages(2 * ahead.blk - pages_at);
+    load_pages(set);
+  };
+  auto put = [&](auto set) {
+    if (item < blocks) store_key(set, into, key[0]);
+    if (item > 0 && item <= blocks) store_value(set, into, value);
     into = into + 1 == NB ? 0 : into + 1;
     ++item;
 #pragma unroll
     for (int i = 0; i < NJ; ++i) value_at[i] = key_at[i] + value_off;
-    if (__builtin_expect(plain > 0, 1)) {
-      --plain;
-      ++ahead.blk;
-      key.rows -= kBlock;
-      locate_pages(2 * ahead.blk - pages_at);
-    } else {
-      value = key;
-      if (item < blocks) {
-        advance(a, st, ahead);
-        key = locate(ahead);
-        bads |= static_cast<unsigned>(key.bad) << (item & 31);
-        if (key.tree == 0 && ahead.blk > 0 && item > 1) {
-          plain = min(min(ahead.nbh - 1, (pages_at >> 1) + 31) - ahead.blk, blocks - 1 - item);
-        }
-      }
-    }
+    value = key[0];
+    if constexpr (DEPTH == 2) key[0] = key[1];
+    key[DEPTH - 1] = locate_next();
     // (On every path, where what is located is needed or not: loads on some paths
     // only are copied, and so waited for, where the paths meet.)
-    load_pages();
+    load_pages(set);
   };
-  load_pages();
-  put();
-  if constexpr (NB == 3) put();
+  load_pages(Even{});
+  if constexpr (DEPTH == 2) {
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) value_at[i] = key_at[i] + value_off;
+    key[1] = key[0];
+    key[1] = locate_next();
+    load_pages(Odd{});
+  }
+  put(Even{});
+  if constexpr (kTurns) put(Odd{});
   start(cur);
   v4f sc[RT][2];
   barrier();
-  scores(0, sc);
+  using All = std::integral_constant<int, RT>;
+  scores(All{}, 0, sc);
   const bool second = kTurns && wave >= 4;
   if (second) barrier();
   int from = cur.blk;  // the unit's first block in this range
   int bad = 0;         // of the unit
-  for (int n = 0, buf = 0;; ++n) {
-    if constexpr (NB == 1) barrier();  // the last step's reads are done
-    put();
-    __builtin_amdgcn_sched_barrier(0);
-    bad |= static_cast<int>(bads >> (n & 31)) & 1;
-    bads &= ~(1u << (n & 31));
+  int n = 0, buf = 0;
+  // Block n's probabilities; item n + 1 goes to LDS meanwhile.
+  auto soften = [&](auto tiles, auto whole, v4u (&pop)[RT][QT]) {
     unsigned vis[RT];
-    v4u pop[RT][QT];
-    if (maxima(cur, sc, vis)) {
-      probabilities(std::true_type{}, sc, vis, pop);
-    } else {
-      probabilities(std::false_type{}, sc, vis, pop);
+    if constexpr (decltype(tiles)::value > 0) {
+      if (maxima(tiles, whole, cur, sc, vis)) {
+        probabilities(tiles, std::true_type{}, sc, vis, pop);
+      } else {
+        probabilities(tiles, std::false_type{}, sc, vis, pop);
+      }
     }
     barrier();
     buf = buf + 1 == NB ? 0 : buf + 1;
-    __builtin_amdgcn_s_setprio(1);
-    add_values(buf, pop);
+  };
+  auto page_step = [&](auto tiles, auto set) {
+    if constexpr (NB == 1) barrier();  // the last step's reads are done
+    put_pages(set);
+    __builtin_amdgcn_sched_barrier(0);
+    v4u pop[RT][QT];
+    soften(tiles, std::true_type{}, pop);
+    if constexpr (decltype(tiles)::value > 0) {
+      __builtin_amdgcn_s_setprio(1);
+      add_values(tiles, buf, pop);
+      scores(tiles, buf, sc);
+      __builtin_amdgcn_s_setprio(0);
+    }
+    if constexpr (kTurns) barrier();
+  };
+  auto page_steps = [&](auto tiles, int steps) {
+#pragma unroll 1
+    for (int i = 0; i < steps; i += DEPTH) {
+      page_step(tiles, Odd{});
+      if constexpr (DEPTH == 2) page_step(tiles, Even{});
+    }
+  };
+  auto step = [&](auto set) {
+    if constexpr (NB == 1) barrier();
+    put(set);
+    __builtin_amdgcn_sched_barrier(0);
+    bad |= static_cast<int>(bads >> (n & 31)) & 1;
+    bads &= ~(1u << (n & 31));
+    v4u pop[RT][QT];
+    soften(All{}, std::false_type{}, pop);
+    add_values(All{}, buf, pop);
     const bool last = n + 1 == blocks;
     if (last || cur.blk + 1 == cur.nb) {
-      __builtin_amdgcn_s_setprio(0);
       finish(cur, from, range.g0 + n, bad != 0);
-      if (last) break;
+      if (last) return false;
       advance(a, st, cur);
       from = bad = 0;
       start(cur);
     } else {
       ++cur.blk;
     }
-    scores(buf, sc);
-    __builtin_amdgcn_s_setprio(0);
+    scores(All{}, buf, sc);
     if constexpr (kTurns) barrier();
+    ++n;
+    return true;
+  };
+  // (Step n puts item n + 1, or in turns n + 2.)
+  static_assert(!kTurns || DEPTH == 1);
+  for (;;) {
+    if (plain >= DEPTH) {
+      // (Every block on its way is of this unit.)
+      bad |= bads != 0 ? 1 : 0;
+      bads = 0;
+      const int steps = plain / DEPTH * DEPTH;
+      // (Or the compiler, not knowing what is on its way from here, waits for all
+      // in every second step.)
+      if constexpr (DEPTH == 2) __builtin_amdgcn_s_waitcnt(0x0f70);
+      // (A tile without rows keeps the scores it had; nothing of it is used.)
+      if (RT > 1 || live) {
+        page_steps(All{}, steps);
+      } else {
+        page_steps(std::integral_constant<int, 0>{}, steps);
+      }
+      plain -= steps;
+      n += steps;
+      item += steps;
+      located += steps;
+      cur.blk += steps;
+      key[DEPTH - 1].rows -= steps * kBlock;
+      if constexpr (DEPTH == 2) key[0].rows = key[1].rows + kBlock;
+      value.rows = key[0].rows + kBlock;
+    }
+    if (!step(Odd{})) break;
+    if constexpr (DEPTH == 2) {
+      if (!step(Even{})) break;
+    }
   }
   if (kTurns && !second) barrier();
 }
 
 template <int PF, int W, int RT>
 __global__ __launch_bounds__(64 * W)
-    __attribute__((amdgpu_waves_per_eu(2))) void tree_mma_kernel(TreeKernelArgs a, TreeStream st) {
+    __attribute__((amdgpu_waves_per_eu(PF == 2 && RT == 1 ? 3 : 2)))
+    void tree_mma_kernel(TreeKernelArgs a, TreeStream st) {
   __shared__ TreeShared<PF, W, RT> sh;
   tree_mma_body<PF, W, RT>(a, st, sh);
 }
@@ -1040,9 +1172,12 @@ struct TreeShape {
   std::size_t rows() const { return static_cast<std::size_t>(waves) * tiles * 16; }
 };
 
-// A unit's rows: enough wavefronts to load pages with, and the fewest row blocks
-// that registers allow, as each reads the pages again.  As many workgroups as
-// fit on the chip at once.
+// A unit's rows and the workgroups that the chip holds at once.  Of 32 sequences
+// with bf16, fp8 and fp32 pages: 64 rows take 125, 100 and 200 us with four
+// wavefronts and 183, 189 and 288 with eight; 128 rows 159, 131 and 287 in two row
+// blocks of four wavefronts, 158, - and 256 in one of eight, -, 123 and - in one of
+// four with two tiles each; 256 rows 324, 262 and 572 in one of eight with two tiles,
+// 359, - and 637 in two blocks of eight, -, 261 and - in two of four with two tiles.
 TreeShape tree_shape(PageType type, std::size_t rows) {
   if (type == PageType::kFP8) {
     return rows <= 64 ? TreeShape{4, 1, 3 * kTreeCus} : TreeShape{4, 2, 2 * kTreeCus};

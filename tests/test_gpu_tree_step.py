@@ -157,6 +157,19 @@ def test_long_histories_split_over_the_device(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,nodes", [(2, 8), (4, 16), (4, 29), (8, 16), (4, 33), (4, 64)])
+def test_results_are_fp32_results(device, dtype, hq, nodes):
+    """Every bit of the fp32 factors takes part, in each shape of the kernel (16 to
+    256 rows a head).  A score's partial sums lie below 4 (in powers of two), so
+    each of its 12 roundings is off by 2^-22 / sqrt(12) in the mean square, and the
+    score by 2^-22: a weight by 2^-22.5 of itself, the row's sums and quotient by
+    2^-23 or so each.  A factor cut to 16 bits moves the scores by 2^-18."""
+    p = Problem(dtype, [3001], hq, 1, nodes, 300 + nodes)
+    got, want = p.run(), p.want()
+    assert np.linalg.norm(got - want) <= 2.0 ** -20 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_what_a_row_does_not_see_does_not_reach_it(device, dtype):
     """NaN and infinities in the slots behind a history, in pages of no
     sequence, in tree rows outside a node's way to its root and behind the
