@@ -33,7 +33,8 @@
  *
  * Extensions beyond the reference's CUDA API (each also in helix_paged.h):
  * fork_sequence with copy-on-write, append_layer_major, copy_layer_out,
- * bf16 pages, and DecodeBatch, the batched decode / chunked-prefill driver.
+ * truncate_sequence, bf16 pages, and DecodeBatch, the batched decode /
+ * chunked-prefill / tree-step driver.
  *
  * Link with -lhelix_paged -lamdhip64; compile with -D__HIP_PLATFORM_AMD__
  * when the compiler is not hipcc. */
@@ -327,6 +328,19 @@ inline void require_float_on(const Tensor& t, int device, std::size_t rank, cons
 
 inline std::size_t dim(const Tensor& t, std::size_t i) {
   return static_cast<std::size_t>(t.shape()[i]);
+}
+
+inline void require_int_on(const Tensor& t, int device, std::span<const std::size_t> dims,
+                           const char* what) {
+  bool fits = t.dtype() == DType::kInt32 && t.device().is_gpu() && t.device().index == device &&
+              t.rank() == dims.size();
+  for (std::size_t i = 0; fits && i < dims.size(); ++i) fits = dim(t, i) == dims[i];
+  if (!fits) {
+    std::string shape;
+    for (const std::size_t n : dims) shape += (shape.empty() ? "" : ", ") + std::to_string(n);
+    throw_error(ErrorCode::kInvalidArgument, std::string(what) + ": expected an int32 tensor [" +
+                                                 shape + "] on GPU " + std::to_string(device));
+  }
 }
 
 inline int current_device() {
@@ -701,6 +715,12 @@ class HipPagedKvCache final {
     detail::check(helix_paged_cache_release_sequence(impl_->cache, sequence.native()));
   }
 
+  /// Extension: back to the first `length` tokens; the pages behind them are
+  /// free again.
+  void truncate_sequence(const HipPagedSequenceHandle& sequence, std::size_t length) {
+    detail::check(helix_paged_cache_truncate_sequence(impl_->cache, sequence.native(), length));
+  }
+
   /// Gather one layer of a sequence into compact [kv_heads, length,
   /// head_dimension] tensors (copy_layer_out, src/kv_cache/paged.cpp:873-950).
   void copy_layer_out(const HipPagedSequenceHandle& sequence, std::size_t layer, Tensor& keys_out,
@@ -1058,6 +1078,82 @@ class DecodeBatch final {
         batch_handle_, layer, query.data_as<float>(), chunk_key.data_as<float>(),
         chunk_value.data_as<float>(), output.data<float>(), stream.native()));
   }
+  /// A tree step: up to `nodes` drafted tokens per sequence are checked at once.
+  /// tree_layer() is one layer's attention (rows [B, heads, nodes, D]; parents
+  /// [B, nodes] int32 or nullptr: chains; node_counts [B] int32 or nullptr: all
+  /// nodes); commit_path() or accept_tree() ends the step.
+  void prepare_tree(std::size_t nodes, const hip::Stream& stream) {
+    step_tokens_ = 0;
+    detail::check(helix_decode_batch_prepare_tree(batch_handle_, nodes, stream.native()));
+    step_tokens_ = nodes;
+    chunked_ = true;
+  }
+  void tree_layer(std::size_t layer, const Tensor& query, const Tensor& tree_key,
+                  const Tensor& tree_value, const Tensor* parents, const Tensor* node_counts,
+                  Tensor& output, const hip::Stream& stream) {
+    chunk_rows(query, "tree query", q_heads_);
+    chunk_rows(tree_key, "tree key", kv_heads_);
+    chunk_rows(tree_value, "tree value", kv_heads_);
+    chunk_rows(output, "tree output", q_heads_);
+    detail::check(helix_decode_batch_tree_layer(
+        batch_handle_, layer, query.data_as<float>(), tree_key.data_as<float>(),
+        tree_value.data_as<float>(), optional_nodes(parents, "parents"),
+        optional_counts(node_counts), output.data<float>(), stream.native()));
+  }
+  /// The rows [layers, B, kv_heads, nodes, D] of the accepted nodes go to their
+  /// pages, and each sequence keeps its accepted tokens (path [B, nodes],
+  /// accepted [B] int32, on the device).  Synchronises the stream.
+  void commit_path(const Tensor& keys, const Tensor& values, const Tensor& path,
+                   const Tensor& accepted, const hip::Stream& stream) {
+    tree_rows(keys, "commit_path keys");
+    tree_rows(values, "commit_path values");
+    nodes_of(path, "path");
+    counts_of(accepted, "accepted");
+    detail::check(helix_decode_batch_commit_path(
+        batch_handle_, keys.data_as<float>(), values.data_as<float>(),
+        path.data_as<std::int32_t>(), accepted.data_as<std::int32_t>(), stream.native()));
+  }
+  /// Verifies the drafts (target [B, nodes, V] probabilities; draft the drafter's,
+  /// or nullptr where every draft was certain; tokens [B, nodes] int32, uniforms
+  /// [B, nodes], bonus_uniforms [B]), writes path, accepted and next_token [B], and
+  /// commits what it accepts.
+  void accept_tree(const Tensor& target, const Tensor* draft, const Tensor& tokens,
+                   const Tensor* parents, const Tensor* node_counts, const Tensor& uniforms,
+                   const Tensor& bonus_uniforms, const Tensor& keys, const Tensor& values,
+                   Tensor& path, Tensor& accepted, Tensor& next_token,
+                   const hip::Stream& stream) {
+    tree_rows(keys, "accept_tree keys");
+    tree_rows(values, "accept_tree values");
+    detail::require_float_on(target, device_, 3, "target");
+    const std::size_t vocab = detail::dim(target, 2);
+    for (const Tensor* t : {&target, draft}) {
+      if (t == nullptr) continue;
+      detail::require_float_on(*t, device_, 3, "draft");
+      detail::require(detail::dim(*t, 0) == batch_ && detail::dim(*t, 1) == step_tokens_ &&
+                          detail::dim(*t, 2) == vocab,
+                      ErrorCode::kInvalidArgument,
+                      "accept_tree: probabilities must be [batch, nodes, vocab]");
+    }
+    detail::require_float_on(uniforms, device_, 2, "uniforms");
+    detail::require_float_on(bonus_uniforms, device_, 1, "bonus uniforms");
+    detail::require(detail::dim(uniforms, 0) == batch_ && detail::dim(uniforms, 1) == step_tokens_ &&
+                        detail::dim(bonus_uniforms, 0) == batch_,
+                    ErrorCode::kInvalidArgument,
+                    "accept_tree: uniforms must be [batch, nodes] and [batch]");
+    nodes_of(tokens, "tokens");
+    nodes_of(path, "path");
+    counts_of(accepted, "accepted");
+    counts_of(next_token, "next_token");
+    const std::size_t row = step_tokens_ * vocab;
+    detail::check(helix_decode_batch_accept_tree(
+        batch_handle_, target.data_as<float>(), row, vocab,
+        draft == nullptr ? nullptr : draft->data_as<float>(), draft == nullptr ? 0 : row,
+        draft == nullptr ? 0 : vocab, vocab, tokens.data_as<std::int32_t>(),
+        optional_nodes(parents, "parents"), optional_counts(node_counts),
+        uniforms.data_as<float>(), bonus_uniforms.data_as<float>(), keys.data_as<float>(),
+        values.data_as<float>(), path.data<std::int32_t>(), accepted.data<std::int32_t>(),
+        next_token.data<std::int32_t>(), stream.native()));
+  }
   [[nodiscard]] std::size_t shared_pages() const {
     std::size_t n = 0;
     detail::check(helix_decode_batch_shared_pages(batch_handle_, &n));
@@ -1080,6 +1176,33 @@ class DecodeBatch final {
                         detail::dim(t, 2) == step_tokens_ && detail::dim(t, 3) == head_dim_,
                     ErrorCode::kInvalidArgument,
                     "DecodeBatch: chunk rows must be [batch, heads, tokens, head_dim]");
+  }
+
+  void tree_rows(const Tensor& t, const char* what) const {
+    detail::require_float_on(t, device_, 5, what);
+    detail::require(detail::dim(t, 0) == layers_ && detail::dim(t, 1) == batch_ &&
+                        detail::dim(t, 2) == kv_heads_ && detail::dim(t, 3) == step_tokens_ &&
+                        detail::dim(t, 4) == head_dim_,
+                    ErrorCode::kInvalidArgument,
+                    "DecodeBatch: tree rows must be [layers, batch, kv_heads, nodes, head_dim]");
+  }
+  void nodes_of(const Tensor& t, const char* what) const {
+    const std::size_t dims[] = {batch_, step_tokens_};
+    detail::require_int_on(t, device_, dims, what);
+  }
+  void counts_of(const Tensor& t, const char* what) const {
+    const std::size_t dims[] = {batch_};
+    detail::require_int_on(t, device_, dims, what);
+  }
+  const std::int32_t* optional_nodes(const Tensor* t, const char* what) const {
+    if (t == nullptr) return nullptr;
+    nodes_of(*t, what);
+    return t->data_as<std::int32_t>();
+  }
+  const std::int32_t* optional_counts(const Tensor* t) const {
+    if (t == nullptr) return nullptr;
+    counts_of(*t, "node counts");
+    return t->data_as<std::int32_t>();
   }
 
   helix_decode_batch* batch_handle_ = nullptr;
