@@ -554,6 +554,7 @@ def decode_workspace(batch, q_heads, kv_heads, max_blocks, pages_per_split=0, de
 
 
 _PAGE_DTYPES = {"f32": 0, "bf16": 1, "fp8": 2}
+_PAGE_WIDTHS = {"f32": 4, "bf16": 2, "fp8": 1}  # bytes of an element
 
 
 def paged_decode_attention(query, key_pool, value_pool, tables, lengths, tail_key, tail_value,
@@ -619,12 +620,17 @@ def append_chunk(keys, values, key_pool, value_pool, slots, stream=None):
 def _require_tensor(t, name, dtypes, shape, device=None, strided=False):
     """A device tensor of one of `dtypes` and of `shape` (None: any size),
     contiguous, or with `strided` contiguous in its last dimension."""
+    try:  # (most calls' arguments are right, and a small call is this long)
+        if (t.dtype in dtypes and t.shape == shape and t.is_contiguous() and
+                (device is None or t.device == device)):
+            return
+    except (AttributeError, TypeError):
+        pass
     import torch
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         names = " or ".join(str(d).replace("torch.", "") for d in dtypes)
         raise HelixError(INVALID_ARGUMENT, f"{name} must be a {names} tensor")
-    if t.shape != shape and (t.dim() != len(shape) or any(
-            n is not None and n != m for n, m in zip(shape, t.shape))):
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
         want = ", ".join("*" if n is None else str(n) for n in shape)
         raise HelixError(INVALID_ARGUMENT,
                          f"{name} must have shape [{want}], got {list(t.shape)}")
@@ -691,38 +697,40 @@ def paged_tree_attention(query, key_pool, value_pool, tables, lengths, tree_key,
         raise HelixError(INVALID_ARGUMENT, "query must have shape [batch, q_heads, nodes, dim]")
     b, hq, t, d = query.shape
     f32, i32 = (torch.float32,), (torch.int32,)
+    dev = query.device
     if pool_shape is None:
+        pool_shape = key_pool.shape
+        width = _PAGE_WIDTHS.get(page_dtype)
         for pool, name in ((key_pool, "key_pool"), (value_pool, "value_pool")):
-            width = {"f32": 4, "bf16": 2, "fp8": 1}.get(page_dtype)
             if width is not None and pool.element_size() != width:
                 raise HelixError(INVALID_ARGUMENT, f"{name} must hold {width}-byte elements")
-            _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), query.device)
-        pool_shape = tuple(key_pool.shape)
+            _require_tensor(pool, name, (pool.dtype,), pool_shape, dev)
         key_pool, value_pool = key_pool.data_ptr(), value_pool.data_ptr()
     if len(pool_shape) != 4:
         raise HelixError(INVALID_ARGUMENT, "pools must have shape [blocks, kv_heads, tokens, dim]")
     n, hkv, p, pd = pool_shape
     if pd != d:
         raise HelixError(INVALID_ARGUMENT, "query and pools must have the same head size")
-    dev = query.device
     _require_tensor(query, "query", f32, (b, hq, t, d))
     _require_tensor(output, "output", f32, (b, hq, t, d), dev)
     _require_tensor(tree_key, "tree_key", f32, (b, hkv, t, d), dev)
     _require_tensor(tree_value, "tree_value", f32, (b, hkv, t, d), dev)
-    _require_tensor(tables, "tables", (torch.int32, torch.uint32), (b, None), dev)
+    shape = getattr(tables, "shape", ())
+    width = shape[1] if len(shape) == 2 else None
+    _require_tensor(tables, "tables", (torch.int32, torch.uint32), (b, width), dev)
     _require_tensor(lengths, "lengths", i32, (b,), dev)
     if parents is not None:
         _require_tensor(parents, "parents", i32, (b, t), dev)
     if node_counts is not None:
         _require_tensor(node_counts, "node_counts", i32, (b,), dev)
-    _require_tensor(workspace, "workspace", (workspace.dtype,), (None,), dev)
+    _require_tensor(workspace, "workspace", (workspace.dtype,), (workspace.numel(),), dev)
     dtype = _PAGE_DTYPES.get(page_dtype, -1)
     with _on(dev):
         check(_lib().helix_paged_tree_attention(
             _address(query), b, hq, hkv, t, d, key_pool, value_pool,
-            n, p, _address(tables), tables.shape[1], _address(lengths), _address(tree_key),
+            n, p, _address(tables), width, _address(lengths), _address(tree_key),
             _address(tree_value), _address(parents), _address(node_counts), _address(output),
-            _address(workspace), workspace.numel() * workspace.element_size(), dtype, k_scale,
+            _address(workspace), workspace.nbytes, dtype, k_scale,
             v_scale, _device_stream(stream, dev)))
 
 
@@ -746,8 +754,9 @@ def _verify_arguments(target, draft, tokens, parents, uniforms, bonus_uniforms, 
     its sizes."""
     import torch
     f32, i32 = (torch.float32,), (torch.int32,)
-    _require_tensor(target, "target", f32, (None, None, None), strided=True)
-    b, t, v = target.shape
+    shape = getattr(target, "shape", ())
+    b, t, v = shape if len(shape) == 3 else (None, None, None)
+    _require_tensor(target, "target", f32, (b, t, v), strided=True)
     dev = target.device
     if draft is not None:
         _require_tensor(draft, "draft", f32, (b, t, v), dev, strided=True)
@@ -787,11 +796,11 @@ def verify_tree(target, draft, tokens, parents, uniforms, bonus_uniforms, path, 
                                          path, accepted, next_token, node_counts)
     b, t, v = target.shape
     dev = target.device
-    _require_tensor(workspace, "workspace", (workspace.dtype,), (None,), dev)
+    _require_tensor(workspace, "workspace", (workspace.dtype,), (workspace.numel(),), dev)
     with _on(dev):
         check(_lib().helix_verify_tree(
             *rows, b, t, v, *lists, *out, _address(workspace),
-            workspace.numel() * workspace.element_size(), _device_stream(stream, dev)))
+            workspace.nbytes, _device_stream(stream, dev)))
 
 
 def append_path(keys, values, key_pool, value_pool, slots, path, accepted, stream=None,
@@ -809,27 +818,28 @@ def append_path(keys, values, key_pool, value_pool, slots, path, accepted, strea
     layers = key_pool.shape[0] if layered else 1
     n, hkv, p, d = key_pool.shape[-4:]
     lead = (layers,) if layered else ()
-    _require_tensor(slots, "slots", (torch.int64,), (None, None), dev)
-    b, t = slots.shape
+    shape = getattr(slots, "shape", ())
+    b, t = shape if len(shape) == 2 else (None, None)
+    _require_tensor(slots, "slots", (torch.int64,), (b, t), dev)
     _require_tensor(keys, "keys", (torch.float32,), (*lead, b, hkv, t, d))
     _require_tensor(values, "values", (torch.float32,), (*lead, b, hkv, t, d), dev)
     _require_tensor(path, "path", (torch.int32,), (b, t), dev)
     _require_tensor(accepted, "accepted", (torch.int32,), (b,), dev)
-    width = {"f32": 4, "bf16": 2, "fp8": 1}.get(page_dtype)
+    width = _PAGE_WIDTHS.get(page_dtype)
     stride = 0
     for pool, name in ((key_pool, "key_pool"), (value_pool, "value_pool")):
         if width is not None and pool.element_size() != width:
             raise HelixError(INVALID_ARGUMENT, f"{name} must hold {width}-byte elements")
         if layered:
-            _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), dev, strided=True)
-            if layers:
-                _require_tensor(pool[0], name, (pool.dtype,), tuple(key_pool.shape[1:]), dev)
+            _require_tensor(pool, name, (pool.dtype,), key_pool.shape, dev, strided=True)
+            if layers and not pool.is_contiguous():  # a layer's pool is, if not all of them
+                _require_tensor(pool[0], name, (pool.dtype,), key_pool.shape[1:], dev)
             if layers > 1:
                 if pool.stride(0) != key_pool.stride(0):
                     raise HelixError(INVALID_ARGUMENT, "pools must have the same layer stride")
                 stride = pool.stride(0)
         else:
-            _require_tensor(pool, name, (pool.dtype,), tuple(key_pool.shape), dev)
+            _require_tensor(pool, name, (pool.dtype,), key_pool.shape, dev)
     with _on(dev):
         check(_lib().helix_paged_append_path(
             _address(keys), _address(values), _address(key_pool), _address(value_pool), layers,

@@ -413,8 +413,10 @@ struct VerifyShape {
     // without a drafter's rows.  Of others, 64 trees of 16 nodes at a vocabulary
     // of 128256 take 41 us with three such launches and 44 with four where three
     // are enough, 64 and 50 where they are not: one that finds nothing to do
-    // takes 2.5 us, a sum left to verify_finish_kernel 15.
-    passes = many ? std::min<std::size_t>(std::max<std::size_t>(nodes - 1, 1), 4) : 1;
+    // takes 2.5 us, a sum left to verify_finish_kernel 15, or less by the
+    // vocabulary (one tree of 6 at 32000: 21 us with one launch, 28 with four).
+    passes = 1;
+    if (many) passes = std::clamp<std::size_t>(std::min(nodes - 1, (vocab + 16384) / 32768), 1, 4);
   }
   std::size_t walk_bytes(std::size_t batch) const { return passes * batch * sizeof(Walk); }
   std::size_t bytes(std::size_t batch) const {

@@ -376,6 +376,22 @@ def test_verification_equals_the_plain_form(device, certain, b, t, v):
 
 
 @pytest.mark.parametrize("certain", [False, True])
+@pytest.mark.parametrize("v", [20011, 49153, 90001, 131072])
+def test_verification_of_many_rejections(device, certain, v):
+    """All nodes are the root's children, hard to accept: a sum over the vocabulary
+    for each, some of the sequences' first children accepted."""
+    rng = np.random.default_rng(v)
+    b, t = 3, 12
+    parents = np.zeros((b, t), np.int32)
+    parents[:, 0] = -1
+    target, draft, tokens = drafts(rng, b, t, v, parents, certain)
+    u = np.full((b, t), 0.9999, np.float32)
+    u[1, 1] = 0.0
+    accepted = Check(target, draft, tokens, parents, u, rng.random(b, np.float32)).run()
+    assert accepted[1] == 2
+
+
+@pytest.mark.parametrize("certain", [False, True])
 def test_verification_at_its_edges(device, certain):
     """Siblings with one token, tokens and parents out of range, ragged counts,
     a bonus number of 0 and just below 1, rows with zeros, a target equal to
