@@ -243,7 +243,7 @@ __device__ __forceinline__ int lane_blocks(const TreeKernelArgs& a, int b) {
 }
 
 // Inclusive sums over the wavefront.
-__device__ __forceinline__ long long lane_scan(int v, int lane) {
+__device__ __forceinline__ long long lane_scan(long long v, int lane) {
   long long sum = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -260,10 +260,9 @@ struct TreeRange {
 __device__ __forceinline__ TreeRange first_place(const TreeKernelArgs& a, const TreeStream& st,
                                                  int group, int lane, TreeCursor& c) {
   long long per_head = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    per_head += uniform_long(__shfl(lane_scan(lane_blocks(a, b0 + lane), lane), 63, 64));
-  }
-  per_head *= st.row_blocks;
+#pragma unroll 4
+  for (int b0 = 0; b0 < a.batch; b0 += 64) per_head += lane_blocks(a, b0 + lane);
+  per_head = uniform_long(__shfl(lane_scan(per_head, lane), 63, 64)) * st.row_blocks;
   const long long total = per_head * a.kv_heads;
   TreeRange r{};
   // (Ranges of one block where there are few: 121 tokens and 5 nodes take 14 us
@@ -275,8 +274,9 @@ __device__ __forceinline__ TreeRange first_place(const TreeKernelArgs& a, const 
   c.kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(r.g0 / per_head));
   const long long rem = r.g0 - c.kvh * per_head;
   long long base = 0;
+  int nb = lane_blocks(a, lane);
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int nb = lane_blocks(a, b0 + lane);
+    const int next = lane_blocks(a, b0 + 64 + lane);
     const long long sum = lane_scan(nb, lane);
     const long long from = (base + sum - nb) * st.row_blocks, to = (base + sum) * st.row_blocks;
     const unsigned long long hit = __ballot(from <= rem && rem < to);
@@ -290,6 +290,7 @@ __device__ __forceinline__ TreeRange first_place(const TreeKernelArgs& a, const 
       break;
     }
     base += uniform_long(__shfl(sum, 63, 64));
+    nb = next;
   }
   return r;
 }
