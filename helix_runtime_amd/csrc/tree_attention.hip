@@ -195,7 +195,8 @@ constexpr int stage_buffers(int pf, int waves, int tiles) {
 }
 
 // Items on their way from memory to registers.  (64 bf16 sequences of 16 nodes:
-// 178 us with two, 190 with one.  fp32 pages gain nothing, and fp8 pages more from
+// 178 us with two, 190 with one; 32 of them 112 with two, 118 with three.  fp32
+// pages gain nothing, and fp8 pages more from
 // the registers of a third workgroup on the CU.)
 constexpr int load_depth(int pf, int tiles) { return pf == 1 && tiles == 1 ? 2 : 1; }
 
