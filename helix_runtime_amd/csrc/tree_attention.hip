@@ -41,11 +41,11 @@
 // computes that part of it again with exact_row.
 //
 // Measured: 64 sequences of 512 to 8192 tokens, 32/8 heads, trees of 16 nodes: fp32
-// pages 367 us and bf16 pages 180 us, both at 4.2 TB/s of pages; loads and LDS
+// pages 356 us and bf16 pages 180 us, both at 4.2 TB/s of pages; loads and LDS
 // writes alone take 330 and 165, products alone 306 and 150.  Trees of 64 nodes,
-// fp8 pages: 466 us (860 TFLOP/s of fp16 products), vector work (16 exponentials
+// fp8 pages: 448 us (900 TFLOP/s of fp16 products), vector work (16 exponentials
 // and as many splits a lane and block) beside the matrix instructions.  One
-// sequence of 131071, 33 nodes, bf16: 309 us.
+// sequence of 131071, 33 nodes, bf16: 297 us.
 #include "prefill_bmma.hpp"
 #include "tree_exact.hpp"
 
@@ -196,8 +196,8 @@ constexpr int stage_buffers(int pf, int waves, int tiles) {
 
 // Items on their way from memory to registers.  (64 bf16 sequences of 16 nodes:
 // 178 us with two, 190 with one; 32 of them 112 with two, 118 with three.  fp32
-// pages gain nothing, and fp8 pages more from
-// the registers of a third workgroup on the CU.)
+// pages gain nothing, and fp8 pages more from the registers of a third workgroup
+// on the CU.)
 constexpr int load_depth(int pf, int tiles) { return pf == 1 && tiles == 1 ? 2 : 1; }
 
 template <int PF, int W, int RT>
