@@ -84,6 +84,10 @@ const std::vector<std::uint32_t>& BlockManager::blocks(std::uint64_t sequence) c
   return require(sequence, "block_table").blocks;
 }
 
+std::uint64_t BlockManager::truncations(std::uint64_t sequence) const {
+  return require(sequence, "truncations").truncations;
+}
+
 std::size_t BlockManager::block_reference_count(std::uint32_t block) const {
   check(block < refs_.size(), Status::kOutOfRange, "block ID is out of range");
   return refs_[block];
@@ -288,6 +292,7 @@ void BlockManager::require_truncatable(std::uint64_t sequence, std::size_t lengt
 void BlockManager::truncate(std::uint64_t sequence, std::size_t length) {
   require_truncatable(sequence, length);
   Sequence& s = sequences_.find(sequence)->second;
+  if (length < s.length) ++s.truncations;
   const std::size_t keep = blocks_for(length, config_.block_tokens);
   if (keep != 0) {
     std::size_t& tokens = tokens_[s.blocks[keep - 1]];

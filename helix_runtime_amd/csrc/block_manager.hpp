@@ -109,6 +109,9 @@ public:
   void truncate(std::uint64_t sequence, std::size_t length);
   // Throws what truncate() would.
   void require_truncatable(std::uint64_t sequence, std::size_t length) const;
+  // How often a live sequence lost tokens so far: equal counts mean that every
+  // token of the earlier time is still in its slot.
+  [[nodiscard]] std::uint64_t truncations(std::uint64_t sequence) const;
 
   // Free blocks the FIFO can still hand out.
   [[nodiscard]] std::size_t free_block_count() const noexcept { return free_count_; }
@@ -126,6 +129,7 @@ private:
   struct Sequence {
     std::size_t length = 0;
     std::vector<std::uint32_t> blocks;
+    std::uint64_t truncations = 0;
   };
 
   [[nodiscard]] const Sequence& require(std::uint64_t id, const char* op) const;

@@ -255,7 +255,6 @@ void DevicePagedCache::truncate(std::uint64_t sequence, std::uint64_t cache_id,
   std::scoped_lock lock(state_->mutex);
   state_->require_sequence(sequence, cache_id, "truncate_sequence");
   state_->manager.truncate(sequence, length);
-  ++state_->truncations;
   state_->releases.fetch_add(1, std::memory_order_release);
 }
 
@@ -407,7 +406,11 @@ DecodeBatch::DecodeBatch(std::shared_ptr<CacheState> state, const std::uint64_t*
   hip_check(hipMemcpy(tables_.data(), host.data(), tables_.size(), hipMemcpyHostToDevice),
             "decode batch table upload");
   mirrored_.resize(batch);
-  for (std::size_t i = 0; i < batch; ++i) mirrored_[i] = s.manager.blocks(sequences[i]).size();
+  truncations_.resize(batch);
+  for (std::size_t i = 0; i < batch; ++i) {
+    mirrored_[i] = s.manager.blocks(sequences[i]).size();
+    truncations_[i] = s.manager.truncations(sequences[i]);
+  }
   mirror_ = std::move(host);
   workspace_ = DeviceBuffer(
       hip::decode_workspace_bytes(batch, q_heads, c.kv_heads, max_blocks_, pages_per_split_),
@@ -495,18 +498,16 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
   step_tokens_ = 0;
   const PagedConfig& c = s.manager.config();
   const std::size_t B = batch();
-  if (seen_truncations_ != s.truncations) {
-    // A member's row may have shrunk and grown again: the entries that still
-    // hold count as mirrored, the others are uploaded with this step.
-    for (std::size_t i = 0; i < B; ++i) {
-      if (!s.manager.contains(sequences_[i])) continue;
-      const std::vector<std::uint32_t>& row = s.manager.blocks(sequences_[i]);
-      const std::size_t most = std::min(mirrored_[i], row.size());
-      std::size_t k = 0;
-      while (k < most && mirror_[i * max_blocks_ + k] == row[k]) ++k;
-      mirrored_[i] = k;
-    }
-    seen_truncations_ = s.truncations;
+  for (std::size_t i = 0; i < B; ++i) {
+    if (!s.manager.contains(sequences_[i]) || uncut(i)) continue;
+    // The row may have shrunk and grown again: the entries that still hold
+    // count as mirrored, the others are uploaded with this step.
+    const std::vector<std::uint32_t>& row = s.manager.blocks(sequences_[i]);
+    const std::size_t most = std::min(mirrored_[i], row.size());
+    std::size_t k = 0;
+    while (k < most && mirror_[i * max_blocks_ + k] == row[k]) ++k;
+    mirrored_[i] = k;
+    truncations_[i] = s.manager.truncations(sequences_[i]);
   }
   check(tokens != 0, Status::kInvalidArgument, "decode batch prepare needs at least one token");
   check(tokens <= max_blocks_ * c.block_tokens, Status::kOutOfRange,
@@ -517,7 +518,7 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
           "decode batch sequence was released");
     const std::size_t len = s.manager.length(sequences_[i]);
     check(s.manager.blocks(sequences_[i]).size() >= mirrored_[i], Status::kInternal,
-          "decode batch table row shrank while the sequence lived");
+          "decode batch table row shrank while the sequence was not cut");
     check(len + tokens <= max_blocks_ * c.block_tokens, Status::kOutOfRange,
           "decode batch sequence reached the batch's max_tokens");
     new_blocks += (len + tokens + c.block_tokens - 1) / c.block_tokens -
@@ -642,17 +643,16 @@ void DecodeBatch::begin_call(hipStream_t stream, const char* op) const {
   check(prepared_, Status::kInvalidArgument, std::string(op) + " before prepare");
   CacheState& s = *state_;
   if (s.releases.load(std::memory_order_acquire) != prepared_releases_) {
-    // Something was released since prepare(): the step is only valid if
-    // every member still lives (their pages are the step's).
+    // Something was released or cut since prepare(): the step is only valid
+    // if every member still lives and lost no token (their pages are the
+    // step's).
     std::scoped_lock lock(s.mutex);
     for (std::uint64_t seq : sequences_) {
       check(s.manager.contains(seq), Status::kInvalidArgument,
             std::string(op) + ": a sequence of the batch was released after prepare");
     }
     for (std::size_t i = 0; i < batch(); ++i) {
-      check(s.manager.length(sequences_[i]) >=
-                static_cast<std::size_t>(host_lengths_[i]) + step_tokens_,
-            Status::kInvalidArgument,
+      check(uncut(i), Status::kInvalidArgument,
             std::string(op) + ": a sequence of the batch was truncated after prepare");
     }
     prepared_releases_ = s.releases.load(std::memory_order_acquire);
@@ -805,29 +805,38 @@ void DecodeBatch::prefill_layer(std::size_t layer, const float* query, const flo
   hip_check(hip::launch_prefill(a, stream), "decode batch prefill launch");
 }
 
+bool DecodeBatch::uncut(std::size_t i) const {
+  const BlockManager& m = state_->manager;
+  return m.contains(sequences_[i]) && m.truncations(sequences_[i]) == truncations_[i];
+}
+
+bool DecodeBatch::holds_step(std::size_t i) const {
+  return uncut(i) && state_->manager.length(sequences_[i]) ==
+                         static_cast<std::size_t>(host_lengths_[i]) + step_tokens_;
+}
+
+void DecodeBatch::cut(std::size_t i, std::size_t length) {
+  BlockManager& m = state_->manager;
+  m.truncate(sequences_[i], length);
+  mirrored_[i] = std::min(mirrored_[i], m.blocks(sequences_[i]).size());
+  truncations_[i] = m.truncations(sequences_[i]);
+}
+
 // Takes the slots of an uncommitted tree step back (under the cache mutex).
 // The step's calls read the pages before them only.
 void DecodeBatch::drop_tree() {
   if (!tree_step_) return;
   CacheState& s = *state_;
   // (A member that someone released, truncated or appended to is theirs.)
-  const auto reserved = [&](std::size_t i) {
-    return s.manager.contains(sequences_[i]) &&
-           s.manager.length(sequences_[i]) ==
-               static_cast<std::size_t>(host_lengths_[i]) + step_tokens_;
-  };
   for (std::size_t i = 0; i < batch(); ++i) {
-    if (reserved(i)) {
+    if (holds_step(i)) {
       s.manager.require_truncatable(sequences_[i], static_cast<std::size_t>(host_lengths_[i]));
     }
   }
   for (std::size_t i = 0; i < batch(); ++i) {
-    if (reserved(i)) {
-      s.manager.truncate(sequences_[i], static_cast<std::size_t>(host_lengths_[i]));
-    }
+    if (holds_step(i)) cut(i, static_cast<std::size_t>(host_lengths_[i]));
   }
   tree_step_ = false;
-  ++s.truncations;
   s.releases.fetch_add(1, std::memory_order_release);
 }
 
@@ -888,6 +897,12 @@ void DecodeBatch::tree_layer(std::size_t layer, const float* query, const float*
 void DecodeBatch::append_path(const float* keys, const float* values, const std::int32_t* path,
                               const std::int32_t* accepted, hipStream_t stream) {
   const PagedConfig& c = state_->manager.config();
+  CacheState& s = *state_;
+  std::scoped_lock lock(s.mutex);
+  for (std::size_t i = 0; i < batch(); ++i) {
+    check(holds_step(i), Status::kInvalidArgument,
+          "decode batch commit_path: a sequence changed after prepare_tree");
+  }
   hip_check(hip::launch_append_path(keys, values, state_->key_pool(0), state_->value_pool(0),
                                     geometry(c), slots(), path, accepted, batch(), step_tokens_,
                                     stream, state_->page_type, c.layers, state_->layer_stride()),
@@ -895,25 +910,17 @@ void DecodeBatch::append_path(const float* keys, const float* values, const std:
   hip_check(hipMemcpyAsync(accepted_.data(), accepted, batch() * sizeof(std::int32_t),
                            hipMemcpyDeviceToHost, stream),
             "decode batch accepted download");
-  CacheState& s = *state_;
-  std::scoped_lock lock(s.mutex);
   synchronize_or_poison(s, stream, "decode batch commit_path");
   const auto* number = static_cast<const std::int32_t*>(accepted_.data());
   for (std::size_t i = 0; i < batch(); ++i) {
     check(number[i] >= 0 && static_cast<std::size_t>(number[i]) <= step_tokens_,
           Status::kInvalidArgument, "decode batch commit_path: accepted counts lie in [0, nodes]");
-    check(s.manager.contains(sequences_[i]) &&
-              s.manager.length(sequences_[i]) ==
-                  static_cast<std::size_t>(host_lengths_[i]) + step_tokens_,
-          Status::kInvalidArgument,
-          "decode batch commit_path: a sequence changed after prepare_tree");
     s.manager.require_truncatable(sequences_[i],
                                   static_cast<std::size_t>(host_lengths_[i] + number[i]));
   }
   for (std::size_t i = 0; i < batch(); ++i) {
-    s.manager.truncate(sequences_[i], static_cast<std::size_t>(host_lengths_[i] + number[i]));
+    cut(i, static_cast<std::size_t>(host_lengths_[i] + number[i]));
   }
-  ++s.truncations;
   s.releases.fetch_add(1, std::memory_order_release);
   tree_step_ = false;
   prepared_ = false;

@@ -80,13 +80,10 @@ struct CacheState {
   std::size_t layer_elements = 0;  // physical_blocks * kv_heads * block_tokens * head_dim
   std::mutex mutex;
   bool poisoned = false;
-  // Releases through the cache so far: a DecodeBatch compares it with the
-  // value at its last prepare() to notice that a member may have been
-  // released between the step's calls.
+  // Releases and truncations through the cache so far: a DecodeBatch compares
+  // it with the value at its last prepare() to notice that a member may have
+  // been released or cut between the step's calls.
   std::atomic<std::uint64_t> releases{0};
-  // Truncations so far, for the same purpose (counted among `releases` too):
-  // the rows of a truncated member's table may have shrunk.
-  std::uint64_t truncations = 0;
   DeviceBuffer staging;            // transient upload area (grown on demand)
 
   // Layer pools: fp32 elements, or bf16 / fp8 bits for a reduced-precision
@@ -178,7 +175,7 @@ private:
 //    does not hold yet;
 //  - a member released after prepare() makes every later per-step call fail
 //    (kInvalidArgument) until the next prepare(), which fails too; so does one
-//    truncated below the step, until the next prepare();
+//    that lost tokens, however long it is by then, until the next prepare();
 //  - a per-step call on a stream other than prepare()'s waits for the step
 //    upload, and prepare() on a stream other than the previous step's last
 //    call waits for that call.  Per-step calls of one step on different
@@ -285,10 +282,12 @@ private:
   static constexpr std::size_t kMinCascadePages = 4;
 
   // Host mirror of the device tables and the entries of each row that the
-  // device copy holds (table rows only grow while a sequence lives).
+  // device copy holds (table rows only grow while a sequence is not cut).
   std::vector<std::uint32_t> mirror_;
   std::vector<std::size_t> mirrored_;
-  std::uint64_t seen_truncations_ = 0;
+  // Each member's truncations at the last prepare, or the batch's own since:
+  // where the manager counts more, someone else cut it.
+  std::vector<std::uint64_t> truncations_;
   // A tree step was prepared and is neither committed nor dropped.
   bool tree_step_ = false;
   DeviceBuffer tree_workspace_;
@@ -302,6 +301,12 @@ private:
   hipEvent_t order_event_ = nullptr;
 
   void reserve_step(std::size_t tokens);
+  // Under the cache mutex: whether member i lives and lost no token since the
+  // last prepare, whether it also ends with the step's slots, and its
+  // truncation by the batch itself.
+  [[nodiscard]] bool uncut(std::size_t i) const;
+  [[nodiscard]] bool holds_step(std::size_t i) const;
+  void cut(std::size_t i, std::size_t length);
   void drop_tree();
   void require_tree_step(const char* op) const;
   void append_path(const float* keys, const float* values, const std::int32_t* path,

@@ -177,7 +177,9 @@ int helix_paged_cache_append_layer_major(helix_paged_cache* cache, helix_sequenc
 /* CudaPagedKvCache::release_sequence (cuda_paged.cpp:613-643). */
 int helix_paged_cache_release_sequence(helix_paged_cache* cache, helix_sequence sequence);
 /* helix_block_manager_truncate of a cache's sequence (extension): metadata
- * only, as release_sequence is. */
+ * only, as release_sequence is.  A decode batch whose prepared step has the
+ * sequence as a member fails that step's later calls, also where the sequence
+ * has grown again by then. */
 int helix_paged_cache_truncate_sequence(helix_paged_cache* cache, helix_sequence sequence,
                                         size_t length);
 /* PagedKvCache::copy_layer_out (paged.cpp:887-893): device outputs

@@ -740,3 +740,94 @@ def test_tree_layers_on_other_streams_and_captured(device):
         graph.replay()
         torch.cuda.synchronize()
         close(host(out), want)
+
+
+def refused(call, status=hx.INVALID_ARGUMENT):
+    with pytest.raises(hx.HelixError) as e:
+        call()
+    assert e.value.status == status
+
+
+def cut_and_grow(s, b, keep, more):
+    """Truncates member b to `keep` tokens and appends `more` others."""
+    k, v = s.normal(s.layers, s.hkv, more, D), s.normal(s.layers, s.hkv, more, D)
+    s.cache.truncate_sequence(s.seqs[b], keep)
+    s.cache.append_layer_major(s.seqs[b], [dev(x) for x in k], [dev(x) for x in v])
+    s.k[b] = np.concatenate([s.k[b][:, :, :keep], on_pages(s.dtype, k, KS)], 2)
+    s.v[b] = np.concatenate([s.v[b][:, :, :keep], on_pages(s.dtype, v, VS)], 2)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "fp8"])
+@pytest.mark.parametrize("keep", [0, 16, 18])
+def test_a_member_cut_after_prepare_ends_an_ordinary_step(device, dtype, keep):
+    """Also where it has grown back to the step's length by then: its tokens, on
+    other pages or on the step's, are not the step's to write."""
+    s = Server(dtype, [20, 33, 16], spare=8)
+    b, B, L = s.batch, s.B, s.layers
+    rows, all_rows = torch.ones(B, s.hkv, D, device="cuda:0"), torch.ones(L, B, s.hkv, 1, D,
+                                                                         device="cuda:0")
+    q = torch.ones(B, s.hq, D, device="cuda:0")
+    b.prepare()
+    cut_and_grow(s, 0, keep, 21 - keep)
+    other = s.cache.create_sequence()  # takes pages that the cut freed
+    filler = [torch.full((s.hkv, 30, D), 5.0, device="cuda:0")] * L
+    s.cache.append_layer_major(other, filler, filler)
+    assert s.cache.length(s.seqs[0]) == 21
+    before = [host(s.cache.retrieve_layer(other, 1)[i]) for i in (0, 1)]
+    refused(lambda: b.append_layer(0, rows, rows))
+    refused(lambda: b.append_all_layers(all_rows, all_rows))
+    refused(lambda: b.attention_layer(0, q, rows, rows, torch.empty_like(q)))
+    refused(lambda: b.append_attention_layer(0, q, rows, rows, torch.empty_like(q)))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        np.testing.assert_array_equal(host(s.cache.retrieve_layer(other, 1)[i]), before[i])
+    s.cache.release_sequence(other)
+    for i in (1, 2):  # (the refused step's slots)
+        s.cache.truncate_sequence(s.seqs[i], s.k[i].shape[2])
+    s.compare()
+    s.decode_step()
+    s.tree_step(5)
+    s.decode_step()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("keep", [0, 17, 20])
+def test_a_member_cut_and_grown_after_prepare_tree_keeps_its_tokens(device, dtype, keep):
+    """The step is refused, and the next prepare takes back the other members'
+    reserved slots only."""
+    s = Server(dtype, [20, 33, 16])
+    b, B, t = s.batch, s.B, 4
+    z = lambda *n, **kw: torch.zeros(*n, device="cuda:0", **kw)  # noqa: E731
+    keys, q, rows = z(s.layers, B, s.hkv, t, D), z(B, s.hq, t, D), z(B, s.hkv, t, D)
+    path, one = z(B, t, dtype=torch.int32), torch.ones(B, dtype=torch.int32, device="cuda:0")
+    for _ in range(2):
+        lengths = [s.k[i].shape[2] for i in range(B)]
+        b.prepare_tree(t)
+        cut_and_grow(s, 0, keep, lengths[0] + t - keep)
+        assert s.cache.length(s.seqs[0]) == lengths[0] + t
+        refused(lambda: b.tree_layer(0, q, rows, rows, None, torch.empty_like(q)))
+        refused(lambda: b.commit_path(keys, keys, path, one))
+        assert [s.cache.length(x) for x in s.seqs] == [n + t for n in lengths]
+        s.decode_step()  # (compares every row)
+        s.tree_step(6)
+
+
+def test_two_batches_over_one_sequence_see_each_others_cuts(device):
+    """A step that another batch's commit cuts into is refused; a cut of no tokens
+    is none."""
+    s = Server("f32", [20, 33], spare=20)
+    other = hx.DecodeBatch(s.cache, s.seqs[:1], s.hq, 512)
+    rows = torch.ones(1, s.hkv, D, device="cuda:0")
+    z = lambda *n, **kw: torch.zeros(*n, device="cuda:0", **kw)  # noqa: E731
+    s.batch.prepare_tree(4)
+    other.prepare()  # behind the tree's slots
+    refused(lambda: s.batch.commit_path(z(2, 2, 2, 4, D), z(2, 2, 2, 4, D),
+                                        z(2, 4, dtype=torch.int32), z(2, dtype=torch.int32)))
+    s.cache.truncate_sequence(s.seqs[0], 25)
+    other.append_layer(0, rows, rows)
+    s.cache.truncate_sequence(s.seqs[0], 24)
+    refused(lambda: other.append_layer(0, rows, rows))
+    s.cache.truncate_sequence(s.seqs[0], 20)
+    s.decode_step()
+    refused(lambda: other.append_layer(0, rows, rows))
+    s.tree_step(3)
