@@ -1126,6 +1126,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeKernelArgs a, TreeS
     // The marked parts of the wavefront's four rows, a row after another; lane
     // i of 64 holds dims 2 i, 2 i + 1 there and hands them over.
     const TreeSequence s = tree_sequence(a, job.b, lane);
+    const unsigned long long broken = __ballot(s.broken != 0);
     const int nbh = (s.hist + kBlock - 1) / kBlock;
     auto tokens = [&](long long blocks) {
       return static_cast<int>(min(static_cast<long long>(s.hist), blocks * kBlock));
@@ -1139,6 +1140,11 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeKernelArgs a, TreeS
       const int one = static_cast<int>(blockIdx.y) * kMergeRows + wave * 4 + r;
       const int one_row = job.rb * rb_rows + one;
       if (one >= rb_rows || one_row >= a.rows || one_row % a.nodes >= s.count) continue;
+      if (((broken >> (one_row % a.nodes)) & 1) != 0) {
+        // (Its NaN may stand in a part that is marked for the tile's other rows.)
+        if (lane >> 4 == r) sum = NAN;
+        continue;
+      }
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
         if (st.part_marks[slot(i) * kMaxTiles + one / 16] == 0) continue;

@@ -831,3 +831,22 @@ def test_two_batches_over_one_sequence_see_each_others_cuts(device):
     s.decode_step()
     refused(lambda: other.append_layer(0, rows, rows))
     s.tree_step(3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hists", [[0, 7], [3001, 40], [20011]])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_wrong_parent_beside_values_that_are_no_numbers(device, dtype, hists, bad):
+    """A tile of rows that a value of an unseen node makes NaN is computed again;
+    its rows with a wrong parent on their way stay NaN, in units of one range and
+    in joined ones, and the others come out as they are."""
+    nodes = 12
+    parents = np.array([[-1, 0, 0, 1, 2, 9, 4, 0, 7, 5, 2, 10]] * len(hists), np.int32)
+    p = Problem(dtype, hists, 8, 2, nodes, 17, parents=parents)
+    p.tv[:, :, 4, 77] = bad  # seen by nodes 4 and 6 alone
+    got, want = p.run(), p.want()
+    lost, seen = [5, 9], [4, 6]
+    rest = [t for t in range(nodes) if t not in lost + seen]
+    assert np.isnan(want[:, :, lost]).all() and np.isfinite(want[:, :, rest]).all()
+    assert np.isnan(got[:, :, lost]).all()
+    close(got, want)
