@@ -422,7 +422,7 @@ DecodeBatch::DecodeBatch(std::shared_ptr<CacheState> state, const std::uint64_t*
     hip_check(hipEventCreateWithFlags(&uploaded_[i], hipEventDisableTiming), "hipEventCreate");
   }
   hip_check(hipEventCreateWithFlags(&order_event_, hipEventDisableTiming), "hipEventCreate");
-  reserve_step(1);
+  reserve_step(kFixedTokens);
 }
 
 DecodeBatch::~DecodeBatch() {
@@ -450,19 +450,21 @@ const std::uint32_t* DecodeBatch::tables() const {
   return static_cast<const std::uint32_t*>(tables_.data());
 }
 const std::int32_t* DecodeBatch::lengths() const {
-  return static_cast<const std::int32_t*>(step_.data());
+  return reinterpret_cast<const std::int32_t*>(step_data());
 }
 const std::int64_t* DecodeBatch::slots() const {
-  return reinterpret_cast<const std::int64_t*>(static_cast<const unsigned char*>(step_.data()) +
+  return reinterpret_cast<const std::int64_t*>(step_data() +
                                                align8(batch() * sizeof(std::int32_t)));
 }
 
 // Step buffers for `tokens` slots per sequence: lengths [B] int32, slots
 // [B, tokens] int64, up to B * max_blocks table updates of 3 words (a step
 // uploads the entries a member gained since the previous step, inside or
-// outside the batch), and for chunks the prefill work-item order, in one
-// device buffer and two pinned staging copies; after them, device only, one
-// redo word per prefill work item (written by the bf16 / fp8 prefill).
+// outside the batch), and for chunks the prefill work-item order, in a device
+// buffer and two pinned staging copies; after them, device only, one redo word
+// per prefill work item (written by the bf16 / fp8 prefill).  The buffer of
+// steps of up to kFixedTokens tokens is made once, with the batch: a captured
+// layer of such a step holds its address, and is valid for every later one.
 std::size_t DecodeBatch::order_offset(std::size_t tokens) const {
   const std::size_t B = batch();
   const std::size_t max_updates = B * max_blocks_;
@@ -483,9 +485,8 @@ void DecodeBatch::reserve_step(std::size_t tokens) {
   DeviceGuard guard(state_->device);
   // The device buffer may still be read by queued kernels of earlier steps.
   hip_check(hipDeviceSynchronize(), "decode batch step resize");
-  step_ = DeviceBuffer(bytes, state_->device);
+  (tokens <= kFixedTokens ? step_ : long_step_) = DeviceBuffer(bytes, state_->device);
   for (auto& pinned : pinned_) pinned = PinnedBuffer(bytes);
-  step_bytes_ = bytes;
   step_capacity_ = tokens;
 }
 
@@ -526,7 +527,8 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
   }
   check(new_blocks <= s.manager.free_block_count(), Status::kResourceExhausted,
         "decode batch prepare: the pool has too few free blocks for the step");
-  reserve_step(tokens);
+  reserve_step(std::max(tokens, kFixedTokens));
+  step_buffer_ = tokens <= kFixedTokens ? &step_ : &long_step_;
   DeviceGuard guard(s.device);
   if (any_call_ && last_stream_ != stream) {
     // The previous step's last call may still read the step buffers and
@@ -590,12 +592,11 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
                      [](const auto& x, const auto& y) { return x.first > y.first; });
     auto* order = reinterpret_cast<std::uint32_t*>(host + order_offset(tokens));
     for (std::size_t n = 0; n < items.size(); ++n) order[n] = items[n].second;
-    hip_check(hipMemcpyAsync(static_cast<unsigned char*>(step_.data()) + order_offset(tokens),
-                             order, items.size() * sizeof(std::uint32_t), hipMemcpyHostToDevice,
+    hip_check(hipMemcpyAsync(step_data() + order_offset(tokens), order, items.size() * sizeof(std::uint32_t), hipMemcpyHostToDevice,
                              stream),
               "decode batch order upload");
   }
-  hip_check(hipMemcpyAsync(step_.data(), host, used, hipMemcpyHostToDevice, stream),
+  hip_check(hipMemcpyAsync(step_data(), host, used, hipMemcpyHostToDevice, stream),
             "decode batch step upload");
   items_ = hip::decode_items(host_lengths_.data(), B, c.kv_heads, max_blocks_, pages_per_split_);
   // The updates follow the slots in the device copy of the step buffer.
@@ -794,12 +795,10 @@ void DecodeBatch::prefill_layer(std::size_t layer, const float* query, const flo
   a.physical_blocks = c.physical_blocks;
   a.page_type = state_->page_type;
   if (step_tokens_ > 1) {
-    a.order = reinterpret_cast<const std::uint32_t*>(
-        static_cast<const unsigned char*>(step_.data()) + order_offset(step_tokens_));
+    a.order = reinterpret_cast<const std::uint32_t*>(step_data() + order_offset(step_tokens_));
   }
   a.redo = reinterpret_cast<std::uint32_t*>(
-      static_cast<unsigned char*>(step_.data()) + order_offset(step_tokens_) +
-      prefill_items(step_tokens_) * sizeof(std::uint32_t));
+      step_data() + order_offset(step_tokens_) + prefill_items(step_tokens_) * sizeof(std::uint32_t));
   DeviceGuard guard(state_->device);
   begin_call(stream, "decode batch prefill");
   hip_check(hip::launch_prefill(a, stream), "decode batch prefill launch");
@@ -844,13 +843,15 @@ void DecodeBatch::prepare_tree(hipStream_t stream, std::size_t nodes) {
   check(nodes != 0 && nodes <= hip::kMaxTreeNodes, Status::kInvalidArgument,
         "decode batch prepare_tree: trees of 1 to 64 nodes");
   const PagedConfig& c = state_->manager.config();
-  const std::size_t bytes = hip::tree_workspace_bytes(batch(), q_heads_, c.kv_heads, nodes);
-  if (tree_workspace_.size() < bytes || accepted_.data() == nullptr) {
+  if (tree_workspace_.data() == nullptr) {
+    // Of trees of any size: a captured tree_layer() holds its address.
+    std::size_t bytes = 0;
+    for (std::size_t n = 1; n <= hip::kMaxTreeNodes; ++n) {
+      bytes = std::max(bytes, hip::tree_workspace_bytes(batch(), q_heads_, c.kv_heads, n));
+    }
     DeviceGuard guard(state_->device);
-    // Queued kernels of earlier steps may still use the smaller one.
-    hip_check(hipDeviceSynchronize(), "decode batch tree workspace");
-    if (tree_workspace_.size() < bytes) tree_workspace_ = DeviceBuffer(bytes, state_->device);
     if (accepted_.data() == nullptr) accepted_ = PinnedBuffer(batch() * sizeof(std::int32_t));
+    tree_workspace_ = DeviceBuffer(bytes, state_->device);
   }
   prepare(stream, nodes);
   tree_step_ = true;

@@ -260,14 +260,19 @@ private:
   std::size_t total_pages_ = 0;
   std::vector<std::int32_t> host_lengths_;
   DeviceBuffer tables_;
-  DeviceBuffer step_;       // lengths [B] int32 | slots [B, tokens] int64 | updates
+  // lengths [B] int32 | slots [B, tokens] int64 | updates: of steps of up to
+  // kFixedTokens tokens (its address is in captured launches and stays), and of
+  // longer ones, grown on demand.
+  DeviceBuffer step_;
+  DeviceBuffer long_step_;
+  static constexpr std::size_t kFixedTokens = hip::kMaxTreeNodes;
   DeviceBuffer workspace_;
   PinnedBuffer pinned_[2];
   hipEvent_t uploaded_[2] = {nullptr, nullptr};
   int next_pinned_ = 0;
-  std::size_t step_bytes_ = 0;
   std::size_t step_capacity_ = 0;  // tokens per sequence the step buffers hold
   std::size_t step_tokens_ = 0;    // tokens of the prepared step
+  const DeviceBuffer* step_buffer_ = &step_;  // the last prepared step's
   bool prepared_ = false;
   hipEvent_t between_event_ = nullptr;
   std::size_t shared_pages_ = 0;  // cascade prefix of the prepared step (0: off)
@@ -301,6 +306,9 @@ private:
   hipEvent_t order_event_ = nullptr;
 
   void reserve_step(std::size_t tokens);
+  [[nodiscard]] unsigned char* step_data() const {
+    return static_cast<unsigned char*>(step_buffer_->data());
+  }
   // Under the cache mutex: whether member i lives and lost no token since the
   // last prepare, whether it also ends with the step's slots, and its
   // truncation by the batch itself.

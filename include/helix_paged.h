@@ -575,7 +575,11 @@ int helix_decode_batch_prefill_layer(helix_decode_batch* b, size_t layer, const 
  * each sequence to its accepted tokens, which frees the pages behind them.
  * accept_tree() verifies the drafts first.  path, accepted and next_token are
  * device arrays.  A tree step that the next prepare call finds uncommitted is
- * dropped: its sequences go back to their lengths before it. */
+ * dropped: its sequences go back to their lengths before it.
+ * A captured tree_layer() may be replayed in every later tree step of as many
+ * nodes, whatever steps lie between: what it reads and writes keeps its address
+ * while the batch lives.  (lengths and slots of a chunk step of more than 64
+ * tokens lie in a buffer of their own.) */
 int helix_decode_batch_prepare_tree(helix_decode_batch* b, size_t nodes, helix_stream stream);
 int helix_decode_batch_tree_layer(helix_decode_batch* b, size_t layer, const float* query,
                                   const float* tree_key, const float* tree_value,

@@ -850,3 +850,42 @@ def test_a_wrong_parent_beside_values_that_are_no_numbers(device, dtype, hists, 
     assert np.isnan(want[:, :, lost]).all() and np.isfinite(want[:, :, rest]).all()
     assert np.isnan(got[:, :, lost]).all()
     close(got, want)
+
+
+def test_a_captured_layer_outlives_larger_steps(device):
+    """What a captured launch reads and writes stays where it is: a graph of trees
+    of 7 nodes is replayed behind trees of 64 and a chunk, and the batch's device
+    state keeps its addresses from the batch's first step on."""
+    s = Server("bf16", [60, 5, 200], layers=1, spare=60)
+    b, nodes = s.batch, 7
+    first = b.device_state()
+    parents = ref.random_trees(s.rng, 3, nodes)
+    q, k, v = s.normal(3, 8, nodes, D), s.normal(3, 2, nodes, D), s.normal(3, 2, nodes, D)
+    args = dev(q), dev(k), dev(v), dev(parents)
+    side, out = torch.cuda.Stream(), torch.zeros(3, 8, nodes, D, device="cuda:0")
+    torch.cuda.synchronize()
+    b.prepare_tree(nodes, stream=side)
+    b.tree_layer(0, *args, out, stream=side)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        b.tree_layer(0, *args, out)
+    for step in range(3):
+        s.tree_step(64)
+        assert b.device_state() == first
+        lengths = [s.k[i].shape[2] for i in range(3)]
+        b.prepare_chunk(100)
+        for seq, n in zip(s.seqs, lengths):
+            s.cache.truncate_sequence(seq, n)
+        b.prepare_tree(nodes, stream=side)
+        side.synchronize()
+        assert b.device_state() == first
+        want = np.zeros((3, 8, nodes, D))
+        for i in range(3):
+            ref.tree_attention(q[i], s.k[i][0], s.v[i][0], on_pages("bf16", k[i], 1),
+                               on_pages("bf16", v[i], 1), parents[i], nodes, want[i])
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        close(host(out), want)
