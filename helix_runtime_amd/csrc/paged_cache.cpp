@@ -665,10 +665,18 @@ void DecodeBatch::begin_call(hipStream_t stream, const char* op) const {
   last_stream_ = stream;
 }
 
+void DecodeBatch::require_ordinary_step(const char* op) const {
+  if (!prepared_) fail(Status::kInvalidArgument, std::string(op) + " before prepare");
+  if (tree_step_) {
+    fail(Status::kInvalidArgument,
+         std::string(op) + ": a tree step takes tree calls (its slots are kept by commit_path)");
+  }
+}
+
 void DecodeBatch::append_layer(std::size_t layer, const float* keys, const float* values,
                                hipStream_t stream) const {
   const PagedConfig& c = state_->manager.config();
-  check(prepared_, Status::kInvalidArgument, "decode batch append before prepare");
+  require_ordinary_step("decode batch append");
   check(layer < c.layers, Status::kOutOfRange, "decode batch layer is out of range");
   check(keys != nullptr && values != nullptr, Status::kInvalidArgument,
         "decode batch append needs key and value rows");
@@ -685,7 +693,7 @@ void DecodeBatch::append_layer(std::size_t layer, const float* keys, const float
 void DecodeBatch::append_all_layers(const float* keys, const float* values,
                                     hipStream_t stream) const {
   const PagedConfig& c = state_->manager.config();
-  check(prepared_, Status::kInvalidArgument, "decode batch append before prepare");
+  require_ordinary_step("decode batch append");
   check(keys != nullptr && values != nullptr, Status::kInvalidArgument,
         "decode batch append needs key and value rows");
   DeviceGuard guard(state_->device);
@@ -730,7 +738,7 @@ void DecodeBatch::attention_layer(std::size_t layer, const float* query, const f
                                   const float* tail_value, float* out, hipStream_t stream,
                                   bool fused_append) const {
   const PagedConfig& c = state_->manager.config();
-  check(prepared_, Status::kInvalidArgument, "decode batch attention before prepare");
+  require_ordinary_step("decode batch attention");
   check(step_tokens_ == 1, Status::kInvalidArgument,
         "decode batch attention needs a one-token step (use prefill for chunks)");
   check(layer < c.layers, Status::kOutOfRange, "decode batch layer is out of range");
@@ -774,7 +782,7 @@ void DecodeBatch::attention_layer(std::size_t layer, const float* query, const f
 void DecodeBatch::prefill_layer(std::size_t layer, const float* query, const float* chunk_key,
                                 const float* chunk_value, float* out, hipStream_t stream) const {
   const PagedConfig& c = state_->manager.config();
-  check(prepared_, Status::kInvalidArgument, "decode batch prefill before prepare");
+  require_ordinary_step("decode batch prefill");
   check(layer < c.layers, Status::kOutOfRange, "decode batch layer is out of range");
   check(query != nullptr && chunk_key != nullptr && chunk_value != nullptr && out != nullptr,
         Status::kInvalidArgument, "decode batch prefill needs query, chunk and output");

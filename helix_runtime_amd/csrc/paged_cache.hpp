@@ -214,7 +214,8 @@ public:
 
   // A step over a tree of `nodes` drafted tokens per sequence: reserves their
   // slots; tree_layer() is each layer's attention, commit_path() keeps the
-  // accepted nodes, accept_tree() verifies the drafts and then does.  A tree
+  // accepted nodes, accept_tree() verifies the drafts and then does.  The append
+  // and attention calls of the other steps are refused until then.  A tree
   // step that the next prepare finds uncommitted is dropped: its members go
   // back to their lengths before it.
   void prepare_tree(hipStream_t stream, std::size_t nodes);
@@ -316,7 +317,9 @@ private:
   [[nodiscard]] bool holds_step(std::size_t i) const;
   void cut(std::size_t i, std::size_t length);
   void drop_tree();
+  // A prepared step that is, or is not, one of prepare_tree().
   void require_tree_step(const char* op) const;
+  void require_ordinary_step(const char* op) const;
   void append_path(const float* keys, const float* values, const std::int32_t* path,
                    const std::int32_t* accepted, hipStream_t stream);
   // Checks that the step is prepared and its members still live, and orders

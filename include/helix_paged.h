@@ -574,8 +574,10 @@ int helix_decode_batch_prefill_layer(helix_decode_batch* b, size_t layer, const 
  * sequences' next slots in every layer, synchronises the stream and truncates
  * each sequence to its accepted tokens, which frees the pages behind them.
  * accept_tree() verifies the drafts first.  path, accepted and next_token are
- * device arrays.  A tree step that the next prepare call finds uncommitted is
- * dropped: its sequences go back to their lengths before it.
+ * device arrays.  The append, attention and prefill calls of the other steps
+ * are refused (HELIX_INVALID_ARGUMENT) until the next prepare call.  A tree
+ * step that the next prepare call finds uncommitted is dropped: its sequences
+ * go back to their lengths before it.
  * A captured tree_layer() may be replayed in every later tree step of as many
  * nodes, whatever steps lie between: what it reads and writes keeps its address
  * while the batch lives.  (lengths and slots of a chunk step of more than 64

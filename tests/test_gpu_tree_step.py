@@ -889,3 +889,24 @@ def test_a_captured_layer_outlives_larger_steps(device):
         graph.replay()
         torch.cuda.synchronize()
         close(host(out), want)
+
+
+@pytest.mark.parametrize("nodes", [1, 4])
+def test_a_tree_step_takes_tree_calls_alone(device, nodes):
+    """The calls of the other steps would write rows that the next prepare drops,
+    or attend as if the nodes were a chunk."""
+    s = Server("f32", [20, 33])
+    b, B, L = s.batch, s.B, s.layers
+    one = lambda *n: torch.ones(*n, device="cuda:0")  # noqa: E731
+    q, rows = one(B, s.hq, nodes, D), one(B, s.hkv, nodes, D)
+    out = torch.full_like(q, 7.0)
+    b.prepare_tree(nodes)
+    refused(lambda: b.append_layer(0, rows, rows))
+    refused(lambda: b.append_all_layers(one(L, *rows.shape), one(L, *rows.shape)))
+    refused(lambda: b.prefill_layer(0, q, rows, rows, out))
+    refused(lambda: b.attention_layer(0, q, rows, rows, out))
+    refused(lambda: b.append_attention_layer(0, q, rows, rows, out))
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    s.tree_step(nodes)  # the step before is dropped
+    s.decode_step()
