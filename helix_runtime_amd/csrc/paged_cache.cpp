@@ -490,7 +490,7 @@ void DecodeBatch::reserve_step(std::size_t tokens) {
   step_capacity_ = tokens;
 }
 
-void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
+void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens, bool tree) {
   CacheState& s = *state_;
   std::scoped_lock lock(s.mutex);
   prepared_ = false;
@@ -571,7 +571,7 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens) {
   }
   const std::size_t used = align8(B * sizeof(std::int32_t)) + B * tokens * sizeof(std::int64_t) +
                            3 * n_updates * sizeof(std::uint32_t);
-  if (tokens > 1) {
+  if (tokens > 1 && !tree) {
     // Longest-first order of the prefill work items: a (sequence, position
     // block) sees its history plus the chunk rows up to the block's end.
     const std::size_t H = c.kv_heads;
@@ -861,7 +861,7 @@ void DecodeBatch::prepare_tree(hipStream_t stream, std::size_t nodes) {
     if (accepted_.data() == nullptr) accepted_ = PinnedBuffer(batch() * sizeof(std::int32_t));
     tree_workspace_ = DeviceBuffer(bytes, state_->device);
   }
-  prepare(stream, nodes);
+  prepare(stream, nodes, true);
   tree_step_ = true;
 }
 

@@ -188,7 +188,8 @@ public:
               std::size_t max_tokens, std::size_t pages_per_split);
   ~DecodeBatch();
 
-  void prepare(hipStream_t stream, std::size_t tokens = 1);
+  // (`tree`: prepare_tree()'s, whose calls need no order of prefill items.)
+  void prepare(hipStream_t stream, std::size_t tokens = 1, bool tree = false);
   void append_layer(std::size_t layer, const float* keys, const float* values,
                     hipStream_t stream) const;
   // append_layer() for every layer in one launch: rows [layers, batch,
