@@ -499,7 +499,8 @@ void DecodeBatch::prepare(hipStream_t stream, std::size_t tokens, bool tree) {
   step_tokens_ = 0;
   const PagedConfig& c = s.manager.config();
   const std::size_t B = batch();
-  for (std::size_t i = 0; i < B; ++i) {
+  const bool quiet = s.releases.load(std::memory_order_acquire) == prepared_releases_;
+  for (std::size_t i = 0; i < B && !quiet; ++i) {  // (something was released or cut)
     if (!s.manager.contains(sequences_[i]) || uncut(i)) continue;
     // The row may have shrunk and grown again: the entries that still hold
     // count as mirrored, the others are uploaded with this step.
