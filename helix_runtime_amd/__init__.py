@@ -554,7 +554,6 @@ def decode_workspace(batch, q_heads, kv_heads, max_blocks, pages_per_split=0, de
 
 
 _PAGE_DTYPES = {"f32": 0, "bf16": 1, "fp8": 2}
-_PAGE_WIDTHS = {"f32": 4, "bf16": 2, "fp8": 1}  # bytes of an element
 
 
 def paged_decode_attention(query, key_pool, value_pool, tables, lengths, tail_key, tail_value,
@@ -643,6 +642,21 @@ def _require_tensor(t, name, dtypes, shape, device=None, strided=False):
         raise HelixError(INVALID_ARGUMENT, f"{name} must be on {device}, got {t.device}")
 
 
+_POOL_DTYPES = {}
+
+
+def _pool_dtypes(page_dtype):
+    """What a pool tensor of page_dtype may be: its values, or their bits."""
+    if not _POOL_DTYPES:
+        import torch
+        _POOL_DTYPES.update(f32=(torch.float32,),
+                            bf16=(torch.bfloat16, torch.int16, torch.uint16),
+                            fp8=(torch.float8_e4m3fn, torch.uint8, torch.int8))
+    if page_dtype not in _POOL_DTYPES:
+        raise HelixError(INVALID_ARGUMENT, 'page_dtype must be "f32", "bf16" or "fp8"')
+    return _POOL_DTYPES[page_dtype]
+
+
 _HERE = contextlib.nullcontext()
 
 
@@ -686,7 +700,8 @@ def paged_tree_attention(query, key_pool, value_pool, tables, lengths, tree_key,
     """Attention of a tree of up to 64 drafted tokens per sequence: query row
     (h, t) sees the sequence's history, the ancestors of node t and node t.
     query, output [B, Hq, T, 128]; pools [N, Hkv, 16, 128] tensors (or raw
-    device addresses with pool_shape) of page_dtype "f32", "bf16" or "fp8";
+    device addresses with pool_shape) of page_dtype "f32", "bf16" (bfloat16, or
+    its bits as int16 / uint16) or "fp8" (float8_e4m3fn, uint8 or int8);
     tables [B, max_blocks] int32/uint32; lengths [B] int32 history tokens;
     tree_key / tree_value [B, Hkv, T, 128]; parents [B, T] int32 (parent of
     each node, before it, or -1 for a root) or None for chains; node_counts [B]
@@ -700,11 +715,9 @@ def paged_tree_attention(query, key_pool, value_pool, tables, lengths, tree_key,
     dev = query.device
     if pool_shape is None:
         pool_shape = key_pool.shape
-        width = _PAGE_WIDTHS.get(page_dtype)
+        dtypes = _pool_dtypes(page_dtype)
         for pool, name in ((key_pool, "key_pool"), (value_pool, "value_pool")):
-            if width is not None and pool.element_size() != width:
-                raise HelixError(INVALID_ARGUMENT, f"{name} must hold {width}-byte elements")
-            _require_tensor(pool, name, (pool.dtype,), pool_shape, dev)
+            _require_tensor(pool, name, dtypes, pool_shape, dev)
         key_pool, value_pool = key_pool.data_ptr(), value_pool.data_ptr()
     if len(pool_shape) != 4:
         raise HelixError(INVALID_ARGUMENT, "pools must have shape [blocks, kv_heads, tokens, dim]")
@@ -806,9 +819,10 @@ def verify_tree(target, draft, tokens, parents, uniforms, bonus_uniforms, path, 
 def append_path(keys, values, key_pool, value_pool, slots, path, accepted, stream=None,
                 page_dtype="f32", k_scale=1.0, v_scale=1.0):
     """Write the rows of the accepted nodes, path[b, i] for i < accepted[b], to
-    slots[b, i]: keys / values [B, Hkv, T, D] and pools [N, Hkv, P, D], or with
-    a leading dimension of layers each (a pool's layers may lie apart); slots
-    [B, T] int64, path [B, T] and accepted [B] int32."""
+    slots[b, i]: keys / values [B, Hkv, T, D] and pools [N, Hkv, P, D] (of the
+    types that paged_tree_attention takes), or with a leading dimension of layers
+    each (a pool's layers may lie apart); slots [B, T] int64, path [B, T] and
+    accepted [B] int32."""
     import torch
     layered = key_pool.dim() == 5
     if key_pool.dim() not in (4, 5):
@@ -825,21 +839,19 @@ def append_path(keys, values, key_pool, value_pool, slots, path, accepted, strea
     _require_tensor(values, "values", (torch.float32,), (*lead, b, hkv, t, d), dev)
     _require_tensor(path, "path", (torch.int32,), (b, t), dev)
     _require_tensor(accepted, "accepted", (torch.int32,), (b,), dev)
-    width = _PAGE_WIDTHS.get(page_dtype)
+    dtypes = _pool_dtypes(page_dtype)
     stride = 0
     for pool, name in ((key_pool, "key_pool"), (value_pool, "value_pool")):
-        if width is not None and pool.element_size() != width:
-            raise HelixError(INVALID_ARGUMENT, f"{name} must hold {width}-byte elements")
         if layered:
-            _require_tensor(pool, name, (pool.dtype,), key_pool.shape, dev, strided=True)
+            _require_tensor(pool, name, dtypes, key_pool.shape, dev, strided=True)
             if layers and not pool.is_contiguous():  # a layer's pool is, if not all of them
-                _require_tensor(pool[0], name, (pool.dtype,), key_pool.shape[1:], dev)
+                _require_tensor(pool[0], name, dtypes, key_pool.shape[1:], dev)
             if layers > 1:
                 if pool.stride(0) != key_pool.stride(0):
                     raise HelixError(INVALID_ARGUMENT, "pools must have the same layer stride")
                 stride = pool.stride(0)
         else:
-            _require_tensor(pool, name, (pool.dtype,), key_pool.shape, dev)
+            _require_tensor(pool, name, dtypes, key_pool.shape, dev)
     with _on(dev):
         check(_lib().helix_paged_append_path(
             _address(keys), _address(values), _address(key_pool), _address(value_pool), layers,

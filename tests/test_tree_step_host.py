@@ -182,6 +182,43 @@ def test_python_append_path_checks_its_tensors(name, value):
     assert e.value.status == hx.INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("page_dtype,dtype", [
+    ("f32", "int32"), ("bf16", "float16"), ("fp8", "bool"), ("fp8", "float8_e5m2"),
+    ("fp8", "float8_e4m3fnuz"), ("f32", "bfloat16"), ("f16", "float16")])
+def test_pools_must_hold_the_page_types_elements(page_dtype, dtype):
+    """An element type of the right width alone would give wrong numbers without
+    an error."""
+    dtype = getattr(torch, dtype)
+    for names in (("key_pool",), ("value_pool",), ("key_pool", "value_pool")):
+        a = tensors()
+        b = dict(keys=torch.zeros(1, 2, 3, 8), values=torch.zeros(1, 2, 3, 8),
+                 slots=torch.zeros(1, 3, dtype=torch.int64),
+                 path=torch.zeros(1, 3, dtype=torch.int32),
+                 accepted=torch.zeros(1, dtype=torch.int32))
+        right = {"f32": torch.float32, "bf16": torch.bfloat16}.get(page_dtype, torch.uint8)
+        for name in ("key_pool", "value_pool"):
+            a[name] = a[name].to(dtype if name in names else right)
+            b[name] = torch.zeros(4, 2, 16, 8).to(dtype if name in names else right)
+        for call, kw in ((hx.paged_tree_attention, a), (hx.append_path, b)):
+            with pytest.raises(hx.HelixError) as e:
+                call(**kw, page_dtype=page_dtype)
+            assert e.value.status == hx.INVALID_ARGUMENT
+            assert "pool must" in str(e.value) or "page_dtype" in str(e.value)
+
+
+@pytest.mark.parametrize("page_dtype,dtypes", [
+    ("f32", ["float32"]), ("bf16", ["bfloat16", "int16", "uint16"]),
+    ("fp8", ["float8_e4m3fn", "uint8", "int8"])])
+def test_pools_may_hold_their_bits(page_dtype, dtypes):
+    """(What is refused then is that they are not on a GPU.)"""
+    for dtype in dtypes:
+        a = tensors()
+        a.update(key_pool=a["key_pool"].to(getattr(torch, dtype)),
+                 value_pool=a["value_pool"].to(getattr(torch, dtype)))
+        with pytest.raises(hx.HelixError, match="on a GPU"):
+            hx.paged_tree_attention(**a, page_dtype=page_dtype)
+
+
 # ------------------------------------------------------------- truncation ----
 def test_truncate_frees_pages_in_table_order():
     m = hx.BlockManager(1, 1, 2, 4, 5)
