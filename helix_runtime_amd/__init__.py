@@ -930,7 +930,7 @@ class DecodeBatch:
         """Reserve the slots of a tree of `nodes` drafted tokens (up to 64) per
         sequence: tree_layer() in every layer, then accept_tree() or
         commit_path().  An uncommitted tree step is dropped by the next
-        prepare call."""
+        prepare call or close()."""
         check(_lib().helix_decode_batch_prepare_tree(self._h, nodes, _stream(stream)))
         self._nodes = nodes
 

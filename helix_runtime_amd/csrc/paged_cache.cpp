@@ -427,6 +427,13 @@ DecodeBatch::DecodeBatch(std::shared_ptr<CacheState> state, const std::uint64_t*
 
 DecodeBatch::~DecodeBatch() {
   // Destructors must not throw: switch devices without the checked guard.
+  if (tree_step_) {
+    try {
+      std::scoped_lock lock(state_->mutex);
+      drop_tree();
+    } catch (...) {  // (a fork made in the step shares its slots' pages)
+    }
+  }
   int previous = -1;
   const bool switched = hipGetDevice(&previous) == hipSuccess && previous != state_->device &&
                         hipSetDevice(state_->device) == hipSuccess;

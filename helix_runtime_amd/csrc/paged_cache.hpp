@@ -217,8 +217,8 @@ public:
   // slots; tree_layer() is each layer's attention, commit_path() keeps the
   // accepted nodes, accept_tree() verifies the drafts and then does.  The append
   // and attention calls of the other steps are refused until then.  A tree
-  // step that the next prepare finds uncommitted is dropped: its members go
-  // back to their lengths before it.
+  // step that the next prepare, or the destructor, finds uncommitted is dropped:
+  // its members go back to their lengths before it.
   void prepare_tree(hipStream_t stream, std::size_t nodes);
   // query, out [batch, q_heads, nodes, 128]; tree_key/value [batch, kv_heads,
   // nodes, 128]; parents [batch, nodes] (nullptr: a chain), node_counts [batch]

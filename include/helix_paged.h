@@ -576,8 +576,11 @@ int helix_decode_batch_prefill_layer(helix_decode_batch* b, size_t layer, const 
  * accept_tree() verifies the drafts first.  path, accepted and next_token are
  * device arrays.  The append, attention and prefill calls of the other steps
  * are refused (HELIX_INVALID_ARGUMENT) until the next prepare call.  A tree
- * step that the next prepare call finds uncommitted is dropped: its sequences
- * go back to their lengths before it.
+ * step that the next prepare call, or the batch's destruction, finds uncommitted
+ * is dropped: its sequences go back to their lengths before it, except those
+ * that were released, truncated or appended to in between.  (A sequence should
+ * not be appended to inside a tree step, or forked past its length before it:
+ * slots that nothing wrote would be among its tokens, or shared.)
  * A captured tree_layer() may be replayed in every later tree step of as many
  * nodes, whatever steps lie between: what it reads and writes keeps its address
  * while the batch lives.  (lengths and slots of a chunk step of more than 64

@@ -910,3 +910,22 @@ def test_a_tree_step_takes_tree_calls_alone(device, nodes):
     assert (out == 7.0).all()
     s.tree_step(nodes)  # the step before is dropped
     s.decode_step()
+
+
+def test_closing_a_batch_drops_its_uncommitted_tree_step(device):
+    """As the next prepare would: members that changed since are left alone."""
+    s = Server("f32", [20, 33, 16, 7])
+    s.batch.prepare_tree(20)
+    assert [s.cache.length(x) for x in s.seqs] == [40, 53, 36, 27]
+    cut_and_grow(s, 0, 18, 22)
+    s.cache.release_sequence(s.seqs[3])
+    del s.seqs[3], s.k[3], s.v[3]
+    s.batch.close()
+    assert [s.cache.length(x) for x in s.seqs] == [40, 33, 16]
+    s.compare()
+    s.B = 3
+    s.batch = hx.DecodeBatch(s.cache, s.seqs, s.hq, 512)
+    s.tree_step(5)
+    s.batch.prepare()  # an ordinary step's slots stay the members'
+    s.batch.close()
+    assert [s.cache.length(x) for x in s.seqs] == [s.k[i].shape[2] + 1 for i in range(3)]
