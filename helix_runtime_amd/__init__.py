@@ -931,7 +931,9 @@ class DecodeBatch:
         sequence: tree_layer() in every layer, then accept_tree() or
         commit_path().  An uncommitted tree step is dropped by the next
         prepare call or close()."""
-        check(_lib().helix_decode_batch_prepare_tree(self._h, nodes, _stream(stream)))
+        import torch
+        dev = torch.device("cuda", self._cache.device)
+        check(_lib().helix_decode_batch_prepare_tree(self._h, nodes, _device_stream(stream, dev)))
         self._nodes = nodes
 
     def tree_layer(self, layer, query, tree_key, tree_value, parents, output, node_counts=None,

@@ -219,6 +219,32 @@ def test_pools_may_hold_their_bits(page_dtype, dtypes):
             hx.paged_tree_attention(**a, page_dtype=page_dtype)
 
 
+def test_prepare_tree_takes_the_current_stream_of_the_caches_device(monkeypatch):
+    """As the step's other calls do, whatever device is the current one."""
+    class Stream:
+        def __init__(self, device=None):
+            self.cuda_stream = 100 + (0 if device is None else torch.device(device).index)
+
+    class Library:
+        def helix_decode_batch_prepare_tree(self, handle, nodes, stream):
+            self.stream = getattr(stream, "value", stream)
+            return 0
+
+        def helix_decode_batch_destroy(self, handle):
+            pass
+
+    lib = Library()
+    monkeypatch.setattr(hx, "_lib", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    batch = hx.DecodeBatch.__new__(hx.DecodeBatch)
+    batch._h, batch._cache = 1, type("Cache", (), {"device": 1})()
+    batch.prepare_tree(4)
+    assert lib.stream == 101
+    batch.prepare_tree(4, stream=Stream("cuda:2"))
+    assert lib.stream == 102
+    batch.close()
+
+
 # ------------------------------------------------------------- truncation ----
 def test_truncate_frees_pages_in_table_order():
     m = hx.BlockManager(1, 1, 2, 4, 5)
