@@ -230,19 +230,18 @@ def test_prepare_tree_takes_the_current_stream_of_the_caches_device(monkeypatch)
             self.stream = getattr(stream, "value", stream)
             return 0
 
-        def helix_decode_batch_destroy(self, handle):
-            pass
-
     lib = Library()
     monkeypatch.setattr(hx, "_lib", lambda: lib)
     monkeypatch.setattr(torch.cuda, "current_stream", Stream)
     batch = hx.DecodeBatch.__new__(hx.DecodeBatch)
     batch._h, batch._cache = 1, type("Cache", (), {"device": 1})()
-    batch.prepare_tree(4)
-    assert lib.stream == 101
-    batch.prepare_tree(4, stream=Stream("cuda:2"))
-    assert lib.stream == 102
-    batch.close()
+    try:
+        batch.prepare_tree(4)
+        assert lib.stream == 101
+        batch.prepare_tree(4, stream=Stream("cuda:2"))
+        assert lib.stream == 102
+    finally:
+        batch._h = None
 
 
 # ------------------------------------------------------------- truncation ----
