@@ -800,7 +800,7 @@ def verify_tree(target, draft, tokens, parents, uniforms, bonus_uniforms, path, 
     that follows them.  target [B, T, V]: row n is the target's distribution
     after node n; draft [B, T, V] or None: row n is the distribution the children
     of node n were drawn from (None: they were certain); both may be strided in
-    their first two dimensions.  tokens [B, T] int32; parents [B, T] int32 or
+    their first two dimensions (nodes share no entries).  tokens [B, T] int32; parents [B, T] int32 or
     None for chains (node 0 is the root); uniforms [B, T] and bonus_uniforms [B]
     in [0, 1); node_counts [B] int32 or None.  Writes path [B, T] (accepted
     nodes from the root, then -1), accepted [B] (their number) and next_token

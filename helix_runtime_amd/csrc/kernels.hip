@@ -216,8 +216,9 @@ __global__ __launch_bounds__(256) void append_slots_kernel(
 // layer's K or V; x over a row's elements, y over (sequence, split), z over
 // (layer, K or V).  A wavefront reads 64 nodes and slots at once, works out where
 // their rows lie, one a lane, and moves the rows i % splits == split one behind
-// another.  What bounds it is the copy: 64 sequences' 5 rows in 32 layers are
-// 169 MB with fp32 pages, 37 us (4.6 TB/s); 6 rows are 114 MB with bf16 ones, 34 us.
+// another.  What bounds it is the copy: 64 sequences' 323 rows in 32 layers are
+// 169 MB with fp32 pages, 38 us (4.4 TB/s); 291 rows are 114 MB with bf16 ones,
+// 35 us (3.3 TB/s, written 8 bytes a lane).
 template <typename S, int W>
 __global__ __launch_bounds__(256) void append_path_kernel(
     const float* __restrict__ keys, const float* __restrict__ values, S* key_pool, S* value_pool,

@@ -40,12 +40,13 @@
 // tile of 16 rows that ends a part with one is marked, and tree_merge_kernel
 // computes that part of it again with exact_row.
 //
-// Measured: 64 sequences of 512 to 8192 tokens, 32/8 heads, trees of 16 nodes: fp32
-// pages 356 us and bf16 pages 180 us, both at 4.2 TB/s of pages; loads and LDS
+// Measured (both launches, after the first hundred calls, which take up to a fifth
+// longer): 64 sequences of 512 to 8192 tokens, 32/8 heads, trees of 16 nodes: fp32
+// pages 360 us and bf16 pages 182 us, both at 4.2 TB/s of pages; loads and LDS
 // writes alone take 330 and 165, products alone 306 and 150.  Trees of 64 nodes,
-// fp8 pages: 448 us (900 TFLOP/s of fp16 products), vector work (16 exponentials
+// fp8 pages: 454 us (885 TFLOP/s of fp16 products), vector work (16 exponentials
 // and as many splits a lane and block) beside the matrix instructions.  One
-// sequence of 131071, 33 nodes, bf16: 297 us.
+// sequence of 131071, 33 nodes, bf16: 303 us.
 #include "prefill_bmma.hpp"
 #include "tree_exact.hpp"
 
@@ -186,7 +187,7 @@ __device__ __forceinline__ void chunk_of_rows(v4f x0, v4f x1, float scale,
 // Whether the two wavefronts of each SIMD take turns (tree_mma_body), and the LDS
 // buffers that takes: an item is put there two steps before its use, or one step,
 // or (fp32 pages, whose three planes would take the space of a second workgroup)
-// just before it.  (131071 bf16 tokens, 33 nodes: 331 us in turns, 351 without.)
+// just before it.  (131071 bf16 tokens, 33 nodes: 302 us in turns, 322 without.)
 constexpr bool in_turns(int pf, int waves, int tiles) {
   return pf == 1 && waves == 8 && tiles == 2;
 }
@@ -195,9 +196,9 @@ constexpr int stage_buffers(int pf, int waves, int tiles) {
 }
 
 // Items on their way from memory to registers.  (64 bf16 sequences of 16 nodes:
-// 178 us with two, 190 with one; 32 of them 112 with two, 118 with three.  fp32
-// pages gain nothing, and fp8 pages more from the registers of a third workgroup
-// on the CU.)
+// 182 us with two, 183 with one; 32 of them 110 with two, 111 with one.  Three, and
+// two of fp32 pages, gained nothing; fp8 pages gained more from the registers of a
+// third workgroup on the CU.)
 constexpr int load_depth(int pf, int tiles) { return pf == 1 && tiles == 1 ? 2 : 1; }
 
 template <int PF, int W, int RT>
@@ -435,7 +436,9 @@ __device__ __forceinline__ void tree_mma_body(const TreeKernelArgs& a, const Tre
   using Global = const __attribute__((address_space(1))) Raw*;
   using GlobalBytes = const __attribute__((address_space(1))) unsigned char*;
   const unsigned lane_at = static_cast<unsigned>(lane) * 16u;
-  auto stream = [&](unsigned long long at, int w) {  // (each byte is read once)
+  // (A unit reads each byte once.  Where its head's rows are several units, past
+  // 256 rows, or 128 with fp8 pages, each of them reads the pages.)
+  auto stream = [&](unsigned long long at, int w) {
     return __builtin_nontemporal_load(
         reinterpret_cast<Global>(reinterpret_cast<GlobalBytes>(at + 1024u * w) + lane_at));
   };
@@ -1188,12 +1191,15 @@ struct TreeShape {
   std::size_t rows() const { return static_cast<std::size_t>(waves) * tiles * 16; }
 };
 
-// A unit's rows and the workgroups that the chip holds at once.  Of 32 sequences
-// with bf16, fp8 and fp32 pages: 64 rows take 125, 100 and 200 us with four
-// wavefronts and 183, 189 and 288 with eight; 128 rows 159, 131 and 287 in two row
-// blocks of four wavefronts, 158, - and 256 in one of eight, -, 123 and - in one of
-// four with two tiles each; 256 rows 324, 262 and 572 in one of eight with two tiles,
-// 359, - and 637 in two blocks of eight, -, 261 and - in two of four with two tiles.
+// A unit's rows and the workgroups that the chip holds at once.  32 sequences of 512
+// to 8192 tokens, 32/8 heads, in us:
+//                          bf16 pages       fp32 pages       fp8 pages
+//   rows of a head       64  128  256     64  128  256     64  128  256
+//   4 wavefronts        110  158  390    192  300  762     92  128  296
+//   4 of two tiles        -    -    -      -    -    -    117  113  242
+//   8 wavefronts        127  143  332    206  249  626      -    -    -
+//   8 of two tiles      209  198  297    432  386  559      -    -    -
+// (An item of fp8 pages is four jobs, of a wavefront each.)
 TreeShape tree_shape(PageType type, std::size_t rows) {
   if (type == PageType::kFP8) {
     return rows <= 64 ? TreeShape{4, 1, 3 * kTreeCus} : TreeShape{4, 2, 2 * kTreeCus};

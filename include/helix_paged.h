@@ -472,8 +472,9 @@ int helix_paged_tree_attention(const float* query, size_t batch, size_t q_heads,
 /* Verification against the target's probabilities, from given uniform random
  * numbers in [0, 1).  target row (b, n) is the target's distribution after node
  * n, draft row (b, n) the one that the children of n were drawn from, each
- * vocab entries with the given batch and node strides (in elements); draft NULL:
- * the drafts were certain.  From n = 0 with w = target row 0, the children of n
+ * vocab entries with the given batch and node strides in elements (a node stride
+ * is vocab at least: nodes share no entries); draft NULL: the drafts were
+ * certain.  From n = 0 with w = target row 0, the children of n
  * are tried in order: child c with token x is accepted, and becomes n, where
  * uniforms[c] * draft_n(x) < w(x); otherwise w becomes max(w - draft_n, 0)
  * divided by its sum.  (draft NULL: accepted where uniforms[c] * m < w(x), m
@@ -613,6 +614,8 @@ int helix_decode_batch_shared_pages(const helix_decode_batch* b, size_t* out);
  * main decode kernel and the merge kernel, so the dominant kernel can be
  * timed alone.  NULL turns it off. */
 int helix_decode_batch_set_timing_event(helix_decode_batch* b, void* event);
+/* (Where it drops a tree step it waits for read leases, as every call that
+ * changes sequences does.) */
 void helix_decode_batch_destroy(helix_decode_batch* b);
 
 /* ------------------------------------------------------ prefix cache ---- */

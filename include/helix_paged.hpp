@@ -1081,7 +1081,9 @@ class DecodeBatch final {
   /// A tree step: up to `nodes` drafted tokens per sequence are checked at once.
   /// tree_layer() is one layer's attention (rows [B, heads, nodes, D]; parents
   /// [B, nodes] int32 or nullptr: chains; node_counts [B] int32 or nullptr: all
-  /// nodes); commit_path() or accept_tree() ends the step.
+  /// nodes); commit_path() or accept_tree() ends the step.  The append, attention
+  /// and prefill calls are refused until then; a step that the next prepare call or
+  /// the destructor finds uncommitted is dropped.
   void prepare_tree(std::size_t nodes, const hip::Stream& stream) {
     step_tokens_ = 0;
     detail::check(helix_decode_batch_prepare_tree(batch_handle_, nodes, stream.native()));
