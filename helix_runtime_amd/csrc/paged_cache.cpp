@@ -311,6 +311,7 @@ DecodeView::DecodeView(std::shared_ptr<CacheState> state, std::uint64_t sequence
               "read_sequence table upload");
   }
   valid_ = true;
+  state_->lease.store(std::this_thread::get_id());
 }
 
 void DecodeView::require_valid(const char* op) const {
@@ -429,7 +430,10 @@ DecodeBatch::~DecodeBatch() {
   // Destructors must not throw: switch devices without the checked guard.
   if (tree_step_) {
     try {
-      std::scoped_lock lock(state_->mutex);
+      // (A view of this thread holds the mutex already.  What it shows are its own
+      // copies, and no page is given out again before it ends.)
+      std::unique_lock lock(state_->mutex, std::defer_lock);
+      if (state_->lease.load() != std::this_thread::get_id()) lock.lock();
       drop_tree();
     } catch (...) {  // (a fork made in the step shares its slots' pages)
     }

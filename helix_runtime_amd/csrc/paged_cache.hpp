@@ -20,6 +20,7 @@
 #include <cstdint>
 #include <memory>
 #include <mutex>
+#include <thread>
 #include <vector>
 
 namespace helix {
@@ -79,6 +80,7 @@ struct CacheState {
   DeviceBuffer slab;
   std::size_t layer_elements = 0;  // physical_blocks * kv_heads * block_tokens * head_dim
   std::mutex mutex;
+  std::atomic<std::thread::id> lease{};  // the thread of the DecodeView that holds it
   bool poisoned = false;
   // Releases and truncations through the cache so far: a DecodeBatch compares
   // it with the value at its last prepare() to notice that a member may have
@@ -142,6 +144,9 @@ private:
 class DecodeView {
 public:
   DecodeView(std::shared_ptr<CacheState> state, std::uint64_t sequence, std::uint64_t cache_id);
+  ~DecodeView() { state_->lease.store(std::thread::id()); }
+  DecodeView(const DecodeView&) = delete;
+  DecodeView& operator=(const DecodeView&) = delete;
   [[nodiscard]] std::size_t length() const;
   [[nodiscard]] const std::vector<std::uint32_t>& physical_blocks() const;
   [[nodiscard]] const std::uint32_t* device_table() const;

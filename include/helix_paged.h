@@ -614,8 +614,8 @@ int helix_decode_batch_shared_pages(const helix_decode_batch* b, size_t* out);
  * main decode kernel and the merge kernel, so the dominant kernel can be
  * timed alone.  NULL turns it off. */
 int helix_decode_batch_set_timing_event(helix_decode_batch* b, void* event);
-/* (Where it drops a tree step it waits for read leases, as every call that
- * changes sequences does.) */
+/* (Where it drops a tree step it waits for other threads' read leases, as every
+ * call that changes sequences does.) */
 void helix_decode_batch_destroy(helix_decode_batch* b);
 
 /* ------------------------------------------------------ prefix cache ---- */

@@ -929,3 +929,17 @@ def test_closing_a_batch_drops_its_uncommitted_tree_step(device):
     s.batch.prepare()  # an ordinary step's slots stay the members'
     s.batch.close()
     assert [s.cache.length(x) for x in s.seqs] == [s.k[i].shape[2] + 1 for i in range(3)]
+
+
+def test_a_batch_with_a_tree_step_closes_inside_a_read_lease(device):
+    s = Server("f32", [20, 33])
+    s.batch.prepare_tree(20)
+    with s.cache.read_sequence(s.seqs[1]) as view:
+        s.batch.close()
+        assert view.length() == 53  # the lease's copy
+    assert [s.cache.length(x) for x in s.seqs] == [20, 33]
+    s.compare()
+    s.batch = hx.DecodeBatch(s.cache, s.seqs, s.hq, 512)
+    with s.cache.read_sequence(s.seqs[0]):
+        pass
+    s.tree_step(4)
