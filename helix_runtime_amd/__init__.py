@@ -27,6 +27,9 @@ __all__ = [
     "paged_decode_attention", "decode_workspace_bytes", "decode_workspace", "append_slots",
     "paged_tree_attention", "tree_workspace_bytes", "tree_workspace", "verify_tree",
     "verify_workspace_bytes", "verify_workspace", "append_path",
+    "rope_tables", "rope_rows", "rope_append", "latent_append", "paged_latent_attention",
+    "latent_workspace_bytes", "latent_workspace", "latent_prefill_attention",
+    "latent_prefill_workspace_bytes", "latent_prefill_workspace",
     "PagedPrefixCache", "PREFIX_INSERTED", "PREFIX_ALREADY_PRESENT", "PREFIX_REJECTED_TOO_LARGE",
     "INVALID_ARGUMENT", "OUT_OF_RANGE", "UNSUPPORTED", "RESOURCE_EXHAUSTED", "RUNTIME", "INTERNAL",
 ]
@@ -859,6 +862,314 @@ def append_path(keys, values, key_pool, value_pool, slots, path, accepted, strea
             _PAGE_DTYPES.get(page_dtype, -1), k_scale, v_scale, _device_stream(stream, dev)))
 
 
+# --------------------------------------- rotary positions, latent cache ----
+ROPE_LAYOUTS = {"pairs": 0, "halves": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "ramp": 3, "bands": 4}
+LATENT_ROPE = 64  # rotated elements of a latent cache's row
+LATENT_NOPE = 128  # key elements of a head without them, and of its value (expanded form)
+_Strides = ctypes.c_size_t * 3
+
+
+def _rows(t, name, shape, device=None):
+    """The address of fp32 rows of `shape` (None: any size), contiguous in their
+    last dimension, and their other strides (None: contiguous)."""
+    _require_tensor(t, name, (_F32(),), shape, device, strided=True)
+    if t.is_contiguous():
+        return t.data_ptr(), None
+    return t.data_ptr(), _Strides(*t.stride()[:-1])
+
+
+_f32 = None
+
+
+def _F32():
+    global _f32
+    if _f32 is None:
+        import torch
+        _f32 = torch.float32
+    return _f32
+
+
+def _optional_rows(t, name, shape, device):
+    return (None, None) if t is None else _rows(t, name, shape, device)
+
+
+def _layout(layout):
+    if layout not in ROPE_LAYOUTS:
+        raise HelixError(INVALID_ARGUMENT, f"layout must be one of {sorted(ROPE_LAYOUTS)}")
+    return ROPE_LAYOUTS[layout]
+
+
+def _rope_cache(cosine, sine, rotary_dim, device):
+    """Checks the tables; their rows and the rotary dimension."""
+    shape = getattr(cosine, "shape", ())
+    rows, pairs = shape if len(shape) == 2 else (None, None)
+    _require_tensor(cosine, "cosine", (_F32(),), (rows, pairs), device)
+    _require_tensor(sine, "sine", (_F32(),), (rows, pairs), device)
+    if rotary_dim is not None and rotary_dim != 2 * pairs:
+        raise HelixError(INVALID_ARGUMENT, "tables must have shape [rows, rotary_dim / 2]")
+    return rows, 2 * pairs
+
+
+def rope_tables(cosine, sine, base=10000.0, first_position=0, scaling="none", factor=1.0,
+                original_length=0, low=None, high=None, amplitude=1.0, stream=None):
+    """Fill cosine and sine [rows, rotary_dim / 2] for positions first_position on:
+    amplitude * cos and sin of position * base^(-2 i / rotary_dim), in 64 bits,
+    rounded once.  scaling changes the frequencies for contexts longer than
+    original_length, the one a model was trained on: "linear" (divided by factor),
+    "ntk" (a larger base), "ramp" (divided where a wave turns at most `low` times
+    over the original length, as they are from `high` turns on, a mean between,
+    linear in the pair's index; 1 and 32 by default) or "bands" (the same, linear in
+    the turns; 1 and 4 by default)."""
+    import torch
+    if scaling not in ROPE_SCALINGS:
+        raise HelixError(INVALID_ARGUMENT, f"scaling must be one of {sorted(ROPE_SCALINGS)}")
+    rows, rotary = _rope_cache(cosine, sine, None, None)
+    if sine.device != cosine.device:
+        raise HelixError(INVALID_ARGUMENT, "cosine and sine must be on one device")
+    low = 1.0 if low is None else low
+    high = (4.0 if scaling == "bands" else 32.0) if high is None else high
+    if not isinstance(first_position, int) or first_position < 0:
+        raise HelixError(INVALID_ARGUMENT, "first_position must be a whole number of 0 at least")
+    dev = cosine.device
+    with _on(dev):
+        check(_lib().helix_rope_tables(
+            cosine.data_ptr(), sine.data_ptr(), rows, first_position, rotary, base,
+            ROPE_SCALINGS[scaling], factor, original_length, low, high, amplitude,
+            _device_stream(stream, dev)))
+
+
+def rope_rows(input, cosine, sine, output=None, positions=None, layout="pairs", rotary_dim=None,
+              inverse=False, stream=None):
+    """Rotate the first rotary_dim elements of rows [tokens, vectors, head_dim]
+    (any strides but the last; the other elements are copied) to output (None: a new
+    tensor; may be input itself).  cosine, sine [rows, rotary_dim / 2]; token t uses
+    row positions[t] (int32) or t.  layout "pairs" turns elements (2 i, 2 i + 1),
+    "halves" (i, i + rotary_dim / 2); inverse turns back (the gradient's way)."""
+    import torch
+    shape = getattr(input, "shape", ())
+    if len(shape) != 3:
+        raise HelixError(INVALID_ARGUMENT, "input must have shape [tokens, vectors, head_dim]")
+    if output is None:
+        output = torch.empty(shape, dtype=torch.float32, device=input.device)
+    x, xs = _rows(input, "input", shape)
+    dev = input.device
+    y, ys = _rows(output, "output", shape, dev)
+    rows, rotary = _rope_cache(cosine, sine, rotary_dim, dev)
+    tokens, vectors, dim = shape
+    if positions is not None:
+        _require_tensor(positions, "positions", (torch.int32,), (tokens,), dev)
+    elif rows < tokens:
+        raise HelixError(INVALID_ARGUMENT, "without positions the tables need a row per token")
+    order = _layout(layout)
+    with _on(dev):
+        check(_lib().helix_rope_rows(
+            x, xs, y, ys, tokens, vectors, dim, rotary, order, bool(inverse),
+            cosine.data_ptr(), sine.data_ptr(), rows, _address(positions),
+            _device_stream(stream, dev)))
+    return output
+
+
+def _append_rows(batch, q_heads, kv_heads, tokens, dim, query, keys, values, query_out, key_out,
+                 value_out, dev):
+    """Checked addresses and strides of a rope append's rows, inputs then outputs."""
+    if (query is None) != (query_out is None):
+        raise HelixError(INVALID_ARGUMENT, "query and query_out go together")
+    q, kv = (batch, q_heads, tokens, dim), (batch, kv_heads, tokens, dim)
+    return (*_optional_rows(query, "query", q, dev), *_rows(keys, "keys", kv, dev),
+            *_rows(values, "values", kv, dev), *_optional_rows(query_out, "query_out", q, dev),
+            *_optional_rows(key_out, "key_out", kv, dev),
+            *_optional_rows(value_out, "value_out", kv, dev))
+
+
+def rope_append(query, keys, values, key_pool, value_pool, starts, slots, cosine, sine,
+                query_out=None, key_out=None, value_out=None, layout="pairs", rotary_dim=None,
+                token_counts=None, stream=None, page_dtype="f32", k_scale=1.0, v_scale=1.0):
+    """Append a step's new rows with the rotation on the way, in one launch.
+    query [B, Hq, T, D] (or None) rotated to query_out; keys [B, Hkv, T, D] rotated to
+    their pages, and to key_out where given; values likewise, not rotated.  All of
+    any strides but the last (a projection's output as it lies); an output may be its
+    input.  Pools [N, Hkv, P, D] of page_dtype; slots [B, T] int64 (outside the
+    pool: no page); row t of sequence b stands at position starts[b] + t (int32);
+    token_counts [B] int32 or None: each sequence's own number of rows."""
+    import torch
+    shape = getattr(keys, "shape", ())
+    if len(shape) != 4:
+        raise HelixError(INVALID_ARGUMENT, "keys must have shape [batch, kv_heads, tokens, dim]")
+    b, hkv, t, d = shape
+    dev = keys.device
+    hq = query.shape[1] if query is not None and query.dim() == 4 else 0
+    rows = _append_rows(b, hq, hkv, t, d, query, keys, values, query_out, key_out, value_out, dev)
+    dtypes = _pool_dtypes(page_dtype)
+    n, _, p, _ = pool_shape = key_pool.shape if key_pool.dim() == 4 else (None, hkv, None, d)
+    if pool_shape[1] != hkv or pool_shape[3] != d:
+        raise HelixError(INVALID_ARGUMENT, "pools must have the heads and head size of the keys")
+    _require_tensor(key_pool, "key_pool", dtypes, pool_shape, dev)
+    _require_tensor(value_pool, "value_pool", dtypes, pool_shape, dev)
+    _require_tensor(slots, "slots", (torch.int64,), (b, t), dev)
+    _require_tensor(starts, "starts", (torch.int32,), (b,), dev)
+    if token_counts is not None:
+        _require_tensor(token_counts, "token_counts", (torch.int32,), (b,), dev)
+    table_rows, rotary = _rope_cache(cosine, sine, rotary_dim, dev)
+    order = _layout(layout)
+    with _on(dev):
+        check(_lib().helix_paged_rope_append(
+            *rows, b, hq, hkv, t, d, key_pool.data_ptr(), value_pool.data_ptr(), n, p,
+            slots.data_ptr(), starts.data_ptr(), _address(token_counts), cosine.data_ptr(),
+            sine.data_ptr(), table_rows, rotary, order, _PAGE_DTYPES[page_dtype],
+            k_scale, v_scale, _device_stream(stream, dev)))
+
+
+def _latent_pool(pool, pool_shape, page_dtype, dev):
+    """A latent cache's pages [N, 16, latent + 64]: address and shape."""
+    dtypes = _pool_dtypes(page_dtype)
+    if pool_shape is None:
+        pool_shape = getattr(pool, "shape", ())
+        if len(pool_shape) == 3:
+            _require_tensor(pool, "pool", dtypes, pool_shape, dev)
+            pool = pool.data_ptr()
+    if len(pool_shape) != 3:
+        raise HelixError(INVALID_ARGUMENT, "pool must have shape [blocks, tokens, latent + 64]")
+    return pool, pool_shape
+
+
+def latent_append(latent, rope_key, pool, starts, slots, cosine, sine, query=None, query_out=None,
+                  layout="pairs", token_counts=None, stream=None, pool_shape=None,
+                  page_dtype="f32", page_scale=1.0):
+    """Append a step's rows to a latent cache, pages [N, 16, latent + 64] of
+    page_dtype (or a raw address with pool_shape): latent [B, T, latent], and rope_key
+    [B, T, 64] rotated behind it.  query [B, Hq, T, 64], the rotated part of the
+    queries, goes to query_out, which may be the last part of the absorbed queries
+    ([B, Hq, T, latent + 64][..., latent:]).  The rest as rope_append."""
+    import torch
+    shape = getattr(latent, "shape", ())
+    if len(shape) != 3:
+        raise HelixError(INVALID_ARGUMENT, "latent must have shape [batch, tokens, latent]")
+    if (query is None) != (query_out is None):
+        raise HelixError(INVALID_ARGUMENT, "query and query_out go together")
+    b, t, n = shape
+    dev = latent.device
+    rows = (*_rows(latent, "latent", (b, t, n)),
+            *_rows(rope_key, "rope_key", (b, t, LATENT_ROPE), dev))
+    hq = query.shape[1] if query is not None and query.dim() == 4 else 0
+    q = (b, hq, t, LATENT_ROPE)
+    rows += (*_optional_rows(query, "query", q, dev),
+             *_optional_rows(query_out, "query_out", q, dev))
+    pages, (blocks, p, width) = _latent_pool(pool, pool_shape, page_dtype, dev)
+    if width != n + LATENT_ROPE:
+        raise HelixError(INVALID_ARGUMENT, "pages must hold rows of latent + 64 elements")
+    _require_tensor(slots, "slots", (torch.int64,), (b, t), dev)
+    _require_tensor(starts, "starts", (torch.int32,), (b,), dev)
+    if token_counts is not None:
+        _require_tensor(token_counts, "token_counts", (torch.int32,), (b,), dev)
+    table_rows, _ = _rope_cache(cosine, sine, LATENT_ROPE, dev)
+    order = _layout(layout)
+    with _on(dev):
+        check(_lib().helix_paged_latent_append(
+            *rows, b, hq, t, n, pages, blocks, p, slots.data_ptr(), starts.data_ptr(),
+            _address(token_counts), cosine.data_ptr(), sine.data_ptr(), table_rows,
+            order, _PAGE_DTYPES[page_dtype], page_scale, _device_stream(stream, dev)))
+
+
+def latent_workspace_bytes(batch, q_heads, tokens, latent=512):
+    out = ctypes.c_size_t()
+    check(_lib().helix_paged_latent_workspace_bytes(batch, q_heads, tokens, latent,
+                                                    ctypes.byref(out)))
+    return out.value
+
+
+def latent_workspace(batch, q_heads, tokens, latent=512, device="cuda:0"):
+    """A workspace for paged_latent_attention (torch uint8 tensor; no initial
+    value needed).  Calls that overlap need one each."""
+    import torch
+    n = latent_workspace_bytes(batch, q_heads, tokens, latent)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def paged_latent_attention(query, pool, tables, lengths, output, workspace, scale,
+                           token_counts=None, stream=None, pool_shape=None, page_dtype="f32",
+                           page_scale=1.0):
+    """Attention over a latent cache, absorbed form: query [B, Hq, T, latent + 64],
+    output [B, Hq, T, latent] (any strides of four elements but the last); pages [N,
+    16, latent + 64] tensors (or a raw address with pool_shape) of page_dtype; tables
+    [B, max_blocks] int32/uint32; lengths [B] int32 tokens in the pages, the step's
+    own (token_counts [B] int32, or T) the last: row t sees the first lengths[b] -
+    token_counts[b] + t + 1.  scale multiplies the scores.  Rows that see nothing are
+    0; rows of `output` behind token_counts stay as they were."""
+    import torch
+    shape = getattr(query, "shape", ())
+    if len(shape) != 4:
+        raise HelixError(INVALID_ARGUMENT, "query must have shape [batch, q_heads, tokens, dim]")
+    b, hq, t, width = shape
+    dev = query.device
+    pages, (blocks, p, w) = _latent_pool(pool, pool_shape, page_dtype, dev)
+    if w != width or width <= LATENT_ROPE:
+        raise HelixError(INVALID_ARGUMENT, "query and pages must have rows of latent + 64 elements")
+    n = width - LATENT_ROPE
+    q = _rows(query, "query", shape)
+    o = _rows(output, "output", (b, hq, t, n), dev)
+    i32 = (torch.int32,)
+    shape = getattr(tables, "shape", ())
+    max_blocks = shape[1] if len(shape) == 2 else None
+    _require_tensor(tables, "tables", (torch.int32, torch.uint32), (b, max_blocks), dev)
+    _require_tensor(lengths, "lengths", i32, (b,), dev)
+    if token_counts is not None:
+        _require_tensor(token_counts, "token_counts", i32, (b,), dev)
+    _require_tensor(workspace, "workspace", (workspace.dtype,), (workspace.numel(),), dev)
+    with _on(dev):
+        check(_lib().helix_paged_latent_attention(
+            *q, b, hq, t, n, pages, blocks, p, tables.data_ptr(), max_blocks, lengths.data_ptr(),
+            _address(token_counts), *o, scale, workspace.data_ptr(), workspace.nbytes,
+            _PAGE_DTYPES[page_dtype], page_scale, _device_stream(stream, dev)))
+
+
+def latent_prefill_workspace_bytes(batch, heads, tokens, keys):
+    out = ctypes.c_size_t()
+    check(_lib().helix_latent_prefill_workspace_bytes(batch, heads, tokens, keys,
+                                                      ctypes.byref(out)))
+    return out.value
+
+
+def latent_prefill_workspace(batch, heads, tokens, keys, device="cuda:0"):
+    """A workspace for latent_prefill_attention (torch uint8 tensor; no initial
+    value needed).  Calls that overlap need one each."""
+    import torch
+    n = latent_prefill_workspace_bytes(batch, heads, tokens, keys)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def latent_prefill_attention(query, key, rope_key, value, output, workspace, scale,
+                             key_lengths=None, token_counts=None, stream=None):
+    """Attention of a latent cache's prompts, expanded form: query [B, H, T, 128 +
+    64], key and value [B, H, S, 128], rope_key [B, S, 64] shared by the heads, output
+    [B, H, T, 128] (any strides of four elements but the last).  Sequence b has
+    key_lengths[b] keys (int32; None: S), its token_counts[b] new tokens' (int32;
+    None: T) the last: row t sees the first key_lengths[b] - token_counts[b] + t + 1.
+    Rows that see nothing are 0; rows of `output` behind token_counts stay as they
+    were."""
+    import torch
+    qs, ks = getattr(query, "shape", ()), getattr(key, "shape", ())
+    if len(qs) != 4 or len(ks) != 4:
+        raise HelixError(INVALID_ARGUMENT,
+                         "query and key must have shape [batch, heads, tokens, dim]")
+    b, h, t, _ = qs
+    s = ks[2]
+    dev = query.device
+    args = (*_rows(query, "query", (b, h, t, LATENT_NOPE + LATENT_ROPE)),
+            *_rows(key, "key", (b, h, s, LATENT_NOPE), dev),
+            *_rows(rope_key, "rope_key", (b, s, LATENT_ROPE), dev),
+            *_rows(value, "value", (b, h, s, LATENT_NOPE), dev))
+    o = _rows(output, "output", (b, h, t, LATENT_NOPE), dev)
+    for x, name in ((key_lengths, "key_lengths"), (token_counts, "token_counts")):
+        if x is not None:
+            _require_tensor(x, name, (torch.int32,), (b,), dev)
+    _require_tensor(workspace, "workspace", (workspace.dtype,), (workspace.numel(),), dev)
+    with _on(dev):
+        check(_lib().helix_latent_prefill_attention(
+            *args, b, h, t, s, _address(key_lengths), _address(token_counts), *o, scale,
+            workspace.data_ptr(), workspace.nbytes, _device_stream(stream, dev)))
+
+
 class DecodeBatch:
     """Batched decode driver over a PagedKvCache (persistent device tables)."""
 
@@ -885,6 +1196,7 @@ class DecodeBatch:
 
     def prepare(self, stream=None):
         check(_lib().helix_decode_batch_prepare(self._h, _stream(stream)))
+        self._tokens = 1
 
     def append_attention_layer(self, layer, query, keys, values, output, stream=None):
         """append_layer + attention_layer in one decode launch (the new token
@@ -896,6 +1208,7 @@ class DecodeBatch:
     def prepare_chunk(self, tokens, stream=None):
         """Reserve `tokens` slots per sequence (chunked prefill step)."""
         check(_lib().helix_decode_batch_prepare_chunk(self._h, tokens, _stream(stream)))
+        self._tokens = tokens
 
     def prefill_layer(self, layer, query, chunk_key, chunk_value, output, stream=None):
         check(_lib().helix_decode_batch_prefill_layer(self._h, layer, _ptr(query),
@@ -920,6 +1233,25 @@ class DecodeBatch:
         length before the step); cosine/sine [rows, dim / 2]."""
         check(_lib().helix_decode_batch_rope(self._h, _ptr(query), _ptr(key), _ptr(cosine),
                                              _ptr(sine), cosine.shape[0], _stream(stream)))
+
+    def rope_append_layer(self, layer, query, keys, values, cosine, sine, query_out, key_out=None,
+                          value_out=None, layout="pairs", rotary_dim=None, stream=None):
+        """rope() and append_layer() in one launch, for chunk steps too: query
+        [batch, q_heads, tokens, dim] (or None) rotated to query_out, keys [batch,
+        kv_heads, tokens, dim] rotated to the step's slots and to key_out, values to
+        theirs and to value_out, each sequence from its length before the step on.
+        Rows may be strided, outputs may be their inputs; key_out and value_out are
+        what attention_layer() or prefill_layer() takes."""
+        import torch
+        dev = torch.device("cuda", self._cache.device)
+        t = getattr(self, "_tokens", 0)
+        rows = _append_rows(self.batch, self.q_heads, self._cache.kv_heads, t,
+                            self._cache.head_dimension, query, keys, values, query_out, key_out,
+                            value_out, dev)
+        table_rows, rotary = _rope_cache(cosine, sine, rotary_dim, dev)
+        check(_lib().helix_decode_batch_rope_append_layer(
+            self._h, layer, *rows, cosine.data_ptr(), sine.data_ptr(), table_rows, rotary,
+            _layout(layout), _device_stream(stream, dev)))
 
     def attention_layer(self, layer, query, tail_key, tail_value, output, stream=None):
         check(_lib().helix_decode_batch_attention_layer(self._h, layer, _ptr(query),

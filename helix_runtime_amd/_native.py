@@ -18,6 +18,7 @@ c_int = ctypes.c_int
 c_u32 = ctypes.c_uint32
 c_u64 = ctypes.c_uint64
 c_float = ctypes.c_float
+c_double = ctypes.c_double
 vp = ctypes.c_void_p
 
 
@@ -175,6 +176,28 @@ SIGNATURES = {
     "helix_paged_append_path": (
         c_int, [vp, vp, vp, vp, c_size, c_size, c_size, c_size, c_size, c_size, vp, vp, vp,
                 c_size, c_size, c_int, c_float, c_float, vp]),
+    # rotary positions of rows, latent cache
+    "helix_rope_tables": (
+        c_int, [vp, vp, c_size, c_size, c_size, c_double, c_int, c_double, c_double, c_double,
+                c_double, c_double, vp]),
+    "helix_rope_rows": (
+        c_int, [vp, vp, vp, vp, c_size, c_size, c_size, c_size, c_int, c_int, vp, vp, c_size, vp,
+                vp]),
+    "helix_paged_rope_append": (
+        c_int, [vp] * 12 + [c_size] * 5 + [vp, vp, c_size, c_size] + [vp] * 5 +
+               [c_size, c_size, c_int, c_int, c_float, c_float, vp]),
+    "helix_paged_latent_append": (
+        c_int, [vp] * 8 + [c_size] * 4 + [vp, c_size, c_size] + [vp] * 5 +
+               [c_size, c_int, c_int, c_float, vp]),
+    "helix_paged_latent_workspace_bytes": (c_int, [c_size] * 4 + [P(c_size)]),
+    "helix_paged_latent_attention": (
+        c_int, [vp, vp, c_size, c_size, c_size, c_size, vp, c_size, c_size, vp, c_size, vp, vp,
+                vp, vp, c_float, vp, c_size, c_int, c_float, vp]),
+    "helix_latent_prefill_workspace_bytes": (c_int, [c_size] * 4 + [P(c_size)]),
+    "helix_latent_prefill_attention": (
+        c_int, [vp] * 8 + [c_size] * 4 + [vp] * 4 + [c_float, vp, c_size, vp]),
+    "helix_decode_batch_rope_append_layer": (
+        c_int, [vp, c_size] + [vp] * 14 + [c_size, c_size, c_int, vp]),
     "helix_decode_batch_prepare_tree": (c_int, [vp, c_size, vp]),
     "helix_decode_batch_tree_layer": (c_int, [vp, c_size, vp, vp, vp, vp, vp, vp, vp]),
     "helix_decode_batch_commit_path": (c_int, [vp, vp, vp, vp, vp, vp]),

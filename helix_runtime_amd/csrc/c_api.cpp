@@ -5,15 +5,19 @@
 
 #include "block_manager.hpp"
 #include "kernels.hpp"
+#include "latent.hpp"
 #include "paged_cache.hpp"
 #include "prefix_cache.hpp"
+#include "rope.hpp"
 #include "status.hpp"
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -1608,6 +1612,597 @@ int helix_prefix_cache_create(helix_paged_cache* cache, const helix_prefix_confi
     require_out(out);
     *out = new helix_prefix_cache(std::make_unique<helix::PrefixCache>(
         std::make_unique<DeviceAnchors>(cache->cache.state()), to_prefix_config(config)));
+  });
+}
+
+}  // extern "C"
+
+// ------------------------------------- rotary positions, latent cache ----
+namespace {
+
+using helix::hip::RopeRowsArgs;
+using helix::hip::Rows;
+
+// Rows [batch, heads, tokens, dim] as an argument: at p, fp32.
+struct RowsView {
+  const float* p = nullptr;
+  Rows at;
+  std::size_t batch = 0, heads = 0, tokens = 0, dim = 0;
+
+  [[nodiscard]] bool empty() const {
+    return p == nullptr || batch == 0 || heads == 0 || tokens == 0 || dim == 0;
+  }
+  // Elements from the first to behind the last.
+  [[nodiscard]] std::size_t span() const {
+    return empty() ? 0
+                   : (batch - 1) * at.batch + (heads - 1) * at.head + (tokens - 1) * at.token + dim;
+  }
+  // The three dimensions as (extent, stride) pairs.
+  struct Dim {
+    std::size_t n, stride;
+  };
+  [[nodiscard]] std::array<Dim, 3> dims() const {
+    return {Dim{batch, at.batch}, Dim{heads, at.head}, Dim{tokens, at.token}};
+  }
+};
+
+// strides {batch, head, token}, or with `shared` {batch, token} of rows without
+// heads; null: contiguous.  Bounds that keep every offset in 64 bits.
+RowsView rows_view(const char* op, const float* p, const std::size_t* strides, std::size_t batch,
+                   std::size_t heads, std::size_t tokens, std::size_t dim, bool shared = false) {
+  constexpr std::size_t kMost = std::size_t{1} << 40;
+  RowsView v{p, {}, batch, heads, tokens, dim};
+  if (strides == nullptr) {
+    v.at = Rows{mul(mul(heads, tokens), dim), mul(tokens, dim), dim};
+  } else if (shared) {
+    v.at = Rows{strides[0], 0, strides[1]};
+  } else {
+    v.at = Rows{strides[0], strides[1], strides[2]};
+  }
+  for (const auto& d : v.dims()) {
+    check(d.n <= 1 || (d.stride <= kMost && d.n - 1 <= kMost / std::max<std::size_t>(d.stride, 1)),
+          Status::kInvalidArgument, op, "strides out of range");
+  }
+  // (A dimension of one row may have any stride.)
+  if (batch <= 1) v.at.batch = 0;
+  if (heads <= 1) v.at.head = 0;
+  if (tokens <= 1) v.at.token = 0;
+  return v;
+}
+
+// Whether no two rows of v share an element.
+bool rows_apart(const RowsView& v) {
+  auto d = v.dims();
+  std::sort(d.begin(), d.end(), [](const auto& x, const auto& y) { return x.stride < y.stride; });
+  std::size_t inner = v.dim;  // extent of the dimensions before
+  for (const auto& x : d) {
+    if (x.n <= 1) continue;
+    if (x.stride < inner) return false;
+    inner = (x.n - 1) * x.stride + inner;
+  }
+  return true;
+}
+
+bool same_rows(const RowsView& a, const RowsView& b) {
+  return a.p == b.p && a.batch == b.batch && a.heads == b.heads && a.tokens == b.tokens &&
+         a.dim == b.dim && a.at.batch == b.at.batch && a.at.head == b.at.head &&
+         a.at.token == b.at.token;
+}
+
+// Whether two sets of rows may share elements.  Rows of one buffer share none
+// where both repeat at the same strides and lie apart within a period: the heads
+// of a projection's output, or parts of a head.
+bool rows_overlap(const RowsView& a, const RowsView& b) {
+  if (!overlap(a.p, a.span() * sizeof(float), b.p, b.span() * sizeof(float))) return false;
+  const auto lo = std::min(reinterpret_cast<std::uintptr_t>(a.p), reinterpret_cast<std::uintptr_t>(b.p));
+  const auto hi = std::max(reinterpret_cast<std::uintptr_t>(a.p), reinterpret_cast<std::uintptr_t>(b.p));
+  if ((hi - lo) % sizeof(float) != 0) return true;
+  const RowsView& first = lo == reinterpret_cast<std::uintptr_t>(a.p) ? a : b;
+  const RowsView& second = &first == &a ? b : a;
+  const std::size_t off = (hi - lo) / sizeof(float);
+  const auto da = first.dims(), db = second.dims();
+  for (std::size_t i = 0; i < 6; ++i) {  // (the period may be a stride of either)
+    const auto& of = i < 3 ? da[i] : db[i - 3];
+    const std::size_t period = of.stride;
+    if (of.n <= 1 || period == 0) continue;
+    auto extent = [&](const std::array<RowsView::Dim, 3>& d, std::size_t dim, bool& fits) {
+      std::size_t n = dim;
+      for (const auto& x : d) {
+        if (x.n <= 1) continue;
+        if (x.stride < period) {
+          n += (x.n - 1) * x.stride;
+        } else {
+          fits = fits && x.stride % period == 0;
+        }
+      }
+      fits = fits && n <= period;
+      return n;
+    };
+    bool fits = true;
+    const std::size_t ea = extent(da, first.dim, fits), eb = extent(db, second.dim, fits);
+    const std::size_t at = off % period;
+    if (fits && at >= ea && at + eb <= period) return false;
+  }
+  return true;
+}
+
+void check_rows_output(const char* op, const RowsView& out) {
+  check(rows_apart(out), Status::kInvalidArgument, op, "output rows share elements");
+}
+
+// No output overlaps rows of another argument, and its own input (null: none) only
+// by being it.
+struct RowsPair {
+  RowsView in, out;
+};
+void check_rows_apart(const char* op, std::initializer_list<RowsPair> pairs) {
+  for (auto i = pairs.begin(); i != pairs.end(); ++i) {
+    if (i->out.empty()) continue;
+    check_rows_output(op, i->out);
+    for (auto j = pairs.begin(); j != pairs.end(); ++j) {
+      const bool own = i == j;
+      check((j->in.empty() || (own && same_rows(i->out, j->in)) || !rows_overlap(i->out, j->in)) &&
+                (j->out.empty() || own || !rows_overlap(i->out, j->out)),
+            Status::kInvalidArgument, op,
+            "outputs must not share elements with other rows of the call");
+    }
+  }
+}
+
+bool clear_of(const RowsView& v, const void* p, std::size_t bytes) {
+  return v.empty() || !overlap(v.p, v.span() * sizeof(float), p, bytes);
+}
+
+helix::hip::RopeStream rope_stream(const RowsView& in, const RowsView& out, std::size_t rotary) {
+  helix::hip::RopeStream s{};
+  s.in = in.p;
+  s.in_at = in.at;
+  s.out = const_cast<float*>(out.p);
+  s.out_at = out.at;
+  s.heads = in.heads;
+  s.dim = in.dim;
+  s.rotary = rotary;
+  return s;
+}
+
+// The rotation itself: tables, layout.
+void set_rope_tables(const char* op, RopeRowsArgs& a, const float* cosine, const float* sine,
+                     std::size_t cache_rows, std::size_t head_dim, std::size_t rotary_dim,
+                     int layout) {
+  check(head_dim != 0 && head_dim % 2 == 0 && head_dim <= (std::size_t{1} << 24),
+        Status::kInvalidArgument, op, "head dimension must be positive and even");
+  check(rotary_dim != 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim, Status::kInvalidArgument,
+        op, "rotary dimension must be positive, even and at most the head dimension");
+  check(layout == HELIX_ROPE_PAIRS || layout == HELIX_ROPE_HALVES, Status::kInvalidArgument, op,
+        "layout must be HELIX_ROPE_PAIRS or HELIX_ROPE_HALVES");
+  check(cache_rows != 0 && cache_rows <= (std::size_t{1} << 40), Status::kInvalidArgument, op,
+        "tables have no rows, or too many");
+  a.cosine = cosine;
+  a.sine = sine;
+  a.table_rows = cache_rows;
+  a.pairs = rotary_dim / 2;
+  a.layout = static_cast<helix::hip::RopeLayout>(layout);
+}
+
+void check_tables_clear(const char* op, const RopeRowsArgs& a, const RowsView& out) {
+  const std::size_t bytes = mul(mul(a.table_rows, a.pairs), sizeof(float));
+  check(clear_of(out, a.cosine, bytes) && clear_of(out, a.sine, bytes), Status::kInvalidArgument,
+        op, "outputs must not alias the tables");
+}
+
+void check_pool(const char* op, std::size_t physical_blocks, std::size_t block_tokens) {
+  check(physical_blocks != 0 && physical_blocks <= std::numeric_limits<std::uint32_t>::max(),
+        Status::kInvalidArgument, op, "physical block count out of range");
+  check(block_tokens != 0 && block_tokens <= (std::size_t{1} << 20), Status::kInvalidArgument, op,
+        "page size out of range");
+}
+
+// Everything of a rope append but the pools, slots and positions.
+RopeRowsArgs rope_append_args(const char* op, const float* query, const size_t* query_strides,
+                              const float* keys, const size_t* key_strides, const float* values,
+                              const size_t* value_strides, float* query_out,
+                              const size_t* query_out_strides, float* key_out,
+                              const size_t* key_out_strides, float* value_out,
+                              const size_t* value_out_strides, std::size_t batch,
+                              std::size_t q_heads, std::size_t kv_heads, std::size_t tokens,
+                              std::size_t head_dim, const float* cosine, const float* sine,
+                              std::size_t cache_rows, std::size_t rotary_dim, int layout) {
+  RopeRowsArgs a{};
+  set_rope_tables(op, a, cosine, sine, cache_rows, head_dim, rotary_dim, layout);
+  check(kv_heads != 0 && kv_heads <= 0xffffffu && q_heads <= 0xffffffu &&
+            batch <= 0x7fffffffu && tokens <= 0x7fffffffu,
+        Status::kInvalidArgument, op, "rows out of range");
+  check(keys && values && cosine && sine && (query == nullptr) == (query_out == nullptr),
+        Status::kInvalidArgument, op, "device pointers must be non-null (query with query_out)");
+  const RowsView q = rows_view(op, query, query_strides, batch, q_heads, tokens, head_dim);
+  const RowsView k = rows_view(op, keys, key_strides, batch, kv_heads, tokens, head_dim);
+  const RowsView v = rows_view(op, values, value_strides, batch, kv_heads, tokens, head_dim);
+  const RowsView qo = rows_view(op, query_out, query_out_strides, batch, q_heads, tokens, head_dim);
+  const RowsView ko = rows_view(op, key_out, key_out_strides, batch, kv_heads, tokens, head_dim);
+  const RowsView vo = rows_view(op, value_out, value_out_strides, batch, kv_heads, tokens, head_dim);
+  check_rows_apart(op, {{q, qo}, {k, ko}, {v, vo}});
+  for (const RowsView* out : {&qo, &ko, &vo}) check_tables_clear(op, a, *out);
+  a.batch = batch;
+  a.tokens = tokens;
+  if (query != nullptr && q_heads != 0) a.streams[a.count++] = rope_stream(q, qo, rotary_dim);
+  a.streams[a.count++] = rope_stream(k, ko, rotary_dim);
+  a.streams[a.count++] = rope_stream(v, vo, 0);
+  check(helix::hip::rope_rows_fit(a), Status::kOutOfRange, op, "too many elements for one launch");
+  return a;
+}
+
+helix::hip::PageFormat row_format(int page_dtype, float scale, const char* op) {
+  return page_format(page_dtype, scale, scale, op);
+}
+
+void check_moved_by_four(const char* op, const RowsView& v) {
+  check(aligned16(v.p) && v.at.batch % 4 == 0 && v.at.head % 4 == 0 && v.at.token % 4 == 0,
+        Status::kInvalidArgument, op, "rows must lie on 16 bytes, with strides of four elements");
+}
+
+void check_latent_shape(const char* op, std::size_t batch, std::size_t q_heads, std::size_t tokens,
+                        std::size_t latent) {
+  check(helix::hip::latent_dim_supported(latent), Status::kUnsupported, op,
+        "the latent part must have 256 or 512 elements");
+  check(batch <= (std::size_t{1} << 20) && q_heads <= (std::size_t{1} << 16) &&
+            tokens <= (std::size_t{1} << 20) && mul(q_heads, tokens) <= (std::size_t{1} << 24),
+        Status::kInvalidArgument, op, "batch, heads or tokens out of range");
+}
+
+void check_expanded_shape(const char* op, std::size_t batch, std::size_t heads, std::size_t tokens,
+                          std::size_t keys) {
+  check(batch <= (std::size_t{1} << 20) && heads <= (std::size_t{1} << 16) &&
+            tokens <= (std::size_t{1} << 24) && keys <= (std::size_t{1} << 24) &&
+            mul(mul(batch, heads), std::max(tokens, keys)) <= (std::size_t{1} << 31),
+        Status::kInvalidArgument, op, "batch, heads, tokens or keys out of range");
+}
+
+}  // namespace
+
+extern "C" {
+
+int helix_rope_tables(float* cosine, float* sine, size_t rows, size_t first_position,
+                      size_t rotary_dim, double base, int scaling, double factor,
+                      double original_length, double low, double high, double amplitude,
+                      helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "rope_tables";
+    check(rotary_dim != 0 && rotary_dim % 2 == 0 && rotary_dim <= (std::size_t{1} << 20),
+          Status::kInvalidArgument, op, "rotary dimension must be positive and even");
+    check(scaling >= HELIX_ROPE_SCALE_NONE && scaling <= HELIX_ROPE_SCALE_BANDS,
+          Status::kInvalidArgument, op, "unknown scaling");
+    check(std::isfinite(base) && base > 1.0 && std::isfinite(factor) && factor >= 1.0 &&
+              std::isfinite(amplitude),
+          Status::kInvalidArgument, op, "base must be above 1, factor 1 at least, all finite");
+    check(scaling != HELIX_ROPE_SCALE_NTK || rotary_dim > 2, Status::kInvalidArgument, op,
+          "this scaling needs more than one pair");
+    check((scaling != HELIX_ROPE_SCALE_RAMP && scaling != HELIX_ROPE_SCALE_BANDS) ||
+              (std::isfinite(original_length) && original_length > 0.0 && low > 0.0 &&
+               std::isfinite(high) && low < high),
+          Status::kInvalidArgument, op,
+          "this scaling needs a positive original length and 0 < low < high");
+    constexpr std::size_t kMost = std::size_t{1} << 31;
+    check(rows <= kMost && first_position <= kMost - rows, Status::kOutOfRange, op,
+          "positions must stay below 2^31");
+    if (rows == 0) return;
+    check(cosine && sine, Status::kInvalidArgument, op, "device pointers must be non-null");
+    const std::size_t bytes = mul(mul(rows, rotary_dim / 2), sizeof(float));
+    check(!overlap(cosine, bytes, sine, bytes), Status::kInvalidArgument, op,
+          "the tables must not overlap");
+    check(bytes / 64 <= (std::size_t{1} << 38), Status::kOutOfRange, op,
+          "too many elements for one launch");
+    helix::hip::RopeTableArgs a{};
+    a.cosine = cosine;
+    a.sine = sine;
+    a.rows = rows;
+    a.first_position = first_position;
+    a.rotary_dim = rotary_dim;
+    a.base = base;
+    a.scaling = static_cast<helix::hip::RopeScaling>(scaling);
+    a.factor = factor;
+    a.original_length = original_length;
+    a.low = low;
+    a.high = high;
+    a.amplitude = amplitude;
+    helix::hip_check(helix::hip::launch_rope_tables(a, as_stream(stream)), op);
+  });
+}
+
+int helix_rope_rows(const float* input, const size_t* input_strides, float* output,
+                    const size_t* output_strides, size_t tokens, size_t vectors, size_t head_dim,
+                    size_t rotary_dim, int layout, int inverse, const float* cosine,
+                    const float* sine, size_t cache_rows, const int32_t* positions,
+                    helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "rope_rows";
+    RopeRowsArgs a{};
+    set_rope_tables(op, a, cosine, sine, cache_rows, head_dim, rotary_dim, layout);
+    check(tokens <= 0x7fffffffu && vectors <= 0xffffffu, Status::kInvalidArgument, op,
+          "rows out of range");
+    if (tokens == 0 || vectors == 0) return;
+    check(input && output && cosine && sine, Status::kInvalidArgument, op,
+          "device pointers must be non-null");
+    // strides {token, vector}; contiguous [tokens, vectors, head_dim].
+    auto view = [&](const float* p, const size_t* strides) {
+      const std::size_t token = strides != nullptr ? strides[0] : mul(vectors, head_dim);
+      const std::size_t s[3] = {0, strides != nullptr ? strides[1] : head_dim, token};
+      return rows_view(op, p, s, 1, vectors, tokens, head_dim);
+    };
+    const RowsView in = view(input, input_strides), out = view(output, output_strides);
+    check_rows_apart(op, {{in, out}});
+    check_tables_clear(op, a, out);
+    a.batch = 1;
+    a.tokens = tokens;
+    a.positions = positions;
+    a.inverse = inverse != 0;
+    a.streams[a.count++] = rope_stream(in, out, rotary_dim);
+    check(helix::hip::rope_rows_fit(a), Status::kOutOfRange, op, "too many elements for one launch");
+    helix::hip_check(helix::hip::launch_rope_rows(a, as_stream(stream)), op);
+  });
+}
+
+int helix_paged_rope_append(const float* query, const size_t* query_strides, const float* keys,
+                            const size_t* key_strides, const float* values,
+                            const size_t* value_strides, float* query_out,
+                            const size_t* query_out_strides, float* key_out,
+                            const size_t* key_out_strides, float* value_out,
+                            const size_t* value_out_strides, size_t batch, size_t q_heads,
+                            size_t kv_heads, size_t tokens, size_t head_dim, void* key_blocks,
+                            void* value_blocks, size_t physical_blocks, size_t block_tokens,
+                            const int64_t* slots, const int32_t* starts,
+                            const int32_t* token_counts, const float* cosine, const float* sine,
+                            size_t cache_rows, size_t rotary_dim, int layout, int page_dtype,
+                            float key_scale, float value_scale, helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "paged_rope_append";
+    const helix::hip::PageFormat fmt = page_format(page_dtype, key_scale, value_scale, op);
+    check_pool(op, physical_blocks, block_tokens);
+    if (batch == 0 || tokens == 0) return;
+    RopeRowsArgs a = rope_append_args(
+        op, query, query_strides, keys, key_strides, values, value_strides, query_out,
+        query_out_strides, key_out, key_out_strides, value_out, value_out_strides, batch, q_heads,
+        kv_heads, tokens, head_dim, cosine, sine, cache_rows, rotary_dim, layout);
+    check(key_blocks && value_blocks && slots && starts, Status::kInvalidArgument, op,
+          "device pointers must be non-null");
+    const std::size_t pool = mul(mul(mul(physical_blocks, mul(kv_heads, block_tokens)), head_dim),
+                                 helix::hip::page_element_bytes(fmt.type));
+    check(!overlap(key_blocks, pool, value_blocks, pool), Status::kInvalidArgument, op,
+          "key and value pools must not overlap");
+    for (int i = 0; i < a.count; ++i) {
+      const helix::hip::RopeStream& s = a.streams[i];
+      for (const void* p : {static_cast<const void*>(key_blocks), static_cast<const void*>(value_blocks)}) {
+        check(clear_of(RowsView{s.in, s.in_at, batch, s.heads, tokens, s.dim}, p, pool) &&
+                  clear_of(RowsView{s.out, s.out_at, batch, s.heads, tokens, s.dim}, p, pool),
+              Status::kInvalidArgument, op, "rows must not lie in the pools");
+      }
+    }
+    for (int i = 0; i < 2; ++i) {
+      helix::hip::RopeStream& s = a.streams[a.count - 2 + i];
+      s.pool = i == 0 ? key_blocks : value_blocks;
+      s.pool_row = head_dim;
+      s.scale = i == 0 ? fmt.k_scale : fmt.v_scale;
+    }
+    a.page_type = fmt.type;
+    a.slots = slots;
+    a.starts = starts;
+    a.token_counts = token_counts;
+    a.physical_blocks = physical_blocks;
+    a.block_tokens = block_tokens;
+    helix::hip_check(helix::hip::launch_rope_rows(a, as_stream(stream)), op);
+  });
+}
+
+int helix_paged_latent_append(const float* latent_rows, const size_t* latent_strides,
+                              const float* rope_key, const size_t* rope_key_strides,
+                              const float* query, const size_t* query_strides, float* query_out,
+                              const size_t* query_out_strides, size_t batch, size_t q_heads,
+                              size_t tokens, size_t latent, void* pages, size_t physical_blocks,
+                              size_t block_tokens, const int64_t* slots, const int32_t* starts,
+                              const int32_t* token_counts, const float* cosine,
+                              const float* sine, size_t cache_rows, int layout, int page_dtype,
+                              float page_scale, helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "paged_latent_append";
+    constexpr std::size_t kRope = helix::hip::kLatentRope;
+    const helix::hip::PageFormat fmt = row_format(page_dtype, page_scale, op);
+    check_pool(op, physical_blocks, block_tokens);
+    check(helix::hip::latent_dim_supported(latent) && block_tokens == helix::hip::kLatentPage,
+          Status::kUnsupported, op,
+          "pages must hold 16 tokens, with a latent part of 256 or 512 elements");
+    RopeRowsArgs a{};
+    set_rope_tables(op, a, cosine, sine, cache_rows, kRope, kRope, layout);
+    check(batch <= 0x7fffffffu && tokens <= 0x7fffffffu && q_heads <= 0xffffffu,
+          Status::kInvalidArgument, op, "rows out of range");
+    if (batch == 0 || tokens == 0) return;
+    check(latent_rows && rope_key && cosine && sine && pages && slots && starts &&
+              (query == nullptr) == (query_out == nullptr),
+          Status::kInvalidArgument, op, "device pointers must be non-null (query with query_out)");
+    const RowsView c = rows_view(op, latent_rows, latent_strides, batch, 1, tokens, latent, true);
+    const RowsView r = rows_view(op, rope_key, rope_key_strides, batch, 1, tokens, kRope, true);
+    const RowsView q = rows_view(op, query, query_strides, batch, q_heads, tokens, kRope);
+    const RowsView qo = rows_view(op, query_out, query_out_strides, batch, q_heads, tokens, kRope);
+    check_rows_apart(op, {{q, qo}, {c, {}}, {r, {}}});
+    check_tables_clear(op, a, qo);
+    const std::size_t pool = mul(mul(physical_blocks, block_tokens * (latent + kRope)),
+                                 helix::hip::page_element_bytes(fmt.type));
+    for (const RowsView* v : {&c, &r, &q, &qo}) {
+      check(clear_of(*v, pages, pool), Status::kInvalidArgument, op, "rows must not lie in the pool");
+    }
+    a.batch = batch;
+    a.tokens = tokens;
+    if (query != nullptr && q_heads != 0) a.streams[a.count++] = rope_stream(q, qo, kRope);
+    a.streams[a.count++] = rope_stream(r, RowsView{}, kRope);
+    a.streams[a.count++] = rope_stream(c, RowsView{}, 0);
+    for (int i = 0; i < 2; ++i) {
+      helix::hip::RopeStream& s = a.streams[a.count - 2 + i];
+      s.pool = pages;
+      s.pool_row = latent + kRope;
+      s.pool_from = i == 0 ? latent : 0;
+      s.scale = fmt.k_scale;
+    }
+    check(helix::hip::rope_rows_fit(a), Status::kOutOfRange, op, "too many elements for one launch");
+    a.page_type = fmt.type;
+    a.slots = slots;
+    a.starts = starts;
+    a.token_counts = token_counts;
+    a.physical_blocks = physical_blocks;
+    a.block_tokens = block_tokens;
+    helix::hip_check(helix::hip::launch_rope_rows(a, as_stream(stream)), op);
+  });
+}
+
+int helix_paged_latent_workspace_bytes(size_t batch, size_t q_heads, size_t tokens, size_t latent,
+                                       size_t* out) {
+  return guarded([&] {
+    require_out(out);
+    check_latent_shape("paged_latent_workspace_bytes", batch, q_heads, tokens, latent);
+    *out = helix::hip::latent_workspace_bytes(batch, q_heads, tokens, latent);
+  });
+}
+
+int helix_paged_latent_attention(const float* query, const size_t* query_strides, size_t batch,
+                                 size_t q_heads, size_t tokens, size_t latent, const void* pages,
+                                 size_t physical_blocks, size_t block_tokens,
+                                 const uint32_t* tables, size_t max_blocks, const int32_t* lengths,
+                                 const int32_t* token_counts, float* output,
+                                 const size_t* output_strides, float scale, void* workspace,
+                                 size_t workspace_bytes, int page_dtype, float page_scale,
+                                 helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "paged_latent_attention";
+    const helix::hip::PageFormat fmt = row_format(page_dtype, page_scale, op);
+    check_latent_shape(op, batch, q_heads, tokens, latent);
+    check_pool(op, physical_blocks, block_tokens);
+    check(block_tokens == helix::hip::kLatentPage, Status::kUnsupported, op,
+          "pages must hold 16 tokens");
+    check(max_blocks != 0 && max_blocks <= static_cast<std::size_t>(
+                                               std::numeric_limits<std::int32_t>::max() / 32),
+          Status::kInvalidArgument, op, "max_blocks out of range");
+    check(std::isfinite(scale), Status::kInvalidArgument, op, "scale must be finite");
+    if (batch == 0 || q_heads == 0 || tokens == 0) return;
+    check(query && pages && tables && lengths && output, Status::kInvalidArgument, op,
+          "device pointers must be non-null");
+    check(aligned16(pages), Status::kInvalidArgument, op, "pages must be 16-byte aligned");
+    const std::size_t row = latent + helix::hip::kLatentRope;
+    const RowsView q = rows_view(op, query, query_strides, batch, q_heads, tokens, row);
+    const RowsView o = rows_view(op, output, output_strides, batch, q_heads, tokens, latent);
+    check_moved_by_four(op, q);
+    check_moved_by_four(op, o);
+    check_rows_apart(op, {{q, {}}, {{}, o}});
+    check(workspace != nullptr && aligned16(workspace), Status::kInvalidArgument, op,
+          "workspace must be a non-null 16-byte aligned device pointer");
+    check(workspace_bytes >= helix::hip::latent_workspace_bytes(batch, q_heads, tokens, latent),
+          Status::kInvalidArgument, op, "workspace is too small");
+    const std::size_t pool = mul(mul(physical_blocks, block_tokens * row),
+                                 helix::hip::page_element_bytes(fmt.type));
+    check(clear_of(o, workspace, workspace_bytes) && clear_of(q, workspace, workspace_bytes) &&
+              clear_of(o, pages, pool) && !overlap(pages, pool, workspace, workspace_bytes),
+          Status::kInvalidArgument, op, "output and workspace must not alias other arguments");
+    helix::hip::LatentArgs a{};
+    a.query = query;
+    a.pool = pages;
+    a.tables = tables;
+    a.lengths = lengths;
+    a.token_counts = token_counts;
+    a.out = output;
+    a.query_at = q.at;
+    a.out_at = o.at;
+    a.workspace = workspace;
+    a.batch = batch;
+    a.q_heads = q_heads;
+    a.tokens = tokens;
+    a.latent = latent;
+    a.max_blocks = max_blocks;
+    a.physical_blocks = physical_blocks;
+    a.scale = scale;
+    a.page_type = fmt.type;
+    a.page_scale = fmt.k_scale;
+    check(helix::hip::latent_fits(a), Status::kUnsupported, op,
+          "the block tables span too many keys for one call");
+    helix::hip_check(helix::hip::launch_latent_attention(a, as_stream(stream)), op);
+  });
+}
+
+int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
+                                         size_t* out) {
+  return guarded([&] {
+    require_out(out);
+    check_expanded_shape("latent_prefill_workspace_bytes", batch, heads, tokens, keys);
+    *out = helix::hip::expanded_workspace_bytes(batch, heads, tokens, keys);
+  });
+}
+
+int helix_latent_prefill_attention(const float* query, const size_t* query_strides,
+                                   const float* key, const size_t* key_strides,
+                                   const float* rope_key, const size_t* rope_key_strides,
+                                   const float* value, const size_t* value_strides, size_t batch,
+                                   size_t heads, size_t tokens, size_t keys,
+                                   const int32_t* key_lengths, const int32_t* token_counts,
+                                   float* output, const size_t* output_strides, float scale,
+                                   void* workspace, size_t workspace_bytes, helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "latent_prefill_attention";
+    constexpr std::size_t kNope = helix::hip::kLatentNope, kRope = helix::hip::kLatentRope;
+    check_expanded_shape(op, batch, heads, tokens, keys);
+    check(std::isfinite(scale), Status::kInvalidArgument, op, "scale must be finite");
+    if (batch == 0 || heads == 0 || tokens == 0) return;
+    check(query && output && (keys == 0 || (key && rope_key && value)), Status::kInvalidArgument,
+          op, "device pointers must be non-null");
+    const RowsView q = rows_view(op, query, query_strides, batch, heads, tokens, kNope + kRope);
+    const RowsView k = rows_view(op, key, key_strides, batch, heads, keys, kNope);
+    const RowsView r = rows_view(op, rope_key, rope_key_strides, batch, 1, keys, kRope, true);
+    const RowsView v = rows_view(op, value, value_strides, batch, heads, keys, kNope);
+    const RowsView o = rows_view(op, output, output_strides, batch, heads, tokens, kNope);
+    for (const RowsView* x : {&q, &k, &r, &v, &o}) check_moved_by_four(op, *x);
+    check_rows_apart(op, {{q, {}}, {k, {}}, {r, {}}, {v, {}}, {{}, o}});
+    check(workspace != nullptr && aligned16(workspace), Status::kInvalidArgument, op,
+          "workspace must be a non-null 16-byte aligned device pointer");
+    check(workspace_bytes >= helix::hip::expanded_workspace_bytes(batch, heads, tokens, keys),
+          Status::kInvalidArgument, op, "workspace is too small");
+    for (const RowsView* x : {&q, &k, &r, &v, &o}) {
+      check(clear_of(*x, workspace, workspace_bytes), Status::kInvalidArgument, op,
+            "the workspace must not alias other arguments");
+    }
+    helix::hip::ExpandedArgs a{};
+    a.query = query;
+    a.key = key;
+    a.rope_key = rope_key;
+    a.value = value;
+    a.key_lengths = key_lengths;
+    a.token_counts = token_counts;
+    a.out = output;
+    a.query_at = q.at;
+    a.key_at = k.at;
+    a.rope_at = r.at;
+    a.value_at = v.at;
+    a.out_at = o.at;
+    a.workspace = workspace;
+    a.batch = batch;
+    a.heads = heads;
+    a.tokens = tokens;
+    a.keys = keys;
+    a.scale = scale;
+    helix::hip_check(helix::hip::launch_expanded_attention(a, as_stream(stream)), op);
+  });
+}
+
+int helix_decode_batch_rope_append_layer(
+    helix_decode_batch* b, size_t layer, const float* query, const size_t* query_strides,
+    const float* keys, const size_t* key_strides, const float* values,
+    const size_t* value_strides, float* query_out, const size_t* query_out_strides,
+    float* key_out, const size_t* key_out_strides, float* value_out,
+    const size_t* value_out_strides, const float* cosine, const float* sine, size_t cache_rows,
+    size_t rotary_dim, int layout, helix_stream stream) {
+  return guarded([&] {
+    constexpr const char* op = "decode batch rope append";
+    check(b != nullptr, Status::kInvalidArgument, "decode batch must not be NULL");
+    b->batch->require_ordinary_step(op);
+    const RopeRowsArgs a = rope_append_args(
+        op, query, query_strides, keys, key_strides, values, value_strides, query_out,
+        query_out_strides, key_out, key_out_strides, value_out, value_out_strides,
+        b->batch->batch(), b->batch->q_heads(), b->batch->kv_heads(), b->batch->step_tokens(),
+        b->batch->head_dim(), cosine, sine, cache_rows, rotary_dim, layout);
+    b->batch->rope_append_layer(layer, a, as_stream(stream));
   });
 }
 

@@ -735,6 +735,28 @@ void DecodeBatch::rope(float* query, float* key, const float* cosine, const floa
             "decode batch rope launch");
 }
 
+void DecodeBatch::rope_append_layer(std::size_t layer, hip::RopeRowsArgs a,
+                                    hipStream_t stream) const {
+  const PagedConfig& c = state_->manager.config();
+  require_ordinary_step("decode batch rope append");
+  check(layer < c.layers, Status::kOutOfRange, "decode batch layer is out of range");
+  DeviceGuard guard(state_->device);
+  begin_call(stream, "decode batch rope append");
+  hip::RopeStream& keys = a.streams[a.count - 2];
+  keys.pool = state_->key_pool(layer);
+  keys.scale = state_->page_type.k_scale;
+  hip::RopeStream& values = a.streams[a.count - 1];
+  values.pool = state_->value_pool(layer);
+  values.scale = state_->page_type.v_scale;
+  keys.pool_row = values.pool_row = c.head_dimension;
+  a.page_type = state_->page_type.type;
+  a.slots = slots();
+  a.starts = lengths();
+  a.physical_blocks = c.physical_blocks;
+  a.block_tokens = c.block_tokens;
+  hip_check(hip::launch_rope_rows(a, stream), "decode batch rope append launch");
+}
+
 void DecodeBatch::append_attention_layer(std::size_t layer, const float* query,
                                          const float* keys, const float* values, float* out,
                                          hipStream_t stream) const {

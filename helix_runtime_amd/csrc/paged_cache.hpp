@@ -11,6 +11,7 @@
 
 #include "block_manager.hpp"
 #include "kernels.hpp"
+#include "rope.hpp"
 #include "tree.hpp"
 
 #include <hip/hip_runtime.h>
@@ -207,6 +208,10 @@ public:
   // [cache_rows, dim / 2] tables as the model's rope cache holds them.
   void rope(float* query, float* key, const float* cosine, const float* sine,
             std::size_t cache_rows, hipStream_t stream) const;
+  // rope() and append_layer() in one launch, for chunk steps too: rows of `a`
+  // (its streams: queries if any, keys, values) turned from each sequence's
+  // length before the step on, keys and values to the step's slots.
+  void rope_append_layer(std::size_t layer, hip::RopeRowsArgs a, hipStream_t stream) const;
   void attention_layer(std::size_t layer, const float* query, const float* tail_key,
                        const float* tail_value, float* out, hipStream_t stream,
                        bool fused_append = false) const;
@@ -241,6 +246,8 @@ public:
   // workspace: the batch's own is used).
   void accept_tree(hip::VerifyArgs v, const float* keys, const float* values, hipStream_t stream);
 
+  // A prepared step that is not one of prepare_tree(), or an error.
+  void require_ordinary_step(const char* op) const;
   [[nodiscard]] const std::uint32_t* tables() const;
   [[nodiscard]] const std::int32_t* lengths() const;
   [[nodiscard]] const std::int64_t* slots() const;
@@ -249,6 +256,9 @@ public:
   [[nodiscard]] std::size_t batch() const noexcept { return sequences_.size(); }
   [[nodiscard]] std::size_t q_heads() const noexcept { return q_heads_; }
   [[nodiscard]] std::size_t kv_heads() const noexcept { return state_->manager.config().kv_heads; }
+  [[nodiscard]] std::size_t head_dim() const noexcept {
+    return state_->manager.config().head_dimension;
+  }
   [[nodiscard]] std::size_t step_tokens() const noexcept { return step_tokens_; }
   [[nodiscard]] std::size_t shared_pages() const noexcept { return shared_pages_; }
   // Measurement hook: when set, attention_layer() records this event between
@@ -323,9 +333,8 @@ private:
   [[nodiscard]] bool holds_step(std::size_t i) const;
   void cut(std::size_t i, std::size_t length);
   void drop_tree();
-  // A prepared step that is, or is not, one of prepare_tree().
+  // A prepared step that is one of prepare_tree().
   void require_tree_step(const char* op) const;
-  void require_ordinary_step(const char* op) const;
   void append_path(const float* keys, const float* values, const std::int32_t* path,
                    const std::int32_t* accepted, hipStream_t stream);
   // Checks that the step is prepared and its members still live, and orders

@@ -509,6 +509,149 @@ int helix_paged_append_path(const float* keys, const float* values, void* key_bl
                             const int32_t* accepted, size_t batch, size_t nodes, int page_dtype,
                             float key_scale, float value_scale, helix_stream stream);
 
+/* ----------------------------- rotary positions of rows (extension) ---- */
+/* Which elements of a rotated part turn together: (2 i, 2 i + 1) as helix_rope
+ * turns them, or (i, i + half of the part). */
+typedef enum helix_rope_layout { HELIX_ROPE_PAIRS = 0, HELIX_ROPE_HALVES = 1 } helix_rope_layout;
+
+/* Frequencies f_i = base^(-2 i / rotary_dim), i < rotary_dim / 2, as they are or
+ * changed for contexts longer than the one a model was trained on:
+ *   LINEAR  f_i / factor;
+ *   NTK     with base * factor^(rotary_dim / (rotary_dim - 2));
+ *   RAMP    (1 - w) f_i + w f_i / factor, w growing linearly in i from 0 at
+ *           max(floor(p(high)), 0) to 1 at min(ceil(p(low)), rotary_dim - 1),
+ *           p(turns) = rotary_dim ln(original_length / (2 pi turns)) / (2 ln base):
+ *           the pair that turns so often over the original length;
+ *   BANDS   (1 - w) f_i / factor + w f_i, w growing linearly in the turns of f_i
+ *           over the original length from 0 at low turns to 1 at high. */
+typedef enum helix_rope_scaling {
+  HELIX_ROPE_SCALE_NONE = 0,
+  HELIX_ROPE_SCALE_LINEAR = 1,
+  HELIX_ROPE_SCALE_NTK = 2,
+  HELIX_ROPE_SCALE_RAMP = 3,
+  HELIX_ROPE_SCALE_BANDS = 4
+} helix_rope_scaling;
+
+/* Tables for helix_rope and the calls below: row r of cosine and sine [rows,
+ * rotary_dim / 2] holds amplitude * cos and sin of (first_position + r) f_i,
+ * computed in 64 bits and rounded once.  base > 1, factor >= 1, positions below
+ * 2^31, amplitude finite; original_length > 0 and 0 < low < high for RAMP and BANDS,
+ * rotary_dim > 2 for NTK. */
+int helix_rope_tables(float* cosine, float* sine, size_t rows, size_t first_position,
+                      size_t rotary_dim, double base, int scaling, double factor,
+                      double original_length, double low, double high, double amplitude,
+                      helix_stream stream);
+
+/* In the calls from here on, rows are fp32 [batch, heads, tokens, dim] with strides
+ * in elements for the first three, {batch, head, token}, so that a projection's
+ * output can be given as it lies; strides NULL: contiguous.  The last dimension is
+ * contiguous.  Rows that are written must not share elements with each other or with
+ * other rows of the call; an output may be its own input.  Rows of four-element
+ * groups that lie on 16 bytes are moved 16 bytes at a time, others element by
+ * element.
+ *
+ * Rotates the first rotary_dim elements of rows [tokens, vectors, head_dim]
+ * (strides {token, vector}; the other elements are copied) by table row
+ * positions[t] (NULL: t), rounding as helix_rope does; a position outside [0,
+ * cache_rows) gives NaN in the rotated part.  cosine, sine [cache_rows,
+ * rotary_dim / 2].  inverse != 0 turns back: the transpose, which a gradient takes. */
+int helix_rope_rows(const float* input, const size_t* input_strides, float* output,
+                    const size_t* output_strides, size_t tokens, size_t vectors, size_t head_dim,
+                    size_t rotary_dim, int layout, int inverse, const float* cosine,
+                    const float* sine, size_t cache_rows, const int32_t* positions,
+                    helix_stream stream);
+
+/* Append of a step's new rows with the rotation on the way, in one launch:
+ *   query [batch, q_heads, tokens, head_dim] (NULL: none) rotated to query_out;
+ *   keys [batch, kv_heads, tokens, head_dim] rotated to their pages, and to key_out
+ *   where that is given; values to their pages, and to value_out.
+ * Row (b, t) stands at position starts[b] + t and goes to slots[b * tokens + t] =
+ * block * block_tokens + offset (outside the pool: to no page; two rows of one slot
+ * race).  Rows t >= token_counts[b] (NULL: all tokens) are neither read nor written.
+ * Rounding, page_dtype and scales as helix_rope_rows and
+ * helix_paged_decode_attention_typed.  Any even head size, any page size. */
+int helix_paged_rope_append(const float* query, const size_t* query_strides, const float* keys,
+                            const size_t* key_strides, const float* values,
+                            const size_t* value_strides, float* query_out,
+                            const size_t* query_out_strides, float* key_out,
+                            const size_t* key_out_strides, float* value_out,
+                            const size_t* value_out_strides, size_t batch, size_t q_heads,
+                            size_t kv_heads, size_t tokens, size_t head_dim, void* key_blocks,
+                            void* value_blocks, size_t physical_blocks, size_t block_tokens,
+                            const int64_t* slots, const int32_t* starts,
+                            const int32_t* token_counts, const float* cosine, const float* sine,
+                            size_t cache_rows, size_t rotary_dim, int layout, int page_dtype,
+                            float key_scale, float value_scale, helix_stream stream);
+
+/* ------------------------------------------- latent cache (extension) ---- */
+/* A cache whose pages [physical_blocks, 16, latent + 64] hold one row a token for
+ * all heads: a latent part and a rotated part of 64.  latent 256 or 512; page_dtype
+ * as above with one scale for the whole row.  (helix_block_manager keeps such a
+ * cache's pages, with one kv head.)
+ *
+ * Append: latent rows [batch, tokens, latent] and rope_key rows [batch, tokens, 64]
+ * (strides {batch, token}), the latter rotated, to their slots; query [batch,
+ * q_heads, tokens, 64] (NULL: none), the rotated part of the queries, to query_out,
+ * which may be a part of the absorbed queries' rows.  The rest as
+ * helix_paged_rope_append. */
+int helix_paged_latent_append(const float* latent_rows, const size_t* latent_strides,
+                              const float* rope_key, const size_t* rope_key_strides,
+                              const float* query, const size_t* query_strides, float* query_out,
+                              const size_t* query_out_strides, size_t batch, size_t q_heads,
+                              size_t tokens, size_t latent, void* pages, size_t physical_blocks,
+                              size_t block_tokens, const int64_t* slots, const int32_t* starts,
+                              const int32_t* token_counts, const float* cosine,
+                              const float* sine, size_t cache_rows, int layout, int page_dtype,
+                              float page_scale, helix_stream stream);
+
+/* Attention in the absorbed form: every head's key is a token's row and its value
+ * the row's latent part.
+ *   query [batch, q_heads, tokens, latent + 64], output [batch, q_heads, tokens,
+ *   latent], on 16 bytes with strides of four elements;
+ *   lengths[b] tokens of sequence b lie in the pages of row b of `tables` [batch,
+ *   max_blocks], its token_counts[b] (NULL: tokens) new ones the last: row t sees
+ *   the first lengths[b] - token_counts[b] + t + 1.
+ * scale multiplies the scores.  A row that sees nothing is 0; rows t >=
+ * token_counts[b] are not computed, and outputs there stay as they were.  A length
+ * outside the table, or a page outside the pool among those that hold the
+ * sequence's tokens, makes the sequence's rows NaN, and nothing is read there.
+ * What a row does not see does not reach it, whatever it holds.  Values that are not
+ * finite make the rows that see them NaN, or what the formula says.
+ * HELIX_UNSUPPORTED for other latent or page sizes.  The workspace needs no initial
+ * value; calls that overlap on one workspace race. */
+int helix_paged_latent_workspace_bytes(size_t batch, size_t q_heads, size_t tokens, size_t latent,
+                                       size_t* out);
+int helix_paged_latent_attention(const float* query, const size_t* query_strides, size_t batch,
+                                 size_t q_heads, size_t tokens, size_t latent, const void* pages,
+                                 size_t physical_blocks, size_t block_tokens,
+                                 const uint32_t* tables, size_t max_blocks, const int32_t* lengths,
+                                 const int32_t* token_counts, float* output,
+                                 const size_t* output_strides, float scale, void* workspace,
+                                 size_t workspace_bytes, int page_dtype, float page_scale,
+                                 helix_stream stream);
+
+/* The same attention in the expanded form, for prompts, where each head has its own
+ * keys and values (expanded from the latent rows) beside the shared rotated part:
+ *   query [batch, heads, tokens, 128 + 64], the last 64 rotated;
+ *   key, value [batch, heads, keys, 128]; rope_key [batch, keys, 64] (strides
+ *   {batch, key}); output [batch, heads, tokens, 128];
+ *   sequence b has key_lengths[b] (NULL: keys) keys, its token_counts[b] (NULL:
+ *   tokens) new tokens' the last: row t sees the first key_lengths[b] -
+ *   token_counts[b] + t + 1.
+ * All on 16 bytes with strides of four elements.  Rows that see nothing, rows behind
+ * token_counts, lengths outside [0, keys], values that are not finite and the
+ * workspace as above. */
+int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
+                                         size_t* out);
+int helix_latent_prefill_attention(const float* query, const size_t* query_strides,
+                                   const float* key, const size_t* key_strides,
+                                   const float* rope_key, const size_t* rope_key_strides,
+                                   const float* value, const size_t* value_strides, size_t batch,
+                                   size_t heads, size_t tokens, size_t keys,
+                                   const int32_t* key_lengths, const int32_t* token_counts,
+                                   float* output, const size_t* output_strides, float scale,
+                                   void* workspace, size_t workspace_bytes, helix_stream stream);
+
 /* A decode driver over a cache: persistent device block tables for a fixed
  * set of sequences.  prepare() reserves one slot per sequence (allocating
  * pages), append_layer() writes it, attention_layer() attends over the
@@ -554,6 +697,18 @@ int helix_decode_batch_append_all_layers(helix_decode_batch* b, const float* key
 int helix_decode_batch_rope(helix_decode_batch* b, float* query, float* key,
                             const float* cosine, const float* sine, size_t cache_rows,
                             helix_stream stream);
+/* Rotation and append of a step's rows of one layer, one-token or chunk, in one
+ * launch: helix_paged_rope_append over the batch, each sequence from its length
+ * before the step on, to the step's slots.  Replaces helix_decode_batch_rope and
+ * append_layer(); key_out and value_out are the rows that attention_layer() or
+ * prefill_layer() takes. */
+int helix_decode_batch_rope_append_layer(
+    helix_decode_batch* b, size_t layer, const float* query, const size_t* query_strides,
+    const float* keys, const size_t* key_strides, const float* values,
+    const size_t* value_strides, float* query_out, const size_t* query_out_strides,
+    float* key_out, const size_t* key_out_strides, float* value_out,
+    const size_t* value_out_strides, const float* cosine, const float* sine, size_t cache_rows,
+    size_t rotary_dim, int layout, helix_stream stream);
 int helix_decode_batch_attention_layer(helix_decode_batch* b, size_t layer, const float* query,
                                        const float* tail_key, const float* tail_value,
                                        float* output, helix_stream stream);

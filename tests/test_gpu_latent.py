@@ -1,0 +1,498 @@
+"""Attention over a latent cache on the GPU, absorbed (paged_latent_attention) and
+expanded (latent_prefill_attention), against plain 64-bit forms
+(latent_reference.py), and a run of the operators as a model would make it.
+
+Held to the tolerance of every attention entry point of the library: max-abs 2e-5
+plus rel 1e-4, on the values the pages hold.  (Scores here have a standard
+deviation of about 1.7 and are sums of 576 or 192 products, each rounded to 2^-24:
+their error stays near 2e-6, which outputs of up to 5 take over.)"""
+
+import numpy as np
+import pytest
+import torch
+
+import helix_runtime_amd as hx
+import latent_reference as ref
+import oracle
+
+pytestmark = pytest.mark.gpu
+
+ATOL, RTOL = 2e-5, 1e-4
+P, ROPE = 16, 64
+SCALE = 192 ** -0.5
+PS = 0.037
+DTYPES = ["f32", "bf16", "fp8"]
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to("cuda:0")
+
+
+def host(t):
+    return t.detach().cpu().numpy()
+
+
+def close(got, want):
+    np.testing.assert_allclose(got, want, atol=ATOL, rtol=RTOL)
+
+
+def i32(x):
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda:0")
+
+
+def held(dtype, x):
+    if dtype == "bf16":
+        return oracle.round_bf16(x)
+    if dtype == "fp8":
+        return oracle.round_fp8(x, PS)
+    return x
+
+
+def to_pool(dtype, x):
+    t = dev(x)
+    if dtype == "bf16":
+        return t.to(torch.bfloat16)
+    if dtype == "fp8":
+        by = torch.full((), PS, device="cuda:0")
+        return (t / by).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    return t
+
+
+class Latent:
+    """Scattered pages and queries of one call; slots that hold no token, and pages
+    that no table names, are NaN."""
+
+    def __init__(self, dtype, latent, lengths, hq, t, seed=0, counts=None):
+        rng = self.rng = np.random.default_rng(seed + 31 * hq + t)
+        self.dtype, self.n, self.hq, self.t = dtype, latent, hq, t
+        self.lengths, self.counts = list(lengths), counts
+        b = self.b = len(self.lengths)
+        pages = [(x + P - 1) // P for x in self.lengths]
+        physical = sum(pages) + 3
+        self.rows = [rng.standard_normal((x, latent + ROPE), dtype=np.float32) for x in self.lengths]
+        pool = np.full((physical, P, latent + ROPE), np.nan, np.float32)
+        order = rng.permutation(physical)
+        self.tables = np.full((b, max(1, max(pages)) + 1), 0xffffffff, np.uint32)
+        at = 0
+        for i, n in enumerate(pages):
+            ids = order[at:at + n]
+            at += n
+            self.tables[i, :n] = ids
+            for j in range(n):
+                part = self.rows[i][j * P:(j + 1) * P]
+                pool[ids[j], :len(part)] = part
+        self.pool = to_pool(dtype, pool)
+        self.q = rng.standard_normal((b, hq, t, latent + ROPE), dtype=np.float32)
+
+    def want(self, before=7.0):
+        out = np.full((self.b, self.hq, self.t, self.n), before, np.float64)
+        for i, x in enumerate(self.lengths):
+            count = self.t if self.counts is None else min(max(int(self.counts[i]), 0), self.t)
+            ref.latent_attention(self.q[i], held(self.dtype, self.rows[i]), x, count, SCALE, self.n,
+                                 out[i])
+        return out
+
+    def arguments(self):
+        return dict(query=dev(self.q), pool=self.pool, tables=dev(self.tables.view(np.int32)),
+                    lengths=i32(self.lengths),
+                    output=torch.full((self.b, self.hq, self.t, self.n), 7.0, device="cuda:0"),
+                    workspace=hx.latent_workspace(self.b, self.hq, self.t, self.n), scale=SCALE,
+                    token_counts=None if self.counts is None else i32(self.counts),
+                    page_dtype=self.dtype, **(dict(page_scale=PS) if self.dtype == "fp8" else {}))
+
+    def run(self, **other):
+        d = {**self.arguments(), **other}
+        d["workspace"].fill_(255)  # what an earlier call left is not read
+        hx.paged_latent_attention(**d)
+        torch.cuda.synchronize()
+        return host(d["output"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("latent", [256, 512])
+@pytest.mark.parametrize("hq,t", [(1, 1), (5, 1), (16, 1), (16, 2), (20, 1), (16, 3), (64, 1), (8, 9),
+                                  (128, 1), (3, 33), (100, 2), (16, 16)])
+def test_absorbed_over_rows(device, dtype, latent, hq, t):
+    p = Latent(dtype, latent, [t, t + 1, 33 + t, 200, 517], hq, t)
+    close(p.run(), p.want())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths", [[1], [15], [16], [17], [31], [32], [33], [63], [64], [65], [1000],
+                                     [5000], [3, 1, 2047, 1, 64, 65], list(range(1, 90))])
+def test_absorbed_over_lengths(device, dtype, lengths):
+    p = Latent(dtype, 512, lengths, 16, 1, seed=sum(lengths))
+    close(p.run(), p.want())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,t", [(16, 5), (40, 2), (2, 70)])
+def test_absorbed_rows_that_see_nothing_or_lie_behind(device, dtype, hq, t):
+    """Counts of none, some, more than there are rows, and more than there are
+    tokens: rows without a token are 0, rows behind the count stay."""
+    counts = [t, 0, 1, t // 2, t + 5, -3, t]
+    p = Latent(dtype, 512, [40, 300, 1, 17, 600, 100, t // 2 + 1], hq, t, seed=5, counts=counts)
+    got, want = p.run(), p.want()
+    close(got, want)
+    assert (got[1] == 7).all() and (got[5] == 7).all() and (got[2, :, 1:] == 7).all()
+    none = t - (t // 2 + 1)  # rows of the last sequence before its first token
+    assert (got[6, :, :none] == 0).all() and (want[6, :, :none] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_absorbed_empty_sequences(device, dtype):
+    p = Latent(dtype, 256, [0, 5, 0], 4, 2, counts=[2, 2, 0])
+    got = p.run()
+    close(got, p.want())
+    assert (got[0] == 0).all() and (got[2] == 7).all()
+    p = Latent(dtype, 256, [0], 4, 1)
+    assert (p.run() == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp8"])
+@pytest.mark.parametrize("hq,t", [(16, 4), (4, 40)])
+def test_absorbed_later_tokens_do_not_reach_earlier_rows(device, dtype, hq, t):
+    """The step's second token is NaN in its latent part, the third infinite in its
+    rotated part (fp8: NaN): the first row is as without them, later rows NaN."""
+    p = Latent(dtype, 512, [t, 30 + t, 95], hq, t, seed=9)
+    want = p.want()
+    for i, x in enumerate(p.lengths):
+        page = lambda pos: (int(p.tables[i, pos // P]), pos % P)  # noqa: E731
+        a, b = page(x - t + 1), page(x - t + 2)
+        if dtype == "fp8":
+            p.pool[a[0], a[1], 7] = 0x7f
+            p.pool[b[0], b[1], 520] = 0x7f
+        else:
+            p.pool[a[0], a[1], 7] = float("nan")
+            p.pool[b[0], b[1], 520] = float("inf")
+    got = p.run()
+    close(got[:, :, 0], want[:, :, 0])
+    # (The NaN stands in a score of every row that sees it.)
+    assert np.isnan(got[:, :, 1:]).all()
+
+
+def test_absorbed_special_queries_stay_in_their_rows(device):
+    p = Latent("bf16", 512, [50, 100], 20, 2)
+    want = p.want()
+    p.q[0, 3, 1, 5] = np.nan
+    p.q[1, 17, 0, 570] = np.nan
+    got = p.run()
+    assert np.isnan(got[0, 3, 1]).all() and np.isnan(got[1, 17, 0]).all()
+    got[0, 3, 1], got[1, 17, 0] = want[0, 3, 1], want[1, 17, 0]
+    close(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_absorbed_large_scores(device, dtype):
+    """Queries of which each follows one key: maxima that move far from block to
+    block, and probabilities that are all but one 0."""
+    p = Latent(dtype, 512, [300], 16, 1, seed=2)
+    rows = held(dtype, p.rows[0])
+    for h in range(16):
+        p.q[0, h, 0] = rows[(h * 37) % 300] * np.float32(0.5 + h)
+    got = p.run()
+    # Scores up to 16 * 576 / 13.9 = 660, off by 660 * 2^-22 = 1.6e-4 at most in 32
+    # bits; the weights of keys that matter are off by as much of themselves.
+    np.testing.assert_allclose(got, p.want(), atol=1e-3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_absorbed_bad_lengths_and_pages(device, dtype):
+    """A length past the table, a negative one, and a page outside the pool make
+    their sequence NaN and leave the others."""
+    p = Latent(dtype, 512, [40, 40, 40, 40, 40], 8, 2)
+    want = p.want()
+    d = p.arguments()
+    d["lengths"] = i32([40, -1, d["tables"].shape[1] * P + 1, 40, 40])
+    d["tables"][3, 1] = p.pool.shape[0]
+    hx.paged_latent_attention(**d)
+    got = host(d["output"])
+    assert np.isnan(got[1:4]).all()
+    close(got[[0, 4]], want[[0, 4]])
+
+
+@pytest.mark.parametrize("hq,t", [(16, 1), (20, 3), (64, 2)])
+def test_absorbed_strides(device, hq, t):
+    """Queries as a product over heads leaves them, outputs as the next one takes
+    them, and a buffer with gaps."""
+    p = Latent("bf16", 512, [70, 5, 130], hq, t)
+    q = torch.zeros(hq, 3, t, 600, device="cuda:0")
+    q[..., 12:588] = dev(p.q).transpose(0, 1)
+    out = torch.full((3, t, hq, 520), 7.0, device="cuda:0")
+    got = p.run(query=q.transpose(0, 1)[..., 12:588], output=out.transpose(1, 2)[..., 4:516])
+    close(got, p.want())
+    assert (host(out)[..., :4] == 7).all() and (host(out)[..., 516:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,hq,t", [("bf16", 16, 3), ("fp8", 128, 1), ("f32", 16, 1)])
+def test_absorbed_long_sequences(device, dtype, hq, t):
+    """131071 tokens beside short ones."""
+    p = Latent(dtype, 512, [131071, 3, 70], hq, t)
+    q = p.q[:, :4]  # (the reference takes some of the heads)
+    got = p.run()
+    p.q, p.hq = q, 4
+    close(got[:, :4], p.want())
+
+
+def test_absorbed_calls_are_equal_bit_by_bit(device):
+    p = Latent("bf16", 512, [4000, 17, 900, 2500], 128, 1)
+    first = p.run()
+    for _ in range(3):
+        assert (p.run() == first).all()
+
+
+def test_absorbed_pools_past_32_bits(device):
+    """Pages whose elements lie past 2^32 of the pool."""
+    n = (1 << 32) // (P * 576) + 40
+    pool = torch.zeros(n, P, 576, dtype=torch.uint8, device="cuda:0")
+    p = Latent("fp8", 512, [100, 60], 16, 1)
+    count = p.pool.shape[0]
+    pool[n - count:] = p.pool
+    tables = p.tables.astype(np.int64)
+    tables[tables < count] += n - count
+    got = p.run(pool=pool, tables=dev(tables.astype(np.uint32).view(np.int32)))
+    close(got, p.want())
+
+
+def test_absorbed_captured_and_replayed(device):
+    """Two graphs with a workspace each, replayed side by side and in turns with
+    other lengths and contents, against eager calls."""
+    p, o = Latent("bf16", 512, [700, 40, 3], 16, 2), Latent("fp8", 512, [90, 1000], 128, 1)
+    sets = [x.arguments() for x in (p, o)]
+    graphs = []
+    for d in sets:
+        hx.paged_latent_attention(**d)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            hx.paged_latent_attention(**d)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for i in range(3):
+        for d in sets:
+            d["query"].mul_(-1.1)
+            d["lengths"].sub_(i)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for d, x in zip(sets, (p, o)):
+            e = dict(d, output=torch.full_like(d["output"], 7.0),
+                     workspace=hx.latent_workspace(x.b, x.hq, x.t))
+            hx.paged_latent_attention(**e)
+            torch.cuda.synchronize()
+            assert torch.equal(torch.nan_to_num(e["output"]), torch.nan_to_num(d["output"]))
+
+
+# --------------------------------------------------------------- expanded ----
+class Expanded:
+    def __init__(self, b, h, t, s, seed=0, counts=None, lengths=None):
+        rng = self.rng = np.random.default_rng(seed + t + s)
+        self.shape, self.counts, self.lengths = (b, h, t, s), counts, lengths
+        normal = lambda *x: rng.standard_normal(x, dtype=np.float32)  # noqa: E731
+        self.q, self.k, self.v = normal(b, h, t, 192), normal(b, h, s, 128), normal(b, h, s, 128)
+        self.r = normal(b, s, 64)
+
+    def want(self, before=7.0):
+        b, h, t, s = self.shape
+        out = np.full((b, h, t, 128), before, np.float64)
+        for i in range(b):
+            count = t if self.counts is None else min(max(int(self.counts[i]), 0), t)
+            n = s if self.lengths is None else int(self.lengths[i])
+            ref.expanded_attention(self.q[i], self.k[i], self.r[i], self.v[i], n, count, SCALE,
+                                   out[i])
+        return out
+
+    def arguments(self):
+        b, h, t, s = self.shape
+        return dict(query=dev(self.q), key=dev(self.k), rope_key=dev(self.r), value=dev(self.v),
+                    output=torch.full((b, h, t, 128), 7.0, device="cuda:0"),
+                    workspace=hx.latent_prefill_workspace(b, h, t, s), scale=SCALE,
+                    key_lengths=None if self.lengths is None else i32(self.lengths),
+                    token_counts=None if self.counts is None else i32(self.counts))
+
+    def run(self, **other):
+        d = {**self.arguments(), **other}
+        d["workspace"].fill_(255)
+        hx.latent_prefill_attention(**d)
+        torch.cuda.synchronize()
+        return host(d["output"])
+
+
+@pytest.mark.parametrize("b,h,t,s", [
+    (1, 1, 1, 1), (1, 2, 1, 100), (2, 1, 5, 5), (1, 3, 16, 16), (2, 2, 17, 33), (1, 1, 63, 64),
+    (1, 2, 64, 64), (1, 1, 65, 65), (3, 1, 33, 200), (1, 2, 128, 128), (1, 1, 130, 257), (1, 1, 300, 301),
+    (2, 5, 40, 600)])
+def test_expanded_over_sizes(device, b, h, t, s):
+    p = Expanded(b, h, t, s)
+    close(p.run(), p.want())
+
+
+@pytest.mark.parametrize("t,s", [(70, 70), (33, 150)])
+def test_expanded_ragged(device, t, s):
+    """Counts and key lengths of each sequence: none, one, all; keys behind a
+    sequence's are NaN and reach nothing; rows without a key are 0."""
+    counts = [t, 0, 1, t // 2, t + 5, -3, t]
+    lengths = [s, 0, 1, t // 2 + 3, s, 5, t // 2]
+    p = Expanded(7, 2, t, s, counts=counts, lengths=lengths)
+    for i, n in enumerate(lengths):
+        p.k[i, :, n:], p.v[i, :, n:], p.r[i, n:] = np.nan, np.inf, np.nan
+    got, want = p.run(), p.want()
+    close(got, want)
+    assert (got[1] == 7).all() and (got[5] == 7).all()
+    assert (got[6, :, :t - t // 2] == 0).all()
+
+
+def test_expanded_later_keys_do_not_reach_earlier_rows(device):
+    """NaN, infinities and the type's extremes in keys and values of later tokens."""
+    p = Expanded(1, 2, 70, 100)
+    want = p.want()
+    p.v[0, :, 60, 5], p.k[0, :, 75, 3], p.r[0, 90, 0] = np.inf, np.nan, -np.inf
+    got = p.run()
+    close(got[:, :, :30], want[:, :, :30])
+    assert np.isnan(got[:, :, 45:]).all()
+    assert not np.isfinite(got[:, :, 30:45, 5]).any()
+    p = Expanded(1, 1, 20, 20)
+    want = p.want()
+    p.k[0, :, 15:], p.v[0, :, 15:] = -3.4e38, 3.4e38
+    got = p.run()
+    close(got[:, :, :15], want[:, :, :15])
+
+
+def test_expanded_sizes_of_numbers(device):
+    """Keys and values a thousand times larger and smaller than each other, from
+    block to block and from element to element."""
+    p = Expanded(1, 2, 40, 300)
+    p.v *= np.exp(p.rng.uniform(-7, 7, p.v.shape[:3] + (1,))).astype(np.float32)
+    p.k *= np.exp(p.rng.uniform(-3, 0.5, p.k.shape)).astype(np.float32)
+    got, want = p.run(), p.want()
+    # Outputs are sums of values up to 4000: held to 2^-18 of the largest that a row
+    # weighs, far above 32-bit rounding and far below 16 bits'.
+    assert (np.abs(got - want) <= 2.0 ** -18 * np.abs(p.v).max()).all()
+    assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want)
+
+
+def test_expanded_bad_lengths(device):
+    p = Expanded(4, 2, 10, 30)
+    want = p.want()
+    got = p.run(key_lengths=i32([30, -1, 31, 30]))
+    assert np.isnan(got[1:3]).all()
+    close(got[[0, 3]], want[[0, 3]])
+
+
+def test_expanded_strides(device):
+    """As projections leave queries, keys and values."""
+    b, h, t, s = 2, 3, 50, 90
+    p = Expanded(b, h, t, s)
+    q = dev(p.q.transpose(0, 2, 1, 3))
+    kv = dev(np.concatenate([p.k, p.v], axis=-1).transpose(0, 2, 1, 3))
+    down = torch.zeros(b, s, 512 + 64, device="cuda:0")
+    down[..., 512:] = dev(p.r)
+    out = torch.full((b, t, h, 128), 7.0, device="cuda:0")
+    got = p.run(query=q.transpose(1, 2), key=kv.transpose(1, 2)[..., :128],
+                value=kv.transpose(1, 2)[..., 128:], rope_key=down[..., 512:],
+                output=out.transpose(1, 2))
+    close(got, p.want())
+
+
+def test_expanded_captured_and_replayed(device):
+    p = Expanded(3, 2, 65, 129, counts=[65, 10, 33], lengths=[129, 100, 33])
+    d = p.arguments()
+    hx.latent_prefill_attention(**d)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hx.latent_prefill_attention(**d)
+    for i in range(3):
+        d["query"].mul_(-1.1)
+        d["value"].add_(0.25)
+        d["key_lengths"].sub_(i)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        e = dict(d, output=torch.full_like(d["output"], 7.0),
+                 workspace=hx.latent_prefill_workspace(*p.shape))
+        hx.latent_prefill_attention(**e)
+        torch.cuda.synchronize()
+        assert torch.equal(e["output"], d["output"])
+
+
+# ------------------------------------------------- as a model would run them ----
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_model_layer_over_prompt_and_steps(device, dtype):
+    """One layer of latent attention: a prompt in the expanded form, then steps of one
+    and of three tokens in the absorbed form over the pages that the appends filled,
+    all against a recomputation in 64 bits from the values the pages hold."""
+    h, n, batch = 4, 256, 3
+    rng = np.random.default_rng(11)
+    up_k, up_v = (rng.standard_normal((h, n, 128)).astype(np.float32) / 16 for _ in range(2))
+    cos, sin = (torch.empty(64, 32, device="cuda:0") for _ in range(2))
+    hx.rope_tables(cos, sin, base=10000.0, scaling="bands", factor=4.0, original_length=32)
+    manager = hx.BlockManager(1, 1, n + ROPE, P, 40)
+    pool = to_pool(dtype, np.full((40, P, n + ROPE), np.nan, np.float32))
+    seqs = [manager.create_sequence() for _ in range(batch)]
+    scale = dict(page_scale=PS) if dtype == "fp8" else {}
+    past = [np.zeros((0, n + ROPE)) for _ in range(batch)]
+    hc, hs = host(cos), host(sin)
+
+    for step, counts in enumerate(([20, 7, 1], [1, 1, 1], [3, 0, 2], [1, 1, 1])):
+        t = max(counts)
+        starts = [manager.length(s) for s in seqs]
+        slots = np.full((batch, t), -1, np.int64)
+        for b, s in enumerate(seqs):
+            if counts[b]:
+                slots[b, :counts[b]] = manager.append(s, counts[b])
+        width = max(len(manager.block_table(s)) for s in seqs)
+        tables = np.zeros((batch, width), np.int32)
+        for b, s in enumerate(seqs):
+            table = manager.block_table(s)
+            tables[b, :len(table)] = table
+        latent = rng.standard_normal((batch, t, n), dtype=np.float32)
+        rope_key = rng.standard_normal((batch, t, ROPE), dtype=np.float32)
+        q = rng.standard_normal((batch, t, h, 192), dtype=np.float32)
+        token_counts, dq = i32(counts), dev(q).transpose(1, 2)
+        absorbed = torch.zeros(batch, h, t, n + ROPE, device="cuda:0")
+        for b in range(h):
+            absorbed[:, b, :, :n] = dq[:, b, :, :128] @ dev(up_k[b]).T
+        hx.latent_append(dev(latent), dev(rope_key), pool, i32(starts), dev(slots), cos, sin,
+                         query=dq[..., 128:], query_out=absorbed[..., n:], layout="halves",
+                         token_counts=token_counts, page_dtype=dtype, **scale)
+        # What the pages hold, in 64 bits.
+        for b in range(batch):
+            for j in range(counts[b]):
+                turned = ref.rotate32(rope_key[b, j], hc[starts[b] + j], hs[starts[b] + j], "halves")
+                row = held(dtype, np.concatenate([latent[b, j], turned])[None].astype(np.float32))
+                past[b] = np.concatenate([past[b], row.astype(np.float64)])
+        out = torch.full((batch, h, t, n), 7.0, device="cuda:0")
+        hx.paged_latent_attention(absorbed, pool, dev(tables), i32([len(x) for x in past]), out,
+                                  hx.latent_workspace(batch, h, t, n), SCALE,
+                                  token_counts=token_counts, page_dtype=dtype, **scale)
+        heads = torch.stack([out[:, i] @ dev(up_v[i]) for i in range(h)], dim=1)
+        want = np.zeros((batch, h, t, 128))
+        for b in range(batch):
+            k, v = past[b][:, :n] @ up_k.astype(np.float64), past[b][:, :n] @ up_v.astype(np.float64)
+            turned = np.stack([ref.rotate32(q[b, j, :, 128:], hc[starts[b] + j], hs[starts[b] + j],
+                                            "halves") for j in range(counts[b])] or
+                              [np.zeros((h, ROPE), np.float32)])
+            whole = np.concatenate([q[b, :len(turned), :, :128], turned], axis=-1)
+            ref.expanded_attention(whole.transpose(1, 0, 2), k, past[b][:, n:], v, len(past[b]),
+                                   counts[b], SCALE, want[b])
+        for b in range(batch):
+            # The two products around the attention are fp32 sums of 128 and 256 terms.
+            np.testing.assert_allclose(host(heads)[b, :, :counts[b]], want[b, :, :counts[b]],
+                                       atol=1e-4, rtol=1e-4)
+        if step == 0:
+            rows = torch.zeros(batch, t, n + ROPE, device="cuda:0")
+            for b in range(batch):
+                rows[b, :counts[b]] = dev(past[b].astype(np.float32))
+            key, value = (torch.stack([rows[..., :n] @ dev(u[i]) for i in range(h)], dim=1)
+                          for u in (up_k, up_v))
+            whole = torch.cat([dq[..., :128], absorbed[..., n:]], dim=-1)
+            expanded = torch.zeros(batch, h, t, 128, device="cuda:0")
+            hx.latent_prefill_attention(whole, key, rows[..., n:], value, expanded,
+                                        hx.latent_prefill_workspace(batch, h, t, t), SCALE,
+                                        key_lengths=token_counts, token_counts=token_counts)
+            for b in range(batch):
+                np.testing.assert_allclose(host(expanded)[b, :, :counts[b]],
+                                           want[b, :, :counts[b]], atol=1e-4, rtol=1e-4)
