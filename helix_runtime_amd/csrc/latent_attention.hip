@@ -1,26 +1,79 @@
 // Absorbed attention over a latent cache:
 //
-//   out_ht = sum_j p_j c_j[:L] / sum_j p_j,  p_j = exp(scale q_ht . c_j - m),
+//   out_r = sum_j p_rj c_j[:L] / sum_j p_rj,  p_rj = exp(scale q_r . c_j - m_r),
 //
-// j over the tokens that row t sees, c_j the row of L + 64 elements that every
-// head shares.
+// r over a sequence's query rows (heads times tokens), j over the tokens that row r
+// sees, c_j the row of W = L + 64 elements that every head shares.
 //
-// One wavefront a row: a lane holds every 64th element of the query, of a key and
-// of the output, one pass over the keys.
+// Work split.  16 or 64 of a sequence's rows form a unit; one pass over the
+// sequence's tokens serves them all.  A unit's tokens are tiles of 32 (fp32 pages:
+// 16).  A fixed grid of workgroups takes equal ranges of the flat list of all units'
+// tiles, whatever the lengths.  A unit inside one range is finished there; one that
+// crosses ranges leaves a partial (maximum, sum, output) per range, and
+// latent_merge_kernel joins them.  A workgroup leaves at most two partials, its first
+// unit's and its last one's, so the workspace depends on the grid, not on the batch.
+// Units of the same sequence lie half the list apart (or a third, ..), so that the
+// workgroups that read the same pages do so at one time, on one XCD.
+//
+// Matrix form.  Per tile scores are S^T = C Q^T and outputs O^T += C^T P^T, a
+// wavefront having 16 rows: a lane holds tokens of one query row, so a row's maximum
+// takes two cross-lane steps and its probabilities are an operand as they are.  The
+// tile lies in LDS once, and is read as rows for the scores and transposed for the
+// outputs.  A wavefront's queries and outputs, 16 x W and 16 x L numbers, stay in its
+// registers: 216 and 128 a lane, one wavefront a SIMD.  fp32 factors are sums of
+// 16-bit terms, each product of terms exact in fp32:
+// - bf16 pages: elements are one bf16 term, queries and probabilities three
+//   (24 bits): 3 products;
+// - fp8 pages: codes are exact in fp16, queries and probabilities two fp16 terms (22
+//   bits and a sign: the rounding of an fp32 number): 2 products.  Terms must stay
+//   above fp16's smallest numbers: a query row is scaled by a power of two that puts
+//   its largest element in [2^10, 2^11), and probabilities (with them sums and
+//   outputs) carry a factor of 2^8;
+// - fp32 pages: the fp32 matrix instructions.
+//
+// Units of 64 rows: four wavefronts with 16 rows each share a tile.  Units of 16 rows
+// (what one token of 16 heads is): the wavefronts take tiles in turn, each by
+// itself, and join what they have at the unit's end.
 #include "bf16.hpp"
 #include "fp8.hpp"
 #include "latent.hpp"
+#include "prefill_bmma.hpp"
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 namespace helix::hip {
 namespace {
 
+using prefill_detail::exp2_ratio;
+using prefill_detail::lds_address;
+using prefill_detail::lds_load16_at;
+using prefill_detail::row_max;
+using prefill_detail::row_sum;
+using prefill_detail::uniform_read;
+using prefill_detail::v4f;
+using prefill_detail::v4s;
+using prefill_detail::v8bf;
+
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int P = static_cast<int>(kLatentPage);
+constexpr int kWaves = 4;
+// fp8 pages: the logarithm of the factor on probabilities.
+constexpr float kProbLog = 8.0f;
+// A row's reference stays while no score is above it by more than this (log2
+// units): fp16's largest number is 2^16.
+constexpr float kSlack = 7.0f;
 
 struct LatentKernelArgs {
   const float* query;
@@ -31,98 +84,1083 @@ struct LatentKernelArgs {
   float* out;
   Rows query_at, out_at;
   int batch, q_heads, tokens, max_blocks;
+  int rows;  // query rows of a sequence: q_heads * tokens
   std::uint32_t physical_blocks;
-  float qscale;  // log2(e) * scale
+  float qscale;  // log2(e) * scale, times the pages' scale
   float page_scale;
 };
 
+// A unit to join: the one that a group's range ends without starting it.
+struct LatentJob {
+  int b, rb;       // sequence (-1: none), row block
+  int first, last; // groups whose ranges start and end the unit
+};
+
+struct LatentStream {
+  float* part_o;   // [2 * groups, RB, L]
+  float* part_ml;  // [2 * groups, RB, 2]
+  LatentJob* jobs; // by unit where there are no more units than groups, else by group
+  int groups;
+  int row_blocks;  // units of a sequence
+  int by_unit;
+};
+
+// x = t[0] + t[1] (+ t[2]), each rounded to nearest; two numbers at a time, packed
+// into words.
 template <int PF>
-__device__ __forceinline__ float page_value(const void* pool, std::size_t e, float scale) {
-  if constexpr (PF == 1) {
-    return bf16_value(static_cast<const unsigned short*>(pool)[e]);
-  } else if constexpr (PF == 2) {
-    return fp8_value(static_cast<const unsigned char*>(pool)[e], scale);
+__device__ __forceinline__ void split_pair(float x, float y, unsigned (&t)[3]) {
+  if constexpr (PF == 2) {
+    const v2h hi = __builtin_convertvector((v2f{x, y}), v2h);
+    x -= static_cast<float>(hi[0]);
+    y -= static_cast<float>(hi[1]);
+    t[0] = __builtin_bit_cast(unsigned, hi);
+    t[1] = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2h));
   } else {
-    return static_cast<const float*>(pool)[e];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const v2bf h = __builtin_convertvector((v2f{x, y}), v2bf);
+      t[i] = __builtin_bit_cast(unsigned, h);
+      x -= __uint_as_float(t[i] << 16);
+      y -= __uint_as_float(t[i] & 0xffff0000u);
+    }
   }
 }
 
+template <int PF>
+__device__ __forceinline__ v4f matrix_step(v4u a, v4u b, v4f c) {
+  if constexpr (PF == 2) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
+                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
+                                                   __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+}
+
+// Four words of fp8 codes as fp16 are two of these.
+__device__ __forceinline__ v4u codes_fp16(unsigned w0, unsigned w1) {
+  return v4u{
+      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false)),
+      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true)),
+      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false)),
+      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true))};
+}
+
+// A tile in LDS: rows of kPitch bytes, whose 16-byte chunks are exchanged within
+// groups of kMask + 1 by an exclusive or with `turn` of the row.  A read of one chunk
+// of 16 rows (scores) and one of 32 bytes of 8 rows, or 64 of 4 (outputs), then hit
+// distinct banks: rows lie 1152 or 640 bytes apart, 128 from a multiple of 256, and
+// fp32 rows on one.
 template <int PF, int L>
-__global__ __launch_bounds__(256) void latent_row_kernel(LatentKernelArgs a) {
-  constexpr int W = L + static_cast<int>(kLatentRope);
-  constexpr int NK = W / 64, NV = L / 64;
-  const int lane = threadIdx.x & 63;
-  const long long rows = static_cast<long long>(a.batch) * a.q_heads * a.tokens;
-  const long long r = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int t = static_cast<int>(r % a.tokens);
-  const int h = static_cast<int>(r / a.tokens % a.q_heads);
-  const int b = static_cast<int>(r / a.tokens / a.q_heads);
-  int count = a.tokens;
-  if (a.token_counts != nullptr) count = min(max(a.token_counts[b], 0), a.tokens);
-  if (t >= count) return;
+struct Tile {
+  static constexpr int W = L + static_cast<int>(kLatentRope);
+  static constexpr int kElem = PF == 0 ? 4 : 2;            // bytes in LDS
+  static constexpr int kPageElem = PF == 0 ? 4 : PF == 1 ? 2 : 1;
+  static constexpr int kTokens = PF == 0 ? 16 : 32;
+  static constexpr int kPages = kTokens / P;
+  static constexpr int kPitch = W * kElem;
+  static constexpr int kBytes = kTokens * kPitch;
+  static constexpr unsigned kMask = PF == 0 ? 15 : 7;
+  // Loads of 16 bytes a lane (fp8: 8) come in four groups of kLoads, a group being
+  // 8 whole rows (fp32: 4).
+  static constexpr int kLoads = W / 64;
+  static constexpr int kGroupRows = PF == 0 ? 4 : 8;
+  static_assert(4 * kLoads * 1024 == kBytes && kGroupRows * kPitch == kLoads * 1024);
+  static constexpr std::size_t kPageBytes = static_cast<std::size_t>(P) * W * kPageElem;
+  static __device__ __forceinline__ unsigned turn(int row) {
+    return PF == 0 ? static_cast<unsigned>(row & 15)
+                   : static_cast<unsigned>((row & 6) | ((row >> 3) & 1));
+  }
+};
+
+// A place in the flat list of tiles.
+struct LatentCursor {
+  int b, rb, blk;
+  int length, count, nb;  // the sequence's tokens, its query tokens, tiles
+  int bad;                // its length lies outside its table
+};
+
+__device__ __forceinline__ int clamped_count(const LatentKernelArgs& a, int b) {
+  return a.token_counts != nullptr ? min(max(a.token_counts[b], 0), a.tokens) : a.tokens;
+}
+
+// Tiles of sequence b: one at least where it has rows.
+template <int KT>
+__device__ __forceinline__ int sequence_tiles(const LatentKernelArgs& a, int b) {
+  if (b >= a.batch || clamped_count(a, b) == 0) return 0;
   const int length = a.lengths[b];
-  bool bad = length < 0 || length > a.max_blocks * P;
-  const int seen = bad ? 0 : max(length - count + t + 1, 0);
-  const float* const q = a.query + b * a.query_at.batch + h * a.query_at.head + t * a.query_at.token;
-  float qv[NK], o[NV];
+  if (length < 0 || length > a.max_blocks * P) return 1;
+  return max((length + KT - 1) / KT, 1);
+}
+
+template <int KT>
+__device__ __forceinline__ void load_sequence(const LatentKernelArgs& a, LatentCursor& c) {
+  const int length = uniform_read(a.lengths + c.b);
+  c.bad = length < 0 || length > a.max_blocks * P;
+  c.length = c.bad ? 0 : length;
+  c.count = a.tokens;
+  if (a.token_counts != nullptr) c.count = min(max(uniform_read(a.token_counts + c.b), 0), a.tokens);
+  c.nb = c.count > 0 ? max((c.length + KT - 1) / KT, 1) : 0;
+}
+
+__device__ __forceinline__ long long uniform_long(long long v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
+  const unsigned hi =
+      __builtin_amdgcn_readfirstlane(static_cast<unsigned>(static_cast<unsigned long long>(v) >> 32));
+  return static_cast<long long>(static_cast<unsigned long long>(hi) << 32 | lo);
+}
+
+// Inclusive sums over the wavefront.
+__device__ __forceinline__ long long lane_scan(long long v, int lane) {
+  long long sum = v;
 #pragma unroll
-  for (int i = 0; i < NK; ++i) qv[i] = q[64 * i + lane] * a.qscale;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) o[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < seen; ++j) {
-    const std::uint32_t page = a.tables[static_cast<std::size_t>(b) * a.max_blocks + j / P];
-    if (page >= a.physical_blocks) {
-      bad = true;
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long t = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += t;
+  }
+  return sum;
+}
+
+// This group's range of tiles [g0, g1) (ranges of `each`) and its first place.
+struct LatentRange {
+  long long g0, g1, each;  // (a range's length fits 31 bits: latent_fits)
+};
+template <int KT>
+__device__ __forceinline__ LatentRange first_place(const LatentKernelArgs& a, const LatentStream& st,
+                                                   int group, int least, int lane, LatentCursor& c) {
+  long long per_block = 0;  // tiles of all sequences' units of one row block
+#pragma unroll 4
+  for (int b0 = 0; b0 < a.batch; b0 += 64) per_block += sequence_tiles<KT>(a, b0 + lane);
+  per_block = uniform_long(__shfl(lane_scan(per_block, lane), 63, 64));
+  const long long total = per_block * st.row_blocks;
+  LatentRange r{};
+  r.each = (total + st.groups - 1) / st.groups;
+  r.each = uniform_long(max((r.each + least - 1) / least * least, 1ll));
+  r.g0 = uniform_long(group * r.each);
+  r.g1 = uniform_long(min(r.g0 + r.each, total));
+  if (r.g0 >= r.g1) return r;
+  c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(r.g0 / per_block));
+  const long long rem = r.g0 - c.rb * per_block;
+  long long base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int nb = sequence_tiles<KT>(a, b0 + lane);
+    const long long sum = lane_scan(nb, lane);
+    const long long from = base + sum - nb, to = base + sum;
+    const unsigned long long hit = __ballot(from <= rem && rem < to);
+    if (hit != 0) {
+      const int src = __ffsll(static_cast<long long>(hit)) - 1;
+      c.b = __builtin_amdgcn_readfirstlane(b0 + src);
+      load_sequence<KT>(a, c);
+      c.blk = __builtin_amdgcn_readfirstlane(
+          static_cast<int>(rem - uniform_long(__shfl(from, src, 64))));
       break;
     }
-    const std::size_t e = (static_cast<std::size_t>(page) * P + j % P) * W + lane;
-    float k[NK], x = 0.f;
+    base += uniform_long(__shfl(sum, 63, 64));
+  }
+  return r;
+}
+
+// The next unit's first place; only called where there is one.
+template <int KT>
+__device__ __forceinline__ void next_unit(const LatentKernelArgs& a, LatentCursor& c) {
+  c.blk = 0;
+  do {
+    if (++c.b == a.batch) {
+      c.b = 0;
+      ++c.rb;
+    }
+    load_sequence<KT>(a, c);
+  } while (c.nb == 0);
+}
+
+// One wavefront's 16 rows of a unit: queries, outputs, references and sums, and what
+// a tile in LDS does to them.
+template <int PF, int L>
+struct LatentRows {
+  using T = Tile<PF, L>;
+  static constexpr int QT = PF == 0 ? 1 : PF == 1 ? 3 : 2;  // terms
+  static constexpr int NS = PF == 0 ? T::W / 16 : T::W / 32;  // steps of the scores' sum
+  static constexpr int ND = L / 16;                           // tiles of output dims
+  static constexpr int NH = T::kTokens / 16;                  // 16-token halves
+
+  v4u q[NS][QT];    // fp32 pages: four fp32 numbers
+  v4f o[ND];        // o[dt][i]: dim 16 dt + 4 grp + i of row col
+  float m, l;       // l: the lane's own tokens
+  float unscale;    // fp8 pages: what undoes the row's power of two
+  int limit;        // tokens that row col sees
+  bool live;        // the row is one of the sequence's
+
+  // Row r of the unit's sequence: its head and token.
+  __device__ __forceinline__ void start(const LatentKernelArgs& a, const LatentCursor& c, int row,
+                                        int grp) {
+    live = row < a.rows;
+    const int h = live ? row / a.tokens : 0;
+    const int t = live ? row - h * a.tokens : 0;
+    live = live && t < c.count;
+    limit = c.length - c.count + t + 1;
+    const float* const src = a.query + static_cast<std::size_t>(c.b) * a.query_at.batch +
+                             static_cast<std::size_t>(h) * a.query_at.head +
+                             static_cast<std::size_t>(t) * a.query_at.token;
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      k[i] = page_value<PF>(a.pool, e + 64 * i, a.page_scale);
-      x += qv[i] * k[i];
+    for (int dt = 0; dt < ND; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
+    // (A row that is none reads the sequence's first one.)
+    auto number = [&](int at) {
+      const v4f x = *reinterpret_cast<const v4f*>(src + at);
+      return live ? x : v4f{0.f, 0.f, 0.f, 0.f};
+    };
+    if constexpr (PF == 0) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        q[s][0] = __builtin_bit_cast(v4u, number(16 * s + 4 * grp) * a.qscale);
+        keep(s);
+      }
+    } else {
+      float grow = a.qscale;
+      if constexpr (PF == 2) {
+        float most = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const v4f x = number(32 * s + 8 * grp + 4 * w);
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])),
+                                     fmaxf(fabsf(x[2]), fabsf(x[3]))));
+          }
+        asm volatile("" ::: "memory");  // (or what was read stays in registers)
+        most = row_max(most);
+        // most * 2^(10 - e) in [2^10, 2^11), as far as 2^(10 - e) is a normal number.
+        const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -110), 120);
+        grow = __uint_as_float(static_cast<unsigned>(127 + 10 - e) << 23);
+        unscale = __uint_as_float(static_cast<unsigned>(127 - 10 + e) << 23);
+        // (Positive, or scores of -infinity would not stay that: the score scale's
+        // sign goes with the queries, which a scale of 0 makes 0.)
+        grow = a.qscale > 0.f ? grow : a.qscale < 0.f ? -grow : 0.f;
+        unscale = fmaxf(unscale * fabsf(a.qscale), 1.2e-38f);
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const v4f x[2] = {number(32 * s + 8 * grp), number(32 * s + 8 * grp + 4)};
+        unsigned w[4][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          split_pair<PF>(x[i >> 1][2 * (i & 1)] * grow, x[i >> 1][2 * (i & 1) + 1] * grow, w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < QT; ++i) q[s][i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
+        keep(s);
+      }
+    }
+  }
+
+  // Half a wavefront's registers are accumulation registers, which matrix instructions
+  // can take any operand from: the queries live there, everything else in the others.
+  // (Said here, or the compiler mixes them and moves both to and fro.)
+  __device__ __forceinline__ void keep(int s) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) asm("" : "+a"(q[s][i]));
+    if (s % 6 == 5) __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // Scores of a tile: sc[h][i] is token 16 h + 4 grp + i of row col.  `beside(u)` is
+  // what else the lane does between the matrix instructions of step u of NS * NH.
+  template <typename F>
+  __device__ __forceinline__ void scores(const unsigned char* tile, int col, int grp, v4f (&sc)[NH],
+                                         F&& beside) const {
+    constexpr int N = NS * NH, A = 4;  // operands come out of LDS A steps ahead
+    // Row col's chunk 4 s + grp: its place within a group of chunks is one of two
+    // (fp32 pages: four), by s.
+    constexpr int V = PF == 0 ? 4 : 2;
+    unsigned at[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      at[i] = static_cast<unsigned>(col * T::kPitch) +
+              ((static_cast<unsigned>(4 * i + grp) ^ T::turn(col)) & T::kMask) * 16u;
+    }
+    v4u k[A];
+    auto read = [&](int u) {
+      const int s = u / NH, h = u % NH;
+      // (Rows 16 h and on turn as rows 0 and on do.)
+      k[u % A] = *reinterpret_cast<const v4u*>(tile + at[s % V] + (s / V) * (V * 64) +
+                                               h * (16 * T::kPitch));
+    };
+#pragma unroll
+    for (int u = 0; u < A; ++u) read(u);
+#pragma unroll
+    for (int h = 0; h < NH; ++h) sc[h] = v4f{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int s = u / NH, h = u % NH;
+      if constexpr (PF == 0) {
+        const v4f x = __builtin_bit_cast(v4f, k[u % A]), y = __builtin_bit_cast(v4f, q[s][0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[h], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int i = QT - 1; i >= 0; --i) sc[h] = matrix_step<PF>(k[u % A], q[s][i], sc[h]);
+      }
+      if (u + A < N) read(u + A);
+      beside(u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // The reference follows the tile's largest scores.
+  __device__ __forceinline__ void follow(const v4f (&sc)[NH]) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      mx = fmaxf(mx, fmaxf(fmaxf(sc[h][0], sc[h][1]), fmaxf(sc[h][2], sc[h][3])));
+    }
+    if constexpr (PF == 2) mx *= unscale;
+    if (__ballot(mx > m + kSlack) != 0) {
+      const float mn = fmaxf(m, row_max(mx));
+      const float alpha = exp2_ratio(m, mn);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+        o[dt] *= alpha;
+        if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      l *= alpha;
+      m = mn;
+    }
+  }
+  // What scores are taken relative to: rows that have seen nothing have no reference.
+  __device__ __forceinline__ float reference() const {
+    return (m == -INFINITY ? 0.f : m) - (PF == 2 ? kProbLog : 0.f);
+  }
+
+  // Probabilities of the scores sc[i / 4][i % 4], i = 2 n, 2 n + 1, as operands.
+  static constexpr int kPairs = 2 * NH;
+  struct Probabilities {
+    unsigned w[kPairs][3];
+    float f[PF == 0 ? 4 : 1];
+  };
+  __device__ __forceinline__ void probability(int n, const v4f (&sc)[NH], float ref,
+                                              Probabilities& p) {
+    const v4f x = sc[n / 2];
+    float y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float s = x[2 * (n % 2) + i];
+      if constexpr (PF == 2) {
+        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, unscale, -ref));
+      } else {
+        y[i] = __builtin_amdgcn_exp2f(s - ref);
+      }
+    }
+    l += y[0] + y[1];
+    if constexpr (PF == 0) {
+      p.f[2 * n] = y[0];
+      p.f[2 * n + 1] = y[1];
+    } else {
+      split_pair<PF>(y[0], y[1], p.w[n]);
+    }
+  }
+
+  // Outputs of the tile.
+  __device__ __forceinline__ void add_values(const unsigned char* tile, int col, int grp,
+                                             const Probabilities& p) {
+    if constexpr (PF == 0) {
+      constexpr int A = 4;
+      // Token 4 grp + i's dim 16 dt + col, chunk 4 dt + col / 4.
+      unsigned at[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int row = 4 * grp + i;
+          at[i][d] = static_cast<unsigned>(row * T::kPitch) +
+                     ((static_cast<unsigned>(4 * d + (col >> 2)) ^ T::turn(row)) & T::kMask) * 16u +
+                     (col & 3) * 4u;
+        }
+      float v[A][4];
+      auto read = [&](int dt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[dt % A][i] = *reinterpret_cast<const float*>(tile + at[i][dt % 4] + (dt / 4) * 256);
+        }
+      };
+#pragma unroll
+      for (int dt = 0; dt < A; ++dt) read(dt);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[dt % A][i], p.f[i], o[dt], 0, 0, 0);
+        }
+        if (dt + A < ND) read(dt + A);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      using LdsV4s = __attribute__((address_space(3))) v4s;
+      constexpr int A = 4;
+      v4u pop[QT];
+#pragma unroll
+      for (int i = 0; i < QT; ++i) pop[i] = v4u{p.w[0][i], p.w[1][i], p.w[2][i], p.w[3][i]};
+      // 32 bytes (16 dims) of tokens 4 grp .. + 3, a quarter of them a lane: chunks
+      // 2 dt and 2 dt + 1 of row 4 grp + col / 4.
+      const int row = 4 * grp + (col >> 2);
+      unsigned at[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        at[d] = static_cast<unsigned>(row * T::kPitch) +
+                ((static_cast<unsigned>(2 * d + ((col >> 1) & 1)) ^ T::turn(row)) & T::kMask) * 16u +
+                (col & 1) * 8u;
+      }
+      v4u v[A];
+      auto read = [&](int dt) {
+        const unsigned char* const from = tile + at[dt % 4] + (dt / 4) * 128;
+        const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from));
+        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from + 16 * T::kPitch));
+        v[dt % A] = __builtin_bit_cast(v4u, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+#pragma unroll
+      for (int dt = 0; dt < A; ++dt) read(dt);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) {
+#pragma unroll
+        for (int i = QT - 1; i >= 0; --i) o[dt] = matrix_step<PF>(v[dt % A], pop[i], o[dt]);
+        if (dt + A < ND) read(dt + A);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  // Scores of a tile whose first token is `first`: those that the row does not see
+  // become -infinity, and NaN where `poison` (bit: token of the tile) has one it sees.
+  __device__ __forceinline__ void mask(int first, unsigned poison, int grp, v4f (&sc)[NH]) const {
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = 16 * h + 4 * grp + i;
+        float x = sc[h][i];
+        if (((poison >> n) & 1u) != 0) x = NAN;
+        sc[h][i] = first + n < limit ? x : -INFINITY;
+      }
+  }
+};
+
+// Where the pages' elements of a tile come from, and their way into LDS.
+template <int PF, int L>
+struct TileLoader {
+  using T = Tile<PF, L>;
+  unsigned off[T::kLoads];  // of the lane's bytes in a group of rows
+
+  __device__ __forceinline__ void start(int lane) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      const unsigned o = static_cast<unsigned>(i * 1024 + lane * 16);
+      const unsigned row = o / T::kPitch, c = (o - row * T::kPitch) / 16;
+      const unsigned from = c ^ (T::turn(static_cast<int>(row)) & T::kMask);
+      off[i] = (row * T::kPitch + from * 16) / (PF == 2 ? 2 : 1);
+    }
+  }
+  // Group g's rows lie in page g / (groups of a page); their turns differ from the
+  // first group's by one exchange.
+  static constexpr int kPageGroups = P / T::kGroupRows;
+  static __device__ __forceinline__ unsigned exchange(int g) {
+    return PF == 0 ? 64u * g : PF == 1 ? 16u * (g & 1) : 8u * (g & 1);
+  }
+  static __device__ __forceinline__ const unsigned char* group_base(const unsigned char* page,
+                                                                    int g) {
+    return page + (g % kPageGroups) * (T::kGroupRows * T::W * T::kPageElem);
+  }
+  // Straight into LDS (bf16 and fp32 pages).
+  __device__ __forceinline__ void direct(const unsigned char* page, int g, unsigned lds) const {
+    const unsigned char* const base = group_base(page, g);
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      lds_load16_at(base, off[i] ^ exchange(g), lds + (g * T::kLoads + i) * 1024u);
+    }
+  }
+  // fp8 codes into registers, and from there as fp16 into LDS.
+  __device__ __forceinline__ void fetch(const unsigned char* page, int g, v2u (&raw)[T::kLoads]) const {
+    using Global = const __attribute__((address_space(1))) v2u*;
+    using GlobalBytes = const __attribute__((address_space(1))) unsigned char*;
+    const auto base = reinterpret_cast<GlobalBytes>(
+        reinterpret_cast<std::uintptr_t>(group_base(page, g)));
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      raw[i] = __builtin_nontemporal_load(reinterpret_cast<Global>(base + (off[i] ^ exchange(g))));
+    }
+  }
+  static __device__ __forceinline__ void store(unsigned char* tile, int g, int lane,
+                                               const v2u (&raw)[T::kLoads]) {
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) {
+      *reinterpret_cast<v4u*>(tile + (g * T::kLoads + i) * 1024 + lane * 16) =
+          codes_fp16(raw[i][0], raw[i][1]);
+    }
+  }
+};
+
+// Rows of the tile that not all of a unit's query rows see must be finite: those
+// behind the sequence's last become 0, and of the step's own tokens those that are
+// not finite; the latter's bits are returned.  Rows 4 `wave` and on by 16 (4 rows at a
+// time, 16 lanes each).
+template <int PF, int L>
+__device__ __forceinline__ unsigned clean_rows(unsigned char* tile, int first, int from, int length,
+                                               int lane, int row0, int row_step) {
+  using T = Tile<PF, L>;
+  unsigned poison = 0;
+  for (int r = row0 + (lane >> 4); r < T::kTokens; r += row_step) {
+    unsigned char* const row = tile + r * T::kPitch;
+    const int token = first + r;
+    bool wipe = token >= length;
+    if (!wipe && token >= from) {
+      unsigned all = 0;  // bit 0: an element that is not finite
+      for (int c = lane & 15; c < T::kPitch / 16; c += 16) {
+        const v4u x = *reinterpret_cast<const v4u*>(row + c * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (PF == 0) {
+            all |= (x[i] & 0x7f800000u) == 0x7f800000u;
+          } else {
+            constexpr unsigned e = PF == 1 ? 0x7f80u : 0x7c00u;
+            all |= (x[i] & e) == e || ((x[i] >> 16) & e) == e;
+          }
+        }
+      }
+      const unsigned long long hit = __ballot(all != 0);
+      wipe = ((hit >> (lane & 48)) & 0xffffull) != 0;
+      if (wipe) poison |= 1u << r;
+    }
+    if (wipe) {
+      for (int c = lane & 15; c < T::kPitch / 16; c += 16) {
+        *reinterpret_cast<v4u*>(row + c * 16) = v4u{0u, 0u, 0u, 0u};
+      }
+    }
+  }
+  return poison;
+}
+
+template <int PF, int L, bool SHARED>
+struct LatentShared {
+  using T = Tile<PF, L>;
+  static constexpr int kBuffers = SHARED ? (PF == 2 ? 3 : 4) : kWaves;
+  __align__(1024) unsigned char tile[kBuffers][T::kBytes];
+  float ml[kWaves][16][2];
+  unsigned poison[kWaves];
+};
+
+// The rows of a finished part, or of a whole unit, from a wavefront.
+struct LatentOutput {
+  int slot;       // of the partial
+  bool complete;  // a whole unit
+  bool bad;
+};
+
+template <int PF, int L>
+__device__ __forceinline__ float finish_factor(const LatentKernelArgs& a, bool complete, bool bad,
+                                               float sum) {
+  const float f = PF == 2 ? a.page_scale : 1.0f;
+  if (!complete) return f;
+  // (A row that has seen nothing has neither sum nor outputs.)
+  return bad ? NAN : sum == 0.f ? 0.f : f / sum;
+}
+
+template <int PF, int L, bool SHARED>
+__device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const LatentStream& st,
+                                            LatentShared<PF, L, SHARED>& sh) {
+  using T = Tile<PF, L>;
+  using R = LatentRows<PF, L>;
+  constexpr int KT = T::kTokens;
+  constexpr int RB = SHARED ? 16 * kWaves : 16;
+  constexpr int NH = R::NH;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int group = static_cast<int>(blockIdx.x);
+  auto barrier = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (st.by_unit == 0 && tid == 0) st.jobs[group] = LatentJob{-1, 0, 0, 0};
+  LatentCursor cur{};
+  // (Four wavefronts take tiles in turn: ranges of whole turns.)
+  const LatentRange range = first_place<KT>(a, st, group, SHARED ? 1 : kWaves, lane, cur);
+  if (range.g0 >= range.g1) return;
+  const int blocks = static_cast<int>(range.g1 - range.g0);
+
+  TileLoader<PF, L> loader;
+  loader.start(lane);
+  const auto* const pool = static_cast<const unsigned char*>(a.pool);
+  // Pages of tile blk of the cursor's sequence.  Behind its tokens the last page
+  // is read again, and without tokens, or where a page is none, page 0; what is read
+  // there takes no part.
+  struct Pages {
+    const unsigned char* at[T::kPages];
+    int bad;
+  };
+  auto locate = [&](const LatentCursor& c, int blk) {
+    Pages p{};
+    p.bad = c.bad;
+    const std::uint32_t* const table = a.tables + static_cast<std::size_t>(c.b) * a.max_blocks;
+    const int last = (c.length - 1) / P;
+#pragma unroll
+    for (int i = 0; i < T::kPages; ++i) {
+      std::uint32_t page = 0;
+      if (c.length > 0) page = uniform_read(table + min(blk * T::kPages + i, last));
+      if (page >= a.physical_blocks) {
+        p.bad = 1;
+        page = 0;
+      }
+      p.at[i] = pool + page * T::kPageBytes;
+    }
+    return p;
+  };
+  auto page_of = [&](const Pages& p, int g) {
+    if constexpr (T::kPages == 1) {
+      return p.at[0];
+    } else {
+      return g < TileLoader<PF, L>::kPageGroups ? p.at[0] : p.at[1];
+    }
+  };
+
+  R rows;
+  // Ends the unit's part, tiles [from, to) of it, the last of which is the range's
+  // n-th.
+  auto part_of = [&](const LatentCursor& c, int from, int to, int n) {
+    const bool starts = from == 0, ends = to == c.nb;
+    const int slot = 2 * group + (starts ? 1 : 0);
+    if (ends && tid == 0) {
+      const long long first = (range.g0 + n - (to - 1)) / range.each;
+      if (st.by_unit != 0) {
+        st.jobs[static_cast<std::size_t>(c.rb) * a.batch + c.b] =
+            LatentJob{starts ? -1 : c.b, c.rb, static_cast<int>(first), group};
+      } else if (!starts) {
+        st.jobs[group] = LatentJob{c.b, c.rb, static_cast<int>(first), group};
+      }
+    }
+    return slot;
+  };
+  // Row `row` of the sequence, dims `at` and on of its output or partial.
+  auto out_row = [&](const LatentCursor& c, int row) {
+    const int h = row / a.tokens, t = row - h * a.tokens;
+    return a.out + static_cast<std::size_t>(c.b) * a.out_at.batch +
+           static_cast<std::size_t>(h) * a.out_at.head + static_cast<std::size_t>(t) * a.out_at.token;
+  };
+
+  if constexpr (SHARED) {
+    constexpr int NB = LatentShared<PF, L, SHARED>::kBuffers;
+    const unsigned lds0 = lds_address(sh.tile[0]);
+    // Tile i of the range goes to buffer i % NB, two steps (fp8: one step and the
+    // registers) ahead of its scores.  Behind the range the last one is read again.
+    LatentCursor ahead = cur;
+    int located = 0;  // the range's tile that `next` is
+    unsigned bads = 0;  // bit i % 32: of tile i
+    v2u raw[PF == 2 ? T::kLoads : 1];
+    Pages next = locate(ahead, ahead.blk);
+    bads = next.bad != 0 ? 1u : 0u;
+    auto locate_next = [&] {
+      if (located + 1 < blocks) {
+        ++located;
+        if (++ahead.blk == ahead.nb) next_unit<KT>(a, ahead);
+        next = locate(ahead, ahead.blk);
+        bads = (bads & ~(1u << (located & 31))) | (next.bad != 0 ? 1u << (located & 31) : 0u);
+      }
+    };
+    int into = 0;
+    auto bump = [&](int& i) { i = i + 1 == NB ? 0 : i + 1; };
+    // The wavefront's quarter of the next tile is sent for (fp8: the one that was
+    // goes to LDS first).
+    auto send = [&] {
+      if constexpr (PF == 2) {
+        TileLoader<PF, L>::store(sh.tile[into], wave, lane, raw);
+        loader.fetch(page_of(next, wave), wave, raw);
+      } else {
+        loader.direct(page_of(next, wave), wave, lds0 + static_cast<unsigned>(into) * T::kBytes);
+      }
+      bump(into);
+      locate_next();
+    };
+    // What was sent for before the last two times is there.
+    auto arrived = [&] {
+      if constexpr (PF != 2) __builtin_amdgcn_s_waitcnt(0x0f70 | T::kLoads);
+    };
+    if constexpr (PF == 2) {
+      loader.fetch(page_of(next, wave), wave, raw);
+      locate_next();
+    }
+    send();
+    send();
+    if constexpr (PF != 2) send();
+    arrived();
+    barrier();
+    int n = 0, buf = 0;  // tile, and its buffer
+    for (;;) {
+      const int row = cur.rb * RB + wave * 16 + col;
+      rows.start(a, cur, row, grp);
+      const int from = cur.blk;
+      const int to = min(cur.nb, cur.blk + (blocks - n));
+      // Tiles before `whole` are seen by every row.
+      const int whole = max(cur.length - cur.count + 1, 0) / KT;
+      int bad = 0;
+      v4f sc[NH];
+      rows.scores(sh.tile[buf], col, grp, sc, [](int) {});
+      for (int blk = from; blk < to; ++blk) {
+        send();
+        bad |= static_cast<int>(bads >> (n & 31)) & 1;
+        typename R::Probabilities p;
+        int after = buf;
+        bump(after);
+        if (blk >= whole) {
+          unsigned poison = clean_rows<PF, L>(sh.tile[buf], blk * KT, cur.length - cur.count + 1,
+                                              cur.length, lane, 4 * wave, 16);
+#pragma unroll
+          for (int bit = 16; bit < 64; bit *= 2) poison |= __shfl_xor(poison, bit, 64);
+          if (lane == 0) sh.poison[wave] = poison;
+          // (Every wavefront took its scores of the tile a step ago.)
+          barrier();
+          poison = sh.poison[0] | sh.poison[1] | sh.poison[2] | sh.poison[3];
+          rows.mask(blk * KT, poison, grp, sc);
+        }
+        rows.follow(sc);
+        const float ref = rows.reference();
+        if (blk + 1 < to) {
+          // This tile's probabilities beside the next one's scores.
+          v4f now[NH];
+#pragma unroll
+          for (int h = 0; h < NH; ++h) now[h] = sc[h];
+          constexpr int kEvery = R::NS * NH / (R::kPairs + 1);
+          rows.scores(sh.tile[after], col, grp, sc, [&](int u) {
+            if (u % kEvery == kEvery - 1 && u / kEvery < R::kPairs) {
+              rows.probability(u / kEvery, now, ref, p);
+            }
+          });
+        } else {
+#pragma unroll
+          for (int i = 0; i < R::kPairs; ++i) rows.probability(i, sc, ref, p);
+        }
+        rows.add_values(sh.tile[buf], col, grp, p);
+        buf = after;
+        ++n;
+        arrived();
+        barrier();
+      }
+      // The part's end.
+      const bool complete = from == 0 && to == cur.nb;
+      const int slot = part_of(cur, from, to, n - 1);
+      const float sum = row_sum(rows.l);
+      const float f = finish_factor<PF, L>(a, complete, bad != 0, sum);
+      if (rows.live) {
+        const int local = wave * 16 + col;
+        float* const dst = (complete ? out_row(cur, row)
+                                     : st.part_o + (static_cast<std::size_t>(slot) * RB + local) * L) +
+                           4 * grp;
+#pragma unroll
+        for (int dt = 0; dt < R::ND; ++dt) *reinterpret_cast<v4f*>(dst + 16 * dt) = rows.o[dt] * f;
+        if (!complete && grp == 0) {
+          float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * RB + local) * 2;
+          ml[0] = rows.m;
+          ml[1] = bad != 0 ? NAN : sum;
+        }
+      }
+      if (n == blocks) break;
+      next_unit<KT>(a, cur);
+    }
+    // (Nothing is on its way into LDS when the workgroup gives it back.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  } else {
+    unsigned char* const tile = sh.tile[wave];
+    const unsigned lds = lds_address(tile);
+    v2u raw[4][PF == 2 ? T::kLoads : 1];
+    int n = 0;
+    for (;;) {
+      const int row = cur.rb * RB + col;
+      const int from = cur.blk;
+      const int to = min(cur.nb, cur.blk + (blocks - n));
+      const int whole = max(cur.length - cur.count + 1, 0) / KT;
+      int bad = 0;
+      auto send = [&](int blk) {
+        const Pages p = locate(cur, blk);
+        bad |= p.bad;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if constexpr (PF == 2) {
+            loader.fetch(page_of(p, g), g, raw[g]);
+          } else {
+            loader.direct(page_of(p, g), g, lds);
+          }
+        }
+      };
+      if (from + wave < to) send(from + wave);
+      rows.start(a, cur, row, grp);
+      for (int blk = from + wave; blk < to; blk += kWaves) {
+        if constexpr (PF == 2) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) TileLoader<PF, L>::store(tile, g, lane, raw[g]);
+          if (blk + kWaves < to) send(blk + kWaves);
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        v4f sc[NH];
+        rows.scores(tile, col, grp, sc, [](int) {});
+        if (blk >= whole) {
+          unsigned poison = clean_rows<PF, L>(tile, blk * KT, cur.length - cur.count + 1, cur.length,
+                                              lane, 0, 4);
+#pragma unroll
+          for (int bit = 16; bit < 64; bit *= 2) poison |= __shfl_xor(poison, bit, 64);
+          rows.mask(blk * KT, poison, grp, sc);
+        }
+        rows.follow(sc);
+        const float ref = rows.reference();
+        typename R::Probabilities p;
+#pragma unroll
+        for (int i = 0; i < R::kPairs; ++i) rows.probability(i, sc, ref, p);
+        rows.add_values(tile, col, grp, p);
+        if constexpr (PF != 2) {
+          if (blk + kWaves < to) {
+            // (The tile's reads are done before it is written again.)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            send(blk + kWaves);
+          }
+        }
+      }
+      // The wavefronts join what they have: each one's outputs, relative to the
+      // largest reference, in its tile.
+      const float own = row_sum(rows.l);
+      if (grp == 0) {
+        sh.ml[wave][col][0] = rows.m;
+        sh.ml[wave][col][1] = own;
+      }
+      if (lane == 0) sh.poison[wave] = static_cast<unsigned>(bad);
+      barrier();
+      float top = sh.ml[0][col][0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sh.ml[w][col][0]);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        // (A reference of -infinity comes with a sum of 0.)
+        const float x = sh.ml[w][col][1];
+        sum += x == 0.f ? 0.f : x * exp2_ratio(sh.ml[w][col][0], top);
+      }
+      bad = static_cast<int>(sh.poison[0] | sh.poison[1] | sh.poison[2] | sh.poison[3]);
+      const float alpha = exp2_ratio(rows.m, top);
+      // Row col's dims 4 u .. + 3 at chunk u ^ (col / 2 and 1 bit), 16 bytes each: the
+      // 16 rows of one write, or read, lie on distinct banks.
+      constexpr int kRowBytes = L * 4;
+      auto place = [&](int r, int u) { return r * kRowBytes + ((u ^ r) & 15) * 16 + (u & ~15) * 16; };
+#pragma unroll
+      for (int dt = 0; dt < R::ND; ++dt) {
+        *reinterpret_cast<v4f*>(tile + place(col, 4 * dt + grp)) = rows.o[dt] * alpha;
+      }
+      barrier();
+      const bool complete = from == 0 && to == cur.nb;
+      const int last = n + (to - from) - 1;
+      const int slot = part_of(cur, from, to, last);
+      const float f = finish_factor<PF, L>(a, complete, bad != 0, sum);
+      // A wavefront adds up four rows, 16 lanes (L / 16 dims each) a row.
+      {
+        const int local = 4 * wave + grp;
+        const int r = cur.rb * RB + local;
+        const float rf = __shfl(f, local, 64);
+        const float rm = __shfl(top, local, 64), rs = __shfl(sum, local, 64);
+        const bool live = __shfl(rows.live ? 1 : 0, local, 64) != 0;
+        if (live) {
+          float* const dst = complete
+                                 ? out_row(cur, r)
+                                 : st.part_o + (static_cast<std::size_t>(slot) * RB + local) * L;
+#pragma unroll
+          for (int i = 0; i < L / 64; ++i) {
+            const int u = 16 * i + col;
+            v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+              x += *reinterpret_cast<const v4f*>(sh.tile[w] + place(local, u));
+            }
+            *reinterpret_cast<v4f*>(dst + 4 * u) = x * rf;
+          }
+          if (!complete && col == 0) {
+            float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * RB + local) * 2;
+            ml[0] = rm;
+            ml[1] = bad != 0 ? NAN : rs;
+          }
+        }
+      }
+      n += to - from;
+      if (n == blocks) break;
+      next_unit<KT>(a, cur);
+      barrier();  // the tiles are read
+    }
+  }
+}
+
+template <int PF, int L, bool SHARED>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+    void latent_kernel(LatentKernelArgs a, LatentStream st) {
+  __shared__ LatentShared<PF, L, SHARED> sh;
+  latent_body<PF, L, SHARED>(a, st, sh);
+}
+
+// Joins the partials of the units that cross ranges: the first group's second slot
+// and the later groups' first ones.  blockIdx.x is a unit or a group, blockIdx.y a row
+// (SPLIT: the wavefronts share its partials) or four rows.
+constexpr int kMostParts = 512;
+template <int L, bool SPLIT>
+__global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, LatentStream st,
+                                                           int rb_rows) {
+  constexpr int NV = L / 256;  // 4 dims each
+  __shared__ v4f sums[SPLIT ? 4 : 1][SPLIT ? L / 4 : 1];
+  __shared__ float weights[4][kMostParts];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  if (st.by_unit != 0 && clamped_count(a, static_cast<int>(blockIdx.x) % a.batch) == 0) return;
+  const LatentJob job = st.jobs[blockIdx.x];
+  if (job.b < 0) return;
+  const int local = SPLIT ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * 4 + wave;
+  const int row = job.rb * rb_rows + local;
+  const int h = row / a.tokens, t = row - h * a.tokens;
+  const bool live = local < rb_rows && row < a.rows && t < clamped_count(a, job.b);
+  const int parts = min(job.last - job.first + 1, kMostParts);
+  auto slot = [&](int i) {
+    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + local;
+  };
+  float top = -INFINITY, sum = 0.f;
+  v4f o[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) o[v] = v4f{0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, st.part_ml[2 * slot(i)]);
+#pragma unroll
+    for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
+    for (int i = lane; i < parts; i += 64) {
+      const float pl = st.part_ml[2 * slot(i) + 1];
+      const float w = pl == 0.f ? 0.f : exp2_ratio(st.part_ml[2 * slot(i)], top);
+      sum += pl * w;
+      weights[wave][i] = w;
     }
 #pragma unroll
-    for (int bit = 32; bit >= 1; bit /= 2) x += __shfl_xor(x, bit, 64);
-    const float mn = fmaxf(m, x);
-    const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float p = x == mn ? 1.0f : __builtin_amdgcn_exp2f(x - mn);
-    l = l * alpha + p;
+    for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
+    constexpr int U = 4;  // partials on their way
+    const int step = SPLIT ? 4 : 1;
+    for (int i0 = SPLIT ? wave : 0; i0 < parts; i0 += U * step) {
+      v4f x[U][NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) o[i] = o[i] * alpha + p * k[i];
-    m = mn;
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * step, parts - 1);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          x[u][v] = reinterpret_cast<const v4f*>(st.part_o + slot(i) * L)[64 * v + lane];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * step;
+        const float w = i < parts ? weights[wave][min(i, parts - 1)] : 0.f;
+        if (w != 0.f) {  // (a part that saw nothing has no outputs to speak of)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) o[v] += x[u][v] * w;
+        }
+      }
+    }
   }
-  const float f = bad ? NAN : seen == 0 ? 0.f : 1.0f / l;
-  float* const out = a.out + b * a.out_at.batch + h * a.out_at.head + t * a.out_at.token;
+  if constexpr (SPLIT) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) out[64 * i + lane] = seen == 0 && !bad ? 0.f : o[i] * f;
+    for (int v = 0; v < NV; ++v) sums[wave][64 * v + lane] = o[v];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      o[v] = (sums[0][64 * v + lane] + sums[1][64 * v + lane]) +
+             (sums[2][64 * v + lane] + sums[3][64 * v + lane]);
+    }
+  }
+  if (!live) return;
+  const float f = sum == 0.f ? 0.f : 1.0f / sum;
+  auto* const dst = reinterpret_cast<v4f*>(
+      a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
+      static_cast<std::size_t>(h) * a.out_at.head + static_cast<std::size_t>(t) * a.out_at.token);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) dst[64 * v + lane] = o[v] * f;
+}
+
+// ----------------------------------------------------------------- host ----
+// A workgroup a CU: a tile of 32 rows of 576 elements takes 36 KB of LDS.
+constexpr std::size_t kGroups = 256;
+static_assert(kGroups + 1 <= kMostParts);
+
+std::size_t unit_rows(std::size_t rows) { return rows <= 16 ? 16 : 64; }
+
+std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
+
+struct LatentLayout {
+  LatentLayout(std::size_t rows, std::size_t latent) {
+    rb = unit_rows(rows);
+    row_blocks = (rows + rb - 1) / rb;
+    auto take = [&](std::size_t n) {
+      const std::size_t at = bytes;
+      bytes += align256(n);
+      return at;
+    };
+    jobs = take(kGroups * sizeof(LatentJob));
+    part_ml = take(2 * kGroups * rb * 2 * sizeof(float));
+    part_o = take(2 * kGroups * rb * latent * sizeof(float));
+  }
+  std::size_t rb, row_blocks, jobs, part_ml, part_o, bytes = 0;
+};
+
+template <int PF, int L>
+hipError_t launch_latent(const LatentKernelArgs& k, const LatentStream& st, std::size_t rb,
+                         hipStream_t stream) {
+  if (rb == 16) {
+    latent_kernel<PF, L, false><<<dim3(static_cast<unsigned>(kGroups)), 64 * kWaves, 0, stream>>>(k, st);
+  } else {
+    latent_kernel<PF, L, true><<<dim3(static_cast<unsigned>(kGroups)), 64 * kWaves, 0, stream>>>(k, st);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const std::size_t jobs =
+      st.by_unit != 0 ? static_cast<std::size_t>(k.batch) * st.row_blocks : kGroups;
+  const unsigned rows = static_cast<unsigned>(std::min<std::size_t>(rb, static_cast<std::size_t>(k.rows)));
+  // Few units: all wavefronts of a workgroup on one row.
+  if (jobs * rows <= 2048) {
+    latent_merge_kernel<L, true>
+        <<<dim3(static_cast<unsigned>(jobs), rows), 256, 0, stream>>>(k, st, static_cast<int>(rb));
+  } else {
+    latent_merge_kernel<L, false><<<dim3(static_cast<unsigned>(jobs), (rows + 3) / 4), 256, 0, stream>>>(
+        k, st, static_cast<int>(rb));
+  }
+  return hipGetLastError();
 }
 
 template <int PF>
-void launch_rows(const LatentKernelArgs& k, std::size_t latent, hipStream_t stream) {
-  const long long rows = static_cast<long long>(k.batch) * k.q_heads * k.tokens;
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-  if (latent == 512) {
-    latent_row_kernel<PF, 512><<<grid, 256, 0, stream>>>(k);
-  } else {
-    latent_row_kernel<PF, 256><<<grid, 256, 0, stream>>>(k);
-  }
+hipError_t launch_page_type(const LatentKernelArgs& k, const LatentStream& st, std::size_t rb,
+                            std::size_t latent, hipStream_t stream) {
+  return latent == 512 ? launch_latent<PF, 512>(k, st, rb, stream)
+                       : launch_latent<PF, 256>(k, st, rb, stream);
 }
 
 }  // namespace
 
-std::size_t latent_workspace_bytes(std::size_t, std::size_t, std::size_t, std::size_t) { return 16; }
+std::size_t latent_workspace_bytes(std::size_t, std::size_t q_heads, std::size_t tokens,
+                                   std::size_t latent) {
+  return LatentLayout(q_heads * tokens, latent).bytes;
+}
 
 bool latent_fits(const LatentArgs& a) {
-  return a.batch == 0 || a.q_heads == 0 || a.tokens == 0 ||
-         a.batch * a.q_heads <= (std::size_t{1} << 32) / a.tokens;
+  // Ranges, and places in them, are counted in 32 bits: of 2^38 tiles, a group's
+  // are 2^30 at most.
+  const std::size_t rows = a.q_heads * a.tokens;
+  const std::size_t units = a.batch * ((rows + 15) / 16);
+  return units == 0 || a.max_blocks + 2 <= (std::size_t{1} << 38) / units;
 }
 
 hipError_t launch_latent_attention(const LatentArgs& a, hipStream_t stream) {
   if (a.batch == 0 || a.q_heads == 0 || a.tokens == 0) return hipSuccess;
   if (!latent_fits(a)) return hipErrorInvalidValue;
+  const LatentLayout layout(a.q_heads * a.tokens, a.latent);
   LatentKernelArgs k{};
   k.query = a.query;
   k.pool = a.pool;
@@ -136,15 +1174,23 @@ hipError_t launch_latent_attention(const LatentArgs& a, hipStream_t stream) {
   k.q_heads = static_cast<int>(a.q_heads);
   k.tokens = static_cast<int>(a.tokens);
   k.max_blocks = static_cast<int>(a.max_blocks);
+  k.rows = static_cast<int>(a.q_heads * a.tokens);
   k.physical_blocks = static_cast<std::uint32_t>(a.physical_blocks);
-  k.qscale = kLog2e * a.scale;
+  k.qscale = kLog2e * a.scale * (a.page_type == PageType::kFP8 ? a.page_scale : 1.0f);
   k.page_scale = a.page_scale;
+  auto* const base = static_cast<unsigned char*>(a.workspace);
+  LatentStream st{};
+  st.jobs = reinterpret_cast<LatentJob*>(base + layout.jobs);
+  st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
+  st.part_o = reinterpret_cast<float*>(base + layout.part_o);
+  st.groups = static_cast<int>(kGroups);
+  st.row_blocks = static_cast<int>(layout.row_blocks);
+  st.by_unit = a.batch * layout.row_blocks <= kGroups ? 1 : 0;
   switch (a.page_type) {
-    case PageType::kBF16: launch_rows<1>(k, a.latent, stream); break;
-    case PageType::kFP8: launch_rows<2>(k, a.latent, stream); break;
-    default: launch_rows<0>(k, a.latent, stream); break;
+    case PageType::kBF16: return launch_page_type<1>(k, st, layout.rb, a.latent, stream);
+    case PageType::kFP8: return launch_page_type<2>(k, st, layout.rb, a.latent, stream);
+    default: return launch_page_type<0>(k, st, layout.rb, a.latent, stream);
   }
-  return hipGetLastError();
 }
 
 }  // namespace helix::hip
