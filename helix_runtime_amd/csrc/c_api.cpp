@@ -2182,6 +2182,8 @@ int helix_latent_prefill_attention(const float* query, const size_t* query_strid
     a.tokens = tokens;
     a.keys = keys;
     a.scale = scale;
+    check(helix::hip::expanded_fits(a), Status::kUnsupported, op,
+          "too many queries and keys for one call");
     helix::hip_check(helix::hip::launch_expanded_attention(a, as_stream(stream)), op);
   });
 }

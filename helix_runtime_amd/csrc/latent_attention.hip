@@ -364,11 +364,11 @@ struct LatentRows {
   }
 
   // Scores of a tile: sc[h][i] is token 16 h + 4 grp + i of row col.  `beside(u)` is
-  // what else the lane does between the matrix instructions of step u of NS * NH.
+  // what else the lane does between the matrix instructions of step u of NS.
   template <typename F>
   __device__ __forceinline__ void scores(const unsigned char* tile, int col, int grp, v4f (&sc)[NH],
                                          F&& beside) const {
-    constexpr int N = NS * NH, A = 4;  // operands come out of LDS A steps ahead
+    constexpr int A = PF == 0 ? 4 : 2;  // operands come out of LDS A steps ahead
     // Row col's chunk 4 s + grp: its place within a group of chunks is one of two
     // (fp32 pages: four), by s.
     constexpr int V = PF == 0 ? 4 : 2;
@@ -378,33 +378,36 @@ struct LatentRows {
       at[i] = static_cast<unsigned>(col * T::kPitch) +
               ((static_cast<unsigned>(4 * i + grp) ^ T::turn(col)) & T::kMask) * 16u;
     }
-    v4u k[A];
-    auto read = [&](int u) {
-      const int s = u / NH, h = u % NH;
-      // (Rows 16 h and on turn as rows 0 and on do.)
-      k[u % A] = *reinterpret_cast<const v4u*>(tile + at[s % V] + (s / V) * (V * 64) +
-                                               h * (16 * T::kPitch));
+    v4u k[A][NH];
+    auto read = [&](int s) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {  // (rows 16 h and on turn as rows 0 and on do)
+        k[s % A][h] = *reinterpret_cast<const v4u*>(tile + at[s % V] + (s / V) * (V * 64) +
+                                                    h * (16 * T::kPitch));
+      }
     };
 #pragma unroll
-    for (int u = 0; u < A; ++u) read(u);
+    for (int s = 0; s < A; ++s) read(s);
 #pragma unroll
     for (int h = 0; h < NH; ++h) sc[h] = v4f{0.f, 0.f, 0.f, 0.f};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int s = u / NH, h = u % NH;
+    for (int s = 0; s < NS; ++s) {
       if constexpr (PF == 0) {
-        const v4f x = __builtin_bit_cast(v4f, k[u % A]), y = __builtin_bit_cast(v4f, q[s][0]);
+        const v4f x = __builtin_bit_cast(v4f, k[s % A][0]), y = __builtin_bit_cast(v4f, q[s][0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sc[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[h], 0, 0, 0);
+          sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[0], 0, 0, 0);
         }
       } else {
+        // Smallest products first; one half's sum waits while the other's runs.
 #pragma unroll
-        for (int i = QT - 1; i >= 0; --i) sc[h] = matrix_step<PF>(k[u % A], q[s][i], sc[h]);
+        for (int i = QT - 1; i >= 0; --i)
+#pragma unroll
+          for (int h = 0; h < NH; ++h) sc[h] = matrix_step<PF>(k[s % A][h], q[s][i], sc[h]);
       }
-      if (u + A < N) read(u + A);
-      beside(u);
+      if (s + A < NS) read(s + A);
+      beside(s);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -524,10 +527,15 @@ struct LatentRows {
       for (int dt = 0; dt < A; ++dt) read(dt);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) {
+      for (int dt = 0; dt < ND; dt += 2) {
 #pragma unroll
-        for (int i = QT - 1; i >= 0; --i) o[dt] = matrix_step<PF>(v[dt % A], pop[i], o[dt]);
-        if (dt + A < ND) read(dt + A);
+        for (int i = QT - 1; i >= 0; --i)
+#pragma unroll
+          for (int d = dt; d < dt + 2; ++d) o[d] = matrix_step<PF>(v[d % A], pop[i], o[d]);
+        if (dt + A < ND) {
+          read(dt + A);
+          read(dt + A + 1);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -832,7 +840,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
           v4f now[NH];
 #pragma unroll
           for (int h = 0; h < NH; ++h) now[h] = sc[h];
-          constexpr int kEvery = R::NS * NH / (R::kPairs + 1);
+          constexpr int kEvery = R::NS / (R::kPairs + 1);
           rows.scores(sh.tile[after], col, grp, sc, [&](int u) {
             if (u % kEvery == kEvery - 1 && u / kEvery < R::kPairs) {
               rows.probability(u / kEvery, now, ref, p);

@@ -6,19 +6,60 @@
 // j over the keys that row t sees, r_j the rotated part of key j that every head
 // shares.
 //
-// One wavefront a row: a lane holds elements lane and lane + 64 of a head's key
-// and value and element lane of the shared part.
+// Work split.  128 rows (64 where there are no more) of a (sequence, head) form a
+// unit, its keys up to the last that one of them sees are tiles of 32.  A fixed grid
+// takes equal ranges of the flat list of all units' tiles; units that cross ranges
+// leave partials (maximum, sum, output), which expanded_merge_kernel joins.  A head's
+// units lie far apart in the list, so that the workgroups that read the same keys do
+// so at one time.
+//
+// Matrix form.  As in the absorbed form: S^T = K Q^T, O^T += V^T P^T, a lane holding
+// keys of one query row.  fp32 numbers are sums of three bf16 terms (24 bits), of
+// whose nine products the six above 2^-26 of the largest are taken: 2.7 times the
+// rate of fp32 matrix instructions.  (Two fp16 terms would take three products, and a
+// common exponent for a tile's keys, which keys that a row must not see would set.)
+// Keys and values are split once a workgroup on their way into LDS; a wavefront has 32
+// rows, so that an operand out of LDS serves twelve matrix instructions.
+#include "bf16.hpp"
 #include "latent.hpp"
+#include "prefill_bmma.hpp"
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
 namespace helix::hip {
 namespace {
 
+using prefill_detail::exp2_ratio;
+using prefill_detail::row_max;
+using prefill_detail::row_sum;
+using prefill_detail::uniform_read;
+using prefill_detail::v4f;
+using prefill_detail::v4s;
+using prefill_detail::v8bf;
+
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kKeyDim = static_cast<int>(kLatentNope + kLatentRope);
+constexpr int kValueDim = static_cast<int>(kLatentNope);
+constexpr int kTile = 32;   // keys
+constexpr int kWaves = 4;
+constexpr int kTerms = 3;
+constexpr int kSteps = kKeyDim / 32;    // of the scores' sum
+constexpr int kDims = kValueDim / 16;   // tiles of output dims
+constexpr int kKeyPitch = kKeyDim * 2;  // bytes of a row of one term in LDS
+constexpr int kValuePitch = kValueDim * 2;
+// Numbers from here on have an infinite first term.
+constexpr float kWild = 0x1.ffp+127f;
+// A row's reference stays while no score is above it by more than this (log2
+// units).
+constexpr float kSlack = 7.0f;
 
 struct ExpandedKernelArgs {
   const float* query;
@@ -33,54 +74,675 @@ struct ExpandedKernelArgs {
   float qscale;  // log2(e) * scale
 };
 
-__global__ __launch_bounds__(256) void expanded_row_kernel(ExpandedKernelArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long long rows = static_cast<long long>(a.batch) * a.heads * a.tokens;
-  const long long r = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int t = static_cast<int>(r % a.tokens);
-  const int h = static_cast<int>(r / a.tokens % a.heads);
-  const int b = static_cast<int>(r / a.tokens / a.heads);
-  int count = a.tokens;
-  if (a.token_counts != nullptr) count = min(max(a.token_counts[b], 0), a.tokens);
-  if (t >= count) return;
-  const int length = a.key_lengths != nullptr ? a.key_lengths[b] : a.keys;
-  const bool bad = length < 0 || length > a.keys;
-  const int seen = bad ? 0 : max(length - count + t + 1, 0);
-  const float* const q = a.query + b * a.query_at.batch + h * a.query_at.head + t * a.query_at.token;
-  const float* const key = a.key + b * a.key_at.batch + h * a.key_at.head;
-  const float* const rope = a.rope_key + b * a.rope_at.batch;
-  const float* const value = a.value + b * a.value_at.batch + h * a.value_at.head;
-  const float q0 = q[lane] * a.qscale, q1 = q[lane + 64] * a.qscale, q2 = q[lane + 128] * a.qscale;
-  float o0 = 0.f, o1 = 0.f, m = -INFINITY, l = 0.f;
-  for (int j = 0; j < seen; ++j) {
-    const float* const k = key + j * a.key_at.token;
-    const float* const v = value + j * a.value_at.token;
-    float x = q0 * k[lane] + q1 * k[lane + 64] + q2 * rope[j * a.rope_at.token + lane];
+// A unit to join: the one that a group's range ends without starting it.
+struct ExpandedJob {
+  int b, h, rb;     // sequence (-1: none), head, row block
+  int first, last;  // groups whose ranges start and end the unit
+};
+
+struct ExpandedStream {
+  float* part_o;     // [2 * groups, RB, 128]
+  float* part_ml;    // [2 * groups, RB, 2]
+  ExpandedJob* jobs; // [groups]
+  int groups;
+  int row_blocks;    // units of a (sequence, head), at most
+};
+
+// x = t[0] + t[1] + t[2], each rounded to nearest; two numbers at a time, packed into
+// words.
+__device__ __forceinline__ void split_pair(float x, float y, unsigned (&t)[kTerms]) {
 #pragma unroll
-    for (int bit = 32; bit >= 1; bit /= 2) x += __shfl_xor(x, bit, 64);
-    const float mn = fmaxf(m, x);
-    const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float p = x == mn ? 1.0f : __builtin_amdgcn_exp2f(x - mn);
-    l = l * alpha + p;
-    o0 = o0 * alpha + p * v[lane];
-    o1 = o1 * alpha + p * v[lane + 64];
-    m = mn;
+  for (int i = 0; i < kTerms; ++i) {
+    const v2bf h = __builtin_convertvector((v2f{x, y}), v2bf);
+    t[i] = __builtin_bit_cast(unsigned, h);
+    x -= __uint_as_float(t[i] << 16);
+    y -= __uint_as_float(t[i] & 0xffff0000u);
   }
-  const float f = bad ? NAN : seen == 0 ? 0.f : 1.0f / l;
-  float* const out = a.out + b * a.out_at.batch + h * a.out_at.head + t * a.out_at.token;
-  out[lane] = o0 * f;
-  out[lane + 64] = o1 * f;
 }
+
+__device__ __forceinline__ v4f matrix_step(v4u a, v4u b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
+                                                 __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+
+// Chunks of 16 bytes are exchanged by row, so that a read of one chunk of 16 rows
+// (scores) and of 32 bytes of 8 rows (outputs) hits distinct banks: key rows lie 128
+// bytes from a multiple of 256 apart, value rows 256.
+__device__ __forceinline__ unsigned key_place(int row, int chunk) {
+  const int turn = (row & 6) | ((row >> 3) & 1);
+  return static_cast<unsigned>(row * kKeyPitch + (chunk ^ turn) * 16);
+}
+__device__ __forceinline__ unsigned value_place(int row, int chunk) {
+  return static_cast<unsigned>(row * kValuePitch + (chunk ^ (2 * (row & 7))) * 16);
+}
+
+// Item i of a range: keys of tile i and values of tile i - 1, what one step takes.
+struct ExpandedShared {
+  struct Item {
+    __align__(1024) unsigned char k[kTerms][kTile * kKeyPitch];
+    __align__(1024) unsigned char v[kTerms][kTile * kValuePitch];
+  };
+  Item item[2];
+  unsigned poison[2][kWaves];  // keys of the item's values that must not be seen
+};
+
+// A place in the flat list of tiles.
+struct ExpandedCursor {
+  int b, h, rb, blk;
+  int length, count, nb;
+  int first;  // keys that the unit's first row sees
+  int bad;    // the length lies outside [0, keys]
+};
+
+__device__ __forceinline__ int clamped_count(const ExpandedKernelArgs& a, int b) {
+  return a.token_counts != nullptr ? min(max(a.token_counts[b], 0), a.tokens) : a.tokens;
+}
+
+// Tiles of a unit of sequence b: one at least where it has rows.
+template <int RB>
+__device__ __forceinline__ int unit_tiles(int length, int count, int rb) {
+  const int row0 = rb * RB;
+  if (row0 >= count) return 0;
+  const int sees = length - count + min(count, row0 + RB);
+  return max((sees + kTile - 1) / kTile, 1);
+}
+
+template <int RB>
+__device__ __forceinline__ int entry_tiles(const ExpandedKernelArgs& a, int row_blocks, long long e) {
+  if (e >= static_cast<long long>(row_blocks) * a.batch) return 0;
+  const int rb = static_cast<int>(e / a.batch);
+  const int b = static_cast<int>(e - static_cast<long long>(rb) * a.batch);
+  int length = a.key_lengths != nullptr ? a.key_lengths[b] : a.keys;
+  if (length < 0 || length > a.keys) length = 0;
+  return unit_tiles<RB>(length, clamped_count(a, b), rb);
+}
+
+template <int RB>
+__device__ __forceinline__ void load_unit(const ExpandedKernelArgs& a, ExpandedCursor& c) {
+  const int length = a.key_lengths != nullptr ? uniform_read(a.key_lengths + c.b) : a.keys;
+  c.bad = length < 0 || length > a.keys;
+  c.length = c.bad ? 0 : length;
+  c.count = a.tokens;
+  if (a.token_counts != nullptr) c.count = min(max(uniform_read(a.token_counts + c.b), 0), a.tokens);
+  c.nb = unit_tiles<RB>(c.length, c.count, c.rb);
+  c.first = c.length - c.count + c.rb * RB + 1;
+}
+
+__device__ __forceinline__ long long uniform_long(long long v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
+  const unsigned hi =
+      __builtin_amdgcn_readfirstlane(static_cast<unsigned>(static_cast<unsigned long long>(v) >> 32));
+  return static_cast<long long>(static_cast<unsigned long long>(hi) << 32 | lo);
+}
+
+// Inclusive sums over the wavefront.
+__device__ __forceinline__ long long lane_scan(long long v, int lane) {
+  long long sum = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long t = __shfl_up(sum, o, 64);
+    if (lane >= o) sum += t;
+  }
+  return sum;
+}
+
+// This group's range of tiles [g0, g1) (ranges of `each`) and its first place.  The
+// list goes by row block, sequence, head and tile.
+struct ExpandedRange {
+  long long g0, g1, each;
+};
+template <int RB>
+__device__ __forceinline__ ExpandedRange first_place(const ExpandedKernelArgs& a,
+                                                     const ExpandedStream& st, int group, int lane,
+                                                     ExpandedCursor& c) {
+  const long long entries = static_cast<long long>(st.row_blocks) * a.batch;
+  long long total = 0;
+  for (long long e0 = 0; e0 < entries; e0 += 64) total += entry_tiles<RB>(a, st.row_blocks, e0 + lane);
+  total = uniform_long(__shfl(lane_scan(total, lane), 63, 64)) * a.heads;
+  ExpandedRange r{};
+  r.each = uniform_long(max((total + st.groups - 1) / st.groups, 1ll));
+  r.g0 = uniform_long(group * r.each);
+  r.g1 = uniform_long(min(r.g0 + r.each, total));
+  if (r.g0 >= r.g1) return r;
+  long long base = 0;
+  for (long long e0 = 0; e0 < entries; e0 += 64) {
+    const long long tiles = static_cast<long long>(entry_tiles<RB>(a, st.row_blocks, e0 + lane)) * a.heads;
+    const long long sum = lane_scan(tiles, lane);
+    const long long from = base + sum - tiles, to = base + sum;
+    const unsigned long long hit = __ballot(from <= r.g0 && r.g0 < to);
+    if (hit != 0) {
+      const int src = __ffsll(static_cast<long long>(hit)) - 1;
+      const long long e = e0 + src;
+      c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(e / a.batch));
+      c.b = __builtin_amdgcn_readfirstlane(static_cast<int>(e - static_cast<long long>(c.rb) * a.batch));
+      load_unit<RB>(a, c);
+      const long long in = r.g0 - uniform_long(__shfl(from, src, 64));
+      c.h = __builtin_amdgcn_readfirstlane(static_cast<int>(in / c.nb));
+      c.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(in - static_cast<long long>(c.h) * c.nb));
+      break;
+    }
+    base += uniform_long(__shfl(sum, 63, 64));
+  }
+  return r;
+}
+
+// The next unit's first place; only called where there is one.
+template <int RB>
+__device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, ExpandedCursor& c) {
+  c.blk = 0;
+  if (++c.h < a.heads) return;
+  c.h = 0;
+  do {
+    if (++c.b == a.batch) {
+      c.b = 0;
+      ++c.rb;
+    }
+    load_unit<RB>(a, c);
+  } while (c.nb == 0);
+}
+
+// RT tiles of 16 query rows a wavefront: units of RB = 64 RT rows.
+template <int RT>
+__device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const ExpandedStream& st,
+                                              ExpandedShared& sh) {
+  constexpr int RB = 16 * kWaves * RT;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int group = static_cast<int>(blockIdx.x);
+  auto barrier = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (tid == 0) st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
+  ExpandedCursor cur{};
+  const ExpandedRange range = first_place<RB>(a, st, group, lane, cur);
+  if (range.g0 >= range.g1) return;
+  const int blocks = static_cast<int>(range.g1 - range.g0);
+
+  // ---- staging: a thread has a key's chunks part, part + 8, .. of eight numbers.
+  const int srow = tid >> 3, part = tid & 7;
+  struct Source {  // a tile's rows
+    const float* k;
+    const float* r;
+    const float* v;
+    int first, length;  // its first key, and the sequence's number
+    int seen;           // keys that every row of the unit sees
+  };
+  auto source = [&](const ExpandedCursor& c) {
+    Source s{};
+    s.k = a.key + static_cast<std::size_t>(c.b) * a.key_at.batch +
+          static_cast<std::size_t>(c.h) * a.key_at.head;
+    s.r = a.rope_key + static_cast<std::size_t>(c.b) * a.rope_at.batch;
+    s.v = a.value + static_cast<std::size_t>(c.b) * a.value_at.batch +
+          static_cast<std::size_t>(c.h) * a.value_at.head;
+    s.first = c.blk * kTile;
+    s.length = c.length;
+    s.seen = c.first;
+    return s;
+  };
+  v4f raw_k[3][2], raw_v[2][2];  // (the third chunk of a key is the shared part's)
+  auto fetch_keys = [&](const Source& s) {
+    if (s.length == 0) return;  // (nothing is there, and nothing of it is used)
+    const std::size_t j = static_cast<std::size_t>(min(s.first + srow, s.length - 1));
+    const float* const k = s.k + j * a.key_at.token + part * 8;
+    const float* const r = s.r + j * a.rope_at.token + part * 8;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      raw_k[0][w] = *reinterpret_cast<const v4f*>(k + 4 * w);
+      raw_k[1][w] = *reinterpret_cast<const v4f*>(k + 64 + 4 * w);
+      raw_k[2][w] = *reinterpret_cast<const v4f*>(r + 4 * w);
+    }
+  };
+  auto fetch_values = [&](const Source& s) {
+    if (s.length == 0) return;
+    const std::size_t j = static_cast<std::size_t>(min(s.first + srow, s.length - 1));
+    const float* const v = s.v + j * a.value_at.token + part * 8;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      raw_v[0][w] = *reinterpret_cast<const v4f*>(v + 4 * w);
+      raw_v[1][w] = *reinterpret_cast<const v4f*>(v + 64 + 4 * w);
+    }
+  };
+  auto put = [&](unsigned char* to, std::size_t plane, unsigned at, const v4f (&x)[2]) {
+    unsigned w[4][kTerms];
+    split_pair(x[0][0], x[0][1], w[0]);
+    split_pair(x[0][2], x[0][3], w[1]);
+    split_pair(x[1][0], x[1][1], w[2]);
+    split_pair(x[1][2], x[1][3], w[3]);
+#pragma unroll
+    for (int i = 0; i < kTerms; ++i) {
+      *reinterpret_cast<v4u*>(to + i * plane + at) = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
+    }
+  };
+  auto put_key = [&](int buf, int i) {
+    put(sh.item[buf].k[0], sizeof(sh.item[buf].k[0]), key_place(srow, part + 8 * i), raw_k[i]);
+  };
+  auto put_value = [&](int buf, int i) {
+    put(sh.item[buf].v[0], sizeof(sh.item[buf].v[0]), value_place(srow, part + 8 * i), raw_v[i]);
+  };
+  // Values of keys that some row of the unit does not see must be finite: those
+  // behind the sequence's last become 0, and of the others those with terms that are
+  // not; the latter's keys are noted.
+  auto clean_values = [&](int buf, const Source& s) {
+    unsigned poison = 0;
+    if (s.first + kTile > s.seen) {
+      const int j = s.first + srow;
+      bool wild = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) wild = wild || !(fabsf(raw_v[i][w][n]) < kWild);
+      const unsigned long long hit = __ballot(wild && j >= s.seen && j < s.length);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (((hit >> (8 * r)) & 0xffull) != 0) poison |= 1u << (8 * wave + r);
+      }
+      const bool wipe = j >= s.length || ((poison >> (srow & 31)) & 1u) != 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) raw_v[i][w][n] = wipe ? 0.f : raw_v[i][w][n];
+    }
+    if (lane == 0) sh.poison[buf][wave] = poison;
+  };
+
+  // ---- the wavefront's rows of a unit: tile t's row `col`.
+  auto unit_row = [&](int t) { return (wave * RT + t) * 16 + col; };
+  v4u q[kSteps][RT][kTerms];
+  v4f o[RT][kDims];  // o[t][dt][i]: dim 16 dt + 4 grp + i of row col
+  float m[RT], l[RT];
+  int limit[RT];  // keys that the row sees
+  auto start = [&](const ExpandedCursor& c) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = c.rb * RB + unit_row(t);
+      const bool live = row < c.count;
+      limit[t] = c.length - c.count + row + 1;
+      const float* const src = a.query + static_cast<std::size_t>(c.b) * a.query_at.batch +
+                               static_cast<std::size_t>(c.h) * a.query_at.head +
+                               static_cast<std::size_t>(live ? row : 0) * a.query_at.token;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        v4f x[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          x[w] = *reinterpret_cast<const v4f*>(src + 32 * s + 8 * grp + 4 * w);
+          x[w] = live ? x[w] * a.qscale : v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        unsigned w[4][kTerms];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_pair(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1], w[i]);
+#pragma unroll
+        for (int i = 0; i < kTerms; ++i) {
+          q[s][t][i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
+          // (Queries live in the accumulation registers, all else in the others.)
+          asm("" : "+a"(q[s][t][i]));
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int dt = 0; dt < kDims; ++dt) o[t][dt] = v4f{0.f, 0.f, 0.f, 0.f};
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+    }
+  };
+
+  // Scores of a tile: sc[t][h][i] is key 16 h + 4 grp + i of tile t's row col.
+  unsigned key_at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) key_at[i] = key_place(col, 4 * i + grp);
+  auto scores = [&](int buf, v4f (&sc)[RT][2], auto&& beside) {
+    v4u k[2][kTerms];
+    auto read = [&](int u) {  // dims 32 (u / 2) and on of keys 16 (u % 2) and on
+      const int s = u / 2, h = u % 2;
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        // (Rows 16 and on are exchanged as rows 0 and on.)
+        k[u % 2][i] = *reinterpret_cast<const v4u*>(sh.item[buf].k[i] + key_at[s % 2] +
+                                                    (s / 2) * 128 + h * (16 * kKeyPitch));
+      }
+    };
+    read(0);
+    read(1);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) sc[t][0] = sc[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 2 * kSteps; ++u) {
+      const int s = u / 2, h = u % 2;
+      // Smallest products first.
+#pragma unroll
+      for (int sum = kTerms - 1; sum >= 0; --sum)
+#pragma unroll
+        for (int i = sum; i >= 0; --i)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) sc[t][h] = matrix_step(k[u % 2][i], q[s][t][sum - i], sc[t][h]);
+      if (u + 2 < 2 * kSteps) read(u + 2);
+      beside(u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // The reference follows the tile's largest scores.
+  auto follow = [&](const v4f (&sc)[RT][2]) {
+    float mx[RT];
+    bool above = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const v4f x = sc[t][0], y = sc[t][1];
+      mx[t] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                    fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+      above = above || mx[t] > m[t] + kSlack;
+    }
+    if (__ballot(above) != 0) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float mn = fmaxf(m[t], row_max(mx[t]));
+        const float alpha = exp2_ratio(m[t], mn);
+#pragma unroll
+        for (int dt = 0; dt < kDims; ++dt) o[t][dt] *= alpha;
+        l[t] *= alpha;
+        m[t] = mn;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // Scores of keys that a row does not see become -infinity, and NaN where `poison`
+  // has one that it sees.
+  auto mask = [&](int first, unsigned poison, v4f (&sc)[RT][2]) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = 16 * h + 4 * grp + i;
+          float x = sc[t][h][i];
+          if (((poison >> n) & 1u) != 0) x = NAN;
+          sc[t][h][i] = first + n < limit[t] ? x : -INFINITY;
+        }
+  };
+  struct Probabilities {
+    unsigned w[RT][4][kTerms];
+  };
+  auto probability = [&](int t, int n, const v4f (&sc)[RT][2], const float (&ref)[RT],
+                         Probabilities& p) {
+    const v4f x = sc[t][n / 2];
+    const float y0 = __builtin_amdgcn_exp2f(x[2 * (n % 2)] - ref[t]);
+    const float y1 = __builtin_amdgcn_exp2f(x[2 * (n % 2) + 1] - ref[t]);
+    l[t] += y0 + y1;
+    split_pair(y0, y1, p.w[t][n]);
+  };
+  const int vrow = 4 * grp + (col >> 2);
+  unsigned value_at[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    value_at[d] = value_place(vrow, 2 * d + ((col >> 1) & 1)) + (col & 1) * 8u;
+  }
+  auto add_values = [&](int buf, const Probabilities& p, auto&& beside) {
+    using LdsV4s = __attribute__((address_space(3))) v4s;
+    v4u pop[RT][kTerms];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        pop[t][i] = v4u{p.w[t][0][i], p.w[t][1][i], p.w[t][2][i], p.w[t][3][i]};
+      }
+    v4u v[2][kTerms];
+    auto read = [&](int dt) {
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        // (Chunks 8 and on lie where chunks 0 and on do, exchanged in their group.)
+        const unsigned char* const from = sh.item[buf].v[i] + (value_at[dt % 4] ^ (dt / 4 * 128u));
+        const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from));
+        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from + 16 * kValuePitch));
+        v[dt % 2][i] = __builtin_bit_cast(v4u, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+    };
+    read(0);
+    read(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int dt = 0; dt < kDims; ++dt) {
+#pragma unroll
+      for (int sum = kTerms - 1; sum >= 0; --sum)
+#pragma unroll
+        for (int i = sum; i >= 0; --i)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) o[t][dt] = matrix_step(v[dt % 2][i], pop[t][sum - i], o[t][dt]);
+      if (dt + 2 < kDims) read(dt + 2);
+      beside(dt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // ---- the range.  Step n: scores of tile n + 1 beside tile n's probabilities, tile
+  // n's outputs beside the way of item n + 2 into LDS, item n + 3 sent for.
+  ExpandedCursor ahead = cur;  // the tile whose keys are sent for
+  int located = 0;
+  Source now = source(ahead), before = now;  // its rows, and the last tile's
+  Source staged = now;                       // rows of the values in the registers
+  auto advance = [&] {
+    before = now;
+    if (located + 1 < blocks) {
+      if (++ahead.blk == ahead.nb) next_unit<RB>(a, ahead);
+      now = source(ahead);
+    }
+    ++located;
+  };
+  auto fetch = [&] {  // keys of tile `located`, values of the one before
+    fetch_keys(now);
+    fetch_values(before);
+    staged = before;
+    advance();
+  };
+  // Items 0 and 1.  (Item 0 has no values: what it puts there is not read.)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) raw_v[i][w] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) raw_k[i][w] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  auto store = [&](int buf) {
+    clean_values(buf, staged);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) put_key(buf, i);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) put_value(buf, i);
+  };
+  fetch();
+  store(0);
+  fetch();
+  store(1);
+  fetch();
+  barrier();
+  int n = 0;
+  for (;;) {
+    start(cur);
+    const int from = cur.blk;
+    const int to = min(cur.nb, cur.blk + (blocks - n));
+    const int whole = max(cur.first, 0) / kTile;  // tiles before are seen by every row
+    v4f sc[RT][2];
+    scores(n & 1, sc, [](int) {});
+    // (Item n's keys are taken before it is written again.)
+    barrier();
+    for (int blk = from; blk < to; ++blk) {
+      const int buf = (n + 1) & 1, into = n & 1;
+      if (blk >= whole) {
+        const unsigned poison = sh.poison[buf][0] | sh.poison[buf][1] | sh.poison[buf][2] |
+                                sh.poison[buf][3];
+        mask(blk * kTile, poison, sc);
+      }
+      follow(sc);
+      float ref[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) ref[t] = m[t] == -INFINITY ? 0.f : m[t];
+      Probabilities p;
+      if (blk + 1 < to) {
+        v4f last[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) last[t][h] = sc[t][h];
+        scores(buf, sc, [&](int u) {
+          if (u < 4 * RT) probability(u / 4, u % 4, last, ref, p);
+        });
+      } else {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) probability(t, i, sc, ref, p);
+      }
+      clean_values(into, staged);
+      add_values(buf, p, [&](int dt) {
+        if (dt < 3) put_key(into, dt);
+        if (dt >= 3 && dt < 5) put_value(into, dt - 3);
+      });
+      fetch();
+      ++n;
+      barrier();
+    }
+    // The part's end.
+    const bool complete = from == 0 && to == cur.nb;
+    const bool starts = from == 0;
+    const int slot = 2 * group + (starts ? 1 : 0);
+    if (to == cur.nb && !starts && tid == 0) {
+      const long long first = (range.g0 + n - to) / range.each;
+      st.jobs[group] = ExpandedJob{cur.b, cur.h, cur.rb, static_cast<int>(first), group};
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const float sum = row_sum(l[t]);
+      const int local = unit_row(t), row = cur.rb * RB + local;
+      if (row >= cur.count) continue;
+      // (A row that has seen nothing has neither sum nor outputs.)
+      const float f = !complete ? 1.0f : cur.bad != 0 ? NAN : sum == 0.f ? 0.f : 1.0f / sum;
+      float* const dst =
+          (complete ? a.out + static_cast<std::size_t>(cur.b) * a.out_at.batch +
+                          static_cast<std::size_t>(cur.h) * a.out_at.head +
+                          static_cast<std::size_t>(row) * a.out_at.token
+                    : st.part_o + (static_cast<std::size_t>(slot) * RB + local) * kValueDim) +
+          4 * grp;
+#pragma unroll
+      for (int dt = 0; dt < kDims; ++dt) *reinterpret_cast<v4f*>(dst + 16 * dt) = o[t][dt] * f;
+      if (!complete && grp == 0) {
+        float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * RB + local) * 2;
+        ml[0] = m[t];
+        ml[1] = cur.bad != 0 ? NAN : sum;
+      }
+    }
+    if (n == blocks) break;
+    next_unit<RB>(a, cur);
+  }
+}
+
+template <int RT>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+    void expanded_kernel(ExpandedKernelArgs a, ExpandedStream st) {
+  __shared__ ExpandedShared sh;
+  expanded_body<RT>(a, st, sh);
+}
+
+// Joins the partials of the units that cross ranges: the first group's second slot
+// and the later groups' first ones.  blockIdx.x is a group, a wavefront takes a row, a
+// lane two dims.
+__global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs a,
+                                                             ExpandedStream st, int rb_rows) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const ExpandedJob job = st.jobs[blockIdx.x];
+  if (job.b < 0) return;
+  const int local = static_cast<int>(blockIdx.y) * 4 + wave;
+  const int row = job.rb * rb_rows + local;
+  if (local >= rb_rows || row >= clamped_count(a, job.b)) return;
+  const int parts = job.last - job.first + 1;
+  auto slot = [&](int i) {
+    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + local;
+  };
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 64) top = fmaxf(top, st.part_ml[2 * slot(i)]);
+#pragma unroll
+  for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
+  float sum = 0.f;
+  v2f o = {0.f, 0.f};
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    float w = 0.f;
+    if (i0 + lane < parts) {
+      const float pl = st.part_ml[2 * slot(i0 + lane) + 1];
+      w = pl == 0.f ? 0.f : exp2_ratio(st.part_ml[2 * slot(i0 + lane)], top);
+      sum += pl * w;
+    }
+    const int end = min(parts - i0, 64);
+    for (int i = 0; i < end; i += 4) {
+      v2f x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        x[u] = reinterpret_cast<const v2f*>(st.part_o + slot(i0 + min(i + u, end - 1)) * kValueDim)[lane];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float wi = i + u < end ? __shfl(w, i + u, 64) : 0.f;
+        if (wi != 0.f) o += x[u] * wi;  // (a part that saw nothing has no outputs)
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
+  const float f = sum == 0.f ? 0.f : 1.0f / sum;
+  float* const dst = a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
+                     static_cast<std::size_t>(job.h) * a.out_at.head +
+                     static_cast<std::size_t>(row) * a.out_at.token;
+  reinterpret_cast<v2f*>(dst)[lane] = o * f;
+}
+
+// ----------------------------------------------------------------- host ----
+constexpr std::size_t kGroups = 256;  // a workgroup a CU: two items take 120 KB of LDS
+
+std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
+
+struct ExpandedLayout {
+  explicit ExpandedLayout(std::size_t tokens) {
+    rb = tokens <= 64 ? 64 : 128;
+    row_blocks = (tokens + rb - 1) / rb;
+    auto take = [&](std::size_t n) {
+      const std::size_t at = bytes;
+      bytes += align256(n);
+      return at;
+    };
+    jobs = take(kGroups * sizeof(ExpandedJob));
+    part_ml = take(2 * kGroups * rb * 2 * sizeof(float));
+    part_o = take(2 * kGroups * rb * kValueDim * sizeof(float));
+  }
+  std::size_t rb, row_blocks, jobs, part_ml, part_o, bytes = 0;
+};
 
 }  // namespace
 
-std::size_t expanded_workspace_bytes(std::size_t, std::size_t, std::size_t, std::size_t) {
-  return 16;
+std::size_t expanded_workspace_bytes(std::size_t, std::size_t, std::size_t tokens, std::size_t) {
+  return ExpandedLayout(tokens).bytes;
+}
+
+bool expanded_fits(const ExpandedArgs& a) {
+  // Ranges, and places in them, are counted in 32 bits: of 2^38 tiles, a group's are
+  // 2^30.
+  const std::size_t units = a.batch * a.heads * ((a.tokens + 63) / 64);
+  return units == 0 || a.keys / kTile + 2 <= (std::size_t{1} << 38) / units;
 }
 
 hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) {
   if (a.batch == 0 || a.heads == 0 || a.tokens == 0) return hipSuccess;
+  if (!expanded_fits(a)) return hipErrorInvalidValue;
+  const ExpandedLayout layout(a.tokens);
   ExpandedKernelArgs k{};
   k.query = a.query;
   k.key = a.key;
@@ -99,9 +761,24 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   k.tokens = static_cast<int>(a.tokens);
   k.keys = static_cast<int>(a.keys);
   k.qscale = kLog2e * a.scale;
-  const std::size_t rows = a.batch * a.heads * a.tokens;
-  if (rows > (std::size_t{1} << 32)) return hipErrorInvalidValue;
-  expanded_row_kernel<<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(k);
+  auto* const base = static_cast<unsigned char*>(a.workspace);
+  ExpandedStream st{};
+  st.jobs = reinterpret_cast<ExpandedJob*>(base + layout.jobs);
+  st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
+  st.part_o = reinterpret_cast<float*>(base + layout.part_o);
+  st.groups = static_cast<int>(kGroups);
+  st.row_blocks = static_cast<int>(layout.row_blocks);
+  const dim3 grid(static_cast<unsigned>(kGroups));
+  if (layout.rb == 64) {
+    expanded_kernel<1><<<grid, 64 * kWaves, 0, stream>>>(k, st);
+  } else {
+    expanded_kernel<2><<<grid, 64 * kWaves, 0, stream>>>(k, st);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const std::size_t rows = std::min(layout.rb, a.tokens);
+  expanded_merge_kernel<<<dim3(static_cast<unsigned>(kGroups), static_cast<unsigned>((rows + 3) / 4)),
+                          256, 0, stream>>>(k, st, static_cast<int>(layout.rb));
   return hipGetLastError();
 }
 

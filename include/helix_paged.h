@@ -639,8 +639,8 @@ int helix_paged_latent_attention(const float* query, const size_t* query_strides
  *   tokens) new tokens' the last: row t sees the first key_lengths[b] -
  *   token_counts[b] + t + 1.
  * All on 16 bytes with strides of four elements.  Rows that see nothing, rows behind
- * token_counts, lengths outside [0, keys], values that are not finite and the
- * workspace as above. */
+ * token_counts, lengths outside [0, keys], values that are not finite (here also
+ * numbers of 3.39e38 and more in size) and the workspace as above. */
 int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
                                          size_t* out);
 int helix_latent_prefill_attention(const float* query, const size_t* query_strides,
