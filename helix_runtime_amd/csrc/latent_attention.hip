@@ -841,9 +841,13 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
 #pragma unroll
           for (int h = 0; h < NH; ++h) now[h] = sc[h];
           constexpr int kEvery = R::NS / (R::kPairs + 1);
+          // (A copy that the compiler does not know, or it takes the exponentials of
+          // both cases out in front.)
+          float ref_here = ref;
+          asm("" : "+v"(ref_here));
           rows.scores(sh.tile[after], col, grp, sc, [&](int u) {
             if (u % kEvery == kEvery - 1 && u / kEvery < R::kPairs) {
-              rows.probability(u / kEvery, now, ref, p);
+              rows.probability(u / kEvery, now, ref_here, p);
             }
           });
         } else {

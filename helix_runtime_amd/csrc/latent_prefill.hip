@@ -306,22 +306,35 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
       raw_v[1][w] = *reinterpret_cast<const v4f*>(v + 64 + 4 * w);
     }
   };
-  auto put = [&](unsigned char* to, std::size_t plane, unsigned at, const v4f (&x)[2]) {
-    unsigned w[4][kTerms];
-    split_pair(x[0][0], x[0][1], w[0]);
-    split_pair(x[0][2], x[0][3], w[1]);
-    split_pair(x[1][0], x[1][1], w[2]);
-    split_pair(x[1][2], x[1][3], w[3]);
-#pragma unroll
-    for (int i = 0; i < kTerms; ++i) {
-      *reinterpret_cast<v4u*>(to + i * plane + at) = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
+  // The way into LDS in small parts, each one term of two numbers: a chunk's four pairs
+  // of numbers, then the next chunk's; its last part writes it.
+  constexpr int kStageParts = 5 * 4 * kTerms;
+  unsigned words[4][kTerms];
+  float sx = 0.f, sy = 0.f;
+  auto term = [](float& x, float& y) {  // the next term of x and y, and what it leaves
+    const unsigned t = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2bf));
+    x -= __uint_as_float(t << 16);
+    y -= __uint_as_float(t & 0xffff0000u);
+    return t;
+  };
+  auto stage = [&](int buf, int i) {
+    const int chunk = i / (4 * kTerms), pair = i / kTerms % 4, level = i % kTerms;
+    if (level == 0) {
+      const v4f x =
+          chunk < 3 ? raw_k[chunk < 3 ? chunk : 0][pair / 2] : raw_v[chunk < 3 ? 0 : chunk - 3][pair / 2];
+      sx = x[2 * (pair % 2)];
+      sy = x[2 * (pair % 2) + 1];
     }
-  };
-  auto put_key = [&](int buf, int i) {
-    put(sh.item[buf].k[0], sizeof(sh.item[buf].k[0]), key_place(srow, part + 8 * i), raw_k[i]);
-  };
-  auto put_value = [&](int buf, int i) {
-    put(sh.item[buf].v[0], sizeof(sh.item[buf].v[0]), value_place(srow, part + 8 * i), raw_v[i]);
+    words[pair][level] = term(sx, sy);
+    if (pair != 3 || level != kTerms - 1) return;
+    unsigned char* const to =
+        chunk < 3 ? sh.item[buf].k[0] + key_place(srow, part + 8 * chunk)
+                  : sh.item[buf].v[0] + value_place(srow, part + 8 * (chunk - 3));
+    const unsigned plane = chunk < 3 ? kTile * kKeyPitch : kTile * kValuePitch;
+#pragma unroll
+    for (int n = 0; n < kTerms; ++n) {
+      *reinterpret_cast<v4u*>(to + n * plane) = v4u{words[0][n], words[1][n], words[2][n], words[3][n]};
+    }
   };
   // Values of keys that some row of the unit does not see must be finite: those
   // behind the sequence's last become 0, and of the others those with terms that are
@@ -394,6 +407,15 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
     }
   };
 
+  // A matrix instruction takes 16 cycles, of which its issue takes 4: the RT ones of a
+  // product have other work put behind them, a part at a time.  (In one piece before
+  // or behind the products of a step, which is how the compiler would have it, the two
+  // add up: 925 us for 4 x 32 heads, 512 rows over 4096 keys.)
+  constexpr int kProducts = 6;
+  auto product = [](int sum, int i) {  // its place in the order below
+    return sum == 2 ? 2 - i : sum == 1 ? 4 - i : 5;
+  };
+
   // Scores of a tile: sc[t][h][i] is key 16 h + 4 grp + i of tile t's row col.
   unsigned key_at[2];
 #pragma unroll
@@ -421,12 +443,13 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
 #pragma unroll
       for (int sum = kTerms - 1; sum >= 0; --sum)
 #pragma unroll
-        for (int i = sum; i >= 0; --i)
+        for (int i = sum; i >= 0; --i) {
 #pragma unroll
           for (int t = 0; t < RT; ++t) sc[t][h] = matrix_step(k[u % 2][i], q[s][t][sum - i], sc[t][h]);
+          beside(kProducts * u + product(sum, i));
+          __builtin_amdgcn_sched_barrier(0);
+        }
       if (u + 2 < 2 * kSteps) read(u + 2);
-      beside(u);
-      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // The reference follows the tile's largest scores.
@@ -471,13 +494,18 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
   struct Probabilities {
     unsigned w[RT][4][kTerms];
   };
-  auto probability = [&](int t, int n, const v4f (&sc)[RT][2], const float (&ref)[RT],
-                         Probabilities& p) {
-    const v4f x = sc[t][n / 2];
-    const float y0 = __builtin_amdgcn_exp2f(x[2 * (n % 2)] - ref[t]);
-    const float y1 = __builtin_amdgcn_exp2f(x[2 * (n % 2) + 1] - ref[t]);
-    l[t] += y0 + y1;
-    split_pair(y0, y1, p.w[t][n]);
+  // In small parts: of two keys their exponentials, then a term each.
+  constexpr int kProbParts = RT * 4 * (1 + kTerms);
+  float py0 = 0.f, py1 = 0.f;
+  auto probability = [&](int i, const v4f (&sc)[RT][2], const float (&ref)[RT], Probabilities& p) {
+    const int pair = i / (1 + kTerms), level = i % (1 + kTerms), t = pair / 4, n = pair % 4;
+    if (level == 0) {
+      py0 = __builtin_amdgcn_exp2f(sc[t][n / 2][2 * (n % 2)] - ref[t]);
+      py1 = __builtin_amdgcn_exp2f(sc[t][n / 2][2 * (n % 2) + 1] - ref[t]);
+      return;
+    }
+    if (level == 1) l[t] += py0 + py1;
+    p.w[t][n][level - 1] = term(py0, py1);
   };
   const int vrow = 4 * grp + (col >> 2);
   unsigned value_at[4];
@@ -513,12 +541,13 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
 #pragma unroll
       for (int sum = kTerms - 1; sum >= 0; --sum)
 #pragma unroll
-        for (int i = sum; i >= 0; --i)
+        for (int i = sum; i >= 0; --i) {
 #pragma unroll
           for (int t = 0; t < RT; ++t) o[t][dt] = matrix_step(v[dt % 2][i], pop[t][sum - i], o[t][dt]);
+          beside(kProducts * dt + product(sum, i));
+          __builtin_amdgcn_sched_barrier(0);
+        }
       if (dt + 2 < kDims) read(dt + 2);
-      beside(dt);
-      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -556,9 +585,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
   auto store = [&](int buf) {
     clean_values(buf, staged);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) put_key(buf, i);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) put_value(buf, i);
+    for (int i = 0; i < kStageParts; ++i) stage(buf, i);
   };
   fetch();
   store(0);
@@ -587,26 +614,40 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
       float ref[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) ref[t] = m[t] == -INFINITY ? 0.f : m[t];
+      clean_values(into, staged);
       Probabilities p;
+      // Of the way into LDS, the parts that the scores' steps have room for.
+      constexpr int kRoom = 2 * kSteps * kProducts - kProbParts;
+      constexpr int kBeside = kRoom < kStageParts ? kRoom : kStageParts;
       if (blk + 1 < to) {
         v4f last[RT][2];
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
           for (int h = 0; h < 2; ++h) last[t][h] = sc[t][h];
-        scores(buf, sc, [&](int u) {
-          if (u < 4 * RT) probability(u / 4, u % 4, last, ref, p);
+        // (A copy that the compiler does not know, or it takes the exponentials of both
+        // cases out in front.)
+        float ref_here[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          ref_here[t] = ref[t];
+          asm("" : "+v"(ref_here[t]));
+        }
+        scores(buf, sc, [&](int i) {
+          if (i < kProbParts) {
+            probability(i, last, ref_here, p);
+          } else if (i - kProbParts < kBeside) {
+            stage(into, i - kProbParts);
+          }
         });
       } else {
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int i = 0; i < kProbParts; ++i) probability(i, sc, ref, p);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) probability(t, i, sc, ref, p);
+        for (int i = 0; i < kBeside; ++i) stage(into, i);
       }
-      clean_values(into, staged);
-      add_values(buf, p, [&](int dt) {
-        if (dt < 3) put_key(into, dt);
-        if (dt >= 3 && dt < 5) put_value(into, dt - 3);
+      add_values(buf, p, [&](int i) {
+        if (i + kBeside < kStageParts) stage(into, i + kBeside);
       });
       fetch();
       ++n;
