@@ -61,6 +61,7 @@ using prefill_detail::v8bf;
 
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -147,29 +148,33 @@ __device__ __forceinline__ v4u codes_fp16(unsigned w0, unsigned w1) {
 }
 
 // A tile in LDS: rows of kPitch bytes, whose 16-byte chunks are exchanged within
-// groups of kMask + 1 by an exclusive or with `turn` of the row.  A read of one chunk
-// of 16 rows (scores) and one of 32 bytes of 8 rows, or 64 of 4 (outputs), then hit
-// distinct banks: rows lie 1152 or 640 bytes apart, 128 from a multiple of 256, and
-// fp32 rows on one.
-template <int PF, int L>
+// groups of kMask + 1 by an exclusive or with `turn` of the row.  A read of a chunk of
+// 16 rows (scores) and one of 16 dims of 4 or 8 rows (outputs) then hit distinct
+// banks: 16-bit rows lie 1152 or 640 bytes apart, 128 from a multiple of 256, fp32 rows
+// on one, and rows of codes 64 from one.  fp8 codes become fp16 on their way into LDS
+// where four wavefronts read them (SHARED), else as they are read.
+template <int PF, int L, bool SHARED>
 struct Tile {
   static constexpr int W = L + static_cast<int>(kLatentRope);
-  static constexpr int kElem = PF == 0 ? 4 : 2;            // bytes in LDS
+  static constexpr bool kCodes = PF == 2 && !SHARED;
+  static constexpr int kElem = PF == 0 ? 4 : kCodes ? 1 : 2;  // bytes in LDS
   static constexpr int kPageElem = PF == 0 ? 4 : PF == 1 ? 2 : 1;
   static constexpr int kTokens = PF == 0 ? 16 : 32;
   static constexpr int kPages = kTokens / P;
   static constexpr int kPitch = W * kElem;
   static constexpr int kBytes = kTokens * kPitch;
-  static constexpr unsigned kMask = PF == 0 ? 15 : 7;
-  // Loads of 16 bytes a lane (fp8: 8) come in four groups of kLoads, a group being
-  // 8 whole rows (fp32: 4).
+  static constexpr unsigned kMask = PF == 0 ? 15 : kCodes ? 3 : 7;
+  // Loads of 16 bytes a lane (8, of codes that become fp16) come in kGroups groups of
+  // kLoads, a group being kGroupRows whole rows.
   static constexpr int kLoads = W / 64;
-  static constexpr int kGroupRows = PF == 0 ? 4 : 8;
-  static_assert(4 * kLoads * 1024 == kBytes && kGroupRows * kPitch == kLoads * 1024);
+  static constexpr int kGroups = kCodes ? 2 : 4;
+  static constexpr int kGroupRows = kTokens / kGroups;
+  static_assert(kGroups * kLoads * 1024 == kBytes && kGroupRows * kPitch == kLoads * 1024);
   static constexpr std::size_t kPageBytes = static_cast<std::size_t>(P) * W * kPageElem;
   static __device__ __forceinline__ unsigned turn(int row) {
-    return PF == 0 ? static_cast<unsigned>(row & 15)
-                   : static_cast<unsigned>((row & 6) | ((row >> 3) & 1));
+    if constexpr (PF == 0) return static_cast<unsigned>(row & 15);
+    if constexpr (kCodes) return static_cast<unsigned>(((row >> 2) & 3) ^ ((row >> 3) & 2));
+    return static_cast<unsigned>((row & 6) | ((row >> 3) & 1));
   }
 };
 
@@ -275,9 +280,9 @@ __device__ __forceinline__ void next_unit(const LatentKernelArgs& a, LatentCurso
 
 // One wavefront's 16 rows of a unit: queries, outputs, references and sums, and what
 // a tile in LDS does to them.
-template <int PF, int L>
+template <int PF, int L, bool SHARED>
 struct LatentRows {
-  using T = Tile<PF, L>;
+  using T = Tile<PF, L, SHARED>;
   static constexpr int QT = PF == 0 ? 1 : PF == 1 ? 3 : 2;  // terms
   static constexpr int NS = PF == 0 ? T::W / 16 : T::W / 32;  // steps of the scores' sum
   static constexpr int ND = L / 16;                           // tiles of output dims
@@ -303,55 +308,54 @@ struct LatentRows {
                              static_cast<std::size_t>(t) * a.query_at.token;
     m = -INFINITY;
     l = 0.f;
+    // All of the row's loads at once.  (A row that is none reads the sequence's first
+    // one; nothing of what comes of it is kept.)
+    constexpr int NX = PF == 0 ? 1 : 2;
+    v4f x[NS][NX];
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
-    // (A row that is none reads the sequence's first one.)
-    auto number = [&](int at) {
-      const v4f x = *reinterpret_cast<const v4f*>(src + at);
-      return live ? x : v4f{0.f, 0.f, 0.f, 0.f};
-    };
-    if constexpr (PF == 0) {
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        q[s][0] = __builtin_bit_cast(v4u, number(16 * s + 4 * grp) * a.qscale);
-        keep(s);
+      for (int w = 0; w < NX; ++w) {
+        x[s][w] = *reinterpret_cast<const v4f*>(src + 16 * NX * s + 4 * NX * grp + 4 * w);
       }
-    } else {
-      float grow = a.qscale;
-      if constexpr (PF == 2) {
-        float most = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    float grow = a.qscale;
+    if constexpr (PF == 2) {
+      float most = 0.f;
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const v4f x = number(32 * s + 8 * grp + 4 * w);
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])),
-                                     fmaxf(fabsf(x[2]), fabsf(x[3]))));
-          }
-        asm volatile("" ::: "memory");  // (or what was read stays in registers)
-        most = row_max(most);
-        // most * 2^(10 - e) in [2^10, 2^11), as far as 2^(10 - e) is a normal number.
-        const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -110), 120);
-        grow = __uint_as_float(static_cast<unsigned>(127 + 10 - e) << 23);
-        unscale = __uint_as_float(static_cast<unsigned>(127 - 10 + e) << 23);
-        // (Positive, or scores of -infinity would not stay that: the score scale's
-        // sign goes with the queries, which a scale of 0 makes 0.)
-        grow = a.qscale > 0.f ? grow : a.qscale < 0.f ? -grow : 0.f;
-        unscale = fmaxf(unscale * fabsf(a.qscale), 1.2e-38f);
-      }
+        for (int w = 0; w < NX; ++w) {
+          const v4f y = x[s][w];
+          most = fmaxf(most, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+        }
+      most = row_max(most);
+      // most * 2^(10 - e) in [2^10, 2^11), as far as 2^(10 - e) is a normal number.
+      const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -110), 120);
+      grow = __uint_as_float(static_cast<unsigned>(127 + 10 - e) << 23);
+      unscale = __uint_as_float(static_cast<unsigned>(127 - 10 + e) << 23);
+      // (Positive, or scores of -infinity would not stay that: the score scale's
+      // sign goes with the queries, which a scale of 0 makes 0.)
+      grow = a.qscale > 0.f ? grow : a.qscale < 0.f ? -grow : 0.f;
+      unscale = fmaxf(unscale * fabsf(a.qscale), 1.2e-38f);
+    }
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const v4f x[2] = {number(32 * s + 8 * grp), number(32 * s + 8 * grp + 4)};
+    for (int s = 0; s < NS; ++s) {
+      if constexpr (PF == 0) {
+        q[s][0] = __builtin_bit_cast(v4u, x[s][0] * grow);
+      } else {
         unsigned w[4][3];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          split_pair<PF>(x[i >> 1][2 * (i & 1)] * grow, x[i >> 1][2 * (i & 1) + 1] * grow, w[i]);
+          split_pair<PF>(x[s][i >> 1][2 * (i & 1)] * grow, x[s][i >> 1][2 * (i & 1) + 1] * grow, w[i]);
         }
 #pragma unroll
         for (int i = 0; i < QT; ++i) q[s][i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
-        keep(s);
       }
+      keep(s);
     }
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
   }
 
   // Half a wavefront's registers are accumulation registers, which matrix instructions
@@ -360,7 +364,6 @@ struct LatentRows {
   __device__ __forceinline__ void keep(int s) {
 #pragma unroll
     for (int i = 0; i < QT; ++i) asm("" : "+a"(q[s][i]));
-    if (s % 6 == 5) __builtin_amdgcn_sched_barrier(0);
   }
 
   // Scores of a tile: sc[h][i] is token 16 h + 4 grp + i of row col.  `beside(u)` is
@@ -368,22 +371,28 @@ struct LatentRows {
   template <typename F>
   __device__ __forceinline__ void scores(const unsigned char* tile, int col, int grp, v4f (&sc)[NH],
                                          F&& beside) const {
-    constexpr int A = PF == 0 ? 4 : 2;  // operands come out of LDS A steps ahead
-    // Row col's chunk 4 s + grp: its place within a group of chunks is one of two
-    // (fp32 pages: four), by s.
+    constexpr int A = PF == 0 ? 4 : T::kCodes ? 3 : 2;  // operands come out of LDS A steps ahead
+    // Row col's chunk 4 s + grp (codes: half of chunk 2 s + grp / 2): its place within
+    // a group of chunks is one of two (fp32 pages: four), by s.
     constexpr int V = PF == 0 ? 4 : 2;
-    unsigned at[V];
+    constexpr int C = T::kCodes ? 2 : 4;  // chunks of a step
+    unsigned at[V][NH];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      at[i] = static_cast<unsigned>(col * T::kPitch) +
-              ((static_cast<unsigned>(4 * i + grp) ^ T::turn(col)) & T::kMask) * 16u;
-    }
-    v4u k[A][NH];
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const int row = 16 * h + col;
+        const int chunk = C * i + (T::kCodes ? grp / 2 : grp);
+        at[i][h] = static_cast<unsigned>(row * T::kPitch) +
+                   ((static_cast<unsigned>(chunk) ^ T::turn(row)) & T::kMask) * 16u +
+                   (T::kCodes ? (grp % 2) * 8u : 0u);
+      }
+    using Operand = std::conditional_t<T::kCodes, v2u, v4u>;
+    Operand raw[A][NH];
     auto read = [&](int s) {
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {  // (rows 16 h and on turn as rows 0 and on do)
-        k[s % A][h] = *reinterpret_cast<const v4u*>(tile + at[s % V] + (s / V) * (V * 64) +
-                                                    h * (16 * T::kPitch));
+      for (int h = 0; h < NH; ++h) {
+        raw[s % A][h] = *reinterpret_cast<const Operand*>(tile + at[s % V][h] + (s / V) * (V * C * 16));
       }
     };
 #pragma unroll
@@ -394,17 +403,26 @@ struct LatentRows {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       if constexpr (PF == 0) {
-        const v4f x = __builtin_bit_cast(v4f, k[s % A][0]), y = __builtin_bit_cast(v4f, q[s][0]);
+        const v4f x = __builtin_bit_cast(v4f, raw[s % A][0]), y = __builtin_bit_cast(v4f, q[s][0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[0], 0, 0, 0);
         }
       } else {
-        // Smallest products first; one half's sum waits while the other's runs.
+        v4u k[NH];
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          if constexpr (T::kCodes) {
+            k[h] = codes_fp16(raw[s % A][h][0], raw[s % A][h][1]);
+          } else {
+            k[h] = raw[s % A][h];
+          }
+        }
+        // Smallest products first.
 #pragma unroll
         for (int i = QT - 1; i >= 0; --i)
 #pragma unroll
-          for (int h = 0; h < NH; ++h) sc[h] = matrix_step<PF>(k[s % A][h], q[s][i], sc[h]);
+          for (int h = 0; h < NH; ++h) sc[h] = matrix_step<PF>(k[h], q[s][i], sc[h]);
       }
       if (s + A < NS) read(s + A);
       beside(s);
@@ -506,32 +524,50 @@ struct LatentRows {
       v4u pop[QT];
 #pragma unroll
       for (int i = 0; i < QT; ++i) pop[i] = v4u{p.w[0][i], p.w[1][i], p.w[2][i], p.w[3][i]};
-      // 32 bytes (16 dims) of tokens 4 grp .. + 3, a quarter of them a lane: chunks
-      // 2 dt and 2 dt + 1 of row 4 grp + col / 4.
-      const int row = 4 * grp + (col >> 2);
-      unsigned at[4];
+      // 16 dims of tokens 4 grp .. + 3 and 16 + 4 grp .. + 3: 32 bytes a token, which
+      // four lanes read (codes: 16 bytes, two lanes), and each lane gets a dim.
+      using LdsV2i = __attribute__((address_space(3))) v2i;
+      constexpr int V = 4;
+      const int row = T::kCodes ? 4 * grp + ((col >> 1) & 3) + 2 * (col & 8) : 4 * grp + (col >> 2);
+      unsigned at[V];
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
+      for (int d = 0; d < V; ++d) {
+        const int chunk = T::kCodes ? d : 2 * d + ((col >> 1) & 1);
         at[d] = static_cast<unsigned>(row * T::kPitch) +
-                ((static_cast<unsigned>(2 * d + ((col >> 1) & 1)) ^ T::turn(row)) & T::kMask) * 16u +
-                (col & 1) * 8u;
+                ((static_cast<unsigned>(chunk) ^ T::turn(row)) & T::kMask) * 16u + (col & 1) * 8u;
       }
-      v4u v[A];
+      using Operand = std::conditional_t<T::kCodes, v2i, v4u>;
+      Operand raw[A];
       auto read = [&](int dt) {
-        const unsigned char* const from = tile + at[dt % 4] + (dt / 4) * 128;
-        const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from));
-        const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from + 16 * T::kPitch));
-        v[dt % A] = __builtin_bit_cast(v4u, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        const unsigned char* const from = tile + at[dt % V] + (dt / V) * (T::kCodes ? 64 : 128);
+        if constexpr (T::kCodes) {
+          raw[dt % A] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsV2i*)(from));
+        } else {
+          const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from));
+          const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from + 16 * T::kPitch));
+          raw[dt % A] =
+              __builtin_bit_cast(v4u, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
       };
 #pragma unroll
       for (int dt = 0; dt < A; ++dt) read(dt);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int dt = 0; dt < ND; dt += 2) {
+        v4u v[2];
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          if constexpr (T::kCodes) {
+            v[d] = codes_fp16(static_cast<unsigned>(raw[(dt + d) % A][0]),
+                              static_cast<unsigned>(raw[(dt + d) % A][1]));
+          } else {
+            v[d] = raw[(dt + d) % A];
+          }
+        }
 #pragma unroll
         for (int i = QT - 1; i >= 0; --i)
 #pragma unroll
-          for (int d = dt; d < dt + 2; ++d) o[d] = matrix_step<PF>(v[d % A], pop[i], o[d]);
+          for (int d = 0; d < 2; ++d) o[dt + d] = matrix_step<PF>(v[d], pop[i], o[dt + d]);
         if (dt + A < ND) {
           read(dt + A);
           read(dt + A + 1);
@@ -557,9 +593,10 @@ struct LatentRows {
 };
 
 // Where the pages' elements of a tile come from, and their way into LDS.
-template <int PF, int L>
+template <int PF, int L, bool SHARED>
 struct TileLoader {
-  using T = Tile<PF, L>;
+  using T = Tile<PF, L, SHARED>;
+  static constexpr bool kConvert = PF == 2 && SHARED;
   unsigned off[T::kLoads];  // of the lane's bytes in a group of rows
 
   __device__ __forceinline__ void start(int lane) {
@@ -568,20 +605,20 @@ struct TileLoader {
       const unsigned o = static_cast<unsigned>(i * 1024 + lane * 16);
       const unsigned row = o / T::kPitch, c = (o - row * T::kPitch) / 16;
       const unsigned from = c ^ (T::turn(static_cast<int>(row)) & T::kMask);
-      off[i] = (row * T::kPitch + from * 16) / (PF == 2 ? 2 : 1);
+      off[i] = (row * T::kPitch + from * 16) / (kConvert ? 2 : 1);
     }
   }
   // Group g's rows lie in page g / (groups of a page); their turns differ from the
   // first group's by one exchange.
   static constexpr int kPageGroups = P / T::kGroupRows;
   static __device__ __forceinline__ unsigned exchange(int g) {
-    return PF == 0 ? 64u * g : PF == 1 ? 16u * (g & 1) : 8u * (g & 1);
+    return PF == 0 ? 64u * g : T::kCodes ? 32u * g : kConvert ? 8u * (g & 1) : 16u * (g & 1);
   }
   static __device__ __forceinline__ const unsigned char* group_base(const unsigned char* page,
                                                                     int g) {
     return page + (g % kPageGroups) * (T::kGroupRows * T::W * T::kPageElem);
   }
-  // Straight into LDS (bf16 and fp32 pages).
+  // Straight into LDS.
   __device__ __forceinline__ void direct(const unsigned char* page, int g, unsigned lds) const {
     const unsigned char* const base = group_base(page, g);
 #pragma unroll
@@ -589,7 +626,7 @@ struct TileLoader {
       lds_load16_at(base, off[i] ^ exchange(g), lds + (g * T::kLoads + i) * 1024u);
     }
   }
-  // fp8 codes into registers, and from there as fp16 into LDS.
+  // Codes into registers, and from there as fp16 into LDS.
   __device__ __forceinline__ void fetch(const unsigned char* page, int g, v2u (&raw)[T::kLoads]) const {
     using Global = const __attribute__((address_space(1))) v2u*;
     using GlobalBytes = const __attribute__((address_space(1))) unsigned char*;
@@ -614,10 +651,10 @@ struct TileLoader {
 // behind the sequence's last become 0, and of the step's own tokens those that are
 // not finite; the latter's bits are returned.  Rows 4 `wave` and on by 16 (4 rows at a
 // time, 16 lanes each).
-template <int PF, int L>
+template <int PF, int L, bool SHARED>
 __device__ __forceinline__ unsigned clean_rows(unsigned char* tile, int first, int from, int length,
                                                int lane, int row0, int row_step) {
-  using T = Tile<PF, L>;
+  using T = Tile<PF, L, SHARED>;
   unsigned poison = 0;
   for (int r = row0 + (lane >> 4); r < T::kTokens; r += row_step) {
     unsigned char* const row = tile + r * T::kPitch;
@@ -631,6 +668,8 @@ __device__ __forceinline__ unsigned clean_rows(unsigned char* tile, int first, i
         for (int i = 0; i < 4; ++i) {
           if constexpr (PF == 0) {
             all |= (x[i] & 0x7f800000u) == 0x7f800000u;
+          } else if constexpr (T::kCodes) {
+            all |= (((x[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
           } else {
             constexpr unsigned e = PF == 1 ? 0x7f80u : 0x7c00u;
             all |= (x[i] & e) == e || ((x[i] >> 16) & e) == e;
@@ -652,18 +691,13 @@ __device__ __forceinline__ unsigned clean_rows(unsigned char* tile, int first, i
 
 template <int PF, int L, bool SHARED>
 struct LatentShared {
-  using T = Tile<PF, L>;
+  using T = Tile<PF, L, SHARED>;
+  // A wavefront by itself has one tile, or two of codes.
+  static constexpr int kRing = T::kCodes ? 2 : 1;
   static constexpr int kBuffers = SHARED ? (PF == 2 ? 3 : 4) : kWaves;
-  __align__(1024) unsigned char tile[kBuffers][T::kBytes];
+  __align__(1024) unsigned char tile[kBuffers][(SHARED ? 1 : kRing) * T::kBytes];
   float ml[kWaves][16][2];
   unsigned poison[kWaves];
-};
-
-// The rows of a finished part, or of a whole unit, from a wavefront.
-struct LatentOutput {
-  int slot;       // of the partial
-  bool complete;  // a whole unit
-  bool bad;
 };
 
 template <int PF, int L>
@@ -678,8 +712,9 @@ __device__ __forceinline__ float finish_factor(const LatentKernelArgs& a, bool c
 template <int PF, int L, bool SHARED>
 __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const LatentStream& st,
                                             LatentShared<PF, L, SHARED>& sh) {
-  using T = Tile<PF, L>;
-  using R = LatentRows<PF, L>;
+  using T = Tile<PF, L, SHARED>;
+  using R = LatentRows<PF, L, SHARED>;
+  using Loader = TileLoader<PF, L, SHARED>;
   constexpr int KT = T::kTokens;
   constexpr int RB = SHARED ? 16 * kWaves : 16;
   constexpr int NH = R::NH;
@@ -700,30 +735,40 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
   if (range.g0 >= range.g1) return;
   const int blocks = static_cast<int>(range.g1 - range.g0);
 
-  TileLoader<PF, L> loader;
+  Loader loader;
   loader.start(lane);
   const auto* const pool = static_cast<const unsigned char*>(a.pool);
-  // Pages of tile blk of the cursor's sequence.  Behind its tokens the last page
-  // is read again, and without tokens, or where a page is none, page 0; what is read
-  // there takes no part.
+  // The pages of a sequence being loaded, 64 at a time: lane i holds page pages_at + i
+  // of pages_of.  Behind its tokens the last page is read again, and without tokens,
+  // or where a page is none, page 0; what is read there takes no part.
+  unsigned page_lane = 0;
+  int pages_of = -1, pages_at = 0, bad_page = 0;
   struct Pages {
     const unsigned char* at[T::kPages];
     int bad;
   };
   auto locate = [&](const LatentCursor& c, int blk) {
     Pages p{};
-    p.bad = c.bad;
-    const std::uint32_t* const table = a.tables + static_cast<std::size_t>(c.b) * a.max_blocks;
-    const int last = (c.length - 1) / P;
+    int first = blk * T::kPages - pages_at;
+    if (__builtin_expect(pages_of != c.b || first < 0 || first + T::kPages > 64, 0)) {
+      pages_of = c.b;
+      pages_at = blk * T::kPages;
+      first = 0;
+      page_lane = 0;
+      bad_page = c.bad;
+      if (c.length > 0) {
+        page_lane = a.tables[static_cast<std::size_t>(c.b) * a.max_blocks +
+                             min(pages_at + lane, (c.length - 1) / P)];
+        const bool outside = page_lane >= a.physical_blocks;
+        if (__ballot(outside) != 0) bad_page = 1;
+        if (outside) page_lane = 0;
+      }
+    }
+    p.bad = bad_page;
 #pragma unroll
     for (int i = 0; i < T::kPages; ++i) {
-      std::uint32_t page = 0;
-      if (c.length > 0) page = uniform_read(table + min(blk * T::kPages + i, last));
-      if (page >= a.physical_blocks) {
-        p.bad = 1;
-        page = 0;
-      }
-      p.at[i] = pool + page * T::kPageBytes;
+      p.at[i] = pool + static_cast<unsigned>(__builtin_amdgcn_readlane(page_lane, first + i)) *
+                           T::kPageBytes;
     }
     return p;
   };
@@ -731,7 +776,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     if constexpr (T::kPages == 1) {
       return p.at[0];
     } else {
-      return g < TileLoader<PF, L>::kPageGroups ? p.at[0] : p.at[1];
+      return g < Loader::kPageGroups ? p.at[0] : p.at[1];
     }
   };
 
@@ -784,7 +829,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     // goes to LDS first).
     auto send = [&] {
       if constexpr (PF == 2) {
-        TileLoader<PF, L>::store(sh.tile[into], wave, lane, raw);
+        Loader::store(sh.tile[into], wave, lane, raw);
         loader.fetch(page_of(next, wave), wave, raw);
       } else {
         loader.direct(page_of(next, wave), wave, lds0 + static_cast<unsigned>(into) * T::kBytes);
@@ -823,7 +868,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
         int after = buf;
         bump(after);
         if (blk >= whole) {
-          unsigned poison = clean_rows<PF, L>(sh.tile[buf], blk * KT, cur.length - cur.count + 1,
+          unsigned poison = clean_rows<PF, L, SHARED>(sh.tile[buf], blk * KT, cur.length - cur.count + 1,
                                               cur.length, lane, 4 * wave, 16);
 #pragma unroll
           for (int bit = 16; bit < 64; bit *= 2) poison |= __shfl_xor(poison, bit, 64);
@@ -884,9 +929,9 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     // (Nothing is on its way into LDS when the workgroup gives it back.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   } else {
-    unsigned char* const tile = sh.tile[wave];
-    const unsigned lds = lds_address(tile);
-    v2u raw[4][PF == 2 ? T::kLoads : 1];
+    constexpr int kRing = LatentShared<PF, L, SHARED>::kRing;
+    unsigned char* const own_tiles = sh.tile[wave];
+    const unsigned lds = lds_address(own_tiles);
     int n = 0;
     for (;;) {
       const int row = cur.rb * RB + col;
@@ -894,33 +939,32 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       const int to = min(cur.nb, cur.blk + (blocks - n));
       const int whole = max(cur.length - cur.count + 1, 0) / KT;
       int bad = 0;
-      auto send = [&](int blk) {
+      // The wavefront's i-th tile of the part into its place.
+      auto send = [&](int i) {
+        const int blk = from + wave + i * kWaves;
+        if (blk >= to) return;
         const Pages p = locate(cur, blk);
         bad |= p.bad;
+        const unsigned into = lds + static_cast<unsigned>(i % kRing) * T::kBytes;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if constexpr (PF == 2) {
-            loader.fetch(page_of(p, g), g, raw[g]);
-          } else {
-            loader.direct(page_of(p, g), g, lds);
-          }
-        }
+        for (int g = 0; g < T::kGroups; ++g) loader.direct(page_of(p, g), g, into);
       };
-      if (from + wave < to) send(from + wave);
-      rows.start(a, cur, row, grp);
-      for (int blk = from + wave; blk < to; blk += kWaves) {
-        if constexpr (PF == 2) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g) TileLoader<PF, L>::store(tile, g, lane, raw[g]);
-          if (blk + kWaves < to) send(blk + kWaves);
+      for (int i = 0; i < kRing; ++i) send(i);
+      rows.start(a, cur, row, grp);
+      for (int i = 0; from + wave + i * kWaves < to; ++i) {
+        const int blk = from + wave + i * kWaves;
+        if (kRing > 1 && blk + kWaves < to) {  // the next tile is on its way behind it
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::kGroups * T::kLoads) : "memory");
         } else {
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
+        unsigned char* const tile = own_tiles + (i % kRing) * T::kBytes;
         v4f sc[NH];
         rows.scores(tile, col, grp, sc, [](int) {});
         if (blk >= whole) {
-          unsigned poison = clean_rows<PF, L>(tile, blk * KT, cur.length - cur.count + 1, cur.length,
-                                              lane, 0, 4);
+          unsigned poison = clean_rows<PF, L, SHARED>(tile, blk * KT, cur.length - cur.count + 1,
+                                                      cur.length, lane, 0, 4);
 #pragma unroll
           for (int bit = 16; bit < 64; bit *= 2) poison |= __shfl_xor(poison, bit, 64);
           rows.mask(blk * KT, poison, grp, sc);
@@ -929,16 +973,13 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
         const float ref = rows.reference();
         typename R::Probabilities p;
 #pragma unroll
-        for (int i = 0; i < R::kPairs; ++i) rows.probability(i, sc, ref, p);
+        for (int j = 0; j < R::kPairs; ++j) rows.probability(j, sc, ref, p);
         rows.add_values(tile, col, grp, p);
-        if constexpr (PF != 2) {
-          if (blk + kWaves < to) {
-            // (The tile's reads are done before it is written again.)
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            send(blk + kWaves);
-          }
-        }
+        // (The tile's reads are done before it is written again.)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        send(i + kRing);
       }
+      unsigned char* const tile = own_tiles;
       // The wavefronts join what they have: each one's outputs, relative to the
       // largest reference, in its tile.
       const float own = row_sum(rows.l);
@@ -1020,12 +1061,17 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 
 // and the later groups' first ones.  blockIdx.x is a unit or a group, blockIdx.y a row
 // (SPLIT: the wavefronts share its partials) or four rows.
 constexpr int kMostParts = 512;
+template <bool SPLIT>
+constexpr int merge_waves() {
+  return SPLIT ? 8 : 4;
+}
 template <int L, bool SPLIT>
-__global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, LatentStream st,
+__global__ __launch_bounds__(64 * merge_waves<SPLIT>()) void latent_merge_kernel(LatentKernelArgs a, LatentStream st,
                                                            int rb_rows) {
   constexpr int NV = L / 256;  // 4 dims each
-  __shared__ v4f sums[SPLIT ? 4 : 1][SPLIT ? L / 4 : 1];
-  __shared__ float weights[4][kMostParts];
+  constexpr int NW = merge_waves<SPLIT>();
+  __shared__ v4f sums[SPLIT ? NW : 1][SPLIT ? L / 4 : 1];
+  __shared__ float weights[NW][kMostParts];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   if (st.by_unit != 0 && clamped_count(a, static_cast<int>(blockIdx.x) % a.batch) == 0) return;
@@ -1055,8 +1101,8 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
     }
 #pragma unroll
     for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
-    constexpr int U = 4;  // partials on their way
-    const int step = SPLIT ? 4 : 1;
+    constexpr int U = SPLIT ? 8 : 4;  // partials on their way
+    constexpr int step = SPLIT ? NW : 1;
     for (int i0 = SPLIT ? wave : 0; i0 < parts; i0 += U * step) {
       v4f x[U][NV];
 #pragma unroll
@@ -1085,8 +1131,9 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
     if (wave != 0) return;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      o[v] = (sums[0][64 * v + lane] + sums[1][64 * v + lane]) +
-             (sums[2][64 * v + lane] + sums[3][64 * v + lane]);
+      o[v] = sums[0][64 * v + lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) o[v] += sums[w][64 * v + lane];
     }
   }
   if (!live) return;
@@ -1139,7 +1186,7 @@ hipError_t launch_latent(const LatentKernelArgs& k, const LatentStream& st, std:
   // Few units: all wavefronts of a workgroup on one row.
   if (jobs * rows <= 2048) {
     latent_merge_kernel<L, true>
-        <<<dim3(static_cast<unsigned>(jobs), rows), 256, 0, stream>>>(k, st, static_cast<int>(rb));
+        <<<dim3(static_cast<unsigned>(jobs), rows), 64 * merge_waves<true>(), 0, stream>>>(k, st, static_cast<int>(rb));
   } else {
     latent_merge_kernel<L, false><<<dim3(static_cast<unsigned>(jobs), (rows + 3) / 4), 256, 0, stream>>>(
         k, st, static_cast<int>(rb));
