@@ -8,7 +8,7 @@
 // Work split.  16 or 64 of a sequence's rows form a unit; one pass over the
 // sequence's tokens serves them all.  A unit's tokens are tiles of 32 (fp32 pages:
 // 16).  A fixed grid of workgroups takes equal ranges of the flat list of all units'
-// tiles, whatever the lengths.  A unit inside one range is finished there; one that
+// tiles, whatever the lengths (and of what units cost beside their tiles).  A unit inside one range is finished there; one that
 // crosses ranges leaves a partial (maximum, sum, output) per range, and
 // latent_merge_kernel joins them.  A workgroup leaves at most two partials, its first
 // unit's and its last one's, so the workspace depends on the grid, not on the batch.
@@ -178,9 +178,21 @@ struct Tile {
   }
 };
 
-// A place in the flat list of tiles.
+// What a unit's start costs a workgroup that has begun with another one, in tiles: its
+// queries have to come and be split, its first tiles are waited for, and the last
+// unit's part joined and written.  (64 sequences of 512 to 8192 tokens, 16 heads, fp8
+// pages: the slowest workgroup takes 52 us where starts count nothing, most take 30.)
+template <bool SHARED>
+constexpr int start_cost() {
+  return SHARED ? 2 : 16;
+}
+
+// A place in the flat list, in which each unit has start_cost() places before its
+// tiles, and what of its unit is in the workgroup's range.
 struct LatentCursor {
-  int b, rb, blk;
+  int b, rb, blk, to;     // the next tile, and the end of the range's
+  int left;               // places of the range behind the unit's
+  long long base;         // the unit's first place
   int length, count, nb;  // the sequence's tokens, its query tokens, tiles
   int bad;                // its length lies outside its table
 };
@@ -226,49 +238,70 @@ __device__ __forceinline__ long long lane_scan(long long v, int lane) {
   return sum;
 }
 
-// This group's range of tiles [g0, g1) (ranges of `each`) and its first place.
-struct LatentRange {
-  long long g0, g1, each;  // (a range's length fits 31 bits: latent_fits)
-};
-template <int KT>
-__device__ __forceinline__ LatentRange first_place(const LatentKernelArgs& a, const LatentStream& st,
-                                                   int group, int least, int lane, LatentCursor& c) {
-  long long per_block = 0;  // tiles of all sequences' units of one row block
+__device__ __forceinline__ long long divide(long long n, long long d) {
+  // (A 64-bit division takes ten times a 32-bit one.)
+  if ((n | d) >> 31 == 0) return static_cast<unsigned>(n) / static_cast<unsigned>(d);
+  return n / d;
+}
+
+// This group's first place, of ranges of `each` places; whether it has a tile.
+template <int KT, int START, int LEAST>
+__device__ __forceinline__ bool first_place(const LatentKernelArgs& a, const LatentStream& st,
+                                            int group, int lane, long long& each, LatentCursor& c) {
+  auto places = [&](int b) {
+    const int nb = sequence_tiles<KT>(a, b);
+    return nb > 0 ? nb + START : 0;
+  };
+  // Places of all sequences' units of one row block.
+  const int mine = places(lane);
+  const long long sums = lane_scan(mine, lane);
+  long long per_block = uniform_long(__shfl(sums, 63, 64));
+  if (a.batch > 64) {
+    long long more = 0;
 #pragma unroll 4
-  for (int b0 = 0; b0 < a.batch; b0 += 64) per_block += sequence_tiles<KT>(a, b0 + lane);
-  per_block = uniform_long(__shfl(lane_scan(per_block, lane), 63, 64));
+    for (int b0 = 64; b0 < a.batch; b0 += 64) more += places(b0 + lane);
+    per_block += uniform_long(__shfl(lane_scan(more, lane), 63, 64));
+  }
   const long long total = per_block * st.row_blocks;
-  LatentRange r{};
-  r.each = (total + st.groups - 1) / st.groups;
-  r.each = uniform_long(max((r.each + least - 1) / least * least, 1ll));
-  r.g0 = uniform_long(group * r.each);
-  r.g1 = uniform_long(min(r.g0 + r.each, total));
-  if (r.g0 >= r.g1) return r;
-  c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(r.g0 / per_block));
-  const long long rem = r.g0 - c.rb * per_block;
+  each = divide(total + st.groups - 1, st.groups);
+  each = uniform_long(max((each + LEAST - 1) / LEAST * LEAST, 1ll));
+  const long long g0 = group * each;
+  const long long have = min(each, total - g0);
+  if (have <= 0) return false;
+  c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(divide(g0, per_block)));
+  const long long rem = g0 - c.rb * per_block;
   long long base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int nb = sequence_tiles<KT>(a, b0 + lane);
-    const long long sum = lane_scan(nb, lane);
-    const long long from = base + sum - nb, to = base + sum;
+    const int n = b0 == 0 ? mine : places(b0 + lane);
+    const long long sum = b0 == 0 ? sums : lane_scan(n, lane);
+    const long long from = base + sum - n, to = base + sum;
     const unsigned long long hit = __ballot(from <= rem && rem < to);
     if (hit != 0) {
       const int src = __ffsll(static_cast<long long>(hit)) - 1;
       c.b = __builtin_amdgcn_readfirstlane(b0 + src);
       load_sequence<KT>(a, c);
-      c.blk = __builtin_amdgcn_readfirstlane(
-          static_cast<int>(rem - uniform_long(__shfl(from, src, 64))));
+      const int in = static_cast<int>(rem - uniform_long(__shfl(from, src, 64)));
+      c.base = uniform_long(g0 - in);
+      c.blk = __builtin_amdgcn_readfirstlane(max(in - START, 0));
+      c.to = __builtin_amdgcn_readfirstlane(
+          static_cast<int>(min(static_cast<long long>(c.nb), in + have - START)));
+      c.left = __builtin_amdgcn_readfirstlane(
+          static_cast<int>(max(have - (c.nb + START - in), 0ll)));
       break;
     }
     base += uniform_long(__shfl(sum, 63, 64));
   }
-  return r;
+  return c.to > c.blk;
 }
 
-// The next unit's first place; only called where there is one.
-template <int KT>
+// Whether the range has tiles of a later unit, and that unit.
+template <int START>
+__device__ __forceinline__ bool more_units(const LatentCursor& c) {
+  return c.left > START;
+}
+template <int KT, int START>
 __device__ __forceinline__ void next_unit(const LatentKernelArgs& a, LatentCursor& c) {
-  c.blk = 0;
+  c.base += c.nb + START;
   do {
     if (++c.b == a.batch) {
       c.b = 0;
@@ -276,6 +309,9 @@ __device__ __forceinline__ void next_unit(const LatentKernelArgs& a, LatentCurso
     }
     load_sequence<KT>(a, c);
   } while (c.nb == 0);
+  c.blk = 0;
+  c.to = min(c.nb, c.left - START);
+  c.left = max(c.left - c.nb - START, 0);
 }
 
 // One wavefront's 16 rows of a unit: queries, outputs, references and sums, and what
@@ -729,11 +765,11 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     __builtin_amdgcn_sched_barrier(0);
   };
   if (st.by_unit == 0 && tid == 0) st.jobs[group] = LatentJob{-1, 0, 0, 0};
+  constexpr int START = start_cost<SHARED>();
   LatentCursor cur{};
+  long long each;
   // (Four wavefronts take tiles in turn: ranges of whole turns.)
-  const LatentRange range = first_place<KT>(a, st, group, SHARED ? 1 : kWaves, lane, cur);
-  if (range.g0 >= range.g1) return;
-  const int blocks = static_cast<int>(range.g1 - range.g0);
+  if (!first_place<KT, START, SHARED ? 1 : kWaves>(a, st, group, lane, each, cur)) return;
 
   Loader loader;
   loader.start(lane);
@@ -781,13 +817,12 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
   };
 
   R rows;
-  // Ends the unit's part, tiles [from, to) of it, the last of which is the range's
-  // n-th.
-  auto part_of = [&](const LatentCursor& c, int from, int to, int n) {
-    const bool starts = from == 0, ends = to == c.nb;
+  // Ends the unit's part, tiles [from, c.to) of it.
+  auto part_of = [&](const LatentCursor& c, int from) {
+    const bool starts = from == 0, ends = c.to == c.nb;
     const int slot = 2 * group + (starts ? 1 : 0);
     if (ends && tid == 0) {
-      const long long first = (range.g0 + n - (to - 1)) / range.each;
+      const long long first = divide(c.base + START, each);
       if (st.by_unit != 0) {
         st.jobs[static_cast<std::size_t>(c.rb) * a.batch + c.b] =
             LatentJob{starts ? -1 : c.b, c.rb, static_cast<int>(first), group};
@@ -816,9 +851,9 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     Pages next = locate(ahead, ahead.blk);
     bads = next.bad != 0 ? 1u : 0u;
     auto locate_next = [&] {
-      if (located + 1 < blocks) {
+      if (ahead.blk + 1 < ahead.to || more_units<START>(ahead)) {
         ++located;
-        if (++ahead.blk == ahead.nb) next_unit<KT>(a, ahead);
+        if (++ahead.blk == ahead.to) next_unit<KT, START>(a, ahead);
         next = locate(ahead, ahead.blk);
         bads = (bads & ~(1u << (located & 31))) | (next.bad != 0 ? 1u << (located & 31) : 0u);
       }
@@ -854,8 +889,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     for (;;) {
       const int row = cur.rb * RB + wave * 16 + col;
       rows.start(a, cur, row, grp);
-      const int from = cur.blk;
-      const int to = min(cur.nb, cur.blk + (blocks - n));
+      const int from = cur.blk, to = cur.to;
       // Tiles before `whole` are seen by every row.
       const int whole = max(cur.length - cur.count + 1, 0) / KT;
       int bad = 0;
@@ -907,7 +941,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       }
       // The part's end.
       const bool complete = from == 0 && to == cur.nb;
-      const int slot = part_of(cur, from, to, n - 1);
+      const int slot = part_of(cur, from);
       const float sum = row_sum(rows.l);
       const float f = finish_factor<PF, L>(a, complete, bad != 0, sum);
       if (rows.live) {
@@ -923,8 +957,8 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
           ml[1] = bad != 0 ? NAN : sum;
         }
       }
-      if (n == blocks) break;
-      next_unit<KT>(a, cur);
+      if (!more_units<START>(cur)) break;
+      next_unit<KT, START>(a, cur);
     }
     // (Nothing is on its way into LDS when the workgroup gives it back.)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -932,11 +966,9 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     constexpr int kRing = LatentShared<PF, L, SHARED>::kRing;
     unsigned char* const own_tiles = sh.tile[wave];
     const unsigned lds = lds_address(own_tiles);
-    int n = 0;
     for (;;) {
       const int row = cur.rb * RB + col;
-      const int from = cur.blk;
-      const int to = min(cur.nb, cur.blk + (blocks - n));
+      const int from = cur.blk, to = cur.to;
       const int whole = max(cur.length - cur.count + 1, 0) / KT;
       int bad = 0;
       // The wavefront's i-th tile of the part into its place.
@@ -1011,8 +1043,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       }
       barrier();
       const bool complete = from == 0 && to == cur.nb;
-      const int last = n + (to - from) - 1;
-      const int slot = part_of(cur, from, to, last);
+      const int slot = part_of(cur, from);
       const float f = finish_factor<PF, L>(a, complete, bad != 0, sum);
       // A wavefront adds up four rows, 16 lanes (L / 16 dims each) a row.
       {
@@ -1042,9 +1073,8 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
           }
         }
       }
-      n += to - from;
-      if (n == blocks) break;
-      next_unit<KT>(a, cur);
+      if (!more_units<START>(cur)) break;
+      next_unit<KT, START>(a, cur);
       barrier();  // the tiles are read
     }
   }
@@ -1209,11 +1239,11 @@ std::size_t latent_workspace_bytes(std::size_t, std::size_t q_heads, std::size_t
 }
 
 bool latent_fits(const LatentArgs& a) {
-  // Ranges, and places in them, are counted in 32 bits: of 2^38 tiles, a group's
+  // Ranges, and places in them, are counted in 32 bits: of 2^38 places, a group's
   // are 2^30 at most.
   const std::size_t rows = a.q_heads * a.tokens;
   const std::size_t units = a.batch * ((rows + 15) / 16);
-  return units == 0 || a.max_blocks + 2 <= (std::size_t{1} << 38) / units;
+  return units == 0 || a.max_blocks + 2 + start_cost<false>() <= (std::size_t{1} << 38) / units;
 }
 
 hipError_t launch_latent_attention(const LatentArgs& a, hipStream_t stream) {
