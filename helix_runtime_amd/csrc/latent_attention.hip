@@ -407,7 +407,7 @@ struct LatentRows {
   template <typename F>
   __device__ __forceinline__ void scores(const unsigned char* tile, int col, int grp, v4f (&sc)[NH],
                                          F&& beside) const {
-    constexpr int A = PF == 0 ? 4 : T::kCodes ? 3 : 2;  // operands come out of LDS A steps ahead
+    constexpr int A = PF == 0 || T::kCodes ? 4 : 2;  // operands come out of LDS A steps ahead
     // Row col's chunk 4 s + grp (codes: half of chunk 2 s + grp / 2): its place within
     // a group of chunks is one of two (fp32 pages: four), by s.
     constexpr int V = PF == 0 ? 4 : 2;
@@ -435,6 +435,17 @@ struct LatentRows {
     for (int s = 0; s < A; ++s) read(s);
 #pragma unroll
     for (int h = 0; h < NH; ++h) sc[h] = v4f{0.f, 0.f, 0.f, 0.f};
+    // Codes become fp16 a step ahead, between the matrix instructions of the step.
+    v4u wide[2][NH];
+    auto widen = [&](int s) {
+      if constexpr (T::kCodes) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          wide[s % 2][h] = codes_fp16(raw[s % A][h][0], raw[s % A][h][1]);
+        }
+      }
+    };
+    widen(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -449,7 +460,7 @@ struct LatentRows {
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
           if constexpr (T::kCodes) {
-            k[h] = codes_fp16(raw[s % A][h][0], raw[s % A][h][1]);
+            k[h] = wide[s % 2][h];
           } else {
             k[h] = raw[s % A][h];
           }
@@ -460,6 +471,7 @@ struct LatentRows {
 #pragma unroll
           for (int h = 0; h < NH; ++h) sc[h] = matrix_step<PF>(k[h], q[s][i], sc[h]);
       }
+      if (s + 1 < NS) widen(s + 1);
       if (s + A < NS) read(s + A);
       beside(s);
       __builtin_amdgcn_sched_barrier(0);
@@ -556,7 +568,7 @@ struct LatentRows {
       }
     } else {
       using LdsV4s = __attribute__((address_space(3))) v4s;
-      constexpr int A = 4;
+      constexpr int A = T::kCodes ? 6 : 4;
       v4u pop[QT];
 #pragma unroll
       for (int i = 0; i < QT; ++i) pop[i] = v4u{p.w[0][i], p.w[1][i], p.w[2][i], p.w[3][i]};
@@ -587,6 +599,17 @@ struct LatentRows {
       };
 #pragma unroll
       for (int dt = 0; dt < A; ++dt) read(dt);
+      v4u wide[4];
+      auto widen = [&](int dt) {
+        if constexpr (T::kCodes) {
+#pragma unroll
+          for (int d = dt; d < dt + 2; ++d) {
+            wide[d % 4] = codes_fp16(static_cast<unsigned>(raw[d % A][0]),
+                                     static_cast<unsigned>(raw[d % A][1]));
+          }
+        }
+      };
+      widen(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int dt = 0; dt < ND; dt += 2) {
@@ -594,8 +617,7 @@ struct LatentRows {
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
           if constexpr (T::kCodes) {
-            v[d] = codes_fp16(static_cast<unsigned>(raw[(dt + d) % A][0]),
-                              static_cast<unsigned>(raw[(dt + d) % A][1]));
+            v[d] = wide[(dt + d) % 4];
           } else {
             v[d] = raw[(dt + d) % A];
           }
@@ -604,6 +626,7 @@ struct LatentRows {
         for (int i = QT - 1; i >= 0; --i)
 #pragma unroll
           for (int d = 0; d < 2; ++d) o[dt + d] = matrix_step<PF>(v[d], pop[i], o[dt + d]);
+        if (dt + 2 < ND) widen(dt + 2);
         if (dt + A < ND) {
           read(dt + A);
           read(dt + A + 1);
