@@ -14,12 +14,21 @@
 // so at one time.
 //
 // Matrix form.  As in the absorbed form: S^T = K Q^T, O^T += V^T P^T, a lane holding
-// keys of one query row.  fp32 numbers are sums of three bf16 terms (24 bits), of
-// whose nine products the six above 2^-26 of the largest are taken: 2.7 times the
-// rate of fp32 matrix instructions.  (Two fp16 terms would take three products, and a
-// common exponent for a tile's keys, which keys that a row must not see would set.)
-// Keys and values are split once a workgroup on their way into LDS; a wavefront has 32
-// rows, so that an operand out of LDS serves twelve matrix instructions.
+// keys of one query row; a wavefront has 32 rows, so that an operand out of LDS serves
+// several matrix instructions.  fp32 numbers are sums of 16-bit terms, split once a
+// workgroup on their way into LDS.
+// - expanded_kernel: two fp16 terms (22 bits and a sign: the rounding of an fp32
+//   number), of whose four products the three above 2^-22 of the largest are taken.
+//   fp16's range asks for powers of two: a query row's own, one for the keys and one
+//   for the values of a unit's part, by the largest of the first tile's numbers that
+//   all its rows see.  Those keys go to [2^4, 2^5) and values to [2^8, 2^9), so that
+//   keys 2^11 and values 2^7 times as large fit; 2^-25 is lost of numbers as scaled.
+//   Probabilities carry a factor of 2^8.
+// - expanded_redo_kernel: three bf16 terms (24 bits, fp32's range), of whose nine
+//   products the six above 2^-26 are taken.  It computes parts again whose unit the
+//   first one marked: with numbers past its range, a sum or output that is not finite
+//   (what a row does not see can show that way), or rows of which the 2^-25 might
+//   count, by the size of their scores or outputs.
 #include "bf16.hpp"
 #include "latent.hpp"
 #include "prefill_bmma.hpp"
@@ -43,6 +52,8 @@ using prefill_detail::v8bf;
 
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -50,7 +61,6 @@ constexpr int kKeyDim = static_cast<int>(kLatentNope + kLatentRope);
 constexpr int kValueDim = static_cast<int>(kLatentNope);
 constexpr int kTile = 32;   // keys
 constexpr int kWaves = 4;
-constexpr int kTerms = 3;
 constexpr int kSteps = kKeyDim / 32;    // of the scores' sum
 constexpr int kDims = kValueDim / 16;   // tiles of output dims
 constexpr int kKeyPitch = kKeyDim * 2;  // bytes of a row of one term in LDS
@@ -58,8 +68,22 @@ constexpr int kValuePitch = kValueDim * 2;
 // Numbers from here on have an infinite first term.
 constexpr float kWild = 0x1.ffp+127f;
 // A row's reference stays while no score is above it by more than this (log2
-// units).
+// units): fp16's largest number is 2^16.
 constexpr float kSlack = 7.0f;
+// fp16 terms: logarithms of the factor on probabilities, and of where the largest
+// numbers of queries, keys and values go, and where numbers begin that do not fit.
+constexpr float kProbLog = 8.0f;
+constexpr int kQueryLog = 10;
+constexpr int kKeyLog = 4;
+constexpr int kValueLog = 8;
+constexpr float kOverflow = 65504.0f;
+// Outputs (of values as scaled) below which 2^-25 may count: it is 2^-21 of them.
+constexpr float kSmallOutput = 0x1p-4f;
+// What undoes the scores' powers of two must be below this, or this times the row's
+// largest score (log2 units): 192 losses of 2^-25 of keys, a third of that each in the
+// mean, at queries below 2^11, half that in the mean, are 2^-14 of it in the mean, and
+// so 2^-22 of a score.
+constexpr float kLargeScores = 0x1p-8f;
 
 struct ExpandedKernelArgs {
   const float* query;
@@ -84,25 +108,57 @@ struct ExpandedStream {
   float* part_o;     // [2 * groups, RB, 128]
   float* part_ml;    // [2 * groups, RB, 2]
   ExpandedJob* jobs; // [groups]
+  // 1: to compute again.
+  int* unit_marks;   // [row blocks, batch, heads]: units that a group has whole
+  int* part_marks;   // [2 * groups]: partials
+  int* group_marks;  // [groups]: any of the group's
   int groups;
   int row_blocks;    // units of a (sequence, head), at most
 };
 
-// x = t[0] + t[1] + t[2], each rounded to nearest; two numbers at a time, packed into
-// words.
-__device__ __forceinline__ void split_pair(float x, float y, unsigned (&t)[kTerms]) {
-#pragma unroll
-  for (int i = 0; i < kTerms; ++i) {
-    const v2bf h = __builtin_convertvector((v2f{x, y}), v2bf);
-    t[i] = __builtin_bit_cast(unsigned, h);
-    x -= __uint_as_float(t[i] << 16);
-    y -= __uint_as_float(t[i] & 0xffff0000u);
+// Terms of an fp32 number, fp16 or bf16, and the products of two numbers' that are
+// taken.
+constexpr int terms(bool f16) { return f16 ? 2 : 3; }
+constexpr int products(bool f16) { return f16 ? 3 : 6; }
+
+// The next term of x and y, packed into a word; x and y become what it leaves.
+template <bool F16>
+__device__ __forceinline__ unsigned next_term(float& x, float& y) {
+  if constexpr (F16) {
+    const v2h h = __builtin_convertvector((v2f{x, y}), v2h);
+    // One mixed-precision instruction a remainder: the compiler must not see that
+    // the factor is -1.
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    x = __builtin_fmaf(static_cast<float>(h[0]), minus, x);
+    y = __builtin_fmaf(static_cast<float>(h[1]), minus, y);
+    return __builtin_bit_cast(unsigned, h);
+  } else {
+    const unsigned t = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2bf));
+    x -= __uint_as_float(t << 16);
+    y -= __uint_as_float(t & 0xffff0000u);
+    return t;
   }
 }
 
+template <bool F16>
 __device__ __forceinline__ v4f matrix_step(v4u a, v4u b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
-                                                 __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  if constexpr (F16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
+                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
+                                                   __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  }
+}
+
+// The power of two that puts `most` into [2^to, 2^(to + 1)), as far as it is a normal
+// number (1 for 0), and what undoes it.
+__device__ __forceinline__ float grow_to(float most, int to, float& unscale) {
+  const int e =
+      most == 0.f ? to : min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 100);
+  unscale = __uint_as_float(static_cast<unsigned>(127 - to + e) << 23);
+  return __uint_as_float(static_cast<unsigned>(127 + to - e) << 23);
 }
 
 // Chunks of 16 bytes are exchanged by row, so that a read of one chunk of 16 rows
@@ -117,21 +173,30 @@ __device__ __forceinline__ unsigned value_place(int row, int chunk) {
 }
 
 // Item i of a range: keys of tile i and values of tile i - 1, what one step takes.
+template <bool F16>
 struct ExpandedShared {
   struct Item {
-    __align__(1024) unsigned char k[kTerms][kTile * kKeyPitch];
-    __align__(1024) unsigned char v[kTerms][kTile * kValuePitch];
+    __align__(1024) unsigned char k[terms(F16)][kTile * kKeyPitch];
+    __align__(1024) unsigned char v[terms(F16)][kTile * kValuePitch];
   };
   Item item[2];
-  unsigned poison[2][kWaves];  // keys of the item's values that must not be seen
+  unsigned poison[2][kWaves];  // bf16 terms: keys of the item's values that must not be seen
+  float most[kWaves];          // fp16 terms: the largest number of a first tile
+  int mark[kWaves];
 };
 
-// A place in the flat list of tiles.
+// What a unit's start costs a workgroup that has begun with another one, in tiles.
+constexpr int kStart = 3;
+
+// A place in the flat list, in which each unit has kStart places before its tiles, and
+// what of its unit is in the workgroup's range.
 struct ExpandedCursor {
-  int b, h, rb, blk;
+  int b, h, rb, blk, to;  // the next tile, and the end of the range's
+  int left;               // places of the range behind the unit's
+  long long base;         // the unit's first place
   int length, count, nb;
-  int first;  // keys that the unit's first row sees
-  int bad;    // the length lies outside [0, keys]
+  int first;              // keys that the unit's first row sees
+  int bad;                // the length lies outside [0, keys]
 };
 
 __device__ __forceinline__ int clamped_count(const ExpandedKernelArgs& a, int b) {
@@ -186,66 +251,92 @@ __device__ __forceinline__ long long lane_scan(long long v, int lane) {
   return sum;
 }
 
-// This group's range of tiles [g0, g1) (ranges of `each`) and its first place.  The
+// This group's first place, of ranges of `each` places; whether it has a tile.  The
 // list goes by row block, sequence, head and tile.
-struct ExpandedRange {
-  long long g0, g1, each;
-};
 template <int RB>
-__device__ __forceinline__ ExpandedRange first_place(const ExpandedKernelArgs& a,
-                                                     const ExpandedStream& st, int group, int lane,
-                                                     ExpandedCursor& c) {
+__device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const ExpandedStream& st,
+                                            int group, int lane, long long& each,
+                                            ExpandedCursor& c) {
   const long long entries = static_cast<long long>(st.row_blocks) * a.batch;
-  long long total = 0;
-  for (long long e0 = 0; e0 < entries; e0 += 64) total += entry_tiles<RB>(a, st.row_blocks, e0 + lane);
-  total = uniform_long(__shfl(lane_scan(total, lane), 63, 64)) * a.heads;
-  ExpandedRange r{};
-  r.each = uniform_long(max((total + st.groups - 1) / st.groups, 1ll));
-  r.g0 = uniform_long(group * r.each);
-  r.g1 = uniform_long(min(r.g0 + r.each, total));
-  if (r.g0 >= r.g1) return r;
+  auto places = [&](long long e) {
+    const int nb = entry_tiles<RB>(a, st.row_blocks, e);
+    return nb > 0 ? static_cast<long long>(nb + kStart) * a.heads : 0ll;
+  };
+  const long long mine = places(lane);
+  const long long sums = lane_scan(mine, lane);
+  long long total = uniform_long(__shfl(sums, 63, 64));
+  if (entries > 64) {
+    long long more = 0;
+    for (long long e0 = 64; e0 < entries; e0 += 64) more += places(e0 + lane);
+    total += uniform_long(__shfl(lane_scan(more, lane), 63, 64));
+  }
+  each = uniform_long(max((total + st.groups - 1) / st.groups, 1ll));
+  const long long g0 = group * each;
+  const long long have = min(each, total - g0);
+  if (have <= 0) return false;
   long long base = 0;
   for (long long e0 = 0; e0 < entries; e0 += 64) {
-    const long long tiles = static_cast<long long>(entry_tiles<RB>(a, st.row_blocks, e0 + lane)) * a.heads;
-    const long long sum = lane_scan(tiles, lane);
-    const long long from = base + sum - tiles, to = base + sum;
-    const unsigned long long hit = __ballot(from <= r.g0 && r.g0 < to);
+    const long long n = e0 == 0 ? mine : places(e0 + lane);
+    const long long sum = e0 == 0 ? sums : lane_scan(n, lane);
+    const long long from = base + sum - n, to = base + sum;
+    const unsigned long long hit = __ballot(from <= g0 && g0 < to);
     if (hit != 0) {
       const int src = __ffsll(static_cast<long long>(hit)) - 1;
       const long long e = e0 + src;
       c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(e / a.batch));
       c.b = __builtin_amdgcn_readfirstlane(static_cast<int>(e - static_cast<long long>(c.rb) * a.batch));
       load_unit<RB>(a, c);
-      const long long in = r.g0 - uniform_long(__shfl(from, src, 64));
-      c.h = __builtin_amdgcn_readfirstlane(static_cast<int>(in / c.nb));
-      c.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(in - static_cast<long long>(c.h) * c.nb));
+      const long long rem = g0 - uniform_long(__shfl(from, src, 64));
+      c.h = __builtin_amdgcn_readfirstlane(static_cast<int>(rem / (c.nb + kStart)));
+      const int in = __builtin_amdgcn_readfirstlane(
+          static_cast<int>(rem - static_cast<long long>(c.h) * (c.nb + kStart)));
+      c.base = uniform_long(g0 - in);
+      c.blk = max(in - kStart, 0);
+      c.to = __builtin_amdgcn_readfirstlane(
+          static_cast<int>(min(static_cast<long long>(c.nb), in + have - kStart)));
+      c.left = __builtin_amdgcn_readfirstlane(
+          static_cast<int>(max(have - (c.nb + kStart - in), 0ll)));
       break;
     }
     base += uniform_long(__shfl(sum, 63, 64));
   }
-  return r;
+  return c.to > c.blk;
 }
 
-// The next unit's first place; only called where there is one.
+__device__ __forceinline__ std::size_t unit_index(const ExpandedKernelArgs& a,
+                                                  const ExpandedCursor& c) {
+  return (static_cast<std::size_t>(c.rb) * a.batch + c.b) * a.heads + c.h;
+}
+
+// Whether the range has tiles of a later unit, and that unit.
+__device__ __forceinline__ bool more_units(const ExpandedCursor& c) { return c.left > kStart; }
 template <int RB>
 __device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, ExpandedCursor& c) {
+  c.base += c.nb + kStart;
+  if (++c.h == a.heads) {
+    c.h = 0;
+    do {
+      if (++c.b == a.batch) {
+        c.b = 0;
+        ++c.rb;
+      }
+      load_unit<RB>(a, c);
+    } while (c.nb == 0);
+  }
   c.blk = 0;
-  if (++c.h < a.heads) return;
-  c.h = 0;
-  do {
-    if (++c.b == a.batch) {
-      c.b = 0;
-      ++c.rb;
-    }
-    load_unit<RB>(a, c);
-  } while (c.nb == 0);
+  c.to = min(c.nb, c.left - kStart);
+  c.left = max(c.left - c.nb - kStart, 0);
 }
 
-// RT tiles of 16 query rows a wavefront: units of RB = 64 RT rows.
-template <int RT>
-__device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const ExpandedStream& st,
-                                              ExpandedShared& sh) {
+// The range that begins at `cur`.  RT tiles of 16 query rows a wavefront: units of RB =
+// 64 RT rows.  F16: which terms (bf16 ones compute again, and mark nothing).  `each`:
+// places of a range.
+template <int RT, bool F16>
+__device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, const ExpandedStream& st,
+                                               ExpandedShared<F16>& sh, ExpandedCursor cur,
+                                               long long each) {
   constexpr int RB = 16 * kWaves * RT;
+  constexpr int kTerms = terms(F16), kProducts = products(F16);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -256,11 +347,6 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (tid == 0) st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
-  ExpandedCursor cur{};
-  const ExpandedRange range = first_place<RB>(a, st, group, lane, cur);
-  if (range.g0 >= range.g1) return;
-  const int blocks = static_cast<int>(range.g1 - range.g0);
 
   // ---- staging: a thread has a key's chunks part, part + 8, .. of eight numbers.
   const int srow = tid >> 3, part = tid & 7;
@@ -270,6 +356,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
     const float* v;
     int first, length;  // its first key, and the sequence's number
     int seen;           // keys that every row of the unit sees
+    int opens;          // the first tile of its unit in the range
   };
   auto source = [&](const ExpandedCursor& c) {
     Source s{};
@@ -281,6 +368,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
     s.first = c.blk * kTile;
     s.length = c.length;
     s.seen = c.first;
+    s.opens = 0;
     return s;
   };
   v4f raw_k[3][2], raw_v[2][2];  // (the third chunk of a key is the shared part's)
@@ -306,17 +394,36 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
       raw_v[1][w] = *reinterpret_cast<const v4f*>(v + 64 + 4 * w);
     }
   };
+  // fp16 terms: the powers of two of the keys and values on their way, what undoes
+  // them by item, and the largest number so far.
+  float key_scale = 1.f, value_scale = 1.f, key_unscale[2] = {1.f, 1.f}, value_unscale[2] = {1.f, 1.f};
+  float most = 0.f;
+  // The largest number among `n` chunks of keys that every row of the unit sees.
+  auto largest = [&](const v4f (*x)[2], int n, const Source& s) {
+    float top = 0.f;
+    if (s.length > 0 && s.first + srow < min(s.seen, s.length)) {
+      for (int i = 0; i < n; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = fabsf(x[i][w][e]);
+            top = fmaxf(top, y < 0x1p100f ? y : 0.f);
+          }
+    }
+#pragma unroll
+    for (int bit = 32; bit >= 1; bit /= 2) top = fmaxf(top, __shfl_xor(top, bit, 64));
+    if (lane == 0) sh.most[wave] = top;
+    barrier();
+    top = fmaxf(fmaxf(sh.most[0], sh.most[1]), fmaxf(sh.most[2], sh.most[3]));
+    barrier();
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
+  };
   // The way into LDS in small parts, each one term of two numbers: a chunk's four pairs
   // of numbers, then the next chunk's; its last part writes it.
   constexpr int kStageParts = 5 * 4 * kTerms;
   unsigned words[4][kTerms];
   float sx = 0.f, sy = 0.f;
-  auto term = [](float& x, float& y) {  // the next term of x and y, and what it leaves
-    const unsigned t = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2bf));
-    x -= __uint_as_float(t << 16);
-    y -= __uint_as_float(t & 0xffff0000u);
-    return t;
-  };
   auto stage = [&](int buf, int i) {
     const int chunk = i / (4 * kTerms), pair = i / kTerms % 4, level = i % kTerms;
     if (level == 0) {
@@ -324,8 +431,14 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
           chunk < 3 ? raw_k[chunk < 3 ? chunk : 0][pair / 2] : raw_v[chunk < 3 ? 0 : chunk - 3][pair / 2];
       sx = x[2 * (pair % 2)];
       sy = x[2 * (pair % 2) + 1];
+      if constexpr (F16) {
+        const float by = chunk < 3 ? key_scale : value_scale;
+        sx *= by;
+        sy *= by;
+        most = fmaxf(most, fmaxf(fabsf(sx), fabsf(sy)));
+      }
     }
-    words[pair][level] = term(sx, sy);
+    words[pair][level] = next_term<F16>(sx, sy);
     if (pair != 3 || level != kTerms - 1) return;
     unsigned char* const to =
         chunk < 3 ? sh.item[buf].k[0] + key_place(srow, part + 8 * chunk)
@@ -336,7 +449,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
       *reinterpret_cast<v4u*>(to + n * plane) = v4u{words[0][n], words[1][n], words[2][n], words[3][n]};
     }
   };
-  // Values of keys that some row of the unit does not see must be finite: those
+  // bf16 terms: values of keys that some row of the unit does not see must be finite: those
   // behind the sequence's last become 0, and of the others those with terms that are
   // not; the latter's keys are noted.
   auto clean_values = [&](int buf, const Source& s) {
@@ -371,8 +484,9 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
   v4u q[kSteps][RT][kTerms];
   v4f o[RT][kDims];  // o[t][dt][i]: dim 16 dt + 4 grp + i of row col
   float m[RT], l[RT];
-  int limit[RT];  // keys that the row sees
-  auto start = [&](const ExpandedCursor& c) {
+  float unscale[RT];  // fp16 terms: what undoes the row's power of two and the keys'
+  int limit[RT];      // keys that the row sees
+  auto start = [&](const ExpandedCursor& c, float key_un) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int row = c.rb * RB + unit_row(t);
@@ -381,17 +495,39 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
       const float* const src = a.query + static_cast<std::size_t>(c.b) * a.query_at.batch +
                                static_cast<std::size_t>(c.h) * a.query_at.head +
                                static_cast<std::size_t>(live ? row : 0) * a.query_at.token;
+      v4f x[kSteps][2];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        v4f x[2];
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          x[w] = *reinterpret_cast<const v4f*>(src + 32 * s + 8 * grp + 4 * w);
-          x[w] = live ? x[w] * a.qscale : v4f{0.f, 0.f, 0.f, 0.f};
+          x[s][w] = *reinterpret_cast<const v4f*>(src + 32 * s + 8 * grp + 4 * w);
         }
+      float grow = a.qscale;
+      unscale[t] = 1.f;
+      if constexpr (F16) {
+        float top = 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const v4f y = x[s][w];
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+          }
+        grow = grow_to(row_max(top), kQueryLog, unscale[t]);
+        // (Positive, or scores of -infinity would not stay that: the score scale's
+        // sign goes with the queries, which a scale of 0 makes 0.)
+        grow = a.qscale > 0.f ? grow : a.qscale < 0.f ? -grow : 0.f;
+        unscale[t] = fmaxf(unscale[t] * fabsf(a.qscale) * key_un, 1.2e-38f);
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
         unsigned w[4][kTerms];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_pair(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1], w[i]);
+        for (int i = 0; i < 4; ++i) {
+          float y0 = x[s][i >> 1][2 * (i & 1)] * grow, y1 = x[s][i >> 1][2 * (i & 1) + 1] * grow;
+#pragma unroll
+          for (int n = 0; n < kTerms; ++n) w[i][n] = next_term<F16>(y0, y1);
+        }
 #pragma unroll
         for (int i = 0; i < kTerms; ++i) {
           q[s][t][i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
@@ -411,9 +547,8 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
   // product have other work put behind them, a part at a time.  (In one piece before
   // or behind the products of a step, which is how the compiler would have it, the two
   // add up: 925 us for 4 x 32 heads, 512 rows over 4096 keys.)
-  constexpr int kProducts = 6;
   auto product = [](int sum, int i) {  // its place in the order below
-    return sum == 2 ? 2 - i : sum == 1 ? 4 - i : 5;
+    return kProducts - (sum + 1) * (sum + 2) / 2 + sum - i;
   };
 
   // Scores of a tile: sc[t][h][i] is key 16 h + 4 grp + i of tile t's row col.
@@ -445,7 +580,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
 #pragma unroll
         for (int i = sum; i >= 0; --i) {
 #pragma unroll
-          for (int t = 0; t < RT; ++t) sc[t][h] = matrix_step(k[u % 2][i], q[s][t][sum - i], sc[t][h]);
+          for (int t = 0; t < RT; ++t) sc[t][h] = matrix_step<F16>(k[u % 2][i], q[s][t][sum - i], sc[t][h]);
           beside(kProducts * u + product(sum, i));
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -461,6 +596,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
       const v4f x = sc[t][0], y = sc[t][1];
       mx[t] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
                     fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+      if constexpr (F16) mx[t] *= unscale[t];
       above = above || mx[t] > m[t] + kSlack;
     }
     if (__ballot(above) != 0) {
@@ -500,12 +636,18 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
   auto probability = [&](int i, const v4f (&sc)[RT][2], const float (&ref)[RT], Probabilities& p) {
     const int pair = i / (1 + kTerms), level = i % (1 + kTerms), t = pair / 4, n = pair % 4;
     if (level == 0) {
-      py0 = __builtin_amdgcn_exp2f(sc[t][n / 2][2 * (n % 2)] - ref[t]);
-      py1 = __builtin_amdgcn_exp2f(sc[t][n / 2][2 * (n % 2) + 1] - ref[t]);
+      const float x = sc[t][n / 2][2 * (n % 2)], y = sc[t][n / 2][2 * (n % 2) + 1];
+      if constexpr (F16) {
+        py0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x, unscale[t], -ref[t]));
+        py1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y, unscale[t], -ref[t]));
+      } else {
+        py0 = __builtin_amdgcn_exp2f(x - ref[t]);
+        py1 = __builtin_amdgcn_exp2f(y - ref[t]);
+      }
       return;
     }
     if (level == 1) l[t] += py0 + py1;
-    p.w[t][n][level - 1] = term(py0, py1);
+    p.w[t][n][level - 1] = next_term<F16>(py0, py1);
   };
   const int vrow = 4 * grp + (col >> 2);
   unsigned value_at[4];
@@ -543,7 +685,7 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
 #pragma unroll
         for (int i = sum; i >= 0; --i) {
 #pragma unroll
-          for (int t = 0; t < RT; ++t) o[t][dt] = matrix_step(v[dt % 2][i], pop[t][sum - i], o[t][dt]);
+          for (int t = 0; t < RT; ++t) o[t][dt] = matrix_step<F16>(v[dt % 2][i], pop[t][sum - i], o[t][dt]);
           beside(kProducts * dt + product(sum, i));
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -553,25 +695,41 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
 
   // ---- the range.  Step n: scores of tile n + 1 beside tile n's probabilities, tile
   // n's outputs beside the way of item n + 2 into LDS, item n + 3 sent for.
-  ExpandedCursor ahead = cur;  // the tile whose keys are sent for
-  int located = 0;
+  ExpandedCursor ahead = cur;   // the tile whose keys are sent for
   Source now = source(ahead), before = now;  // its rows, and the last tile's
-  Source staged = now;                       // rows of the values in the registers
-  auto advance = [&] {
-    before = now;
-    if (located + 1 < blocks) {
-      if (++ahead.blk == ahead.nb) next_unit<RB>(a, ahead);
-      now = source(ahead);
-    }
-    ++located;
-  };
-  auto fetch = [&] {  // keys of tile `located`, values of the one before
+  now.opens = 1;
+  Source staged_k = now, staged_v = now;     // what the registers hold
+  // Keys of the next tile and values of the one before.  (Behind the range the last
+  // one again, which no one reads.)
+  auto fetch = [&] {
     fetch_keys(now);
     fetch_values(before);
-    staged = before;
-    advance();
+    staged_k = now;
+    staged_v = before;
+    before = now;
+    if (ahead.blk + 1 < ahead.to) {
+      ++ahead.blk;
+      now.first += kTile;
+      now.opens = 0;
+    } else if (more_units(ahead)) {
+      next_unit<RB>(a, ahead);
+      now = source(ahead);
+      now.opens = 1;
+    } else {
+      now.opens = 0;
+    }
   };
-  // Items 0 and 1.  (Item 0 has no values: what it puts there is not read.)
+  // Before an item's way into LDS: its powers of two, or its values made finite.
+  auto ready = [&](int buf) {
+    if constexpr (F16) {
+      if (staged_k.opens != 0) key_scale = grow_to(largest(raw_k, 3, staged_k), kKeyLog, key_unscale[buf]);
+      if (staged_k.opens == 0) key_unscale[buf] = key_unscale[buf ^ 1];
+      if (staged_v.opens != 0) value_scale = grow_to(largest(raw_v, 2, staged_v), kValueLog, value_unscale[buf]);
+      if (staged_v.opens == 0) value_unscale[buf] = value_unscale[buf ^ 1];
+    } else {
+      clean_values(buf, staged_v);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -582,22 +740,20 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
 #pragma unroll
     for (int w = 0; w < 2; ++w) raw_k[i][w] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  auto store = [&](int buf) {
-    clean_values(buf, staged);
+  // Items 0 and 1.  (Item 0's values, the first tile's, are not read.)
 #pragma unroll
-    for (int i = 0; i < kStageParts; ++i) stage(buf, i);
-  };
-  fetch();
-  store(0);
-  fetch();
-  store(1);
+  for (int item = 0; item < 2; ++item) {
+    fetch();
+    ready(item);
+#pragma unroll
+    for (int i = 0; i < kStageParts; ++i) stage(item, i);
+  }
   fetch();
   barrier();
   int n = 0;
   for (;;) {
-    start(cur);
-    const int from = cur.blk;
-    const int to = min(cur.nb, cur.blk + (blocks - n));
+    start(cur, (n & 1) != 0 ? key_unscale[1] : key_unscale[0]);
+    const int from = cur.blk, to = cur.to;
     const int whole = max(cur.first, 0) / kTile;  // tiles before are seen by every row
     v4f sc[RT][2];
     scores(n & 1, sc, [](int) {});
@@ -606,15 +762,21 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
     for (int blk = from; blk < to; ++blk) {
       const int buf = (n + 1) & 1, into = n & 1;
       if (blk >= whole) {
-        const unsigned poison = sh.poison[buf][0] | sh.poison[buf][1] | sh.poison[buf][2] |
-                                sh.poison[buf][3];
+        unsigned poison = 0;
+        if constexpr (!F16) {
+          poison = sh.poison[buf][0] | sh.poison[buf][1] | sh.poison[buf][2] | sh.poison[buf][3];
+        }
         mask(blk * kTile, poison, sc);
       }
       follow(sc);
       float ref[RT];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) ref[t] = m[t] == -INFINITY ? 0.f : m[t];
-      clean_values(into, staged);
+      for (int t = 0; t < RT; ++t) ref[t] = (m[t] == -INFINITY ? 0.f : m[t]) - (F16 ? kProbLog : 0.f);
+      if (into != 0) {  // (which item's the powers are is known to the compiler)
+        ready(1);
+      } else {
+        ready(0);
+      }
       Probabilities p;
       // Of the way into LDS, the parts that the scores' steps have room for.
       constexpr int kRoom = 2 * kSteps * kProducts - kProbParts;
@@ -647,27 +809,44 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
         for (int i = 0; i < kBeside; ++i) stage(into, i);
       }
       add_values(buf, p, [&](int i) {
-        if (i + kBeside < kStageParts) stage(into, i + kBeside);
+        constexpr int kLeft = kStageParts - kBeside, kSlots = kDims * kProducts;
+#pragma unroll
+        for (int j = i * kLeft / kSlots; j < (i + 1) * kLeft / kSlots; ++j) stage(into, kBeside + j);
       });
       fetch();
       ++n;
       barrier();
     }
     // The part's end.
-    const bool complete = from == 0 && to == cur.nb;
-    const bool starts = from == 0;
+    const bool starts = from == 0, ends = to == cur.nb, complete = starts && ends;
     const int slot = 2 * group + (starts ? 1 : 0);
-    if (to == cur.nb && !starts && tid == 0) {
-      const long long first = (range.g0 + n - to) / range.each;
-      st.jobs[group] = ExpandedJob{cur.b, cur.h, cur.rb, static_cast<int>(first), group};
-    }
+    // (The last tile's values were in item n.)
+    const float value_un = (n & 1) != 0 ? value_unscale[1] : value_unscale[0];
+    bool wrong = F16 && !(most < kOverflow);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const float sum = row_sum(l[t]);
       const int local = unit_row(t), row = cur.rb * RB + local;
+      if (F16) {
+        float top = 0.f;
+        bool nan = !(sum < INFINITY);
+#pragma unroll
+        for (int dt = 0; dt < kDims; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            top = fmaxf(top, fabsf(o[t][dt][i]));
+            nan = nan || !(fabsf(o[t][dt][i]) < INFINITY);
+          }
+        top = row_max(top);
+        // (An empty row beside a NaN is computed again too: 0 times it is not 0.)
+        const bool lost = sum != 0.f && (top < kSmallOutput * sum ||
+                                         unscale[t] > kLargeScores * fmaxf(fabsf(m[t]), 1.f));
+        wrong = wrong || (row < cur.count && (nan || lost));
+      }
       if (row >= cur.count) continue;
       // (A row that has seen nothing has neither sum nor outputs.)
-      const float f = !complete ? 1.0f : cur.bad != 0 ? NAN : sum == 0.f ? 0.f : 1.0f / sum;
+      float f = F16 ? value_un : 1.0f;
+      if (complete) f = cur.bad != 0 ? NAN : sum == 0.f ? 0.f : f / sum;
       float* const dst =
           (complete ? a.out + static_cast<std::size_t>(cur.b) * a.out_at.batch +
                           static_cast<std::size_t>(cur.h) * a.out_at.head +
@@ -682,77 +861,156 @@ __device__ __forceinline__ void expanded_body(const ExpandedKernelArgs& a, const
         ml[1] = cur.bad != 0 ? NAN : sum;
       }
     }
-    if (n == blocks) break;
+    if constexpr (F16) {
+      const bool any = __ballot(wrong) != 0;
+      if (lane == 0) sh.mark[wave] = any ? 1 : 0;
+      barrier();
+      if (tid == 0) {
+        const int mark = sh.mark[0] | sh.mark[1] | sh.mark[2] | sh.mark[3];
+        *(complete ? st.unit_marks + unit_index(a, cur) : st.part_marks + slot) = mark;
+        if (mark != 0) st.group_marks[group] = 1;
+        if (ends && !starts) {
+          st.jobs[group] = ExpandedJob{cur.b, cur.h, cur.rb,
+                                       static_cast<int>((cur.base + kStart) / each), group};
+        }
+      }
+    }
+    if (!more_units(cur)) break;
     next_unit<RB>(a, cur);
   }
+  if constexpr (!F16) barrier();  // (another unit may follow)
 }
 
 template <int RT>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
     void expanded_kernel(ExpandedKernelArgs a, ExpandedStream st) {
-  __shared__ ExpandedShared sh;
-  expanded_body<RT>(a, st, sh);
+  __shared__ ExpandedShared<true> sh;
+  constexpr int RB = 16 * kWaves * RT;
+  const int group = static_cast<int>(blockIdx.x);
+  if (threadIdx.x == 0) {
+    st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
+    st.group_marks[group] = 0;
+  }
+  ExpandedCursor cur{};
+  long long each;
+  if (!first_place<RB>(a, st, group, static_cast<int>(threadIdx.x) & 63, each, cur)) return;
+  expanded_range<RT, true>(a, st, sh, cur, each);
+}
+
+// The same ranges' parts of units that are marked, again.
+template <int RT>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+    void expanded_redo_kernel(ExpandedKernelArgs a, ExpandedStream st) {
+  __shared__ ExpandedShared<false> sh;
+  constexpr int RB = 16 * kWaves * RT;
+  const int tid = static_cast<int>(threadIdx.x);
+  int marks = 0;
+  for (int g = tid; g < st.groups; g += 64 * kWaves) marks |= st.group_marks[g];
+  if (__syncthreads_or(marks) == 0) return;
+  ExpandedCursor cur{};
+  long long each;
+  if (!first_place<RB>(a, st, static_cast<int>(blockIdx.x), tid & 63, each, cur)) return;
+  for (;;) {
+    // A unit in several parts is marked if one of them is.
+    int mark = 0;
+    if (cur.blk == 0 && cur.to == cur.nb) {
+      mark = st.unit_marks[unit_index(a, cur)];
+    } else {
+      const int first = static_cast<int>((cur.base + kStart) / each);
+      const int last = static_cast<int>((cur.base + kStart + cur.nb - 1) / each);
+      for (int g = first + tid; g <= last; g += 64 * kWaves) {
+        mark |= st.part_marks[2 * g + (g == first ? 1 : 0)];
+      }
+    }
+    if (__syncthreads_or(mark) != 0) {
+      ExpandedCursor one = cur;
+      one.left = 0;
+      expanded_range<RT, false>(a, st, sh, one, each);
+    }
+    if (!more_units(cur)) break;
+    next_unit<RB>(a, cur);
+  }
 }
 
 // Joins the partials of the units that cross ranges: the first group's second slot
-// and the later groups' first ones.  blockIdx.x is a group, a wavefront takes a row, a
-// lane two dims.
+// and the later groups' first ones.  blockIdx.x is a group; 16 lanes take a row, 8
+// dims each, and 16 partials' statistics at a time.
+constexpr int kMergeRows = 16;
 __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs a,
                                                              ExpandedStream st, int rb_rows) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, part = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const ExpandedJob job = st.jobs[blockIdx.x];
   if (job.b < 0) return;
-  const int local = static_cast<int>(blockIdx.y) * 4 + wave;
+  const int local = static_cast<int>(blockIdx.y) * kMergeRows + wave * 4 + (lane >> 4);
   const int row = job.rb * rb_rows + local;
-  if (local >= rb_rows || row >= clamped_count(a, job.b)) return;
+  const bool live = local < rb_rows && row < clamped_count(a, job.b);
+  if (__ballot(live) == 0) return;
+  const int at = live ? local : 0;
   const int parts = job.last - job.first + 1;
   auto slot = [&](int i) {
-    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + local;
+    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + at;
   };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 64) top = fmaxf(top, st.part_ml[2 * slot(i)]);
-#pragma unroll
-  for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
-  float sum = 0.f;
-  v2f o = {0.f, 0.f};
-  for (int i0 = 0; i0 < parts; i0 += 64) {
-    float w = 0.f;
-    if (i0 + lane < parts) {
-      const float pl = st.part_ml[2 * slot(i0 + lane) + 1];
-      w = pl == 0.f ? 0.f : exp2_ratio(st.part_ml[2 * slot(i0 + lane)], top);
-      sum += pl * w;
+  float top = -INFINITY, sum = 0.f;
+  v4f o[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+  for (int i0 = 0; i0 < parts; i0 += 16) {
+    float pm = -INFINITY, pl = 0.f;
+    if (live && i0 + part < parts) {
+      const v2f x = *reinterpret_cast<const v2f*>(st.part_ml + 2 * slot(i0 + part));
+      pm = x[0];
+      pl = x[1];
     }
-    const int end = min(parts - i0, 64);
+    float mx = pm;
+#pragma unroll
+    for (int k = 8; k > 0; k /= 2) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
+    const float mn = fmaxf(top, mx);
+    const float alpha = exp2_ratio(top, mn);
+    // (A part that saw nothing has no outputs to speak of.)
+    const float w = pl == 0.f ? 0.f : exp2_ratio(pm, mn);
+    float add = w * pl;
+#pragma unroll
+    for (int k = 8; k > 0; k /= 2) add += __shfl_xor(add, k, 64);
+    sum = sum * alpha + add;
+    o[0] *= alpha;
+    o[1] *= alpha;
+    top = mn;
+    const int end = min(parts - i0, 16);
     for (int i = 0; i < end; i += 4) {
-      v2f x[4];
+      v4f x[4][2];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        x[u] = reinterpret_cast<const v2f*>(st.part_o + slot(i0 + min(i + u, end - 1)) * kValueDim)[lane];
+        const auto* from =
+            reinterpret_cast<const v4f*>(st.part_o + slot(i0 + min(i + u, end - 1)) * kValueDim) + 2 * part;
+        x[u][0] = from[0];
+        x[u][1] = from[1];
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const float wi = i + u < end ? __shfl(w, i + u, 64) : 0.f;
-        if (wi != 0.f) o += x[u] * wi;  // (a part that saw nothing has no outputs)
+        const float wi = __shfl(w, (lane & 48) + min(i + u, end - 1), 64);
+        if (i + u < end && wi != 0.f) {
+          o[0] += x[u][0] * wi;
+          o[1] += x[u][1] * wi;
+        }
       }
     }
   }
-#pragma unroll
-  for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
+  if (!live) return;
   const float f = sum == 0.f ? 0.f : 1.0f / sum;
-  float* const dst = a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
-                     static_cast<std::size_t>(job.h) * a.out_at.head +
-                     static_cast<std::size_t>(row) * a.out_at.token;
-  reinterpret_cast<v2f*>(dst)[lane] = o * f;
+  auto* const dst = reinterpret_cast<v4f*>(a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
+                                           static_cast<std::size_t>(job.h) * a.out_at.head +
+                                           static_cast<std::size_t>(row) * a.out_at.token) +
+                    2 * part;
+  dst[0] = o[0] * f;
+  dst[1] = o[1] * f;
 }
 
 // ----------------------------------------------------------------- host ----
-constexpr std::size_t kGroups = 256;  // a workgroup a CU: two items take 120 KB of LDS
+constexpr std::size_t kGroups = 256;  // a workgroup a CU: a wavefront a SIMD, for its registers
 
 std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
 
 struct ExpandedLayout {
-  explicit ExpandedLayout(std::size_t tokens) {
+  ExpandedLayout(std::size_t batch, std::size_t heads, std::size_t tokens) {
     rb = tokens <= 64 ? 64 : 128;
     row_blocks = (tokens + rb - 1) / rb;
     auto take = [&](std::size_t n) {
@@ -761,29 +1019,48 @@ struct ExpandedLayout {
       return at;
     };
     jobs = take(kGroups * sizeof(ExpandedJob));
+    unit_marks = take(batch * heads * row_blocks * sizeof(int));
+    part_marks = take(2 * kGroups * sizeof(int));
+    group_marks = take(kGroups * sizeof(int));
     part_ml = take(2 * kGroups * rb * 2 * sizeof(float));
     part_o = take(2 * kGroups * rb * kValueDim * sizeof(float));
   }
-  std::size_t rb, row_blocks, jobs, part_ml, part_o, bytes = 0;
+  std::size_t rb, row_blocks, jobs, unit_marks, part_marks, group_marks, part_ml, part_o, bytes = 0;
 };
+
+template <int RT>
+hipError_t launch_expanded(const ExpandedKernelArgs& k, const ExpandedStream& st, hipStream_t stream) {
+  constexpr int RB = 16 * kWaves * RT;
+  const dim3 grid(static_cast<unsigned>(kGroups));
+  expanded_kernel<RT><<<grid, 64 * kWaves, 0, stream>>>(k, st);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  expanded_redo_kernel<RT><<<grid, 64 * kWaves, 0, stream>>>(k, st);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const unsigned rows = static_cast<unsigned>(std::min(RB, k.tokens));
+  expanded_merge_kernel<<<dim3(grid.x, (rows + kMergeRows - 1) / kMergeRows), 256, 0, stream>>>(k, st, RB);
+  return hipGetLastError();
+}
 
 }  // namespace
 
-std::size_t expanded_workspace_bytes(std::size_t, std::size_t, std::size_t tokens, std::size_t) {
-  return ExpandedLayout(tokens).bytes;
+std::size_t expanded_workspace_bytes(std::size_t batch, std::size_t heads, std::size_t tokens,
+                                     std::size_t) {
+  return ExpandedLayout(batch, heads, tokens).bytes;
 }
 
 bool expanded_fits(const ExpandedArgs& a) {
   // Ranges, and places in them, are counted in 32 bits: of 2^38 tiles, a group's are
   // 2^30.
   const std::size_t units = a.batch * a.heads * ((a.tokens + 63) / 64);
-  return units == 0 || a.keys / kTile + 2 <= (std::size_t{1} << 38) / units;
+  return units == 0 || a.keys / kTile + 2 + kStart <= (std::size_t{1} << 38) / units;
 }
 
 hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) {
   if (a.batch == 0 || a.heads == 0 || a.tokens == 0) return hipSuccess;
   if (!expanded_fits(a)) return hipErrorInvalidValue;
-  const ExpandedLayout layout(a.tokens);
+  const ExpandedLayout layout(a.batch, a.heads, a.tokens);
   ExpandedKernelArgs k{};
   k.query = a.query;
   k.key = a.key;
@@ -805,22 +1082,14 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   auto* const base = static_cast<unsigned char*>(a.workspace);
   ExpandedStream st{};
   st.jobs = reinterpret_cast<ExpandedJob*>(base + layout.jobs);
+  st.unit_marks = reinterpret_cast<int*>(base + layout.unit_marks);
+  st.part_marks = reinterpret_cast<int*>(base + layout.part_marks);
+  st.group_marks = reinterpret_cast<int*>(base + layout.group_marks);
   st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
   st.part_o = reinterpret_cast<float*>(base + layout.part_o);
   st.groups = static_cast<int>(kGroups);
   st.row_blocks = static_cast<int>(layout.row_blocks);
-  const dim3 grid(static_cast<unsigned>(kGroups));
-  if (layout.rb == 64) {
-    expanded_kernel<1><<<grid, 64 * kWaves, 0, stream>>>(k, st);
-  } else {
-    expanded_kernel<2><<<grid, 64 * kWaves, 0, stream>>>(k, st);
-  }
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const std::size_t rows = std::min(layout.rb, a.tokens);
-  expanded_merge_kernel<<<dim3(static_cast<unsigned>(kGroups), static_cast<unsigned>((rows + 3) / 4)),
-                          256, 0, stream>>>(k, st, static_cast<int>(layout.rb));
-  return hipGetLastError();
+  return layout.rb == 64 ? launch_expanded<1>(k, st, stream) : launch_expanded<2>(k, st, stream);
 }
 
 }  // namespace helix::hip

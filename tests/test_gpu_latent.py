@@ -373,6 +373,67 @@ def test_expanded_sizes_of_numbers(device):
     assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want)
 
 
+@pytest.mark.parametrize("b,h,t,s", [(1, 2, 40, 300), (4, 40, 130, 140)])
+@pytest.mark.parametrize("kind", ["large keys", "large values", "large later values", "small values",
+                                  "small later values", "zero keys first", "weightless values first"])
+def test_expanded_range_of_numbers(device, b, h, t, s, kind):
+    """Numbers past 16 bits' range, units alone and in parts: as precise as 32 bits
+    are.  Scores keep their size, so their error stays near 2e-6 as above; an
+    output's is twice that of the values' sizes that it weighs, held to five times
+    that."""
+    p = Expanded(b, h, t, s)
+    first = slice(0, 33)
+    if kind == "large keys":
+        p.q, p.k, p.r = p.q * 2.0 ** -60, p.k * 2.0 ** 60, p.r * 2.0 ** 60
+    elif kind == "large values":
+        p.v *= np.float32(2.0 ** 90)
+    elif kind == "large later values":
+        p.v[:, :, 100:] *= np.float32(2.0 ** 40)
+    elif kind == "small values":
+        p.v *= np.float32(2.0 ** -90)
+    elif kind == "small later values":
+        p.v[:, :, 33:] *= np.float32(2.0 ** -40)
+    elif kind == "zero keys first":
+        p.q, p.k, p.r = p.q * 2.0 ** 30, p.k * 2.0 ** -30, p.r * 2.0 ** -30
+        p.k[:, :, first], p.r[:, first] = 0, 0
+    else:
+        # Scores of about -57 beside the others' of 2.
+        p.q[..., 0], p.k[:, :, first, 0] = 8, -100
+        p.k[:, :, 33:, 0] = 0
+        p.v[:, :, first] *= np.float32(2.0 ** 30)
+    p.q, p.k, p.r = (x.astype(np.float32) for x in (p.q, p.k, p.r))
+    got, want = p.run(), p.want()
+    p.v = np.abs(p.v)
+    held_to = np.full(t, 2e-5)
+    if kind == "weightless values first":
+        # Rows that see those keys alone have scores of size 58, not of size 2.  The sum
+        # is rounded at each matrix step, 6 steps of up to 6 products: to 58 * 2^-24 / 3 **
+        # 0.5 in the mean, 36 ** 0.5 times that together, 1.2e-5; twice that for an output,
+        # and five times that again for the largest of 80 thousand.
+        held_to[:max(33 - (s - t), 0)] = 1.2e-4
+    assert (np.abs(got - want) <= held_to[:, None] * p.want()).all()
+
+
+def test_expanded_empty_rows_beside_nan(device):
+    """Rows without a key are 0 whatever the keys and values of the unit's other rows,
+    of the sequence before and behind the sequence are."""
+    t, s = 70, 90
+    lengths = [20, 0, s, 0, 65] * 20
+    p = Expanded(100, 3, t, s, lengths=lengths)
+    for i, n in enumerate(lengths):
+        p.v[i, :, n:], p.k[i, :, n:], p.r[i, n:] = np.nan, np.nan, np.nan
+        if i % 10 < 5:
+            p.v[i, :, 0] = np.inf if i % 2 else np.nan
+    got, want = p.run(), p.want()
+    for i, n in enumerate(lengths):
+        empty = max(t - n, 0)
+        assert (got[i, :, :empty] == 0).all(), i
+        if i % 10 < 5:
+            assert not np.isfinite(got[i, :, empty:]).any(), i
+        else:
+            close(got[i], want[i])
+
+
 def test_expanded_bad_lengths(device):
     p = Expanded(4, 2, 10, 30)
     want = p.want()
