@@ -71,12 +71,11 @@ constexpr float kWild = 0x1.ffp+127f;
 // units): fp16's largest number is 2^16.
 constexpr float kSlack = 7.0f;
 // fp16 terms: logarithms of the factor on probabilities, and of where the largest
-// numbers of queries, keys and values go, and where numbers begin that do not fit.
+// numbers of queries, keys and values go.
 constexpr float kProbLog = 8.0f;
 constexpr int kQueryLog = 10;
 constexpr int kKeyLog = 4;
 constexpr int kValueLog = 8;
-constexpr float kOverflow = 65504.0f;
 // Outputs (of values as scaled) below which 2^-25 may count: it is 2^-21 of them.
 constexpr float kSmallOutput = 0x1p-4f;
 // What undoes the scores' powers of two must be below this, or this times the row's
@@ -121,23 +120,49 @@ struct ExpandedStream {
 constexpr int terms(bool f16) { return f16 ? 2 : 3; }
 constexpr int products(bool f16) { return f16 ? 3 : 6; }
 
-// The next term of x and y, packed into a word; x and y become what it leaves.
+// fp16 terms of x and y, packed into words: the first, of `scale` times the numbers (or
+// of the numbers), and the second, what the first one leaves.  A mixed-precision
+// instruction a number: the compiler must not see that it adds 0, multiplies by 1, or
+// knows a half of the word.
+__device__ __forceinline__ unsigned first_half_term(float x, float y, float scale) {
+  float zero = 0.0f;
+  asm("" : "+s"(zero));
+  const v2h h{static_cast<_Float16>(__builtin_fmaf(x, scale, zero)),
+              static_cast<_Float16>(__builtin_fmaf(y, scale, zero))};
+  unsigned word = __builtin_bit_cast(unsigned, h);
+  asm("" : "+v"(word));
+  return word;
+}
+__device__ __forceinline__ unsigned first_half_term(float x, float y) {
+  unsigned word = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2h));
+  asm("" : "+v"(word));
+  return word;
+}
+__device__ __forceinline__ unsigned second_half_term(float x, float y, float scale, unsigned first) {
+  const v2h h = __builtin_bit_cast(v2h, first);
+  const v2h r{static_cast<_Float16>(__builtin_fmaf(x, scale, -static_cast<float>(h[0]))),
+              static_cast<_Float16>(__builtin_fmaf(y, scale, -static_cast<float>(h[1])))};
+  return __builtin_bit_cast(unsigned, r);
+}
+__device__ __forceinline__ unsigned second_half_term(float x, float y, unsigned first) {
+  float one = 1.0f;
+  asm("" : "+s"(one));
+  return second_half_term(x, y, one, first);
+}
+// The next bf16 term; x and y become what it leaves.
+__device__ __forceinline__ unsigned next_bf16_term(float& x, float& y) {
+  const unsigned t = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2bf));
+  x -= __uint_as_float(t << 16);
+  y -= __uint_as_float(t & 0xffff0000u);
+  return t;
+}
+// Term `n`; `words` has those before it.
 template <bool F16>
-__device__ __forceinline__ unsigned next_term(float& x, float& y) {
+__device__ __forceinline__ void next_term(float& x, float& y, int n, unsigned* words) {
   if constexpr (F16) {
-    const v2h h = __builtin_convertvector((v2f{x, y}), v2h);
-    // One mixed-precision instruction a remainder: the compiler must not see that
-    // the factor is -1.
-    float minus = -1.0f;
-    asm("" : "+s"(minus));
-    x = __builtin_fmaf(static_cast<float>(h[0]), minus, x);
-    y = __builtin_fmaf(static_cast<float>(h[1]), minus, y);
-    return __builtin_bit_cast(unsigned, h);
+    words[n] = n == 0 ? first_half_term(x, y) : second_half_term(x, y, words[0]);
   } else {
-    const unsigned t = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2bf));
-    x -= __uint_as_float(t << 16);
-    y -= __uint_as_float(t & 0xffff0000u);
-    return t;
+    words[n] = next_bf16_term(x, y);
   }
 }
 
@@ -394,10 +419,9 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       raw_v[1][w] = *reinterpret_cast<const v4f*>(v + 64 + 4 * w);
     }
   };
-  // fp16 terms: the powers of two of the keys and values on their way, what undoes
-  // them by item, and the largest number so far.
+  // fp16 terms: the powers of two of the keys and values on their way, and what undoes
+  // them by item.
   float key_scale = 1.f, value_scale = 1.f, key_unscale[2] = {1.f, 1.f}, value_unscale[2] = {1.f, 1.f};
-  float most = 0.f;
   // The largest number among `n` chunks of keys that every row of the unit sees.
   auto largest = [&](const v4f (*x)[2], int n, const Source& s) {
     float top = 0.f;
@@ -431,14 +455,14 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
           chunk < 3 ? raw_k[chunk < 3 ? chunk : 0][pair / 2] : raw_v[chunk < 3 ? 0 : chunk - 3][pair / 2];
       sx = x[2 * (pair % 2)];
       sy = x[2 * (pair % 2) + 1];
-      if constexpr (F16) {
-        const float by = chunk < 3 ? key_scale : value_scale;
-        sx *= by;
-        sy *= by;
-        most = fmaxf(most, fmaxf(fabsf(sx), fabsf(sy)));
-      }
     }
-    words[pair][level] = next_term<F16>(sx, sy);
+    if constexpr (F16) {
+      const float by = chunk < 3 ? key_scale : value_scale;
+      words[pair][level] = level == 0 ? first_half_term(sx, sy, by)
+                                      : second_half_term(sx, sy, by, words[pair][0]);
+    } else {
+      words[pair][level] = next_bf16_term(sx, sy);
+    }
     if (pair != 3 || level != kTerms - 1) return;
     unsigned char* const to =
         chunk < 3 ? sh.item[buf].k[0] + key_place(srow, part + 8 * chunk)
@@ -526,7 +550,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
         for (int i = 0; i < 4; ++i) {
           float y0 = x[s][i >> 1][2 * (i & 1)] * grow, y1 = x[s][i >> 1][2 * (i & 1) + 1] * grow;
 #pragma unroll
-          for (int n = 0; n < kTerms; ++n) w[i][n] = next_term<F16>(y0, y1);
+          for (int n = 0; n < kTerms; ++n) next_term<F16>(y0, y1, n, w[i]);
         }
 #pragma unroll
         for (int i = 0; i < kTerms; ++i) {
@@ -647,7 +671,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       return;
     }
     if (level == 1) l[t] += py0 + py1;
-    p.w[t][n][level - 1] = next_term<F16>(py0, py1);
+    next_term<F16>(py0, py1, level - 1, p.w[t][n]);
   };
   const int vrow = 4 * grp + (col >> 2);
   unsigned value_at[4];
@@ -822,7 +846,8 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     const int slot = 2 * group + (starts ? 1 : 0);
     // (The last tile's values were in item n.)
     const float value_un = (n & 1) != 0 ? value_unscale[1] : value_unscale[0];
-    bool wrong = F16 && !(most < kOverflow);
+    // (A number that does not fit has terms of infinity and of less that: their sum is NaN.)
+    bool wrong = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const float sum = row_sum(l[t]);
