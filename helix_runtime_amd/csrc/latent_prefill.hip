@@ -385,11 +385,14 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   };
   auto source = [&](const ExpandedCursor& c) {
     Source s{};
-    s.k = a.key + static_cast<std::size_t>(c.b) * a.key_at.batch +
-          static_cast<std::size_t>(c.h) * a.key_at.head;
-    s.r = a.rope_key + static_cast<std::size_t>(c.b) * a.rope_at.batch;
-    s.v = a.value + static_cast<std::size_t>(c.b) * a.value_at.batch +
-          static_cast<std::size_t>(c.h) * a.value_at.head;
+    s.k = s.r = s.v = a.query + static_cast<std::size_t>(c.b) * a.query_at.batch;
+    if (c.length > 0) {
+      s.k = a.key + static_cast<std::size_t>(c.b) * a.key_at.batch +
+            static_cast<std::size_t>(c.h) * a.key_at.head;
+      s.r = a.rope_key + static_cast<std::size_t>(c.b) * a.rope_at.batch;
+      s.v = a.value + static_cast<std::size_t>(c.b) * a.value_at.batch +
+            static_cast<std::size_t>(c.h) * a.value_at.head;
+    }
     s.first = c.blk * kTile;
     s.length = c.length;
     s.seen = c.first;
@@ -397,30 +400,27 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     return s;
   };
   v4f raw_k[3][2], raw_v[2][2];  // (the third chunk of a key is the shared part's)
-  auto fetch_keys = [&](const Source& s) {
-    if (s.length == 0) return;  // (nothing is there, and nothing of it is used)
-    const std::size_t j = static_cast<std::size_t>(min(s.first + srow, s.length - 1));
-    const float* const k = s.k + j * a.key_at.token + part * 8;
-    const float* const r = s.r + j * a.rope_at.token + part * 8;
+  // Chunk i: three of a key's row, two of a value's.  (Of an empty sequence nothing is
+  // there, and nothing of it is used: a query's numbers are.)
+  auto fetch = [&](int i, const Source& sk, const Source& sv) {
+    const Source& s = i < 3 ? sk : sv;
+    const std::size_t j = static_cast<std::size_t>(max(min(s.first + srow, s.length - 1), 0));
+    const float* const from = i < 2    ? s.k + j * a.key_at.token + i * 64
+                              : i == 2 ? s.r + j * a.rope_at.token
+                                       : s.v + j * a.value_at.token + (i - 3) * 64;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      raw_k[0][w] = *reinterpret_cast<const v4f*>(k + 4 * w);
-      raw_k[1][w] = *reinterpret_cast<const v4f*>(k + 64 + 4 * w);
-      raw_k[2][w] = *reinterpret_cast<const v4f*>(r + 4 * w);
-    }
-  };
-  auto fetch_values = [&](const Source& s) {
-    if (s.length == 0) return;
-    const std::size_t j = static_cast<std::size_t>(min(s.first + srow, s.length - 1));
-    const float* const v = s.v + j * a.value_at.token + part * 8;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      raw_v[0][w] = *reinterpret_cast<const v4f*>(v + 4 * w);
-      raw_v[1][w] = *reinterpret_cast<const v4f*>(v + 64 + 4 * w);
+      const v4f x = *reinterpret_cast<const v4f*>(from + part * 8 + 4 * w);
+      if (i < 3) {
+        raw_k[i < 3 ? i : 0][w] = x;
+      } else {
+        raw_v[i < 3 ? 0 : i - 3][w] = x;
+      }
     }
   };
   // fp16 terms: the powers of two of the keys and values on their way, and what undoes
   // them by item.
+  Source staged_k{}, staged_v{};  // what the registers hold, or are sent for
   float key_scale = 1.f, value_scale = 1.f, key_unscale[2] = {1.f, 1.f}, value_unscale[2] = {1.f, 1.f};
   // The largest number among `n` chunks of keys that every row of the unit sees.
   auto largest = [&](const v4f (*x)[2], int n, const Source& s) {
@@ -464,6 +464,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       words[pair][level] = next_bf16_term(sx, sy);
     }
     if (pair != 3 || level != kTerms - 1) return;
+    fetch(chunk, staged_k, staged_v);
     unsigned char* const to =
         chunk < 3 ? sh.item[buf].k[0] + key_place(srow, part + 8 * chunk)
                   : sh.item[buf].v[0] + value_place(srow, part + 8 * (chunk - 3));
@@ -718,16 +719,14 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   };
 
   // ---- the range.  Step n: scores of tile n + 1 beside tile n's probabilities, tile
-  // n's outputs beside the way of item n + 2 into LDS, item n + 3 sent for.
+  // n's outputs beside the way of item n + 2 into LDS; behind each chunk's way, that of
+  // item n + 3 is sent for.
   ExpandedCursor ahead = cur;   // the tile whose keys are sent for
   Source now = source(ahead), before = now;  // its rows, and the last tile's
   now.opens = 1;
-  Source staged_k = now, staged_v = now;     // what the registers hold
   // Keys of the next tile and values of the one before.  (Behind the range the last
   // one again, which no one reads.)
-  auto fetch = [&] {
-    fetch_keys(now);
-    fetch_values(before);
+  auto advance = [&] {
     staged_k = now;
     staged_v = before;
     before = now;
@@ -754,25 +753,19 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       clean_values(buf, staged_v);
     }
   };
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w) raw_v[i][w] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w) raw_k[i][w] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
   // Items 0 and 1.  (Item 0's values, the first tile's, are not read.)
 #pragma unroll
   for (int item = 0; item < 2; ++item) {
-    fetch();
+    if (item == 0) {
+      advance();
+#pragma unroll
+      for (int i = 0; i < 5; ++i) fetch(i, staged_k, staged_v);
+    }
     ready(item);
+    advance();
 #pragma unroll
     for (int i = 0; i < kStageParts; ++i) stage(item, i);
   }
-  fetch();
   barrier();
   int n = 0;
   for (;;) {
@@ -801,6 +794,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       } else {
         ready(0);
       }
+      advance();
       Probabilities p;
       // Of the way into LDS, the parts that the scores' steps have room for.
       constexpr int kRoom = 2 * kSteps * kProducts - kProbParts;
@@ -837,7 +831,6 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
 #pragma unroll
         for (int j = i * kLeft / kSlots; j < (i + 1) * kLeft / kSlots; ++j) stage(into, kBeside + j);
       });
-      fetch();
       ++n;
       barrier();
     }
