@@ -50,6 +50,7 @@ using prefill_detail::v4f;
 using prefill_detail::v4s;
 using prefill_detail::v8bf;
 
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -60,7 +61,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeyDim = static_cast<int>(kLatentNope + kLatentRope);
 constexpr int kValueDim = static_cast<int>(kLatentNope);
 constexpr int kTile = 32;   // keys
-constexpr int kWaves = 4;
+constexpr int kMostWaves = 8;
 constexpr int kSteps = kKeyDim / 32;    // of the scores' sum
 constexpr int kDims = kValueDim / 16;   // tiles of output dims
 constexpr int kKeyPitch = kKeyDim * 2;  // bytes of a row of one term in LDS
@@ -205,9 +206,9 @@ struct ExpandedShared {
     __align__(1024) unsigned char v[terms(F16)][kTile * kValuePitch];
   };
   Item item[2];
-  unsigned poison[2][kWaves];  // bf16 terms: keys of the item's values that must not be seen
-  float most[kWaves];          // fp16 terms: the largest number of a first tile
-  int mark[kWaves];
+  unsigned poison[2][4];  // bf16 terms: keys of the item's values that must not be seen
+  float most[kMostWaves]; // fp16 terms: the largest number of a first tile
+  int mark[kMostWaves];
 };
 
 // What a unit's start costs a workgroup that has begun with another one, in tiles.
@@ -356,11 +357,11 @@ __device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, ExpandedC
 // The range that begins at `cur`.  RT tiles of 16 query rows a wavefront: units of RB =
 // 64 RT rows.  F16: which terms (bf16 ones compute again, and mark nothing).  `each`:
 // places of a range.
-template <int RT, bool F16>
+template <int WAVES, int RT, bool F16>
 __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, const ExpandedStream& st,
                                                ExpandedShared<F16>& sh, ExpandedCursor cur,
                                                long long each) {
-  constexpr int RB = 16 * kWaves * RT;
+  constexpr int RB = 16 * WAVES * RT;
   constexpr int kTerms = terms(F16), kProducts = products(F16);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -373,8 +374,12 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  // ---- staging: a thread has a key's chunks part, part + 8, .. of eight numbers.
-  const int srow = tid >> 3, part = tid & 7;
+  // ---- staging: of a key and of a value, a thread has chunks of eight numbers, kLanes
+  // apart, and of the shared part one of kShared numbers.
+  constexpr int kLanes = 64 * WAVES / kTile;
+  constexpr int kOwn = kValueDim / 8 / kLanes, kShared = static_cast<int>(kLatentRope) / kLanes;
+  constexpr int kPieces = 2 * kOwn + 1;
+  const int srow = tid / kLanes, part = tid % kLanes;
   struct Source {  // a tile's rows
     const float* k;
     const float* r;
@@ -399,22 +404,23 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     s.opens = 0;
     return s;
   };
-  v4f raw_k[3][2], raw_v[2][2];  // (the third chunk of a key is the shared part's)
-  // Chunk i: three of a key's row, two of a value's.  (Of an empty sequence nothing is
-  // there, and nothing of it is used: a query's numbers are.)
+  v4f raw_k[kOwn + 1][2], raw_v[kOwn][2];  // (a key's last chunk is the shared part's)
+  // Chunk i: a key's, then a value's.  (Of an empty sequence nothing is there, and
+  // nothing of it is used: a query's numbers are.)
   auto fetch = [&](int i, const Source& sk, const Source& sv) {
-    const Source& s = i < 3 ? sk : sv;
+    const Source& s = i <= kOwn ? sk : sv;
     const std::size_t j = static_cast<std::size_t>(max(min(s.first + srow, s.length - 1), 0));
-    const float* const from = i < 2    ? s.k + j * a.key_at.token + i * 64
-                              : i == 2 ? s.r + j * a.rope_at.token
-                                       : s.v + j * a.value_at.token + (i - 3) * 64;
+    const float* const from = i < kOwn    ? s.k + j * a.key_at.token + i * kLanes * 8 + part * 8
+                              : i == kOwn ? s.r + j * a.rope_at.token + part * kShared
+                                          : s.v + j * a.value_at.token +
+                                                (i - kOwn - 1) * kLanes * 8 + part * 8;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const v4f x = *reinterpret_cast<const v4f*>(from + part * 8 + 4 * w);
-      if (i < 3) {
-        raw_k[i < 3 ? i : 0][w] = x;
+    for (int w = 0; w < (i == kOwn ? kShared / 4 : 2); ++w) {
+      const v4f x = *reinterpret_cast<const v4f*>(from + 4 * w);
+      if (i <= kOwn) {
+        raw_k[i <= kOwn ? i : 0][w] = x;
       } else {
-        raw_v[i < 3 ? 0 : i - 3][w] = x;
+        raw_v[i <= kOwn ? 0 : i - kOwn - 1][w] = x;
       }
     }
   };
@@ -422,16 +428,18 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   // them by item.
   Source staged_k{}, staged_v{};  // what the registers hold, or are sent for
   float key_scale = 1.f, value_scale = 1.f, key_unscale[2] = {1.f, 1.f}, value_unscale[2] = {1.f, 1.f};
-  // The largest number among `n` chunks of keys that every row of the unit sees.
-  auto largest = [&](const v4f (*x)[2], int n, const Source& s) {
+  // The largest of the numbers (keys', or values') of keys that every row of the unit
+  // sees.
+  auto largest = [&](bool keys, const Source& s) {
     float top = 0.f;
     if (s.length > 0 && s.first + srow < min(s.seen, s.length)) {
-      for (int i = 0; i < n; ++i)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+      for (int i = 0; i < (keys ? kOwn + 1 : kOwn); ++i)
+#pragma unroll
+        for (int w = 0; w < (keys && i == kOwn ? kShared / 4 : 2); ++w)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float y = fabsf(x[i][w][e]);
+            const float y = fabsf(keys ? raw_k[i][w][e] : raw_v[i < kOwn ? i : 0][w][e]);
             top = fmaxf(top, y < 0x1p100f ? y : 0.f);
           }
     }
@@ -439,51 +447,65 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     for (int bit = 32; bit >= 1; bit /= 2) top = fmaxf(top, __shfl_xor(top, bit, 64));
     if (lane == 0) sh.most[wave] = top;
     barrier();
-    top = fmaxf(fmaxf(sh.most[0], sh.most[1]), fmaxf(sh.most[2], sh.most[3]));
+    top = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.most[w]);
     barrier();
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
   };
-  // The way into LDS in small parts, each one term of two numbers: a chunk's four pairs
-  // of numbers, then the next chunk's; its last part writes it.
-  constexpr int kStageParts = 5 * 4 * kTerms;
+  // The way into LDS in small parts, each one term of two numbers: a chunk's pairs of
+  // numbers, then the next chunk's; its last part writes it.
+  constexpr int kPairs = 2 * kOwn * 4 + kShared / 2;
+  constexpr int kStageParts = kPairs * kTerms;
   unsigned words[4][kTerms];
   float sx = 0.f, sy = 0.f;
   auto stage = [&](int buf, int i) {
-    const int chunk = i / (4 * kTerms), pair = i / kTerms % 4, level = i % kTerms;
+    const int level = i % kTerms, at = i / kTerms;
+    const bool before = at < 4 * kOwn, shared = !before && at < 4 * kOwn + kShared / 2;
+    const int in = before || shared ? at : at - kShared / 2 + 4;  // (as if all had four pairs)
+    const int chunk = in / 4, pair = in % 4;
     if (level == 0) {
-      const v4f x =
-          chunk < 3 ? raw_k[chunk < 3 ? chunk : 0][pair / 2] : raw_v[chunk < 3 ? 0 : chunk - 3][pair / 2];
+      const v4f x = chunk <= kOwn ? raw_k[chunk <= kOwn ? chunk : 0][pair / 2]
+                                  : raw_v[chunk <= kOwn ? 0 : chunk - kOwn - 1][pair / 2];
       sx = x[2 * (pair % 2)];
       sy = x[2 * (pair % 2) + 1];
     }
     if constexpr (F16) {
-      const float by = chunk < 3 ? key_scale : value_scale;
+      const float by = chunk <= kOwn ? key_scale : value_scale;
       words[pair][level] = level == 0 ? first_half_term(sx, sy, by)
                                       : second_half_term(sx, sy, by, words[pair][0]);
     } else {
       words[pair][level] = next_bf16_term(sx, sy);
     }
-    if (pair != 3 || level != kTerms - 1) return;
+    if (pair != (shared ? kShared / 2 : 4) - 1 || level != kTerms - 1) return;
     fetch(chunk, staged_k, staged_v);
     unsigned char* const to =
-        chunk < 3 ? sh.item[buf].k[0] + key_place(srow, part + 8 * chunk)
-                  : sh.item[buf].v[0] + value_place(srow, part + 8 * (chunk - 3));
-    const unsigned plane = chunk < 3 ? kTile * kKeyPitch : kTile * kValuePitch;
+        chunk < kOwn    ? sh.item[buf].k[0] + key_place(srow, part + kLanes * chunk)
+        : chunk == kOwn ? sh.item[buf].k[0] + key_place(srow, 16 + part * kShared / 8) +
+                              part * kShared * 2 % 16
+                        : sh.item[buf].v[0] + value_place(srow, part + kLanes * (chunk - kOwn - 1));
+    const unsigned plane = chunk <= kOwn ? kTile * kKeyPitch : kTile * kValuePitch;
 #pragma unroll
     for (int n = 0; n < kTerms; ++n) {
-      *reinterpret_cast<v4u*>(to + n * plane) = v4u{words[0][n], words[1][n], words[2][n], words[3][n]};
+      if (shared && kShared == 4) {
+        *reinterpret_cast<v2u*>(to + n * plane) = v2u{words[0][n], words[1][n]};
+      } else {
+        *reinterpret_cast<v4u*>(to + n * plane) =
+            v4u{words[0][n], words[1][n], words[2][n], words[3][n]};
+      }
     }
   };
   // bf16 terms: values of keys that some row of the unit does not see must be finite: those
   // behind the sequence's last become 0, and of the others those with terms that are
   // not; the latter's keys are noted.
   auto clean_values = [&](int buf, const Source& s) {
+    static_assert(F16 || kLanes == 8, "eight threads a key");
     unsigned poison = 0;
     if (s.first + kTile > s.seen) {
       const int j = s.first + srow;
       bool wild = false;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kOwn; ++i)
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -495,7 +517,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       }
       const bool wipe = j >= s.length || ((poison >> (srow & 31)) & 1u) != 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kOwn; ++i)
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -745,9 +767,9 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   // Before an item's way into LDS: its powers of two, or its values made finite.
   auto ready = [&](int buf) {
     if constexpr (F16) {
-      if (staged_k.opens != 0) key_scale = grow_to(largest(raw_k, 3, staged_k), kKeyLog, key_unscale[buf]);
+      if (staged_k.opens != 0) key_scale = grow_to(largest(true, staged_k), kKeyLog, key_unscale[buf]);
       if (staged_k.opens == 0) key_unscale[buf] = key_unscale[buf ^ 1];
-      if (staged_v.opens != 0) value_scale = grow_to(largest(raw_v, 2, staged_v), kValueLog, value_unscale[buf]);
+      if (staged_v.opens != 0) value_scale = grow_to(largest(false, staged_v), kValueLog, value_unscale[buf]);
       if (staged_v.opens == 0) value_unscale[buf] = value_unscale[buf ^ 1];
     } else {
       clean_values(buf, staged_v);
@@ -759,7 +781,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     if (item == 0) {
       advance();
 #pragma unroll
-      for (int i = 0; i < 5; ++i) fetch(i, staged_k, staged_v);
+      for (int i = 0; i < kPieces; ++i) fetch(i, staged_k, staged_v);
     }
     ready(item);
     advance();
@@ -884,7 +906,9 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       if (lane == 0) sh.mark[wave] = any ? 1 : 0;
       barrier();
       if (tid == 0) {
-        const int mark = sh.mark[0] | sh.mark[1] | sh.mark[2] | sh.mark[3];
+        int mark = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) mark |= sh.mark[w];
         *(complete ? st.unit_marks + unit_index(a, cur) : st.part_marks + slot) = mark;
         if (mark != 0) st.group_marks[group] = 1;
         if (ends && !starts) {
@@ -899,11 +923,11 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   if constexpr (!F16) barrier();  // (another unit may follow)
 }
 
-template <int RT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4)))
     void expanded_kernel(ExpandedKernelArgs a, ExpandedStream st) {
   __shared__ ExpandedShared<true> sh;
-  constexpr int RB = 16 * kWaves * RT;
+  constexpr int RB = 16 * WAVES;
   const int group = static_cast<int>(blockIdx.x);
   if (threadIdx.x == 0) {
     st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
@@ -912,18 +936,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 
   ExpandedCursor cur{};
   long long each;
   if (!first_place<RB>(a, st, group, static_cast<int>(threadIdx.x) & 63, each, cur)) return;
-  expanded_range<RT, true>(a, st, sh, cur, each);
+  expanded_range<WAVES, 1, true>(a, st, sh, cur, each);
 }
 
 // The same ranges' parts of units that are marked, again.
 template <int RT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
     void expanded_redo_kernel(ExpandedKernelArgs a, ExpandedStream st) {
   __shared__ ExpandedShared<false> sh;
-  constexpr int RB = 16 * kWaves * RT;
+  constexpr int RB = 64 * RT;
   const int tid = static_cast<int>(threadIdx.x);
   int marks = 0;
-  for (int g = tid; g < st.groups; g += 64 * kWaves) marks |= st.group_marks[g];
+  for (int g = tid; g < st.groups; g += 256) marks |= st.group_marks[g];
   if (__syncthreads_or(marks) == 0) return;
   ExpandedCursor cur{};
   long long each;
@@ -936,14 +960,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 
     } else {
       const int first = static_cast<int>((cur.base + kStart) / each);
       const int last = static_cast<int>((cur.base + kStart + cur.nb - 1) / each);
-      for (int g = first + tid; g <= last; g += 64 * kWaves) {
+      for (int g = first + tid; g <= last; g += 256) {
         mark |= st.part_marks[2 * g + (g == first ? 1 : 0)];
       }
     }
     if (__syncthreads_or(mark) != 0) {
       ExpandedCursor one = cur;
       one.left = 0;
-      expanded_range<RT, false>(a, st, sh, one, each);
+      expanded_range<4, RT, false>(a, st, sh, one, each);
     }
     if (!more_units(cur)) break;
     next_unit<RB>(a, cur);
@@ -1048,12 +1072,12 @@ struct ExpandedLayout {
 
 template <int RT>
 hipError_t launch_expanded(const ExpandedKernelArgs& k, const ExpandedStream& st, hipStream_t stream) {
-  constexpr int RB = 16 * kWaves * RT;
+  constexpr int RB = 64 * RT;
   const dim3 grid(static_cast<unsigned>(kGroups));
-  expanded_kernel<RT><<<grid, 64 * kWaves, 0, stream>>>(k, st);
+  expanded_kernel<4 * RT><<<grid, 256 * RT, 0, stream>>>(k, st);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  expanded_redo_kernel<RT><<<grid, 64 * kWaves, 0, stream>>>(k, st);
+  expanded_redo_kernel<RT><<<grid, 256, 0, stream>>>(k, st);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const unsigned rows = static_cast<unsigned>(std::min(RB, k.tokens));
