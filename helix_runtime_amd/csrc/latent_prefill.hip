@@ -191,7 +191,7 @@ __device__ __forceinline__ float grow_to(float most, int to, float& unscale) {
 // (scores) and of 32 bytes of 8 rows (outputs) hits distinct banks: key rows lie 128
 // bytes from a multiple of 256 apart, value rows 256.
 __device__ __forceinline__ unsigned key_place(int row, int chunk) {
-  const int turn = (row & 6) | ((row >> 3) & 1);
+  const int turn = (row & 2) | ((row & 8) >> 1);
   return static_cast<unsigned>(row * kKeyPitch + (chunk ^ turn) * 16);
 }
 __device__ __forceinline__ unsigned value_place(int row, int chunk) {
