@@ -20,10 +20,10 @@
 // - expanded_kernel: two fp16 terms (22 bits and a sign: the rounding of an fp32
 //   number), of whose four products the three above 2^-22 of the largest are taken.
 //   fp16's range asks for powers of two: a query row's own, one for the keys and one
-//   for the values of a unit's part, by the largest of the first tile's numbers that
-//   all its rows see.  Those keys go to [2^4, 2^5) and values to [2^8, 2^9), so that
-//   keys 2^11 and values 2^7 times as large fit; 2^-25 is lost of numbers as scaled.
-//   Probabilities carry a factor of 2^8.
+//   for the values of a unit's part, by the largest numbers of its first eight keys
+//   that all its rows see.  Those keys go to [2^4, 2^5) and values to [2^6, 2^7), so
+//   that keys 2^11 and values 2^9 times as large fit; 2^-25 is lost of numbers as
+//   scaled.  Probabilities carry a factor of 2^8.
 // - expanded_redo_kernel: three bf16 terms (24 bits, fp32's range), of whose nine
 //   products the six above 2^-26 are taken.  It computes parts again whose unit the
 //   first one marked: with numbers past its range, a sum or output that is not finite
@@ -38,6 +38,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 namespace helix::hip {
 namespace {
@@ -62,6 +63,7 @@ constexpr int kKeyDim = static_cast<int>(kLatentNope + kLatentRope);
 constexpr int kValueDim = static_cast<int>(kLatentNope);
 constexpr int kTile = 32;   // keys
 constexpr int kMostWaves = 8;
+constexpr int kSample = 8;  // keys of a part that give its powers of two
 constexpr int kSteps = kKeyDim / 32;    // of the scores' sum
 constexpr int kDims = kValueDim / 16;   // tiles of output dims
 constexpr int kKeyPitch = kKeyDim * 2;  // bytes of a row of one term in LDS
@@ -76,7 +78,7 @@ constexpr float kSlack = 7.0f;
 constexpr float kProbLog = 8.0f;
 constexpr int kQueryLog = 10;
 constexpr int kKeyLog = 4;
-constexpr int kValueLog = 8;
+constexpr int kValueLog = 6;
 // Outputs (of values as scaled) below which 2^-25 may count: it is 2^-21 of them.
 constexpr float kSmallOutput = 0x1p-4f;
 // What undoes the scores' powers of two must be below this, or this times the row's
@@ -108,10 +110,10 @@ struct ExpandedStream {
   float* part_o;     // [2 * groups, RB, 128]
   float* part_ml;    // [2 * groups, RB, 2]
   ExpandedJob* jobs; // [groups]
-  // 1: to compute again.
-  int* unit_marks;   // [row blocks, batch, heads]: units that a group has whole
-  int* part_marks;   // [2 * groups]: partials
-  int* group_marks;  // [groups]: any of the group's
+  // A byte a wavefront: 1 if its rows are to be computed again.
+  unsigned char* unit_marks;   // [row blocks, batch, heads, waves]: units that a group has whole
+  unsigned char* part_marks;   // [2 * groups, waves]: partials
+  unsigned char* group_marks;  // [groups, waves]: any of the group's
   int groups;
   int row_blocks;    // units of a (sequence, head), at most
 };
@@ -198,17 +200,21 @@ __device__ __forceinline__ unsigned value_place(int row, int chunk) {
   return static_cast<unsigned>(row * kValuePitch + (chunk ^ (2 * (row & 7))) * 16);
 }
 
-// Item i of a range: keys of tile i and values of tile i - 1, what one step takes.
+// Item i of a range: keys of tile i and values of tile i - 1, what one step takes.  Of
+// eight wavefronts four are half a step behind: item i + 2 is on its way while the last
+// of item i is read.
 template <bool F16>
 struct ExpandedShared {
   struct Item {
     __align__(1024) unsigned char k[terms(F16)][kTile * kKeyPitch];
     __align__(1024) unsigned char v[terms(F16)][kTile * kValuePitch];
   };
-  Item item[2];
+  static constexpr int kItems = F16 ? 3 : 2;
+  Item item[kItems];
   unsigned poison[2][4];  // bf16 terms: keys of the item's values that must not be seen
-  float most[kMostWaves]; // fp16 terms: the largest number of a first tile
-  int mark[kMostWaves];
+  // fp16 terms: what undoes the powers of two of an item's keys and values, where a unit's
+  // begin with it, by the item's number modulo 4.
+  float key_unscale[kMostWaves][4], value_unscale[kMostWaves][4];
 };
 
 // What a unit's start costs a workgroup that has begun with another one, in tiles.
@@ -424,34 +430,48 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       }
     }
   };
-  // fp16 terms: the powers of two of the keys and values on their way, and what undoes
-  // them by item.
   Source staged_k{}, staged_v{};  // what the registers hold, or are sent for
-  float key_scale = 1.f, value_scale = 1.f, key_unscale[2] = {1.f, 1.f}, value_unscale[2] = {1.f, 1.f};
-  // The largest of the numbers (keys', or values') of keys that every row of the unit
-  // sees.
-  auto largest = [&](bool keys, const Source& s) {
-    float top = 0.f;
-    if (s.length > 0 && s.first + srow < min(s.seen, s.length)) {
+  // fp16 terms: the powers of two of the keys and values on their way, and the next
+  // unit's of the values.
+  float key_scale = 1.f, value_scale = 1.f, next_value_scale = 1.f, next_value_unscale = 1.f;
+  // Those of the unit that begins with the keys on their way, by the first of its keys
+  // that all its rows see.  Each wavefront finds them for itself.
+  auto sample = [&](int item) {
+    const Source& s = staged_k;
+    const int have = min(min(s.seen, s.length) - s.first, kSample);
+    float top[2] = {0.f, 0.f};
+    if (have > 0) {
+      const int r = lane / kSample, c = lane % kSample;
+      const std::size_t j = static_cast<std::size_t>(s.first + min(r, have - 1));
+      const float* const k = s.k + j * a.key_at.token + 4 * c;
+      const float* const rope = s.r + j * a.rope_at.token + 4 * c;
+      const float* const v = s.v + j * a.value_at.token + 4 * c;
+      auto take = [](float& most, v4f x) {
 #pragma unroll
-      for (int i = 0; i < (keys ? kOwn + 1 : kOwn); ++i)
+        for (int e = 0; e < 4; ++e) {
+          const float y = fabsf(x[e]);
+          most = fmaxf(most, y < 0x1p100f ? y : 0.f);
+        }
+      };
 #pragma unroll
-        for (int w = 0; w < (keys && i == kOwn ? kShared / 4 : 2); ++w)
+      for (int i = 0; i < kValueDim; i += 4 * kSample) {
+        take(top[0], *reinterpret_cast<const v4f*>(k + i));
+        take(top[1], *reinterpret_cast<const v4f*>(v + i));
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = fabsf(keys ? raw_k[i][w][e] : raw_v[i < kOwn ? i : 0][w][e]);
-            top = fmaxf(top, y < 0x1p100f ? y : 0.f);
-          }
+      for (int i = 0; i < static_cast<int>(kLatentRope); i += 4 * kSample) {
+        take(top[0], *reinterpret_cast<const v4f*>(rope + i));
+      }
     }
 #pragma unroll
-    for (int bit = 32; bit >= 1; bit /= 2) top = fmaxf(top, __shfl_xor(top, bit, 64));
-    if (lane == 0) sh.most[wave] = top;
-    barrier();
-    top = 0.f;
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sh.most[w]);
-    barrier();
-    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
+      for (int bit = 32; bit >= 1; bit /= 2) top[i] = fmaxf(top[i], __shfl_xor(top[i], bit, 64));
+    }
+    float key_un;
+    key_scale = grow_to(top[0], kKeyLog, key_un);
+    next_value_scale = grow_to(top[1], kValueLog, next_value_unscale);
+    if (lane == 0) sh.key_unscale[wave][item & 3] = key_un;
   };
   // The way into LDS in small parts, each one term of two numbers: a chunk's pairs of
   // numbers, then the next chunk's; its last part writes it.
@@ -479,11 +499,12 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     }
     if (pair != (shared ? kShared / 2 : 4) - 1 || level != kTerms - 1) return;
     fetch(chunk, staged_k, staged_v);
+    auto& into = sh.item[buf];
     unsigned char* const to =
-        chunk < kOwn    ? sh.item[buf].k[0] + key_place(srow, part + kLanes * chunk)
-        : chunk == kOwn ? sh.item[buf].k[0] + key_place(srow, 16 + part * kShared / 8) +
+        chunk < kOwn    ? into.k[0] + key_place(srow, part + kLanes * chunk)
+        : chunk == kOwn ? into.k[0] + key_place(srow, 16 + part * kShared / 8) +
                               part * kShared * 2 % 16
-                        : sh.item[buf].v[0] + value_place(srow, part + kLanes * (chunk - kOwn - 1));
+                        : into.v[0] + value_place(srow, part + kLanes * (chunk - kOwn - 1));
     const unsigned plane = chunk <= kOwn ? kTile * kKeyPitch : kTile * kValuePitch;
 #pragma unroll
     for (int n = 0; n < kTerms; ++n) {
@@ -764,13 +785,15 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       now.opens = 0;
     }
   };
-  // Before an item's way into LDS: its powers of two, or its values made finite.
-  auto ready = [&](int buf) {
+  // Before item i's way into LDS, into `buf`: its powers of two, or its values made
+  // finite.
+  auto ready = [&](int i, int buf) {
     if constexpr (F16) {
-      if (staged_k.opens != 0) key_scale = grow_to(largest(true, staged_k), kKeyLog, key_unscale[buf]);
-      if (staged_k.opens == 0) key_unscale[buf] = key_unscale[buf ^ 1];
-      if (staged_v.opens != 0) value_scale = grow_to(largest(false, staged_v), kValueLog, value_unscale[buf]);
-      if (staged_v.opens == 0) value_unscale[buf] = value_unscale[buf ^ 1];
+      if (staged_v.opens != 0) {
+        value_scale = next_value_scale;
+        if (lane == 0) sh.value_unscale[wave][i & 3] = next_value_unscale;
+      }
+      if (staged_k.opens != 0) sample(i);
     } else {
       clean_values(buf, staged_v);
     }
@@ -783,23 +806,28 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) fetch(i, staged_k, staged_v);
     }
-    ready(item);
+    ready(item, item);
     advance();
 #pragma unroll
     for (int i = 0; i < kStageParts; ++i) stage(item, i);
   }
   barrier();
-  int n = 0;
+  constexpr int kItems = ExpandedShared<F16>::kItems;
+  constexpr bool kBehind = WAVES == 8;  // whether four wavefronts are half a step behind
+  if (kBehind && wave >= 4) barrier();
+  int n = 0, slot = 0;  // n modulo kItems
+  auto later = [](int at, int by) { return at + by >= kItems ? at + by - kItems : at + by; };
   for (;;) {
-    start(cur, (n & 1) != 0 ? key_unscale[1] : key_unscale[0]);
+    start(cur, F16 ? sh.key_unscale[wave][n & 3] : 1.f);
+    const float value_un = F16 ? sh.value_unscale[wave][(n + 1) & 3] : 1.f;
     const int from = cur.blk, to = cur.to;
     const int whole = max(cur.first, 0) / kTile;  // tiles before are seen by every row
     v4f sc[RT][2];
-    scores(n & 1, sc, [](int) {});
-    // (Item n's keys are taken before it is written again.)
-    barrier();
+    scores(slot, sc, [](int) {});
+    // (Of two items, this one's keys are taken before it is written again.)
+    if constexpr (kItems == 2) barrier();
     for (int blk = from; blk < to; ++blk) {
-      const int buf = (n + 1) & 1, into = n & 1;
+      const int buf = later(slot, 1), into = later(slot, 2);
       if (blk >= whole) {
         unsigned poison = 0;
         if constexpr (!F16) {
@@ -811,11 +839,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       float ref[RT];
 #pragma unroll
       for (int t = 0; t < RT; ++t) ref[t] = (m[t] == -INFINITY ? 0.f : m[t]) - (F16 ? kProbLog : 0.f);
-      if (into != 0) {  // (which item's the powers are is known to the compiler)
-        ready(1);
-      } else {
-        ready(0);
-      }
+      ready(n + 2, into);
       advance();
       Probabilities p;
       // Of the way into LDS, the parts that the scores' steps have room for.
@@ -836,31 +860,33 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
           asm("" : "+v"(ref_here[t]));
         }
         scores(buf, sc, [&](int i) {
-          if (i < kProbParts) {
-            probability(i, last, ref_here, p);
-          } else if (i - kProbParts < kBeside) {
-            stage(into, i - kProbParts);
+          if (i < kBeside) {
+            stage(into, i);
+          } else if (i - kBeside < kProbParts) {
+            probability(i - kBeside, last, ref_here, p);
           }
+          if (kBehind && i == kBeside - 1) barrier();
         });
       } else {
 #pragma unroll
-        for (int i = 0; i < kProbParts; ++i) probability(i, sc, ref, p);
-#pragma unroll
         for (int i = 0; i < kBeside; ++i) stage(into, i);
+        if (kBehind) barrier();
+#pragma unroll
+        for (int i = 0; i < kProbParts; ++i) probability(i, sc, ref, p);
       }
+      static_assert(!kBehind || kBeside == kStageParts, "an item is whole before the values");
       add_values(buf, p, [&](int i) {
         constexpr int kLeft = kStageParts - kBeside, kSlots = kDims * kProducts;
 #pragma unroll
         for (int j = i * kLeft / kSlots; j < (i + 1) * kLeft / kSlots; ++j) stage(into, kBeside + j);
       });
       ++n;
+      slot = buf;
       barrier();
     }
     // The part's end.
     const bool starts = from == 0, ends = to == cur.nb, complete = starts && ends;
-    const int slot = 2 * group + (starts ? 1 : 0);
-    // (The last tile's values were in item n.)
-    const float value_un = (n & 1) != 0 ? value_unscale[1] : value_unscale[0];
+    const int partial = 2 * group + (starts ? 1 : 0);
     // (A number that does not fit has terms of infinity and of less that: their sum is NaN.)
     bool wrong = false;
 #pragma unroll
@@ -891,26 +917,25 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
           (complete ? a.out + static_cast<std::size_t>(cur.b) * a.out_at.batch +
                           static_cast<std::size_t>(cur.h) * a.out_at.head +
                           static_cast<std::size_t>(row) * a.out_at.token
-                    : st.part_o + (static_cast<std::size_t>(slot) * RB + local) * kValueDim) +
+                    : st.part_o + (static_cast<std::size_t>(partial) * RB + local) * kValueDim) +
           4 * grp;
 #pragma unroll
       for (int dt = 0; dt < kDims; ++dt) *reinterpret_cast<v4f*>(dst + 16 * dt) = o[t][dt] * f;
       if (!complete && grp == 0) {
-        float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * RB + local) * 2;
+        float* const ml = st.part_ml + (static_cast<std::size_t>(partial) * RB + local) * 2;
         ml[0] = m[t];
         ml[1] = cur.bad != 0 ? NAN : sum;
       }
     }
     if constexpr (F16) {
       const bool any = __ballot(wrong) != 0;
-      if (lane == 0) sh.mark[wave] = any ? 1 : 0;
-      barrier();
+      if (lane == 0) {
+        unsigned char* const mark =
+            complete ? st.unit_marks + unit_index(a, cur) * WAVES : st.part_marks + partial * WAVES;
+        mark[wave] = any ? 1 : 0;
+        if (any) st.group_marks[group * WAVES + wave] = 1;
+      }
       if (tid == 0) {
-        int mark = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) mark |= sh.mark[w];
-        *(complete ? st.unit_marks + unit_index(a, cur) : st.part_marks + slot) = mark;
-        if (mark != 0) st.group_marks[group] = 1;
         if (ends && !starts) {
           st.jobs[group] = ExpandedJob{cur.b, cur.h, cur.rb,
                                        static_cast<int>((cur.base + kStart) / each), group};
@@ -920,6 +945,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     if (!more_units(cur)) break;
     next_unit<RB>(a, cur);
   }
+  if (kBehind && wave < 4) barrier();
   if constexpr (!F16) barrier();  // (another unit may follow)
 }
 
@@ -929,10 +955,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
   __shared__ ExpandedShared<true> sh;
   constexpr int RB = 16 * WAVES;
   const int group = static_cast<int>(blockIdx.x);
-  if (threadIdx.x == 0) {
-    st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
-    st.group_marks[group] = 0;
-  }
+  if (threadIdx.x == 0) st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
+  if (threadIdx.x % 64 == 0) st.group_marks[group * WAVES + threadIdx.x / 64] = 0;
   ExpandedCursor cur{};
   long long each;
   if (!first_place<RB>(a, st, group, static_cast<int>(threadIdx.x) & 63, each, cur)) return;
@@ -946,22 +970,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
   __shared__ ExpandedShared<false> sh;
   constexpr int RB = 64 * RT;
   const int tid = static_cast<int>(threadIdx.x);
-  int marks = 0;
-  for (int g = tid; g < st.groups; g += 256) marks |= st.group_marks[g];
-  if (__syncthreads_or(marks) == 0) return;
+  // (Marks of the wavefronts that had a unit, in one word.)
+  using Marks = std::conditional_t<RT == 2, unsigned long long, unsigned>;
+  const auto* const unit_marks = reinterpret_cast<const Marks*>(st.unit_marks);
+  const auto* const part_marks = reinterpret_cast<const Marks*>(st.part_marks);
+  const auto* const group_marks = reinterpret_cast<const Marks*>(st.group_marks);
+  static_assert(sizeof(Marks) == 4 * RT, "a byte a wavefront");
+  bool marked = false;
+  for (int g = tid; g < st.groups; g += 256) marked = marked || group_marks[g] != 0;
+  if (__syncthreads_or(marked) == 0) return;
   ExpandedCursor cur{};
   long long each;
   if (!first_place<RB>(a, st, static_cast<int>(blockIdx.x), tid & 63, each, cur)) return;
   for (;;) {
     // A unit in several parts is marked if one of them is.
-    int mark = 0;
+    bool mark = false;
     if (cur.blk == 0 && cur.to == cur.nb) {
-      mark = st.unit_marks[unit_index(a, cur)];
+      mark = unit_marks[unit_index(a, cur)] != 0;
     } else {
       const int first = static_cast<int>((cur.base + kStart) / each);
       const int last = static_cast<int>((cur.base + kStart + cur.nb - 1) / each);
       for (int g = first + tid; g <= last; g += 256) {
-        mark |= st.part_marks[2 * g + (g == first ? 1 : 0)];
+        mark = mark || part_marks[2 * g + (g == first ? 1 : 0)] != 0;
       }
     }
     if (__syncthreads_or(mark) != 0) {
@@ -1061,9 +1091,9 @@ struct ExpandedLayout {
       return at;
     };
     jobs = take(kGroups * sizeof(ExpandedJob));
-    unit_marks = take(batch * heads * row_blocks * sizeof(int));
-    part_marks = take(2 * kGroups * sizeof(int));
-    group_marks = take(kGroups * sizeof(int));
+    unit_marks = take(batch * heads * row_blocks * rb / 16);
+    part_marks = take(2 * kGroups * rb / 16);
+    group_marks = take(kGroups * rb / 16);
     part_ml = take(2 * kGroups * rb * 2 * sizeof(float));
     part_o = take(2 * kGroups * rb * kValueDim * sizeof(float));
   }
@@ -1124,9 +1154,9 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   auto* const base = static_cast<unsigned char*>(a.workspace);
   ExpandedStream st{};
   st.jobs = reinterpret_cast<ExpandedJob*>(base + layout.jobs);
-  st.unit_marks = reinterpret_cast<int*>(base + layout.unit_marks);
-  st.part_marks = reinterpret_cast<int*>(base + layout.part_marks);
-  st.group_marks = reinterpret_cast<int*>(base + layout.group_marks);
+  st.unit_marks = base + layout.unit_marks;
+  st.part_marks = base + layout.part_marks;
+  st.group_marks = base + layout.group_marks;
   st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
   st.part_o = reinterpret_cast<float*>(base + layout.part_o);
   st.groups = static_cast<int>(kGroups);
