@@ -2183,7 +2183,7 @@ int helix_latent_prefill_attention(const float* query, const size_t* query_strid
     a.keys = keys;
     a.scale = scale;
     check(helix::hip::expanded_fits(a), Status::kUnsupported, op,
-          "too many queries and keys for one call");
+          "too many queries and keys for one call, or rows of keys too far apart");
     helix::hip_check(helix::hip::launch_expanded_attention(a, as_stream(stream)), op);
   });
 }

@@ -68,7 +68,8 @@ struct ExpandedArgs {
 };
 std::size_t expanded_workspace_bytes(std::size_t batch, std::size_t heads, std::size_t tokens,
                                      std::size_t keys);
-// Whether the launch's tiles of keys can be counted; where not, it fails.
+// Whether the launch's tiles of keys can be counted, and keys' rows are below 2^25
+// numbers apart; where not, it fails.
 bool expanded_fits(const ExpandedArgs& a);
 hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream);
 

@@ -10,8 +10,8 @@
 // unit, its keys up to the last that one of them sees are tiles of 32.  A fixed grid
 // takes equal ranges of the flat list of all units' tiles; units that cross ranges
 // leave partials (maximum, sum, output), which expanded_merge_kernel joins.  A head's
-// units lie far apart in the list, so that the workgroups that read the same keys do
-// so at one time.
+// units follow each other in the list, and an XCD has ranges that do, so that row
+// blocks that read the same keys at about the same time find them in its L2.
 //
 // Matrix form.  As in the absorbed form: S^T = K Q^T, O^T += V^T P^T, a lane holding
 // keys of one query row; a wavefront has 32 rows, so that an operand out of LDS serves
@@ -63,6 +63,7 @@ constexpr int kKeyDim = static_cast<int>(kLatentNope + kLatentRope);
 constexpr int kValueDim = static_cast<int>(kLatentNope);
 constexpr int kTile = 32;   // keys
 constexpr int kMostWaves = 8;
+constexpr std::size_t kMostStride = std::size_t{1} << 25;  // of a key's row, in numbers
 constexpr int kSample = 8;  // keys of a part that give its powers of two
 constexpr int kSteps = kKeyDim / 32;    // of the scores' sum
 constexpr int kDims = kValueDim / 16;   // tiles of output dims
@@ -115,7 +116,6 @@ struct ExpandedStream {
   unsigned char* part_marks;   // [2 * groups, waves]: partials
   unsigned char* group_marks;  // [groups, waves]: any of the group's
   int groups;
-  int row_blocks;    // units of a (sequence, head), at most
 };
 
 // Terms of an fp32 number, fp16 or bf16, and the products of two numbers' that are
@@ -244,16 +244,35 @@ __device__ __forceinline__ int unit_tiles(int length, int count, int rb) {
   return max((sees + kTile - 1) / kTile, 1);
 }
 
+// Places of a sequence's row blocks, for each head: the sum over them of unit_tiles and
+// kStart.  Of all but the last block the tiles grow by RB / kTile a block, from 1 up.
 template <int RB>
-__device__ __forceinline__ int entry_tiles(const ExpandedKernelArgs& a, int row_blocks, long long e) {
-  if (e >= static_cast<long long>(row_blocks) * a.batch) return 0;
-  const int rb = static_cast<int>(e / a.batch);
-  const int b = static_cast<int>(e - static_cast<long long>(rb) * a.batch);
-  int length = a.key_lengths != nullptr ? a.key_lengths[b] : a.keys;
-  if (length < 0 || length > a.keys) length = 0;
-  return unit_tiles<RB>(length, clamped_count(a, b), rb);
+__device__ __forceinline__ long long head_places(int length, int count) {
+  if (count <= 0) return 0;
+  constexpr long long kGrow = RB / kTile;
+  const long long blocks = (count + RB - 1) / RB;
+  const int before = length - count;
+  // (Rounded up, whatever the sign.)
+  const long long tiles = before >= 0 ? (before + kTile - 1) / kTile : -(-before / kTile);
+  const long long ones = tiles >= 1 ? 0 : min((-tiles) / kGrow, blocks - 1);
+  const long long rest = blocks - 1 - ones;
+  return ones + rest * tiles + kGrow * (rest * (ones + blocks) / 2) +
+         max((length + kTile - 1) / kTile, 1) + kStart * blocks;
 }
 
+template <int RB>
+__device__ __forceinline__ long long sequence_places(const ExpandedKernelArgs& a, long long b) {
+  if (b >= a.batch) return 0;
+  int length = a.key_lengths != nullptr ? a.key_lengths[b] : a.keys;
+  if (length < 0 || length > a.keys) length = 0;
+  return head_places<RB>(length, clamped_count(a, static_cast<int>(b)));
+}
+
+template <int RB>
+__device__ __forceinline__ void set_unit(ExpandedCursor& c) {
+  c.nb = unit_tiles<RB>(c.length, c.count, c.rb);
+  c.first = c.length - c.count + c.rb * RB + 1;
+}
 template <int RB>
 __device__ __forceinline__ void load_unit(const ExpandedKernelArgs& a, ExpandedCursor& c) {
   const int length = a.key_lengths != nullptr ? uniform_read(a.key_lengths + c.b) : a.keys;
@@ -261,8 +280,7 @@ __device__ __forceinline__ void load_unit(const ExpandedKernelArgs& a, ExpandedC
   c.length = c.bad ? 0 : length;
   c.count = a.tokens;
   if (a.token_counts != nullptr) c.count = min(max(uniform_read(a.token_counts + c.b), 0), a.tokens);
-  c.nb = unit_tiles<RB>(c.length, c.count, c.rb);
-  c.first = c.length - c.count + c.rb * RB + 1;
+  set_unit<RB>(c);
 }
 
 __device__ __forceinline__ long long uniform_long(long long v) {
@@ -283,23 +301,27 @@ __device__ __forceinline__ long long lane_scan(long long v, int lane) {
   return sum;
 }
 
-// This group's first place, of ranges of `each` places; whether it has a tile.  The
-// list goes by row block, sequence, head and tile.
+// The range of a workgroup: consecutive ones go to an XCD, which has every eighth
+// workgroup.
+constexpr int kXcds = 8;
+__device__ __forceinline__ int range_of(int block, int groups) {
+  return block % kXcds * (groups / kXcds) + block / kXcds;
+}
+
+// Range `group`'s first place, of ranges of `each` places; whether it has a tile.  The
+// list goes by sequence, head, row block and tile.
 template <int RB>
 __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const ExpandedStream& st,
                                             int group, int lane, long long& each,
                                             ExpandedCursor& c) {
-  const long long entries = static_cast<long long>(st.row_blocks) * a.batch;
-  auto places = [&](long long e) {
-    const int nb = entry_tiles<RB>(a, st.row_blocks, e);
-    return nb > 0 ? static_cast<long long>(nb + kStart) * a.heads : 0ll;
-  };
-  const long long mine = places(lane);
+  const long long mine = sequence_places<RB>(a, lane) * a.heads;
   const long long sums = lane_scan(mine, lane);
   long long total = uniform_long(__shfl(sums, 63, 64));
-  if (entries > 64) {
+  if (a.batch > 64) {
     long long more = 0;
-    for (long long e0 = 64; e0 < entries; e0 += 64) more += places(e0 + lane);
+    for (long long b0 = 64; b0 < a.batch; b0 += 64) {
+      more += sequence_places<RB>(a, b0 + lane) * a.heads;
+    }
     total += uniform_long(__shfl(lane_scan(more, lane), 63, 64));
   }
   each = uniform_long(max((total + st.groups - 1) / st.groups, 1ll));
@@ -307,31 +329,44 @@ __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const E
   const long long have = min(each, total - g0);
   if (have <= 0) return false;
   long long base = 0;
-  for (long long e0 = 0; e0 < entries; e0 += 64) {
-    const long long n = e0 == 0 ? mine : places(e0 + lane);
-    const long long sum = e0 == 0 ? sums : lane_scan(n, lane);
+  for (long long b0 = 0; b0 < a.batch; b0 += 64) {
+    const long long n = b0 == 0 ? mine : sequence_places<RB>(a, b0 + lane) * a.heads;
+    const long long sum = b0 == 0 ? sums : lane_scan(n, lane);
     const long long from = base + sum - n, to = base + sum;
     const unsigned long long hit = __ballot(from <= g0 && g0 < to);
     if (hit != 0) {
       const int src = __ffsll(static_cast<long long>(hit)) - 1;
-      const long long e = e0 + src;
-      c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(e / a.batch));
-      c.b = __builtin_amdgcn_readfirstlane(static_cast<int>(e - static_cast<long long>(c.rb) * a.batch));
-      load_unit<RB>(a, c);
-      const long long rem = g0 - uniform_long(__shfl(from, src, 64));
-      c.h = __builtin_amdgcn_readfirstlane(static_cast<int>(rem / (c.nb + kStart)));
-      const int in = __builtin_amdgcn_readfirstlane(
-          static_cast<int>(rem - static_cast<long long>(c.h) * (c.nb + kStart)));
-      c.base = uniform_long(g0 - in);
-      c.blk = max(in - kStart, 0);
-      c.to = __builtin_amdgcn_readfirstlane(
-          static_cast<int>(min(static_cast<long long>(c.nb), in + have - kStart)));
-      c.left = __builtin_amdgcn_readfirstlane(
-          static_cast<int>(max(have - (c.nb + kStart - in), 0ll)));
+      c.b = __builtin_amdgcn_readfirstlane(static_cast<int>(b0) + src);
+      base = uniform_long(__shfl(from, src, 64));
       break;
     }
     base += uniform_long(__shfl(sum, 63, 64));
   }
+  c.rb = 0;
+  load_unit<RB>(a, c);
+  const long long head = uniform_long(head_places<RB>(c.length, c.count));
+  c.h = __builtin_amdgcn_readfirstlane(static_cast<int>((g0 - base) / head));
+  base += c.h * head;
+  for (int rb0 = 0;; rb0 += 64) {
+    const int tiles = unit_tiles<RB>(c.length, c.count, rb0 + lane);
+    const long long n = tiles > 0 ? tiles + kStart : 0;
+    const long long sum = lane_scan(n, lane);
+    const unsigned long long hit = __ballot(base + sum - n <= g0 && g0 < base + sum);
+    if (hit != 0 || rb0 >= c.count / RB) {
+      const int src = hit != 0 ? __ffsll(static_cast<long long>(hit)) - 1 : 0;
+      c.rb = __builtin_amdgcn_readfirstlane(rb0 + src);
+      c.base = uniform_long(base + __shfl(sum - n, src, 64));
+      break;
+    }
+    base += uniform_long(__shfl(sum, 63, 64));
+  }
+  load_unit<RB>(a, c);
+  const int in = __builtin_amdgcn_readfirstlane(static_cast<int>(g0 - c.base));
+  c.blk = max(in - kStart, 0);
+  c.to = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(min(static_cast<long long>(c.nb), in + have - kStart)));
+  c.left =
+      __builtin_amdgcn_readfirstlane(static_cast<int>(max(have - (c.nb + kStart - in), 0ll)));
   return c.to > c.blk;
 }
 
@@ -345,16 +380,17 @@ __device__ __forceinline__ bool more_units(const ExpandedCursor& c) { return c.l
 template <int RB>
 __device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, ExpandedCursor& c) {
   c.base += c.nb + kStart;
-  if (++c.h == a.heads) {
-    c.h = 0;
-    do {
-      if (++c.b == a.batch) {
-        c.b = 0;
-        ++c.rb;
-      }
-      load_unit<RB>(a, c);
-    } while (c.nb == 0);
+  if (++c.rb * RB >= c.count) {
+    c.rb = 0;
+    if (++c.h == a.heads) {
+      c.h = 0;
+      do {
+        ++c.b;
+        load_unit<RB>(a, c);
+      } while (c.nb == 0);
+    }
   }
+  set_unit<RB>(c);
   c.blk = 0;
   c.to = min(c.nb, c.left - kStart);
   c.left = max(c.left - c.nb - kStart, 0);
@@ -373,7 +409,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int group = static_cast<int>(blockIdx.x);
+  const int group = range_of(static_cast<int>(blockIdx.x), st.groups);
   auto barrier = [] {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -386,43 +422,54 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   constexpr int kOwn = kValueDim / 8 / kLanes, kShared = static_cast<int>(kLatentRope) / kLanes;
   constexpr int kPieces = 2 * kOwn + 1;
   const int srow = tid / kLanes, part = tid % kLanes;
-  struct Source {  // a tile's rows
+  struct Source {  // a tile: its first rows
     const float* k;
     const float* r;
     const float* v;
-    int first, length;  // its first key, and the sequence's number
-    int seen;           // keys that every row of the unit sees
-    int opens;          // the first tile of its unit in the range
+    int last;   // its last key, or a later one, in the sequence: -1 if that is empty
+    int seen;   // its keys that every row of the unit sees: a later one's number too, or < 0
+    int opens;  // the first tile of its unit in the range
   };
   auto source = [&](const ExpandedCursor& c) {
     Source s{};
+    const std::size_t j = static_cast<std::size_t>(c.blk) * kTile;
+    // (Of an empty sequence nothing is there, and nothing of it is used: a query's
+    // numbers are.)
     s.k = s.r = s.v = a.query + static_cast<std::size_t>(c.b) * a.query_at.batch;
     if (c.length > 0) {
       s.k = a.key + static_cast<std::size_t>(c.b) * a.key_at.batch +
-            static_cast<std::size_t>(c.h) * a.key_at.head;
-      s.r = a.rope_key + static_cast<std::size_t>(c.b) * a.rope_at.batch;
+            static_cast<std::size_t>(c.h) * a.key_at.head + j * a.key_at.token;
+      s.r = a.rope_key + static_cast<std::size_t>(c.b) * a.rope_at.batch + j * a.rope_at.token;
       s.v = a.value + static_cast<std::size_t>(c.b) * a.value_at.batch +
-            static_cast<std::size_t>(c.h) * a.value_at.head;
+            static_cast<std::size_t>(c.h) * a.value_at.head + j * a.value_at.token;
     }
-    s.first = c.blk * kTile;
-    s.length = c.length;
-    s.seen = c.first;
-    s.opens = 0;
+    s.last = c.length - 1 - c.blk * kTile;
+    s.seen = c.first - c.blk * kTile;
+    s.opens = 1;
     return s;
   };
+  // What the registers hold, or are sent for: keys of a tile, and values of the one
+  // before.
+  Source keys = source(cur), values = keys;
+  values.opens = 0;
   v4f raw_k[kOwn + 1][2], raw_v[kOwn][2];  // (a key's last chunk is the shared part's)
-  // Chunk i: a key's, then a value's.  (Of an empty sequence nothing is there, and
-  // nothing of it is used: a query's numbers are.)
-  auto fetch = [&](int i, const Source& sk, const Source& sv) {
-    const Source& s = i <= kOwn ? sk : sv;
-    const std::size_t j = static_cast<std::size_t>(max(min(s.first + srow, s.length - 1), 0));
-    const float* const from = i < kOwn    ? s.k + j * a.key_at.token + i * kLanes * 8 + part * 8
-                              : i == kOwn ? s.r + j * a.rope_at.token + part * kShared
-                                          : s.v + j * a.value_at.token +
-                                                (i - kOwn - 1) * kLanes * 8 + part * 8;
+  // Bytes from a tile's first row, 32 bits: a row's stride is below kMostStride.
+  auto row_offset = [&](int last, std::size_t stride, int numbers) {
+    const unsigned row = static_cast<unsigned>(max(min(srow, last), 0));
+    return (__umul24(row, static_cast<unsigned>(stride / 4)) + static_cast<unsigned>(part * numbers / 4)) *
+           16u;
+  };
+  // Chunk i: a key's, then a value's.
+  auto fetch = [&](int i) {
+    const float* const base = i < kOwn ? keys.k : i == kOwn ? keys.r : values.v;
+    const unsigned offset = i < kOwn    ? row_offset(keys.last, a.key_at.token, 8)
+                            : i == kOwn ? row_offset(keys.last, a.rope_at.token, kShared)
+                                        : row_offset(values.last, a.value_at.token, 8);
+    const auto* const from = reinterpret_cast<const unsigned char*>(base) + offset +
+                             (i < kOwn ? i : i == kOwn ? 0 : i - kOwn - 1) * kLanes * 32;
 #pragma unroll
     for (int w = 0; w < (i == kOwn ? kShared / 4 : 2); ++w) {
-      const v4f x = *reinterpret_cast<const v4f*>(from + 4 * w);
+      const v4f x = *reinterpret_cast<const v4f*>(from + 16 * w);
       if (i <= kOwn) {
         raw_k[i <= kOwn ? i : 0][w] = x;
       } else {
@@ -430,19 +477,18 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       }
     }
   };
-  Source staged_k{}, staged_v{};  // what the registers hold, or are sent for
   // fp16 terms: the powers of two of the keys and values on their way, and the next
   // unit's of the values.
   float key_scale = 1.f, value_scale = 1.f, next_value_scale = 1.f, next_value_unscale = 1.f;
   // Those of the unit that begins with the keys on their way, by the first of its keys
   // that all its rows see.  Each wavefront finds them for itself.
   auto sample = [&](int item) {
-    const Source& s = staged_k;
-    const int have = min(min(s.seen, s.length) - s.first, kSample);
+    const Source& s = keys;
+    const int have = min(min(s.seen, s.last + 1), kSample);
     float top[2] = {0.f, 0.f};
     if (have > 0) {
       const int r = lane / kSample, c = lane % kSample;
-      const std::size_t j = static_cast<std::size_t>(s.first + min(r, have - 1));
+      const std::size_t j = static_cast<std::size_t>(min(r, have - 1));
       const float* const k = s.k + j * a.key_at.token + 4 * c;
       const float* const rope = s.r + j * a.rope_at.token + 4 * c;
       const float* const v = s.v + j * a.value_at.token + 4 * c;
@@ -498,7 +544,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       words[pair][level] = next_bf16_term(sx, sy);
     }
     if (pair != (shared ? kShared / 2 : 4) - 1 || level != kTerms - 1) return;
-    fetch(chunk, staged_k, staged_v);
+    fetch(chunk);
     auto& into = sh.item[buf];
     unsigned char* const to =
         chunk < kOwn    ? into.k[0] + key_place(srow, part + kLanes * chunk)
@@ -522,8 +568,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   auto clean_values = [&](int buf, const Source& s) {
     static_assert(F16 || kLanes == 8, "eight threads a key");
     unsigned poison = 0;
-    if (s.first + kTile > s.seen) {
-      const int j = s.first + srow;
+    if (kTile > s.seen) {
       bool wild = false;
 #pragma unroll
       for (int i = 0; i < kOwn; ++i)
@@ -531,12 +576,12 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int n = 0; n < 4; ++n) wild = wild || !(fabsf(raw_v[i][w][n]) < kWild);
-      const unsigned long long hit = __ballot(wild && j >= s.seen && j < s.length);
+      const unsigned long long hit = __ballot(wild && srow >= s.seen && srow <= s.last);
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         if (((hit >> (8 * r)) & 0xffull) != 0) poison |= 1u << (8 * wave + r);
       }
-      const bool wipe = j >= s.length || ((poison >> (srow & 31)) & 1u) != 0;
+      const bool wipe = srow > s.last || ((poison >> (srow & 31)) & 1u) != 0;
 #pragma unroll
       for (int i = 0; i < kOwn; ++i)
 #pragma unroll
@@ -764,47 +809,43 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   // ---- the range.  Step n: scores of tile n + 1 beside tile n's probabilities, tile
   // n's outputs beside the way of item n + 2 into LDS; behind each chunk's way, that of
   // item n + 3 is sent for.
-  ExpandedCursor ahead = cur;   // the tile whose keys are sent for
-  Source now = source(ahead), before = now;  // its rows, and the last tile's
-  now.opens = 1;
+  ExpandedCursor ahead = cur;  // the tile whose keys are sent for
   // Keys of the next tile and values of the one before.  (Behind the range the last
   // one again, which no one reads.)
   auto advance = [&] {
-    staged_k = now;
-    staged_v = before;
-    before = now;
+    values = keys;
+    keys.opens = 0;
     if (ahead.blk + 1 < ahead.to) {
       ++ahead.blk;
-      now.first += kTile;
-      now.opens = 0;
+      keys.k += kTile * a.key_at.token;
+      keys.r += kTile * a.rope_at.token;
+      keys.v += kTile * a.value_at.token;
+      keys.last -= kTile;
+      keys.seen -= kTile;
     } else if (more_units(ahead)) {
       next_unit<RB>(a, ahead);
-      now = source(ahead);
-      now.opens = 1;
-    } else {
-      now.opens = 0;
+      keys = source(ahead);
     }
   };
   // Before item i's way into LDS, into `buf`: its powers of two, or its values made
   // finite.
   auto ready = [&](int i, int buf) {
     if constexpr (F16) {
-      if (staged_v.opens != 0) {
+      if (values.opens != 0) {
         value_scale = next_value_scale;
         if (lane == 0) sh.value_unscale[wave][i & 3] = next_value_unscale;
       }
-      if (staged_k.opens != 0) sample(i);
+      if (keys.opens != 0) sample(i);
     } else {
-      clean_values(buf, staged_v);
+      clean_values(buf, values);
     }
   };
   // Items 0 and 1.  (Item 0's values, the first tile's, are not read.)
 #pragma unroll
   for (int item = 0; item < 2; ++item) {
     if (item == 0) {
-      advance();
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) fetch(i, staged_k, staged_v);
+      for (int i = 0; i < kPieces; ++i) fetch(i);
     }
     ready(item, item);
     advance();
@@ -954,7 +995,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     void expanded_kernel(ExpandedKernelArgs a, ExpandedStream st) {
   __shared__ ExpandedShared<true> sh;
   constexpr int RB = 16 * WAVES;
-  const int group = static_cast<int>(blockIdx.x);
+  const int group = range_of(static_cast<int>(blockIdx.x), st.groups);
   if (threadIdx.x == 0) st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
   if (threadIdx.x % 64 == 0) st.group_marks[group * WAVES + threadIdx.x / 64] = 0;
   ExpandedCursor cur{};
@@ -981,7 +1022,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
   if (__syncthreads_or(marked) == 0) return;
   ExpandedCursor cur{};
   long long each;
-  if (!first_place<RB>(a, st, static_cast<int>(blockIdx.x), tid & 63, each, cur)) return;
+  if (!first_place<RB>(a, st, range_of(static_cast<int>(blockIdx.x), st.groups), tid & 63, each, cur)) return;
   for (;;) {
     // A unit in several parts is marked if one of them is.
     bool mark = false;
@@ -1126,6 +1167,9 @@ bool expanded_fits(const ExpandedArgs& a) {
   // Ranges, and places in them, are counted in 32 bits: of 2^38 tiles, a group's are
   // 2^30.
   const std::size_t units = a.batch * a.heads * ((a.tokens + 63) / 64);
+  if (a.keys > 1 && std::max({a.key_at.token, a.rope_at.token, a.value_at.token}) >= kMostStride) {
+    return false;
+  }
   return units == 0 || a.keys / kTile + 2 + kStart <= (std::size_t{1} << 38) / units;
 }
 
@@ -1150,6 +1194,7 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   k.heads = static_cast<int>(a.heads);
   k.tokens = static_cast<int>(a.tokens);
   k.keys = static_cast<int>(a.keys);
+  if (a.keys <= 1) k.key_at.token = k.rope_at.token = k.value_at.token = 0;
   k.qscale = kLog2e * a.scale;
   auto* const base = static_cast<unsigned char*>(a.workspace);
   ExpandedStream st{};
@@ -1160,7 +1205,6 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
   st.part_o = reinterpret_cast<float*>(base + layout.part_o);
   st.groups = static_cast<int>(kGroups);
-  st.row_blocks = static_cast<int>(layout.row_blocks);
   return layout.rb == 64 ? launch_expanded<1>(k, st, stream) : launch_expanded<2>(k, st, stream);
 }
 

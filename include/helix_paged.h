@@ -638,9 +638,12 @@ int helix_paged_latent_attention(const float* query, const size_t* query_strides
  *   sequence b has key_lengths[b] (NULL: keys) keys, its token_counts[b] (NULL:
  *   tokens) new tokens' the last: row t sees the first key_lengths[b] -
  *   token_counts[b] + t + 1.
- * All on 16 bytes with strides of four elements.  Rows that see nothing, rows behind
- * token_counts, lengths outside [0, keys], values that are not finite (here also
- * numbers of 3.39e38 and more in size) and the workspace as above. */
+ * All on 16 bytes with strides of four elements; keys of a head less than 2^25 elements
+ * apart (else HELIX_UNSUPPORTED).  Rows that see nothing, rows behind token_counts,
+ * lengths outside [0, keys], values that are not finite (here also numbers of 3.39e38
+ * and more in size) and the workspace as above.  Numbers are taken as two fp16 terms of
+ * a power of two times them; query rows whose numbers do not fit are computed again with
+ * three bf16 terms, which takes about four times as long for them. */
 int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
                                          size_t* out);
 int helix_latent_prefill_attention(const float* query, const size_t* query_strides,

@@ -188,6 +188,14 @@ def test_latent_prefill_refusals(bad, status):
     refused(lib, prefill(lib, **bad), status)
 
 
+def test_latent_prefill_rows_far_apart():
+    """Rows of keys 2^25 numbers apart are refused; a single one has no next."""
+    far = dict(v=2**50, vs=strides(2**26, 2**26, 2**25), batch=1, heads=1, keys=2)
+    refused(hx.load(), prefill(hx.load(), **far), hx.UNSUPPORTED)
+    far = dict(far, vs=strides(2**26, 2**26, 2**25), keys=1, tokens=0)
+    assert prefill(hx.load(), **far) == 0
+
+
 def test_attention_of_nothing_is_no_call():
     lib = hx.load()
     assert latent(lib, batch=0) == 0 and latent(lib, hq=0) == 0 and latent(lib, tokens=0) == 0
