@@ -174,7 +174,7 @@ struct Tile {
   static __device__ __forceinline__ unsigned turn(int row) {
     if constexpr (PF == 0) return static_cast<unsigned>(row & 15);
     if constexpr (kCodes) return static_cast<unsigned>(((row >> 2) & 3) ^ ((row >> 3) & 2));
-    return static_cast<unsigned>((row & 6) | ((row >> 3) & 1));
+    return static_cast<unsigned>(row & 6);
   }
 };
 
@@ -671,7 +671,7 @@ struct TileLoader {
   // first group's by one exchange.
   static constexpr int kPageGroups = P / T::kGroupRows;
   static __device__ __forceinline__ unsigned exchange(int g) {
-    return PF == 0 ? 64u * g : T::kCodes ? 32u * g : kConvert ? 8u * (g & 1) : 16u * (g & 1);
+    return PF == 0 ? 64u * g : T::kCodes ? 32u * g : 0u;
   }
   static __device__ __forceinline__ const unsigned char* group_base(const unsigned char* page,
                                                                     int g) {
