@@ -1111,91 +1111,183 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 
 }
 
 // Joins the partials of the units that cross ranges: the first group's second slot
-// and the later groups' first ones.  blockIdx.x is a unit or a group, blockIdx.y a row
-// (SPLIT: the wavefronts share its partials) or four rows.
+// and the later groups' first ones.  blockIdx.x is a unit or a group.
 constexpr int kMostParts = 512;
-template <bool SPLIT>
-constexpr int merge_waves() {
-  return SPLIT ? 8 : 4;
+struct MergeRow {
+  int row, h, t;
+  bool live;
+};
+__device__ __forceinline__ MergeRow merge_row(const LatentKernelArgs& a, const LatentJob& job,
+                                              int rb_rows, int local) {
+  MergeRow r;
+  r.row = job.rb * rb_rows + local;
+  r.h = r.row / a.tokens;
+  r.t = r.row - r.h * a.tokens;
+  r.live = local < rb_rows && r.row < a.rows && r.t < clamped_count(a, job.b);
+  return r;
 }
-template <int L, bool SPLIT>
-__global__ __launch_bounds__(64 * merge_waves<SPLIT>()) void latent_merge_kernel(LatentKernelArgs a, LatentStream st,
+__device__ __forceinline__ std::size_t merge_slot(const LatentJob& job, int rb_rows, int local, int i) {
+  return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + local;
+}
+__device__ __forceinline__ float* merge_out(const LatentKernelArgs& a, const LatentJob& job,
+                                            const MergeRow& r) {
+  return a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
+         static_cast<std::size_t>(r.h) * a.out_at.head + static_cast<std::size_t>(r.t) * a.out_at.token;
+}
+
+// Units in few parts: a wavefront has one of the four rows of blockIdx.y.  Where a unit
+// has many all the same, the four share each row's.
+constexpr int kFewParts = 16;
+template <int L>
+__global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, LatentStream st,
                                                            int rb_rows) {
   constexpr int NV = L / 256;  // 4 dims each
-  constexpr int NW = merge_waves<SPLIT>();
-  __shared__ v4f sums[SPLIT ? NW : 1][SPLIT ? L / 4 : 1];
-  __shared__ float weights[NW][kMostParts];
+  constexpr int U = 4;         // partials on their way
+  __shared__ float weights[4][kMostParts];
+  __shared__ v4f sums[4][L / 4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   if (st.by_unit != 0 && clamped_count(a, static_cast<int>(blockIdx.x) % a.batch) == 0) return;
   const LatentJob job = st.jobs[blockIdx.x];
   if (job.b < 0) return;
-  const int local = SPLIT ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * 4 + wave;
-  const int row = job.rb * rb_rows + local;
-  const int h = row / a.tokens, t = row - h * a.tokens;
-  const bool live = local < rb_rows && row < a.rows && t < clamped_count(a, job.b);
+  const int local0 = static_cast<int>(blockIdx.y) * 4, local = local0 + wave;
+  const MergeRow r = merge_row(a, job, rb_rows, local);
   const int parts = min(job.last - job.first + 1, kMostParts);
-  auto slot = [&](int i) {
-    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + local;
-  };
   float top = -INFINITY, sum = 0.f;
-  v4f o[NV];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) o[v] = v4f{0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, st.part_ml[2 * slot(i)]);
+  if (r.live) {
+    for (int i = lane; i < parts; i += 64) {
+      top = fmaxf(top, st.part_ml[2 * merge_slot(job, rb_rows, local, i)]);
+    }
 #pragma unroll
     for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
     for (int i = lane; i < parts; i += 64) {
-      const float pl = st.part_ml[2 * slot(i) + 1];
-      const float w = pl == 0.f ? 0.f : exp2_ratio(st.part_ml[2 * slot(i)], top);
-      sum += pl * w;
+      const float* const ml = st.part_ml + 2 * merge_slot(job, rb_rows, local, i);
+      const float w = ml[1] == 0.f ? 0.f : exp2_ratio(ml[0], top);
+      sum += ml[1] * w;
       weights[wave][i] = w;
     }
 #pragma unroll
     for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
-    constexpr int U = SPLIT ? 8 : 4;  // partials on their way
-    constexpr int step = SPLIT ? NW : 1;
-    for (int i0 = SPLIT ? wave : 0; i0 < parts; i0 += U * step) {
+  }
+  // Of row local0 + w its partials first, first + step, ..
+  auto gather = [&](int w, int first, int step, v4f (&o)[NV]) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) o[v] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = first; i0 < parts; i0 += U * step) {
       v4f x[U][NV];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = min(i0 + u * step, parts - 1);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          x[u][v] = reinterpret_cast<const v4f*>(st.part_o + slot(i) * L)[64 * v + lane];
+          x[u][v] = reinterpret_cast<const v4f*>(
+              st.part_o + merge_slot(job, rb_rows, local0 + w, i) * L)[64 * v + lane];
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * step;
-        const float w = i < parts ? weights[wave][min(i, parts - 1)] : 0.f;
-        if (w != 0.f) {  // (a part that saw nothing has no outputs to speak of)
+        const float f = i < parts ? weights[w][min(i, parts - 1)] : 0.f;
+        if (f != 0.f) {  // (a part that saw nothing has no outputs to speak of)
 #pragma unroll
-          for (int v = 0; v < NV; ++v) o[v] += x[u][v] * w;
+          for (int v = 0; v < NV; ++v) o[v] += x[u][v] * f;
         }
       }
     }
-  }
-  if constexpr (SPLIT) {
+  };
+  v4f o[NV];
+  if (parts <= kFewParts) {
+    if (r.live) gather(wave, 0, 1, o);
+  } else {
+    for (int w = 0; w < 4; ++w) {
+      __syncthreads();
+      if (!merge_row(a, job, rb_rows, local0 + w).live) continue;
+      v4f own[NV];
+      gather(w, wave, 4, own);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) sums[wave][64 * v + lane] = o[v];
-    __syncthreads();
-    if (wave != 0) return;
+      for (int v = 0; v < NV; ++v) sums[wave][64 * v + lane] = own[v];
+      __syncthreads();
+      if (wave != w) continue;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      o[v] = sums[0][64 * v + lane];
+      for (int v = 0; v < NV; ++v) {
+        o[v] = sums[0][64 * v + lane];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) o[v] += sums[w][64 * v + lane];
+        for (int k = 1; k < 4; ++k) o[v] += sums[k][64 * v + lane];
+      }
     }
   }
-  if (!live) return;
+  if (!r.live) return;
   const float f = sum == 0.f ? 0.f : 1.0f / sum;
-  auto* const dst = reinterpret_cast<v4f*>(
-      a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
-      static_cast<std::size_t>(h) * a.out_at.head + static_cast<std::size_t>(t) * a.out_at.token);
+  auto* const dst = reinterpret_cast<v4f*>(merge_out(a, job, r));
 #pragma unroll
   for (int v = 0; v < NV; ++v) dst[64 * v + lane] = o[v] * f;
+}
+
+// Few units in many parts: a workgroup has 128 dims (blockIdx.z) of a row (blockIdx.y),
+// each half of its eight wavefronts every 16th partial.
+constexpr int kSplitDims = 128;
+template <int L>
+__global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArgs a, LatentStream st,
+                                                                 int rb_rows) {
+  constexpr int kShares = 16, U = 8;
+  __shared__ float weights[kMostParts];
+  __shared__ float lead[8], total[8];
+  __shared__ v4f sums[kShares][kSplitDims / 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (st.by_unit != 0 && clamped_count(a, static_cast<int>(blockIdx.x) % a.batch) == 0) return;
+  const LatentJob job = st.jobs[blockIdx.x];
+  if (job.b < 0) return;
+  const int local = static_cast<int>(blockIdx.y);
+  const MergeRow r = merge_row(a, job, rb_rows, local);
+  if (!r.live) return;
+  const int parts = min(job.last - job.first + 1, kMostParts);
+  // A thread has a partial's maximum and sum.
+  float pm = -INFINITY, pl = 0.f;
+  if (tid < parts) {
+    const float* const ml = st.part_ml + 2 * merge_slot(job, rb_rows, local, tid);
+    pm = ml[0];
+    pl = ml[1];
+  }
+  float top = pm;
+#pragma unroll
+  for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
+  if (lane == 0) lead[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, lead[w]);
+  const float own = pl == 0.f ? 0.f : exp2_ratio(pm, top);
+  weights[tid] = own;
+  float sum = pl * own;
+#pragma unroll
+  for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
+  if (lane == 0) total[wave] = sum;
+  __syncthreads();
+  const int share = tid / (kSplitDims / 4), at = tid % (kSplitDims / 4);
+  const int dim = static_cast<int>(blockIdx.z) * kSplitDims + 4 * at;
+  v4f o = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = share; i0 < parts; i0 += U * kShares) {
+    v4f x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = *reinterpret_cast<const v4f*>(
+          st.part_o + merge_slot(job, rb_rows, local, min(i0 + u * kShares, parts - 1)) * L + dim);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kShares;
+      const float f = i < parts ? weights[i] : 0.f;
+      if (f != 0.f) o += x[u] * f;
+    }
+  }
+  sums[share][at] = o;
+  __syncthreads();
+  if (share != 0) return;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) sum += total[w];
+#pragma unroll
+  for (int k = 1; k < kShares; ++k) o += sums[k][at];
+  *reinterpret_cast<v4f*>(merge_out(a, job, r) + dim) = o * (sum == 0.f ? 0.f : 1.0f / sum);
 }
 
 // ----------------------------------------------------------------- host ----
@@ -1236,12 +1328,11 @@ hipError_t launch_latent(const LatentKernelArgs& k, const LatentStream& st, std:
   const std::size_t jobs =
       st.by_unit != 0 ? static_cast<std::size_t>(k.batch) * st.row_blocks : kGroups;
   const unsigned rows = static_cast<unsigned>(std::min<std::size_t>(rb, static_cast<std::size_t>(k.rows)));
-  // Few units: all wavefronts of a workgroup on one row.
-  if (jobs * rows <= 2048) {
-    latent_merge_kernel<L, true>
-        <<<dim3(static_cast<unsigned>(jobs), rows), 64 * merge_waves<true>(), 0, stream>>>(k, st, static_cast<int>(rb));
+  if (jobs * kFewParts <= kGroups) {
+    latent_split_merge_kernel<L>
+        <<<dim3(static_cast<unsigned>(jobs), rows, L / kSplitDims), 512, 0, stream>>>(k, st, static_cast<int>(rb));
   } else {
-    latent_merge_kernel<L, false><<<dim3(static_cast<unsigned>(jobs), (rows + 3) / 4), 256, 0, stream>>>(
+    latent_merge_kernel<L><<<dim3(static_cast<unsigned>(jobs), (rows + 3) / 4), 256, 0, stream>>>(
         k, st, static_cast<int>(rb));
   }
   return hipGetLastError();
