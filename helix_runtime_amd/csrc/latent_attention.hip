@@ -106,24 +106,20 @@ struct LatentStream {
   int by_unit;
 };
 
-// x = t[0] + t[1] (+ t[2]), each rounded to nearest; two numbers at a time, packed
-// into words.
+// The next term of x and y, rounded to nearest and packed into a word; x and y become
+// what it leaves.
 template <int PF>
-__device__ __forceinline__ void split_pair(float x, float y, unsigned (&t)[3]) {
+__device__ __forceinline__ unsigned next_term(float& x, float& y) {
   if constexpr (PF == 2) {
-    const v2h hi = __builtin_convertvector((v2f{x, y}), v2h);
-    x -= static_cast<float>(hi[0]);
-    y -= static_cast<float>(hi[1]);
-    t[0] = __builtin_bit_cast(unsigned, hi);
-    t[1] = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2h));
+    const v2h h = __builtin_convertvector((v2f{x, y}), v2h);
+    x -= static_cast<float>(h[0]);
+    y -= static_cast<float>(h[1]);
+    return __builtin_bit_cast(unsigned, h);
   } else {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const v2bf h = __builtin_convertvector((v2f{x, y}), v2bf);
-      t[i] = __builtin_bit_cast(unsigned, h);
-      x -= __uint_as_float(t[i] << 16);
-      y -= __uint_as_float(t[i] & 0xffff0000u);
-    }
+    const unsigned t = __builtin_bit_cast(unsigned, __builtin_convertvector((v2f{x, y}), v2bf));
+    x -= __uint_as_float(t << 16);
+    y -= __uint_as_float(t & 0xffff0000u);
+    return t;
   }
 }
 
@@ -383,7 +379,9 @@ struct LatentRows {
         unsigned w[4][3];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          split_pair<PF>(x[s][i >> 1][2 * (i & 1)] * grow, x[s][i >> 1][2 * (i & 1) + 1] * grow, w[i]);
+          float y0 = x[s][i >> 1][2 * (i & 1)] * grow, y1 = x[s][i >> 1][2 * (i & 1) + 1] * grow;
+#pragma unroll
+          for (int n = 0; n < QT; ++n) w[i][n] = next_term<PF>(y0, y1);
         }
 #pragma unroll
         for (int i = 0; i < QT; ++i) q[s][i] = v4u{w[0][i], w[1][i], w[2][i], w[3][i]};
@@ -402,8 +400,11 @@ struct LatentRows {
     for (int i = 0; i < QT; ++i) asm("" : "+a"(q[s][i]));
   }
 
-  // Scores of a tile: sc[h][i] is token 16 h + 4 grp + i of row col.  `beside(u)` is
-  // what else the lane does between the matrix instructions of step u of NS.
+  // Scores of a tile: sc[h][i] is token 16 h + 4 grp + i of row col.  `beside(i)` is
+  // what else the lane does behind the i-th of kSlots products of terms: a matrix
+  // instruction takes 16 cycles, of which its issue takes 4, and only what is issued
+  // between two of them goes beside the first.
+  static constexpr int kSlots = NS * QT;
   template <typename F>
   __device__ __forceinline__ void scores(const unsigned char* tile, int col, int grp, v4f (&sc)[NH],
                                          F&& beside) const {
@@ -455,6 +456,7 @@ struct LatentRows {
         for (int i = 0; i < 4; ++i) {
           sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[0], 0, 0, 0);
         }
+        beside(s);
       } else {
         v4u k[NH];
 #pragma unroll
@@ -467,13 +469,15 @@ struct LatentRows {
         }
         // Smallest products first.
 #pragma unroll
-        for (int i = QT - 1; i >= 0; --i)
+        for (int i = QT - 1; i >= 0; --i) {
 #pragma unroll
           for (int h = 0; h < NH; ++h) sc[h] = matrix_step<PF>(k[h], q[s][i], sc[h]);
+          beside(QT * s + QT - 1 - i);
+          if (SHARED) __builtin_amdgcn_sched_barrier(0);
+        }
       }
       if (s + 1 < NS) widen(s + 1);
       if (s + A < NS) read(s + A);
-      beside(s);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -503,34 +507,37 @@ struct LatentRows {
     return (m == -INFINITY ? 0.f : m) - (PF == 2 ? kProbLog : 0.f);
   }
 
-  // Probabilities of the scores sc[i / 4][i % 4], i = 2 n, 2 n + 1, as operands.
+  // Probabilities of the scores as operands, in small parts: of two tokens their
+  // exponentials, then a term each.
   static constexpr int kPairs = 2 * NH;
+  static constexpr int kPartsOfPair = PF == 0 ? 1 : 1 + QT;
+  static constexpr int kProbParts = kPairs * kPartsOfPair;
   struct Probabilities {
     unsigned w[kPairs][3];
     float f[PF == 0 ? 4 : 1];
+    float y[2];  // what the terms so far leave
   };
-  __device__ __forceinline__ void probability(int n, const v4f (&sc)[NH], float ref,
+  __device__ __forceinline__ void probability(int part, const v4f (&sc)[NH], float ref,
                                               Probabilities& p) {
-    const v4f x = sc[n / 2];
-    float y[2];
+    const int n = part / kPartsOfPair, level = part % kPartsOfPair;
+    if (level == 0) {
+      const v4f x = sc[n / 2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float s = x[2 * (n % 2) + i];
-      if constexpr (PF == 2) {
-        y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, unscale, -ref));
-      } else {
-        y[i] = __builtin_amdgcn_exp2f(s - ref);
+      for (int i = 0; i < 2; ++i) {
+        const float s = x[2 * (n % 2) + i];
+        if constexpr (PF == 2) {
+          p.y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, unscale, -ref));
+        } else {
+          p.y[i] = __builtin_amdgcn_exp2f(s - ref);
+        }
+        if constexpr (PF == 0) p.f[2 * n + i] = p.y[i];
       }
-    }
-    l += y[0] + y[1];
-    if constexpr (PF == 0) {
-      p.f[2 * n] = y[0];
-      p.f[2 * n + 1] = y[1];
+      if constexpr (PF == 0) l += p.y[0] + p.y[1];
     } else {
-      split_pair<PF>(y[0], y[1], p.w[n]);
+      if (level == 1) l += p.y[0] + p.y[1];
+      p.w[n][level - 1] = next_term<PF>(p.y[0], p.y[1]);
     }
   }
-
   // Outputs of the tile.
   __device__ __forceinline__ void add_values(const unsigned char* tile, int col, int grp,
                                              const Probabilities& p) {
@@ -679,11 +686,11 @@ struct TileLoader {
   }
   // Straight into LDS.
   __device__ __forceinline__ void direct(const unsigned char* page, int g, unsigned lds) const {
-    const unsigned char* const base = group_base(page, g);
 #pragma unroll
-    for (int i = 0; i < T::kLoads; ++i) {
-      lds_load16_at(base, off[i] ^ exchange(g), lds + (g * T::kLoads + i) * 1024u);
-    }
+    for (int i = 0; i < T::kLoads; ++i) direct(page, g, lds, i);
+  }
+  __device__ __forceinline__ void direct(const unsigned char* page, int g, unsigned lds, int i) const {
+    lds_load16_at(group_base(page, g), off[i] ^ exchange(g), lds + (g * T::kLoads + i) * 1024u);
   }
   // Codes into registers, and from there as fp16 into LDS.
   __device__ __forceinline__ void fetch(const unsigned char* page, int g, v2u (&raw)[T::kLoads]) const {
@@ -884,16 +891,24 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
     int into = 0;
     auto bump = [&](int& i) { i = i + 1 == NB ? 0 : i + 1; };
     // The wavefront's quarter of the next tile is sent for (fp8: the one that was
-    // goes to LDS first).
-    auto send = [&] {
+    // goes to LDS first), a load at a time.
+    auto send = [&](int i) {
       if constexpr (PF == 2) {
+        if (i != 0) return;
         Loader::store(sh.tile[into], wave, lane, raw);
         loader.fetch(page_of(next, wave), wave, raw);
       } else {
-        loader.direct(page_of(next, wave), wave, lds0 + static_cast<unsigned>(into) * T::kBytes);
+        loader.direct(page_of(next, wave), wave, lds0 + static_cast<unsigned>(into) * T::kBytes, i);
       }
+    };
+    auto sent = [&] {
       bump(into);
       locate_next();
+    };
+    auto send_all = [&] {
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) send(i);
+      sent();
     };
     // What was sent for before the last two times is there.
     auto arrived = [&] {
@@ -903,9 +918,9 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       loader.fetch(page_of(next, wave), wave, raw);
       locate_next();
     }
-    send();
-    send();
-    if constexpr (PF != 2) send();
+    send_all();
+    send_all();
+    if constexpr (PF != 2) send_all();
     arrived();
     barrier();
     int n = 0, buf = 0;  // tile, and its buffer
@@ -919,7 +934,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       v4f sc[NH];
       rows.scores(sh.tile[buf], col, grp, sc, [](int) {});
       for (int blk = from; blk < to; ++blk) {
-        send();
+        if constexpr (PF == 2) send(0);
         bad |= static_cast<int>(bads >> (n & 31)) & 1;
         typename R::Probabilities p;
         int after = buf;
@@ -942,20 +957,26 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
           v4f now[NH];
 #pragma unroll
           for (int h = 0; h < NH; ++h) now[h] = sc[h];
-          constexpr int kEvery = R::NS / (R::kPairs + 1);
+          constexpr int kApart = (R::kSlots - R::kProbParts) / T::kLoads;
+          static_assert(kApart > 0, "a slot a part");
           // (A copy that the compiler does not know, or it takes the exponentials of
           // both cases out in front.)
           float ref_here = ref;
           asm("" : "+v"(ref_here));
-          rows.scores(sh.tile[after], col, grp, sc, [&](int u) {
-            if (u % kEvery == kEvery - 1 && u / kEvery < R::kPairs) {
-              rows.probability(u / kEvery, now, ref_here, p);
-            }
+          rows.scores(sh.tile[after], col, grp, sc, [&](int i) {
+            if (i < R::kProbParts) rows.probability(i, now, ref_here, p);
+            const int j = i - R::kProbParts;
+            if (PF != 2 && j >= 0 && j % kApart == 0 && j / kApart < T::kLoads) send(j / kApart);
           });
         } else {
 #pragma unroll
-          for (int i = 0; i < R::kPairs; ++i) rows.probability(i, sc, ref, p);
+          for (int i = 0; i < R::kProbParts; ++i) rows.probability(i, sc, ref, p);
+          if constexpr (PF != 2) {
+#pragma unroll
+            for (int i = 0; i < T::kLoads; ++i) send(i);
+          }
         }
+        sent();
         rows.add_values(sh.tile[buf], col, grp, p);
         buf = after;
         ++n;
@@ -1028,7 +1049,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
         const float ref = rows.reference();
         typename R::Probabilities p;
 #pragma unroll
-        for (int j = 0; j < R::kPairs; ++j) rows.probability(j, sc, ref, p);
+        for (int j = 0; j < R::kProbParts; ++j) rows.probability(j, sc, ref, p);
         rows.add_values(tile, col, grp, p);
         // (The tile's reads are done before it is written again.)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
