@@ -401,14 +401,16 @@ struct LatentRows {
   }
 
   // Scores of a tile: sc[h][i] is token 16 h + 4 grp + i of row col.  `beside(i)` is
-  // what else the lane does behind the i-th of kSlots products of terms: a matrix
-  // instruction takes 16 cycles, of which its issue takes 4, and only what is issued
+  // what else the lane does behind the i-th of kSlots matrix instructions: one
+  //  takes 16 cycles, of which its issue takes 4, and only what is issued
   // between two of them goes beside the first.
-  static constexpr int kSlots = NS * QT;
+  static constexpr int kSlots = NS * (PF == 0 ? 1 : QT * NH);
+  static constexpr bool kSpread = SHARED && PF != 0;  // a matrix instruction at a time
   template <typename F>
   __device__ __forceinline__ void scores(const unsigned char* tile, int col, int grp, v4f (&sc)[NH],
                                          F&& beside) const {
     constexpr int A = PF == 0 || T::kCodes ? 4 : 2;  // operands come out of LDS A steps ahead
+    constexpr int AR = kSpread ? A + 1 : A;          // (kSpread: while the step's are in use)
     // Row col's chunk 4 s + grp (codes: half of chunk 2 s + grp / 2): its place within
     // a group of chunks is one of two (fp32 pages: four), by s.
     constexpr int V = PF == 0 ? 4 : 2;
@@ -425,12 +427,13 @@ struct LatentRows {
                    (T::kCodes ? (grp % 2) * 8u : 0u);
       }
     using Operand = std::conditional_t<T::kCodes, v2u, v4u>;
-    Operand raw[A][NH];
+    Operand raw[AR][NH];
+    auto read_half = [&](int s, int h) {
+      raw[s % AR][h] = *reinterpret_cast<const Operand*>(tile + at[s % V][h] + (s / V) * (V * C * 16));
+    };
     auto read = [&](int s) {
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        raw[s % A][h] = *reinterpret_cast<const Operand*>(tile + at[s % V][h] + (s / V) * (V * C * 16));
-      }
+      for (int h = 0; h < NH; ++h) read_half(s, h);
     };
 #pragma unroll
     for (int s = 0; s < A; ++s) read(s);
@@ -442,7 +445,7 @@ struct LatentRows {
       if constexpr (T::kCodes) {
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
-          wide[s % 2][h] = codes_fp16(raw[s % A][h][0], raw[s % A][h][1]);
+          wide[s % 2][h] = codes_fp16(raw[s % AR][h][0], raw[s % AR][h][1]);
         }
       }
     };
@@ -451,7 +454,7 @@ struct LatentRows {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       if constexpr (PF == 0) {
-        const v4f x = __builtin_bit_cast(v4f, raw[s % A][0]), y = __builtin_bit_cast(v4f, q[s][0]);
+        const v4f x = __builtin_bit_cast(v4f, raw[s % AR][0]), y = __builtin_bit_cast(v4f, q[s][0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[0], 0, 0, 0);
@@ -464,20 +467,24 @@ struct LatentRows {
           if constexpr (T::kCodes) {
             k[h] = wide[s % 2][h];
           } else {
-            k[h] = raw[s % A][h];
+            k[h] = raw[s % AR][h];
           }
         }
         // Smallest products first.
 #pragma unroll
         for (int i = QT - 1; i >= 0; --i) {
 #pragma unroll
-          for (int h = 0; h < NH; ++h) sc[h] = matrix_step<PF>(k[h], q[s][i], sc[h]);
-          beside(QT * s + QT - 1 - i);
-          if (SHARED) __builtin_amdgcn_sched_barrier(0);
+          for (int h = 0; h < NH; ++h) {
+            sc[h] = matrix_step<PF>(k[h], q[s][i], sc[h]);
+            const int at_step = NH * (QT - 1 - i) + h;
+            if (kSpread && at_step % 2 == 1 && at_step / 2 < NH && s + A < NS) read_half(s + A, at_step / 2);
+            if (kSpread || h == NH - 1) beside(NH * QT * s + at_step);
+            if (kSpread) __builtin_amdgcn_sched_barrier(0);
+          }
         }
       }
       if (s + 1 < NS) widen(s + 1);
-      if (s + A < NS) read(s + A);
+      if (!kSpread && s + A < NS) read(s + A);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -507,10 +514,10 @@ struct LatentRows {
     return (m == -INFINITY ? 0.f : m) - (PF == 2 ? kProbLog : 0.f);
   }
 
-  // Probabilities of the scores as operands, in small parts: of two tokens their
-  // exponentials, then a term each.
+  // Probabilities of the scores as operands, in small parts: of two tokens an
+  // exponential each, then a term of both each.
   static constexpr int kPairs = 2 * NH;
-  static constexpr int kPartsOfPair = PF == 0 ? 1 : 1 + QT;
+  static constexpr int kPartsOfPair = PF == 0 ? 1 : 2 + QT;
   static constexpr int kProbParts = kPairs * kPartsOfPair;
   struct Probabilities {
     unsigned w[kPairs][3];
@@ -520,10 +527,10 @@ struct LatentRows {
   __device__ __forceinline__ void probability(int part, const v4f (&sc)[NH], float ref,
                                               Probabilities& p) {
     const int n = part / kPartsOfPair, level = part % kPartsOfPair;
-    if (level == 0) {
+    if (PF == 0 || level < 2) {
       const v4f x = sc[n / 2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = PF == 0 ? 0 : level; i < (PF == 0 ? 2 : level + 1); ++i) {
         const float s = x[2 * (n % 2) + i];
         if constexpr (PF == 2) {
           p.y[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, unscale, -ref));
@@ -534,8 +541,8 @@ struct LatentRows {
       }
       if constexpr (PF == 0) l += p.y[0] + p.y[1];
     } else {
-      if (level == 1) l += p.y[0] + p.y[1];
-      p.w[n][level - 1] = next_term<PF>(p.y[0], p.y[1]);
+      if (level == 2) l += p.y[0] + p.y[1];
+      p.w[n][level - 2] = next_term<PF>(p.y[0], p.y[1]);
     }
   }
   // Outputs of the tile.
@@ -576,6 +583,7 @@ struct LatentRows {
     } else {
       using LdsV4s = __attribute__((address_space(3))) v4s;
       constexpr int A = T::kCodes ? 6 : 4;
+      constexpr int AR = kSpread ? A + 2 : A;
       v4u pop[QT];
 #pragma unroll
       for (int i = 0; i < QT; ++i) pop[i] = v4u{p.w[0][i], p.w[1][i], p.w[2][i], p.w[3][i]};
@@ -592,17 +600,22 @@ struct LatentRows {
                 ((static_cast<unsigned>(chunk) ^ T::turn(row)) & T::kMask) * 16u + (col & 1) * 8u;
       }
       using Operand = std::conditional_t<T::kCodes, v2i, v4u>;
-      Operand raw[A];
-      auto read = [&](int dt) {
+      Operand raw[AR];
+      // Tokens 4 grp and on, then (part 1) those 16 behind them.
+      auto read_part = [&](int dt, int part) {
         const unsigned char* const from = tile + at[dt % V] + (dt / V) * (T::kCodes ? 64 : 128);
         if constexpr (T::kCodes) {
-          raw[dt % A] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsV2i*)(from));
+          if (part == 0) raw[dt % AR] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LdsV2i*)(from));
         } else {
-          const v4s v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from));
-          const v4s v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from + 16 * T::kPitch));
-          raw[dt % A] =
-              __builtin_bit_cast(v4u, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+          const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsV4s*)(from + part * 16 * T::kPitch));
+          const v2u y = __builtin_bit_cast(v2u, x);
+          raw[dt % AR][2 * part] = y[0];
+          raw[dt % AR][2 * part + 1] = y[1];
         }
+      };
+      auto read = [&](int dt) {
+        read_part(dt, 0);
+        read_part(dt, 1);
       };
 #pragma unroll
       for (int dt = 0; dt < A; ++dt) read(dt);
@@ -611,8 +624,8 @@ struct LatentRows {
         if constexpr (T::kCodes) {
 #pragma unroll
           for (int d = dt; d < dt + 2; ++d) {
-            wide[d % 4] = codes_fp16(static_cast<unsigned>(raw[d % A][0]),
-                                     static_cast<unsigned>(raw[d % A][1]));
+            wide[d % 4] = codes_fp16(static_cast<unsigned>(raw[d % AR][0]),
+                                     static_cast<unsigned>(raw[d % AR][1]));
           }
         }
       };
@@ -626,15 +639,20 @@ struct LatentRows {
           if constexpr (T::kCodes) {
             v[d] = wide[(dt + d) % 4];
           } else {
-            v[d] = raw[(dt + d) % A];
+            v[d] = raw[(dt + d) % AR];
           }
         }
 #pragma unroll
         for (int i = QT - 1; i >= 0; --i)
 #pragma unroll
-          for (int d = 0; d < 2; ++d) o[dt + d] = matrix_step<PF>(v[d], pop[i], o[dt + d]);
+          for (int d = 0; d < 2; ++d) {
+            o[dt + d] = matrix_step<PF>(v[d], pop[i], o[dt + d]);
+            const int at_step = 2 * (QT - 1 - i) + d;
+            if (kSpread && at_step < 4 && dt + A < ND) read_part(dt + A + at_step / 2, at_step % 2);
+            if (kSpread) __builtin_amdgcn_sched_barrier(0);
+          }
         if (dt + 2 < ND) widen(dt + 2);
-        if (dt + A < ND) {
+        if (!kSpread && dt + A < ND) {
           read(dt + A);
           read(dt + A + 1);
         }
