@@ -180,7 +180,7 @@ struct Tile {
 // pages: the slowest workgroup takes 52 us where starts count nothing, most take 30.)
 template <bool SHARED>
 constexpr int start_cost() {
-  return SHARED ? 2 : 16;
+  return SHARED ? 4 : 24;
 }
 
 // A place in the flat list, in which each unit has start_cost() places before its
