@@ -439,6 +439,7 @@ struct LatentRows {
     for (int s = 0; s < A; ++s) read(s);
 #pragma unroll
     for (int h = 0; h < NH; ++h) sc[h] = v4f{0.f, 0.f, 0.f, 0.f};
+    [[maybe_unused]] v4f step_sum[2];
     // Codes become fp16 a step ahead, between the matrix instructions of the step.
     v4u wide[2][NH];
     auto widen = [&](int s) {
@@ -455,10 +456,16 @@ struct LatentRows {
     for (int s = 0; s < NS; ++s) {
       if constexpr (PF == 0) {
         const v4f x = __builtin_bit_cast(v4f, raw[s % AR][0]), y = __builtin_bit_cast(v4f, q[s][0]);
+        // A step's sum by itself, and the last one's to the others': one sum of 576
+        // products would be off by three times as much.
+        v4f& sum = step_sum[s % 2];
+        sum = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sc[0], 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], sum, 0, 0, 0);
         }
+        if (s > 0) sc[0] += step_sum[(s + 1) % 2];
+        if (s + 1 == NS) sc[0] += sum;
         beside(s);
       } else {
         v4u k[NH];
