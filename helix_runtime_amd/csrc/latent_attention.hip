@@ -439,7 +439,9 @@ struct LatentRows {
     for (int s = 0; s < A; ++s) read(s);
 #pragma unroll
     for (int h = 0; h < NH; ++h) sc[h] = v4f{0.f, 0.f, 0.f, 0.f};
-    [[maybe_unused]] v4f step_sum[2];
+    [[maybe_unused]] v4f step_sum[2], low[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) low[h] = v4f{0.f, 0.f, 0.f, 0.f};
     // Codes become fp16 a step ahead, between the matrix instructions of the step.
     v4u wide[2][NH];
     auto widen = [&](int s) {
@@ -482,7 +484,10 @@ struct LatentRows {
         for (int i = QT - 1; i >= 0; --i) {
 #pragma unroll
           for (int h = 0; h < NH; ++h) {
-            sc[h] = matrix_step<PF>(k[h], q[s][i], sc[h]);
+            // (Sums of the smaller terms' products by themselves: the rounding of the
+            // larger ones' is then that of a third, or half, as many.)
+            v4f& sum = i == 0 ? sc[h] : low[h];
+            sum = matrix_step<PF>(k[h], q[s][i], sum);
             const int at_step = NH * (QT - 1 - i) + h;
             if (kSpread && at_step % 2 == 1 && at_step / 2 < NH && s + A < NS) read_half(s + A, at_step / 2);
             if (kSpread || h == NH - 1) beside(NH * QT * s + at_step);
@@ -493,6 +498,10 @@ struct LatentRows {
       if (s + 1 < NS) widen(s + 1);
       if (!kSpread && s + A < NS) read(s + A);
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (PF != 0) {
+#pragma unroll
+      for (int h = 0; h < NH; ++h) sc[h] += low[h];
     }
   }
 
