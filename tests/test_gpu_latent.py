@@ -241,6 +241,29 @@ def test_absorbed_calls_are_equal_bit_by_bit(device):
         assert (p.run() == first).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,t", [(16, 1), (40, 2)])
+@pytest.mark.parametrize("sign", [-1, 0])
+def test_absorbed_other_scales(device, dtype, hq, t, sign):
+    """A negative scale turns the scores about; with none every token counts alike."""
+    p = Latent(dtype, 512, [100, 0, 33], hq, t)
+    got = p.run(scale=sign * SCALE)
+    p.q = p.q * np.float32(sign)
+    close(got, p.want())
+
+
+@pytest.mark.parametrize("dtype,hq,t", [("f32", 16, 1), ("fp8", 8, 2), ("bf16", 40, 2)])
+def test_absorbed_many_sequences(device, dtype, hq, t):
+    """More units than workgroups, empty ones and one of many parts among them."""
+    rng = np.random.default_rng(5)
+    lengths = [int(x) for x in rng.integers(0, 40, 300)]
+    lengths[7], lengths[150], lengths[299] = 30000, 0, 700
+    counts = [int(x) for x in rng.integers(-1, t + 2, 300)]
+    counts[7] = t
+    p = Latent(dtype, 256, lengths, hq, t, counts=counts)
+    close(p.run(), p.want())
+
+
 def test_absorbed_pools_past_32_bits(device):
     """Pages whose elements lie past 2^32 of the pool."""
     n = (1 << 32) // (P * 576) + 40
@@ -455,6 +478,60 @@ def test_expanded_strides(device):
                 value=kv.transpose(1, 2)[..., 128:], rope_key=down[..., 512:],
                 output=out.transpose(1, 2))
     close(got, p.want())
+
+
+@pytest.mark.parametrize("t,s", [(50, 90), (130, 200)])
+@pytest.mark.parametrize("sign", [-1, 0])
+def test_expanded_other_scales(device, t, s, sign):
+    p = Expanded(1, 2, t, s)
+    got = p.run(scale=sign * SCALE)
+    p.q = p.q * np.float32(sign)
+    close(got, p.want())
+
+
+@pytest.mark.parametrize("b,h,t,s", [(20, 20, 50, 300), (6, 50, 130, 400), (70, 3, 20, 60)])
+def test_expanded_many_units(device, b, h, t, s):
+    """More units than workgroups, or more sequences than a wavefront has lanes; some
+    without rows or keys."""
+    rng = np.random.default_rng(b)
+    p = Expanded(b, h, t, s, counts=[int(x) for x in rng.integers(-1, t + 2, b)],
+                 lengths=[int(x) for x in rng.integers(0, s + 1, b)])
+    close(p.run(), p.want())
+
+
+@pytest.mark.parametrize("t", [20, 100])
+def test_expanded_rows_far_apart(device, t):
+    """Keys' rows as far apart as they may be, and sequences past 2^32 bytes."""
+    b, h, s, far = 2, 1, 40, (1 << 25) - 4
+    p = Expanded(b, h, t, s)
+    d = p.arguments()
+    room = torch.zeros(s * far, device="cuda:0")
+    value = room.as_strided((b, h, s, 128), (256, 256, far, 1))
+    value.copy_(d["value"])
+    key = room.as_strided((b, h, s, 128), ((1 << 30) + 64, 128, 512, 1), 1024)
+    key.copy_(d["key"])
+    close(p.run(value=value, key=key), p.want())
+
+
+def test_calls_on_streams_at_once(device):
+    """Calls of both forms on two streams, a workspace each, on tensors of a third."""
+    sets = [(hx.paged_latent_attention, Latent("bf16", 512, [900, 33, 5000], 16, 3).arguments()),
+            (hx.paged_latent_attention, Latent("fp8", 512, [5000, 33], 16, 1).arguments()),
+            (hx.latent_prefill_attention, Expanded(2, 9, 150, 700).arguments())]
+    outs = []
+    for call, d in sets:
+        call(**d)
+        torch.cuda.synchronize()
+        outs.append(d["output"].clone())
+        d["output"].fill_(7.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        for (call, d), stream in zip(sets, streams):
+            call(**d, stream=stream)
+    torch.cuda.synchronize()
+    for (_, d), out in zip(sets, outs):
+        assert torch.equal(d["output"], out)
 
 
 def test_expanded_captured_and_replayed(device):
