@@ -883,9 +883,13 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       ready(n + 2, into);
       advance();
       Probabilities p;
-      // Of the way into LDS, the parts that the scores' steps have room for.
+      // Of the way into LDS, the parts beside the scores: those that their steps have room
+      // for, or, where wavefronts are half a step behind, the keys', which the others
+      // read first.
+      constexpr int kKeyParts = (4 * kOwn + kShared / 2) * kTerms;
       constexpr int kRoom = 2 * kSteps * kProducts - kProbParts;
-      constexpr int kBeside = kRoom < kStageParts ? kRoom : kStageParts;
+      constexpr int kBeside = kBehind ? kKeyParts : kRoom < kStageParts ? kRoom : kStageParts;
+      static_assert(kBeside <= kRoom, "a slot a part");
       if (blk + 1 < to) {
         v4f last[RT][2];
 #pragma unroll
@@ -915,7 +919,6 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
 #pragma unroll
         for (int i = 0; i < kProbParts; ++i) probability(i, sc, ref, p);
       }
-      static_assert(!kBehind || kBeside == kStageParts, "an item is whole before the values");
       add_values(buf, p, [&](int i) {
         constexpr int kLeft = kStageParts - kBeside, kSlots = kDims * kProducts;
 #pragma unroll
