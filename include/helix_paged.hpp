@@ -1018,6 +1018,34 @@ class DecodeBatch final {
                                           cosine.data_as<float>(), sine.data_as<float>(),
                                           detail::dim(cosine, 0), stream.native()));
   }
+  /// Rotation and append of a step's rows of one layer in one launch, after prepare()
+  /// or prepare_chunk(): query and keys (rows as append_layer() takes them) rotated
+  /// by the tables [rows, rotary_dim / 2] to query_out and key_out, which may be the
+  /// same tensors, and keys and values to the step's slots.  key_out and `values` are
+  /// then what attention_layer() or prefill_layer() takes.
+  void rope_append_layer(std::size_t layer, const Tensor& query, const Tensor& keys,
+                         const Tensor& values, Tensor& query_out, Tensor& key_out,
+                         const Tensor& cosine, const Tensor& sine, helix_rope_layout layout,
+                         const hip::Stream& stream) {
+    const auto check_rows = [&](const Tensor& t, const char* what, std::size_t heads) {
+      chunked_ ? chunk_rows(t, what, heads) : rows(t, what, heads);
+    };
+    check_rows(query, "rope query", q_heads_);
+    check_rows(query_out, "rope query output", q_heads_);
+    check_rows(keys, "rope keys", kv_heads_);
+    check_rows(key_out, "rope key output", kv_heads_);
+    check_rows(values, "values", kv_heads_);
+    detail::require_float_on(cosine, device_, 2, "rope cosine");
+    detail::require_float_on(sine, device_, 2, "rope sine");
+    detail::require(cosine.shape() == sine.shape(), ErrorCode::kInvalidArgument,
+                    "rope_append_layer: tables must be [rows, rotary_dim / 2]");
+    detail::check(helix_decode_batch_rope_append_layer(
+        batch_handle_, layer, query.data_as<float>(), nullptr, keys.data_as<float>(), nullptr,
+        values.data_as<float>(), nullptr, query_out.data<float>(), nullptr, key_out.data<float>(),
+        nullptr, nullptr, nullptr, cosine.data_as<float>(), sine.data_as<float>(),
+        detail::dim(cosine, 0), 2 * detail::dim(cosine, 1), static_cast<int>(layout),
+        stream.native()));
+  }
   void attention_layer(std::size_t layer, const Tensor& query, const Tensor& tail_key,
                        const Tensor& tail_value, Tensor& output, const hip::Stream& stream) {
     rows(query, "query", q_heads_);
