@@ -103,6 +103,7 @@ struct LatentStream {
   LatentJob* jobs; // by unit where there are no more units than groups, else by group
   int groups;
   int row_blocks;  // units of a sequence
+  int share;       // groups of a row block, or 0: none of its own
   int by_unit;
 };
 
@@ -258,14 +259,20 @@ __device__ __forceinline__ bool first_place(const LatentKernelArgs& a, const Lat
     for (int b0 = 64; b0 < a.batch; b0 += 64) more += places(b0 + lane);
     per_block += uniform_long(__shfl(lane_scan(more, lane), 63, 64));
   }
-  const long long total = per_block * st.row_blocks;
-  each = divide(total + st.groups - 1, st.groups);
+  // A row block's list to its share of the groups, or all of them to all.
+  const int block = st.share > 0 ? group / st.share : 0;
+  if (st.share > 0 && block >= st.row_blocks) return false;
+  const int first_group = block * st.share;
+  const long long total = st.share > 0 ? per_block : per_block * st.row_blocks;
+  const int groups = st.share > 0 ? st.share : st.groups;
+  each = divide(total + groups - 1, groups);
   each = uniform_long(max((each + LEAST - 1) / LEAST * LEAST, 1ll));
-  const long long g0 = group * each;
-  const long long have = min(each, total - g0);
+  const long long at = (group - first_group) * each;
+  const long long have = min(each, total - at);
   if (have <= 0) return false;
-  c.rb = __builtin_amdgcn_readfirstlane(static_cast<int>(divide(g0, per_block)));
-  const long long rem = g0 - c.rb * per_block;
+  c.rb = __builtin_amdgcn_readfirstlane(block + static_cast<int>(divide(at, per_block)));
+  const long long rem = at - (c.rb - block) * per_block;
+  const long long g0 = group * each;
   long long base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int n = b0 == 0 ? mine : places(b0 + lane);
@@ -1443,6 +1450,8 @@ hipError_t launch_latent_attention(const LatentArgs& a, hipStream_t stream) {
   st.part_o = reinterpret_cast<float*>(base + layout.part_o);
   st.groups = static_cast<int>(kGroups);
   st.row_blocks = static_cast<int>(layout.row_blocks);
+  const int share = static_cast<int>(kGroups / layout.row_blocks);
+  st.share = layout.row_blocks > 1 ? share / kXcds * kXcds : 0;
   st.by_unit = a.batch * layout.row_blocks <= kGroups ? 1 : 0;
   switch (a.page_type) {
     case PageType::kBF16: return launch_page_type<1>(k, st, layout.rb, a.latent, stream);

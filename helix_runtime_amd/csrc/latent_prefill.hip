@@ -303,7 +303,6 @@ __device__ __forceinline__ long long lane_scan(long long v, int lane) {
 
 // The range of a workgroup: consecutive ones go to an XCD, which has every eighth
 // workgroup.
-constexpr int kXcds = 8;
 __device__ __forceinline__ int range_of(int block, int groups) {
   return block % kXcds * (groups / kXcds) + block / kXcds;
 }
