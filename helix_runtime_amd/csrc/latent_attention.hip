@@ -98,8 +98,9 @@ struct LatentJob {
 };
 
 struct LatentStream {
-  float* part_o;   // [2 * groups, RB, L]
-  float* part_ml;  // [2 * groups, RB, 2]
+  float* part_o;   // [2 * groups, part_rows, L]
+  float* part_ml;  // [2 * groups, part_rows, 2]
+  int part_rows;   // a unit's rows, or 16 where there are no more
   LatentJob* jobs; // by unit where there are no more units than groups, else by group
   int groups;
   int row_blocks;  // units of a sequence
@@ -1032,12 +1033,12 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       if (rows.live) {
         const int local = wave * 16 + col;
         float* const dst = (complete ? out_row(cur, row)
-                                     : st.part_o + (static_cast<std::size_t>(slot) * RB + local) * L) +
+                                     : st.part_o + (static_cast<std::size_t>(slot) * st.part_rows + local) * L) +
                            4 * grp;
 #pragma unroll
         for (int dt = 0; dt < R::ND; ++dt) *reinterpret_cast<v4f*>(dst + 16 * dt) = rows.o[dt] * f;
         if (!complete && grp == 0) {
-          float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * RB + local) * 2;
+          float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * st.part_rows + local) * 2;
           ml[0] = rows.m;
           ml[1] = bad != 0 ? NAN : sum;
         }
@@ -1140,7 +1141,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
         if (live) {
           float* const dst = complete
                                  ? out_row(cur, r)
-                                 : st.part_o + (static_cast<std::size_t>(slot) * RB + local) * L;
+                                 : st.part_o + (static_cast<std::size_t>(slot) * st.part_rows + local) * L;
 #pragma unroll
           for (int i = 0; i < L / 64; ++i) {
             const int u = 16 * i + col;
@@ -1152,7 +1153,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
             *reinterpret_cast<v4f*>(dst + 4 * u) = x * rf;
           }
           if (!complete && col == 0) {
-            float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * RB + local) * 2;
+            float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * st.part_rows + local) * 2;
             ml[0] = rm;
             ml[1] = bad != 0 ? NAN : rs;
           }
@@ -1188,8 +1189,8 @@ __device__ __forceinline__ MergeRow merge_row(const LatentKernelArgs& a, const L
   r.live = local < rb_rows && r.row < a.rows && r.t < clamped_count(a, job.b);
   return r;
 }
-__device__ __forceinline__ std::size_t merge_slot(const LatentJob& job, int rb_rows, int local, int i) {
-  return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + local;
+__device__ __forceinline__ std::size_t merge_slot(const LatentJob& job, int part_rows, int local, int i) {
+  return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * part_rows + local;
 }
 __device__ __forceinline__ float* merge_out(const LatentKernelArgs& a, const LatentJob& job,
                                             const MergeRow& r) {
@@ -1218,12 +1219,12 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
   float top = -INFINITY, sum = 0.f;
   if (r.live) {
     for (int i = lane; i < parts; i += 64) {
-      top = fmaxf(top, st.part_ml[2 * merge_slot(job, rb_rows, local, i)]);
+      top = fmaxf(top, st.part_ml[2 * merge_slot(job, st.part_rows, local, i)]);
     }
 #pragma unroll
     for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
     for (int i = lane; i < parts; i += 64) {
-      const float* const ml = st.part_ml + 2 * merge_slot(job, rb_rows, local, i);
+      const float* const ml = st.part_ml + 2 * merge_slot(job, st.part_rows, local, i);
       const float w = ml[1] == 0.f ? 0.f : exp2_ratio(ml[0], top);
       sum += ml[1] * w;
       weights[wave][i] = w;
@@ -1243,7 +1244,7 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           x[u][v] = reinterpret_cast<const v4f*>(
-              st.part_o + merge_slot(job, rb_rows, local0 + w, i) * L)[64 * v + lane];
+              st.part_o + merge_slot(job, st.part_rows, local0 + w, i) * L)[64 * v + lane];
         }
       }
 #pragma unroll
@@ -1306,7 +1307,7 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
   // A thread has a partial's maximum and sum.
   float pm = -INFINITY, pl = 0.f;
   if (tid < parts) {
-    const float* const ml = st.part_ml + 2 * merge_slot(job, rb_rows, local, tid);
+    const float* const ml = st.part_ml + 2 * merge_slot(job, st.part_rows, local, tid);
     pm = ml[0];
     pl = ml[1];
   }
@@ -1332,7 +1333,7 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       x[u] = *reinterpret_cast<const v4f*>(
-          st.part_o + merge_slot(job, rb_rows, local, min(i0 + u * kShares, parts - 1)) * L + dim);
+          st.part_o + merge_slot(job, st.part_rows, local, min(i0 + u * kShares, parts - 1)) * L + dim);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1357,24 +1358,38 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
 constexpr std::size_t kGroups = 256;
 static_assert(kGroups + 1 <= kMostParts);
 
-std::size_t unit_rows(std::size_t rows) { return rows <= 16 ? 16 : 64; }
+// Rows of a unit.  Units of 16 rows are ahead, as their wavefronts need not wait for
+// each other (64 sequences of 2048 tokens, 32 rows, fp8 pages: 42 us for 53, fp32
+// 135 for 177; one of 131071 tokens, 48 rows, bf16: 54 for 60), as long as the units
+// that read the same pages find them in L2: where there are many others, or the pages'
+// rows are long, each one's pages come from memory (64 sequences, 64 rows, fp32: 204
+// us for 184; 256 rows of 1024 tokens, fp8: 116 for 86).  With a tile or less for each
+// workgroup the join of what a workgroup's wavefronts have is longer than the tile (one
+// sequence of 500 tokens, 16 rows: 20 us for 16).
+std::size_t unit_rows(const LatentArgs& a) {
+  const std::size_t units = a.batch * ((a.q_heads * a.tokens + 15) / 16);
+  const bool f32 = a.page_type == PageType::kF32;
+  const std::size_t tiles = a.batch * ((a.max_blocks + (f32 ? 0 : 1)) / (f32 ? 1 : 2));
+  if (tiles <= 256) return 64;
+  return a.q_heads * a.tokens <= 16 || units <= (f32 ? 128u : 384u) ? 16 : 64;
+}
 
 std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
 
+// Room for units of 64 rows, where there are as many.
 struct LatentLayout {
   LatentLayout(std::size_t rows, std::size_t latent) {
-    rb = unit_rows(rows);
-    row_blocks = (rows + rb - 1) / rb;
+    const std::size_t part_rows = rows <= 16 ? 16 : 64;
     auto take = [&](std::size_t n) {
       const std::size_t at = bytes;
       bytes += align256(n);
       return at;
     };
     jobs = take(kGroups * sizeof(LatentJob));
-    part_ml = take(2 * kGroups * rb * 2 * sizeof(float));
-    part_o = take(2 * kGroups * rb * latent * sizeof(float));
+    part_ml = take(2 * kGroups * part_rows * 2 * sizeof(float));
+    part_o = take(2 * kGroups * part_rows * latent * sizeof(float));
   }
-  std::size_t rb, row_blocks, jobs, part_ml, part_o, bytes = 0;
+  std::size_t jobs, part_ml, part_o, bytes = 0;
 };
 
 template <int PF, int L>
@@ -1449,14 +1464,16 @@ hipError_t launch_latent_attention(const LatentArgs& a, hipStream_t stream) {
   st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
   st.part_o = reinterpret_cast<float*>(base + layout.part_o);
   st.groups = static_cast<int>(kGroups);
-  st.row_blocks = static_cast<int>(layout.row_blocks);
-  const int share = static_cast<int>(kGroups / layout.row_blocks);
-  st.share = layout.row_blocks > 1 ? share / kXcds * kXcds : 0;
-  st.by_unit = a.batch * layout.row_blocks <= kGroups ? 1 : 0;
+  const std::size_t rb = unit_rows(a), row_blocks = (a.q_heads * a.tokens + rb - 1) / rb;
+  st.part_rows = rb == 16 || a.q_heads * a.tokens <= 16 ? 16 : 64;
+  st.row_blocks = static_cast<int>(row_blocks);
+  const int share = static_cast<int>(kGroups / row_blocks);
+  st.share = row_blocks > 1 ? share / kXcds * kXcds : 0;
+  st.by_unit = a.batch * row_blocks <= kGroups ? 1 : 0;
   switch (a.page_type) {
-    case PageType::kBF16: return launch_page_type<1>(k, st, layout.rb, a.latent, stream);
-    case PageType::kFP8: return launch_page_type<2>(k, st, layout.rb, a.latent, stream);
-    default: return launch_page_type<0>(k, st, layout.rb, a.latent, stream);
+    case PageType::kBF16: return launch_page_type<1>(k, st, rb, a.latent, stream);
+    case PageType::kFP8: return launch_page_type<2>(k, st, rb, a.latent, stream);
+    default: return launch_page_type<0>(k, st, rb, a.latent, stream);
   }
 }
 

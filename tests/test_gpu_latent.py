@@ -58,9 +58,24 @@ def to_pool(dtype, x):
     return t
 
 
+def pytest_generate_tests(metafunc):
+    """Each test of the absorbed form with tables as long as they have to be and with
+    longer ones: the kernel's units may be of 64 or of 16 rows."""
+    if metafunc.function.__name__.startswith("test_absorbed"):
+        metafunc.fixturenames.append("room")
+        metafunc.parametrize("room", [0, 1040], indirect=True)
+
+
+@pytest.fixture
+def room(request, monkeypatch):
+    monkeypatch.setattr(Latent, "room", request.param)
+
+
 class Latent:
     """Scattered pages and queries of one call; slots that hold no token, and pages
     that no table names, are NaN."""
+
+    room = 0  # pages that the table could name besides
 
     def __init__(self, dtype, latent, lengths, hq, t, seed=0, counts=None):
         rng = self.rng = np.random.default_rng(seed + 31 * hq + t)
@@ -72,7 +87,7 @@ class Latent:
         self.rows = [rng.standard_normal((x, latent + ROPE), dtype=np.float32) for x in self.lengths]
         pool = np.full((physical, P, latent + ROPE), np.nan, np.float32)
         order = rng.permutation(physical)
-        self.tables = np.full((b, max(1, max(pages)) + 1), 0xffffffff, np.uint32)
+        self.tables = np.full((b, max(1, max(pages)) + 1 + self.room), 0xffffffff, np.uint32)
         at = 0
         for i, n in enumerate(pages):
             ids = order[at:at + n]
