@@ -33,7 +33,7 @@
 //
 // Units of 64 rows: four wavefronts with 16 rows each share a tile.  Units of 16 rows
 // (what one token of 16 heads is): the wavefronts take tiles in turn, each by
-// itself, and join what they have at the unit's end.
+// itself, and join what they have at the unit's end.  unit_rows() says which.
 #include "bf16.hpp"
 #include "fp8.hpp"
 #include "latent.hpp"
@@ -1358,20 +1358,21 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
 constexpr std::size_t kGroups = 256;
 static_assert(kGroups + 1 <= kMostParts);
 
-// Rows of a unit.  Units of 16 rows are ahead, as their wavefronts need not wait for
-// each other (64 sequences of 2048 tokens, 32 rows, fp8 pages: 42 us for 53, fp32
-// 135 for 177; one of 131071 tokens, 48 rows, bf16: 54 for 60), as long as the units
-// that read the same pages find them in L2: where there are many others, or the pages'
-// rows are long, each one's pages come from memory (64 sequences, 64 rows, fp32: 204
-// us for 184; 256 rows of 1024 tokens, fp8: 116 for 86).  With a tile or less for each
-// workgroup the join of what a workgroup's wavefronts have is longer than the tile (one
-// sequence of 500 tokens, 16 rows: 20 us for 16).
+// Rows of a unit.  The wavefronts of 16-row units need not wait for each other, but
+// each unit brings the pages into LDS for itself.  Two units of the same pages are
+// ahead of one of 64 rows (pages cold; one sequence of 131071 tokens, 32 rows, bf16: 52
+// us for 61; 64 of 2048, fp32: 136 for 178), and up to 256 units of fp8 pages, whose
+// rows are half as long (64 of 2048, 64 rows: 53 for 61; 48 of them, 128 rows: 85 for
+// 81); three or four of bf16 or fp32 pages are not (64 rows, bf16: 74 for 66; 64 of
+// 2048, 40 rows, fp32: 200 for 179).  With a tile or less for each workgroup the join of
+// what a workgroup's wavefronts have takes longer than a tile (one sequence of 500
+// tokens, 16 rows: 20 us for 16).
 std::size_t unit_rows(const LatentArgs& a) {
-  const std::size_t units = a.batch * ((a.q_heads * a.tokens + 15) / 16);
-  const bool f32 = a.page_type == PageType::kF32;
-  const std::size_t tiles = a.batch * ((a.max_blocks + (f32 ? 0 : 1)) / (f32 ? 1 : 2));
-  if (tiles <= 256) return 64;
-  return a.q_heads * a.tokens <= 16 || units <= (f32 ? 128u : 384u) ? 16 : 64;
+  const std::size_t rows = a.q_heads * a.tokens, units = a.batch * ((rows + 15) / 16);
+  const std::size_t tile_pages = a.page_type == PageType::kF32 ? 1 : 2;
+  const std::size_t tiles = a.batch * ((a.max_blocks + tile_pages - 1) / tile_pages);
+  if (tiles <= kGroups) return 64;
+  return rows <= 32 || (a.page_type == PageType::kFP8 && units <= kGroups) ? 16 : 64;
 }
 
 std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
