@@ -1146,8 +1146,8 @@ def latent_prefill_attention(query, key, rope_key, value, output, workspace, sca
     key_lengths[b] keys (int32; None: S), its token_counts[b] new tokens' (int32;
     None: T) the last: row t sees the first key_lengths[b] - token_counts[b] + t + 1.
     Rows that see nothing are 0; rows of `output` behind token_counts stay as they
-    were.  (Numbers that vary by more than fp16's range within a head take about four
-    times as long.)"""
+    were.  (Numbers that vary by more than fp16's range within a head take up to two
+    and a half times as long.)"""
     import torch
     qs, ks = getattr(query, "shape", ()), getattr(key, "shape", ())
     if len(qs) != 4 or len(ks) != 4:

@@ -8,12 +8,14 @@
 // Work split.  16 or 64 of a sequence's rows form a unit; one pass over the
 // sequence's tokens serves them all.  A unit's tokens are tiles of 32 (fp32 pages:
 // 16).  A fixed grid of workgroups takes equal ranges of the flat list of all units'
-// tiles, whatever the lengths (and of what units cost beside their tiles).  A unit inside one range is finished there; one that
-// crosses ranges leaves a partial (maximum, sum, output) per range, and
-// latent_merge_kernel joins them.  A workgroup leaves at most two partials, its first
-// unit's and its last one's, so the workspace depends on the grid, not on the batch.
-// Units of the same sequence lie half the list apart (or a third, ..), so that the
-// workgroups that read the same pages do so at one time, on one XCD.
+// tiles, whatever the lengths (and of what units cost beside their tiles).  A unit
+// inside one range is finished there; one that crosses ranges leaves a partial
+// (maximum, sum, output) per range, which latent_merge_kernel joins.  A workgroup
+// leaves at most two partials, its first unit's and its last one's, so the workspace
+// depends on the grid, not on the batch.  Each row block has its own share of the
+// workgroups, a multiple of the XCDs: those that read the same pages do so at one time,
+// on one XCD.  (One sequence of 131071 tokens, 64 rows in units of 16: 104 us with one
+// list for all row blocks, 65 so.)
 //
 // Matrix form.  Per tile scores are S^T = C Q^T and outputs O^T += C^T P^T, a
 // wavefront having 16 rows: a lane holds tokens of one query row, so a row's maximum
@@ -30,6 +32,12 @@
 //   its largest element in [2^10, 2^11), and probabilities (with them sums and
 //   outputs) carry a factor of 2^8;
 // - fp32 pages: the fp32 matrix instructions.
+//
+// What bounds it.  64 sequences of 512 to 8192 tokens, 16 heads, fp8 pages: 104 MB, 22
+// us at a large copy's rate, 40 here, of which 12 are the start (the queries' way into
+// registers, the first pages') and 9 the join of parts.  128 heads, bf16 pages: 54 Gflop,
+// three times that in products, 133 us at the rate of a large bf16 matrix product, 150
+// here.  One sequence of 131071 tokens, 48 rows, bf16: 151 MB, 32 us, 62 here.
 //
 // Units of 64 rows: four wavefronts with 16 rows each share a tile.  Units of 16 rows
 // (what one token of 16 heads is): the wavefronts take tiles in turn, each by
@@ -179,7 +187,8 @@ struct Tile {
 // What a unit's start costs a workgroup that has begun with another one, in tiles: its
 // queries have to come and be split, its first tiles are waited for, and the last
 // unit's part joined and written.  (64 sequences of 512 to 8192 tokens, 16 heads, fp8
-// pages: the slowest workgroup takes 52 us where starts count nothing, most take 30.)
+// pages: the slowest workgroup takes 52 us where starts count nothing, most take 30; the
+// call takes 43 us with 12, 41 with 16, 38 with 24, 39 with 36.)
 template <bool SHARED>
 constexpr int start_cost() {
   return SHARED ? 4 : 24;
@@ -1199,7 +1208,9 @@ __device__ __forceinline__ float* merge_out(const LatentKernelArgs& a, const Lat
 }
 
 // Units in few parts: a wavefront has one of the four rows of blockIdx.y.  Where a unit
-// has many all the same, the four share each row's.
+// has many all the same, the four share each row's.  (64 sequences of 4096 tokens, 16
+// rows, bf16 pages: 68 us with their join this way, 79 the other; one of 131071 tokens,
+// 32 rows: 110 this way, 62 the other.)
 constexpr int kFewParts = 16;
 template <int L>
 __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, LatentStream st,

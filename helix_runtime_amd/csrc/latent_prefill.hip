@@ -8,15 +8,15 @@
 //
 // Work split.  128 rows (64 where there are no more) of a (sequence, head) form a
 // unit, its keys up to the last that one of them sees are tiles of 32.  A fixed grid
-// takes equal ranges of the flat list of all units' tiles; units that cross ranges
-// leave partials (maximum, sum, output), which expanded_merge_kernel joins.  A head's
-// units follow each other in the list, and an XCD has ranges that do, so that row
-// blocks that read the same keys at about the same time find them in its L2.
+// takes equal ranges of the flat list of all units' tiles (and of what units cost
+// beside them); units that cross ranges leave partials (maximum, sum, output), which
+// expanded_merge_kernel joins.  A head's units follow each other in the list, and an
+// XCD has ranges that do, so that row blocks that read the same keys at about the same
+// time find them in its L2: a third fewer reads past it.
 //
 // Matrix form.  As in the absorbed form: S^T = K Q^T, O^T += V^T P^T, a lane holding
-// keys of one query row; a wavefront has 32 rows, so that an operand out of LDS serves
-// several matrix instructions.  fp32 numbers are sums of 16-bit terms, split once a
-// workgroup on their way into LDS.
+// keys of one query row, a wavefront 16 rows.  fp32 numbers are sums of 16-bit terms,
+// split once a workgroup on their way into LDS.
 // - expanded_kernel: two fp16 terms (22 bits and a sign: the rounding of an fp32
 //   number), of whose four products the three above 2^-22 of the largest are taken.
 //   fp16's range asks for powers of two: a query row's own, one for the keys and one
@@ -29,6 +29,16 @@
 //   first one marked: with numbers past its range, a sum or output that is not finite
 //   (what a row does not see can show that way), or rows of which the 2^-25 might
 //   count, by the size of their scores or outputs.
+//
+// What bounds it: 4 x 32 heads, 512 rows over 4096 keys are 161 Gflop, three times
+// that in products of terms: 413 us at the rate of a large fp16 matrix product, 574 here
+// (600 to 1450 where parts are computed again).  Of a step's 4300 cycles a SIMD's
+// matrix instructions take 2080, its other vector instructions 1300; the two of its
+// wavefronts take turns, and what is left are the waits of one for the other at the
+// step's two barriers and the scalar work between tiles.  Steps on the way: three bf16
+// terms and six products throughout 936 us; two fp16 terms 653; eight wavefronts of 16
+// rows, two a SIMD, for four of 32: 634; four of them half a step behind 610; tiles by
+// scalar bases 584.
 #include "bf16.hpp"
 #include "latent.hpp"
 #include "prefill_bmma.hpp"
@@ -217,7 +227,9 @@ struct ExpandedShared {
   float key_unscale[kMostWaves][4], value_unscale[kMostWaves][4];
 };
 
-// What a unit's start costs a workgroup that has begun with another one, in tiles.
+// What a unit's start costs a workgroup that has begun with another one, in tiles: its
+// queries have to come and be split, and the last unit's part is written.  (5 x 20
+// heads of up to 257 rows: 42 us with 1, 36 with 2 or 3, 38 with 6.)
 constexpr int kStart = 3;
 
 // A place in the flat list, in which each unit has kStart places before its tiles, and
@@ -658,7 +670,8 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   // A matrix instruction takes 16 cycles, of which its issue takes 4: the RT ones of a
   // product have other work put behind them, a part at a time.  (In one piece before
   // or behind the products of a step, which is how the compiler would have it, the two
-  // add up: 925 us for 4 x 32 heads, 512 rows over 4096 keys.)
+  // add up: two matrix and four other instructions take 41 cycles in turn, eight others
+  // in one piece 50 by themselves.)
   auto product = [](int sum, int i) {  // its place in the order below
     return kProducts - (sum + 1) * (sum + 2) / 2 + sum - i;
   };
@@ -1124,6 +1137,9 @@ constexpr std::size_t kGroups = 256;  // a workgroup a CU: a wavefront a SIMD, f
 
 std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
 
+// Units of 64 rows (four wavefronts) where there are no more: 16 x 16 heads, 64 rows
+// over 2048 keys take 131 us, in units of 128 168; 512 rows over 4096 keys take 574 in
+// units of 128, 864 in units of 64, whose keys are split twice as often.
 struct ExpandedLayout {
   ExpandedLayout(std::size_t batch, std::size_t heads, std::size_t tokens) {
     rb = tokens <= 64 ? 64 : 128;

@@ -643,7 +643,7 @@ int helix_paged_latent_attention(const float* query, const size_t* query_strides
  * lengths outside [0, keys], values that are not finite (here also numbers of 3.39e38
  * and more in size) and the workspace as above.  Numbers are taken as two fp16 terms of
  * a power of two times them; query rows whose numbers do not fit are computed again with
- * three bf16 terms, which takes about four times as long for them. */
+ * three bf16 terms, which takes two and a half times as long in all. */
 int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
                                          size_t* out);
 int helix_latent_prefill_attention(const float* query, const size_t* query_strides,
