@@ -21,8 +21,8 @@
 //   number), of whose four products the three above 2^-22 of the largest are taken.
 //   fp16's range asks for powers of two: a query row's own, one for the keys and one
 //   for the values of a unit's part, by the largest numbers of its first eight keys
-//   that all its rows see.  Those keys go to [2^4, 2^5) and values to [2^6, 2^7), so
-//   that keys 2^11 and values 2^9 times as large fit; 2^-25 is lost of numbers as
+//   that all its rows see.  Those keys go to [2^4, 2^5) and values to [2^8, 2^9), so
+//   that keys 2^11 and values 2^7 times as large fit; 2^-25 is lost of numbers as
 //   scaled.  Probabilities carry a factor of 2^8.
 // - expanded_redo_kernel: three bf16 terms (24 bits, fp32's range), of whose nine
 //   products the six above 2^-26 are taken.  It computes parts again whose unit the
@@ -89,7 +89,7 @@ constexpr float kSlack = 7.0f;
 constexpr float kProbLog = 8.0f;
 constexpr int kQueryLog = 10;
 constexpr int kKeyLog = 4;
-constexpr int kValueLog = 6;
+constexpr int kValueLog = 8;
 // Outputs (of values as scaled) below which 2^-25 may count: it is 2^-21 of them.
 constexpr float kSmallOutput = 0x1p-4f;
 // What undoes the scores' powers of two must be below this, or this times the row's

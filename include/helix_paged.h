@@ -641,9 +641,11 @@ int helix_paged_latent_attention(const float* query, const size_t* query_strides
  * All on 16 bytes with strides of four elements; keys of a head less than 2^25 elements
  * apart (else HELIX_UNSUPPORTED).  Rows that see nothing, rows behind token_counts,
  * lengths outside [0, keys], values that are not finite (here also numbers of 3.39e38
- * and more in size) and the workspace as above.  Numbers are taken as two fp16 terms of
- * a power of two times them; query rows whose numbers do not fit are computed again with
- * three bf16 terms, which takes two and a half times as long in all. */
+ * and more in size) and the workspace as above.
+ * Numbers are taken as two fp16 terms of a power of two times them: off by the rounding
+ * of a 32-bit number, or by 2^-33 of the largest values of a part's first keys, where
+ * that is more.  Query rows whose numbers do not fit, or by their size would lose more,
+ * are computed again with three bf16 terms: two and a half times as long in all. */
 int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
                                          size_t* out);
 int helix_latent_prefill_attention(const float* query, const size_t* query_strides,

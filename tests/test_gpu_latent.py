@@ -412,7 +412,7 @@ def test_expanded_sizes_of_numbers(device):
 
 
 @pytest.mark.parametrize("b,h,t,s", [(1, 2, 40, 300), (4, 40, 130, 140)])
-@pytest.mark.parametrize("kind", ["large keys", "large values", "large later values", "small values",
+@pytest.mark.parametrize("kind", ["large keys", "large values", "a large dim", "large later values", "small values",
                                   "small later values", "zero keys first", "weightless values first"])
 def test_expanded_range_of_numbers(device, b, h, t, s, kind):
     """Numbers past 16 bits' range, units alone and in parts: as precise as 32 bits
@@ -425,6 +425,9 @@ def test_expanded_range_of_numbers(device, b, h, t, s, kind):
         p.q, p.k, p.r = p.q * 2.0 ** -60, p.k * 2.0 ** 60, p.r * 2.0 ** 60
     elif kind == "large values":
         p.v *= np.float32(2.0 ** 90)
+    elif kind == "a large dim":
+        # (2^-33 of 2^12 times 4 is a tenth of what the others are held to.)
+        p.v[..., 5] *= np.float32(2.0 ** 12)
     elif kind == "large later values":
         p.v[:, :, 100:] *= np.float32(2.0 ** 40)
     elif kind == "small values":
@@ -470,6 +473,20 @@ def test_expanded_empty_rows_beside_nan(device):
             assert not np.isfinite(got[i, :, empty:]).any(), i
         else:
             close(got[i], want[i])
+
+
+@pytest.mark.parametrize("t", [10, 100])
+def test_nothing_to_do(device, t):
+    """No sequence has a row, or a key: outputs stay, or are 0."""
+    p = Expanded(3, 2, t, 40, counts=[0, -1, 0])
+    assert (p.run() == 7).all()
+    p = Expanded(3, 2, t, 40, lengths=[0, 0, 0])
+    assert (p.run() == 0).all()
+    for room in (0, 1040):
+        p = Latent("bf16", 256, [0, 0], 16, t)
+        p.tables = np.full((2, 1 + room), 0xffffffff, np.uint32)
+        assert (p.run() == 0).all()
+        assert (p.run(token_counts=i32([0, -1])) == 7).all()
 
 
 def test_expanded_bad_lengths(device):
