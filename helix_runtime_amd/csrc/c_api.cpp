@@ -1753,6 +1753,14 @@ bool clear_of(const RowsView& v, const void* p, std::size_t bytes) {
   return v.empty() || !overlap(v.p, v.span() * sizeof(float), p, bytes);
 }
 
+// `n` indexes that a call reads lie neither in its output nor in its workspace.
+void check_indexes_apart(const char* op, const void* p, std::size_t n, const RowsView& output,
+                         const void* workspace, std::size_t workspace_bytes) {
+  const std::size_t bytes = mul(n, sizeof(std::int32_t));
+  check(p == nullptr || (clear_of(output, p, bytes) && !overlap(p, bytes, workspace, workspace_bytes)),
+        Status::kInvalidArgument, op, "output and workspace must not alias other arguments");
+}
+
 helix::hip::RopeStream rope_stream(const RowsView& in, const RowsView& out, std::size_t rotary) {
   helix::hip::RopeStream s{};
   s.in = in.p;
@@ -2098,6 +2106,9 @@ int helix_paged_latent_attention(const float* query, const size_t* query_strides
     check(clear_of(o, workspace, workspace_bytes) && clear_of(q, workspace, workspace_bytes) &&
               clear_of(o, pages, pool) && !overlap(pages, pool, workspace, workspace_bytes),
           Status::kInvalidArgument, op, "output and workspace must not alias other arguments");
+    check_indexes_apart(op, tables, mul(batch, max_blocks), o, workspace, workspace_bytes);
+    check_indexes_apart(op, lengths, batch, o, workspace, workspace_bytes);
+    check_indexes_apart(op, token_counts, batch, o, workspace, workspace_bytes);
     helix::hip::LatentArgs a{};
     a.query = query;
     a.pool = pages;
@@ -2163,6 +2174,8 @@ int helix_latent_prefill_attention(const float* query, const size_t* query_strid
       check(clear_of(*x, workspace, workspace_bytes), Status::kInvalidArgument, op,
             "the workspace must not alias other arguments");
     }
+    check_indexes_apart(op, key_lengths, batch, o, workspace, workspace_bytes);
+    check_indexes_apart(op, token_counts, batch, o, workspace, workspace_bytes);
     helix::hip::ExpandedArgs a{};
     a.query = query;
     a.key = key;

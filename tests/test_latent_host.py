@@ -188,6 +188,20 @@ def test_latent_prefill_refusals(bad, status):
     refused(lib, prefill(lib, **bad), status)
 
 
+def test_latent_indexes_apart():
+    """Tables and lengths in the output or the workspace."""
+    lib = hx.load()
+    for bad in (dict(tables_at=69206016 + 64), dict(lengths=69206016 + 8),
+                dict(tables_at=134217728 + 64), dict(lengths=134217728 + (1 << 20))):
+        refused(lib, latent(lib, **bad), hx.INVALID_ARGUMENT)
+    for at in (64 * MB + 16, 128 * MB + 16):
+        out = 64 * MB
+        for index in ((at, None), (None, at)):
+            refused(lib, lib.helix_latent_prefill_attention(
+                MB, None, 16 * MB, None, 32 * MB, None, 48 * MB, None, 2, 3, 10, 20, *index, out, None,
+                0.1, 128 * MB, 16 << 30, None), hx.INVALID_ARGUMENT)
+
+
 def test_latent_prefill_rows_far_apart():
     """Rows of keys 2^25 numbers apart are refused; a single one has no next."""
     far = dict(v=2**50, vs=strides(2**26, 2**26, 2**25), batch=1, heads=1, keys=2)
