@@ -256,6 +256,12 @@ __device__ __forceinline__ int unit_tiles(int length, int count, int rb) {
   return max((sees + kTile - 1) / kTile, 1);
 }
 
+__device__ __forceinline__ long long divide(long long n, long long d) {
+  // (A 64-bit division takes ten times a 32-bit one.)
+  if ((n | d) >> 31 == 0) return static_cast<unsigned>(n) / static_cast<unsigned>(d);
+  return n / d;
+}
+
 // Places of a sequence's row blocks, for each head: the sum over them of unit_tiles and
 // kStart.  Of all but the last block the tiles grow by RB / kTile a block, from 1 up.
 template <int RB>
@@ -272,12 +278,18 @@ __device__ __forceinline__ long long head_places(int length, int count) {
          max((length + kTile - 1) / kTile, 1) + kStart * blocks;
 }
 
-template <int RB>
-__device__ __forceinline__ long long sequence_places(const ExpandedKernelArgs& a, long long b) {
-  if (b >= a.batch) return 0;
-  int length = a.key_lengths != nullptr ? a.key_lengths[b] : a.keys;
-  if (length < 0 || length > a.keys) length = 0;
-  return head_places<RB>(length, clamped_count(a, static_cast<int>(b)));
+// A sequence's number of keys (0 where it is none) and of rows.
+struct SequenceSize {
+  int length, count, bad;
+};
+__device__ __forceinline__ SequenceSize sequence_size(const ExpandedKernelArgs& a, long long b) {
+  SequenceSize s{0, 0, 0};
+  if (b >= a.batch) return s;
+  s.length = a.key_lengths != nullptr ? a.key_lengths[b] : a.keys;
+  s.count = clamped_count(a, static_cast<int>(b));
+  s.bad = s.length < 0 || s.length > a.keys;
+  if (s.bad != 0) s.length = 0;
+  return s;
 }
 
 template <int RB>
@@ -325,38 +337,40 @@ template <int RB>
 __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const ExpandedStream& st,
                                             int group, int lane, long long& each,
                                             ExpandedCursor& c) {
-  const long long mine = sequence_places<RB>(a, lane) * a.heads;
-  const long long sums = lane_scan(mine, lane);
+  const SequenceSize mine = sequence_size(a, lane);
+  auto places = [&](const SequenceSize& s) { return head_places<RB>(s.length, s.count) * a.heads; };
+  const long long own = places(mine);
+  const long long sums = lane_scan(own, lane);
   long long total = uniform_long(__shfl(sums, 63, 64));
   if (a.batch > 64) {
     long long more = 0;
-    for (long long b0 = 64; b0 < a.batch; b0 += 64) {
-      more += sequence_places<RB>(a, b0 + lane) * a.heads;
-    }
+    for (long long b0 = 64; b0 < a.batch; b0 += 64) more += places(sequence_size(a, b0 + lane));
     total += uniform_long(__shfl(lane_scan(more, lane), 63, 64));
   }
-  each = uniform_long(max((total + st.groups - 1) / st.groups, 1ll));
+  each = uniform_long(max(divide(total + st.groups - 1, st.groups), 1ll));
   const long long g0 = group * each;
   const long long have = min(each, total - g0);
   if (have <= 0) return false;
   long long base = 0;
   for (long long b0 = 0; b0 < a.batch; b0 += 64) {
-    const long long n = b0 == 0 ? mine : sequence_places<RB>(a, b0 + lane) * a.heads;
+    const SequenceSize size = b0 == 0 ? mine : sequence_size(a, b0 + lane);
+    const long long n = b0 == 0 ? own : places(size);
     const long long sum = b0 == 0 ? sums : lane_scan(n, lane);
     const long long from = base + sum - n, to = base + sum;
     const unsigned long long hit = __ballot(from <= g0 && g0 < to);
     if (hit != 0) {
       const int src = __ffsll(static_cast<long long>(hit)) - 1;
       c.b = __builtin_amdgcn_readfirstlane(static_cast<int>(b0) + src);
+      c.length = __builtin_amdgcn_readlane(size.length, src);
+      c.count = __builtin_amdgcn_readlane(size.count, src);
+      c.bad = __builtin_amdgcn_readlane(size.bad, src);
       base = uniform_long(__shfl(from, src, 64));
       break;
     }
     base += uniform_long(__shfl(sum, 63, 64));
   }
-  c.rb = 0;
-  load_unit<RB>(a, c);
   const long long head = uniform_long(head_places<RB>(c.length, c.count));
-  c.h = __builtin_amdgcn_readfirstlane(static_cast<int>((g0 - base) / head));
+  c.h = __builtin_amdgcn_readfirstlane(static_cast<int>(divide(g0 - base, head)));
   base += c.h * head;
   for (int rb0 = 0;; rb0 += 64) {
     const int tiles = unit_tiles<RB>(c.length, c.count, rb0 + lane);
@@ -371,7 +385,7 @@ __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const E
     }
     base += uniform_long(__shfl(sum, 63, 64));
   }
-  load_unit<RB>(a, c);
+  set_unit<RB>(c);
   const int in = __builtin_amdgcn_readfirstlane(static_cast<int>(g0 - c.base));
   c.blk = max(in - kStart, 0);
   c.to = __builtin_amdgcn_readfirstlane(
@@ -867,7 +881,6 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
   barrier();
   constexpr int kItems = ExpandedShared<F16>::kItems;
   constexpr bool kBehind = WAVES == 8;  // whether four wavefronts are half a step behind
-  if (kBehind && wave >= 4) barrier();
   int n = 0, slot = 0;  // n modulo kItems
   auto later = [](int at, int by) { return at + by >= kItems ? at + by - kItems : at + by; };
   for (;;) {
@@ -879,6 +892,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     scores(slot, sc, [](int) {});
     // (Of two items, this one's keys are taken before it is written again.)
     if constexpr (kItems == 2) barrier();
+    if (kBehind && n == 0 && wave >= 4) barrier();
     for (int blk = from; blk < to; ++blk) {
       const int buf = later(slot, 1), into = later(slot, 2);
       if (blk >= whole) {
@@ -994,7 +1008,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       if (tid == 0) {
         if (ends && !starts) {
           st.jobs[group] = ExpandedJob{cur.b, cur.h, cur.rb,
-                                       static_cast<int>((cur.base + kStart) / each), group};
+                                       static_cast<int>(divide(cur.base + kStart, each)), group};
         }
       }
     }
