@@ -1228,37 +1228,55 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
   const int local0 = static_cast<int>(blockIdx.y) * 4, local = local0 + wave;
   const MergeRow r = merge_row(a, job, rb_rows, local);
   const int parts = min(job.last - job.first + 1, kMostParts);
+  // Partials `first`, first + step, .. of row local0 + w on their way.
+  using Parts = v4f[U][NV];
+  auto load = [&](int w, int first, int step, Parts& x) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(first + u * step, parts - 1);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        x[u][v] = reinterpret_cast<const v4f*>(
+            st.part_o + merge_slot(job, st.part_rows, local0 + w, i) * L)[64 * v + lane];
+      }
+    }
+  };
+  // The first ones are sent for before their weights are known.
+  Parts begun;
+  const int first = parts <= kFewParts ? 0 : wave, step = parts <= kFewParts ? 1 : 4;
+  if (r.live && parts <= kFewParts) load(wave, first, step, begun);
   float top = -INFINITY, sum = 0.f;
   if (r.live) {
-    for (int i = lane; i < parts; i += 64) {
-      top = fmaxf(top, st.part_ml[2 * merge_slot(job, st.part_rows, local, i)]);
-    }
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+      const int i = i0 + lane;
+      v2f ml = {-INFINITY, 0.f};
+      if (i < parts) {
+        ml = *reinterpret_cast<const v2f*>(st.part_ml + 2 * merge_slot(job, st.part_rows, local, i));
+      }
+      float most = ml[0];
 #pragma unroll
-    for (int k = 32; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
-    for (int i = lane; i < parts; i += 64) {
-      const float* const ml = st.part_ml + 2 * merge_slot(job, st.part_rows, local, i);
-      const float w = ml[1] == 0.f ? 0.f : exp2_ratio(ml[0], top);
-      sum += ml[1] * w;
-      weights[wave][i] = w;
-    }
+      for (int k = 32; k > 0; k /= 2) most = fmaxf(most, __shfl_xor(most, k, 64));
+      // (Weights so far are relative to the largest so far.)
+      const float now = fmaxf(top, most);
+      const float turn = exp2_ratio(top, now);
+      if (turn != 1.f) {
+        for (int j = lane; j < i0; j += 64) weights[wave][j] *= turn;
+      }
+      const float f = ml[1] == 0.f ? 0.f : exp2_ratio(ml[0], now);
+      if (i < parts) weights[wave][i] = f;
+      float add = ml[1] * f;
 #pragma unroll
-    for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
+      for (int k = 32; k > 0; k /= 2) add += __shfl_xor(add, k, 64);
+      sum = sum * turn + add;
+      top = now;
+    }
   }
-  // Of row local0 + w its partials first, first + step, ..
-  auto gather = [&](int w, int first, int step, v4f (&o)[NV]) {
+  // Of row local0 + w, partials first, first + step, ..; the first U are in x.
+  auto gather = [&](int w, Parts& x, v4f (&o)[NV]) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) o[v] = v4f{0.f, 0.f, 0.f, 0.f};
     for (int i0 = first; i0 < parts; i0 += U * step) {
-      v4f x[U][NV];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = min(i0 + u * step, parts - 1);
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          x[u][v] = reinterpret_cast<const v4f*>(
-              st.part_o + merge_slot(job, st.part_rows, local0 + w, i) * L)[64 * v + lane];
-        }
-      }
+      if (i0 != first) load(w, i0, step, x);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * step;
@@ -1272,13 +1290,14 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
   };
   v4f o[NV];
   if (parts <= kFewParts) {
-    if (r.live) gather(wave, 0, 1, o);
+    if (r.live) gather(wave, begun, o);
   } else {
     for (int w = 0; w < 4; ++w) {
       __syncthreads();
       if (!merge_row(a, job, rb_rows, local0 + w).live) continue;
       v4f own[NV];
-      gather(w, wave, 4, own);
+      load(w, first, step, begun);
+      gather(w, begun, own);
 #pragma unroll
       for (int v = 0; v < NV; ++v) sums[wave][64 * v + lane] = own[v];
       __syncthreads();

@@ -1093,14 +1093,27 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
   auto slot = [&](int i) {
     return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + at;
   };
+  // Four partials at a time on their way, the first ones before their weights are known.
+  v4f x[4][2];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const auto* from = reinterpret_cast<const v4f*>(
+                             st.part_o + slot(min(i0 + u, parts - 1)) * kValueDim) +
+                         2 * part;
+      x[u][0] = from[0];
+      x[u][1] = from[1];
+    }
+  };
+  load(0);
   float top = -INFINITY, sum = 0.f;
   v4f o[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
   for (int i0 = 0; i0 < parts; i0 += 16) {
     float pm = -INFINITY, pl = 0.f;
     if (live && i0 + part < parts) {
-      const v2f x = *reinterpret_cast<const v2f*>(st.part_ml + 2 * slot(i0 + part));
-      pm = x[0];
-      pl = x[1];
+      const v2f ml = *reinterpret_cast<const v2f*>(st.part_ml + 2 * slot(i0 + part));
+      pm = ml[0];
+      pl = ml[1];
     }
     float mx = pm;
 #pragma unroll
@@ -1118,14 +1131,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
     top = mn;
     const int end = min(parts - i0, 16);
     for (int i = 0; i < end; i += 4) {
-      v4f x[4][2];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const auto* from =
-            reinterpret_cast<const v4f*>(st.part_o + slot(i0 + min(i + u, end - 1)) * kValueDim) + 2 * part;
-        x[u][0] = from[0];
-        x[u][1] = from[1];
-      }
+      if (i0 + i != 0) load(i0 + i);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float wi = __shfl(w, (lane & 48) + min(i + u, end - 1), 64);
