@@ -10,9 +10,10 @@
 // unit, its keys up to the last that one of them sees are tiles of 32.  A fixed grid
 // takes equal ranges of the flat list of all units' tiles (and of what units cost
 // beside them); units that cross ranges leave partials (maximum, sum, output), which
-// expanded_merge_kernel joins.  A head's units follow each other in the list, and an
+// expanded_merge_kernel joins.  A head's units lie near each other in the list, and an
 // XCD has ranges that do, so that row blocks that read the same keys at about the same
-// time find them in its L2: a third fewer reads past it.
+// time find them in its L2: of 21 million cache lines of the case below 9 are read past
+// it, with row blocks apart 20.
 //
 // Matrix form.  As in the absorbed form: S^T = K Q^T, O^T += V^T P^T, a lane holding
 // keys of one query row, a wavefront 16 rows.  fp32 numbers are sums of 16-bit terms,
@@ -31,14 +32,14 @@
 //   count, by the size of their scores or outputs.
 //
 // What bounds it: 4 x 32 heads, 512 rows over 4096 keys are 161 Gflop, three times
-// that in products of terms: 413 us at the rate of a large fp16 matrix product, 574 here
-// (600 to 1450 where parts are computed again).  Of a step's 4300 cycles a SIMD's
+// that in products of terms: 413 us at the rate of a large fp16 matrix product, 543 here
+// (1300 to 1450 where parts are computed again).  Of a step's 4300 cycles a SIMD's
 // matrix instructions take 2080, its other vector instructions 1300; the two of its
 // wavefronts take turns, and what is left are the waits of one for the other at the
 // step's two barriers and the scalar work between tiles.  Steps on the way: three bf16
 // terms and six products throughout 936 us; two fp16 terms 653; eight wavefronts of 16
 // rows, two a SIMD, for four of 32: 634; four of them half a step behind 610; tiles by
-// scalar bases 584.
+// scalar bases 584; heads woven 543.
 #include "bf16.hpp"
 #include "latent.hpp"
 #include "prefill_bmma.hpp"
@@ -126,6 +127,7 @@ struct ExpandedStream {
   unsigned char* part_marks;   // [2 * groups, waves]: partials
   unsigned char* group_marks;  // [groups, waves]: any of the group's
   int groups;
+  int weave;  // heads whose units take turns in the list: what a range has units of
 };
 
 // Terms of an fp32 number, fp16 or bf16, and the products of two numbers' that are
@@ -236,6 +238,7 @@ constexpr int kStart = 3;
 // what of its unit is in the workgroup's range.
 struct ExpandedCursor {
   int b, h, rb, blk, to;  // the next tile, and the end of the range's
+  int h0;                 // the first head of those woven with it
   int left;               // places of the range behind the unit's
   long long base;         // the unit's first place
   int length, count, nb;
@@ -332,7 +335,8 @@ __device__ __forceinline__ int range_of(int block, int groups) {
 }
 
 // Range `group`'s first place, of ranges of `each` places; whether it has a tile.  The
-// list goes by sequence, head, row block and tile.
+// list goes by sequence, `weave` heads at a time, row block, head of those, and tile:
+// ranges of so many units begin a head's row blocks at one time.
 template <int RB>
 __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const ExpandedStream& st,
                                             int group, int lane, long long& each,
@@ -370,22 +374,29 @@ __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const E
     base += uniform_long(__shfl(sum, 63, 64));
   }
   const long long head = uniform_long(head_places<RB>(c.length, c.count));
-  c.h = __builtin_amdgcn_readfirstlane(static_cast<int>(divide(g0 - base, head)));
-  base += c.h * head;
+  const int woven = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(divide(g0 - base, head * st.weave)));
+  c.h0 = woven * st.weave;
+  base += c.h0 * head;
+  const int heads = min(st.weave, a.heads - c.h0);
   for (int rb0 = 0;; rb0 += 64) {
     const int tiles = unit_tiles<RB>(c.length, c.count, rb0 + lane);
-    const long long n = tiles > 0 ? tiles + kStart : 0;
+    const long long n = tiles > 0 ? static_cast<long long>(tiles + kStart) * heads : 0;
     const long long sum = lane_scan(n, lane);
     const unsigned long long hit = __ballot(base + sum - n <= g0 && g0 < base + sum);
     if (hit != 0 || rb0 >= c.count / RB) {
       const int src = hit != 0 ? __ffsll(static_cast<long long>(hit)) - 1 : 0;
       c.rb = __builtin_amdgcn_readfirstlane(rb0 + src);
-      c.base = uniform_long(base + __shfl(sum - n, src, 64));
+      base = uniform_long(base + __shfl(sum - n, src, 64));
       break;
     }
     base += uniform_long(__shfl(sum, 63, 64));
   }
   set_unit<RB>(c);
+  const int before = __builtin_amdgcn_readfirstlane(
+      static_cast<int>(divide(g0 - base, c.nb + kStart)));
+  c.h = c.h0 + before;
+  c.base = uniform_long(base + static_cast<long long>(before) * (c.nb + kStart));
   const int in = __builtin_amdgcn_readfirstlane(static_cast<int>(g0 - c.base));
   c.blk = max(in - kStart, 0);
   c.to = __builtin_amdgcn_readfirstlane(
@@ -403,16 +414,21 @@ __device__ __forceinline__ std::size_t unit_index(const ExpandedKernelArgs& a,
 // Whether the range has tiles of a later unit, and that unit.
 __device__ __forceinline__ bool more_units(const ExpandedCursor& c) { return c.left > kStart; }
 template <int RB>
-__device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, ExpandedCursor& c) {
+__device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, const ExpandedStream& st,
+                                          ExpandedCursor& c) {
   c.base += c.nb + kStart;
-  if (++c.rb * RB >= c.count) {
-    c.rb = 0;
-    if (++c.h == a.heads) {
-      c.h = 0;
-      do {
-        ++c.b;
-        load_unit<RB>(a, c);
-      } while (c.nb == 0);
+  if (++c.h == min(c.h0 + st.weave, a.heads)) {
+    c.h = c.h0;
+    if (++c.rb * RB >= c.count) {
+      c.rb = 0;
+      c.h = c.h0 = c.h0 + st.weave;
+      if (c.h0 >= a.heads) {
+        c.h = c.h0 = 0;
+        do {
+          ++c.b;
+          load_unit<RB>(a, c);
+        } while (c.nb == 0);
+      }
     }
   }
   set_unit<RB>(c);
@@ -849,7 +865,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       keys.last -= kTile;
       keys.seen -= kTile;
     } else if (more_units(ahead)) {
-      next_unit<RB>(a, ahead);
+      next_unit<RB>(a, st, ahead);
       keys = source(ahead);
     }
   };
@@ -1013,7 +1029,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       }
     }
     if (!more_units(cur)) break;
-    next_unit<RB>(a, cur);
+    next_unit<RB>(a, st, cur);
   }
   if (kBehind && wave < 4) barrier();
   if constexpr (!F16) barrier();  // (another unit may follow)
@@ -1070,7 +1086,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
       expanded_range<4, RT, false>(a, st, sh, one, each);
     }
     if (!more_units(cur)) break;
-    next_unit<RB>(a, cur);
+    next_unit<RB>(a, st, cur);
   }
 }
 
@@ -1243,6 +1259,15 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   st.part_ml = reinterpret_cast<float*>(base + layout.part_ml);
   st.part_o = reinterpret_cast<float*>(base + layout.part_o);
   st.groups = static_cast<int>(kGroups);
+  // Row blocks over a long history are about as long as each other, and read a key at
+  // about one time where a range's units are of as many heads (4 x 32 heads, 512 rows
+  // over 4096 keys: 553 us for 578, a third fewer reads past L2).  Those of a prompt
+  // by itself grow, and so do their ranges' distances (64 heads, 2048 rows and keys:
+  // 382 for 346).
+  const std::size_t units = a.batch * a.heads * layout.row_blocks;
+  st.weave = a.keys / 2 < a.tokens
+                 ? 1
+                 : static_cast<int>(std::clamp<std::size_t>(units / kGroups, 1, a.heads));
   return layout.rb == 64 ? launch_expanded<1>(k, st, stream) : launch_expanded<2>(k, st, stream);
 }
 

@@ -531,6 +531,17 @@ def test_expanded_many_units(device, b, h, t, s):
     close(p.run(), p.want())
 
 
+@pytest.mark.parametrize("b,h,t,s", [(5, 61, 130, 300), (13, 61, 50, 120), (2, 400, 65, 140)])
+def test_expanded_heads_that_no_number_divides(device, b, h, t, s):
+    """Histories longer than the step, and units of several heads to a workgroup: some
+    sequences without rows, or shorter than their tables say."""
+    rng = np.random.default_rng(h)
+    p = Expanded(b, h, t, s, counts=[int(x) for x in rng.integers(t // 2, t + 2, b)],
+                 lengths=[int(x) for x in rng.integers(s // 2, s + 1, b)])
+    p.counts[0] = 0
+    close(p.run(), p.want())
+
+
 @pytest.mark.parametrize("t", [20, 100])
 def test_expanded_rows_far_apart(device, t):
     """Keys' rows as far apart as they may be, and sequences past 2^32 bytes."""
