@@ -437,8 +437,8 @@ __device__ __forceinline__ void next_unit(const ExpandedKernelArgs& a, const Exp
   c.left = max(c.left - c.nb - kStart, 0);
 }
 
-// The range that begins at `cur`.  RT tiles of 16 query rows a wavefront: units of RB =
-// 64 RT rows.  F16: which terms (bf16 ones compute again, and mark nothing).  `each`:
+// The range that begins at `cur`.  RT tiles of 16 query rows a wavefront, units of RB
+// rows.  F16: which terms (bf16 ones compute again, and mark nothing).  `each`:
 // places of a range.
 template <int WAVES, int RT, bool F16>
 __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, const ExpandedStream& st,
