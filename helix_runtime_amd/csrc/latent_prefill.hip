@@ -112,7 +112,7 @@ struct ExpandedKernelArgs {
   float qscale;  // log2(e) * scale
 };
 
-// A unit to join: the one that a group's range ends without starting it.
+// A unit to join: one that a group's range ends without starting it.
 struct ExpandedJob {
   int b, h, rb;     // sequence (-1: none), head, row block
   int first, last;  // groups whose ranges start and end the unit
@@ -121,12 +121,13 @@ struct ExpandedJob {
 struct ExpandedStream {
   float* part_o;     // [2 * groups, RB, 128]
   float* part_ml;    // [2 * groups, RB, 2]
-  ExpandedJob* jobs; // [groups]
+  ExpandedJob* jobs; // by unit where there are no more units than groups, else by group
   // A byte a wavefront: 1 if its rows are to be computed again.
   unsigned char* unit_marks;   // [row blocks, batch, heads, waves]: units that a group has whole
   unsigned char* part_marks;   // [2 * groups, waves]: partials
   unsigned char* group_marks;  // [groups, waves]: any of the group's
   int groups;
+  int by_unit;
   int weave;  // heads whose units take turns in the list: what a range has units of
 };
 
@@ -1022,9 +1023,10 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
         if (any) st.group_marks[group * WAVES + wave] = 1;
       }
       if (tid == 0) {
-        if (ends && !starts) {
-          st.jobs[group] = ExpandedJob{cur.b, cur.h, cur.rb,
-                                       static_cast<int>(divide(cur.base + kStart, each)), group};
+        if (ends && (!starts || st.by_unit != 0)) {
+          st.jobs[st.by_unit != 0 ? unit_index(a, cur) : static_cast<std::size_t>(group)] =
+              ExpandedJob{starts ? -1 : cur.b, cur.h, cur.rb,
+                          static_cast<int>(divide(cur.base + kStart, each)), group};
         }
       }
     }
@@ -1041,7 +1043,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
   __shared__ ExpandedShared<true> sh;
   constexpr int RB = 16 * WAVES;
   const int group = range_of(static_cast<int>(blockIdx.x), st.groups);
-  if (threadIdx.x == 0) st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
+  if (threadIdx.x == 0 && st.by_unit == 0) st.jobs[group] = ExpandedJob{-1, 0, 0, 0, 0};
   if (threadIdx.x % 64 == 0) st.group_marks[group * WAVES + threadIdx.x / 64] = 0;
   ExpandedCursor cur{};
   long long each;
@@ -1091,24 +1093,96 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
 }
 
 // Joins the partials of the units that cross ranges: the first group's second slot
-// and the later groups' first ones.  blockIdx.x is a group; 16 lanes take a row, 8
-// dims each, and 16 partials' statistics at a time.
-constexpr int kMergeRows = 16;
-__global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs a,
-                                                             ExpandedStream st, int rb_rows) {
+// and the later groups' first ones.  blockIdx.x is a unit or a group; 16 lanes take a
+// row, 8 dims each.  A workgroup has `wg_rows` rows, 16 or 4.
+constexpr int kFewParts = 16;
+__global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs a, ExpandedStream st,
+                                                             int rb_rows, int wg_rows) {
+  __shared__ v4f sums[4][64][2];
+  __shared__ float totals[4][4];
   const int lane = threadIdx.x & 63, part = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  if (st.by_unit != 0) {  // (of units without rows no one says anything)
+    const int entry = static_cast<int>(blockIdx.x) / a.heads;
+    if (entry / a.batch * rb_rows >= clamped_count(a, entry % a.batch)) return;
+  }
   const ExpandedJob job = st.jobs[blockIdx.x];
   if (job.b < 0) return;
-  const int local = static_cast<int>(blockIdx.y) * kMergeRows + wave * 4 + (lane >> 4);
-  const int row = job.rb * rb_rows + local;
-  const bool live = local < rb_rows && row < clamped_count(a, job.b);
+  const int parts = job.last - job.first + 1;
+  const int count = clamped_count(a, job.b);
+  const int local0 = static_cast<int>(blockIdx.y) * wg_rows;
+  auto slot_of = [&](int i, int row) {
+    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + row;
+  };
+  auto finish = [&](int row, const v4f (&o)[2], float sum) {
+    const float f = sum == 0.f ? 0.f : 1.0f / sum;
+    auto* const dst = reinterpret_cast<v4f*>(
+                          a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
+                          static_cast<std::size_t>(job.h) * a.out_at.head +
+                          static_cast<std::size_t>(job.rb * rb_rows + row) * a.out_at.token) +
+                      2 * part;
+    dst[0] = o[0] * f;
+    dst[1] = o[1] * f;
+  };
+  if (parts > kFewParts) {
+    // Many parts: the wavefronts have every fourth one of the same four rows.
+    for (int q = 0; q < wg_rows; q += 4) {
+      const int local = local0 + q + (lane >> 4);
+      const bool live = local < rb_rows && job.rb * rb_rows + local < count;
+      const int row = live ? local : 0;
+      float top = -INFINITY;
+      for (int i = part; i < parts; i += 16) top = fmaxf(top, st.part_ml[2 * slot_of(i, row)]);
+#pragma unroll
+      for (int k = 8; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
+      float sum = 0.f;
+      v4f o[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+      constexpr int U = 4;
+      for (int i0 = wave; i0 < parts; i0 += 4 * U) {
+        v4f x[U][2];
+        v2f ml[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const std::size_t at = slot_of(min(i0 + 4 * u, parts - 1), row);
+          ml[u] = *reinterpret_cast<const v2f*>(st.part_ml + 2 * at);
+          const auto* from = reinterpret_cast<const v4f*>(st.part_o + at * kValueDim) + 2 * part;
+          x[u][0] = from[0];
+          x[u][1] = from[1];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          // (A part that saw nothing has no outputs to speak of.)
+          const bool some = i0 + 4 * u < parts && ml[u][1] != 0.f;
+          const float w = some ? exp2_ratio(ml[u][0], top) : 0.f;
+          if (w != 0.f) {
+            o[0] += x[u][0] * w;
+            o[1] += x[u][1] * w;
+          }
+          if (some) sum += ml[u][1] * w;
+        }
+      }
+      __syncthreads();
+      sums[wave][lane][0] = o[0];
+      sums[wave][lane][1] = o[1];
+      if (part == 0) totals[wave][lane >> 4] = sum;
+      __syncthreads();
+      if (wave == 0 && live) {
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          o[0] += sums[w][lane][0];
+          o[1] += sums[w][lane][1];
+          sum += totals[w][lane >> 4];
+        }
+        finish(local, o, sum);
+      }
+    }
+    return;
+  }
+  if (wave * 4 >= wg_rows) return;
+  const int local = local0 + wave * 4 + (lane >> 4);
+  const bool live = local < rb_rows && job.rb * rb_rows + local < count;
   if (__ballot(live) == 0) return;
   const int at = live ? local : 0;
-  const int parts = job.last - job.first + 1;
-  auto slot = [&](int i) {
-    return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + at;
-  };
+  auto slot = [&](int i) { return slot_of(i, at); };
   // Four partials at a time on their way, the first ones before their weights are known.
   v4f x[4][2];
   auto load = [&](int i0) {
@@ -1158,14 +1232,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
       }
     }
   }
-  if (!live) return;
-  const float f = sum == 0.f ? 0.f : 1.0f / sum;
-  auto* const dst = reinterpret_cast<v4f*>(a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
-                                           static_cast<std::size_t>(job.h) * a.out_at.head +
-                                           static_cast<std::size_t>(row) * a.out_at.token) +
-                    2 * part;
-  dst[0] = o[0] * f;
-  dst[1] = o[1] * f;
+  if (live) finish(local, o, sum);
 }
 
 // ----------------------------------------------------------------- host ----
@@ -1196,7 +1263,8 @@ struct ExpandedLayout {
 };
 
 template <int RT>
-hipError_t launch_expanded(const ExpandedKernelArgs& k, const ExpandedStream& st, hipStream_t stream) {
+hipError_t launch_expanded(const ExpandedKernelArgs& k, const ExpandedStream& st, std::size_t units,
+                           hipStream_t stream) {
   constexpr int RB = 64 * RT;
   const dim3 grid(static_cast<unsigned>(kGroups));
   expanded_kernel<4 * RT><<<grid, 256 * RT, 0, stream>>>(k, st);
@@ -1205,8 +1273,14 @@ hipError_t launch_expanded(const ExpandedKernelArgs& k, const ExpandedStream& st
   expanded_redo_kernel<RT><<<grid, 256, 0, stream>>>(k, st);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const unsigned rows = static_cast<unsigned>(std::min(RB, k.tokens));
-  expanded_merge_kernel<<<dim3(grid.x, (rows + kMergeRows - 1) / kMergeRows), 256, 0, stream>>>(k, st, RB);
+  const std::size_t rows = static_cast<std::size_t>(std::min(RB, k.tokens));
+  const std::size_t jobs = st.by_unit != 0 ? units : kGroups;
+  // Few units, so in many parts: workgroups of four rows.  (One head's 114 rows over
+  // 7920 keys, twice: 39 us so, 107 with workgroups of 16 rows whose wavefronts have four
+  // each.)
+  const std::size_t wg_rows = units * kFewParts <= kGroups ? 4 : 16;
+  const dim3 joins(static_cast<unsigned>(jobs), static_cast<unsigned>((rows + wg_rows - 1) / wg_rows));
+  expanded_merge_kernel<<<joins, 256, 0, stream>>>(k, st, RB, static_cast<int>(wg_rows));
   return hipGetLastError();
 }
 
@@ -1265,10 +1339,12 @@ hipError_t launch_expanded_attention(const ExpandedArgs& a, hipStream_t stream) 
   // by itself grow, and so do their ranges' distances (64 heads, 2048 rows and keys:
   // 382 for 346).
   const std::size_t units = a.batch * a.heads * layout.row_blocks;
+  st.by_unit = units <= kGroups ? 1 : 0;
   st.weave = a.keys / 2 < a.tokens
                  ? 1
                  : static_cast<int>(std::clamp<std::size_t>(units / kGroups, 1, a.heads));
-  return layout.rb == 64 ? launch_expanded<1>(k, st, stream) : launch_expanded<2>(k, st, stream);
+  return layout.rb == 64 ? launch_expanded<1>(k, st, units, stream)
+                         : launch_expanded<2>(k, st, units, stream);
 }
 
 }  // namespace helix::hip

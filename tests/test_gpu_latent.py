@@ -542,6 +542,31 @@ def test_expanded_heads_that_no_number_divides(device, b, h, t, s):
     close(p.run(), p.want())
 
 
+@pytest.mark.parametrize("b,h,t,s", [(1, 1, 20, 3000), (2, 1, 114, 2500), (1, 3, 130, 2000),
+                                     (1, 16, 70, 1500)])
+def test_expanded_few_units_in_many_parts(device, b, h, t, s):
+    p = Expanded(b, h, t, s)
+    close(p.run(), p.want())
+
+
+def test_expanded_one_long_sequence_among_many(device):
+    """Broadcast keys of 300 sequences, of which one sees all and is in many parts."""
+    b, t, s = 300, 20, 4000
+    p = Expanded(b, 1, t, 1, lengths=[25] * b)
+    p.lengths[100] = s
+    d = p.arguments()
+    p.shape = (b, 1, t, s)
+    for name, key, tail in (("k", "key", (1, s, 128)), ("v", "value", (1, s, 128)),
+                            ("r", "rope_key", (s, 64))):
+        one = p.rng.standard_normal((1, *tail), dtype=np.float32)
+        setattr(p, name, np.broadcast_to(one, (b, *tail)))
+        d[key] = dev(one).expand(b, *tail)
+    d["workspace"] = hx.latent_prefill_workspace(b, 1, t, s)
+    d["workspace"].fill_(255)
+    hx.latent_prefill_attention(**d)
+    close(host(d["output"]), p.want())
+
+
 @pytest.mark.parametrize("t", [20, 100])
 def test_expanded_rows_far_apart(device, t):
     """Keys' rows as far apart as they may be, and sequences past 2^32 bytes."""
