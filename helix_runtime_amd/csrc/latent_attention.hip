@@ -38,7 +38,7 @@
 // registers, the first pages') and 8 the joins of wavefronts and of parts.  128 heads,
 // bf16 pages: 54 Gflop, three times that in products, 133 us at the rate of a large
 // bf16 matrix product, 148 here.  One sequence of 131071 tokens, 48 rows, bf16: 151
-// MB, 32 us, 61 here.
+// MB, 32 us, 61 to 65 here.
 //
 // Units of 64 rows: four wavefronts with 16 rows each share a tile.  Units of 16 rows
 // (what one token of 16 heads is): the wavefronts take tiles in turn, each by

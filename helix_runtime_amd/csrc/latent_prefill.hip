@@ -32,8 +32,8 @@
 //   count, by the size of their scores or outputs.
 //
 // What bounds it: 4 x 32 heads, 512 rows over 4096 keys are 161 Gflop, three times
-// that in products of terms: 413 us at the rate of a large fp16 matrix product, 543 here
-// (1300 to 1450 where parts are computed again).  Of a step's 4300 cycles a SIMD's
+// that in products of terms: 413 us at the rate of a large fp16 matrix product, 543 to
+// 558 here (1300 to 1450 where parts are computed again).  Of a step's 4300 cycles a SIMD's
 // matrix instructions take 2080, its other vector instructions 1300; the two of its
 // wavefronts take turns, and what is left are the waits of one for the other at the
 // step's two barriers and the scalar work between tiles.  Steps on the way: three bf16
