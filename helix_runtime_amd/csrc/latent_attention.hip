@@ -818,13 +818,20 @@ struct LatentShared {
   unsigned poison[kWaves];
 };
 
+// A row that has seen nothing has neither sum nor outputs, and is 0.  One all of whose
+// scores are minus infinity has no sum either, but weights of 0 / 0: NaN.  Among
+// partials the latter's reference is the lowest finite number instead of minus
+// infinity, which weighs as little.
+constexpr float kNoWeights = -3.402823466e38f;
+__device__ __forceinline__ float row_factor(float sum, bool some, float f) {
+  return sum != 0.f ? f / sum : some ? NAN : 0.f;
+}
 template <int PF, int L>
 __device__ __forceinline__ float finish_factor(const LatentKernelArgs& a, bool complete, bool bad,
-                                               float sum) {
+                                               float sum, bool some) {
   const float f = PF == 2 ? a.page_scale : 1.0f;
   if (!complete) return f;
-  // (A row that has seen nothing has neither sum nor outputs.)
-  return bad ? NAN : sum == 0.f ? 0.f : f / sum;
+  return bad ? NAN : row_factor(sum, some, f);
 }
 
 template <int PF, int L, bool SHARED>
@@ -1039,7 +1046,8 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       const bool complete = from == 0 && to == cur.nb;
       const int slot = part_of(cur, from);
       const float sum = row_sum(rows.l);
-      const float f = finish_factor<PF, L>(a, complete, bad != 0, sum);
+      const bool some = from * KT < rows.limit;  // of the part's tokens
+      const float f = finish_factor<PF, L>(a, complete, bad != 0, sum, some);
       if (rows.live) {
         const int local = wave * 16 + col;
         float* const dst = (complete ? out_row(cur, row)
@@ -1049,7 +1057,7 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
         for (int dt = 0; dt < R::ND; ++dt) *reinterpret_cast<v4f*>(dst + 16 * dt) = rows.o[dt] * f;
         if (!complete && grp == 0) {
           float* const ml = st.part_ml + (static_cast<std::size_t>(slot) * st.part_rows + local) * 2;
-          ml[0] = rows.m;
+          ml[0] = sum == 0.f && some ? kNoWeights : rows.m;
           ml[1] = bad != 0 ? NAN : sum;
         }
       }
@@ -1140,7 +1148,9 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
       barrier();
       const bool complete = from == 0 && to == cur.nb;
       const int slot = part_of(cur, from);
-      const float f = finish_factor<PF, L>(a, complete, bad != 0, sum);
+      const bool some = from * KT < rows.limit;  // of the part's tokens
+      const float f = finish_factor<PF, L>(a, complete, bad != 0, sum, some);
+      if (sum == 0.f && some) top = kNoWeights;
       // A wavefront adds up four rows, 16 lanes (L / 16 dims each) a row.
       {
         const int local = 4 * wave + grp;
@@ -1311,7 +1321,7 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(LatentKernelArgs a, L
     }
   }
   if (!r.live) return;
-  const float f = sum == 0.f ? 0.f : 1.0f / sum;
+  const float f = row_factor(sum, top != -INFINITY, 1.0f);
   auto* const dst = reinterpret_cast<v4f*>(merge_out(a, job, r));
 #pragma unroll
   for (int v = 0; v < NV; ++v) dst[64 * v + lane] = o[v] * f;
@@ -1381,7 +1391,7 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
   for (int w = 0; w < 8; ++w) sum += total[w];
 #pragma unroll
   for (int k = 1; k < kShares; ++k) o += sums[k][at];
-  *reinterpret_cast<v4f*>(merge_out(a, job, r) + dim) = o * (sum == 0.f ? 0.f : 1.0f / sum);
+  *reinterpret_cast<v4f*>(merge_out(a, job, r) + dim) = o * row_factor(sum, top != -INFINITY, 1.0f);
 }
 
 // ----------------------------------------------------------------- host ----

@@ -98,6 +98,10 @@ constexpr float kSmallOutput = 0x1p-4f;
 // mean, at queries below 2^11, half that in the mean, are 2^-14 of it in the mean, and
 // so 2^-22 of a score.
 constexpr float kLargeScores = 0x1p-8f;
+// The reference of a part of a row that sees keys whose scores are all minus infinity:
+// it weighs as little as a part that sees nothing, but a row of nothing else is NaN, as
+// 0 / 0 is, and not 0.
+constexpr float kNoWeights = -3.402823466e38f;
 
 struct ExpandedKernelArgs {
   const float* query;
@@ -405,6 +409,12 @@ __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const E
   c.left =
       __builtin_amdgcn_readfirstlane(static_cast<int>(max(have - (c.nb + kStart - in), 0ll)));
   return c.to > c.blk;
+}
+
+// What a row's outputs are multiplied by at its end, `f` times the inverse of its sum: 0
+// for one that has seen nothing, and has neither.
+__device__ __forceinline__ float row_factor(float sum, bool some, float f) {
+  return sum != 0.f ? f / sum : some ? NAN : 0.f;
 }
 
 __device__ __forceinline__ std::size_t unit_index(const ExpandedKernelArgs& a,
@@ -997,9 +1007,9 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
         wrong = wrong || (row < cur.count && (nan || lost));
       }
       if (row >= cur.count) continue;
-      // (A row that has seen nothing has neither sum nor outputs.)
+      const bool some = from * kTile < limit[t];  // of the part's keys
       float f = F16 ? value_un : 1.0f;
-      if (complete) f = cur.bad != 0 ? NAN : sum == 0.f ? 0.f : f / sum;
+      if (complete) f = cur.bad != 0 ? NAN : row_factor(sum, some, f);
       float* const dst =
           (complete ? a.out + static_cast<std::size_t>(cur.b) * a.out_at.batch +
                           static_cast<std::size_t>(cur.h) * a.out_at.head +
@@ -1010,7 +1020,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       for (int dt = 0; dt < kDims; ++dt) *reinterpret_cast<v4f*>(dst + 16 * dt) = o[t][dt] * f;
       if (!complete && grp == 0) {
         float* const ml = st.part_ml + (static_cast<std::size_t>(partial) * RB + local) * 2;
-        ml[0] = m[t];
+        ml[0] = sum == 0.f && some ? kNoWeights : m[t];
         ml[1] = cur.bad != 0 ? NAN : sum;
       }
     }
@@ -1114,8 +1124,8 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
   auto slot_of = [&](int i, int row) {
     return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + row;
   };
-  auto finish = [&](int row, const v4f (&o)[2], float sum) {
-    const float f = sum == 0.f ? 0.f : 1.0f / sum;
+  auto finish = [&](int row, const v4f (&o)[2], float sum, float top) {
+    const float f = row_factor(sum, top != -INFINITY, 1.0f);
     auto* const dst = reinterpret_cast<v4f*>(
                           a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
                           static_cast<std::size_t>(job.h) * a.out_at.head +
@@ -1172,7 +1182,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
           o[1] += sums[w][lane][1];
           sum += totals[w][lane >> 4];
         }
-        finish(local, o, sum);
+        finish(local, o, sum, top);
       }
     }
     return;
@@ -1232,7 +1242,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
       }
     }
   }
-  if (live) finish(local, o, sum);
+  if (live) finish(local, o, sum, top);
 }
 
 // ----------------------------------------------------------------- host ----

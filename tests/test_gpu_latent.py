@@ -212,6 +212,29 @@ def test_absorbed_large_scores(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,hq,t", [([3, 40, 700], 16, 4), ([5000], 16, 1), ([100] * 30 + [9000], 20, 2)])
+def test_absorbed_scores_that_are_all_minus_infinity(device, dtype, lengths, hq, t):
+    """Scores of -16 times 6e37 leave 32 bits' range: weights that are 0 / 0, so NaN and
+    not the 0 of a row that sees nothing, in whole units and in parts of one."""
+    p = Latent(dtype, 512, lengths, hq, t, seed=3)
+    p.q[..., 516] = 0
+    want = p.want()
+    p.q *= np.float32(SCALE)
+    p.q[:, ::2, :, 516] = 6e37
+    for i, n in enumerate(lengths):
+        at = torch.arange(n)
+        page = torch.from_numpy(p.tables[i, :(n + P - 1) // P].astype(np.int64))[at // P]
+        # (-416 PS, which fp8 pages hold, is -15.4.)
+        p.pool[page, at % P, 516] = 0xfd if dtype == "fp8" else -16
+    got = p.run(scale=1.0)
+    for i, n in enumerate(lengths):
+        none = max(t - n, 0)
+        assert (got[i, :, :none] == 0).all()
+        assert np.isnan(got[i, ::2, none:]).all()
+        close(got[i, 1::2], want[i, 1::2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_absorbed_bad_lengths_and_pages(device, dtype):
     """A length past the table, a negative one, and a page outside the pool make
     their sequence NaN and leave the others."""
@@ -396,6 +419,22 @@ def test_expanded_later_keys_do_not_reach_earlier_rows(device):
     p.k[0, :, 15:], p.v[0, :, 15:] = -3.4e38, 3.4e38
     got = p.run()
     close(got[:, :, :15], want[:, :, :15])
+
+
+@pytest.mark.parametrize("b,h,t,s", [(1, 2, 20, 300), (2, 1, 30, 20), (4, 40, 130, 140), (1, 1, 20, 3000)])
+def test_expanded_scores_that_are_all_minus_infinity(device, b, h, t, s):
+    """As in the absorbed form: NaN, not the 0 of a row that sees nothing."""
+    p = Expanded(b, h, t, s)
+    p.q[..., 3], p.k[..., 3] = 0, -16
+    want = p.want()
+    p.q *= np.float32(SCALE)
+    p.q[:, :, ::3, 3] = 6e37
+    got = p.run(scale=1.0)
+    none = max(t - s, 0)
+    assert (got[:, :, :none] == 0).all()
+    large = np.arange(t) % 3 == 0
+    assert np.isnan(got[:, :, large & (np.arange(t) >= none)]).all()
+    close(got[:, :, ~large], want[:, :, ~large])
 
 
 def test_expanded_sizes_of_numbers(device):
