@@ -356,7 +356,7 @@ struct LatentRows {
     const float* const src = a.query + static_cast<std::size_t>(c.b) * a.query_at.batch +
                              static_cast<std::size_t>(h) * a.query_at.head +
                              static_cast<std::size_t>(t) * a.query_at.token;
-    m = -INFINITY;
+    m = live ? -INFINITY : INFINITY;  // (a row that is none never moves the others)
     l = 0.f;
     // All of the row's loads at once.  (A row that is none reads the sequence's first
     // one; nothing of what comes of it is kept.)
@@ -523,7 +523,9 @@ struct LatentRows {
     }
   }
 
-  // The reference follows the tile's largest scores.
+  // A row's reference follows the tile's largest score where that is far above it.  (By
+  // the row's own scores alone: no bit of it depends on another row's numbers, which may
+  // be of tokens that it does not see, or of no query at all.)
   __device__ __forceinline__ void follow(const v4f (&sc)[NH]) {
     float mx = -INFINITY;
 #pragma unroll
@@ -532,7 +534,8 @@ struct LatentRows {
     }
     if constexpr (PF == 2) mx *= unscale;
     if (__ballot(mx > m + kSlack) != 0) {
-      const float mn = fmaxf(m, row_max(mx));
+      const float most = row_max(mx);
+      const float mn = most > m + kSlack ? most : m;
       const float alpha = exp2_ratio(m, mn);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {

@@ -703,7 +703,7 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int dt = 0; dt < kDims; ++dt) o[t][dt] = v4f{0.f, 0.f, 0.f, 0.f};
-      m[t] = -INFINITY;
+      m[t] = live ? -INFINITY : INFINITY;  // (a row that is none never moves the others)
       l[t] = 0.f;
     }
   };
@@ -753,7 +753,8 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
       if (u + 2 < 2 * kSteps) read(u + 2);
     }
   };
-  // The reference follows the tile's largest scores.
+  // A row's reference follows the tile's largest score where that is far above it.  (By
+  // the row's own scores alone: no bit of it depends on keys that only others see.)
   auto follow = [&](const v4f (&sc)[RT][2]) {
     float mx[RT];
     bool above = false;
@@ -768,7 +769,8 @@ __device__ __forceinline__ void expanded_range(const ExpandedKernelArgs& a, cons
     if (__ballot(above) != 0) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const float mn = fmaxf(m[t], row_max(mx[t]));
+        const float most = row_max(mx[t]);
+        const float mn = most > m[t] + kSlack ? most : m[t];
         const float alpha = exp2_ratio(m[t], mn);
 #pragma unroll
         for (int dt = 0; dt < kDims; ++dt) o[t][dt] *= alpha;

@@ -646,7 +646,9 @@ int helix_paged_latent_attention(const float* query, const size_t* query_strides
  * Numbers are taken as two fp16 terms of a power of two times them: off by the rounding
  * of a 32-bit number, or by 2^-33 of the largest values of a part's first keys, where
  * that is more.  Query rows whose numbers do not fit, or by their size would lose more,
- * are computed again with three bf16 terms: two and a half times as long in all. */
+ * are computed again with three bf16 terms: two and a half times as long in all.  So are
+ * the up to 127 rows beside them, whose last bits may change (by values past the range
+ * among keys that only some of them see, too). */
 int helix_latent_prefill_workspace_bytes(size_t batch, size_t heads, size_t tokens, size_t keys,
                                          size_t* out);
 int helix_latent_prefill_attention(const float* query, const size_t* query_strides,

@@ -186,6 +186,28 @@ def test_absorbed_later_tokens_do_not_reach_earlier_rows(device, dtype, hq, t):
     assert np.isnan(got[:, :, 1:]).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,t", [(16, 4), (5, 20), (40, 3), (128, 2)])
+def test_absorbed_unseen_numbers_change_no_bit(device, dtype, hq, t):
+    """Queries behind the counts, slots that hold no token, and the step's last token:
+    rows that do not see them are equal bit by bit whatever they hold."""
+    counts = [t, 1, t // 2, t, 2]
+    p = Latent(dtype, 512, [300, 1000, 37, 90, 2100], hq, t, seed=11, counts=counts)
+    got = []
+    for size in (0.0, 1.0, 5.0, 40.0):
+        rng = np.random.default_rng(int(size))
+        some = lambda *s: size * rng.standard_normal(s, dtype=np.float32)  # noqa: E731
+        for i, (n, count) in enumerate(zip(p.lengths, counts)):
+            p.q[i, :, count:] = some(hq, t - count, p.n + ROPE)
+            page, at = int(p.tables[i, (n - 1) // P]), (n - 1) % P
+            p.pool[page, at:] = to_pool(dtype, some(P - at, p.n + ROPE))
+        got.append(p.run())
+    for i, count in enumerate(counts):
+        for other in got[1:]:
+            assert (other[i, :, :count - 1] == got[0][i, :, :count - 1]).all()
+            assert (other[i, :, count:] == 7).all()
+
+
 def test_absorbed_special_queries_stay_in_their_rows(device):
     p = Latent("bf16", 512, [50, 100], 20, 2)
     want = p.want()
@@ -419,6 +441,25 @@ def test_expanded_later_keys_do_not_reach_earlier_rows(device):
     p.k[0, :, 15:], p.v[0, :, 15:] = -3.4e38, 3.4e38
     got = p.run()
     close(got[:, :, :15], want[:, :, :15])
+
+
+@pytest.mark.parametrize("b,h,t,s", [(4, 3, 70, 100), (4, 2, 200, 500), (4, 70, 30, 300)])
+def test_expanded_unseen_numbers_change_no_bit(device, b, h, t, s):
+    """As in the absorbed form, with numbers of a size that no part is computed again
+    for."""
+    counts, lengths = [t, 1, t // 2, t - 1], [s, s - 1, s // 2, 2 * t // 3]
+    p = Expanded(b, h, t, s, counts=counts, lengths=lengths)
+    got = []
+    for size in (0.1, 1.0, 3.0):
+        rng = np.random.default_rng(int(10 * size))
+        for i, (n, count) in enumerate(zip(lengths, counts)):
+            for x in (p.q[i, :, count:], p.k[i, :, n - 1:], p.r[i, n - 1:], p.v[i, :, n - 1:]):
+                x[...] = size * rng.standard_normal(x.shape, dtype=np.float32)
+        got.append(p.run())
+    for i, count in enumerate(counts):
+        for other in got[1:]:
+            assert (other[i, :, :count - 1] == got[0][i, :, :count - 1]).all()
+            assert (other[i, :, count:] == 7).all()
 
 
 @pytest.mark.parametrize("b,h,t,s", [(1, 2, 20, 300), (2, 1, 30, 20), (4, 40, 130, 140), (1, 1, 20, 3000)])
