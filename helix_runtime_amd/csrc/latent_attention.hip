@@ -380,8 +380,9 @@ struct LatentRows {
           most = fmaxf(most, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
         }
       most = row_max(most);
-      // most * 2^(10 - e) in [2^10, 2^11), as far as 2^(10 - e) is a normal number.
-      const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -110), 120);
+      // most * 2^(10 - e) in [2^10, 2^11) for any number, or below for those of less than
+      // 2^-110, as far as 2^(10 - e) is a normal number.
+      const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -110), 127);
       grow = __uint_as_float(static_cast<unsigned>(127 + 10 - e) << 23);
       unscale = __uint_as_float(static_cast<unsigned>(127 - 10 + e) << 23);
       // (Positive, or scores of -infinity would not stay that: the score scale's

@@ -234,6 +234,22 @@ def test_absorbed_large_scores(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_absorbed_largest_queries(device, dtype):
+    """Queries up to fp32's largest numbers, whose scores are of size 1."""
+    p = Latent(dtype, 512, [40, 700, 3000], 16, 1, seed=4)
+    p.q[:] = 0
+    p.q[..., 520] = np.exp2(p.rng.uniform(125, 127.99, p.q.shape[:3]))
+    for i, n in enumerate(p.lengths):
+        at = torch.arange(n)
+        page = torch.from_numpy(p.tables[i, :(n + P - 1) // P].astype(np.int64))[at // P]
+        p.rows[i][:, 520] = p.rng.uniform(-0.25, 0.25, n) * PS
+        p.pool[page, at % P, 520] = to_pool(dtype, p.rows[i][:, 520])
+    got = p.run(scale=1e-36)
+    p.q *= np.float32(1e-36 / SCALE)
+    close(got, p.want())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lengths,hq,t", [([3, 40, 700], 16, 4), ([5000], 16, 1), ([100] * 30 + [9000], 20, 2)])
 def test_absorbed_scores_that_are_all_minus_infinity(device, dtype, lengths, hq, t):
     """Scores of -16 times 6e37 leave 32 bits' range: weights that are 0 / 0, so NaN and
