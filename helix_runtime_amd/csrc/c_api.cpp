@@ -1798,6 +1798,31 @@ void check_tables_clear(const char* op, const RopeRowsArgs& a, const RowsView& o
         op, "outputs must not alias the tables");
 }
 
+// Tables, positions, slots and counts that a call reads lie in nothing that it writes,
+// its rows and its pools (`pool` bytes each): other workgroups read them meanwhile.
+void check_reads_apart(const char* op, const RopeRowsArgs& a, std::size_t pool) {
+  const std::size_t tables = mul(mul(a.table_rows, a.pairs), sizeof(float));
+  const std::size_t rows = mul(a.batch, a.tokens);
+  const struct {
+    const void* p;
+    std::size_t bytes;
+  } reads[] = {{a.cosine, tables},
+               {a.sine, tables},
+               {a.positions, mul(rows, sizeof(std::int32_t))},
+               {a.starts, mul(a.batch, sizeof(std::int32_t))},
+               {a.token_counts, mul(a.batch, sizeof(std::int32_t))},
+               {a.slots, mul(rows, sizeof(std::int64_t))}};
+  for (int i = 0; i < a.count; ++i) {
+    const helix::hip::RopeStream& s = a.streams[i];
+    const RowsView out{s.out, s.out_at, a.batch, s.heads, a.tokens, s.dim};
+    for (const auto& r : reads) {
+      check(clear_of(out, r.p, r.bytes) && !overlap(s.pool, pool, r.p, r.bytes),
+            Status::kInvalidArgument, op,
+            "outputs and pools must not alias tables, positions, starts, slots or counts");
+    }
+  }
+}
+
 void check_pool(const char* op, std::size_t physical_blocks, std::size_t block_tokens) {
   check(physical_blocks != 0 && physical_blocks <= std::numeric_limits<std::uint32_t>::max(),
         Status::kInvalidArgument, op, "physical block count out of range");
@@ -1944,6 +1969,7 @@ int helix_rope_rows(const float* input, const size_t* input_strides, float* outp
     a.positions = positions;
     a.inverse = inverse != 0;
     a.streams[a.count++] = rope_stream(in, out, rotary_dim);
+    check_reads_apart(op, a, 0);
     check(helix::hip::rope_rows_fit(a), Status::kOutOfRange, op, "too many elements for one launch");
     helix::hip_check(helix::hip::launch_rope_rows(a, as_stream(stream)), op);
   });
@@ -1996,6 +2022,7 @@ int helix_paged_rope_append(const float* query, const size_t* query_strides, con
     a.token_counts = token_counts;
     a.physical_blocks = physical_blocks;
     a.block_tokens = block_tokens;
+    check_reads_apart(op, a, pool);
     helix::hip_check(helix::hip::launch_rope_rows(a, as_stream(stream)), op);
   });
 }
@@ -2055,6 +2082,7 @@ int helix_paged_latent_append(const float* latent_rows, const size_t* latent_str
     a.token_counts = token_counts;
     a.physical_blocks = physical_blocks;
     a.block_tokens = block_tokens;
+    check_reads_apart(op, a, pool);
     helix::hip_check(helix::hip::launch_rope_rows(a, as_stream(stream)), op);
   });
 }

@@ -545,8 +545,8 @@ int helix_rope_tables(float* cosine, float* sine, size_t rows, size_t first_posi
 /* In the calls from here on, rows are fp32 [batch, heads, tokens, dim] with strides
  * in elements for the first three, {batch, head, token}, so that a projection's
  * output can be given as it lies; strides NULL: contiguous.  The last dimension is
- * contiguous.  Rows that are written must not share elements with each other or with
- * other rows of the call; an output may be its own input.  Rows of four-element
+ * contiguous.  Rows and pages that are written must not share elements with each other
+ * or with anything else of the call; an output may be its own input.  Rows of four-element
  * groups that lie on 16 bytes are moved 16 bytes at a time, others element by
  * element.
  *

@@ -226,6 +226,43 @@ def test_workspace_sizes():
             call()
 
 
+@pytest.mark.parametrize("at", [8 * MB - 12, 8 * MB, 8 * MB + 6140])
+def test_rows_positions_apart(at):
+    """Positions (four) in the output (4 x 3 x 128 numbers)."""
+    lib = hx.load()
+    refused(lib, rows(lib, pos=at), hx.INVALID_ARGUMENT, b"positions")
+
+
+# What rope_append writes: query rows, key rows, value rows and both pools.
+@pytest.mark.parametrize("at", [64 * MB + 4096, 80 * MB + 128, 90 * MB + 128, 128 * MB + 512, 256 * MB + 512])
+@pytest.mark.parametrize("what", [("slots", b"slots"), ("starts", b"starts"), ("counts", b"counts"),
+                                  ("cos", b"tables"), ("sin", b"tables")])
+def test_append_indexes_apart(what, at):
+    lib = hx.load()
+    index = {"slots": 512 * MB, "starts": 513 * MB, "counts": 516 * MB, "cos": 514 * MB, "sin": 515 * MB,
+             what[0]: at}
+    rc = lib.helix_paged_rope_append(
+        MB, None, 16 * MB, None, 32 * MB, None, 64 * MB, None, 80 * MB, None, 90 * MB, None, 2, 32, 8, 10,
+        128, 128 * MB, 256 * MB, 100, 16, index["slots"], index["starts"], index["counts"], index["cos"],
+        index["sin"], 10, 128, 1, 1, 1.0, 1.0, None)
+    refused(lib, rc, hx.INVALID_ARGUMENT, what[1])
+
+
+# And latent_append: query rows, and the pages (100 of 16 x 576 numbers).
+@pytest.mark.parametrize("at", [16 * MB + 4096, 64 * MB + 100 * 16 * 576 * 4 - 16])
+@pytest.mark.parametrize("what", [("slots", b"slots"), ("starts", b"starts"), ("counts", b"counts"),
+                                  ("cos", b"tables"), ("sin", b"tables")])
+def test_latent_append_indexes_apart(what, at):
+    lib = hx.load()
+    index = {"slots": 512 * MB, "starts": 513 * MB, "counts": 516 * MB, "cos": 514 * MB, "sin": 515 * MB,
+             what[0]: at}
+    rc = lib.helix_paged_latent_append(
+        MB, None, 2 * MB, None, 4 * MB, None, 16 * MB, strides(16 * 10 * 576, 10 * 576, 576), 2, 16, 10, 512,
+        64 * MB, 100, 16, index["slots"], index["starts"], index["counts"], index["cos"], index["sin"], 10,
+        0, 0, 1.0, None)
+    refused(lib, rc, hx.INVALID_ARGUMENT, what[1])
+
+
 # ---------------------------------------------------------- Python checks ----
 def wrong(call, text):
     with pytest.raises(hx.HelixError) as e:
