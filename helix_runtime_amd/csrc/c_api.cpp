@@ -2240,11 +2240,26 @@ int helix_decode_batch_rope_append_layer(
     constexpr const char* op = "decode batch rope append";
     check(b != nullptr, Status::kInvalidArgument, "decode batch must not be NULL");
     b->batch->require_ordinary_step(op);
-    const RopeRowsArgs a = rope_append_args(
+    RopeRowsArgs a = rope_append_args(
         op, query, query_strides, keys, key_strides, values, value_strides, query_out,
         query_out_strides, key_out, key_out_strides, value_out, value_out_strides,
         b->batch->batch(), b->batch->q_heads(), b->batch->kv_heads(), b->batch->step_tokens(),
         b->batch->head_dim(), cosine, sine, cache_rows, rotary_dim, layout);
+    a.slots = b->batch->slots();
+    a.starts = b->batch->lengths();
+    check_reads_apart(op, a, 0);
+    auto clear = [&](const RowsView& v) {
+      return v.empty() || !b->batch->overlaps_pool(v.p, v.span() * sizeof(float));
+    };
+    const std::size_t tables = mul(mul(a.table_rows, a.pairs), sizeof(float));
+    check(!b->batch->overlaps_pool(a.cosine, tables) && !b->batch->overlaps_pool(a.sine, tables),
+          Status::kInvalidArgument, op, "tables must not lie in the pools");
+    for (int i = 0; i < a.count; ++i) {
+      const helix::hip::RopeStream& s = a.streams[i];
+      check(clear(RowsView{s.in, s.in_at, a.batch, s.heads, a.tokens, s.dim}) &&
+                clear(RowsView{s.out, s.out_at, a.batch, s.heads, a.tokens, s.dim}),
+            Status::kInvalidArgument, op, "rows must not lie in the pools");
+    }
     b->batch->rope_append_layer(layer, a, as_stream(stream));
   });
 }

@@ -750,8 +750,6 @@ void DecodeBatch::rope_append_layer(std::size_t layer, hip::RopeRowsArgs a,
   values.scale = state_->page_type.v_scale;
   keys.pool_row = values.pool_row = c.head_dimension;
   a.page_type = state_->page_type.type;
-  a.slots = slots();
-  a.starts = lengths();
   a.physical_blocks = c.physical_blocks;
   a.block_tokens = c.block_tokens;
   hip_check(hip::launch_rope_rows(a, stream), "decode batch rope append launch");

@@ -209,8 +209,9 @@ public:
   void rope(float* query, float* key, const float* cosine, const float* sine,
             std::size_t cache_rows, hipStream_t stream) const;
   // rope() and append_layer() in one launch, for chunk steps too: rows of `a`
-  // (its streams: queries if any, keys, values) turned from each sequence's
-  // length before the step on, keys and values to the step's slots.
+  // (its streams: queries if any, keys, values, clear of the pools; slots() and
+  // lengths()) turned from each sequence's length before the step on, keys and values
+  // to the step's slots.
   void rope_append_layer(std::size_t layer, hip::RopeRowsArgs a, hipStream_t stream) const;
   void attention_layer(std::size_t layer, const float* query, const float* tail_key,
                        const float* tail_value, float* out, hipStream_t stream,
@@ -260,6 +261,9 @@ public:
     return state_->manager.config().head_dimension;
   }
   [[nodiscard]] std::size_t step_tokens() const noexcept { return step_tokens_; }
+  [[nodiscard]] bool overlaps_pool(const void* p, std::size_t bytes) const {
+    return state_->overlaps_pool(p, bytes);
+  }
   [[nodiscard]] std::size_t shared_pages() const noexcept { return shared_pages_; }
   // Measurement hook: when set, attention_layer() records this event between
   // the main decode kernel and the merge kernel.

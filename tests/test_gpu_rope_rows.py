@@ -3,6 +3,8 @@ bit against the formula with every product and sum rounded to fp32, in both
 layouts, over all of a head or a part, strided, in place, ragged, on every page
 type, alone and as a step of DecodeBatch."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -392,6 +394,41 @@ def test_a_tree_step_refuses_the_call(device):
     with pytest.raises(hx.HelixError) as e:
         batch.rope_append_layer(0, x, x.clone(), x.clone(), cos, sin, x)
     assert "tree step" in str(e.value)
+    batch.close()
+    cache.close()
+
+
+def test_a_step_refuses_rows_in_its_own_memory(device):
+    """Rows and tables in the cache's pages (of any layer), outputs on the step's lengths
+    or slots."""
+    lib = hx.load()
+    cache = hx.PagedKvCache(2, 2, 128, 16, 16)
+    batch = hx.DecodeBatch(cache, [cache.create_sequence()], 4, 64)
+    batch.prepare()
+    x = torch.zeros(3, 1, 4, 1, 128, device="cuda:0")
+    out = torch.zeros_like(x)
+    cos, sin = (torch.ones(64, 64, device="cuda:0") for _ in range(2))
+    tables, lengths, slots = (ctypes.c_void_p() for _ in range(3))
+    hx.check(lib.helix_decode_batch_tables(batch._h, *(ctypes.byref(p) for p in (tables, lengths, slots)),
+                                           None, None))
+    good = [x[0].data_ptr(), x[1].data_ptr(), x[2].data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
+            out[2].data_ptr(), cos.data_ptr(), sin.data_ptr()]
+
+    def call(rows):
+        args = [a for p in rows[:6] for a in (p, None)]
+        return lib.helix_decode_batch_rope_append_layer(batch._h, 0, *args, *rows[6:], 64, 128, 0, None)
+
+    assert call(good) == 0
+    torch.cuda.synchronize()
+    before = [[host(p) for p in cache.layer_pools(layer)] for layer in range(2)]
+    for i in range(8):
+        inside = [p for layer in range(2) for p in cache.layer_pool_pointers(layer)]
+        for at in inside + ([lengths.value, slots.value] if 3 <= i < 6 else []):
+            assert call(good[:i] + [at] + good[i + 1:]) == hx.INVALID_ARGUMENT
+            assert b"alias" in lib.helix_last_error() or b"pools" in lib.helix_last_error()
+    for layer in range(2):
+        for p, q in zip(before[layer], cache.layer_pools(layer)):
+            assert (p == host(q)).all()
     batch.close()
     cache.close()
 
