@@ -7,15 +7,15 @@
 //
 // Work split.  16 or 64 of a sequence's rows form a unit; one pass over the
 // sequence's tokens serves them all.  A unit's tokens are tiles of 32 (fp32 pages:
-// 16).  A fixed grid of workgroups takes equal ranges of the flat list of all units'
-// tiles, whatever the lengths (and of what units cost beside their tiles).  A unit
+// 16).  A row block's units of all sequences are a flat list of tiles (and of what units
+// cost beside them), of which its share of a fixed grid of workgroups takes equal
+// ranges, whatever the lengths; more than 32 row blocks have one list.  A unit
 // inside one range is finished there; one that crosses ranges leaves a partial
 // (maximum, sum, output) per range, which latent_merge_kernel joins.  A workgroup
 // leaves at most two partials, its first unit's and its last one's, so the workspace
-// depends on the grid, not on the batch.  Each row block has its own share of the
-// workgroups, a multiple of the XCDs: those that read the same pages do so at one time,
-// on one XCD.  (One sequence of 131071 tokens, 64 rows in units of 16: 104 us with one
-// list for all row blocks, 65 so.)
+// depends on the grid, not on the batch.  Row blocks read the same pages at one time
+// so, and as far as latent_share() says on one XCD.  (One sequence of 131071 tokens, 64
+// rows in units of 16: 104 us with one list for all row blocks, 65 so.)
 //
 // Matrix form.  Per tile scores are S^T = C Q^T and outputs O^T += C^T P^T, a
 // wavefront having 16 rows: a lane holds tokens of one query row, so a row's maximum
@@ -1513,8 +1513,7 @@ hipError_t launch_latent_attention(const LatentArgs& a, hipStream_t stream) {
   const std::size_t rb = unit_rows(a), row_blocks = (a.q_heads * a.tokens + rb - 1) / rb;
   st.part_rows = rb == 16 || a.q_heads * a.tokens <= 16 ? 16 : 64;
   st.row_blocks = static_cast<int>(row_blocks);
-  const int share = static_cast<int>(kGroups / row_blocks);
-  st.share = row_blocks > 1 ? share / kXcds * kXcds : 0;
+  st.share = static_cast<int>(latent_share(kGroups, row_blocks));
   st.by_unit = a.batch * row_blocks <= kGroups ? 1 : 0;
   switch (a.page_type) {
     case PageType::kBF16: return launch_page_type<1>(k, st, rb, a.latent, stream);
