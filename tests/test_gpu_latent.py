@@ -340,6 +340,23 @@ def test_absorbed_many_sequences(device, dtype, hq, t):
     close(p.run(), p.want())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,hq,t", [([300, 50, 700, 33], 128, 20), ([300, 50, 1700, 33], 64, 9),
+                                          ([90, 200, 0, 1000], 64, 17), ([700, 3], 16, 40), ([2000, 30], 16, 17),
+                                          ([5000], 20, 54)])
+def test_absorbed_many_row_blocks(device, dtype, lengths, hq, t):
+    """9 to 80 units of a sequence, with one list of tiles for all of them and with one
+    each, ragged, sequences without rows among them."""
+    counts = [t, 0, t // 3, t + 1][:len(lengths)]
+    p = Latent(dtype, 512, lengths, hq, t, seed=13, counts=counts)
+    got = p.run()
+    heads = sorted({0, 1, hq // 3, hq - 2, hq - 1})
+    p.q, p.hq = p.q[:, heads], len(heads)
+    close(got[:, heads], p.want())
+    for i, count in enumerate(counts):
+        assert (got[i, :, min(count, t):] == 7).all() and np.isfinite(got[i]).all()
+
+
 def test_absorbed_pools_past_32_bits(device):
     """Pages whose elements lie past 2^32 of the pool."""
     n = (1 << 32) // (P * 576) + 40
@@ -643,6 +660,21 @@ def test_expanded_heads_that_no_number_divides(device, b, h, t, s):
 def test_expanded_few_units_in_many_parts(device, b, h, t, s):
     p = Expanded(b, h, t, s)
     close(p.run(), p.want())
+
+
+@pytest.mark.parametrize("h,t,s", [(1, 8300, 8400), (9, 8250, 17000), (2, 8200, 300)])
+def test_expanded_many_row_blocks(device, h, t, s):
+    """More than 64 units of a head, whose heads take turns in the second case: sampled
+    rows."""
+    p = Expanded(1, h, t, s)
+    got = p.run()
+    assert np.isfinite(got).all()
+    for head in {0, h // 2, h - 1}:
+        key = np.concatenate([p.k[0, head], p.r[0]], axis=-1).astype(np.float64)
+        for row in [0, 1, 127, 128, 4000, 8000, 8063, 8064, 8191, 8192, t - 2, t - 1]:
+            n = max(s - t + row + 1, 0)
+            x = (p.q[0, head, row].astype(np.float64) @ key[:n].T * SCALE)[None]
+            close(got[0, head, row], ref.softmax_sum(x, p.v[0, head, :n].astype(np.float64))[0])
 
 
 def test_expanded_one_long_sequence_among_many(device):
