@@ -914,8 +914,8 @@ def _rope_cache(cosine, sine, rotary_dim, device):
 def rope_tables(cosine, sine, base=10000.0, first_position=0, scaling="none", factor=1.0,
                 original_length=0, low=None, high=None, amplitude=1.0, stream=None):
     """Fill cosine and sine [rows, rotary_dim / 2] for positions first_position on:
-    amplitude * cos and sin of position * base^(-2 i / rotary_dim), in 64 bits,
-    rounded once.  scaling changes the frequencies for contexts longer than
+    amplitude * cos and sin of position * base^(-2 i / rotary_dim), in 64 bits (angles
+    are off by position * 2^-50 at most), rounded once.  scaling changes the frequencies for contexts longer than
     original_length, the one a model was trained on: "linear" (divided by factor),
     "ntk" (a larger base), "ramp" (divided where a wave turns at most `low` times
     over the original length, as they are from `high` turns on, a mean between,

@@ -534,8 +534,10 @@ typedef enum helix_rope_scaling {
 
 /* Tables for helix_rope and the calls below: row r of cosine and sine [rows,
  * rotary_dim / 2] holds amplitude * cos and sin of (first_position + r) f_i,
- * computed in 64 bits and rounded once.  base > 1, factor >= 1, positions below
- * 2^31, amplitude finite; original_length > 0 and 0 < low < high for RAMP and BANDS,
+ * computed in 64 bits and rounded once: angles are off by position * 2^-50 at most (BANDS
+ * with high at least twice low: 2^-48), which at 2^20 is a thirty-second of the rounding of
+ * values near 1, and at 2^25 as much as it.  base > 1, factor >= 1, positions below 2^31,
+ * amplitude finite; original_length > 0 and 0 < low < high for RAMP and BANDS,
  * rotary_dim > 2 for NTK. */
 int helix_rope_tables(float* cosine, float* sine, size_t rows, size_t first_position,
                       size_t rotary_dim, double base, int scaling, double factor,

@@ -4,6 +4,7 @@ layouts, over all of a head or a part, strided, in place, ragged, on every page
 type, alone and as a step of DecodeBatch."""
 
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -83,6 +84,50 @@ def test_tables(device, scaling, rows, rotary, first):
     for got, exact in zip((cos, sin), want):
         exact = exact * amplitude
         assert (np.abs(host(got) - exact) <= 2.0 ** -24 * np.abs(exact) + tol).all()
+
+
+def wide_frequencies(rotary, base, scaling="none", factor=1.0, original_length=0):
+    wide = np.longdouble
+    i = np.arange(rotary // 2, dtype=wide)
+    f = wide(base) ** (-2 * i / rotary)
+    if scaling == "linear":
+        return f / factor
+    if scaling == "ntk":
+        return f * wide(factor) ** (-2 * i / (rotary - 2))
+    if scaling == "ramp":
+        def pair(turns):
+            return rotary * math.log(original_length / (2 * math.pi * turns)) / (2 * math.log(base))
+        a, b = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), rotary - 1)
+        w = np.clip((i - a) / max(b - a, 0.001), 0, 1)
+        return (1 - w) * f + w * f / factor
+    if scaling == "bands":
+        w = np.clip((original_length * f / (2 * np.arccos(wide(-1))) - 1) / 3, 0, 1)
+        return (1 - w) * f / factor + w * f
+    return f
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(), dict(scaling="linear", factor=3.0), dict(scaling="ntk", factor=7.0),
+    dict(scaling="ramp", factor=5.0, original_length=4096), dict(scaling="bands", factor=7.0, original_length=8192)])
+@pytest.mark.parametrize("rotary", [4, 64, 128, 250])
+@pytest.mark.parametrize("base", [1.5, 10000.0, 1e6])
+def test_tables_against_wider_numbers(device, scaling, rotary, base):
+    """Against angles of 64-bit mantissas (off by position * 2^-60 at most): one rounding,
+    and angles that are off by position * 2^-50 (bands: 2^-48)."""
+    if np.finfo(np.longdouble).nmant < 63:
+        pytest.skip("no wider numbers here")
+    f = wide_frequencies(rotary, base, **scaling)
+    share = 2.0 ** -48 if scaling.get("scaling") == "bands" else 2.0 ** -50
+    for last in (1, 2**17, 2**20, 2**24, 2**31):
+        first = max(last - 40, 0)
+        cos, sin = (torch.empty(last - first, rotary // 2, device="cuda:0") for _ in range(2))
+        hx.rope_tables(cos, sin, base=base, first_position=first, **scaling)
+        angles = np.arange(first, last, dtype=np.longdouble)[:, None] * f
+        for got, exact in zip((cos, sin), (np.cos(angles), np.sin(angles))):
+            off = np.abs(host(got) - exact)
+            # (Rounded to the nearest: half a step of what lies below the next power of two.)
+            step = np.exp2(np.floor(np.log2(np.maximum(np.abs(exact), 2.0 ** -126))) - 24)
+            assert (off <= step + share * last + 2.0 ** -45).all()
 
 
 def test_tables_are_what_the_rotation_takes(device):
