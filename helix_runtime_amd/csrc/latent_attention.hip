@@ -46,6 +46,7 @@
 #include "bf16.hpp"
 #include "fp8.hpp"
 #include "latent.hpp"
+#include "latent_detail.hpp"
 #include "prefill_bmma.hpp"
 
 #include <hip/hip_runtime.h>
@@ -58,6 +59,15 @@
 namespace helix::hip {
 namespace {
 
+using latent_detail::align256;
+using latent_detail::clamped_count;
+using latent_detail::divide;
+using latent_detail::kNoWeights;
+using latent_detail::lane_scan;
+using latent_detail::matrix_step;
+using latent_detail::row_factor;
+using latent_detail::uniform_long;
+using latent_detail::v4u;
 using prefill_detail::exp2_ratio;
 using prefill_detail::lds_address;
 using prefill_detail::lds_load16_at;
@@ -66,13 +76,10 @@ using prefill_detail::row_sum;
 using prefill_detail::uniform_read;
 using prefill_detail::v4f;
 using prefill_detail::v4s;
-using prefill_detail::v8bf;
 
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
-typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
@@ -131,17 +138,6 @@ __device__ __forceinline__ unsigned next_term(float& x, float& y) {
     x -= __uint_as_float(t << 16);
     y -= __uint_as_float(t & 0xffff0000u);
     return t;
-  }
-}
-
-template <int PF>
-__device__ __forceinline__ v4f matrix_step(v4u a, v4u b, v4f c) {
-  if constexpr (PF == 2) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
-                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
-                                                   __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   }
 }
 
@@ -205,10 +201,6 @@ struct LatentCursor {
   int bad;                // its length lies outside its table
 };
 
-__device__ __forceinline__ int clamped_count(const LatentKernelArgs& a, int b) {
-  return a.token_counts != nullptr ? min(max(a.token_counts[b], 0), a.tokens) : a.tokens;
-}
-
 // Tiles of sequence b: one at least where it has rows.
 template <int KT>
 __device__ __forceinline__ int sequence_tiles(const LatentKernelArgs& a, int b) {
@@ -226,30 +218,6 @@ __device__ __forceinline__ void load_sequence(const LatentKernelArgs& a, LatentC
   c.count = a.tokens;
   if (a.token_counts != nullptr) c.count = min(max(uniform_read(a.token_counts + c.b), 0), a.tokens);
   c.nb = c.count > 0 ? max((c.length + KT - 1) / KT, 1) : 0;
-}
-
-__device__ __forceinline__ long long uniform_long(long long v) {
-  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
-  const unsigned hi =
-      __builtin_amdgcn_readfirstlane(static_cast<unsigned>(static_cast<unsigned long long>(v) >> 32));
-  return static_cast<long long>(static_cast<unsigned long long>(hi) << 32 | lo);
-}
-
-// Inclusive sums over the wavefront.
-__device__ __forceinline__ long long lane_scan(long long v, int lane) {
-  long long sum = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long t = __shfl_up(sum, o, 64);
-    if (lane >= o) sum += t;
-  }
-  return sum;
-}
-
-__device__ __forceinline__ long long divide(long long n, long long d) {
-  // (A 64-bit division takes ten times a 32-bit one.)
-  if ((n | d) >> 31 == 0) return static_cast<unsigned>(n) / static_cast<unsigned>(d);
-  return n / d;
 }
 
 // This group's first place, of ranges of `each` places; whether it has a tile.
@@ -506,7 +474,7 @@ struct LatentRows {
             // (Sums of the smaller terms' products by themselves: the rounding of the
             // larger ones' is then that of a third, or half, as many.)
             v4f& sum = i == 0 ? sc[h] : low[h];
-            sum = matrix_step<PF>(k[h], q[s][i], sum);
+            sum = matrix_step<PF == 2>(k[h], q[s][i], sum);
             const int at_step = NH * (QT - 1 - i) + h;
             if (kSpread && at_step % 2 == 1 && at_step / 2 < NH && s + A < NS) read_half(s + A, at_step / 2);
             if (kSpread || h == NH - 1) beside(NH * QT * s + at_step);
@@ -684,7 +652,7 @@ struct LatentRows {
         for (int i = QT - 1; i >= 0; --i)
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
-            o[dt + d] = matrix_step<PF>(v[d], pop[i], o[dt + d]);
+            o[dt + d] = matrix_step<PF == 2>(v[d], pop[i], o[dt + d]);
             const int at_step = 2 * (QT - 1 - i) + d;
             if (kSpread && at_step < 4 && dt + A < ND) read_part(dt + A + at_step / 2, at_step % 2);
             if (kSpread) __builtin_amdgcn_sched_barrier(0);
@@ -822,14 +790,6 @@ struct LatentShared {
   unsigned poison[kWaves];
 };
 
-// A row that has seen nothing has neither sum nor outputs, and is 0.  One all of whose
-// scores are minus infinity has no sum either, but weights of 0 / 0: NaN.  Among
-// partials the latter's reference is the lowest finite number instead of minus
-// infinity, which weighs as little.
-constexpr float kNoWeights = -3.402823466e38f;
-__device__ __forceinline__ float row_factor(float sum, bool some, float f) {
-  return sum != 0.f ? f / sum : some ? NAN : 0.f;
-}
 template <int PF, int L>
 __device__ __forceinline__ float finish_factor(const LatentKernelArgs& a, bool complete, bool bad,
                                                float sum, bool some) {
@@ -1419,8 +1379,6 @@ std::size_t unit_rows(const LatentArgs& a) {
   if (tiles <= kGroups) return 64;
   return rows <= 32 || (a.page_type == PageType::kFP8 && units <= kGroups) ? 16 : 64;
 }
-
-std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
 
 // Room for units of 64 rows, where there are as many.
 struct LatentLayout {

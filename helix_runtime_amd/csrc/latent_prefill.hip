@@ -42,6 +42,7 @@
 // scalar bases 584; heads woven 543.
 #include "bf16.hpp"
 #include "latent.hpp"
+#include "latent_detail.hpp"
 #include "prefill_bmma.hpp"
 
 #include <hip/hip_runtime.h>
@@ -54,19 +55,25 @@
 namespace helix::hip {
 namespace {
 
+using latent_detail::align256;
+using latent_detail::clamped_count;
+using latent_detail::divide;
+using latent_detail::kNoWeights;
+using latent_detail::lane_scan;
+using latent_detail::matrix_step;
+using latent_detail::row_factor;
+using latent_detail::uniform_long;
+using latent_detail::v4u;
 using prefill_detail::exp2_ratio;
 using prefill_detail::row_max;
 using prefill_detail::row_sum;
 using prefill_detail::uniform_read;
 using prefill_detail::v4f;
 using prefill_detail::v4s;
-using prefill_detail::v8bf;
 
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
-typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -98,10 +105,6 @@ constexpr float kSmallOutput = 0x1p-4f;
 // mean, at queries below 2^11, half that in the mean, are 2^-14 of it in the mean, and
 // so 2^-22 of a score.
 constexpr float kLargeScores = 0x1p-8f;
-// The reference of a part of a row that sees keys whose scores are all minus infinity:
-// it weighs as little as a part that sees nothing, but a row of nothing else is NaN, as
-// 0 / 0 is, and not 0.
-constexpr float kNoWeights = -3.402823466e38f;
 
 struct ExpandedKernelArgs {
   const float* query;
@@ -186,17 +189,6 @@ __device__ __forceinline__ void next_term(float& x, float& y, int n, unsigned* w
   }
 }
 
-template <bool F16>
-__device__ __forceinline__ v4f matrix_step(v4u a, v4u b, v4f c) {
-  if constexpr (F16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
-                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
-                                                   __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-  }
-}
-
 // The power of two that puts `most` into [2^to, 2^(to + 1)), as far as it is a normal
 // number (1 for 0), and what undoes it.
 __device__ __forceinline__ float grow_to(float most, int to, float& unscale) {
@@ -251,10 +243,6 @@ struct ExpandedCursor {
   int bad;                // the length lies outside [0, keys]
 };
 
-__device__ __forceinline__ int clamped_count(const ExpandedKernelArgs& a, int b) {
-  return a.token_counts != nullptr ? min(max(a.token_counts[b], 0), a.tokens) : a.tokens;
-}
-
 // Tiles of a unit of sequence b: one at least where it has rows.
 template <int RB>
 __device__ __forceinline__ int unit_tiles(int length, int count, int rb) {
@@ -262,12 +250,6 @@ __device__ __forceinline__ int unit_tiles(int length, int count, int rb) {
   if (row0 >= count) return 0;
   const int sees = length - count + min(count, row0 + RB);
   return max((sees + kTile - 1) / kTile, 1);
-}
-
-__device__ __forceinline__ long long divide(long long n, long long d) {
-  // (A 64-bit division takes ten times a 32-bit one.)
-  if ((n | d) >> 31 == 0) return static_cast<unsigned>(n) / static_cast<unsigned>(d);
-  return n / d;
 }
 
 // Places of a sequence's row blocks, for each head: the sum over them of unit_tiles and
@@ -313,24 +295,6 @@ __device__ __forceinline__ void load_unit(const ExpandedKernelArgs& a, ExpandedC
   c.count = a.tokens;
   if (a.token_counts != nullptr) c.count = min(max(uniform_read(a.token_counts + c.b), 0), a.tokens);
   set_unit<RB>(c);
-}
-
-__device__ __forceinline__ long long uniform_long(long long v) {
-  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
-  const unsigned hi =
-      __builtin_amdgcn_readfirstlane(static_cast<unsigned>(static_cast<unsigned long long>(v) >> 32));
-  return static_cast<long long>(static_cast<unsigned long long>(hi) << 32 | lo);
-}
-
-// Inclusive sums over the wavefront.
-__device__ __forceinline__ long long lane_scan(long long v, int lane) {
-  long long sum = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long t = __shfl_up(sum, o, 64);
-    if (lane >= o) sum += t;
-  }
-  return sum;
 }
 
 // The range of a workgroup: consecutive ones go to an XCD, which has every eighth
@@ -409,12 +373,6 @@ __device__ __forceinline__ bool first_place(const ExpandedKernelArgs& a, const E
   c.left =
       __builtin_amdgcn_readfirstlane(static_cast<int>(max(have - (c.nb + kStart - in), 0ll)));
   return c.to > c.blk;
-}
-
-// What a row's outputs are multiplied by at its end, `f` times the inverse of its sum: 0
-// for one that has seen nothing, and has neither.
-__device__ __forceinline__ float row_factor(float sum, bool some, float f) {
-  return sum != 0.f ? f / sum : some ? NAN : 0.f;
 }
 
 __device__ __forceinline__ std::size_t unit_index(const ExpandedKernelArgs& a,
@@ -1249,8 +1207,6 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
 
 // ----------------------------------------------------------------- host ----
 constexpr std::size_t kGroups = 256;  // a workgroup a CU: a wavefront a SIMD, for its registers
-
-std::size_t align256(std::size_t n) { return (n + 255) & ~std::size_t{255}; }
 
 // Units of 64 rows (four wavefronts) where there are no more: 16 x 16 heads, 64 rows
 // over 2048 keys take 131 us, in units of 128 168; 512 rows over 4096 keys take 574 in
