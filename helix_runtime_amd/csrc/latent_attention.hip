@@ -968,7 +968,8 @@ __device__ __forceinline__ void latent_body(const LatentKernelArgs& a, const Lat
 #pragma unroll
           for (int bit = 16; bit < 64; bit *= 2) poison |= __shfl_xor(poison, bit, 64);
           if (lane == 0) sh.poison[wave] = poison;
-          // (Every wavefront took its scores of the tile a step ago.)
+          // (Of a unit's first tile other wavefronts may be taking scores still: those of
+          // rows that are wiped meanwhile are ones that mask() replaces.)
           barrier();
           poison = sh.poison[0] | sh.poison[1] | sh.poison[2] | sh.poison[3];
           rows.mask(blk * KT, poison, grp, sc);

@@ -1209,8 +1209,8 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
 constexpr std::size_t kGroups = 256;  // a workgroup a CU: a wavefront a SIMD, for its registers
 
 // Units of 64 rows (four wavefronts) where there are no more: 16 x 16 heads, 64 rows
-// over 2048 keys take 131 us, in units of 128 168; 512 rows over 4096 keys take 574 in
-// units of 128, 864 in units of 64, whose keys are split twice as often.
+// over 2048 keys take 134 us, in units of 128 152; 4 x 32 heads, 512 rows over 4096 keys
+// take 545 in units of 128, 850 in units of 64, whose keys are split twice as often.
 struct ExpandedLayout {
   ExpandedLayout(std::size_t batch, std::size_t heads, std::size_t tokens) {
     rb = tokens <= 64 ? 64 : 128;
