@@ -473,7 +473,7 @@ def test_a_step_refuses_rows_in_its_own_memory(device):
             assert b"alias" in lib.helix_last_error() or b"pools" in lib.helix_last_error()
     for layer in range(2):
         for p, q in zip(before[layer], cache.layer_pools(layer)):
-            assert (p == host(q)).all()
+            same_bits(p, host(q))  # (pages that hold nothing yet hold anything)
     batch.close()
     cache.close()
 
