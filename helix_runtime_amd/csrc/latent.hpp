@@ -46,14 +46,17 @@ struct LatentArgs {
 // Workgroups of each of the `row_blocks` units of a sequence, or 0: none of its own, all
 // of them for one list.  A multiple of the XCDs keeps those that read the same pages at
 // one time on one XCD (one sequence of 32768 tokens, bf16, three row blocks of 64: 52 us
-// so, 54 with shares of 85, 57 with one list), unless more than a sixteenth of them would
-// have nothing to do: 17 row blocks of 16 sequences of 2048 tokens, bf16, take 285 us on
-// 136 workgroups and 188 on 255, 9 of them 121 and 113, 11 row blocks of 16 rows over 65536
-// tokens, fp8, 82 and 68 (with one list 195, 116 and 80).
+// so, 54 with shares of 85, 57 with one list), unless more than three sixteenths of them
+// would have nothing to do.  17 row blocks of 16 sequences of 2048 tokens, bf16, take 285 us
+// on 136 workgroups and 188 on 255; 11 row blocks of 16 rows over 65536 tokens, fp8, 82 on
+// 176 and 68 on 253 (with one list 195 and 80).  Between 208 and 231 workgroups it goes
+// either way: 13 row blocks of 33 sequences, bf16, 247 us and 225, but as many sequences of
+// one length as a multiple of eight has workgroups are best left a workgroup each (7 row
+// blocks of 64 rows, 8 sequences, fp8, on 224 of them 47 us, on 252 59).
 constexpr std::size_t latent_share(std::size_t groups, std::size_t row_blocks) {
   if (row_blocks <= 1 || groups / row_blocks < kXcds) return 0;
   const std::size_t share = groups / row_blocks, whole = share / kXcds * kXcds;
-  return 16 * whole * row_blocks >= 15 * groups ? whole : share;
+  return 16 * whole * row_blocks >= 13 * groups ? whole : share;
 }
 
 std::size_t latent_workspace_bytes(std::size_t batch, std::size_t q_heads, std::size_t tokens,
