@@ -65,6 +65,7 @@ using latent_detail::divide;
 using latent_detail::kNoWeights;
 using latent_detail::lane_scan;
 using latent_detail::matrix_step;
+using latent_detail::part_sum;
 using latent_detail::row_factor;
 using latent_detail::uniform_long;
 using latent_detail::v4u;
@@ -1326,7 +1327,7 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
   for (int w = 0; w < 8; ++w) top = fmaxf(top, lead[w]);
   const float own = pl == 0.f ? 0.f : exp2_ratio(pm, top);
   weights[tid] = own;
-  float sum = pl * own;
+  float sum = part_sum(pm, pl, own, top);
 #pragma unroll
   for (int k = 32; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
   if (lane == 0) total[wave] = sum;
@@ -1356,7 +1357,7 @@ __global__ __launch_bounds__(512) void latent_split_merge_kernel(LatentKernelArg
   for (int w = 0; w < 8; ++w) sum += total[w];
 #pragma unroll
   for (int k = 1; k < kShares; ++k) o += sums[k][at];
-  *reinterpret_cast<v4f*>(merge_out(a, job, r) + dim) = o * row_factor(sum, top != -INFINITY, 1.0f);
+  *reinterpret_cast<v4f*>(merge_out(a, job, r) + dim) = o * row_factor(sum, false, 1.0f);
 }
 
 // ----------------------------------------------------------------- host ----

@@ -68,5 +68,11 @@ constexpr float kNoWeights = -3.402823466e38f;
 __device__ __forceinline__ float row_factor(float sum, bool some, float f) {
   return sum != 0.f ? f / sum : some ? NAN : 0.f;
 }
+// What a partial adds to the sum of a row whose largest reference is `top`: its own sum
+// times its weight, or, where all that the row sees has no weights, NaN.  (A join that
+// knows `top` before it adds needs it no longer then: it takes a register less.)
+__device__ __forceinline__ float part_sum(float reference, float sum, float weight, float top) {
+  return sum == 0.f && reference == top && top != -INFINITY ? NAN : sum * weight;
+}
 
 }  // namespace helix::hip::latent_detail

@@ -61,6 +61,7 @@ using latent_detail::divide;
 using latent_detail::kNoWeights;
 using latent_detail::lane_scan;
 using latent_detail::matrix_step;
+using latent_detail::part_sum;
 using latent_detail::row_factor;
 using latent_detail::uniform_long;
 using latent_detail::v4u;
@@ -1084,8 +1085,8 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
   auto slot_of = [&](int i, int row) {
     return static_cast<std::size_t>(2 * (job.first + i) + (i == 0 ? 1 : 0)) * rb_rows + row;
   };
-  auto finish = [&](int row, const v4f (&o)[2], float sum, float top) {
-    const float f = row_factor(sum, top != -INFINITY, 1.0f);
+  auto finish = [&](int row, const v4f (&o)[2], float sum) {
+    const float f = row_factor(sum, false, 1.0f);
     auto* const dst = reinterpret_cast<v4f*>(
                           a.out + static_cast<std::size_t>(job.b) * a.out_at.batch +
                           static_cast<std::size_t>(job.h) * a.out_at.head +
@@ -1121,13 +1122,13 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           // (A part that saw nothing has no outputs to speak of.)
-          const bool some = i0 + 4 * u < parts && ml[u][1] != 0.f;
-          const float w = some ? exp2_ratio(ml[u][0], top) : 0.f;
+          if (i0 + 4 * u >= parts) continue;
+          const float w = ml[u][1] != 0.f ? exp2_ratio(ml[u][0], top) : 0.f;
           if (w != 0.f) {
             o[0] += x[u][0] * w;
             o[1] += x[u][1] * w;
           }
-          if (some) sum += ml[u][1] * w;
+          sum += part_sum(ml[u][0], ml[u][1], w, top);
         }
       }
       __syncthreads();
@@ -1142,7 +1143,7 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
           o[1] += sums[w][lane][1];
           sum += totals[w][lane >> 4];
         }
-        finish(local, o, sum, top);
+        finish(local, o, sum);
       }
     }
     return;
@@ -1166,43 +1167,35 @@ __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedKernelArgs 
     }
   };
   load(0);
-  float top = -INFINITY, sum = 0.f;
+  // A lane of the row has a partial's maximum and sum.
+  static_assert(kFewParts <= 16, "16 lanes a row");
+  float pm = -INFINITY, pl = 0.f;
+  if (live && part < parts) {
+    const v2f ml = *reinterpret_cast<const v2f*>(st.part_ml + 2 * slot(part));
+    pm = ml[0];
+    pl = ml[1];
+  }
+  float top = pm;
+#pragma unroll
+  for (int k = 8; k > 0; k /= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
+  // (A part that saw nothing has no outputs to speak of.)
+  const float w = pl == 0.f ? 0.f : exp2_ratio(pm, top);
+  float sum = part_sum(pm, pl, w, top);
+#pragma unroll
+  for (int k = 8; k > 0; k /= 2) sum += __shfl_xor(sum, k, 64);
   v4f o[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
-  for (int i0 = 0; i0 < parts; i0 += 16) {
-    float pm = -INFINITY, pl = 0.f;
-    if (live && i0 + part < parts) {
-      const v2f ml = *reinterpret_cast<const v2f*>(st.part_ml + 2 * slot(i0 + part));
-      pm = ml[0];
-      pl = ml[1];
-    }
-    float mx = pm;
+  for (int i = 0; i < parts; i += 4) {
+    if (i != 0) load(i);
 #pragma unroll
-    for (int k = 8; k > 0; k /= 2) mx = fmaxf(mx, __shfl_xor(mx, k, 64));
-    const float mn = fmaxf(top, mx);
-    const float alpha = exp2_ratio(top, mn);
-    // (A part that saw nothing has no outputs to speak of.)
-    const float w = pl == 0.f ? 0.f : exp2_ratio(pm, mn);
-    float add = w * pl;
-#pragma unroll
-    for (int k = 8; k > 0; k /= 2) add += __shfl_xor(add, k, 64);
-    sum = sum * alpha + add;
-    o[0] *= alpha;
-    o[1] *= alpha;
-    top = mn;
-    const int end = min(parts - i0, 16);
-    for (int i = 0; i < end; i += 4) {
-      if (i0 + i != 0) load(i0 + i);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float wi = __shfl(w, (lane & 48) + min(i + u, end - 1), 64);
-        if (i + u < end && wi != 0.f) {
-          o[0] += x[u][0] * wi;
-          o[1] += x[u][1] * wi;
-        }
+    for (int u = 0; u < 4; ++u) {
+      const float wi = __shfl(w, (lane & 48) + min(i + u, parts - 1), 64);
+      if (i + u < parts && wi != 0.f) {
+        o[0] += x[u][0] * wi;
+        o[1] += x[u][1] * wi;
       }
     }
   }
-  if (live) finish(local, o, sum, top);
+  if (live) finish(local, o, sum);
 }
 
 // ----------------------------------------------------------------- host ----
