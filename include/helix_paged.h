@@ -618,8 +618,9 @@ int helix_paged_latent_append(const float* latent_rows, const size_t* latent_str
  * outside the table, or a page outside the pool among those that hold the
  * sequence's tokens, makes the sequence's rows NaN, and nothing is read there.
  * What a row does not see does not reach it, whatever it holds.  Values that are not
- * finite make the rows that see them NaN, or what the formula says.  A row all of
- * whose scores are minus infinity, or below fp32's range, is NaN (0 / 0).
+ * finite (bf16 pages: also queries of 2.3e38 and more over the scale's size) make the rows
+ * that see them NaN, or what the formula says.  A row all of whose scores are minus
+ * infinity, or below fp32's range, is NaN (0 / 0).
  * HELIX_UNSUPPORTED for other latent or page sizes.  The workspace needs no initial
  * value; calls that overlap on one workspace race. */
 int helix_paged_latent_workspace_bytes(size_t batch, size_t q_heads, size_t tokens, size_t latent,
